@@ -49,7 +49,9 @@ enum {
   PSB_DEVERR_WORKSPACE = 8,     /* split-K work exceeded the workspace */
   PSB_DEVERR_TIMEOUT = 16,      /* an async copy / MMA wait exceeded its bound */
   PSB_DEVERR_SEQLENS = 32,      /* cu_seqlens not non-decreasing within [0, total] */
-  PSB_DEVERR_LIMIT = 64         /* psb_select_tokens: a row had no tokens left to generate */
+  PSB_DEVERR_LIMIT = 64,        /* psb_select_tokens: a row had no tokens left to generate */
+  PSB_DEVERR_POOL = 128,        /* extend_step / trim_tables: not enough free blocks, or a malformed free list */
+  PSB_DEVERR_ROWS = 256         /* extend_step / trim_tables: a store row named twice */
 };
 
 /* per-row status bits written by psb_select_tokens */
@@ -396,6 +398,145 @@ int psb_add_rms_norm(const void* x, int64_t x_stride, void* residual, int64_t re
  */
 int psb_silu_and_mul(const void* gate_up, int64_t gate_up_stride, void* out, int64_t out_stride, int32_t rows,
                      int32_t intermediate, int32_t dtype, psb_stream_t stream);
+
+/*
+ * The 4-bit KV pool.  A K or V row x of head_dim values (one token, one kv
+ * head) of element type T is kept as one 4-bit code per value and one
+ * (step, mid) pair of type T:
+ *     lo, hi = min x, max x;   mid = T(lo / 2 + hi / 2);
+ *     step = T(max(hi - mid, mid - lo) / 7.5);
+ *     code = clamp(floor((x - mid) / step) + 8, 0, 15)   (8 where step is 0);
+ * and stands for the values mid + step * (code - 7.5).  Every operation before
+ * a rounding to T is fp32.  A row holding an infinity or a NaN is stored as
+ * mid = NaN, step = 0: it stands for NaN throughout.  Two contiguous pools,
+ * each starting on 16 bytes:
+ *     kv_codes  uint8 [num_layers, num_blocks, num_kv_heads, 2, block_size, head_dim / 2]
+ *     kv_params T     [num_layers, num_blocks, num_kv_heads, 2, block_size, 2]
+ * K at index 0 and V at index 1 of the fourth axis; byte j of a code row holds
+ * element 2 j in its low and 2 j + 1 in its high half; a pair is (step, mid).
+ * head_dim is even and at most 256.  A bf16 token with head_dim 64 takes 36
+ * bytes a row instead of 128.  No counterpart in the reference, whose pool is
+ * in the model's type (pagedserve/engine/kv_cache.py:10-16); slots, block
+ * tables and lengths are the ones of that pool.
+ */
+
+/*
+ * reshape_and_cache_int4: psb_reshape_and_cache into the 4-bit pool.  key and
+ * value are of ``dtype`` = T.  A negative slot writes nothing; a slot past the
+ * pool is skipped and flagged (PSB_DEVERR_SLOT_RANGE).  The live slots of one
+ * call are distinct.  A programmatic dependent launch.
+ */
+int psb_reshape_and_cache_int4(const void* key, int64_t key_stride_t, int64_t key_stride_h, const void* value,
+                               int64_t value_stride_t, int64_t value_stride_h, void* kv_codes, void* kv_params,
+                               const int64_t* slot_mapping, int32_t num_tokens, int32_t layer, int32_t num_layers,
+                               int64_t num_blocks, int32_t num_kv_heads, int32_t block_size, int32_t head_dim,
+                               int32_t dtype, int32_t* error_flag, psb_stream_t stream);
+
+/*
+ * rope_reshape_and_cache_int4: psb_rope_reshape_and_cache into the 4-bit pool.
+ * query_out and key_out are bit-identical to that call's; the rotated key, as
+ * rounded to ``dtype``, is what is quantised.  query_out may be query and
+ * key_out may be key; neither may overlap another argument otherwise.
+ */
+int psb_rope_reshape_and_cache_int4(const void* query, int64_t q_stride_t, int64_t q_stride_h, void* query_out,
+                                    int64_t qo_stride_t, int64_t qo_stride_h, const void* key, int64_t k_stride_t,
+                                    int64_t k_stride_h, void* key_out, int64_t ko_stride_t, int64_t ko_stride_h,
+                                    const void* value, int64_t v_stride_t, int64_t v_stride_h, const void* cos,
+                                    const void* sin, int64_t cs_stride_t, void* kv_codes, void* kv_params,
+                                    const int64_t* slot_mapping, int32_t num_tokens, int32_t num_q_heads,
+                                    int32_t layer, int32_t num_layers, int64_t num_blocks, int32_t num_kv_heads,
+                                    int32_t block_size, int32_t head_dim, int32_t dtype, int32_t* error_flag,
+                                    psb_stream_t stream);
+
+/*
+ * gather_cache_int4: the values stored at given slots, key_out and value_out
+ * [num_tokens, num_kv_heads, head_dim] of ``dtype`` (element strides, unit
+ * stride along head_dim): mid + step * (code - 7.5) evaluated in fp32 and
+ * rounded once.  A negative slot gives zeros; a slot past the pool gives zeros
+ * and is flagged (PSB_DEVERR_SLOT_RANGE).
+ */
+int psb_gather_cache_int4(const void* kv_codes, const void* kv_params, const int64_t* slot_mapping, void* key_out,
+                          int64_t key_stride_t, int64_t key_stride_h, void* value_out, int64_t value_stride_t,
+                          int64_t value_stride_h, int32_t num_tokens, int32_t layer, int32_t num_layers,
+                          int64_t num_blocks, int32_t num_kv_heads, int32_t block_size, int32_t head_dim,
+                          int32_t dtype, int32_t* error_flag, psb_stream_t stream);
+
+/* Workspace bytes of psb_paged_decode_int4 (0 for an invalid geometry).  The
+ * workspace starts on 16 bytes and needs no initialisation; calls that may
+ * overlap on the GPU use different ones. */
+size_t psb_paged_decode_int4_workspace_size(int32_t batch, int32_t q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                            int32_t block_size, int32_t max_context, int32_t dtype);
+
+/*
+ * paged_decode_int4: psb_paged_decode over the 4-bit pool: out[b, h] =
+ * softmax(scale * q[b, h] . K_b^T) V_b over the first context_lens[b] tokens,
+ * K and V being the values the codes stand for; a sequence of length 0 gives
+ * zeros.  query and out are of ``dtype`` = T.  The codes enter the products as
+ * they are (exactly) and step and mid are applied to the sums in fp32, so the
+ * only 16-bit rounding is that of step * probability before P V.  Lengths and
+ * tables are read before the kernel waits on its stream predecessor, as
+ * psb_paged_decode reads them.  Error behaviour is psb_paged_decode's.
+ */
+int psb_paged_decode_int4(const void* query, int64_t q_stride_b, int64_t q_stride_h, void* out, int64_t o_stride_b,
+                          int64_t o_stride_h, const void* kv_codes, const void* kv_params,
+                          const int32_t* block_tables, int64_t table_stride, const int32_t* context_lens,
+                          int32_t batch, int32_t q_heads, int32_t layer, int32_t num_layers, int64_t num_blocks,
+                          int32_t num_kv_heads, int32_t block_size, int32_t head_dim, int32_t dtype,
+                          int32_t max_context, float scale, void* workspace, size_t workspace_bytes,
+                          int32_t* error_flag, psb_stream_t stream);
+
+/*
+ * paged_prefill_int4: psb_paged_prefill over the 4-bit pool.  Sequence i's
+ * query rows cu_seqlens[i] .. cu_seqlens[i+1] are the last positions of its
+ * context_lens[i] tokens in the pool; rows of ``out`` behind the last sequence
+ * are left as they were.  Error behaviour is psb_paged_prefill's.
+ */
+int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv_codes,
+                           const void* kv_params, const int32_t* block_tables, int64_t table_stride,
+                           const int32_t* context_lens, void* out, int64_t o_stride_t, int64_t o_stride_h,
+                           const int32_t* cu_seqlens, int32_t num_seqs, int32_t total_tokens, int32_t max_seqlen,
+                           int32_t max_context, int32_t q_heads, int32_t layer, int32_t num_layers,
+                           int64_t num_blocks, int32_t num_kv_heads, int32_t block_size, int32_t head_dim,
+                           int32_t dtype, float scale, int32_t* error_flag, psb_stream_t stream);
+
+/*
+ * extend_step: psb_pack_step that also allocates.  The host-side BlockManager
+ * (pagedserve/engine/block_manager.py:6-155: a FIFO free list) as device
+ * state: ``free_blocks`` int32 [num_blocks] is a ring of free block ids,
+ * ``free_state`` int32 [4] = {head, count, 0, 0} (the third word is used
+ * during a call).  Entry b holds ceil(starts[b] / block_size) blocks in row
+ * req_rows[b] of ``table_store`` ([store_rows, store_width], row stride
+ * store_stride) and gets query_lens[b] new tokens: the blocks it lacks are
+ * taken from the head of the ring in entry order and appended to its row.
+ * cu_seqlens, context_lens, slot_mapping, positions and block_tables are
+ * psb_pack_step's.  An entry with req_rows[b] < 0 is padding: its query_lens[b]
+ * tokens get slot -1 and position 0, its length is 0, its table zero.
+ *
+ * A step that cannot be carried out whole changes neither the store nor the
+ * free list and is flagged: not enough free blocks (PSB_DEVERR_POOL), a row
+ * named twice (PSB_DEVERR_ROWS), a row out of range, a negative start or count,
+ * more blocks than store_width or out_width (PSB_DEVERR_CONTEXT), total not the
+ * sum of query_lens (PSB_DEVERR_SEQLENS).  Every slot is then -1, every length
+ * and table entry 0.  Calls on one free list must not overlap on the GPU.
+ */
+int psb_extend_step(int32_t* table_store, int64_t store_stride, int32_t store_rows, int32_t store_width,
+                    const int32_t* req_rows, const int32_t* starts, const int32_t* query_lens, int32_t batch,
+                    int32_t* free_blocks, int32_t num_blocks, int32_t* free_state, int32_t total, int32_t block_size,
+                    int32_t* cu_seqlens, int32_t* context_lens, int64_t* slot_mapping, int64_t* positions,
+                    int32_t* block_tables, int32_t out_width, int32_t* error_flag, psb_stream_t stream);
+
+/*
+ * trim_tables: gives blocks back.  Entry b of ``held_lens[b]`` tokens keeps
+ * ``keep_lens[b]`` of them (0: the request has finished): the blocks past
+ * ceil(keep / block_size) go to the tail of the ring, entry by entry in table
+ * order, and their store entries become 0.  Rows, checks and the all-or-nothing
+ * rule are psb_extend_step's (keep > held is PSB_DEVERR_CONTEXT, more blocks
+ * than the ring has room for PSB_DEVERR_POOL).
+ */
+int psb_trim_tables(int32_t* table_store, int64_t store_stride, int32_t store_rows, int32_t store_width,
+                    const int32_t* req_rows, const int32_t* held_lens, const int32_t* keep_lens, int32_t batch,
+                    int32_t* free_blocks, int32_t num_blocks, int32_t* free_state, int32_t block_size,
+                    int32_t* error_flag, psb_stream_t stream);
 
 /*
  * bounded_wait_check: a self-test with no counterpart in the reference.  One

@@ -25,6 +25,8 @@ DEVERR_BITS = {
     16: "async wait exceeded its bound",
     32: "cu_seqlens malformed",
     64: "a row had no tokens left to generate",
+    128: "not enough free blocks, or a malformed free list",
+    256: "a table-store row was named twice",
 }
 
 _c_void_p, _i32, _i64, _f32, _sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
@@ -89,6 +91,29 @@ SIGNATURES = {
     "psb_pack_step": (ctypes.c_int, [
         _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _c_void_p, _c_void_p,
         _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p]),
+    "psb_reshape_and_cache_int4": (ctypes.c_int, [
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _i64,
+        _i32, _i32, _i32, _i32, _c_void_p, _c_void_p]),
+    "psb_rope_reshape_and_cache_int4": (ctypes.c_int, [
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64,
+        _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _i64, _i32, _i32,
+        _i32, _i32, _c_void_p, _c_void_p]),
+    "psb_gather_cache_int4": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i32, _i32, _i32, _i64, _i32,
+        _i32, _i32, _i32, _c_void_p, _c_void_p]),
+    "psb_paged_decode_int4_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "psb_paged_decode_int4": (ctypes.c_int, [
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i32,
+        _i32, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _c_void_p, _sz, _c_void_p, _c_void_p]),
+    "psb_paged_prefill_int4": (ctypes.c_int, [
+        _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p,
+        _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _c_void_p, _c_void_p]),
+    "psb_extend_step": (ctypes.c_int, [
+        _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _i32, _c_void_p, _i32, _i32,
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p]),
+    "psb_trim_tables": (ctypes.c_int, [
+        _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _i32, _c_void_p, _i32,
+        _c_void_p, _c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -42,4 +42,11 @@ struct Int4PrefillParams {
   int32_t* err;
 };
 
+// Tensor-core decode (int4_decode_fast.cu): whether a geometry is covered, its
+// scratch bytes and the launch.  q rows and out rows start on 16 bytes.
+bool int4_decode_fast_geometry(int dtype, int batch, int hkv, int group, int head_dim, int block_size,
+                               int max_context);
+size_t int4_decode_fast_workspace(int group, int head_dim);
+int int4_decode_fast_launch(const Int4DecodeParams& p, int dtype, cudaStream_t s);
+
 }  // namespace psb

@@ -245,7 +245,12 @@ extern "C" size_t psb_paged_decode_int4_workspace_size(int32_t batch, int32_t q_
       head_dim > kInt4MaxDim || block_size <= 0 || max_context < 0 ||
       (dtype != PSB_F32 && dtype != PSB_F16 && dtype != PSB_BF16))
     return 0;
-  return std::max<size_t>(256, gen_workspace(batch, num_kv_heads, q_heads / num_kv_heads, head_dim, max_context));
+  // for whichever path the geometry allows (the fast path also needs aligned
+  // rows, known only at the call)
+  const int group = q_heads / num_kv_heads;
+  const size_t fast = int4_decode_fast_geometry(dtype, batch, num_kv_heads, group, head_dim, block_size, max_context)
+                          ? int4_decode_fast_workspace(group, head_dim) : 0;
+  return std::max({size_t(256), fast, gen_workspace(batch, num_kv_heads, group, head_dim, max_context)});
 }
 
 extern "C" int psb_paged_decode_int4(const void* query, int64_t q_stride_b, int64_t q_stride_h, void* out,
@@ -295,6 +300,10 @@ extern "C" int psb_paged_decode_int4(const void* query, int64_t q_stride_b, int6
   p.part = static_cast<float*>(workspace);
   p.err = error_flag;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const bool aligned = q_stride_b % 8 == 0 && q_stride_h % 8 == 0 && o_stride_b % 8 == 0 && o_stride_h % 8 == 0 &&
+                       reinterpret_cast<uintptr_t>(query) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  if (aligned && int4_decode_fast_geometry(dtype, batch, num_kv_heads, p.group, head_dim, block_size, max_context))
+    return int4_decode_fast_launch(p, dtype, s);
   switch (dtype) {
     case PSB_BF16: return launch_generic<__nv_bfloat16>(p, s);
     case PSB_F16: return launch_generic<__half>(p, s);

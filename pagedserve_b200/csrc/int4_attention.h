@@ -22,6 +22,7 @@ struct Int4DecodeParams {
   float scale_log2;     // scale * log2(e)
   float* part;          // split partials
   int32_t* err;
+  uint64_t tile_div;    // tensor-core path: 2^32 / (block_size / 16), rounded up
 };
 
 struct Int4PrefillParams {
@@ -45,7 +46,7 @@ struct Int4PrefillParams {
 // Tensor-core decode (int4_decode_fast.cu): whether a geometry is covered, its
 // scratch bytes and the launch.  q rows and out rows start on 16 bytes.
 bool int4_decode_fast_geometry(int dtype, int batch, int hkv, int group, int head_dim, int block_size,
-                               int max_context);
+                               int max_context, int num_layers, int64_t num_blocks);
 size_t int4_decode_fast_workspace(int group, int head_dim);
 int int4_decode_fast_launch(const Int4DecodeParams& p, int dtype, cudaStream_t s);
 

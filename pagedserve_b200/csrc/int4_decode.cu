@@ -248,7 +248,7 @@ extern "C" size_t psb_paged_decode_int4_workspace_size(int32_t batch, int32_t q_
   // for whichever path the geometry allows (the fast path also needs aligned
   // rows, known only at the call)
   const int group = q_heads / num_kv_heads;
-  const size_t fast = int4_decode_fast_geometry(dtype, batch, num_kv_heads, group, head_dim, block_size, max_context)
+  const size_t fast = int4_decode_fast_geometry(dtype, batch, num_kv_heads, group, head_dim, block_size, max_context, 1, 1)
                           ? int4_decode_fast_workspace(group, head_dim) : 0;
   return std::max({size_t(256), fast, gen_workspace(batch, num_kv_heads, group, head_dim, max_context)});
 }
@@ -299,10 +299,12 @@ extern "C" int psb_paged_decode_int4(const void* query, int64_t q_stride_b, int6
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part = static_cast<float*>(workspace);
   p.err = error_flag;
+  p.tile_div = 0;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool aligned = q_stride_b % 8 == 0 && q_stride_h % 8 == 0 && o_stride_b % 8 == 0 && o_stride_h % 8 == 0 &&
                        reinterpret_cast<uintptr_t>(query) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  if (aligned && int4_decode_fast_geometry(dtype, batch, num_kv_heads, p.group, head_dim, block_size, max_context))
+  if (aligned && int4_decode_fast_geometry(dtype, batch, num_kv_heads, p.group, head_dim, block_size, max_context,
+                                            num_layers, num_blocks))
     return int4_decode_fast_launch(p, dtype, s);
   switch (dtype) {
     case PSB_BF16: return launch_generic<__nv_bfloat16>(p, s);

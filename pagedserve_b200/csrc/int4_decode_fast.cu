@@ -9,34 +9,37 @@
 // below fp32; probabilities are rounded there by every 16-bit attention of
 // this library), the second sum is a scalar per head in fp32.
 //
-// Products.  mma.sync m16n8k16 with the tokens of a 16-token tile as rows of
-// S^T = K Q^T (8 q heads are the 8 columns) and head_dim as rows of
+// Products.  mma.sync m16n8k16 in f16 with the tokens of a 16-token tile as
+// rows of S^T = K Q^T (8 q heads are the 8 columns) and head_dim as rows of
 // O^T = V^T P^T.  The codes are the A operand in both, so a lane needs no more
 // than its own words of a code row: which element of head_dim an index k or a
 // row stands for is free as long as q (loaded once) and the output agree.  A
-// code becomes a 16-bit operand without conversion instructions:
-//   bf16: (w >> 4 i) & 0x000f000f | 0x4300 is 128 + c; for K the 128 is taken
-//         out by starting the accumulator at -135.5 sum(q) (4 or 8 products
-//         deep, so nothing builds up); for V, whose accumulator runs over the
-//         whole context, one paired add makes it c - 8 exactly.
-//   f16:  (w >> 8 i) & 0x000f000f is the subnormal c 2^-24 and & 0x00f000f0 is
-//         c 2^-20, exactly; products of the two kinds go to accumulators of
-//         their own (K) or rows of their own (V), and a product with ones sums
-//         the rounded p_t step_t for the -7.5.
+// code becomes an operand by one AND: (w >> 8 i) & 0x000f000f is the pair of
+// f16 subnormals c 2^-24, & 0x00f000f0 the pair c 2^-20, both exact.  The
+// other operand is brought to f16 whatever T is, without losing anything T
+// keeps: q times the power of two that takes the head tile's largest |q| to
+// 2^14 (what falls below f16's range then is under 2^-38 of that largest);
+// p step times a power of two that keeps it below 2^15, so it has f16's 11
+// bits down to 2^-29 of the largest so far.  That one rounding is the only one
+// below fp32.  A product with ones sums the rounded p step for the -7.5.
 // P^T is S^T's accumulator layout transposed: two movmatrix per tile.
 //
-// What bounds it.  A tile of head_dim 64 is 1152 bytes against 4096 in bf16,
-// so the same bytes per second need 3.6 times the instructions of
-// paged_decode; at about 150 warp instructions a tile the four schedulers of
-// an SM could issue some 30 bytes per clock, close to the SM's share of HBM.
+// What bounds it.  A 16-token tile of head_dim 64 is 1152 bytes against 4096
+// in bf16, so the same bytes per second need 3.6 times the instructions of
+// paged_decode: the issue slots of the four schedulers bound it next to HBM.
+// Hence codes by AND, two tiles at a time (independent work, one vote and one
+// set of loop instructions for both), each token's four factors worked out by
+// one lane and handed round through shared memory, the exponents' reference
+// folded into the score's multiply-add, and addresses and validity worked out
+// for 32 items at once, one per lane.
 //
-// Split.  The tiles of all sequences, in (kv head, sequence, tile) order, are
-// dealt evenly over the warps of the grid (one CTA of 16 warps per SM; 8 where
-// two head tiles of 128 need the registers).  A warp streams its run through a
-// private shared-memory ring (16-byte cp.async, one group per tile).  A
-// sequence inside one warp's run is written at once; pieces of one sequence
-// within a CTA are joined in shared memory, and only those cut by a CTA
-// boundary (at most one per CTA) leave a partial for int4_combine_kernel.
+// Split.  The items (32 tokens) of all sequences, in (kv head, sequence,
+// position) order, are dealt evenly over the warps of the grid (one CTA per
+// SM).  A warp streams its run through a private shared-memory ring (16-byte
+// cp.async, one group per item).  A sequence inside one warp's run is written
+// at once; pieces of one sequence within a CTA are joined in shared memory,
+// and only a sequence cut by a CTA boundary (at most one per CTA) leaves
+// partials, for int4_combine_kernel.
 #include <algorithm>
 
 #include "common.cuh"
@@ -48,22 +51,32 @@ namespace psb {
 namespace {
 
 constexpr int kMaxCtas = 160;       // grid limit (one CTA per SM; B200 has 148)
-constexpr int kMaxBatch = 4096;     // sequences whose lengths fit in shared memory
-constexpr int kMinTiles = 2;        // tiles per warp below which fewer CTAs take part
+constexpr int kMaxBatch = 2560;     // sequences whose lengths fit in shared memory
+constexpr int kMinItems = 1;        // items per warp below which fewer CTAs take part
 
 template <int D, int HT>
 struct Geo {
-  static constexpr int kWarps = D * HT > 128 ? 8 : 16;
+  static constexpr int kWarps = D * HT == 64 ? 16 : (D * HT == 128 ? 12 : 8);
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kStages = D == 64 ? 6 : (HT == 1 ? 3 : 4);
+  static constexpr int kStages = D == 64 ? 3 : (HT == 1 ? 2 : 3);
   static constexpr int kRows = 8 * HT;                  // q heads of a tile
   static constexpr int kCodeBytes = 16 * D / 2;         // K (or V) codes of 16 tokens
-  static constexpr int kStage = 2 * kCodeBytes + 128;   // K codes, V codes, K params, V params
+  static constexpr int kTile = 2 * kCodeBytes + 128;    // K codes, V codes, K params, V params
+  static constexpr int kStage = 2 * kTile;              // an item: two tiles
   static constexpr int kRing = kStages * kStage;
   static constexpr int kPartFloats = kRows * (D + 2);   // one piece: [rows][D] output, [rows][2] max, sum
+  static constexpr int kFactors = 32 * 16;              // (K step, K mid, V step, V mid) of an item's tokens
   static_assert(kRing >= kPartFloats * 4, "a warp's last piece fits its ring");
-  static constexpr size_t fixed_smem() { return static_cast<size_t>(kWarps) * (kRing + kPartFloats * 4); }
+  // per warp: ring | first piece | factors; then the join's weights [rows][2 warps], (max, sum) [rows][2 warps]
+  static constexpr size_t per_warp() { return kRing + kPartFloats * 4 + kFactors; }
+  static constexpr size_t fixed_smem() { return kWarps * per_warp() + sizeof(float) * kRows * 2 * kWarps * 3; }
   static size_t smem(int batch) { return fixed_smem() + sizeof(int32_t) * (2 * static_cast<size_t>(batch) + 1); }
+};
+
+// What a CTA leaves for int4_combine_kernel: the sequence cut at its end that
+// began in it (c1: the last CTA with a piece; 0: none).
+struct Cut {
+  int32_t grp, b, c1, pad;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -84,49 +97,29 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
 }
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
-// 4-bit codes as 16-bit operands; pair i (0 .. 3) of a word is its nibbles i
-// and i + 4.
-template <typename T> struct Nib;
-template <> struct Nib<__nv_bfloat16> {
-  static constexpr bool kSums = false;             // no product with ones
-  static constexpr float kKStart = -(128.f + 7.5f);  // per unit of sum(q), in K's accumulator
-  static constexpr float kVMid = 0.5f;             // V's codes enter as c - 8
-  __device__ static uint32_t k(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
-  __device__ static uint32_t v(uint32_t w, int i) {
-    uint32_t d;
-    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(k(w, i)), "r"(0xc308c308u));  // - 136
-    return d;
-  }
-};
-template <> struct Nib<__half> {
-  static constexpr bool kSums = true;
-  static constexpr float kKStart = 0.f;
-  static constexpr float kVMid = 0.f;
-  __device__ static uint32_t k(uint32_t w, int i) { return (w >> (8 * (i >> 1))) & (i & 1 ? 0x00f000f0u : 0x000f000fu); }
-  __device__ static uint32_t v(uint32_t w, int i) { return k(w, i); }
-};
-
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t w);
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
-  return __half22float2(*reinterpret_cast<__half2*>(&w));
+// Pair i (0 .. 3) of a code word, its nibbles i and i + 4, as two f16: c 2^-24
+// for even i, c 2^-20 for odd i.
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t w8, int i) {
+  return (i < 2 ? w : w8) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
 }
 
-template <typename T>
-__device__ __forceinline__ float growth_limit();  // log2 of how far a row's max may grow before it is moved
-// p stays below 2^8 (bf16) or 2^2 (f16, where p step <= 4 * 8736 must stay finite)
-template <> __device__ __forceinline__ float growth_limit<__nv_bfloat16>() { return 8.f; }
-template <> __device__ __forceinline__ float growth_limit<__half>() { return 2.f; }
+// d = a b (the accumulator starts at zero)
+__device__ __forceinline__ void mma_f16_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 
-__device__ __forceinline__ int tiles_of(int ctx) { return ctx <= 0 ? 1 : (ctx + 15) >> 4; }
+constexpr float kGrowth = 4.f;     // a score may exceed the exponents' reference by this (log2) before it is moved
+constexpr int kPBits = 11;         // p step is scaled to at most 2^kGrowth 2^kPBits = 2^15
+constexpr float kTwo24 = 16777216.f;
 
-// s_ctx[b] = clamped context, pre[b] = tiles before sequence b, pre[B] = all.
-// Called by every thread of a CTA of at most 32 warps.
+__device__ __forceinline__ int items_of(int ctx) { return ctx <= 0 ? 1 : (ctx + 31) >> 5; }
+
+// s_ctx[b] = clamped context, pre[b] = items before sequence b, pre[B] = all.
+// Called by every thread of a CTA.
 __device__ int build_prefix(const Int4DecodeParams& p, int32_t* pre, int32_t* s_ctx, bool flag) {
   __shared__ int32_t warp_sums[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthr = blockDim.x;
@@ -140,7 +133,7 @@ __device__ int build_prefix(const Int4DecodeParams& p, int32_t* pre, int32_t* s_
       n = n < 0 ? 0 : p.max_context;
     }
     s_ctx[b] = n;
-    local += tiles_of(n);
+    local += items_of(n);
   }
   int incl = local;
 #pragma unroll
@@ -150,14 +143,17 @@ __device__ int build_prefix(const Int4DecodeParams& p, int32_t* pre, int32_t* s_
   }
   if (lane == 31) warp_sums[warp] = incl;
   __syncthreads();
-  int run = incl - local, total = 0;
-  for (int w = 0; w < nthr / 32; ++w) {
-    if (w < warp) run += warp_sums[w];
-    total += warp_sums[w];
+  int sums = lane < nthr / 32 ? warp_sums[lane] : 0;  // every warp scans the warps' sums
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, sums, o);
+    if (lane >= o) sums += v;
   }
+  const int total = __shfl_sync(0xffffffffu, sums, 31);
+  int run = incl - local + (warp ? __shfl_sync(0xffffffffu, sums, warp - 1) : 0);
   for (int b = begin; b < end; ++b) {
     pre[b] = run;
-    run += tiles_of(s_ctx[b]);
+    run += items_of(s_ctx[b]);
   }
   if (tid == 0) pre[p.batch] = total;
   __syncthreads();
@@ -176,60 +172,88 @@ __device__ __forceinline__ int find_seq(const int32_t* pre, int batch, int i) {
 
 // The item list dealt over ``parts``: part w starts at floor(n w / parts).
 struct Deal {
-  int q, r, parts;
-  __device__ Deal(int n, int parts_) : q(n / parts_), r(n % parts_), parts(parts_) {}
-  __device__ int start(int w) const { return w * q + (r * w) / parts; }  // r, w < 2560: no overflow
+  uint32_t q, r, parts;
+  __device__ Deal(int n, int parts_) : q(static_cast<uint32_t>(n) / parts_), r(n - q * parts_), parts(parts_) {}
+  __device__ int start(uint32_t w) const { return w * q + (r * w) / parts; }  // r, w <= 2560: no overflow
 };
-
-// CTAs that take part for n items.
-__device__ __forceinline__ int active_ctas(int n, int warps, int grid) {
-  return min(grid, max(1, (n + warps * kMinTiles - 1) / (warps * kMinTiles)));
-}
 
 template <typename T, int D, int HT>
 __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(const Int4DecodeParams p) {
   using G = Geo<D, HT>;
   constexpr int kW = G::kWarps, kS = G::kStages, kRows = G::kRows;
-  constexpr int kM = D / 16;   // products per 16 tokens, K and V alike
+  constexpr int kM = D / 16;      // products per 16 tokens, K and V alike
   constexpr int kWords = D / 32;  // code words per lane: K per row, V per token / 2
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int32_t s_unit[2 * kW];  // the unit of each warp's first and last piece, -1: none
+  __shared__ int32_t s_grp[2 * kW], s_seq[2 * kW];  // (head tile, sequence) of each warp's first and last piece, -1: none
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * G::kRing;
-  float* first_piece = reinterpret_cast<float*>(smem + kW * G::kRing) + warp * G::kPartFloats;
-  int32_t* pre = reinterpret_cast<int32_t*>(smem + G::fixed_smem());
-  int32_t* s_ctx = pre + p.batch + 1;
+  uint8_t* const ring = smem + warp * G::kRing;
+  float* const pieces0 = reinterpret_cast<float*>(smem + kW * G::kRing);
+  float4* const factors = reinterpret_cast<float4*>(smem + kW * (G::kRing + G::kPartFloats * 4)) + warp * 32;
+  float* const s_w = reinterpret_cast<float*>(smem + kW * G::per_warp());  // [rows][2 kW] weights of the pieces
+  float2* const s_ml = reinterpret_cast<float2*>(s_w + kRows * 2 * kW);    // [rows][2 kW] (max, sum) at a run's first piece
+  int32_t* const pre = reinterpret_cast<int32_t*>(smem + G::fixed_smem());
+  int32_t* const s_ctx = pre + p.batch + 1;
 
   const int B = p.batch, BS = p.block_size;
   const int hgroups = (p.group + kRows - 1) / kRows;  // head tiles per kv head
-  if (tid < 2 * kW) s_unit[tid] = -1;
+  if (tid < 2 * kW) s_grp[tid] = -1;
   const int n_seq = build_prefix(p, pre, s_ctx, blockIdx.x == 0);
   const int n_items = n_seq * (p.hkv * hgroups);
-  const int act = active_ctas(n_items, kW, gridDim.x);
-  if (static_cast<int>(blockIdx.x) >= act) return;
+  const int act = min(static_cast<int>(gridDim.x), (n_items + kW * kMinItems - 1) / (kW * kMinItems));
+  Cut* const cuts = reinterpret_cast<Cut*>(p.part);
+  float* const part = p.part + kMaxCtas * (sizeof(Cut) / sizeof(float));
+  if (static_cast<int>(blockIdx.x) >= act) {
+    pdl_wait();
+    if (tid == 0) cuts[blockIdx.x] = Cut{0, 0, 0, 0};
+    return;
+  }
   const Deal deal(n_items, act * kW);
-  const int gw = blockIdx.x * kW + warp;
-  const int my_a = deal.start(gw), my_e = deal.start(gw + 1);
+  const int starts = deal.start(blockIdx.x * kW + min(lane, kW));  // lane w: of the CTA's warp w
+  const int my_a = __shfl_sync(0xffffffffu, starts, warp), my_e = __shfl_sync(0xffffffffu, starts, warp + 1);
+  const int cta_a = __shfl_sync(0xffffffffu, starts, 0), cta_e = __shfl_sync(0xffffffffu, starts, kW);
 
   // ---- 32 items at a time, one per lane ------------------------------------
-  // meta: bits 0-4 valid tokens, 5 first item of the warp's share of its unit,
-  // 6 last of it, 7 first of the unit, 8 last of the unit
+  // meta: bits 0-4 and 5-9 valid tokens of the two tiles (0: nothing to read),
+  // 10 first item of the warp's share of its sequence, 11 last of it, 12 first
+  // of the sequence, 13 last of it, 14 last item of the chunk; row16: pool
+  // rows / 16 of the two K tiles
   struct Chunk {
-    int beg, n, blk, meta, unit, sub;
+    int beg, n, meta, grp, b;
+    uint32_t row16[2];
   };
   auto build_chunk = [&](int beg) -> Chunk {
-    Chunk c{beg, min(32, my_e - beg), -1, 0, 0, 0};
+    Chunk c{beg, min(32, my_e - beg), 0, 0, 0, {0u, 0u}};
     if (lane < c.n) {
-      const int i = beg + lane, grp = i / n_seq, r = i - grp * n_seq;
-      const int b = find_seq(pre, B, r), j = r - pre[b];
-      const int ctx = s_ctx[b], nt = tiles_of(ctx);
-      const int valid = max(0, min(16, ctx - 16 * j));
-      c.meta = valid | (j == 0 || i == my_a ? 32 : 0) | (j == nt - 1 || i == my_e - 1 ? 64 : 0) | (j == 0 ? 128 : 0) |
-               (j == nt - 1 ? 256 : 0);
-      c.unit = grp * B + b;
-      const int pos = 16 * j;
-      c.sub = pos % BS;
-      if (valid > 0) c.blk = __ldg(p.tables + static_cast<int64_t>(b) * p.table_stride + pos / BS);
+      const int i = beg + lane;
+      c.grp = static_cast<uint32_t>(i) / static_cast<uint32_t>(n_seq);
+      const int r = i - c.grp * n_seq;
+      c.b = find_seq(pre, B, r);
+      const int j = r - pre[c.b], ctx = s_ctx[c.b], ni = items_of(ctx);
+      const int kvh = hgroups == 1 ? c.grp : c.grp / hgroups;
+      c.meta = (j == 0 || i == my_a ? 1 << 10 : 0) | (j == ni - 1 || i == my_e - 1 ? 1 << 11 : 0) |
+               (j == 0 ? 1 << 12 : 0) | (j == ni - 1 ? 1 << 13 : 0) | (lane == c.n - 1 ? 1 << 14 : 0);
+      const int32_t* row = p.tables + static_cast<int64_t>(c.b) * p.table_stride;
+      int valid[2], blk[2];
+      uint32_t sub[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t tile = 2 * j + k;  // tile of the sequence; BS / 16 tiles a block
+        const uint32_t bi = static_cast<uint32_t>((static_cast<uint64_t>(tile) * p.tile_div) >> 32);
+        valid[k] = max(0, min(16, ctx - 16 * static_cast<int>(tile)));
+        blk[k] = valid[k] > 0 ? __ldg(row + bi) : 0;
+        sub[k] = tile - bi * (BS >> 4);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (blk[k] < 0 || blk[k] >= p.num_blocks) {
+          flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
+          valid[k] = 0;
+        }
+        // K rows of (layer, block, kv head): 2 BS rows of K and V per tile of the pool
+        if (valid[k] > 0)
+          c.row16[k] = static_cast<uint32_t>((p.layer_tiles + static_cast<int64_t>(blk[k]) * p.hkv + kvh) * (BS >> 3)) + sub[k];
+        c.meta |= valid[k] << (5 * k);
+      }
     }
     return c;
   };
@@ -244,8 +268,9 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
     }
   }
   int ib = 0;
-  uint32_t issued = 0, consumed = 0;
-  int slot_meta = 0, slot_unit = 0;  // lane s: of ring stage s (bit 9 of the meta: data was copied)
+  int in_flight = 0;
+  uint32_t st_in = 0, st = 0;                    // ring stages: next to fill, next to read
+  int slot_meta = 0, slot_grp = 0, slot_b = 0;   // lane s: of ring stage s
   const uint32_t ring_u = smem_u32(ring);
   const uint64_t pol = l2_policy_evict_first();
   // Row pi(r) of a tile is the token at index r of the products: chosen so
@@ -256,44 +281,47 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
   // D 128: 16-byte column c of row r is kept at c ^ 2 ((r >> 1) & 1), so that
   // V's 8-byte reads of four tokens spread over all banks
   auto swz = [](int row) { return D == 128 ? ((row >> 1) & 1) << 1 : 0; };
-  auto issue_one = [&]() {
-    const uint32_t st = issued % kS;
-    int blk = __shfl_sync(0xffffffffu, cur.blk, ib);
-    int mt = __shfl_sync(0xffffffffu, cur.meta, ib);
-    const int unit = __shfl_sync(0xffffffffu, cur.unit, ib);
-    const int sub = __shfl_sync(0xffffffffu, cur.sub, ib);
-    bool ok = (mt & 31) > 0;
-    if (ok && (blk < 0 || blk >= p.num_blocks)) {
-      if (lane == 0) flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
-      ok = false;
-    }
-    if (ok) {
-      const int kvh = (unit / B) / hgroups;
-      const int64_t krow = int4_row(p.layer_tiles + static_cast<int64_t>(blk) * p.hkv + kvh, 0, sub, BS);
-      const uint32_t dst = ring_u + st * G::kStage;
-      const uint8_t* ks = p.codes + krow * (D / 2);
-      const uint8_t* vs = ks + static_cast<int64_t>(BS) * (D / 2);
+  // per-lane ends of the copies: 16-byte piece lane (and lane + 32) of a code
+  // tile, piece lane % 4 of the K (lane < 4) or V (lane < 8) parameters
+  uint32_t cp_dst[D / 64];
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        const int ch = lane + 32 * i;  // 16-byte piece of the tile
-        uint32_t o = ch * 16;
-        if (D == 128) o = (ch >> 2) * 64 + (((ch & 3) ^ swz(ch >> 2)) << 4);
-        cp_async16_hint(dst + o, ks + ch * 16, pol);
-        cp_async16_hint(dst + G::kCodeBytes + o, vs + ch * 16, pol);
+  for (int i = 0; i < D / 64; ++i) {
+    const int ch = lane + 32 * i;
+    cp_dst[i] = ring_u + (D == 128 ? (ch >> 2) * 64 + (((ch & 3) ^ swz(ch >> 2)) << 4) : ch * 16);
+  }
+  const uint32_t cp_par = ring_u + 2 * G::kCodeBytes + lane * 16;
+  const uint8_t* const src_k = p.codes + lane * 16;
+  const uint8_t* const src_v = src_k + static_cast<int64_t>(BS) * (D / 2);
+  const char* const src_par = reinterpret_cast<const char*>(p.params) + (lane & 3) * 16 + ((lane >> 2) & 1) * (static_cast<int64_t>(BS) * 4);
+  auto issue_one = [&]() {
+    const int mt = __shfl_sync(0xffffffffu, cur.meta, ib);
+    const int grp = __shfl_sync(0xffffffffu, cur.grp, ib), b = __shfl_sync(0xffffffffu, cur.b, ib);
+    const uint32_t r0 = __shfl_sync(0xffffffffu, cur.row16[0], ib), r1 = __shfl_sync(0xffffffffu, cur.row16[1], ib);
+    const uint32_t off = st_in * G::kStage;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (mt & (31 << (5 * k))) {
+        const uint64_t row = k ? r1 : r0;
+        const uint8_t* ks = src_k + row * G::kCodeBytes;
+        const uint8_t* vs = src_v + row * G::kCodeBytes;
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          cp_async16_hint(cp_dst[i] + off + k * G::kTile, ks + 512 * i, pol);
+          cp_async16_hint(cp_dst[i] + off + k * G::kTile + G::kCodeBytes, vs + 512 * i, pol);
+        }
+        if (lane < 8) cp_async16(cp_par + off + k * G::kTile, src_par + row * 64);
       }
-      if (lane < 8) {
-        const char* ps = reinterpret_cast<const char*>(p.params) + krow * 4 + (lane >> 2) * (static_cast<int64_t>(BS) * 4);
-        cp_async16(dst + 2 * G::kCodeBytes + lane * 16, ps + (lane & 3) * 16);
-      }
-      mt |= 512;
     }
     cp_async_commit();
-    if (lane == static_cast<int>(st)) {
+    if (lane == static_cast<int>(st_in)) {
       slot_meta = mt;
-      slot_unit = unit;
+      slot_grp = grp;
+      slot_b = b;
     }
-    ++issued;
-    if (++ib == cur.n) {
+    st_in = st_in + 1 == kS ? 0 : st_in + 1;
+    ++in_flight;
+    ++ib;
+    if (mt & (1 << 14)) {
       c_ok = n_ok;
       cur = nxt;
       ib = 0;
@@ -306,151 +334,214 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
   };
 
   // Only lengths and tables have been read so far; the pool and q may still be
-  // being written by the stream predecessor.
+  // being written by the stream predecessor, the workspace be read by it.
   pdl_wait();
   pdl_launch_dependents();
-  while (c_ok && issued < kS) issue_one();
+#pragma unroll 1
+  for (int i = 0; i < kS && c_ok; ++i) issue_one();
 
   uint32_t qb[HT][kM][2];         // B fragments of q
   float qs[HT][2];                // sum(q) of heads 2 t, 2 t + 1
   float o[HT][kM][4];             // (element of row g | g + 8) x (head 2 t | 2 t + 1)
-  float sp[HT][4];                // sums of the rounded p step (f16)
-  float m[HT][2], l[HT][2], z[HT][2];
-  int unit = 0;
-  bool whole = false;
+  float sp[HT][4];                // sums of the rounded, scaled p step
+  float nref[HT][2];              // minus the exponents' reference
+  float l[HT][2], z[HT][2];       // sum p, sum p mid
+  float kfac = 0.f;               // score of one unit of the accumulator, per step
+  float vscale = 1.f, vlim = 0.f; // scale of p step; the largest step it allows
+  int grp = 0, b = 0;
+  bool whole = false, fresh = true;  // fresh: no score seen yet
   int pieces = 0;
   const float sc = p.scale_log2;
-  constexpr float kTwo24 = 16777216.f;
   const int row0 = pi(g);         // tokens of rows g and g + 8: row0, 8 + row0
+  const uint32_t k_row = D == 64 ? row0 * 32 + t * 8 : row0 * 64 + ((t ^ swz(row0)) << 4);  // swz(row0 + 8) == swz(row0)
+  uint32_t v_row[2];              // V: tokens of products 2 t, 2 t + 1 (those of 2 t + 8, 2 t + 9: 8 rows on)
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = pi(2 * t + r);
+    v_row[r] = G::kCodeBytes + (D == 64 ? row * 32 + g * 4 : row * 64 + (((g >> 1) ^ swz(row)) << 4) + (g & 1) * 8);
+  }
+  const uint32_t par_off = (lane >> 4) * G::kTile + 2 * G::kCodeBytes + (lane & 15) * 4;  // K parameters of token ``lane``
 
-  while (consumed != issued) {
-    const uint32_t st = consumed % kS;
+  while (in_flight) {
     const int mt = __shfl_sync(0xffffffffu, slot_meta, st);
-    if (mt & 32) {
-      // ---- a unit's first tile: q fragments ---------------------------------
-      unit = __shfl_sync(0xffffffffu, slot_unit, st);
-      whole = mt & 128;
-      const int grp = unit / B, b = unit - grp * B;
-      const int kvh = grp / hgroups, h0 = (grp - kvh * hgroups) * kRows;
+    if (mt & (1 << 10)) {
+      // ---- a sequence's first item here: q fragments --------------------------
+      grp = __shfl_sync(0xffffffffu, slot_grp, st);
+      b = __shfl_sync(0xffffffffu, slot_b, st);
+      whole = mt & (1 << 12);
+      fresh = true;
+      const int kvh = hgroups == 1 ? grp : grp / hgroups, h0 = (grp - kvh * hgroups) * kRows;
+      uint4 x[HT][kWords];  // 8 elements each: those of one code word
+      float top = 0.f;
 #pragma unroll
       for (int ht = 0; ht < HT; ++ht) {
         const int hh = h0 + ht * 8 + g;
         const bool live = hh < p.group;
         const T* src = reinterpret_cast<const T*>(p.q) + b * p.qsb + (kvh * p.group + (live ? hh : 0)) * p.qsh + t * (D / 4);
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+          x[ht][w] = make_uint4(0, 0, 0, 0);
+          if (live) x[ht][w] = *reinterpret_cast<const uint4*>(src + 8 * w);
+          const uint32_t* e = &x[ht][w].x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack2<T>(e[i]);
+            if (finite_f32(f.x)) top = fmaxf(top, fabsf(f.x));
+            if (finite_f32(f.y)) top = fmaxf(top, fabsf(f.y));
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const int qe = top > 0.f ? max(-100, min(100, ilogb_f32(top))) : 0;
+      const float qsc = exp2_int(14 - qe);
+      kfac = sc * kTwo24 * exp2_int(qe - 14);
+#pragma unroll
+      for (int ht = 0; ht < HT; ++ht) {
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
-          uint4 x = make_uint4(0, 0, 0, 0);  // 8 elements: one code word's
-          if (live) x = *reinterpret_cast<const uint4*>(src + 8 * w);
-          const float2 a0 = unpack2<T>(x.x), a1 = unpack2<T>(x.y), a2 = unpack2<T>(x.z), a3 = unpack2<T>(x.w);
+          const float2 a0 = unpack2<T>(x[ht][w].x), a1 = unpack2<T>(x[ht][w].y), a2 = unpack2<T>(x[ht][w].z),
+                       a3 = unpack2<T>(x[ht][w].w);
           sum += ((a0.x + a0.y) + (a1.x + a1.y)) + ((a2.x + a2.y) + (a3.x + a3.y));
-          // elements (i, i + 4) of the word, for products 4 (w / 2) + i
-          qb[ht][4 * (w >> 1) + 0][w & 1] = prmt(x.x, x.z, 0x5410);
-          qb[ht][4 * (w >> 1) + 1][w & 1] = prmt(x.x, x.z, 0x7632);
-          qb[ht][4 * (w >> 1) + 2][w & 1] = prmt(x.y, x.w, 0x5410);
-          qb[ht][4 * (w >> 1) + 3][w & 1] = prmt(x.y, x.w, 0x7632);
+          // elements (i, i + 4) of the word, for products 4 (w / 2) + i; odd
+          // products' codes are 16 times as large
+          const float q16 = qsc * 0.0625f;
+          qb[ht][4 * (w >> 1) + 0][w & 1] = pack2<__half>(a0.x * qsc, a2.x * qsc);
+          qb[ht][4 * (w >> 1) + 1][w & 1] = pack2<__half>(a0.y * q16, a2.y * q16);
+          qb[ht][4 * (w >> 1) + 2][w & 1] = pack2<__half>(a1.x * qsc, a3.x * qsc);
+          qb[ht][4 * (w >> 1) + 3][w & 1] = pack2<__half>(a1.y * q16, a3.y * q16);
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        qs[ht][0] = __shfl_sync(0xffffffffu, sum, 8 * t);      // head 2 t is lanes 8 t ..
+        qs[ht][0] = __shfl_sync(0xffffffffu, sum, 8 * t);  // head 2 t is lanes 8 t .. 8 t + 3
         qs[ht][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          m[ht][e] = -INFINITY;
-          l[ht][e] = z[ht][e] = 0.f;
-        }
+        for (int e = 0; e < 2; ++e) nref[ht][e] = l[ht][e] = z[ht][e] = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) sp[ht][e] = 0.f;
 #pragma unroll
         for (int i = 0; i < kM; ++i) o[ht][i][0] = o[ht][i][1] = o[ht][i][2] = o[ht][i][3] = 0.f;
       }
+      vscale = 1.f;
+      vlim = 0.f;
     }
     // the oldest copy is complete once at most the newer ones are pending;
     // near the end of the run fewer are pending than that, so wait for all
-    if (issued - consumed == kS) cp_async_wait<kS - 1>(); else cp_async_wait<0>();
+    if (in_flight == kS) cp_async_wait<kS - 1>(); else cp_async_wait<0>();
     __syncwarp();
-    if (mt & 512) {
-      const int valid = mt & 31;
-      const uint8_t* kt = ring + st * G::kStage;
-      const uint8_t* vt = kt + G::kCodeBytes;
-      const uint32_t* par = reinterpret_cast<const uint32_t*>(kt + 2 * G::kCodeBytes);
+    if (mt & 1023) {
+      const uint8_t* const item = ring + st * G::kStage;
+      const int valid0 = mt & 31, valid1 = (mt >> 5) & 31;
+      // ---- the tokens' factors, one token a lane ---------------------------------
+      {
+        const bool live = (lane & 15) < (lane < 16 ? valid0 : valid1);  // rows past the context may hold anything
+        uint32_t kpar = 0, vpar = 0;
+        if (live) {
+          kpar = *reinterpret_cast<const uint32_t*>(item + par_off);
+          vpar = *reinterpret_cast<const uint32_t*>(item + par_off + 64);
+        }
+        const float2 kp = unpack2<T>(kpar), vp = unpack2<T>(vpar);
+        if (__any_sync(0xffffffffu, vp.x > vlim)) {  // a larger step than the scale of p step allows
+          float top = vp.x;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          const int e = max(-100, ilogb_f32(top)) + 1;  // top < 2^e
+          const float nv = exp2_int(kPBits - e);
+          const float ratio = fresh ? 0.f : nv / vscale;  // the sums are zero before the first score
+          vlim = exp2_int(min(e, 127));
+          vscale = nv;
+#pragma unroll
+          for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+            for (int i = 0; i < kM; ++i) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) o[ht][i][k] *= ratio;
+            }
+            sp[ht][0] *= ratio;
+            sp[ht][1] *= ratio;
+          }
+        }
+        // the code's -7.5 goes with mid
+        factors[lane] = make_float4(kp.x * kfac, fmaf(kp.x, -7.5f, kp.y) * sc, vp.x * vscale, vp.y);
+      }
       // ---- S^T = K Q^T ---------------------------------------------------------
-      uint32_t kw[2][kWords];
+      float s[2][HT][4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = row0 + 8 * r;
-        if constexpr (D == 64) {
-          const uint2 x = *reinterpret_cast<const uint2*>(kt + row * 32 + t * 8);
-          kw[r][0] = x.x;
-          kw[r][1] = x.y;
-        } else {
-          const uint4 x = *reinterpret_cast<const uint4*>(kt + row * 64 + ((t ^ swz(row)) << 4));
-          kw[r][0] = x.x;
-          kw[r][1] = x.y;
-          kw[r][2] = x.z;
-          kw[r][3] = x.w;
-        }
-      }
-      float s[HT][4], s1[HT][4];
+      for (int k = 0; k < 2; ++k) {
+        uint32_t kw[2][kWords], kw8[2][kWords];
 #pragma unroll
-      for (int ht = 0; ht < HT; ++ht) {
-        s[ht][0] = s[ht][2] = Nib<T>::kKStart * qs[ht][0];
-        s[ht][1] = s[ht][3] = Nib<T>::kKStart * qs[ht][1];
-        s1[ht][0] = s1[ht][1] = s1[ht][2] = s1[ht][3] = 0.f;
-      }
+        for (int r = 0; r < 2; ++r) {
+          const uint8_t* src = item + k * G::kTile + k_row + r * (8 * D / 2);
+          if constexpr (D == 64) {
+            const uint2 x = *reinterpret_cast<const uint2*>(src);
+            kw[r][0] = x.x;
+            kw[r][1] = x.y;
+          } else {
+            const uint4 x = *reinterpret_cast<const uint4*>(src);
+            kw[r][0] = x.x;
+            kw[r][1] = x.y;
+            kw[r][2] = x.z;
+            kw[r][3] = x.w;
+          }
 #pragma unroll
-      for (int i = 0; i < kM; ++i) {
-        const int w = 2 * (i >> 2), nb = i & 3;
-        const uint32_t a0 = Nib<T>::k(kw[0][w], nb), a1 = Nib<T>::k(kw[1][w], nb);
-        const uint32_t a2 = Nib<T>::k(kw[0][w + 1], nb), a3 = Nib<T>::k(kw[1][w + 1], nb);
-#pragma unroll
-        for (int ht = 0; ht < HT; ++ht)
-          mma_16816<T>(Nib<T>::kSums && (i & 1) ? s1[ht] : s[ht], a0, a1, a2, a3, qb[ht][i][0], qb[ht][i][1]);
-      }
-      // ---- scores (log2 scale), probabilities ----------------------------------
-      float2 kp[2], vp[2];  // (step, mid) of tokens row0 and 8 + row0
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        kp[r] = unpack2<T>(par[row0 + 8 * r]);
-        vp[r] = unpack2<T>(par[16 + row0 + 8 * r]);
-      }
-      const bool ok0 = row0 < valid, ok1 = row0 + 8 < valid;
-      if (valid < 16) {  // rows past the context may hold anything
-        if (!ok0) kp[0] = vp[0] = make_float2(0.f, 0.f);
-        if (!ok1) kp[1] = vp[1] = make_float2(0.f, 0.f);
-      }
-      float x[HT][4];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float ks = kp[r].x * sc, km = kp[r].y * sc;
-        if (Nib<T>::kSums) {
-          km = fmaf(-7.5f, ks, km);
-          ks *= kTwo24;
+          for (int w = 0; w < kWords; ++w) kw8[r][w] = kw[r][w] >> 8;
         }
 #pragma unroll
-        for (int ht = 0; ht < HT; ++ht) {
+        for (int i = 0; i < kM; ++i) {
+          const int w = 2 * (i >> 2), nb = i & 3;
+          const uint32_t a0 = code_pair(kw[0][w], kw8[0][w], nb), a1 = code_pair(kw[1][w], kw8[1][w], nb);
+          const uint32_t a2 = code_pair(kw[0][w + 1], kw8[0][w + 1], nb), a3 = code_pair(kw[1][w + 1], kw8[1][w + 1], nb);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float a = s[ht][2 * r + e];
-            if (Nib<T>::kSums) a = fmaf(s1[ht][2 * r + e], 0.0625f, a);
-            x[ht][2 * r + e] = fmaf(ks, a, km * qs[ht][e]);
+          for (int ht = 0; ht < HT; ++ht) {
+            if (i == 0) mma_f16_first(s[k][ht], a0, a1, a2, a3, qb[ht][i][0], qb[ht][i][1]);
+            else mma_16816<__half>(s[k][ht], a0, a1, a2, a3, qb[ht][i][0], qb[ht][i][1]);
           }
         }
       }
-      if (valid < 16) {
+      __syncwarp();  // factors written
+      // ---- scores minus reference (log2 scale) -----------------------------------
+      float vs[2][2], vm[2][2];
+      float top[HT][2];
 #pragma unroll
-        for (int ht = 0; ht < HT; ++ht) {
-          if (!ok0) x[ht][0] = x[ht][1] = -INFINITY;
-          if (!ok1) x[ht][2] = x[ht][3] = -INFINITY;
+      for (int ht = 0; ht < HT; ++ht) top[ht][0] = top[ht][1] = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float4 f = factors[16 * k + 8 * r + row0];
+          vs[k][r] = f.z;
+          vm[k][r] = f.w;
+#pragma unroll
+          for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              s[k][ht][2 * r + e] = fmaf(f.x, s[k][ht][2 * r + e], fmaf(f.y, qs[ht][e], nref[ht][e]));
+          }
         }
       }
-      // The maximum the exponents refer to moves only when some score is above
-      // it by more than the limit: most tiles touch no accumulator.
-      bool grow = false;
+      if (valid0 < 16 || valid1 < 16) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if (row0 + 8 * r >= (k ? valid1 : valid0)) {
+#pragma unroll
+              for (int ht = 0; ht < HT; ++ht) s[k][ht][2 * r] = s[k][ht][2 * r + 1] = -INFINITY;
+            }
+          }
+        }
+      }
+      // The reference moves only when some score is above it by more than the
+      // limit: most items touch no accumulator.
+      bool grow = fresh;
 #pragma unroll
       for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) grow = grow || fmaxf(x[ht][e], x[ht][2 + e]) > m[ht][e] + growth_limit<T>();
+        for (int e = 0; e < 2; ++e) {
+          top[ht][e] = fmaxf(fmaxf(s[0][ht][e], s[0][ht][2 + e]), fmaxf(s[1][ht][e], s[1][ht][2 + e]));
+          grow = grow || top[ht][e] > kGrowth;
+        }
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -458,15 +549,21 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
           float al[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(x[ht][e], x[ht][2 + e]);
+            float mx = top[ht][e];
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            mx = fmaxf(mx, m[ht][e]);
-            al[e] = m[ht][e] == -INFINITY ? 0.f : ex2_approx(m[ht][e] - mx);
-            m[ht][e] = mx;
+            // the first reference is the first maximum (finite whatever the scores are)
+            mx = fresh ? fminf(fmaxf(mx, -3e38f), 3e38f) : fmaxf(mx, 0.f);
+            al[e] = fresh ? 0.f : ex2_approx(-mx);
+            nref[ht][e] -= mx;
             l[ht][e] *= al[e];
             z[ht][e] *= al[e];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              s[k][ht][e] -= mx;
+              s[k][ht][2 + e] -= mx;
+            }
           }
 #pragma unroll
           for (int i = 0; i < kM; ++i) {
@@ -475,101 +572,103 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
             o[ht][i][2] *= al[0];
             o[ht][i][3] *= al[1];
           }
-          if (Nib<T>::kSums) {
-            sp[ht][0] *= al[0];
-            sp[ht][1] *= al[1];
+          sp[ht][0] *= al[0];
+          sp[ht][1] *= al[1];
+        }
+        fresh = false;
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        // ---- probabilities, P^T ----------------------------------------------------
+        uint32_t pb[HT][2];  // B fragments
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+          for (int ht = 0; ht < HT; ++ht) {
+            float pr[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              pr[e] = ex2_approx(s[k][ht][2 * r + e]);
+              l[ht][e] += pr[e];
+              z[ht][e] = fmaf(pr[e], vm[k][r], z[ht][e]);
+            }
+            pb[ht][r] = movmatrix_t(pack2<__half>(pr[0] * vs[k][r], pr[1] * vs[k][r]));
           }
         }
-      }
-      uint32_t pb[HT][2];  // B fragments of P^T
-      const float vm0 = fmaf(Nib<T>::kVMid, vp[0].x, vp[0].y), vm1 = fmaf(Nib<T>::kVMid, vp[1].x, vp[1].y);
+        // ---- O^T += V^T P^T ----------------------------------------------------------
+        uint32_t vw[4][D / 64];
 #pragma unroll
-      for (int ht = 0; ht < HT; ++ht) {
-        float pr[4];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float mu = m[ht][e] == -INFINITY ? 0.f : m[ht][e];
-          pr[e] = ex2_approx(x[ht][e] - mu);
-          pr[2 + e] = ex2_approx(x[ht][2 + e] - mu);
-          l[ht][e] += pr[e] + pr[2 + e];
-          z[ht][e] = fmaf(pr[e], vm0, fmaf(pr[2 + e], vm1, z[ht][e]));
+        for (int r = 0; r < 4; ++r) {
+          const uint8_t* src = item + k * G::kTile + v_row[r & 1] + (r >> 1) * (8 * D / 2);
+          if constexpr (D == 64) {
+            vw[r][0] = *reinterpret_cast<const uint32_t*>(src);
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(src);
+            vw[r][0] = w.x;
+            vw[r][1] = w.y;
+          }
         }
-        pb[ht][0] = movmatrix_t(pack2<T>(pr[0] * vp[0].x, pr[1] * vp[0].x));
-        pb[ht][1] = movmatrix_t(pack2<T>(pr[2] * vp[1].x, pr[3] * vp[1].x));
-      }
-      // ---- O^T += V^T P^T --------------------------------------------------------
-      uint32_t vw[4][D / 64];  // tokens pi(2 t), pi(2 t + 1) and those plus 8
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = pi(2 * t + (r & 1)) + 8 * (r >> 1);
-        if constexpr (D == 64) {
-          vw[r][0] = *reinterpret_cast<const uint32_t*>(vt + row * 32 + g * 4);
-        } else {
-          const uint2 w = *reinterpret_cast<const uint2*>(vt + row * 64 + (((g >> 1) ^ swz(row)) << 4) + (g & 1) * 8);
-          vw[r][0] = w.x;
-          vw[r][1] = w.y;
+        for (int q = 0; q < D / 64; ++q) {
+          const uint32_t x01 = prmt(vw[0][q], vw[1][q], 0x5410), y01 = prmt(vw[0][q], vw[1][q], 0x7632);
+          const uint32_t x23 = prmt(vw[2][q], vw[3][q], 0x5410), y23 = prmt(vw[2][q], vw[3][q], 0x7632);
+          const uint32_t x01h = x01 >> 8, y01h = y01 >> 8, x23h = x23 >> 8, y23h = y23 >> 8;
+#pragma unroll
+          for (int nb = 0; nb < 4; ++nb) {
+            const uint32_t a0 = code_pair(x01, x01h, nb), a1 = code_pair(y01, y01h, nb), a2 = code_pair(x23, x23h, nb),
+                           a3 = code_pair(y23, y23h, nb);
+#pragma unroll
+            for (int ht = 0; ht < HT; ++ht) mma_16816<__half>(o[ht][4 * q + nb], a0, a1, a2, a3, pb[ht][0], pb[ht][1]);
+          }
         }
-      }
-#pragma unroll
-      for (int q = 0; q < D / 64; ++q) {
-        const uint32_t x01 = prmt(vw[0][q], vw[1][q], 0x5410), y01 = prmt(vw[0][q], vw[1][q], 0x7632);
-        const uint32_t x23 = prmt(vw[2][q], vw[3][q], 0x5410), y23 = prmt(vw[2][q], vw[3][q], 0x7632);
-#pragma unroll
-        for (int nb = 0; nb < 4; ++nb) {
-          const uint32_t a0 = Nib<T>::v(x01, nb), a1 = Nib<T>::v(y01, nb), a2 = Nib<T>::v(x23, nb),
-                         a3 = Nib<T>::v(y23, nb);
-#pragma unroll
-          for (int ht = 0; ht < HT; ++ht) mma_16816<T>(o[ht][4 * q + nb], a0, a1, a2, a3, pb[ht][0], pb[ht][1]);
-        }
-      }
-      if (Nib<T>::kSums) {
 #pragma unroll
         for (int ht = 0; ht < HT; ++ht)
-          mma_16816<T>(sp[ht], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[ht][0], pb[ht][1]);
+          mma_16816<__half>(sp[ht], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[ht][0], pb[ht][1]);
       }
     }
     __syncwarp();
-    ++consumed;
+    --in_flight;
+    st = st + 1 == kS ? 0 : st + 1;
     if (c_ok) issue_one();  // refill the stage just freed
 
-    if (mt & 64) {
-      // ---- the warp's share of the unit is done --------------------------------
-      const int grp = unit / B, b = unit - grp * B;
-      const int kvh = grp / hgroups, h0 = (grp - kvh * hgroups) * kRows;
-      whole = whole && (mt & 256);
+    if (mt & (1 << 11)) {
+      // ---- the warp's share of the sequence is done ----------------------------
+      const int kvh = hgroups == 1 ? grp : grp / hgroups, h0 = (grp - kvh * hgroups) * kRows;
+      whole = whole && (mt & (1 << 13));
       float* piece = nullptr;
       if (!whole) {
         // the first piece has its own place; the other one ends the run, when
         // the warp's ring is free
         const int k = pieces++;
-        piece = k == 0 ? first_piece : reinterpret_cast<float*>(ring);
-        if (lane == 0) s_unit[2 * warp + k] = unit;
-        if (k == 1) __syncwarp();
+        piece = k == 0 ? pieces0 + warp * G::kPartFloats : reinterpret_cast<float*>(ring);
+        if (lane == 0) {
+          s_grp[2 * warp + k] = grp;
+          s_seq[2 * warp + k] = b;
+        }
       }
+      const float vinv = 1.f / vscale;  // a power of two: exact
 #pragma unroll
       for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float ll = l[ht][e], zz = z[ht][e];
+        for (int d = 4; d < 32; d <<= 1) {
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            ll += __shfl_xor_sync(0xffffffffu, ll, d);
-            zz += __shfl_xor_sync(0xffffffffu, zz, d);
+          for (int e = 0; e < 2; ++e) {
+            l[ht][e] += __shfl_xor_sync(0xffffffffu, l[ht][e], d);
+            z[ht][e] += __shfl_xor_sync(0xffffffffu, z[ht][e], d);
           }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float base = -7.5f * sp[ht][e];
           // elements (D / 8) g + 8 q + {0 .. 7}: nibbles 0-3 are row g, 4-7 row g + 8
           float r[D / 8];
 #pragma unroll
           for (int q = 0; q < D / 64; ++q) {
 #pragma unroll
             for (int nb = 0; nb < 4; ++nb) {
-              float a = o[ht][4 * q + nb][e], c = o[ht][4 * q + nb][2 + e];
-              if (Nib<T>::kSums) {
-                const float w = nb & 1 ? kTwo24 / 16.f : kTwo24;
-                a = fmaf(a, w, -7.5f * sp[ht][e]);
-                c = fmaf(c, w, -7.5f * sp[ht][e]);
-              }
-              r[8 * q + nb] = a + zz;
-              r[8 * q + 4 + nb] = c + zz;
+              const float w = nb & 1 ? kTwo24 / 16.f : kTwo24;
+              r[8 * q + nb] = fmaf(fmaf(o[ht][4 * q + nb][e], w, base), vinv, z[ht][e]);
+              r[8 * q + 4 + nb] = fmaf(fmaf(o[ht][4 * q + nb][2 + e], w, base), vinv, z[ht][e]);
             }
           }
           const int hr = ht * 8 + 2 * t + e, hh = h0 + hr;
@@ -578,11 +677,11 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
 #pragma unroll
             for (int q = 0; q < D / 32; ++q) dst[q] = make_float4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
             if (g == 0) {
-              piece[kRows * D + 2 * hr] = m[ht][e];
-              piece[kRows * D + 2 * hr + 1] = ll;
+              piece[kRows * D + 2 * hr] = fresh ? -INFINITY : -nref[ht][e];
+              piece[kRows * D + 2 * hr + 1] = l[ht][e];
             }
           } else if (hh < p.group) {
-            const float inv = ll == 0.f ? 0.f : 1.f / ll;
+            const float inv = l[ht][e] == 0.f ? 0.f : 1.f / l[ht][e];
             T* dst = reinterpret_cast<T*>(p.out) + b * p.osb + (kvh * p.group + hh) * p.osh + g * (D / 8);
 #pragma unroll
             for (int q = 0; q < D / 64; ++q) {
@@ -600,113 +699,180 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
   }
 
   // ---- join the pieces of this CTA ----------------------------------------------
+  // Piece slot s = 2 warp + (0 | 1); the pieces of one sequence are a run of
+  // slots (with empty ones between).  First the weights, a lane per slot and a
+  // warp per q head, then the outputs, a thread per element.
   __syncthreads();
-  const int mine = lane < 2 * kW ? s_unit[lane] : -1;
-  const uint32_t peers = __match_any_sync(0xffffffffu, mine);
-  uint32_t leaders = __ballot_sync(0xffffffffu, mine >= 0 && lane == __ffs(peers) - 1);
-  const int cta_a = deal.start(blockIdx.x * kW), cta_e = deal.start((blockIdx.x + 1) * kW);
-  for (int k = 0; leaders; ++k) {
-    const int lead = __ffs(leaders) - 1;
-    leaders &= leaders - 1;
-    const uint32_t run = __shfl_sync(0xffffffffu, peers, lead);
-    const int u = __shfl_sync(0xffffffffu, mine, lead);
-    const int grp = u / B, b = u - grp * B;
-    const int u_a = grp * n_seq + pre[b], u_e = grp * n_seq + pre[b + 1];
-    const int kvh = grp / hgroups, h0 = (grp - kvh * hgroups) * kRows;
-    for (int hr = (warp + kW - (k * kRows) % kW) % kW; hr < kRows; hr += kW) {  // rows over warps, run after run
-      auto piece_of = [&](int s) -> const float* {
-        return (s & 1) ? reinterpret_cast<const float*>(smem + (s >> 1) * G::kRing)
-                       : reinterpret_cast<const float*>(smem + kW * G::kRing) + (s >> 1) * G::kPartFloats;
-      };
-      float mx = -INFINITY, ll = 0.f, acc[D / 32];
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-      for (uint32_t r = run; r; r &= r - 1) mx = fmaxf(mx, piece_of(__ffs(r) - 1)[kRows * D + 2 * hr]);
-      const float mu = mx == -INFINITY ? 0.f : mx;
-      for (uint32_t r = run; r; r &= r - 1) {
-        const float* pc = piece_of(__ffs(r) - 1);
-        const float w = ex2_approx(pc[kRows * D + 2 * hr] - mu);
-        ll = fmaf(pc[kRows * D + 2 * hr + 1], w, ll);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(pc[hr * D + lane + 32 * i], w, acc[i]);
+  const int my_grp = lane < 2 * kW ? s_grp[lane] : -1;
+  const int my_b = my_grp >= 0 ? s_seq[lane] : -1 - lane;
+  const uint64_t key = (static_cast<uint64_t>(static_cast<uint32_t>(my_grp)) << 32) | static_cast<uint32_t>(my_b);
+  const uint32_t peers = __match_any_sync(0xffffffffu, key);
+  const int first = __ffs(peers) - 1;
+  uint32_t leaders = __ballot_sync(0xffffffffu, my_grp >= 0 && lane == first);
+  auto piece_of = [&](int s) -> const float* {
+    return (s & 1) ? reinterpret_cast<const float*>(smem + (s >> 1) * G::kRing) : pieces0 + (s >> 1) * G::kPartFloats;
+  };
+  for (int hr = warp; hr < kRows; hr += kW) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (my_grp >= 0) ml = *reinterpret_cast<const float2*>(piece_of(lane) + kRows * D + 2 * hr);
+    float mx = ml.x;
+    for (uint32_t r = peers; __any_sync(0xffffffffu, r); r &= r - 1) {
+      const float v = __shfl_sync(0xffffffffu, ml.x, r ? __ffs(r) - 1 : lane);
+      mx = fmaxf(mx, v);
+    }
+    const float w = my_grp >= 0 ? ex2_approx(ml.x - (mx == -INFINITY ? 0.f : mx)) : 0.f;
+    const float lw = ml.y * w;
+    float sum = 0.f;
+    for (uint32_t r = peers; __any_sync(0xffffffffu, r); r &= r - 1) {
+      const float v = __shfl_sync(0xffffffffu, lw, r ? __ffs(r) - 1 : lane);
+      if (r) sum += v;
+    }
+    if (lane < 2 * kW) {
+      s_w[hr * 2 * kW + lane] = w;
+      s_ml[hr * 2 * kW + lane] = make_float2(mx, sum);
+    }
+  }
+  // extent of the lane's sequence in items; what it is cut by
+  const int u_a = my_grp >= 0 ? my_grp * n_seq + pre[my_b] : 0;
+  const int u_e = my_grp >= 0 ? my_grp * n_seq + pre[my_b + 1] : 0;
+  const bool cut_a = u_a < cta_a, cut_e = u_e > cta_e;
+  if (warp == 0) {
+    // the sequence that begins here and runs past the end of the CTA, if any
+    const uint32_t tail = __ballot_sync(0xffffffffu, my_grp >= 0 && cut_e && !cut_a);
+    Cut c{0, 0, 0, 0};
+    if (tail) {
+      const int src = __ffs(tail) - 1;
+      const int end = __shfl_sync(0xffffffffu, u_e, src);
+      c.grp = __shfl_sync(0xffffffffu, my_grp, src);
+      c.b = __shfl_sync(0xffffffffu, my_b, src);
+      c.c1 = blockIdx.x;
+      for (int c0 = blockIdx.x + 1; c0 < act; c0 += 32) {  // CTAs that start before its end
+        const bool in = c0 + lane < act && deal.start((c0 + lane) * kW) < end;
+        const int n = __popc(__ballot_sync(0xffffffffu, in));
+        c.c1 += n;
+        if (n < 32) break;
       }
-      if (u_a >= cta_a && u_e <= cta_e) {
-        if (h0 + hr < p.group) {
-          const float inv = ll == 0.f ? 0.f : 1.f / ll;
-          T* dst = reinterpret_cast<T*>(p.out) + b * p.osb + (kvh * p.group + h0 + hr) * p.osh;
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) dst[lane + 32 * i] = Elem<T>::from_float(acc[i] * inv);
-        }
+    }
+    if (lane == 0) cuts[blockIdx.x] = c;
+  }
+  __syncthreads();
+  for (; leaders; leaders &= leaders - 1) {
+    const int lead = __ffs(leaders) - 1;
+    const uint32_t run = __shfl_sync(0xffffffffu, peers, lead);
+    const int rg = __shfl_sync(0xffffffffu, my_grp, lead), rb = __shfl_sync(0xffffffffu, my_b, lead);
+    const bool ca = __shfl_sync(0xffffffffu, cut_a, lead), ce = __shfl_sync(0xffffffffu, cut_e, lead);
+    const int kvh = hgroups == 1 ? rg : rg / hgroups, h0 = (rg - kvh * hgroups) * kRows;
+    for (int e = tid; e < kRows * D; e += G::kThreads) {
+      const int hr = e / D, d = e - hr * D;
+      float acc = 0.f;
+      for (uint32_t r = run; r; r &= r - 1) {
+        const int sl = __ffs(r) - 1;
+        acc = fmaf(piece_of(sl)[e], s_w[hr * 2 * kW + sl], acc);
+      }
+      const float2 ml = s_ml[hr * 2 * kW + lead];
+      if (!ca && !ce) {
+        if (h0 + hr < p.group)
+          reinterpret_cast<T*>(p.out)[rb * p.osb + (kvh * p.group + h0 + hr) * p.osh + d] =
+              Elem<T>::from_float(ml.y == 0.f ? 0.f : acc / ml.y);
       } else {
         // cut at the CTA's start (slot 0) or only at its end (slot 1)
-        float* dst = p.part + static_cast<int64_t>(2 * blockIdx.x + (u_a < cta_a ? 0 : 1)) * G::kPartFloats;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) dst[hr * D + lane + 32 * i] = acc[i];
-        if (lane == 0) {
-          dst[kRows * D + 2 * hr] = mx;
-          dst[kRows * D + 2 * hr + 1] = ll;
-        }
+        float* dst = part + static_cast<int64_t>(2 * blockIdx.x + (ca ? 0 : 1)) * G::kPartFloats;
+        dst[e] = acc;
+        if (d == 0) *reinterpret_cast<float2*>(dst + kRows * D + 2 * hr) = ml;
       }
     }
   }
 }
 
-// Joins the partials of the unit cut by CTA boundary blockIdx.x (the first
-// boundary that cuts it; other boundaries of the same unit have nothing to
-// do): one warp per q head.  Starts while the decode runs and works out its
-// unit from the lengths alone, as the decode dealt them.
+// Joins the partials of the sequence that CTA blockIdx.x of the decode left
+// cut at its end: kRows x kSplit warps, warp (row, k) takes every kSplit-th
+// partial of q head ``row``, and the kSplit sums meet in shared memory.
+constexpr int kCombineWarps = 32;
+
 template <typename T, int D, int HT>
-__global__ void __launch_bounds__(8 * HT * 32) int4_combine_kernel(const Int4DecodeParams p, int decode_grid) {
+__global__ void __launch_bounds__(kCombineWarps * 32) int4_combine_kernel(const Int4DecodeParams p) {
   using G = Geo<D, HT>;
-  extern __shared__ int32_t sm[];
-  int32_t* pre = sm;
-  int32_t* s_ctx = pre + p.batch + 1;
-  const int lane = threadIdx.x & 31, hr = threadIdx.x >> 5, B = p.batch;
-  const int hgroups = (p.group + G::kRows - 1) / G::kRows;
-  const int n_seq = build_prefix(p, pre, s_ctx, false);
-  const int n_items = n_seq * (p.hkv * hgroups);
-  const int act = active_ctas(n_items, G::kWarps, decode_grid);
+  constexpr int kRows = G::kRows, kSplit = kCombineWarps / kRows;
+  __shared__ float s_acc[kCombineWarps][D];
+  __shared__ float2 s_ml[kCombineWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hr = warp % kRows, k = warp / kRows;
+  const int hgroups = (p.group + kRows - 1) / kRows;
   const int c0 = blockIdx.x;
   pdl_wait();
   pdl_launch_dependents();
-  if (c0 + 1 >= act) return;
-  const Deal deal(n_items, act * G::kWarps);
-  const int cut = deal.start((c0 + 1) * G::kWarps);
-  if (cut >= n_items) return;
-  const int grp = cut / n_seq, r = cut - grp * n_seq;
-  const int b = find_seq(pre, B, r);
-  const int u_a = grp * n_seq + pre[b], u_e = grp * n_seq + pre[b + 1];
-  if (u_a >= cut || u_a < deal.start(c0 * G::kWarps)) return;  // not cut here, or cut before
-  int c1 = c0 + 1;
-  while (c1 + 1 < act && deal.start((c1 + 1) * G::kWarps) < u_e) ++c1;
-  const int kvh = grp / hgroups, hh = (grp - kvh * hgroups) * G::kRows + hr;
-  if (hh >= p.group) return;
-  auto piece_of = [&](int c) { return p.part + static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * G::kPartFloats; };
+  const int4 cut = __ldcg(reinterpret_cast<const int4*>(p.part) + c0);
+  const int grp = cut.x, b = cut.y, np = cut.z - c0 + 1;  // c0's own and those of the CTAs after it
+  if (cut.z <= c0) return;
+  const float* part = p.part + kMaxCtas * (sizeof(Cut) / sizeof(float));
+  auto piece_of = [&](int i) { return part + static_cast<int64_t>(2 * (c0 + i) + (i == 0 ? 1 : 0)) * G::kPartFloats; };
   float mx = -INFINITY, ll = 0.f, acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-  for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, __ldcg(piece_of(c) + G::kRows * D + 2 * hr));
+  constexpr int kBatch = 8;
+  for (int i0 = k; i0 < np; i0 += kSplit * kBatch) {
+    float2 ml[kBatch];
+    float v[kBatch][D / 32];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  const float mu = mx == -INFINITY ? 0.f : mx;
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const float* pc = piece_of(c);
-    const float w = ex2_approx(__ldcg(pc + G::kRows * D + 2 * hr) - mu);
-    ll = fmaf(__ldcg(pc + G::kRows * D + 2 * hr + 1), w, ll);
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = i0 + j * kSplit;
+      ml[j] = make_float2(-INFINITY, 0.f);
+      if (i < np) {
+        const float* pc = piece_of(i);
+        ml[j] = __ldcg(reinterpret_cast<const float2*>(pc + kRows * D + 2 * hr));
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(__ldcg(pc + hr * D + lane + 32 * i), w, acc[i]);
+        for (int q = 0; q < D / 32; ++q) v[j][q] = __ldcg(pc + hr * D + lane + 32 * q);
+      } else {
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) v[j][q] = 0.f;
+      }
+    }
+    float mn = mx;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) mn = fmaxf(mn, ml[j].x);
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    const float al = ex2_approx(mx - mu);  // 0 at first
+    mx = mn;
+    ll *= al;
+#pragma unroll
+    for (int q = 0; q < D / 32; ++q) acc[q] *= al;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const float w = ex2_approx(ml[j].x - mu);
+      ll = fmaf(ml[j].y, w, ll);
+#pragma unroll
+      for (int q = 0; q < D / 32; ++q) acc[q] = fmaf(v[j][q], w, acc[q]);
+    }
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+#pragma unroll
+  for (int q = 0; q < D / 32; ++q) s_acc[warp][lane + 32 * q] = acc[q];
+  if (lane == 0) s_ml[warp] = make_float2(mx, ll);
+  __syncthreads();
+  const int kvh = hgroups == 1 ? grp : grp / hgroups, hh = (grp - kvh * hgroups) * kRows + hr;
+  if (k > 0 || hh >= p.group) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < kSplit; ++j) top = fmaxf(top, s_ml[j * kRows + hr].x);
+  const float mu = top == -INFINITY ? 0.f : top;
+  ll = 0.f;
+#pragma unroll
+  for (int q = 0; q < D / 32; ++q) acc[q] = 0.f;
+#pragma unroll
+  for (int j = 0; j < kSplit; ++j) {
+    const float2 ml = s_ml[j * kRows + hr];
+    const float w = ex2_approx(ml.x - mu);
+    ll = fmaf(ml.y, w, ll);
+#pragma unroll
+    for (int q = 0; q < D / 32; ++q) acc[q] = fmaf(s_acc[j * kRows + hr][lane + 32 * q], w, acc[q]);
+  }
   T* dst = reinterpret_cast<T*>(p.out) + b * p.osb + (kvh * p.group + hh) * p.osh;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) dst[lane + 32 * i] = Elem<T>::from_float(acc[i] * inv);
+  for (int q = 0; q < D / 32; ++q) dst[lane + 32 * q] = Elem<T>::from_float(ll == 0.f ? 0.f : acc[q] / ll);
 }
 
 // Upper bound of the items from the host-known longest context.
 int64_t max_items(int batch, int hkv, int group, int rows, int max_context) {
   return static_cast<int64_t>(batch) * hkv * ((group + rows - 1) / rows) *
-         std::max<int64_t>(1, (static_cast<int64_t>(max_context) + 15) / 16);
+         std::max<int64_t>(1, (static_cast<int64_t>(max_context) + 31) / 32);
 }
 
 template <typename T, int D, int HT>
@@ -718,15 +884,14 @@ int launch_fast(const Int4DecodeParams& p, cudaStream_t stream, int sms) {
   int occ = 0;
   if (!kernel_occupancy(reinterpret_cast<const void*>(kern), G::kThreads, smem, &occ) || occ < 1) return PSB_ERR_CUDA;
   const int64_t items = max_items(p.batch, p.hkv, p.group, G::kRows, p.max_context);
-  const int64_t want = (items + G::kWarps * kMinTiles - 1) / (G::kWarps * kMinTiles);
+  const int64_t want = (items + G::kWarps * kMinItems - 1) / (G::kWarps * kMinItems);
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, std::min(sms, kMaxCtas))));
   discard_stale_error();
   cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(G::kThreads), smem, stream, p);
   if (e != cudaSuccess) return record_cuda_error(e);
   if (grid > 1) {
     if (!prefer_max_shared(reinterpret_cast<const void*>(comb))) return PSB_ERR_CUDA;
-    const size_t csmem = sizeof(int32_t) * (2 * static_cast<size_t>(p.batch) + 1);
-    e = launch_pdl(comb, dim3(static_cast<unsigned>(grid - 1)), dim3(8 * HT * 32), csmem, stream, p, grid);
+    e = launch_pdl(comb, dim3(static_cast<unsigned>(grid - 1)), dim3(kCombineWarps * 32), 0, stream, p);
     if (e != cudaSuccess) return record_cuda_error(e);
   }
   return check_launch();
@@ -737,19 +902,26 @@ int head_tiles(int group) { return group <= 8 ? 1 : 2; }
 }  // namespace
 
 bool int4_decode_fast_geometry(int dtype, int batch, int hkv, int group, int head_dim, int block_size,
-                               int max_context) {
+                               int max_context, int num_layers, int64_t num_blocks) {
   const int rows = 8 * head_tiles(group);
   return (dtype == PSB_BF16 || dtype == PSB_F16) && (head_dim == 64 || head_dim == 128) && block_size % 16 == 0 &&
-         batch <= kMaxBatch && max_items(batch, hkv, group, rows, max_context) < (int64_t(1) << 31) - 64;
+         batch <= kMaxBatch && max_items(batch, hkv, group, rows, max_context) < (int64_t(1) << 31) - 64 &&
+         static_cast<int64_t>(num_layers) * num_blocks * hkv * 2 * (block_size / 16) < (int64_t(1) << 32) &&
+         static_cast<int64_t>(max_context / 16 + 2) * (block_size / 16) < (int64_t(1) << 32);
 }
 
 size_t int4_decode_fast_workspace(int group, int head_dim) {
-  return sizeof(float) * 2 * kMaxCtas * static_cast<size_t>(8 * head_tiles(group)) * (head_dim + 2);
+  return sizeof(Cut) * kMaxCtas + sizeof(float) * 2 * kMaxCtas * static_cast<size_t>(8 * head_tiles(group)) * (head_dim + 2);
 }
 
-int int4_decode_fast_launch(const Int4DecodeParams& p, int dtype, cudaStream_t s) {
+int int4_decode_fast_launch(const Int4DecodeParams& p_in, int dtype, cudaStream_t s) {
   const int sms = device_sm_count();
   if (sms <= 0) return PSB_ERR_CUDA;
+  Int4DecodeParams p = p_in;
+  // floor(t / n) of a tile number t < 2^27 by n = block_size / 16 tiles a
+  // block, as t ceil(2^32 / n) / 2^32: exact while t (n - 1) < 2^32
+  const uint32_t n = static_cast<uint32_t>(p.block_size) / 16;
+  p.tile_div = ((uint64_t(1) << 32) + n - 1) / n;
   const bool bf = dtype == PSB_BF16;
   if (head_tiles(p.group) == 1) {
     if (p.head_dim == 64)

@@ -34,13 +34,14 @@
 // for 32 items at once, one per lane.
 //
 // Split.  The items (32 tokens) of all sequences, in (kv head, sequence,
-// position) order, are dealt evenly over the warps of the grid (one CTA per
-// SM).  A warp streams its run through a private shared-memory ring (16-byte
-// cp.async, one group per item).  A sequence inside one warp's run is written
+// position) order, are dealt evenly over the consumer warps of the grid (one CTA
+// per SM).  Each has a private shared-memory ring, filled by bulk copies that
+// lane w of the CTA's copying warp issues for consumer w.  A sequence inside one warp's run is written
 // at once; pieces of one sequence within a CTA are joined in shared memory,
 // and only a sequence cut by a CTA boundary (at most one per CTA) leaves
 // partials, for int4_combine_kernel.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -58,17 +59,12 @@ template <int D, int HT>
 struct Geo {
   static constexpr int kWarps = D * HT == 64 ? 16 : (D * HT == 128 ? 12 : 8);
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kStages = D == 64 ? 3 : (HT == 1 ? 2 : 3);
   static constexpr int kRows = 8 * HT;                  // q heads of a tile
   static constexpr int kCodeBytes = 16 * D / 2;         // K (or V) codes of 16 tokens
-  static constexpr int kTile = 2 * kCodeBytes + 128;    // K codes, V codes, K params, V params
-  static constexpr int kStage = 2 * kTile;              // an item: two tiles
-  static constexpr int kRing = kStages * kStage;
   static constexpr int kPartFloats = kRows * (D + 2);   // one piece: [rows][D] output, [rows][2] max, sum
   static constexpr int kFactors = 32 * 16;              // (K step, K mid, V step, V mid) of an item's tokens
-  static_assert(kRing >= kPartFloats * 4, "a warp's last piece fits its ring");
-  // per warp: ring | first piece | factors; then the join's weights [rows][2 warps], (max, sum) [rows][2 warps]
-  static constexpr size_t per_warp() { return kRing + kPartFloats * 4 + kFactors; }
+  // per warp: first piece | last piece | factors; then the join's weights [rows][2 warps] and (max, sum)
+  static constexpr size_t per_warp() { return 2 * kPartFloats * 4 + kFactors; }
   static constexpr size_t fixed_smem() { return kWarps * per_warp() + sizeof(float) * kRows * 2 * kWarps * 3; }
   static size_t smem(int batch) { return fixed_smem() + sizeof(int32_t) * (2 * static_cast<size_t>(batch) + 1); }
 };
@@ -78,17 +74,6 @@ struct Geo {
 struct Cut {
   int32_t grp, b, c1, pad;
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async16_hint(uint32_t dst, const void* src, uint64_t pol) {
-  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(pol)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
   uint32_t d;
@@ -180,15 +165,14 @@ struct Deal {
 template <typename T, int D, int HT>
 __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(const Int4DecodeParams p) {
   using G = Geo<D, HT>;
-  constexpr int kW = G::kWarps, kS = G::kStages, kRows = G::kRows;
+  constexpr int kW = G::kWarps, kRows = G::kRows;
   constexpr int kM = D / 16;      // products per 16 tokens, K and V alike
   constexpr int kWords = D / 32;  // code words per lane: K per row, V per token / 2
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int32_t s_grp[2 * kW], s_seq[2 * kW];  // (head tile, sequence) of each warp's first and last piece, -1: none
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  uint8_t* const ring = smem + warp * G::kRing;
-  float* const pieces0 = reinterpret_cast<float*>(smem + kW * G::kRing);
-  float4* const factors = reinterpret_cast<float4*>(smem + kW * (G::kRing + G::kPartFloats * 4)) + warp * 32;
+  float* const pieces = reinterpret_cast<float*>(smem);  // [warps][first, last]
+  float4* const factors = reinterpret_cast<float4*>(smem + kW * 2 * G::kPartFloats * 4) + warp * 32;
   float* const s_w = reinterpret_cast<float*>(smem + kW * G::per_warp());  // [rows][2 kW] weights of the pieces
   float2* const s_ml = reinterpret_cast<float2*>(s_w + kRows * 2 * kW);    // [rows][2 kW] (max, sum) at a run's first piece
   int32_t* const pre = reinterpret_cast<int32_t*>(smem + G::fixed_smem());
@@ -209,137 +193,74 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
   }
   const Deal deal(n_items, act * kW);
   const int starts = deal.start(blockIdx.x * kW + min(lane, kW));  // lane w: of the CTA's warp w
-  const int my_a = __shfl_sync(0xffffffffu, starts, warp), my_e = __shfl_sync(0xffffffffu, starts, warp + 1);
   const int cta_a = __shfl_sync(0xffffffffu, starts, 0), cta_e = __shfl_sync(0xffffffffu, starts, kW);
 
-  // ---- 32 items at a time, one per lane ------------------------------------
-  // meta: bits 0-4 and 5-9 valid tokens of the two tiles (0: nothing to read),
-  // 10 first item of the warp's share of its sequence, 11 last of it, 12 first
-  // of the sequence, 13 last of it, 14 last item of the chunk; row16: pool
-  // rows / 16 of the two K tiles
+  const int my_a = __shfl_sync(0xffffffffu, starts, warp), my_e = __shfl_sync(0xffffffffu, starts, warp + 1);
+
+  // ---- 32 items at a time, one per lane: where their tiles are ---------------
+  // row16: pool rows / 16 of the two K tiles (below 2^31; 0 where there is
+  // none: it is read all the same and masked), the top bit set where the
+  // tile's block is outside the pool; any_bad: some tile of the run is
   struct Chunk {
-    int beg, n, meta, grp, b;
     uint32_t row16[2];
   };
+  constexpr uint32_t kBad = 1u << 31;
+  bool any_bad = false;
+  int seg_grp = 0, seg_b = 0, seg_j = 0;  // head tile, sequence and item in it of the warp's next share
   auto build_chunk = [&](int beg) -> Chunk {
-    Chunk c{beg, min(32, my_e - beg), 0, 0, 0, {0u, 0u}};
-    if (lane < c.n) {
-      const int i = beg + lane;
-      c.grp = static_cast<uint32_t>(i) / static_cast<uint32_t>(n_seq);
-      const int r = i - c.grp * n_seq;
-      c.b = find_seq(pre, B, r);
-      const int j = r - pre[c.b], ctx = s_ctx[c.b], ni = items_of(ctx);
-      const int kvh = hgroups == 1 ? c.grp : c.grp / hgroups;
-      c.meta = (j == 0 || i == my_a ? 1 << 10 : 0) | (j == ni - 1 || i == my_e - 1 ? 1 << 11 : 0) |
-               (j == 0 ? 1 << 12 : 0) | (j == ni - 1 ? 1 << 13 : 0) | (lane == c.n - 1 ? 1 << 14 : 0);
-      const int32_t* row = p.tables + static_cast<int64_t>(c.b) * p.table_stride;
-      int valid[2], blk[2];
+    Chunk c{{0u, 0u}};
+    const int i = beg + lane;
+    if (i < my_e) {
+      const int grp = static_cast<uint32_t>(i) / static_cast<uint32_t>(n_seq);
+      const int r = i - grp * n_seq;
+      const int b = find_seq(pre, B, r), j = r - pre[b], ctx = s_ctx[b];
+      const int kvh = hgroups == 1 ? grp : grp / hgroups;
+      const int32_t* row = p.tables + static_cast<int64_t>(b) * p.table_stride;
+      int blk[2];
       uint32_t sub[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const uint32_t tile = 2 * j + k;  // tile of the sequence; BS / 16 tiles a block
         const uint32_t bi = static_cast<uint32_t>((static_cast<uint64_t>(tile) * p.tile_div) >> 32);
-        valid[k] = max(0, min(16, ctx - 16 * static_cast<int>(tile)));
-        blk[k] = valid[k] > 0 ? __ldg(row + bi) : 0;
+        blk[k] = 16 * static_cast<int>(tile) < ctx ? __ldg(row + bi) : -1;
         sub[k] = tile - bi * (BS >> 4);
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        if (blk[k] < 0 || blk[k] >= p.num_blocks) {
-          flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
-          valid[k] = 0;
-        }
-        // K rows of (layer, block, kv head): 2 BS rows of K and V per tile of the pool
-        if (valid[k] > 0)
+        if (blk[k] >= 0 && blk[k] < p.num_blocks) {
+          // rows of (layer, block, kv head) in the pool: 2 BS of K and V
           c.row16[k] = static_cast<uint32_t>((p.layer_tiles + static_cast<int64_t>(blk[k]) * p.hkv + kvh) * (BS >> 3)) + sub[k];
-        c.meta |= valid[k] << (5 * k);
+        } else if (16 * (2 * j + k) < ctx) {
+          flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
+          c.row16[k] = kBad;
+        }
+      }
+      if (i == my_a) {
+        seg_grp = grp;
+        seg_b = b;
+        seg_j = j;
       }
     }
+    any_bad = any_bad || __any_sync(0xffffffffu, (c.row16[0] | c.row16[1]) & kBad);
     return c;
   };
   Chunk cur{}, nxt{};
-  bool c_ok = false, n_ok = false;
-  if (my_e > my_a) {
+  if (my_a < my_e) {
     cur = build_chunk(my_a);
-    c_ok = true;
-    if (my_a + cur.n < my_e) {
-      nxt = build_chunk(my_a + cur.n);
-      n_ok = true;
-    }
+    seg_grp = __shfl_sync(0xffffffffu, seg_grp, 0);
+    seg_b = __shfl_sync(0xffffffffu, seg_b, 0);
+    seg_j = __shfl_sync(0xffffffffu, seg_j, 0);
+    if (my_e - my_a > 32) nxt = build_chunk(my_a + 32);
   }
-  int ib = 0;
-  int in_flight = 0;
-  uint32_t st_in = 0, st = 0;                    // ring stages: next to fill, next to read
-  int slot_meta = 0, slot_grp = 0, slot_b = 0;   // lane s: of ring stage s
-  const uint32_t ring_u = smem_u32(ring);
-  const uint64_t pol = l2_policy_evict_first();
-  // Row pi(r) of a tile is the token at index r of the products: chosen so
-  // that the lanes of one shared-memory phase read distinct banks - D 64: four
-  // K rows of 32 bytes are 0, 1, 2, 3 modulo 4; D 128: two K rows differ in
-  // parity; both: a V load's four tokens differ modulo 4.
-  auto pi = [](int r) { return (r & 1) ? 4 + (((r >> 1) + (D == 64 ? 2 : 1)) & 3) : r >> 1; };
-  // D 128: 16-byte column c of row r is kept at c ^ 2 ((r >> 1) & 1), so that
-  // V's 8-byte reads of four tokens spread over all banks
-  auto swz = [](int row) { return D == 128 ? ((row >> 1) & 1) << 1 : 0; };
-  // per-lane ends of the copies: 16-byte piece lane (and lane + 32) of a code
-  // tile, piece lane % 4 of the K (lane < 4) or V (lane < 8) parameters
-  uint32_t cp_dst[D / 64];
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const int ch = lane + 32 * i;
-    cp_dst[i] = ring_u + (D == 128 ? (ch >> 2) * 64 + (((ch & 3) ^ swz(ch >> 2)) << 4) : ch * 16);
-  }
-  const uint32_t cp_par = ring_u + 2 * G::kCodeBytes + lane * 16;
-  const uint8_t* const src_k = p.codes + lane * 16;
-  const uint8_t* const src_v = src_k + static_cast<int64_t>(BS) * (D / 2);
-  const char* const src_par = reinterpret_cast<const char*>(p.params) + (lane & 3) * 16 + ((lane >> 2) & 1) * (static_cast<int64_t>(BS) * 4);
-  auto issue_one = [&]() {
-    const int mt = __shfl_sync(0xffffffffu, cur.meta, ib);
-    const int grp = __shfl_sync(0xffffffffu, cur.grp, ib), b = __shfl_sync(0xffffffffu, cur.b, ib);
-    const uint32_t r0 = __shfl_sync(0xffffffffu, cur.row16[0], ib), r1 = __shfl_sync(0xffffffffu, cur.row16[1], ib);
-    const uint32_t off = st_in * G::kStage;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (mt & (31 << (5 * k))) {
-        const uint64_t row = k ? r1 : r0;
-        const uint8_t* ks = src_k + row * G::kCodeBytes;
-        const uint8_t* vs = src_v + row * G::kCodeBytes;
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          cp_async16_hint(cp_dst[i] + off + k * G::kTile, ks + 512 * i, pol);
-          cp_async16_hint(cp_dst[i] + off + k * G::kTile + G::kCodeBytes, vs + 512 * i, pol);
-        }
-        if (lane < 8) cp_async16(cp_par + off + k * G::kTile, src_par + row * 64);
-      }
-    }
-    cp_async_commit();
-    if (lane == static_cast<int>(st_in)) {
-      slot_meta = mt;
-      slot_grp = grp;
-      slot_b = b;
-    }
-    st_in = st_in + 1 == kS ? 0 : st_in + 1;
-    ++in_flight;
-    ++ib;
-    if (mt & (1 << 14)) {
-      c_ok = n_ok;
-      cur = nxt;
-      ib = 0;
-      n_ok = false;
-      if (c_ok && cur.beg + cur.n < my_e) {
-        nxt = build_chunk(cur.beg + cur.n);
-        n_ok = true;
-      }
-    }
-  };
 
   // Only lengths and tables have been read so far; the pool and q may still be
   // being written by the stream predecessor, the workspace be read by it.
   pdl_wait();
   pdl_launch_dependents();
-#pragma unroll 1
-  for (int i = 0; i < kS && c_ok; ++i) issue_one();
-
+  // Row pi(r) of a tile is the token at index r (0 .. 7; those of 8 .. 15 are 8
+  // rows on) of the products: the four tokens of a lane group's V load are
+  // adjacent rows, one run of memory.
+  auto pi = [](int r) { return (r >> 1) + 4 * (r & 1); };
   uint32_t qb[HT][kM][2];         // B fragments of q
   float qs[HT][2];                // sum(q) of heads 2 t, 2 t + 1
   float o[HT][kM][4];             // (element of row g | g + 8) x (head 2 t | 2 t + 1)
@@ -348,29 +269,87 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
   float l[HT][2], z[HT][2];       // sum p, sum p mid
   float kfac = 0.f;               // score of one unit of the accumulator, per step
   float vscale = 1.f, vlim = 0.f; // scale of p step; the largest step it allows
-  int grp = 0, b = 0;
-  bool whole = false, fresh = true;  // fresh: no score seen yet
-  int pieces = 0;
+  int n_pieces = 0;
   const float sc = p.scale_log2;
   const int row0 = pi(g);         // tokens of rows g and g + 8: row0, 8 + row0
-  const uint32_t k_row = D == 64 ? row0 * 32 + t * 8 : row0 * 64 + ((t ^ swz(row0)) << 4);  // swz(row0 + 8) == swz(row0)
-  uint32_t v_row[2];              // V: tokens of products 2 t, 2 t + 1 (those of 2 t + 8, 2 t + 9: 8 rows on)
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = pi(2 * t + r);
-    v_row[r] = G::kCodeBytes + (D == 64 ? row * 32 + g * 4 : row * 64 + (((g >> 1) ^ swz(row)) << 4) + (g & 1) * 8);
-  }
-  const uint32_t par_off = (lane >> 4) * G::kTile + 2 * G::kCodeBytes + (lane & 15) * 4;  // K parameters of token ``lane``
 
-  while (in_flight) {
-    const int mt = __shfl_sync(0xffffffffu, slot_meta, st);
-    if (mt & (1 << 10)) {
-      // ---- a sequence's first item here: q fragments --------------------------
-      grp = __shfl_sync(0xffffffffu, slot_grp, st);
-      b = __shfl_sync(0xffffffffu, slot_b, st);
-      whole = mt & (1 << 12);
-      fresh = true;
-      const int kvh = hgroups == 1 ? grp : grp / hgroups, h0 = (grp - kvh * hgroups) * kRows;
+  // An item's codes and parameters live in registers; each part of the next
+  // item is loaded as soon as this item's part has been used, so about one
+  // item per warp (2.3 KB at D 64, 37 KB an SM) is always on its way.
+  using KVec = typename std::conditional<D == 64, uint2, uint4>::type;
+  using VVec = typename std::conditional<D == 64, uint32_t, uint2>::type;
+  KVec kx[2][2];
+  VVec vx[2][4];
+  uint32_t kpar = 0, vpar = 0;    // parameters of token ``lane`` of the item
+  uint32_t bad = 0, bad_next = 0; // bit k: tile k's block is outside the pool
+  const uint8_t* const src_k = p.codes + row0 * (D / 2) + t * (D / 8);
+  const uint8_t* const src_v = p.codes + static_cast<int64_t>(BS) * (D / 2) + pi(2 * t) * (D / 2) + g * (D / 16);
+  const char* const src_par = reinterpret_cast<const char*>(p.params) + (lane & 15) * 4;
+  const int64_t par_v = static_cast<int64_t>(BS) * 4;
+  int next = my_a;                // next item to load
+  uint32_t r0 = 0, r1 = 0;        // its tiles
+  auto advance = [&]() {  // past the run's end: item 0 of the pool, read and not used
+    if (next < my_e) {
+      const int ib = (next - my_a) & 31;
+      r0 = __shfl_sync(0xffffffffu, cur.row16[0], ib);
+      r1 = __shfl_sync(0xffffffffu, cur.row16[1], ib);
+      if (any_bad) {
+        bad_next = (r0 >> 31) | (r1 >> 31) << 1;
+        r0 &= ~kBad;
+        r1 &= ~kBad;
+      }
+      ++next;
+      if (ib == 31) {
+        cur = nxt;
+        if (my_e - next > 32) nxt = build_chunk(next + 32);
+      }
+    }
+  };
+  auto load_k = [&]() {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint8_t* src = src_k + static_cast<uint64_t>(k ? r1 : r0) * G::kCodeBytes;
+      kx[k][0] = __ldcs(reinterpret_cast<const KVec*>(src));
+      kx[k][1] = __ldcs(reinterpret_cast<const KVec*>(src + 8 * (D / 2)));
+    }
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint8_t* src = src_v + static_cast<uint64_t>(k ? r1 : r0) * G::kCodeBytes;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)  // tokens of products 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        vx[k][r] = __ldcs(reinterpret_cast<const VVec*>(src + ((r & 1) * 4 + (r >> 1) * 8) * (D / 2)));
+    }
+  };
+  auto load_par = [&]() {
+    const char* src = src_par + static_cast<uint64_t>(lane < 16 ? r0 : r1) * 64;
+    kpar = __ldcs(reinterpret_cast<const uint32_t*>(src));
+    vpar = __ldcs(reinterpret_cast<const uint32_t*>(src + par_v));
+  };
+  if (my_a < my_e) {
+    advance();
+    bad = bad_next;
+    load_par();
+    load_k();
+    load_v();
+  }
+
+  for (int at = my_a; at < my_e;) {
+    // ---- the warp's share of one sequence: items seg_j .. of (seg_grp, seg_b) ----
+    const int grp = seg_grp, b = seg_b, ctx = s_ctx[b], ni = items_of(ctx);
+    int todo = min(ni - seg_j, my_e - at);
+    const bool whole = todo == ni;
+    int tokens = ctx - 32 * seg_j;  // from this item on
+    at += todo;
+    seg_j = 0;
+    if (++seg_b == B) {
+      seg_b = 0;
+      ++seg_grp;
+    }
+    bool fresh = true;  // no score seen yet
+    const int kvh = hgroups == 1 ? grp : grp / hgroups, h0 = (grp - kvh * hgroups) * kRows;
+    {
       uint4 x[HT][kWords];  // 8 elements each: those of one code word
       float top = 0.f;
 #pragma unroll
@@ -426,21 +405,19 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
       vscale = 1.f;
       vlim = 0.f;
     }
-    // the oldest copy is complete once at most the newer ones are pending;
-    // near the end of the run fewer are pending than that, so wait for all
-    if (in_flight == kS) cp_async_wait<kS - 1>(); else cp_async_wait<0>();
-    __syncwarp();
-    if (mt & 1023) {
-      const uint8_t* const item = ring + st * G::kStage;
-      const int valid0 = mt & 31, valid1 = (mt >> 5) & 31;
+    for (; todo > 0; --todo, tokens -= 32) {
+      const bool all = tokens >= 32 && bad == 0;
+      int valid0 = 16, valid1 = 16;
+      if (!all) {
+        valid0 = bad & 1 ? 0 : max(0, min(16, tokens));
+        valid1 = bad & 2 ? 0 : max(0, min(16, tokens - 16));
+      }
+      const bool some = valid0 + valid1 > 0;
+      advance();
+      bad = bad_next;
       // ---- the tokens' factors, one token a lane ---------------------------------
       {
-        const bool live = (lane & 15) < (lane < 16 ? valid0 : valid1);  // rows past the context may hold anything
-        uint32_t kpar = 0, vpar = 0;
-        if (live) {
-          kpar = *reinterpret_cast<const uint32_t*>(item + par_off);
-          vpar = *reinterpret_cast<const uint32_t*>(item + par_off + 64);
-        }
+        if (!all && (lane & 15) >= (lane < 16 ? valid0 : valid1)) kpar = vpar = 0;  // rows past the context may hold anything
         const float2 kp = unpack2<T>(kpar), vp = unpack2<T>(vpar);
         if (__any_sync(0xffffffffu, vp.x > vlim)) {  // a larger step than the scale of p step allows
           float top = vp.x;
@@ -464,6 +441,7 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
         }
         // the code's -7.5 goes with mid
         factors[lane] = make_float4(kp.x * kfac, fmaf(kp.x, -7.5f, kp.y) * sc, vp.x * vscale, vp.y);
+        load_par();
       }
       // ---- S^T = K Q^T ---------------------------------------------------------
       float s[2][HT][4];
@@ -472,20 +450,12 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
         uint32_t kw[2][kWords], kw8[2][kWords];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint8_t* src = item + k * G::kTile + k_row + r * (8 * D / 2);
-          if constexpr (D == 64) {
-            const uint2 x = *reinterpret_cast<const uint2*>(src);
-            kw[r][0] = x.x;
-            kw[r][1] = x.y;
-          } else {
-            const uint4 x = *reinterpret_cast<const uint4*>(src);
-            kw[r][0] = x.x;
-            kw[r][1] = x.y;
-            kw[r][2] = x.z;
-            kw[r][3] = x.w;
-          }
+          const uint32_t* x = reinterpret_cast<const uint32_t*>(&kx[k][r]);
 #pragma unroll
-          for (int w = 0; w < kWords; ++w) kw8[r][w] = kw[r][w] >> 8;
+          for (int w = 0; w < kWords; ++w) {
+            kw[r][w] = x[w];
+            kw8[r][w] = x[w] >> 8;
+          }
         }
 #pragma unroll
         for (int i = 0; i < kM; ++i) {
@@ -499,6 +469,7 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
           }
         }
       }
+      load_k();
       __syncwarp();  // factors written
       // ---- scores minus reference (log2 scale) -----------------------------------
       float vs[2][2], vm[2][2];
@@ -520,7 +491,7 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
           }
         }
       }
-      if (valid0 < 16 || valid1 < 16) {
+      if (!all) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
 #pragma unroll
@@ -534,7 +505,7 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
       }
       // The reference moves only when some score is above it by more than the
       // limit: most items touch no accumulator.
-      bool grow = fresh;
+      bool grow = fresh && some;
 #pragma unroll
       for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
@@ -599,14 +570,9 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
         uint32_t vw[4][D / 64];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const uint8_t* src = item + k * G::kTile + v_row[r & 1] + (r >> 1) * (8 * D / 2);
-          if constexpr (D == 64) {
-            vw[r][0] = *reinterpret_cast<const uint32_t*>(src);
-          } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(src);
-            vw[r][0] = w.x;
-            vw[r][1] = w.y;
-          }
+          const uint32_t* x = reinterpret_cast<const uint32_t*>(&vx[k][r]);
+#pragma unroll
+          for (int w = 0; w < D / 64; ++w) vw[r][w] = x[w];
         }
 #pragma unroll
         for (int q = 0; q < D / 64; ++q) {
@@ -625,22 +591,15 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
         for (int ht = 0; ht < HT; ++ht)
           mma_16816<__half>(sp[ht], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[ht][0], pb[ht][1]);
       }
+      load_v();
+      __syncwarp();  // factors read
     }
-    __syncwarp();
-    --in_flight;
-    st = st + 1 == kS ? 0 : st + 1;
-    if (c_ok) issue_one();  // refill the stage just freed
-
-    if (mt & (1 << 11)) {
+    {
       // ---- the warp's share of the sequence is done ----------------------------
-      const int kvh = hgroups == 1 ? grp : grp / hgroups, h0 = (grp - kvh * hgroups) * kRows;
-      whole = whole && (mt & (1 << 13));
       float* piece = nullptr;
       if (!whole) {
-        // the first piece has its own place; the other one ends the run, when
-        // the warp's ring is free
-        const int k = pieces++;
-        piece = k == 0 ? pieces0 + warp * G::kPartFloats : reinterpret_cast<float*>(ring);
+        const int k = n_pieces++;  // a run's first share and its last
+        piece = pieces + (2 * warp + k) * G::kPartFloats;
         if (lane == 0) {
           s_grp[2 * warp + k] = grp;
           s_seq[2 * warp + k] = b;
@@ -698,6 +657,7 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
     }
   }
 
+
   // ---- join the pieces of this CTA ----------------------------------------------
   // Piece slot s = 2 warp + (0 | 1); the pieces of one sequence are a run of
   // slots (with empty ones between).  First the weights, a lane per slot and a
@@ -709,9 +669,7 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
   const uint32_t peers = __match_any_sync(0xffffffffu, key);
   const int first = __ffs(peers) - 1;
   uint32_t leaders = __ballot_sync(0xffffffffu, my_grp >= 0 && lane == first);
-  auto piece_of = [&](int s) -> const float* {
-    return (s & 1) ? reinterpret_cast<const float*>(smem + (s >> 1) * G::kRing) : pieces0 + (s >> 1) * G::kPartFloats;
-  };
+  auto piece_of = [&](int s) -> const float* { return pieces + s * G::kPartFloats; };
   for (int hr = warp; hr < kRows; hr += kW) {
     float2 ml = make_float2(-INFINITY, 0.f);
     if (my_grp >= 0) ml = *reinterpret_cast<const float2*>(piece_of(lane) + kRows * D + 2 * hr);
@@ -906,7 +864,7 @@ bool int4_decode_fast_geometry(int dtype, int batch, int hkv, int group, int hea
   const int rows = 8 * head_tiles(group);
   return (dtype == PSB_BF16 || dtype == PSB_F16) && (head_dim == 64 || head_dim == 128) && block_size % 16 == 0 &&
          batch <= kMaxBatch && max_items(batch, hkv, group, rows, max_context) < (int64_t(1) << 31) - 64 &&
-         static_cast<int64_t>(num_layers) * num_blocks * hkv * 2 * (block_size / 16) < (int64_t(1) << 32) &&
+         static_cast<int64_t>(num_layers) * num_blocks * hkv * 2 * (block_size / 16) < (int64_t(1) << 31) &&
          static_cast<int64_t>(max_context / 16 + 2) * (block_size / 16) < (int64_t(1) << 32);
 }
 

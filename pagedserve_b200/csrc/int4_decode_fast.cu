@@ -80,6 +80,22 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
+// max(a, |x|) of packed pairs, a NaN in x passed over
+template <typename T>
+__device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t x);
+template <>
+__device__ __forceinline__ uint32_t abs_max2<__nv_bfloat16>(uint32_t a, uint32_t x) {
+  uint32_t d;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(x & 0x7fff7fffu));
+  return d;
+}
+template <>
+__device__ __forceinline__ uint32_t abs_max2<__half>(uint32_t a, uint32_t x) {
+  uint32_t d;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(x & 0x7fff7fffu));
+  return d;
+}
+
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
 // Pair i (0 .. 3) of a code word, its nibbles i and i + 4, as two f16: c 2^-24
@@ -233,6 +249,8 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
         } else if (16 * (2 * j + k) < ctx) {
           flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
           c.row16[k] = kBad;
+        } else if (k == 1) {
+          c.row16[1] = c.row16[0] & ~kBad;  // no second tile: the first one again
         }
       }
       if (i == my_a) {
@@ -327,7 +345,23 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
     kpar = __ldcs(reinterpret_cast<const uint32_t*>(src));
     vpar = __ldcs(reinterpret_cast<const uint32_t*>(src + par_v));
   };
+  uint4 x[HT][kWords];  // q rows of a share: 8 elements a code word
+  auto load_q = [&](int grp, int b) {
+    const int kvh = hgroups == 1 ? grp : grp / hgroups, h0 = (grp - kvh * hgroups) * kRows;
+#pragma unroll
+    for (int ht = 0; ht < HT; ++ht) {
+      const int hh = h0 + ht * 8 + g;
+      const bool live = hh < p.group;
+      const T* src = reinterpret_cast<const T*>(p.q) + b * p.qsb + (kvh * p.group + (live ? hh : 0)) * p.qsh + t * (D / 4);
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        x[ht][w] = make_uint4(0, 0, 0, 0);
+        if (live) x[ht][w] = *reinterpret_cast<const uint4*>(src + 8 * w);
+      }
+    }
+  };
   if (my_a < my_e) {
+    load_q(seg_grp, seg_b);
     advance();
     bad = bad_next;
     load_par();
@@ -338,6 +372,7 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
   for (int at = my_a; at < my_e;) {
     // ---- the warp's share of one sequence: items seg_j .. of (seg_grp, seg_b) ----
     const int grp = seg_grp, b = seg_b, ctx = s_ctx[b], ni = items_of(ctx);
+    if (at != my_a) load_q(grp, b);  // the first share's were loaded before its codes
     int todo = min(ni - seg_j, my_e - at);
     const bool whole = todo == ni;
     int tokens = ctx - 32 * seg_j;  // from this item on
@@ -350,23 +385,31 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
     bool fresh = true;  // no score seen yet
     const int kvh = hgroups == 1 ? grp : grp / hgroups, h0 = (grp - kvh * hgroups) * kRows;
     {
-      uint4 x[HT][kWords];  // 8 elements each: those of one code word
-      float top = 0.f;
+      uint32_t top2 = 0;
 #pragma unroll
       for (int ht = 0; ht < HT; ++ht) {
-        const int hh = h0 + ht * 8 + g;
-        const bool live = hh < p.group;
-        const T* src = reinterpret_cast<const T*>(p.q) + b * p.qsb + (kvh * p.group + (live ? hh : 0)) * p.qsh + t * (D / 4);
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
-          x[ht][w] = make_uint4(0, 0, 0, 0);
-          if (live) x[ht][w] = *reinterpret_cast<const uint4*>(src + 8 * w);
           const uint32_t* e = &x[ht][w].x;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack2<T>(e[i]);
-            if (finite_f32(f.x)) top = fmaxf(top, fabsf(f.x));
-            if (finite_f32(f.y)) top = fmaxf(top, fabsf(f.y));
+          for (int i = 0; i < 4; ++i) top2 = abs_max2<T>(top2, e[i]);
+        }
+      }
+      const float2 top_f = unpack2<T>(top2);
+      float top = fmaxf(top_f.x, top_f.y);
+      if (!finite_f32(top)) {  // an infinity: its own head's affair, the others keep their scale
+        top = 0.f;
+#pragma unroll
+        for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) {
+            const uint32_t* e = &x[ht][w].x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = unpack2<T>(e[i]);
+              if (finite_f32(f.x)) top = fmaxf(top, fabsf(f.x));
+              if (finite_f32(f.y)) top = fmaxf(top, fabsf(f.y));
+            }
           }
         }
       }
@@ -425,19 +468,21 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
           for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
           const int e = max(-100, ilogb_f32(top)) + 1;  // top < 2^e
           const float nv = exp2_int(kPBits - e);
-          const float ratio = fresh ? 0.f : nv / vscale;  // the sums are zero before the first score
+          if (!fresh) {
+            const float ratio = nv / vscale;
+#pragma unroll
+            for (int ht = 0; ht < HT; ++ht) {
+#pragma unroll
+              for (int i = 0; i < kM; ++i) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[ht][i][k] *= ratio;
+              }
+              sp[ht][0] *= ratio;
+              sp[ht][1] *= ratio;
+            }
+          }
           vlim = exp2_int(min(e, 127));
           vscale = nv;
-#pragma unroll
-          for (int ht = 0; ht < HT; ++ht) {
-#pragma unroll
-            for (int i = 0; i < kM; ++i) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) o[ht][i][k] *= ratio;
-            }
-            sp[ht][0] *= ratio;
-            sp[ht][1] *= ratio;
-          }
         }
         // the code's -7.5 goes with mid
         factors[lane] = make_float4(kp.x * kfac, fmaf(kp.x, -7.5f, kp.y) * sc, vp.x * vscale, vp.y);
@@ -526,25 +571,30 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             // the first reference is the first maximum (finite whatever the scores are)
             mx = fresh ? fminf(fmaxf(mx, -3e38f), 3e38f) : fmaxf(mx, 0.f);
-            al[e] = fresh ? 0.f : ex2_approx(-mx);
+            al[e] = ex2_approx(-mx);
             nref[ht][e] -= mx;
-            l[ht][e] *= al[e];
-            z[ht][e] *= al[e];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               s[k][ht][e] -= mx;
               s[k][ht][2 + e] -= mx;
             }
           }
+          if (!fresh) {
 #pragma unroll
-          for (int i = 0; i < kM; ++i) {
-            o[ht][i][0] *= al[0];
-            o[ht][i][1] *= al[1];
-            o[ht][i][2] *= al[0];
-            o[ht][i][3] *= al[1];
+            for (int e = 0; e < 2; ++e) {
+              l[ht][e] *= al[e];
+              z[ht][e] *= al[e];
+            }
+#pragma unroll
+            for (int i = 0; i < kM; ++i) {
+              o[ht][i][0] *= al[0];
+              o[ht][i][1] *= al[1];
+              o[ht][i][2] *= al[0];
+              o[ht][i][3] *= al[1];
+            }
+            sp[ht][0] *= al[0];
+            sp[ht][1] *= al[1];
           }
-          sp[ht][0] *= al[0];
-          sp[ht][1] *= al[1];
         }
         fresh = false;
       }
@@ -659,32 +709,41 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
 
 
   // ---- join the pieces of this CTA ----------------------------------------------
-  // Piece slot s = 2 warp + (0 | 1); the pieces of one sequence are a run of
-  // slots (with empty ones between).  First the weights, a lane per slot and a
-  // warp per q head, then the outputs, a thread per element.
+  // Piece slot s = 2 warp + (0 | 1); slots are in item order, so the pieces of
+  // one sequence are consecutive (with empty slots between).  First the
+  // weights, a lane per slot and a warp per q head, then the outputs, a group
+  // of threads per sequence.
   __syncthreads();
   const int my_grp = lane < 2 * kW ? s_grp[lane] : -1;
-  const int my_b = my_grp >= 0 ? s_seq[lane] : -1 - lane;
-  const uint64_t key = (static_cast<uint64_t>(static_cast<uint32_t>(my_grp)) << 32) | static_cast<uint32_t>(my_b);
-  const uint32_t peers = __match_any_sync(0xffffffffu, key);
-  const int first = __ffs(peers) - 1;
-  uint32_t leaders = __ballot_sync(0xffffffffu, my_grp >= 0 && lane == first);
-  auto piece_of = [&](int s) -> const float* { return pieces + s * G::kPartFloats; };
+  const int my_b = my_grp >= 0 ? s_seq[lane] : 0;
+  const uint32_t used = __ballot_sync(0xffffffffu, my_grp >= 0);
+  const uint32_t below = used & ((1u << lane) - 1u);
+  const int prev = below ? 31 - __clz(below) : lane;
+  const int prev_grp = __shfl_sync(0xffffffffu, my_grp, prev), prev_b = __shfl_sync(0xffffffffu, my_b, prev);
+  const bool same = below != 0 && prev_grp == my_grp && prev_b == my_b;
+  const uint32_t leaders = __ballot_sync(0xffffffffu, my_grp >= 0 && !same);
+  const uint32_t upto = leaders & ((2u << lane) - 1u);
+  const int lead = upto ? 31 - __clz(upto) : 0;                // first slot of the lane's run
+  const uint32_t after = leaders & ~((2u << lane) - 1u);
+  const int last = after ? __ffs(after) - 2 : 31;              // its last slot (maybe an empty one)
   for (int hr = warp; hr < kRows; hr += kW) {
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (my_grp >= 0) ml = *reinterpret_cast<const float2*>(piece_of(lane) + kRows * D + 2 * hr);
+    if (my_grp >= 0) ml = *reinterpret_cast<const float2*>(pieces + lane * G::kPartFloats + kRows * D + 2 * hr);
     float mx = ml.x;
-    for (uint32_t r = peers; __any_sync(0xffffffffu, r); r &= r - 1) {
-      const float v = __shfl_sync(0xffffffffu, ml.x, r ? __ffs(r) - 1 : lane);
-      mx = fmaxf(mx, v);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const float v = __shfl_up_sync(0xffffffffu, mx, d);
+      if (lane - d >= lead) mx = fmaxf(mx, v);
     }
+    mx = __shfl_sync(0xffffffffu, mx, last);
     const float w = my_grp >= 0 ? ex2_approx(ml.x - (mx == -INFINITY ? 0.f : mx)) : 0.f;
-    const float lw = ml.y * w;
-    float sum = 0.f;
-    for (uint32_t r = peers; __any_sync(0xffffffffu, r); r &= r - 1) {
-      const float v = __shfl_sync(0xffffffffu, lw, r ? __ffs(r) - 1 : lane);
-      if (r) sum += v;
+    float sum = ml.y * w;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const float v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane - d >= lead) sum += v;
     }
+    sum = __shfl_sync(0xffffffffu, sum, last);
     if (lane < 2 * kW) {
       s_w[hr * 2 * kW + lane] = w;
       s_ml[hr * 2 * kW + lane] = make_float2(mx, sum);
@@ -694,7 +753,7 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
   const int u_a = my_grp >= 0 ? my_grp * n_seq + pre[my_b] : 0;
   const int u_e = my_grp >= 0 ? my_grp * n_seq + pre[my_b + 1] : 0;
   const bool cut_a = u_a < cta_a, cut_e = u_e > cta_e;
-  if (warp == 0) {
+  if (warp == kW - 1) {
     // the sequence that begins here and runs past the end of the CTA, if any
     const uint32_t tail = __ballot_sync(0xffffffffu, my_grp >= 0 && cut_e && !cut_a);
     Cut c{0, 0, 0, 0};
@@ -714,28 +773,43 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
     if (lane == 0) cuts[blockIdx.x] = c;
   }
   __syncthreads();
-  for (; leaders; leaders &= leaders - 1) {
-    const int lead = __ffs(leaders) - 1;
-    const uint32_t run = __shfl_sync(0xffffffffu, peers, lead);
-    const int rg = __shfl_sync(0xffffffffu, my_grp, lead), rb = __shfl_sync(0xffffffffu, my_b, lead);
-    const bool ca = __shfl_sync(0xffffffffu, cut_a, lead), ce = __shfl_sync(0xffffffffu, cut_e, lead);
+  // a group of kRows D / 4 threads per run, four elements a thread
+  constexpr int kGroup = kRows * D / 4, kGroups = G::kThreads >= kGroup ? G::kThreads / kGroup : 1;
+  const int my_group = kGroups == 1 ? 0 : tid / kGroup;
+  uint32_t runs = leaders;
+  for (int k = 0; runs; runs &= runs - 1, ++k) {
+    const int r0s = __ffs(runs) - 1;
+    const uint32_t later = runs & (runs - 1);
+    const uint32_t run = used & (later ? (1u << (__ffs(later) - 1)) - 1u : ~0u) & ~((1u << r0s) - 1u);
+    const int rg = __shfl_sync(0xffffffffu, my_grp, r0s), rb = __shfl_sync(0xffffffffu, my_b, r0s);
+    const bool ca = __shfl_sync(0xffffffffu, cut_a, r0s), ce = __shfl_sync(0xffffffffu, cut_e, r0s);
+    if (my_group >= kGroups || k % kGroups != my_group) continue;  // warp-uniform: a group is whole warps
     const int kvh = hgroups == 1 ? rg : rg / hgroups, h0 = (rg - kvh * hgroups) * kRows;
-    for (int e = tid; e < kRows * D; e += G::kThreads) {
-      const int hr = e / D, d = e - hr * D;
-      float acc = 0.f;
+    for (int e = kGroups == 1 ? tid : tid - my_group * kGroup; e < kGroup; e += kGroups == 1 ? G::kThreads : kGroup) {
+      const int hr = e / (D / 4), d = 4 * (e - hr * (D / 4));
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       for (uint32_t r = run; r; r &= r - 1) {
         const int sl = __ffs(r) - 1;
-        acc = fmaf(piece_of(sl)[e], s_w[hr * 2 * kW + sl], acc);
+        const float w = s_w[hr * 2 * kW + sl];
+        const float4 v = *reinterpret_cast<const float4*>(pieces + sl * G::kPartFloats + 4 * e);
+        acc.x = fmaf(v.x, w, acc.x);
+        acc.y = fmaf(v.y, w, acc.y);
+        acc.z = fmaf(v.z, w, acc.z);
+        acc.w = fmaf(v.w, w, acc.w);
       }
-      const float2 ml = s_ml[hr * 2 * kW + lead];
+      const float2 ml = s_ml[hr * 2 * kW + r0s];
       if (!ca && !ce) {
-        if (h0 + hr < p.group)
-          reinterpret_cast<T*>(p.out)[rb * p.osb + (kvh * p.group + h0 + hr) * p.osh + d] =
-              Elem<T>::from_float(ml.y == 0.f ? 0.f : acc / ml.y);
+        if (h0 + hr < p.group) {
+          const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+          uint2 v;
+          v.x = pack2<T>(acc.x * inv, acc.y * inv);
+          v.y = pack2<T>(acc.z * inv, acc.w * inv);
+          *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + rb * p.osb + (kvh * p.group + h0 + hr) * p.osh + d) = v;
+        }
       } else {
         // cut at the CTA's start (slot 0) or only at its end (slot 1)
         float* dst = part + static_cast<int64_t>(2 * blockIdx.x + (ca ? 0 : 1)) * G::kPartFloats;
-        dst[e] = acc;
+        *reinterpret_cast<float4*>(dst + 4 * e) = acc;
         if (d == 0) *reinterpret_cast<float2*>(dst + kRows * D + 2 * hr) = ml;
       }
     }

@@ -57,7 +57,7 @@ constexpr int kMinItems = 1;        // items per warp below which fewer CTAs tak
 
 template <int D, int HT>
 struct Geo {
-  static constexpr int kWarps = D * HT == 64 ? 16 : (D * HT == 128 ? 12 : 8);
+  static constexpr int kWarps = D * HT == 64 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kRows = 8 * HT;                  // q heads of a tile
   static constexpr int kCodeBytes = 16 * D / 2;         // K (or V) codes of 16 tokens

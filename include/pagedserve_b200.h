@@ -485,6 +485,12 @@ int psb_paged_decode_int4(const void* query, int64_t q_stride_b, int64_t q_strid
                           int32_t max_context, float scale, void* workspace, size_t workspace_bytes,
                           int32_t* error_flag, psb_stream_t stream);
 
+/* Workspace bytes of psb_paged_prefill_int4 (0 for an invalid geometry); the
+ * rules of psb_paged_decode_int4's. */
+size_t psb_paged_prefill_int4_workspace_size(int32_t total_tokens, int32_t num_seqs, int32_t q_heads,
+                                             int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                             int32_t max_context, int32_t dtype);
+
 /*
  * paged_prefill_int4: psb_paged_prefill over the 4-bit pool.  Sequence i's
  * query rows cu_seqlens[i] .. cu_seqlens[i+1] are the last positions of its
@@ -497,7 +503,8 @@ int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h
                            const int32_t* cu_seqlens, int32_t num_seqs, int32_t total_tokens, int32_t max_seqlen,
                            int32_t max_context, int32_t q_heads, int32_t layer, int32_t num_layers,
                            int64_t num_blocks, int32_t num_kv_heads, int32_t block_size, int32_t head_dim,
-                           int32_t dtype, float scale, int32_t* error_flag, psb_stream_t stream);
+                           int32_t dtype, float scale, void* workspace, size_t workspace_bytes, int32_t* error_flag,
+                           psb_stream_t stream);
 
 /*
  * extend_step: psb_pack_step that also allocates.  The host-side BlockManager

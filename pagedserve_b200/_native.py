@@ -105,9 +105,11 @@ SIGNATURES = {
     "psb_paged_decode_int4": (ctypes.c_int, [
         _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i32,
         _i32, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _c_void_p, _sz, _c_void_p, _c_void_p]),
+    "psb_paged_prefill_int4_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "psb_paged_prefill_int4": (ctypes.c_int, [
         _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p,
-        _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _c_void_p, _c_void_p]),
+        _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _c_void_p, _sz, _c_void_p,
+        _c_void_p]),
     "psb_extend_step": (ctypes.c_int, [
         _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _i32, _c_void_p, _i32, _i32,
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p]),

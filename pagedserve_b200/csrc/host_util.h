@@ -94,6 +94,11 @@ bool encode_pool_tile_map(CUtensorMap* map, const void* pool, int64_t tiles, int
 bool encode_rows_map(CUtensorMap* map, const void* base, int64_t rows, int heads, int head_dim, int64_t row_stride,
                      int64_t head_stride, int box_rows, CUtensorMapDataType dt);
 
+// The same with boxes of ``box_rows`` rows of ``box_heads`` consecutive heads:
+// in shared memory the heads of a row are consecutive 128-byte lines.
+bool encode_row_groups_map(CUtensorMap* map, const void* base, int64_t rows, int heads, int head_dim, int64_t row_stride,
+                           int64_t head_stride, int box_heads, int box_rows, CUtensorMapDataType dt);
+
 // 3D tensor map over a paged K or V pool [layers * blocks * kv heads tiles,
 // block_size rows, head_dim]: one box is one (layer, block, kv head) tile of
 // block_size x head_dim, 128-byte swizzled.

@@ -50,4 +50,11 @@ bool int4_decode_fast_geometry(int dtype, int batch, int hkv, int group, int hea
 size_t int4_decode_fast_workspace(int group, int head_dim);
 int int4_decode_fast_launch(const Int4DecodeParams& p, int dtype, cudaStream_t s);
 
+// Tensor-core prefill (int4_prefill_tc.cu): whether a geometry is covered, its
+// scratch bytes and the launch.  q rows start on 16 bytes.
+bool int4_prefill_tc_geometry(int dtype, int total, int num_seqs, int q_heads, int hkv, int head_dim, int block_size,
+                              int max_context);
+size_t int4_prefill_tc_workspace();
+int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspace, cudaStream_t s);
+
 }  // namespace psb

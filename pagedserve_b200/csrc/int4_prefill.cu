@@ -143,6 +143,17 @@ __global__ void check_seqlens_kernel(const int32_t* cu, int32_t n, int32_t total
 
 using namespace psb;
 
+extern "C" size_t psb_paged_prefill_int4_workspace_size(int32_t total_tokens, int32_t num_seqs, int32_t q_heads,
+                                                        int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                                        int32_t max_context, int32_t dtype) {
+  if (total_tokens < 0 || num_seqs < 0 || num_kv_heads <= 0 || q_heads <= 0 || q_heads % num_kv_heads ||
+      head_dim <= 0 || head_dim % 2 || head_dim > kInt4MaxDim || block_size <= 0 || max_context < 0 ||
+      (dtype != PSB_F32 && dtype != PSB_F16 && dtype != PSB_BF16))
+    return 0;
+  return int4_prefill_tc_geometry(dtype, total_tokens, num_seqs, q_heads, num_kv_heads, head_dim, block_size, max_context)
+             ? int4_prefill_tc_workspace() : 256;
+}
+
 extern "C" int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv_codes,
                                       const void* kv_params, const int32_t* block_tables, int64_t table_stride,
                                       const int32_t* context_lens, void* out, int64_t o_stride_t, int64_t o_stride_h,
@@ -150,7 +161,8 @@ extern "C" int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t
                                       int32_t max_seqlen, int32_t max_context, int32_t q_heads, int32_t layer,
                                       int32_t num_layers, int64_t num_blocks, int32_t num_kv_heads,
                                       int32_t block_size, int32_t head_dim, int32_t dtype, float scale,
-                                      int32_t* error_flag, psb_stream_t stream) {
+                                      void* workspace, size_t workspace_bytes, int32_t* error_flag,
+                                      psb_stream_t stream) {
   if (num_seqs < 0 || total_tokens < 0 || max_seqlen < 0 || max_context < max_seqlen || q_heads <= 0 ||
       num_kv_heads <= 0 || q_heads % num_kv_heads || head_dim <= 0 || head_dim % 2 || head_dim > kInt4MaxDim ||
       num_layers <= 0 || layer < 0 || layer >= num_layers || num_blocks <= 0 || block_size <= 0 ||
@@ -159,8 +171,13 @@ extern "C" int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t
   if (dtype != PSB_F32 && dtype != PSB_F16 && dtype != PSB_BF16) return PSB_ERR_INVALID;
   if (num_seqs == 0 || total_tokens == 0) return PSB_OK;
   if (!q || !kv_codes || !kv_params || !out || !cu_seqlens || !block_tables || !context_lens) return PSB_ERR_INVALID;
-  if (reinterpret_cast<uintptr_t>(kv_codes) % 16 || reinterpret_cast<uintptr_t>(kv_params) % 16)
+  if (reinterpret_cast<uintptr_t>(kv_codes) % 16 || reinterpret_cast<uintptr_t>(kv_params) % 16 ||
+      reinterpret_cast<uintptr_t>(workspace) % 16)
     return PSB_ERR_INVALID;
+  if (workspace == nullptr ||
+      workspace_bytes < psb_paged_prefill_int4_workspace_size(total_tokens, num_seqs, q_heads, num_kv_heads, head_dim,
+                                                              block_size, max_context, dtype))
+    return PSB_ERR_WORKSPACE;
   Int4PrefillParams p;
   p.q = q;
   p.qst = q_stride_t;
@@ -191,6 +208,12 @@ extern "C" int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t
     discard_stale_error();
     check_seqlens_kernel<<<1, 256, 0, s>>>(cu_seqlens, num_seqs, total_tokens, error_flag);
   }
+  // the tensor-core path reads q by TMA: 16-byte bases and strides
+  const bool aligned = q_stride_t % 8 == 0 && q_stride_h % 8 == 0 && q_stride_t > 0 && q_stride_h > 0 &&
+                       reinterpret_cast<uintptr_t>(q) % 16 == 0;
+  if (aligned && int4_prefill_tc_geometry(dtype, total_tokens, num_seqs, q_heads, num_kv_heads, head_dim, block_size,
+                                          max_context))
+    return int4_prefill_tc_launch(p, dtype, static_cast<float*>(workspace), s);
   switch (dtype) {
     case PSB_BF16: return launch_generic<__nv_bfloat16>(p, s);
     case PSB_F16: return launch_generic<__half>(p, s);

@@ -832,13 +832,22 @@ def paged_decode_int4(query: torch.Tensor, kv_codes: torch.Tensor, kv_params: to
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def prefill_int4_workspace_bytes(total: int, num_seqs: int, q_heads: int, hkv: int, head_dim: int, block_size: int,
+                                 max_context: int, dtype: torch.dtype) -> int:
+    lib = _native.load()
+    return int(lib.psb_paged_prefill_int4_workspace_size(total, num_seqs, q_heads, hkv, head_dim, block_size,
+                                                         max_context, dtype_code(dtype)))
+
+
 def paged_prefill_int4(q: torch.Tensor, kv_codes: torch.Tensor, kv_params: torch.Tensor, block_tables: torch.Tensor,
                        context_lens: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int, layer: int,
                        scale: float | None = None, out: torch.Tensor | None = None, max_context: int | None = None,
-                       error_flag: torch.Tensor | None = None) -> torch.Tensor:
+                       workspace: torch.Tensor | None = None, error_flag: torch.Tensor | None = None) -> torch.Tensor:
     """``paged_prefill`` over a 4-bit pool (psb_paged_prefill_int4): ``q [T,
     Hq, D]`` of ``kv_params``' dtype, the rest as in ``paged_prefill``.  Rows
-    of ``out`` that belong to no sequence keep what they held."""
+    of ``out`` that belong to no sequence keep what they held.  Scratch as in
+    ``paged_decode_int4`` (``prefill_int4_workspace_bytes``)."""
     nl, nb, hkv, bs, d = _int4_geometry(kv_codes, kv_params)
     if q.ndim != 3 or q.shape[2] != d:
         raise ValueError(f"q must be [T, Hq, {d}]")
@@ -872,18 +881,24 @@ def paged_prefill_int4(q: torch.Tensor, kv_codes: torch.Tensor, kv_params: torch
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     _check_flag(error_flag)
     dev = kv_codes.device
-    _one_device(dev, q, kv_params, block_tables, context_lens, cu_seqlens, out, error_flag)
+    _one_device(dev, q, kv_params, block_tables, context_lens, cu_seqlens, out, workspace, error_flag)
     if out is None:
         out = torch.empty(q.shape, dtype=dtype, device=dev)
     if out.shape != q.shape or out.stride(2) != 1 or out.dtype != dtype:
         raise ValueError("out must match q with unit stride along head_dim")
+    if workspace is None:
+        workspace = torch.empty(prefill_int4_workspace_bytes(t, batch, hq, hkv, d, bs, int(max_context), dtype),
+                                dtype=torch.uint8, device=dev)
+    elif not workspace.is_contiguous() or workspace.data_ptr() % 16:
+        raise ValueError("workspace must be contiguous and start on 16 bytes")
     lib = _native.load()
     with _on(dev):
         _native.check(lib.psb_paged_prefill_int4(
             q.data_ptr(), q.stride(0), q.stride(1), kv_codes.data_ptr(), kv_params.data_ptr(),
             block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(), out.data_ptr(), out.stride(0),
             out.stride(1), cu_seqlens.data_ptr(), batch, t, int(max_seqlen), int(max_context), hq, layer, nl, nb, hkv,
-            bs, d, _DTYPES[dtype], scale, _ptr(error_flag), _stream(dev)), "paged_prefill_int4")
+            bs, d, _DTYPES[dtype], scale, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+            _ptr(error_flag), _stream(dev)), "paged_prefill_int4")
     return out
 
 

@@ -180,11 +180,14 @@ def test_c_entries_check_their_arguments():
     assert lib.psb_paged_decode_int4(None, 0, 0, None, 0, 0, None, None, None, 4, None, 1, 14, 0, 1, 8, 2, 16, 64, bf,
                                      64, 0.125, None, 0, None, None) == inv
     assert lib.psb_paged_prefill_int4(None, 0, 0, None, None, None, 4, None, None, 0, 0, None, 1, 5, 5, 64, 14, 0, 1,
-                                      8, 2, 16, 64, bf, 0.125, None, None) == inv
+                                      8, 2, 16, 64, bf, 0.125, None, 0, None, None) == inv
     assert lib.psb_paged_prefill_int4(None, 0, 0, None, None, None, 4, None, None, 0, 0, None, 0, 0, 0, 64, 14, 0, 1,
-                                      8, 2, 16, 64, bf, 0.125, None, None) == ok
+                                      8, 2, 16, 64, bf, 0.125, None, 0, None, None) == ok
     assert lib.psb_paged_prefill_int4(None, 0, 0, None, None, None, 3, None, None, 0, 0, None, 0, 0, 0, 64, 14, 0, 1,
-                                      8, 2, 16, 64, bf, 0.125, None, None) == inv  # tables narrower than max_context
+                                      8, 2, 16, 64, bf, 0.125, None, 0, None, None) == inv  # tables narrower than max_context
+    psize = lib.psb_paged_prefill_int4_workspace_size
+    assert psize(100, 2, 14, 2, 64, 16, 4096, bf) > 0 and psize(100, 2, 14, 3, 64, 16, 4096, bf) == 0
+    assert psize(100, 2, 14, 2, 63, 16, 4096, bf) == 0 and psize(-1, 2, 14, 2, 64, 16, 4096, bf) == 0
     assert lib.psb_extend_step(None, 4, 1, 4, None, None, None, 0, None, 5, None, 0, 16, None, None, None, None, None,
                                4, None, None) == ok
     assert lib.psb_extend_step(None, 4, 1, 4, None, None, None, 2, None, 5, None, 0, 16, None, None, None, None, None,

@@ -73,8 +73,10 @@ constexpr uint32_t kOffF = kOffV + kStages * kKvTile;
 constexpr uint32_t kOffBars = kOffF + kStages * sizeof(Factors);
 constexpr uint32_t kOffTab = kOffBars + 256;
 
+// A tile cut at a CTA's end that began in it: its kv head, first row of q and
+// tokens, and the last CTA with a piece (0: none).
 struct Cut {
-  int32_t kvh, tile, c1, pad;  // tile cut at a CTA's end that began in it; c1: last CTA with a piece (0: none)
+  int32_t kvh, row0, c1, tokens;
 };
 
 struct TcParams {
@@ -104,6 +106,9 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
+
+// A wait of a whole warp: its lanes give up together or not at all.
+__device__ __forceinline__ bool warp_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
 
 // What every role knows of the batch: lengths per sequence, tiles, steps.
 struct Plan {
@@ -472,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         load(nxt);
         look();
         const int st = g % kStages;
-        if (g >= kStages && !mbar_wait(bar_free + st, (g / kStages - 1) & 1)) {
+        if (g >= kStages && !warp_ok(mbar_wait(bar_free + st, (g / kStages - 1) & 1))) {
           fail = true;
           break;
         }
@@ -563,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     float pend_l = 0.f, pend_z = 0.f, pend_m = 0.f;
     Seg pend{};
     auto write_pending = [&](int pg) -> bool {
-      if (!mbar_wait(bar_pv + (pg & 1), (pg >> 1) & 1)) return false;
+      if (!warp_ok(mbar_wait(bar_pv + (pg & 1), (pg >> 1) & 1))) return false;
       tc_fence_after();
       const uint32_t t_po = t_lane + kOCol + (pend_k & 1) * kDim;
       const bool whole = pend.j0 == 0 && pend.n == pend.n_kv;
@@ -620,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int last = rtok < TQ && tok < plan.len[s.seq] ? start + tok : -1;
       const uint32_t t_o = t_lane + kOCol + (k & 1) * kDim;
       // sum of the row's q
-      if (!mbar_wait(bar_q + (k & 1), (k >> 1) & 1)) {
+      if (!warp_ok(mbar_wait(bar_q + (k & 1), (k >> 1) & 1))) {
         fail = true;
         break;
       }
@@ -642,7 +647,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       auto step = [&](int i) -> bool {
         const int st = g % kStages;
         const uint32_t ph = (g / kStages) & 1;
-        if (!mbar_wait(bar_s + (g & 1), (g >> 1) & 1) || !mbar_wait(bar_k + st, ph) || !mbar_wait(bar_v + st, ph)) return false;
+        if (!warp_ok(mbar_wait(bar_s + (g & 1), (g >> 1) & 1) && mbar_wait(bar_k + st, ph) && mbar_wait(bar_v + st, ph)))
+          return false;
         tc_fence_after();
         const Factors& f = fac[st];
         uint32_t sr[kBN];
@@ -691,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const float up = grow ? fminf(fmaxf(mx, -3e38f), 3e38f) : 0.f;
           const float al = grow ? (fresh ? 0.f : ex2_approx(-up)) : 1.f;
           if (i > 0) {  // O holds P V of the earlier steps once the last of them is done
-            if (!mbar_wait(bar_pv + ((g - 1) & 1), ((g - 1) >> 1) & 1)) return false;
+            if (!warp_ok(mbar_wait(bar_pv + ((g - 1) & 1), ((g - 1) >> 1) & 1))) return false;
             tc_fence_after();
             const float ao = al * exp2_int(max(-126, vexp - ve));
 #pragma unroll
@@ -768,8 +774,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int64_t t_a = static_cast<int64_t>(kvh) * n_steps + s_sfirst[tile];
       const int64_t t_e = static_cast<int64_t>(kvh) * n_steps + s_sfirst[tile + 1];
       if (t_a >= my_a && t_e > my_e) {
+        const int seq = last_le(s_tfirst, p.num_seqs, tile), first = (tile - s_tfirst[seq]) * TQ;
         c.kvh = kvh;
-        c.tile = tile;
+        c.row0 = s_q0[seq] + first;
+        c.tokens = min(TQ, s_len[seq] - first);
         c.c1 = cta;
         for (int c0 = cta + 1; c0 < act; c0 += 32) {  // CTAs that start before its end
           const bool in = c0 + lane < act && cta_start(min(c0 + lane, act)) < t_e;
@@ -802,18 +810,7 @@ __global__ void __launch_bounds__(kThreads) int4_prefill_combine_kernel(const Tc
   const float* const part = tp.part + kMaxCtas * (sizeof(Cut) / sizeof(float));
   const int row = threadIdx.x >> 1, half = threadIdx.x & 1;
   const int rtok = row / tp.group, rhead = row - rtok * tp.group;
-  // the tile's sequence: tiles are numbered over the sequences in order
-  int t = cut.y, seq = 0, len = 0;
-  for (; seq < p.num_seqs; ++seq) {
-    const int a = p.cu[seq], b = p.cu[seq + 1];
-    len = a < 0 || b < a || b > p.total ? 0 : b - a;
-    const int ctx = p.ctx[seq];
-    if (len > 0 && (ctx < len || ctx > p.max_context)) len = min(len, min(max(ctx, len), p.max_context));
-    const int tiles = (len + tp.tq - 1) / tp.tq;
-    if (t < tiles) break;
-    t -= tiles;
-  }
-  if (seq == p.num_seqs || rtok >= tp.tq || t * tp.tq + rtok >= len) return;
+  if (rtok >= cut.w) return;
   auto piece_of = [&](int c) { return part + static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * kPartFloats; };
   float m = -INFINITY, l = 0.f, o[32];
 #pragma unroll
@@ -837,7 +834,7 @@ __global__ void __launch_bounds__(kThreads) int4_prefill_combine_kernel(const Tc
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* out = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(p.cu[seq] + t * tp.tq + rtok) * p.ost +
+  T* out = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(cut.y + rtok) * p.ost +
            static_cast<int64_t>(cut.x * tp.group + rhead) * p.osh + 32 * half;
 #pragma unroll
   for (int d = 0; d < 32; ++d) out[d] = Elem<T>::from_float(o[d] * inv);

@@ -7,8 +7,13 @@
 // quantises the rounded key; gather_cache_int4 returns the values stored at
 // given slots.  The format is in int4_cache.cuh.
 //
-// One warp takes one row (q, k or v of one head of one token): lane l holds
-// the element pairs l, l + 32, ... and a pair is one byte of codes.
+// All three are bound by HBM (a 16 K-token pack of 14 + 2 heads moves 80 MB,
+// three quarters of it q in and out), so a thread moves 16-byte pieces: one of
+// each half of a row, which the rotation pairs, and the rows' extremes meet in
+// two to five shuffles between the row's threads.  A thread's eight codes of a
+// piece are one word.  Rows that are not 16-byte aligned, or whose pieces are
+// not a power of two, take a warp per row instead: lane l holds the element
+// pairs l, l + 32, ... and a pair is one byte of codes.
 #include <algorithm>
 
 #include "common.cuh"
@@ -152,6 +157,127 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_kernel(const Int4Wri
   }
 }
 
+// VEC consecutive elements, moved as one 16-byte access.
+template <typename T>
+struct Piece16 {
+  static constexpr int kVec = 16 / sizeof(T);
+  alignas(16) T e[kVec];
+  __device__ __forceinline__ void load(const T* src) { *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(src); }
+  __device__ __forceinline__ void store(T* dst) const { *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(e); }
+};
+
+// Codes of a piece: 8 a word (16-bit types) or 4 in its low half (fp32).
+template <typename T>
+__device__ __forceinline__ uint32_t piece_codes(const Piece16<T>& x, float step, float mid) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < Piece16<T>::kVec; ++i) w |= int4_code(Elem<T>::to_float(x.e[i]), step, mid) << (4 * i);
+  return w;
+}
+
+// One thread per (token, head, piece of a half row); ``pieces`` consecutive
+// lanes hold one row.  (Idx: int32 while every index fits.)
+template <typename T, bool ROPE, typename Idx>
+__global__ void __launch_bounds__(kWriteThreads) int4_write_vec_kernel(const Int4WriteParams p, int pieces) {
+  constexpr int VEC = Piece16<T>::kVec;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int half = p.head_dim / 2;
+  const int heads = (ROPE ? p.hq : 0) + 2 * p.hkv;
+  const Idx per_tok = static_cast<Idx>(heads) * pieces, total = per_tok * p.tokens;
+  const int lane = threadIdx.x & 31;
+  for (Idx base = (blockIdx.x * static_cast<Idx>(kWriteThreads) + threadIdx.x) & ~static_cast<Idx>(31); base < total;
+       base += static_cast<Idx>(gridDim.x) * kWriteThreads) {
+    const Idx i = min(base + lane, total - 1);  // lanes past the end repeat the last piece: same bytes, same place
+    const Idx t = i / per_tok;
+    const int r = static_cast<int>(i - t * per_tok);
+    int h = r / pieces;
+    const int e0 = (r - h * pieces) * VEC;
+    int role = 1;  // 0 q, 1 k, 2 v
+    if (ROPE) {
+      role = h < p.hq ? 0 : 1;
+      h -= role ? p.hq : 0;
+    }
+    if (role && h >= p.hkv) {
+      role = 2;
+      h -= p.hkv;
+    }
+    const T* src = reinterpret_cast<const T*>(role == 0 ? p.q : role == 1 ? p.k : p.v) +
+                   t * (role == 0 ? p.qst : role == 1 ? p.kst : p.vst) +
+                   h * (role == 0 ? p.qsh : role == 1 ? p.ksh : p.vsh) + e0;
+    Piece16<T> a, b;
+    a.load(src);
+    b.load(src + half);
+    int64_t slot = -1;
+    if (role) slot = __ldg(p.slots + t);
+    if (ROPE && role < 2) {
+      const T* cs = reinterpret_cast<const T*>(p.cos) + t * p.cst + e0;
+      const T* sn = reinterpret_cast<const T*>(p.sin) + t * p.cst + e0;
+      Piece16<T> c1, c2, s1, s2;
+      c1.load(cs);
+      c2.load(cs + half);
+      s1.load(sn);
+      s2.load(sn + half);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float x = Elem<T>::to_float(a.e[j]), y = Elem<T>::to_float(b.e[j]);
+        a.e[j] = Elem<T>::from_float(__fadd_rn(rnd<T>(__fmul_rn(x, Elem<T>::to_float(c1.e[j]))),
+                                               rnd<T>(__fmul_rn(-y, Elem<T>::to_float(s1.e[j])))));
+        b.e[j] = Elem<T>::from_float(__fadd_rn(rnd<T>(__fmul_rn(y, Elem<T>::to_float(c2.e[j]))),
+                                               rnd<T>(__fmul_rn(x, Elem<T>::to_float(s2.e[j])))));
+      }
+    }
+    if (ROPE) {
+      __syncwarp();  // in place: lanes that repeat the last piece have read it before it is written
+      T* dst = role == 0 ? reinterpret_cast<T*>(p.qo) + t * p.qost + h * p.qosh + e0
+                         : role == 1 && p.ko ? reinterpret_cast<T*>(p.ko) + t * p.kost + h * p.kosh + e0 : nullptr;
+      if (dst != nullptr) {
+        a.store(dst);
+        b.store(dst + half);
+      }
+    }
+    if (!__any_sync(0xffffffffu, slot >= 0)) continue;
+    float lo = INFINITY, hi = -INFINITY, bad = 0.f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float x = Elem<T>::to_float(a.e[j]), y = Elem<T>::to_float(b.e[j]);
+      lo = fminf(lo, fminf(x, y));
+      hi = fmaxf(hi, fmaxf(x, y));
+      if (!finite_f32(x) || !finite_f32(y)) bad = 1.f;
+    }
+    for (int o = 1; o < pieces; o <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      bad = fmaxf(bad, __shfl_xor_sync(0xffffffffu, bad, o));
+    }
+    if (slot < 0) continue;
+    if (slot >= p.pool_slots) {
+      if (e0 == 0 && h == 0 && role == 1) flag_error(p.err, PSB_DEVERR_SLOT_RANGE);
+      continue;
+    }
+    T step, mid;
+    int4_row_params<T>(lo, hi, bad == 0.f, step, mid);
+    const float st = Elem<T>::to_float(step), md = Elem<T>::to_float(mid);
+    const int64_t blk = slot / p.block_size;
+    const int64_t row = int4_row(p.layer_tiles + blk * p.hkv + h, role - 1, static_cast<int>(slot - blk * p.block_size),
+                                 p.block_size);
+    uint8_t* dst = p.codes + row * half + e0 / 2;
+    const uint32_t ca = piece_codes(a, st, md), cb = piece_codes(b, st, md);
+    if constexpr (VEC == 8) {
+      *reinterpret_cast<uint32_t*>(dst) = ca;
+      *reinterpret_cast<uint32_t*>(dst + half / 2) = cb;
+    } else {
+      *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(ca);
+      *reinterpret_cast<uint16_t*>(dst + half / 2) = static_cast<uint16_t>(cb);
+    }
+    if (e0 == 0) {
+      T* pr = reinterpret_cast<T*>(p.params) + row * 2;
+      pr[0] = step;
+      pr[1] = mid;
+    }
+  }
+}
+
 struct Int4GatherParams {
   const uint8_t* codes;
   const char* params;
@@ -199,29 +325,102 @@ __global__ void __launch_bounds__(kWriteThreads) int4_gather_kernel(const Int4Ga
   }
 }
 
+// One thread per VEC elements of a row.
+template <typename T>
+__global__ void __launch_bounds__(kWriteThreads) int4_gather_vec_kernel(const Int4GatherParams p) {
+  constexpr int VEC = Piece16<T>::kVec;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int pieces = p.head_dim / VEC;
+  const int64_t per_tok = static_cast<int64_t>(2) * p.hkv * pieces, total = per_tok * p.tokens;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kWriteThreads) + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * kWriteThreads) {
+    const int64_t t = i / per_tok;
+    int r = static_cast<int>(i - t * per_tok);
+    const int hv = r / pieces, e0 = (r - hv * pieces) * VEC;
+    const int kv = hv >= p.hkv ? 1 : 0, h = hv - kv * p.hkv;
+    const int64_t slot = __ldg(p.slots + t);
+    Piece16<T> x;
+    *reinterpret_cast<uint4*>(x.e) = make_uint4(0, 0, 0, 0);
+    if (slot >= p.pool_slots) {
+      if (r == 0) flag_error(p.err, PSB_DEVERR_SLOT_RANGE);
+    } else if (slot >= 0) {
+      const int64_t blk = slot / p.block_size;
+      const int64_t row = int4_row(p.layer_tiles + blk * p.hkv + h, kv, static_cast<int>(slot - blk * p.block_size),
+                                   p.block_size);
+      const uint8_t* src = p.codes + row * (p.head_dim / 2) + e0 / 2;
+      const uint32_t w = VEC == 8 ? *reinterpret_cast<const uint32_t*>(src) : *reinterpret_cast<const uint16_t*>(src);
+      const T* pr = reinterpret_cast<const T*>(p.params) + row * 2;
+      const float st = Elem<T>::to_float(pr[0]), md = Elem<T>::to_float(pr[1]);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x.e[j] = Elem<T>::from_float(int4_value((w >> (4 * j)) & 15u, st, md));
+    }
+    x.store((kv ? reinterpret_cast<T*>(p.v) + t * p.vst + h * p.vsh : reinterpret_cast<T*>(p.k) + t * p.kst + h * p.ksh) + e0);
+  }
+}
+
+bool aligned16(const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; }
+
+// Whether rows of these strides (elements of ``esz`` bytes) start on 16 bytes.
+bool rows16(const void* ptr, int64_t st, int64_t sh, int esz) {
+  return aligned16(ptr) && st * esz % 16 == 0 && sh * esz % 16 == 0;
+}
+
+// Lanes per row of the vector kernel, 0 when it does not apply.
 template <typename T, bool ROPE>
-int launch_write(const Int4WriteParams& p, cudaStream_t s, int sms) {
-  const int64_t units = static_cast<int64_t>(p.tokens) * ((ROPE ? p.hq : 0) + 2 * p.hkv);
-  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((units + 7) / 8, static_cast<int64_t>(sms) * 8));
-  const auto kern = int4_write_kernel<T, ROPE>;
+int write_pieces(const Int4WriteParams& p) {
+  constexpr int esz = sizeof(T), VEC = Piece16<T>::kVec;
+  const int half = p.head_dim / 2, pieces = half / VEC;
+  if (half % VEC || pieces > 32 || (pieces & (pieces - 1))) return 0;
+  bool ok = rows16(p.k, p.kst, p.ksh, esz) && rows16(p.v, p.vst, p.vsh, esz);
+  if (ROPE) {
+    ok = ok && rows16(p.cos, p.cst, 0, esz) && rows16(p.sin, p.cst, 0, esz);
+    if (p.hq > 0) ok = ok && rows16(p.q, p.qst, p.qsh, esz) && rows16(p.qo, p.qost, p.qosh, esz);
+    if (p.ko != nullptr) ok = ok && rows16(p.ko, p.kost, p.kosh, esz);
+  }
+  return ok ? pieces : 0;
+}
+
+// One wave of resident CTAs striding over ``threads`` threads' work.
+int64_t wave(const void* kern, int64_t threads, int sms) {
+  const int occ = std::max(1, std::min(resident_ctas(kern, kWriteThreads, 0), 8));
+  return std::max<int64_t>(1, std::min<int64_t>((threads + kWriteThreads - 1) / kWriteThreads,
+                                                static_cast<int64_t>(sms) * occ));
+}
+
+template <typename... K, typename... A>
+int launch_stream(void (*kern)(K...), int64_t blocks, cudaStream_t s, A... args) {
   if (!prefer_max_l1(reinterpret_cast<const void*>(kern))) return PSB_ERR_CUDA;
   discard_stale_error();
-  const cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(kWriteThreads), 0, s, p);
+  const cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(kWriteThreads), 0, s, args...);
   if (e != cudaSuccess) return record_cuda_error(e);
   return check_launch();
 }
 
+template <typename T, bool ROPE>
+int launch_write(const Int4WriteParams& p, cudaStream_t s, int sms) {
+  const int64_t rows = static_cast<int64_t>(p.tokens) * ((ROPE ? p.hq : 0) + 2 * p.hkv);
+  if (const int pieces = write_pieces<T, ROPE>(p)) {
+    const int64_t units = rows * pieces;
+    // int32 indices while the last one and a grid stride past it fit
+    const auto kern = units + static_cast<int64_t>(sms) * 8 * kWriteThreads < (int64_t(1) << 31)
+                          ? int4_write_vec_kernel<T, ROPE, int32_t> : int4_write_vec_kernel<T, ROPE, int64_t>;
+    return launch_stream(kern, wave(reinterpret_cast<const void*>(kern), units, sms), s, p, pieces);
+  }
+  const auto kern = int4_write_kernel<T, ROPE>;
+  return launch_stream(kern, wave(reinterpret_cast<const void*>(kern), rows * 32, sms), s, p);
+}
+
 template <typename T>
 int launch_gather(const Int4GatherParams& p, cudaStream_t s, int sms) {
-  const int64_t total = static_cast<int64_t>(p.tokens) * p.hkv * p.head_dim;
-  const int64_t blocks = std::max<int64_t>(
-      1, std::min<int64_t>((total + kWriteThreads - 1) / kWriteThreads, static_cast<int64_t>(sms) * 8));
+  constexpr int esz = sizeof(T), VEC = Piece16<T>::kVec;
+  const int64_t elems = static_cast<int64_t>(p.tokens) * 2 * p.hkv * p.head_dim;
+  if (p.head_dim % VEC == 0 && rows16(p.k, p.kst, p.ksh, esz) && rows16(p.v, p.vst, p.vsh, esz)) {
+    const auto kern = int4_gather_vec_kernel<T>;
+    return launch_stream(kern, wave(reinterpret_cast<const void*>(kern), elems / VEC, sms), s, p);
+  }
   const auto kern = int4_gather_kernel<T>;
-  if (!prefer_max_l1(reinterpret_cast<const void*>(kern))) return PSB_ERR_CUDA;
-  discard_stale_error();
-  const cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(kWriteThreads), 0, s, p);
-  if (e != cudaSuccess) return record_cuda_error(e);
-  return check_launch();
+  return launch_stream(kern, wave(reinterpret_cast<const void*>(kern), elems / 2, sms), s, p);
 }
 
 bool geometry_ok(int32_t num_tokens, int32_t layer, int32_t num_layers, int64_t num_blocks, int32_t num_kv_heads,

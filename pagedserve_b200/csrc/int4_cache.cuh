@@ -57,6 +57,23 @@ __device__ __forceinline__ uint32_t int4_code(float x, float step, float mid) {
   return static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f));
 }
 
+// The same code for a step of a 16-bit type, without the division: the
+// quotient's floor is estimated with inv ~ 1 / step (a finite normal number)
+// and put right by the signs of two exact remainders.  That is the floor of
+// the exact quotient, and of the rounded one too: d = fl(x - mid) and n step
+// (at most 15 bits) are multiples of d's last place, so a quotient that is not
+// the integer n is further from it than half a last place of n, and rounding
+// never reaches n.
+__device__ __forceinline__ uint32_t int4_code16(float x, float step, float mid, float inv) {
+  constexpr float kMagic = 12582912.f;  // 1.5 2^23: adding it rounds to an integer
+  const float d = __fsub_rn(x, mid);
+  float f = __fadd_rn(__fmul_rn(d, inv), kMagic) - kMagic;
+  if (fmaf(-f, step, d) < 0.f) f -= 1.f;
+  else if (fmaf(-(f + 1.f), step, d) >= 0.f) f += 1.f;
+  const int c = __float_as_int(f + kMagic) - __float_as_int(kMagic) + 8;
+  return static_cast<uint32_t>(min(max(c, 0), 15));
+}
+
 __device__ __forceinline__ float int4_value(uint32_t code, float step, float mid) {
   return fmaf(step, static_cast<float>(code) - kInt4Mid, mid);
 }

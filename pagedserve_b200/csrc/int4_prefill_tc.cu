@@ -595,9 +595,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         }
         if (!whole) {
+          if (live)
 #pragma unroll
-          for (int d = 0; d < 32; d += 4)
-            *reinterpret_cast<float4*>(dst + row * kDim + 32 * h + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+            for (int d = 0; d < 32; d += 4)
+              *reinterpret_cast<float4*>(dst + row * kDim + 32 * h + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
         } else if (live) {
           if (out16) {
 #pragma unroll
@@ -798,46 +799,73 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // Joins the partials of the tile that CTA blockIdx.x left cut at its end: a
-// thread takes half a row of the tile.
+// quarter of the tile's rows per CTA, kWarpRows rows per warp, two elements a
+// lane, kBatch partials in flight.
+constexpr int kCombineRows = 32, kWarpRows = kCombineRows / (kThreads / 32), kBatch = 4;
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) int4_prefill_combine_kernel(const TcParams tp) {
   const Int4PrefillParams& p = tp.a;
   pdl_wait();
   pdl_launch_dependents();
-  const int c0 = blockIdx.x;
+  const int c0 = blockIdx.x, lane = threadIdx.x & 31;
   const int4 cut = __ldcg(reinterpret_cast<const int4*>(tp.part) + c0);
-  if (cut.z <= c0) return;
+  const int row0 = blockIdx.y * kCombineRows + (threadIdx.x >> 5) * kWarpRows;
+  if (cut.z <= c0 || row0 >= cut.w * tp.group) return;
   const float* const part = tp.part + kMaxCtas * (sizeof(Cut) / sizeof(float));
-  const int row = threadIdx.x >> 1, half = threadIdx.x & 1;
-  const int rtok = row / tp.group, rhead = row - rtok * tp.group;
-  if (rtok >= cut.w) return;
   auto piece_of = [&](int c) { return part + static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * kPartFloats; };
-  float m = -INFINITY, l = 0.f, o[32];
+  float m[kWarpRows], l[kWarpRows];
+  float2 o[kWarpRows];
 #pragma unroll
-  for (int d = 0; d < 32; ++d) o[d] = 0.f;
-  for (int c = c0; c <= cut.z; ++c) {
-    const float* pc = piece_of(c);
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(pc + kRows * kDim + 2 * row));
-    float4 v[8];
+  for (int r = 0; r < kWarpRows; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+    o[r] = make_float2(0.f, 0.f);
+  }
+  for (int c = c0; c <= cut.z; c += kBatch) {
+    float2 ml[kBatch][kWarpRows], v[kBatch][kWarpRows];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) v[d] = __ldcg(reinterpret_cast<const float4*>(pc + row * kDim + 32 * half) + d);
-    const float mn = fmaxf(m, ml.x), mu = mn == -INFINITY ? 0.f : mn;
-    const float a = ex2_approx(m - mu), w = ex2_approx(ml.x - mu);
-    m = mn;
-    l = fmaf(l, a, ml.y * w);
+    for (int j = 0; j < kBatch; ++j) {
 #pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      o[4 * d] = fmaf(o[4 * d], a, v[d].x * w);
-      o[4 * d + 1] = fmaf(o[4 * d + 1], a, v[d].y * w);
-      o[4 * d + 2] = fmaf(o[4 * d + 2], a, v[d].z * w);
-      o[4 * d + 3] = fmaf(o[4 * d + 3], a, v[d].w * w);
+      for (int r = 0; r < kWarpRows; ++r) {
+        ml[j][r] = make_float2(-INFINITY, 0.f);
+        v[j][r] = make_float2(0.f, 0.f);
+        if (c + j <= cut.z) {
+          const float* pc = piece_of(c + j);
+          ml[j][r] = __ldcg(reinterpret_cast<const float2*>(pc + kRows * kDim + 2 * (row0 + r)));
+          v[j][r] = __ldcg(reinterpret_cast<const float2*>(pc + (row0 + r) * kDim) + lane);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kWarpRows; ++r) {
+      float mn = m[r];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) mn = fmaxf(mn, ml[j][r].x);
+      const float mu = mn == -INFINITY ? 0.f : mn, a = ex2_approx(m[r] - mu);
+      m[r] = mn;
+      l[r] *= a;
+      o[r].x *= a;
+      o[r].y *= a;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const float w = ex2_approx(ml[j][r].x - mu);
+        l[r] = fmaf(ml[j][r].y, w, l[r]);
+        o[r].x = fmaf(v[j][r].x, w, o[r].x);
+        o[r].y = fmaf(v[j][r].y, w, o[r].y);
+      }
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* out = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(cut.y + rtok) * p.ost +
-           static_cast<int64_t>(cut.x * tp.group + rhead) * p.osh + 32 * half;
 #pragma unroll
-  for (int d = 0; d < 32; ++d) out[d] = Elem<T>::from_float(o[d] * inv);
+  for (int r = 0; r < kWarpRows; ++r) {
+    const int rtok = (row0 + r) / tp.group, rhead = row0 + r - rtok * tp.group;
+    if (rtok >= cut.w) continue;
+    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+    T* out = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(cut.y + rtok) * p.ost +
+             static_cast<int64_t>(cut.x * tp.group + rhead) * p.osh + 2 * lane;
+    out[0] = Elem<T>::from_float(o[r].x * inv);
+    out[1] = Elem<T>::from_float(o[r].y * inv);
+  }
 }
 
 size_t tc_smem(int num_seqs, int max_tiles) {
@@ -891,7 +919,7 @@ int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspa
   cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, s, tp, tq);
   if (e != cudaSuccess) return record_cuda_error(e);
   if (grid > 1) {
-    e = launch_pdl(comb, dim3(static_cast<unsigned>(grid - 1)), dim3(kThreads), 0, s, tp);
+    e = launch_pdl(comb, dim3(static_cast<unsigned>(grid - 1), kRows / kCombineRows), dim3(kThreads), 0, s, tp);
     if (e != cudaSuccess) return record_cuda_error(e);
   }
   return check_launch();

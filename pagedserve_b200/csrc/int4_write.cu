@@ -170,35 +170,97 @@ struct Piece16 {
 template <typename T>
 __device__ __forceinline__ uint32_t piece_codes(const Piece16<T>& x, float step, float mid) {
   uint32_t w = 0;
+  if constexpr (sizeof(T) == 2) {
+    if (step > 1e-30f) {
+      const float inv = __frcp_rn(step);
+#pragma unroll
+      for (int i = 0; i < Piece16<T>::kVec; ++i) w |= int4_code16(Elem<T>::to_float(x.e[i]), step, mid, inv) << (4 * i);
+      return w;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < Piece16<T>::kVec; ++i) w |= int4_code(Elem<T>::to_float(x.e[i]), step, mid) << (4 * i);
   return w;
 }
 
+// a b and a + b of packed 16-bit pairs, rounded as PyTorch rounds the two
+// operations (an explicit .rn is never contracted into a multiply-add).
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> {
+  __device__ static uint32_t mul(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  __device__ static uint32_t add(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+};
+template <> struct Pair<__half> {
+  __device__ static uint32_t mul(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  __device__ static uint32_t add(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+};
+
+// (a, b) -> (a cos - b sin, b cos + a sin), each product and sum rounded to T.
+template <typename T>
+__device__ __forceinline__ void rotate(Piece16<T>& a, Piece16<T>& b, const Piece16<T>& c1, const Piece16<T>& c2,
+                                       const Piece16<T>& s1, const Piece16<T>& s2) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t* x = reinterpret_cast<uint32_t*>(a.e);
+    uint32_t* y = reinterpret_cast<uint32_t*>(b.e);
+    const uint32_t* p1 = reinterpret_cast<const uint32_t*>(c1.e);
+    const uint32_t* p2 = reinterpret_cast<const uint32_t*>(c2.e);
+    const uint32_t* q1 = reinterpret_cast<const uint32_t*>(s1.e);
+    const uint32_t* q2 = reinterpret_cast<const uint32_t*>(s2.e);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t u = x[j], v = y[j];
+      x[j] = Pair<T>::add(Pair<T>::mul(u, p1[j]), Pair<T>::mul(v ^ 0x80008000u, q1[j]));
+      y[j] = Pair<T>::add(Pair<T>::mul(v, p2[j]), Pair<T>::mul(u, q2[j]));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < Piece16<T>::kVec; ++j) {
+      const float x = a.e[j], y = b.e[j];
+      a.e[j] = __fadd_rn(__fmul_rn(x, c1.e[j]), __fmul_rn(-y, s1.e[j]));
+      b.e[j] = __fadd_rn(__fmul_rn(y, c2.e[j]), __fmul_rn(x, s2.e[j]));
+    }
+  }
+}
+
 // One thread per (token, head, piece of a half row); ``pieces`` consecutive
-// lanes hold one row.  (Idx: int32 while every index fits.)
+// lanes hold one row.  The q rows of all tokens come first, then the k and v
+// rows, so that a warp's lanes share a path.  (Idx: int32 while every index fits.)
 template <typename T, bool ROPE, typename Idx>
 __global__ void __launch_bounds__(kWriteThreads) int4_write_vec_kernel(const Int4WriteParams p, int pieces) {
   constexpr int VEC = Piece16<T>::kVec;
   pdl_launch_dependents();
   pdl_wait();
   const int half = p.head_dim / 2;
-  const int heads = (ROPE ? p.hq : 0) + 2 * p.hkv;
-  const Idx per_tok = static_cast<Idx>(heads) * pieces, total = per_tok * p.tokens;
+  const Idx q_tok = static_cast<Idx>(ROPE ? p.hq : 0) * pieces, kv_tok = static_cast<Idx>(2 * p.hkv) * pieces;
+  const Idx q_total = q_tok * p.tokens, total = q_total + kv_tok * p.tokens;
   const int lane = threadIdx.x & 31;
   for (Idx base = (blockIdx.x * static_cast<Idx>(kWriteThreads) + threadIdx.x) & ~static_cast<Idx>(31); base < total;
        base += static_cast<Idx>(gridDim.x) * kWriteThreads) {
     const Idx i = min(base + lane, total - 1);  // lanes past the end repeat the last piece: same bytes, same place
-    const Idx t = i / per_tok;
-    const int r = static_cast<int>(i - t * per_tok);
+    const bool is_q = ROPE && i < q_total;
+    const Idx u = is_q ? i : i - q_total, per = is_q ? q_tok : kv_tok;
+    const Idx t = u / per;
+    const int r = static_cast<int>(u - t * per);
     int h = r / pieces;
     const int e0 = (r - h * pieces) * VEC;
-    int role = 1;  // 0 q, 1 k, 2 v
-    if (ROPE) {
-      role = h < p.hq ? 0 : 1;
-      h -= role ? p.hq : 0;
-    }
-    if (role && h >= p.hkv) {
+    int role = is_q ? 0 : 1;  // 0 q, 1 k, 2 v
+    if (!is_q && h >= p.hkv) {
       role = 2;
       h -= p.hkv;
     }
@@ -218,14 +280,7 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_vec_kernel(const Int
       c2.load(cs + half);
       s1.load(sn);
       s2.load(sn + half);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float x = Elem<T>::to_float(a.e[j]), y = Elem<T>::to_float(b.e[j]);
-        a.e[j] = Elem<T>::from_float(__fadd_rn(rnd<T>(__fmul_rn(x, Elem<T>::to_float(c1.e[j]))),
-                                               rnd<T>(__fmul_rn(-y, Elem<T>::to_float(s1.e[j])))));
-        b.e[j] = Elem<T>::from_float(__fadd_rn(rnd<T>(__fmul_rn(y, Elem<T>::to_float(c2.e[j]))),
-                                               rnd<T>(__fmul_rn(x, Elem<T>::to_float(s2.e[j])))));
-      }
+      rotate(a, b, c1, c2, s1, s2);
     }
     if (ROPE) {
       __syncwarp();  // in place: lanes that repeat the last piece have read it before it is written

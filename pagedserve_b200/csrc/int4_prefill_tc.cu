@@ -34,6 +34,7 @@
 // waiter: a stage's next phase needs its own release, a step's barriers
 // alternate and step g + 2 needs step g's products.
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -906,10 +907,14 @@ int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspa
   const size_t smem = tc_smem(p.num_seqs, tp.max_tiles);
   // the register split draws on what the block was launched with
   static_assert(168 + 88 == 2 * 128, "two warpgroups' shares");
-  cudaFuncAttributes fa;
-  const cudaError_t fe = cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(kern));
-  if (fe != cudaSuccess) return record_cuda_error(fe);
-  if (fa.numRegs < 128) return PSB_ERR_UNSUPPORTED;
+  static std::atomic<bool> checked[2];  // per element type
+  if (!checked[dtype == PSB_BF16].load(std::memory_order_relaxed)) {
+    cudaFuncAttributes fa;
+    const cudaError_t fe = cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(kern));
+    if (fe != cudaSuccess) return record_cuda_error(fe);
+    if (fa.numRegs < 128) return PSB_ERR_UNSUPPORTED;
+    checked[dtype == PSB_BF16].store(true, std::memory_order_relaxed);
+  }
   int occ = 0;
   if (!kernel_occupancy(reinterpret_cast<const void*>(kern), kThreads, smem, &occ) || occ < 1) return PSB_ERR_CUDA;
   // an upper bound of the steps

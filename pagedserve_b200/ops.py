@@ -575,53 +575,78 @@ def select_tokens(logits: torch.Tensor, eos_ids: torch.Tensor, remaining: torch.
 
 
 # -- 4-bit KV pool ---------------------------------------------------------------------------------------------
+#
+# A call's host time is most of a small batch's step, so the checks below read
+# every tensor attribute once, compare device indices rather than devices, and
+# leave the wording of an error to the branch that raises it.
 
 INT4_MAX_HEAD_DIM = 256
 
 
-def _one_device(device: torch.device, *tensors: torch.Tensor | None) -> None:
-    """Every tensor on ``device``, a CUDA one (the last of a call's checks)."""
-    if device.type != "cuda":
-        raise ValueError("B200 paged attention requires CUDA tensors")
+def _cuda_index(*tensors: torch.Tensor | None) -> int:
+    """The CUDA device index all of ``tensors`` are on (the last of a call's checks)."""
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"every tensor must be on {device}: got one on {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"every tensor must be on {tensors[0].device}: got one on {t.device}")
+    if dev < 0:
+        raise ValueError("B200 paged attention requires CUDA tensors")
+    return dev
 
 
-class _Nothing:
-    def __enter__(self):
-        return None
+def _call(dev: int, fn, what: str, *args) -> None:
+    """``fn(*args, stream)`` on ``dev``'s current stream with ``dev`` the current device."""
+    if _raw_stream is not None and torch._C._cuda_getDevice() == dev:
+        status = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if status != _native.PSB_OK:
+        _native.check(status, what)
 
-    def __exit__(self, *exc):
-        return False
+
+class _Scratch(threading.local):
+    """Scratch of the split kernels: one growing buffer per host thread,
+    device and stream, so that no two calls that may overlap on the GPU share
+    one.  A call that is being captured gets a tensor of its own from the
+    graph's pool instead (a graph may be replayed on any stream)."""
+
+    def __init__(self):
+        self.buffers: dict[tuple[int, int], torch.Tensor] = {}
+
+    def get(self, nbytes: int, dev: int) -> torch.Tensor:
+        if (_raw_stream is None or torch._C._cuda_getDevice() != dev  # (whose capture could not be asked for)
+                or torch._C._cuda_isCurrentStreamCapturing()):
+            return torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{dev}")
+        stream = _raw_stream(dev)
+        buf = self.buffers.get((dev, stream))
+        if buf is None or buf.numel() < nbytes:
+            buf = self.buffers[(dev, stream)] = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{dev}")
+        return buf
 
 
-_NOTHING = _Nothing()
-
-
-def _on(device: torch.device):
-    """Makes ``device`` the current one while a kernel is launched on its
-    stream (nothing to do, and nothing paid, when it already is)."""
-    return _NOTHING if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+_scratch = _Scratch()
 
 
 def _int4_geometry(kv_codes: torch.Tensor, kv_params: torch.Tensor):
-    """(layers, blocks, kv heads, block size, head dim) of a 4-bit pool."""
+    """(layers, blocks, kv heads, block size, head dim, dtype, its code) of a 4-bit pool."""
     cs, ps = kv_codes.shape, kv_params.shape
     if len(cs) != 6 or cs[3] != 2 or kv_codes.dtype != torch.uint8:
         raise ValueError("kv_codes must be uint8 [num_layers, num_blocks, num_kv_heads, 2, block_size, head_dim / 2]")
-    if len(ps) != 6 or ps[:5] != cs[:5] or ps[5] != 2:
+    nl, nb, hkv, _, bs, half = cs
+    if ps != (nl, nb, hkv, 2, bs, 2):
         raise ValueError("kv_params must be [num_layers, num_blocks, num_kv_heads, 2, block_size, 2] like kv_codes")
-    if kv_params.dtype not in _DTYPES:
-        raise ValueError(f"Unsupported dtype {kv_params.dtype}")
+    dtype = kv_params.dtype
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"Unsupported dtype {dtype}")
     if not (kv_codes.is_contiguous() and kv_params.is_contiguous()):
         raise ValueError("KV pools must be contiguous")
-    if kv_codes.data_ptr() % 16 or kv_params.data_ptr() % 16:
+    if (kv_codes.data_ptr() | kv_params.data_ptr()) & 15:
         raise ValueError("KV pools must start on 16 bytes")
-    d = 2 * cs[5]
-    if d > INT4_MAX_HEAD_DIM:
+    if half > INT4_MAX_HEAD_DIM // 2:
         raise ValueError(f"4-bit pools hold head_dim up to {INT4_MAX_HEAD_DIM}")
-    return cs[0], cs[1], cs[2], cs[4], d
+    return nl, nb, hkv, bs, 2 * half, dtype, code
 
 
 def _check_flag(error_flag: torch.Tensor | None) -> None:
@@ -629,18 +654,19 @@ def _check_flag(error_flag: torch.Tensor | None) -> None:
         raise ValueError("error_flag must be an int32 tensor of at least one element")
 
 
-def _int4_rows(key, value, hkv: int, d: int, dtype) -> int:
-    if key.ndim != 3 or key.shape[1] != hkv or key.shape[2] != d or value.shape != key.shape:
+def _int4_rows(key: torch.Tensor, value: torch.Tensor, hkv: int, d: int, dtype) -> int:
+    shape = key.shape
+    if len(shape) != 3 or shape[1] != hkv or shape[2] != d or value.shape != shape:
         raise ValueError(f"key/value must be [T, {hkv}, {d}]")
     if key.dtype != dtype or value.dtype != dtype:
         raise ValueError("key/value dtype must match the cache dtype (that of kv_params)")
-    if key.stride(2) != 1 or value.stride(2) != 1:
+    if key.stride()[2] != 1 or value.stride()[2] != 1:
         raise ValueError("key/value need unit stride along head_dim")
-    return key.shape[0]
+    return shape[0]
 
 
 def _int4_slots(slot_mapping: torch.Tensor, t: int) -> torch.Tensor:
-    if slot_mapping.dtype != torch.int64 or slot_mapping.ndim != 1 or slot_mapping.shape[0] != t:
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (t,):
         raise ValueError("slot_mapping must be int64 [T]")
     return slot_mapping.contiguous()
 
@@ -654,20 +680,17 @@ def reshape_and_cache_int4(key: torch.Tensor, value: torch.Tensor, kv_codes: tor
     ``kv_codes[layer]`` / ``kv_params[layer]`` at ``slot_mapping [T]`` (int64;
     negative: nothing is written; live slots distinct).
     """
-    nl, nb, hkv, bs, d = _int4_geometry(kv_codes, kv_params)
-    t = _int4_rows(key, value, hkv, d, kv_params.dtype)
+    nl, nb, hkv, bs, d, dtype, code = _int4_geometry(kv_codes, kv_params)
+    t = _int4_rows(key, value, hkv, d, dtype)
     slot_mapping = _int4_slots(slot_mapping, t)
     if not 0 <= layer < nl:
         raise ValueError("Invalid layer")
     _check_flag(error_flag)
-    dev = kv_codes.device
-    _one_device(dev, key, value, kv_params, slot_mapping, error_flag)
-    lib = _native.load()
-    with _on(dev):
-        _native.check(lib.psb_reshape_and_cache_int4(
-            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
-            kv_codes.data_ptr(), kv_params.data_ptr(), slot_mapping.data_ptr(), t, layer, nl, nb, hkv, bs, d,
-            _DTYPES[kv_params.dtype], _ptr(error_flag), _stream(dev)), "reshape_and_cache_int4")
+    dev = _cuda_index(kv_codes, kv_params, key, value, slot_mapping, error_flag)
+    ks, vs = key.stride(), value.stride()
+    _call(dev, _native.load().psb_reshape_and_cache_int4, "reshape_and_cache_int4",
+          key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], kv_codes.data_ptr(), kv_params.data_ptr(),
+          slot_mapping.data_ptr(), t, layer, nl, nb, hkv, bs, d, code, _ptr(error_flag))
 
 
 def rope_reshape_and_cache_int4(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cos: torch.Tensor,
@@ -682,49 +705,50 @@ def rope_reshape_and_cache_int4(query: torch.Tensor, key: torch.Tensor, value: t
     Returns ``(query_out, key_out)`` with the same defaults: new tensors,
     ``query_out=query`` to rotate in place, ``key_out=False`` for none.
     """
-    nl, nb, hkv, bs, d = _int4_geometry(kv_codes, kv_params)
-    dtype = kv_params.dtype
-    if query.ndim != 3 or query.shape[2] != d:
+    nl, nb, hkv, bs, d, dtype, code = _int4_geometry(kv_codes, kv_params)
+    shape = query.shape
+    if len(shape) != 3 or shape[2] != d:
         raise ValueError(f"query must be [T, Hq, {d}]")
-    t = query.shape[0]
+    t = shape[0]
     if _int4_rows(key, value, hkv, d, dtype) != t:
         raise ValueError(f"key/value must be [{t}, {hkv}, {d}]")
-    cos = cos.reshape(-1, d)
-    sin = sin.reshape(-1, d)
-    if cos.shape[0] != t or sin.shape != cos.shape:
-        raise ValueError(f"cos/sin must hold one [{d}] row per token")
-    if cos.stride(1) != 1 or sin.stride(1) != 1 or cos.stride(0) != sin.stride(0):
+    if cos.shape != (t, d) or sin.shape != (t, d):
+        cos, sin = cos.reshape(-1, d), sin.reshape(-1, d)
+        if cos.shape[0] != t or sin.shape != cos.shape:
+            raise ValueError(f"cos/sin must hold one [{d}] row per token")
+    cst = cos.stride()
+    if cst != sin.stride() or cst[1] != 1:
         cos, sin = cos.contiguous(), sin.contiguous()
+        cst = (d, 1)
     if query.dtype != dtype or cos.dtype != dtype or sin.dtype != dtype:
         raise ValueError("query/key/value/cos/sin dtype must match the cache dtype (that of kv_params)")
-    if query.stride(2) != 1:
+    qs = query.stride()
+    if qs[2] != 1:
         raise ValueError("unit stride along head_dim is required")
     slot_mapping = _int4_slots(slot_mapping, t)
     if not 0 <= layer < nl:
         raise ValueError("Invalid layer")
     _check_flag(error_flag)
-    dev = kv_codes.device
-    _one_device(dev, query, key, value, cos, sin, kv_params, slot_mapping, query_out,
-                key_out if isinstance(key_out, torch.Tensor) else None, error_flag)
     if query_out is None:
-        query_out = torch.empty(query.shape, dtype=dtype, device=query.device)
-    elif query_out.shape != query.shape or query_out.dtype != dtype or query_out.stride(2) != 1:
+        query_out = torch.empty_like(query)
+    elif query_out.shape != shape or query_out.dtype != dtype:
         raise ValueError("query_out must match query's shape and dtype with unit stride along head_dim")
     if key_out is None:
-        key_out = torch.empty(key.shape, dtype=dtype, device=key.device)
+        key_out = torch.empty_like(key)
     elif key_out is False:
         key_out = None
-    elif key_out.shape != key.shape or key_out.dtype != dtype or key_out.stride(2) != 1:
+    elif key_out.shape != key.shape or key_out.dtype != dtype:
         raise ValueError("key_out must match key's shape and dtype with unit stride along head_dim")
-    lib = _native.load()
-    with _on(dev):
-        _native.check(lib.psb_rope_reshape_and_cache_int4(
-            query.data_ptr(), query.stride(0), query.stride(1), query_out.data_ptr(), query_out.stride(0),
-            query_out.stride(1), key.data_ptr(), key.stride(0), key.stride(1), _ptr(key_out),
-            key_out.stride(0) if key_out is not None else 0, key_out.stride(1) if key_out is not None else 0,
-            value.data_ptr(), value.stride(0), value.stride(1), cos.data_ptr(), sin.data_ptr(), cos.stride(0),
-            kv_codes.data_ptr(), kv_params.data_ptr(), slot_mapping.data_ptr(), t, query.shape[1], layer, nl, nb, hkv,
-            bs, d, _DTYPES[dtype], _ptr(error_flag), _stream(dev)), "rope_reshape_and_cache_int4")
+    qos, kos = query_out.stride(), key_out.stride() if key_out is not None else (0, 0, 1)
+    if qos[2] != 1 or kos[2] != 1:
+        raise ValueError("query_out / key_out need unit stride along head_dim")
+    dev = _cuda_index(kv_codes, kv_params, query, key, value, cos, sin, slot_mapping, query_out, key_out, error_flag)
+    ks, vs = key.stride(), value.stride()
+    _call(dev, _native.load().psb_rope_reshape_and_cache_int4, "rope_reshape_and_cache_int4",
+          query.data_ptr(), qs[0], qs[1], query_out.data_ptr(), qos[0], qos[1], key.data_ptr(), ks[0], ks[1],
+          _ptr(key_out), kos[0], kos[1], value.data_ptr(), vs[0], vs[1], cos.data_ptr(), sin.data_ptr(), cst[0],
+          kv_codes.data_ptr(), kv_params.data_ptr(), slot_mapping.data_ptr(), t, shape[1], layer, nl, nb, hkv, bs, d,
+          code, _ptr(error_flag))
     return query_out, key_out
 
 
@@ -734,38 +758,40 @@ def gather_cache_int4(kv_codes: torch.Tensor, kv_params: torch.Tensor, slot_mapp
     """``(key, value) [T, Hkv, D]``: the values a 4-bit pool holds at
     ``slot_mapping [T]`` (int64; zeros for a negative slot), in ``kv_params``'
     dtype (psb_gather_cache_int4)."""
-    nl, nb, hkv, bs, d = _int4_geometry(kv_codes, kv_params)
-    if slot_mapping.ndim != 1:
-        raise ValueError("slot_mapping must be int64 [T]")
-    t = slot_mapping.shape[0]
+    nl, nb, hkv, bs, d, dtype, code = _int4_geometry(kv_codes, kv_params)
+    t = slot_mapping.shape[0] if slot_mapping.ndim == 1 else -1
     slot_mapping = _int4_slots(slot_mapping, t)
     if not 0 <= layer < nl:
         raise ValueError("Invalid layer")
     _check_flag(error_flag)
-    shape, dtype, dev = (t, hkv, d), kv_params.dtype, kv_codes.device
-    _one_device(dev, kv_params, slot_mapping, key_out, value_out, error_flag)
+    shape = (t, hkv, d)
     if key_out is None:
-        key_out = torch.empty(shape, dtype=dtype, device=dev)
+        key_out = kv_params.new_empty(shape)
     if value_out is None:
-        value_out = torch.empty(shape, dtype=dtype, device=dev)
-    for x in (key_out, value_out):
-        if x.shape != shape or x.dtype != dtype or x.stride(2) != 1:
-            raise ValueError(f"key_out/value_out must be [{t}, {hkv}, {d}] {dtype} with unit stride along head_dim")
-    lib = _native.load()
-    with _on(dev):
-        _native.check(lib.psb_gather_cache_int4(
-            kv_codes.data_ptr(), kv_params.data_ptr(), slot_mapping.data_ptr(), key_out.data_ptr(), key_out.stride(0),
-            key_out.stride(1), value_out.data_ptr(), value_out.stride(0), value_out.stride(1), t, layer, nl, nb, hkv,
-            bs, d, _DTYPES[dtype], _ptr(error_flag), _stream(dev)), "gather_cache_int4")
+        value_out = kv_params.new_empty(shape)
+    ks, vs = key_out.stride(), value_out.stride()
+    if (key_out.shape != shape or value_out.shape != shape or key_out.dtype != dtype or value_out.dtype != dtype
+            or ks[2] != 1 or vs[2] != 1):
+        raise ValueError(f"key_out/value_out must be [{t}, {hkv}, {d}] {dtype} with unit stride along head_dim")
+    dev = _cuda_index(kv_codes, kv_params, slot_mapping, key_out, value_out, error_flag)
+    _call(dev, _native.load().psb_gather_cache_int4, "gather_cache_int4",
+          kv_codes.data_ptr(), kv_params.data_ptr(), slot_mapping.data_ptr(), key_out.data_ptr(), ks[0], ks[1],
+          value_out.data_ptr(), vs[0], vs[1], t, layer, nl, nb, hkv, bs, d, code, _ptr(error_flag))
     return key_out, value_out
 
 
-@functools.lru_cache(maxsize=256)
+@functools.lru_cache(maxsize=1024)
 def decode_int4_workspace_bytes(batch: int, q_heads: int, hkv: int, head_dim: int, block_size: int, max_context: int,
                                 dtype: torch.dtype) -> int:
+    """Scratch bytes of ``paged_decode_int4`` (psb_paged_decode_int4_workspace_size)."""
     lib = _native.load()
     return int(lib.psb_paged_decode_int4_workspace_size(batch, q_heads, hkv, head_dim, block_size, max_context,
                                                         dtype_code(dtype)))
+
+
+def _check_workspace(workspace: torch.Tensor) -> None:
+    if not workspace.is_contiguous() or workspace.data_ptr() % 16:
+        raise ValueError("workspace must be contiguous and start on 16 bytes")
 
 
 def paged_decode_int4(query: torch.Tensor, kv_codes: torch.Tensor, kv_params: torch.Tensor,
@@ -775,66 +801,70 @@ def paged_decode_int4(query: torch.Tensor, kv_codes: torch.Tensor, kv_params: to
     """``paged_decode`` over a 4-bit pool (psb_paged_decode_int4).
 
     ``query [B, Hq, D]`` or ``[B, Hq, 1, D]`` of ``kv_params``' dtype; tables,
-    lengths, ``max_context`` and ``scale`` as in ``paged_decode``.  The
-    split-K scratch is allocated per call from PyTorch's caching allocator
-    (so calls on different streams, and captured graphs, never share it)
-    unless ``workspace`` (uint8, ``decode_int4_workspace_bytes``) is given.
+    lengths, ``max_context`` and ``scale`` as in ``paged_decode``.  The split-K
+    scratch is kept per host thread, device and stream (a captured call has
+    its own) unless ``workspace`` (``decode_int4_workspace_bytes``) is given,
+    which calls that may overlap on the GPU must not share.
     """
-    nl, nb, hkv, bs, d = _int4_geometry(kv_codes, kv_params)
+    nl, nb, hkv, bs, d, dtype, code = _int4_geometry(kv_codes, kv_params)
     q3 = query.squeeze(2) if query.ndim == 4 else query
-    if q3.ndim != 3 or q3.shape[2] != d:
+    shape = q3.shape
+    if len(shape) != 3 or shape[2] != d:
         raise ValueError("query must be [B, Hq, D] or [B, Hq, 1, D]")
-    bsz, hq, _ = q3.shape
+    bsz, hq, _ = shape
     if bsz == 0:
         raise ValueError("Batch must not be empty")
     if hq == 0 or hq % hkv:
         raise ValueError("Query heads must be divisible by KV heads")
-    dtype = kv_params.dtype
     if q3.dtype != dtype:
         raise ValueError("Query dtype must match cache dtype (that of kv_params)")
-    if q3.stride(2) != 1:
+    qs = q3.stride()
+    if qs[2] != 1:
         q3 = q3.contiguous()
-    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.shape[0] != bsz:
+        qs = q3.stride()
+    ts = block_tables.shape
+    if block_tables.dtype != torch.int32 or len(ts) != 2 or ts[0] != bsz:
         raise ValueError("block_tables must be int32 [B, max_blocks]")
-    if block_tables.stride(1) != 1:
+    tst = block_tables.stride()
+    if tst[1] != 1:
         block_tables = block_tables.contiguous()
-    if context_lens.dtype != torch.int32 or context_lens.ndim != 1 or context_lens.shape[0] != bsz:
+        tst = block_tables.stride()
+    if context_lens.dtype != torch.int32 or context_lens.shape != (bsz,):
         raise ValueError("context_lens must be int32 [B]")
     context_lens = context_lens.contiguous()
     if not 0 <= layer < nl:
         raise ValueError("Invalid layer")
-    width = block_tables.shape[1] * bs
+    width = ts[1] * bs
     if max_context is None:
         max_context = width
     elif not 0 <= max_context <= width:
         raise ValueError("max_context must be at most block_tables' width in tokens")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     _check_flag(error_flag)
-    dev = kv_codes.device
-    _one_device(dev, q3, kv_params, block_tables, context_lens, out, workspace, error_flag)
+    dev = _cuda_index(kv_codes, kv_params, q3, block_tables, context_lens, out, workspace, error_flag)
     if out is None:
-        out = torch.empty(query.shape, dtype=dtype, device=dev)
+        out = torch.empty_like(query)
+        if out.stride()[-1] != 1:
+            out = out.contiguous()
     o3 = out.squeeze(2) if out.ndim == 4 else out
-    if o3.shape != q3.shape or o3.stride(2) != 1 or o3.dtype != dtype:
+    os_ = o3.stride()
+    if o3.shape != shape or o3.dtype != dtype or os_[2] != 1:
         raise ValueError("out must match query's shape/dtype with unit stride along head_dim")
     if workspace is None:
-        workspace = torch.empty(decode_int4_workspace_bytes(bsz, hq, hkv, d, bs, int(max_context), dtype),
-                                dtype=torch.uint8, device=dev)
-    elif not workspace.is_contiguous() or workspace.data_ptr() % 16:
-        raise ValueError("workspace must be contiguous and start on 16 bytes")
-    lib = _native.load()
-    with _on(dev):
-        _native.check(lib.psb_paged_decode_int4(
-            q3.data_ptr(), q3.stride(0), q3.stride(1), o3.data_ptr(), o3.stride(0), o3.stride(1), kv_codes.data_ptr(),
-            kv_params.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(), bsz, hq,
-            layer, nl, nb, hkv, bs, d, _DTYPES[dtype], int(max_context), scale, workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _ptr(error_flag), _stream(dev)), "paged_decode_int4")
+        workspace = _scratch.get(decode_int4_workspace_bytes(bsz, hq, hkv, d, bs, int(max_context), dtype), dev)
+    else:
+        _check_workspace(workspace)
+    _call(dev, _native.load().psb_paged_decode_int4, "paged_decode_int4",
+          q3.data_ptr(), qs[0], qs[1], o3.data_ptr(), os_[0], os_[1], kv_codes.data_ptr(), kv_params.data_ptr(),
+          block_tables.data_ptr(), tst[0], context_lens.data_ptr(), bsz, hq, layer, nl, nb, hkv, bs, d, code,
+          int(max_context), scale, workspace.data_ptr(), workspace.nbytes, _ptr(error_flag))
     return out
 
 
-@functools.lru_cache(maxsize=256)
+@functools.lru_cache(maxsize=1024)
 def prefill_int4_workspace_bytes(total: int, num_seqs: int, q_heads: int, hkv: int, head_dim: int, block_size: int,
                                  max_context: int, dtype: torch.dtype) -> int:
+    """Scratch bytes of ``paged_prefill_int4`` (psb_paged_prefill_int4_workspace_size)."""
     lib = _native.load()
     return int(lib.psb_paged_prefill_int4_workspace_size(total, num_seqs, q_heads, hkv, head_dim, block_size,
                                                          max_context, dtype_code(dtype)))
@@ -848,30 +878,35 @@ def paged_prefill_int4(q: torch.Tensor, kv_codes: torch.Tensor, kv_params: torch
     Hq, D]`` of ``kv_params``' dtype, the rest as in ``paged_prefill``.  Rows
     of ``out`` that belong to no sequence keep what they held.  Scratch as in
     ``paged_decode_int4`` (``prefill_int4_workspace_bytes``)."""
-    nl, nb, hkv, bs, d = _int4_geometry(kv_codes, kv_params)
-    if q.ndim != 3 or q.shape[2] != d:
+    nl, nb, hkv, bs, d, dtype, code = _int4_geometry(kv_codes, kv_params)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != d:
         raise ValueError(f"q must be [T, Hq, {d}]")
-    t, hq, _ = q.shape
+    t, hq, _ = shape
     if hq == 0 or hq % hkv:
         raise ValueError("Query heads must be divisible by KV heads")
-    dtype = kv_params.dtype
     if q.dtype != dtype:
         raise ValueError("q dtype must match the cache dtype (that of kv_params)")
     if cu_seqlens.dtype != torch.int32 or cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must be int32 [B+1]")
     batch = cu_seqlens.shape[0] - 1
-    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.shape[0] != batch:
+    ts = block_tables.shape
+    if block_tables.dtype != torch.int32 or len(ts) != 2 or ts[0] != batch:
         raise ValueError("block_tables must be int32 [B, max_blocks]")
-    if context_lens.dtype != torch.int32 or context_lens.ndim != 1 or context_lens.shape[0] != batch:
+    if context_lens.dtype != torch.int32 or context_lens.shape != (batch,):
         raise ValueError("context_lens must be int32 [B]")
     if not 0 <= layer < nl:
         raise ValueError("Invalid layer")
-    if q.stride(2) != 1:
+    qs = q.stride()
+    if qs[2] != 1:
         q = q.contiguous()
-    if block_tables.stride(1) != 1:
+        qs = q.stride()
+    tst = block_tables.stride()
+    if tst[1] != 1:
         block_tables = block_tables.contiguous()
+        tst = block_tables.stride()
     cu_seqlens, context_lens = cu_seqlens.contiguous(), context_lens.contiguous()
-    width = block_tables.shape[1] * bs
+    width = ts[1] * bs
     if max_context is None:
         max_context = width
     elif max_context > width:
@@ -880,25 +915,21 @@ def paged_prefill_int4(q: torch.Tensor, kv_codes: torch.Tensor, kv_params: torch
         raise ValueError("max_seqlen must be at most max_context")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     _check_flag(error_flag)
-    dev = kv_codes.device
-    _one_device(dev, q, kv_params, block_tables, context_lens, cu_seqlens, out, workspace, error_flag)
+    dev = _cuda_index(kv_codes, kv_params, q, block_tables, context_lens, cu_seqlens, out, workspace, error_flag)
     if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=dev)
-    if out.shape != q.shape or out.stride(2) != 1 or out.dtype != dtype:
+        out = torch.empty_like(q)
+    os_ = out.stride()
+    if out.shape != shape or out.dtype != dtype or os_[2] != 1:
         raise ValueError("out must match q with unit stride along head_dim")
     if workspace is None:
-        workspace = torch.empty(prefill_int4_workspace_bytes(t, batch, hq, hkv, d, bs, int(max_context), dtype),
-                                dtype=torch.uint8, device=dev)
-    elif not workspace.is_contiguous() or workspace.data_ptr() % 16:
-        raise ValueError("workspace must be contiguous and start on 16 bytes")
-    lib = _native.load()
-    with _on(dev):
-        _native.check(lib.psb_paged_prefill_int4(
-            q.data_ptr(), q.stride(0), q.stride(1), kv_codes.data_ptr(), kv_params.data_ptr(),
-            block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(), out.data_ptr(), out.stride(0),
-            out.stride(1), cu_seqlens.data_ptr(), batch, t, int(max_seqlen), int(max_context), hq, layer, nl, nb, hkv,
-            bs, d, _DTYPES[dtype], scale, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-            _ptr(error_flag), _stream(dev)), "paged_prefill_int4")
+        workspace = _scratch.get(prefill_int4_workspace_bytes(t, batch, hq, hkv, d, bs, int(max_context), dtype), dev)
+    else:
+        _check_workspace(workspace)
+    _call(dev, _native.load().psb_paged_prefill_int4, "paged_prefill_int4",
+          q.data_ptr(), qs[0], qs[1], kv_codes.data_ptr(), kv_params.data_ptr(), block_tables.data_ptr(), tst[0],
+          context_lens.data_ptr(), out.data_ptr(), os_[0], os_[1], cu_seqlens.data_ptr(), batch, t, int(max_seqlen),
+          int(max_context), hq, layer, nl, nb, hkv, bs, d, code, scale, workspace.data_ptr(), workspace.nbytes,
+          _ptr(error_flag))
     return out
 
 
@@ -906,21 +937,24 @@ def paged_prefill_int4(q: torch.Tensor, kv_codes: torch.Tensor, kv_params: torch
 
 
 def _tables_args(table_store, rows, first, second, free_blocks, free_state, names, error_flag):
-    """The checks extend_step and trim_tables share; returns the three plan rows, contiguous."""
-    if table_store.dtype != torch.int32 or table_store.ndim != 2 or table_store.stride(1) != 1 \
-            or table_store.stride(0) < table_store.shape[1]:
+    """The checks extend_step and trim_tables share; returns the store's
+    (row stride, rows, width), the batch, and the three plan rows, contiguous."""
+    i32 = torch.int32
+    shape = table_store.shape
+    stride = table_store.stride()
+    if table_store.dtype != i32 or len(shape) != 2 or stride[1] != 1 or stride[0] < shape[1]:
         raise ValueError("table_store must be int32 [R, W] with unit column stride and rows that do not overlap")
-    b = rows.shape[0] if rows.ndim == 1 else -1
-    for name, x in zip(names, (rows, first, second)):
-        if x.dtype != torch.int32 or x.ndim != 1 or x.shape[0] != b:
-            raise ValueError(f"{name} must be int32 [B]")
-    if free_blocks.dtype != torch.int32 or free_blocks.ndim != 1 or not free_blocks.is_contiguous() \
-            or free_blocks.shape[0] == 0:
+    plan = rows.shape
+    if (rows.dtype != i32 or first.dtype != i32 or second.dtype != i32 or len(plan) != 1 or first.shape != plan
+            or second.shape != plan):
+        raise ValueError(f"{', '.join(names)} must be int32 [B]")
+    fs = free_blocks.shape
+    if free_blocks.dtype != i32 or len(fs) != 1 or fs[0] == 0 or not free_blocks.is_contiguous():
         raise ValueError("free_blocks must be a contiguous int32 [num_blocks] tensor")
-    if free_state.dtype != torch.int32 or free_state.shape != (4,) or not free_state.is_contiguous():
+    if free_state.dtype != i32 or free_state.shape != (4,) or not free_state.is_contiguous():
         raise ValueError("free_state must be a contiguous int32 [4] tensor (head, count, 0, 0)")
     _check_flag(error_flag)
-    return rows.contiguous(), first.contiguous(), second.contiguous()
+    return (stride[0], shape[0], shape[1]), plan[0], rows.contiguous(), first.contiguous(), second.contiguous()
 
 
 def free_list(num_blocks: int, device: torch.device | str, order=None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -950,20 +984,19 @@ def extend_step(table_store: torch.Tensor, req_rows: torch.Tensor, starts: torch
     free blocks, 256: a row named twice, 4: a bad row, start, count or width,
     32: ``total`` is not the sum) and gives slots of -1 and lengths of 0.
     """
-    rows, starts, query_lens = _tables_args(table_store, req_rows, starts, query_lens, free_blocks, free_state,
-                                            ("req_rows", "starts", "query_lens"), error_flag)
-    bsz, total = rows.shape[0], int(total)
-    width = table_store.shape[1] if out_width is None else int(out_width)
+    store, bsz, rows, starts, query_lens = _tables_args(table_store, req_rows, starts, query_lens, free_blocks,
+                                                        free_state, ("req_rows", "starts", "query_lens"), error_flag)
+    total = int(total)
+    width = store[2] if out_width is None else int(out_width)
     if total < 0 or width <= 0 or block_size <= 0:
         raise ValueError("total must not be negative, out_width and block_size must be positive")
-    dev = table_store.device
-    _one_device(dev, rows, starts, query_lens, free_blocks, free_state, error_flag)
+    dev = _cuda_index(table_store, rows, starts, query_lens, free_blocks, free_state, error_flag)
     if out is None:
-        cu = torch.empty(bsz + 1, dtype=torch.int32, device=dev)
-        ctx = torch.empty(bsz, dtype=torch.int32, device=dev)
-        slots = torch.empty(total, dtype=torch.int64, device=dev)
-        pos = torch.empty(total, dtype=torch.int64, device=dev)
-        tables = torch.empty((bsz, width), dtype=torch.int32, device=dev)
+        cu = rows.new_empty(bsz + 1)
+        ctx = rows.new_empty(bsz)
+        slots = rows.new_empty(total, dtype=torch.int64)
+        pos = rows.new_empty(total, dtype=torch.int64)
+        tables = rows.new_empty((bsz, width))
     else:
         cu, ctx, slots, pos, tables = out
         ok = (cu.shape == (bsz + 1,) and cu.dtype == torch.int32 and ctx.shape == (bsz,) and ctx.dtype == torch.int32
@@ -973,20 +1006,16 @@ def extend_step(table_store: torch.Tensor, req_rows: torch.Tensor, starts: torch
         if not ok:
             raise ValueError("out must be contiguous (cu_seqlens [B+1] i32, context_lens [B] i32, slot_mapping [T] "
                              "i64, positions [T] i64, block_tables [B, out_width] i32)")
-        _one_device(dev, *out)
+        _cuda_index(table_store, *out)
     if bsz == 0:
         if total:
             raise ValueError("total must be 0 for an empty batch")
         cu.zero_()
         return cu, ctx, slots, pos, tables
-    lib = _native.load()
-    with _on(dev):
-        _native.check(lib.psb_extend_step(
-            table_store.data_ptr(), table_store.stride(0), table_store.shape[0], table_store.shape[1],
-            rows.data_ptr(), starts.data_ptr(), query_lens.data_ptr(), bsz, free_blocks.data_ptr(),
-            free_blocks.shape[0], free_state.data_ptr(), total, int(block_size), cu.data_ptr(), ctx.data_ptr(),
-            slots.data_ptr(), pos.data_ptr(), tables.data_ptr(), width, _ptr(error_flag), _stream(dev)),
-            "extend_step")
+    _call(dev, _native.load().psb_extend_step, "extend_step",
+          table_store.data_ptr(), *store, rows.data_ptr(), starts.data_ptr(), query_lens.data_ptr(), bsz,
+          free_blocks.data_ptr(), free_blocks.shape[0], free_state.data_ptr(), total, int(block_size), cu.data_ptr(),
+          ctx.data_ptr(), slots.data_ptr(), pos.data_ptr(), tables.data_ptr(), width, _ptr(error_flag))
     return cu, ctx, slots, pos, tables
 
 
@@ -999,16 +1028,12 @@ def trim_tables(table_store: torch.Tensor, req_rows: torch.Tensor, held_lens: to
     free ring entry by entry, in table order, as ``BlockManager.free`` returns
     them.  Checked and refused as a whole, like ``extend_step``.
     """
-    rows, held_lens, keep_lens = _tables_args(table_store, req_rows, held_lens, keep_lens, free_blocks, free_state,
-                                              ("req_rows", "held_lens", "keep_lens"), error_flag)
+    store, bsz, rows, held_lens, keep_lens = _tables_args(table_store, req_rows, held_lens, keep_lens, free_blocks,
+                                                          free_state, ("req_rows", "held_lens", "keep_lens"),
+                                                          error_flag)
     if block_size <= 0:
         raise ValueError("block_size must be positive")
-    dev = table_store.device
-    _one_device(dev, rows, held_lens, keep_lens, free_blocks, free_state, error_flag)
-    lib = _native.load()
-    with _on(dev):
-        _native.check(lib.psb_trim_tables(
-            table_store.data_ptr(), table_store.stride(0), table_store.shape[0], table_store.shape[1],
-            rows.data_ptr(), held_lens.data_ptr(), keep_lens.data_ptr(), rows.shape[0], free_blocks.data_ptr(),
-            free_blocks.shape[0], free_state.data_ptr(), int(block_size), _ptr(error_flag), _stream(dev)),
-            "trim_tables")
+    dev = _cuda_index(table_store, rows, held_lens, keep_lens, free_blocks, free_state, error_flag)
+    _call(dev, _native.load().psb_trim_tables, "trim_tables",
+          table_store.data_ptr(), *store, rows.data_ptr(), held_lens.data_ptr(), keep_lens.data_ptr(), bsz,
+          free_blocks.data_ptr(), free_blocks.shape[0], free_state.data_ptr(), int(block_size), _ptr(error_flag))

@@ -9,6 +9,11 @@ Public surface:
 * ``rope_and_write_tokens`` - the glue's rotary embedding fused with the write
 * ``ops.reshape_and_cache / paged_decode / varlen_prefill / pack_step`` -
   tensor-level API over the C ABI (include/pagedserve_b200.h)
+* ``PagedKVCache(kv_bits=4)`` - the same cache as 4-bit codes, taken by the
+  drop-ins above, ``PagedModelRunner`` and ``ReplicaEngine``; tensor level:
+  ``ops.*_int4``
+* ``ops.extend_step / trim_tables`` - block allocation and release on the
+  device, so that a step needs no host bookkeeping
 * ``select_next_tokens`` / ``read_selection`` - the step's greedy argmax and
   stop test on the device, one host sync per batch (replaces the per-row
   ``.item()`` loop of pagedserve/engine/continuous_batcher.py:333-360)

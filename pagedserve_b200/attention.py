@@ -21,6 +21,9 @@ whose ``metadata_epoch`` changes on every allocation, growth or release, the
 device copies (table, lengths, slots) are kept on the cache object and reused
 while the epoch, the request ids and the positions are unchanged; any other
 cache object is rebuilt on every call, as in the reference.
+
+Each entry point takes a ``PagedKVCache`` of 4-bit codes (``kv_bits=4``) as
+well: the same checks and metadata, then the 4-bit pool's kernels.
 """
 
 from __future__ import annotations
@@ -309,9 +312,22 @@ def paged_decode_attention(query: torch.Tensor, cache, request_ids: Sequence[str
     if meta is not None:
         return meta.launch(query, layer)
     meta = _validated_metadata(query, cache, request_ids, positions, layer)
+    if _is_int4(cache.kv_cache):
+        return _decode_int4(meta, cache, query, layer)
     out = _launch(meta, cache, query, layer)
     _remember(cache, sig, meta)
     return out
+
+
+def _is_int4(kv) -> bool:
+    """Whether a cache's pools hold 4-bit codes (a reference cache has no such attribute)."""
+    return getattr(kv, "kv_bits", 16) == 4
+
+
+def _decode_int4(meta, cache, query, layer):
+    kv = cache.kv_cache
+    return ops.paged_decode_int4(query, kv.kv_codes, kv.kv_params, meta.tables, meta.lengths, layer,
+                                 max_context=meta.width * cache.block_size)
 
 
 # The layer calls of one decode iteration repeat the same lists and tensors of
@@ -384,7 +400,7 @@ def _validated_metadata(query, cache, request_ids, positions, layer):
         raise ValueError("Query heads must be divisible by KV heads")
     if dtype != kv.dtype:
         raise ValueError("Query dtype must match cache dtype")
-    k_cache = kv.k_cache
+    k_cache = kv.kv_codes if _is_int4(kv) else kv.k_cache
     if dev != k_cache.get_device():
         raise ValueError("Query and cache must be on the same device")
     if not 0 <= layer < k_cache.shape[0]:
@@ -405,7 +421,8 @@ def paged_decode_attention_with_write(query: torch.Tensor, key: torch.Tensor, va
     ``triton_paged_decode_attention(query, cache, request_ids, positions,
     layer)`` (:126-135): ``key``/``value`` are ``[B, Hkv, D]`` (or
     ``[B, Hkv, 1, D]``) and row b lands at ``positions[b]``, the last position
-    the query attends to.  Runs as ``psb_paged_decode_append``.
+    the query attends to.  Runs as ``psb_paged_decode_append`` (a 4-bit pool:
+    as a write launch and the attention).
     """
     sig = (query.shape, query.dtype, query.get_device(), key.shape, key.dtype, key.get_device(), value.shape,
            value.dtype, value.get_device())
@@ -428,6 +445,9 @@ def paged_decode_attention_with_write(query: torch.Tensor, key: torch.Tensor, va
     dev = query.get_device()
     if key.get_device() != dev or value.get_device() != dev:
         raise ValueError("new K/V must be on the query's device")
+    if _is_int4(kv):  # the row's minimum and maximum are needed before its codes: a launch of its own
+        _write_rows(kv, key, value, _slots(cache, request_ids, positions, query.device), layer)
+        return _decode_int4(meta, cache, query, layer)
     out = _launch(meta, cache, query, layer, key, value)
     _remember(cache, sig, meta)
     return out
@@ -461,7 +481,16 @@ def write_tokens(cache, request_ids: Sequence[str], positions: Sequence[int], la
         raise ValueError(f"K/V tensors must have dtype {kv.dtype}")
 
     slot_t = _slots(cache, request_ids, positions, key.device)
-    ops.reshape_and_cache(key, value, kv.k_cache, kv.v_cache, slot_t, layer)
+    _write_rows(kv, key, value, slot_t, layer)
+
+
+def _write_rows(kv, key, value, slots, layer) -> None:
+    if key.ndim == 4:  # [B, Hkv, 1, D]
+        key, value = key.squeeze(2), value.squeeze(2)
+    if _is_int4(kv):
+        ops.reshape_and_cache_int4(key, value, kv.kv_codes, kv.kv_params, slots, layer)
+    else:
+        ops.reshape_and_cache(key, value, kv.k_cache, kv.v_cache, slots, layer)
 
 
 def rope_and_write_tokens(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cos: torch.Tensor,
@@ -489,6 +518,11 @@ def rope_and_write_tokens(query: torch.Tensor, key: torch.Tensor, value: torch.T
     if len(request_ids) != batch or len(positions) != batch:
         raise ValueError("Request IDs and positions must match batch size")
     slot_t = _slots(cache, request_ids, positions, key.device)
+    if _is_int4(kv):
+        q_rot, _ = ops.rope_reshape_and_cache_int4(query.squeeze(2), key, value, cos.reshape(batch, -1),
+                                                   sin.reshape(batch, -1), kv.kv_codes, kv.kv_params, slot_t, layer,
+                                                   key_out=False)
+        return q_rot.unsqueeze(2)
     q_rot, _ = ops.rope_reshape_and_cache(query.squeeze(2), key, value, cos.reshape(batch, -1),
                                           sin.reshape(batch, -1), kv.k_cache, kv.v_cache, slot_t, layer,
                                           key_out=False)

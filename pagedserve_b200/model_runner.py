@@ -156,20 +156,48 @@ def rope_tables(cfg: QwenConfig, device, dtype) -> tuple[torch.Tensor, torch.Ten
 
 
 class PagedModelRunner:
-    """Batched Qwen2 decode and packed prefill over a ``PagedKVCache``'s pools."""
+    """Batched Qwen2 decode and packed prefill over a ``PagedKVCache``'s pools.
 
-    def __init__(self, weights: QwenWeights, k_cache: torch.Tensor, v_cache: torch.Tensor, block_size: int = 16):
+    ``kv_bits=4``: ``k_cache`` and ``v_cache`` are the ``kv_codes`` and
+    ``kv_params`` of a 4-bit pool.  A prompt then still attends to its own
+    unrounded keys and values (they are at hand in the pass that makes them);
+    every later token attends to what the pool holds.
+    """
+
+    def __init__(self, weights: QwenWeights, k_cache: torch.Tensor, v_cache: torch.Tensor, block_size: int = 16,
+                 kv_bits: int = 16):
         cfg = weights.cfg
-        if k_cache.shape[0] != cfg.layers or tuple(k_cache.shape[2:]) != (cfg.kv_heads, block_size, cfg.head_dim):
+        if kv_bits not in (4, 16):
+            raise ValueError("kv_bits must be 4 or 16")
+        self.kv_bits = kv_bits
+        if kv_bits == 4:
+            heads = (cfg.kv_heads, 2, block_size)
+            if (k_cache.dtype != torch.uint8 or k_cache.shape[0] != cfg.layers
+                    or tuple(k_cache.shape[2:]) != heads + (cfg.head_dim // 2,)
+                    or tuple(v_cache.shape) != tuple(k_cache.shape[:5]) + (2,)):
+                raise ValueError("the pools do not match the model: expected uint8 "
+                                 f"[{cfg.layers}, blocks, {cfg.kv_heads}, 2, {block_size}, {cfg.head_dim // 2}] codes "
+                                 "and as many parameter pairs")
+        elif k_cache.shape[0] != cfg.layers or tuple(k_cache.shape[2:]) != (cfg.kv_heads, block_size, cfg.head_dim):
             raise ValueError("the pools do not match the model: expected "
                              f"[{cfg.layers}, blocks, {cfg.kv_heads}, {block_size}, {cfg.head_dim}]")
-        if k_cache.dtype != weights.dtype:
+        if v_cache.dtype != weights.dtype or (kv_bits != 4 and k_cache.dtype != weights.dtype):
             raise ValueError("pool and weight dtypes differ")
         self.cfg, self.w = cfg, weights
         self.k_cache, self.v_cache = k_cache, v_cache
         self.block_size = block_size
         self.cos, self.sin = rope_tables(cfg, weights.device, weights.dtype)
         self.scale = 1.0 / math.sqrt(cfg.head_dim)
+
+    # -- the pool's operators -----------------------------------------------------
+    def _rope_write(self, q, k, v, cos, sin, slots, layer: int, key_out):
+        op = ops.rope_reshape_and_cache_int4 if self.kv_bits == 4 else ops.rope_reshape_and_cache
+        return op(q, k, v, cos, sin, self.k_cache, self.v_cache, slots, layer, key_out=key_out)
+
+    def _paged_decode(self, q, block_tables, context_lens, layer: int, max_context: int, out=None):
+        op = ops.paged_decode_int4 if self.kv_bits == 4 else ops.paged_decode
+        return op(q, self.k_cache, self.v_cache, block_tables, context_lens, layer, scale=self.scale, out=out,
+                  max_context=max_context)
 
     # -- pieces shared by both passes -----------------------------------------
     def _qkv(self, x: torch.Tensor, layer: int):
@@ -203,8 +231,7 @@ class PagedModelRunner:
             if layer > 0:
                 ops.add_rms_norm(mlp_out, w.ln1[layer], eps, residual=residual, out=x)
             q, k, v = self._qkv(x, layer)
-            q_rot, k_rot = ops.rope_reshape_and_cache(q, k, v, cos, sin, self.k_cache, self.v_cache, slots, layer,
-                                                      key_out=None if want_keys else False)
+            q_rot, k_rot = self._rope_write(q, k, v, cos, sin, slots, layer, None if want_keys else False)
             attn = attend(q_rot, k_rot, v, layer)
             o = F.linear(attn.view(attn.shape[0], -1), w.o[layer])
             ops.add_rms_norm(o, w.ln2[layer], eps, residual=residual, out=x)
@@ -226,8 +253,7 @@ class PagedModelRunner:
         max_context = block_tables.shape[1] * self.block_size if max_context is None else max_context
 
         def attend(q_rot, _k, _v, layer):
-            return ops.paged_decode(q_rot, self.k_cache, self.v_cache, block_tables, context_lens, layer,
-                                    scale=self.scale, max_context=max_context)
+            return self._paged_decode(q_rot, block_tables, context_lens, layer, max_context)
         return self._layers(tokens, positions, slots, attend, want_keys=False)
 
     # -- packed prefill ----------------------------------------------------------
@@ -268,8 +294,7 @@ class PagedModelRunner:
                 ops.varlen_prefill(q_rot[:tp], k_rot[:tp], v[:tp], prefill_cu, max_seqlen, scale=self.scale,
                                    out=out[:tp])
             if q_rot.shape[0] > tp:
-                ops.paged_decode(q_rot[tp:], self.k_cache, self.v_cache, block_tables, context_lens, layer,
-                                 scale=self.scale, out=out[tp:], max_context=max_context)
+                self._paged_decode(q_rot[tp:], block_tables, context_lens, layer, max_context, out=out[tp:])
             return out
         return self._layers(tokens, positions, slots, attend, want_keys=True, last_rows=last_rows)
 

@@ -12,6 +12,11 @@
 * ``select_tokens``      greedy next token + stop check of every row on the
   device (replaces ``logits[:, -1, :].argmax`` and the per-row ``.item()``
   loop of pagedserve/engine/continuous_batcher.py:333-360)
+* ``reshape_and_cache_int4``, ``rope_reshape_and_cache_int4``,
+  ``gather_cache_int4``, ``paged_decode_int4``, ``paged_prefill_int4``  the
+  write, read-back and attention over a pool of 4-bit codes
+* ``extend_step``, ``trim_tables``  ``pack_step`` with the block allocation
+  on the device too, and its reverse (``BlockManager``'s free list as a ring)
 
 Every function requires CUDA tensors, launches on the current stream and
 returns without synchronising.  There is no CPU path.

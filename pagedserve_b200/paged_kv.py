@@ -13,7 +13,9 @@ raised follow the reference so callers can switch without edits:
 
 Added for the batched path: ``PagedKVCache.table_rows`` (a padded int32
 table for a list of requests, built in one numpy pass) and
-``PagedKVCache.slot_of`` (the int64 slot a position maps to).
+``PagedKVCache.slot_of`` (the int64 slot a position maps to); and pools that
+hold 4-bit codes (``kv_bits=4``: ``kv_codes`` and ``kv_params`` in place of
+``k_cache`` and ``v_cache``, the layout of ``ops.reshape_and_cache_int4``).
 """
 
 from __future__ import annotations
@@ -22,6 +24,8 @@ from collections import deque
 
 import numpy as np
 import torch
+
+from . import ops
 
 
 class BlockManager:
@@ -130,10 +134,17 @@ class BlockTable:
 
 
 class KVCache:
-    """The K and V pools, ``[num_layers, num_blocks, num_kv_heads, block_size, head_dim]`` each."""
+    """The K and V pools, ``[num_layers, num_blocks, num_kv_heads, block_size, head_dim]`` each.
+
+    ``kv_bits=4``: both in ``kv_codes`` (uint8 ``[num_layers, num_blocks,
+    num_kv_heads, 2, block_size, head_dim / 2]``) and ``kv_params`` (``dtype``
+    ``[..., 2, block_size, 2]``: the step and the offset of every row), with
+    ``k_cache`` and ``v_cache`` None; rows go in and out as ``dtype`` on a
+    CUDA device, and ``read_block`` returns copies instead of views.
+    """
 
     def __init__(self, num_blocks: int, num_layers: int, num_kv_heads: int, head_dim: int, block_size: int = 16,
-                 dtype: torch.dtype = torch.bfloat16, device: str | torch.device = "cuda"):
+                 dtype: torch.dtype = torch.bfloat16, device: str | torch.device = "cuda", kv_bits: int = 16):
         for name, val in (("num_blocks", num_blocks), ("num_layers", num_layers), ("num_kv_heads", num_kv_heads),
                           ("head_dim", head_dim), ("block_size", block_size)):
             if val <= 0:
@@ -145,6 +156,19 @@ class KVCache:
         self.block_size = block_size
         self.dtype = dtype
         self.device = torch.device(device)
+        if kv_bits not in (4, 16):
+            raise ValueError("kv_bits must be 4 or 16 (16: the pools hold dtype itself)")
+        self.kv_bits = kv_bits
+        self.kv_codes = self.kv_params = None
+        if kv_bits == 4:
+            if head_dim % 2 or head_dim > ops.INT4_MAX_HEAD_DIM:
+                raise ValueError(f"4-bit pools need an even head_dim of at most {ops.INT4_MAX_HEAD_DIM}")
+            ops.dtype_code(dtype)  # refuses what the kernels do not take
+            shape = (num_layers, num_blocks, num_kv_heads, 2, block_size)
+            self.kv_codes = torch.empty(shape + (head_dim // 2,), dtype=torch.uint8, device=self.device)
+            self.kv_params = torch.empty(shape + (2,), dtype=dtype, device=self.device)
+            self.k_cache = self.v_cache = None
+            return
         shape = (num_layers, num_blocks, num_kv_heads, block_size, head_dim)
         self.k_cache = torch.empty(shape, dtype=dtype, device=self.device)
         self.v_cache = torch.empty(shape, dtype=dtype, device=self.device)
@@ -157,7 +181,8 @@ class KVCache:
     def block_bytes(self) -> int:
         """K+V bytes of one physical block across all layers."""
         esz = torch.empty((), dtype=self.dtype).element_size()
-        return self.num_layers * 2 * self.num_kv_heads * self.block_size * self.head_dim * esz
+        row = self.head_dim // 2 + 2 * esz if self.kv_bits == 4 else self.head_dim * esz
+        return self.num_layers * 2 * self.num_kv_heads * self.block_size * row
 
     @property
     def total_bytes(self) -> int:
@@ -179,23 +204,47 @@ class KVCache:
                 raise ValueError(f"Invalid {name} shape: expected {self.block_shape}, got {tuple(t.shape)}")
             if t.dtype != self.dtype:
                 raise ValueError(f"Invalid {name} dtype: expected {self.dtype}, got {t.dtype}")
+        if self.kv_bits == 4:
+            self._write_rows(layer, self._block_slots(block_id), key.transpose(0, 1), value.transpose(0, 1))
+            return
         self.k_cache[layer, block_id].copy_(key)
         self.v_cache[layer, block_id].copy_(value)
 
     def read_block(self, layer: int, block_id: int) -> tuple[torch.Tensor, torch.Tensor]:
         self._check_layer(layer)
         self._check_block(block_id)
+        if self.kv_bits == 4:
+            key, value = self._read_rows(layer, self._block_slots(block_id))
+            return key.transpose(0, 1), value.transpose(0, 1)
         return self.k_cache[layer, block_id], self.v_cache[layer, block_id]
+
+    # -- rows of a 4-bit pool ---------------------------------------------------
+    def _block_slots(self, block_id: int) -> torch.Tensor:
+        first = block_id * self.block_size
+        return torch.arange(first, first + self.block_size, dtype=torch.int64, device=self.device)
+
+    def _write_rows(self, layer: int, slots: torch.Tensor, key: torch.Tensor, value: torch.Tensor) -> None:
+        """Quantise ``key, value [T, Hkv, D]`` into ``slots [T]``."""
+        if not key.is_cuda:
+            raise ValueError("4-bit pools are written and read on a CUDA device")
+        ops.reshape_and_cache_int4(key, value, self.kv_codes, self.kv_params, slots, layer)
+
+    def _read_rows(self, layer: int, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        if not slots.is_cuda:
+            raise ValueError("4-bit pools are written and read on a CUDA device")
+        return ops.gather_cache_int4(self.kv_codes, self.kv_params, slots, layer)
 
 
 class PagedKVCache:
     """Block allocation + per-request tables + the pools, behind one object."""
 
     def __init__(self, num_blocks: int, num_layers: int, num_kv_heads: int, head_dim: int, block_size: int = 16,
-                 dtype: torch.dtype = torch.bfloat16, device: str | torch.device = "cuda", free_order=None):
+                 dtype: torch.dtype = torch.bfloat16, device: str | torch.device = "cuda", free_order=None,
+                 kv_bits: int = 16):
         self.block_manager = BlockManager(num_blocks=num_blocks, block_size=block_size, free_order=free_order)
         self.kv_cache = KVCache(num_blocks=num_blocks, num_layers=num_layers, num_kv_heads=num_kv_heads,
-                                head_dim=head_dim, block_size=block_size, dtype=dtype, device=device)
+                                head_dim=head_dim, block_size=block_size, dtype=dtype, device=device,
+                                kv_bits=kv_bits)
         self._tables: dict[str, BlockTable] = {}
         self._counts: dict[str, int] = {}
         self._epoch = 0
@@ -342,6 +391,12 @@ class PagedKVCache:
             raise ValueError(f"Expected K/V shape {shape}; got key={tuple(key.shape)}, value={tuple(value.shape)}")
         if key.dtype != self.kv_cache.dtype or value.dtype != self.kv_cache.dtype:
             raise ValueError(f"K/V tensors must have dtype {self.kv_cache.dtype}")
+        if self.kv_cache.kv_bits == 4:
+            kv = self.kv_cache
+            if key.device != kv.kv_codes.device or value.device != kv.kv_codes.device:
+                raise ValueError("K/V tensors must be on the same devices as their respective cache tensors")
+            kv._write_rows(layer, self._slot_tensor(block, offset), key[None], value[None])
+            return
         if key.device != self.kv_cache.k_cache.device or value.device != self.kv_cache.v_cache.device:
             raise ValueError("K/V tensors must be on the same devices as their respective cache tensors")
         self.kv_cache.k_cache[layer, block, :, offset, :].copy_(key)
@@ -349,7 +404,13 @@ class PagedKVCache:
 
     def read_token(self, request_id: str, layer: int, token_position: int) -> tuple[torch.Tensor, torch.Tensor]:
         block, offset = self._locate(request_id, token_position)
+        if self.kv_cache.kv_bits == 4:
+            key, value = self.kv_cache._read_rows(layer, self._slot_tensor(block, offset))
+            return key[0], value[0]
         return (self.kv_cache.k_cache[layer, block, :, offset, :], self.kv_cache.v_cache[layer, block, :, offset, :])
+
+    def _slot_tensor(self, block: int, offset: int) -> torch.Tensor:
+        return torch.full((1,), block * self.block_size + offset, dtype=torch.int64, device=self.kv_cache.device)
 
     # -- batched helpers for the B200 path -----------------------------------
     def slot_of(self, request_id: str, token_position: int) -> int:

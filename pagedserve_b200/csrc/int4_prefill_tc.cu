@@ -2,14 +2,16 @@
 // 5th-generation tensor cores: bf16/f16, head_dim 64, any block_size, up to
 // 128 q heads per kv head.
 //
-// Mathematics.  As in int4_decode_fast.cu: with codes c, step and mid per
-// (token, kv head), q . k_t = step_t (q . (c_t - 7.5)) + mid_t sum(q) and
-// sum_t p_t v_t = sum_t (p_t step_t)(c_t - 7.5) + sum_t p_t mid_t.  The codes
-// become exact 16-bit operands in shared memory; step and mid act on scores
-// and probabilities in fp32.  K's operand is 128 + c (bf16) or 1024 + c (f16),
-// a constant high byte over the code, and the offset goes with mid; V's is
-// (c - 7.5) 2^-9 in f16 whatever T is, next to p step scaled by a power of two
-// and rounded to f16 - the one rounding below fp32.
+// Mathematics.  A row's values are mid + step (c - 7.5).  K goes to the tensor
+// cores as two operands of type T: each value rounded to T and what that
+// leaves out, rounded again (together 2^-17 of the value or less), so that S
+// needs nothing but the softmax's own scale.  V goes as f16 steps times codes:
+// step (c - 7.5) scaled by a power of two and rounded (2^-12), next to
+// probabilities rounded to f16 (2^-12); the mids, which no cancellation with
+// the codes may touch, are summed in fp32 beside the denominator.  The codes
+// could also stay bare with step and mid applied to S and P in fp32: that
+// reads four factors per key from shared memory in every softmax thread
+// (measured: 57% of the shared-memory cycles, no faster).
 //
 // Tiles.  The q heads of a kv head read the same keys, so a tile's 128 rows
 // are TQ = 128 / group consecutive tokens times the group's heads (one TMA box
@@ -21,14 +23,18 @@
 // long prefix has fewer tiles than the GPU has SMs).
 //
 // CTA: eight warps.  Warps 0-3 are the softmax (thread r = TMEM lane r = row r
-// of the tile).  In warps 4-7 one lane issues the Q loads and S = Q K^T (four
-// tcgen05.mma M 128 N 64 K 16, one step ahead, two TMEM S buffers), one lane
-// O += P V (P read from TMEM over the S it came from, two O buffers in turn),
-// and two warps decode K and V into a ring of kStages shared-memory stages
-// (128-byte swizzle), together with the 64 tokens' factors.  A warp pair's
-// two roles are swapped in the second half of the grid, so that the decoding
-// warps of an SM's two CTAs sit on different schedulers.  The softmax half has
-// 168 registers, the other 88 (setmaxnreg; 256 x 128 at launch).
+// of the tile).  In warps 4-7 one lane issues the Q loads and the products -
+// S = Q K^T (eight tcgen05.mma M 128 N 64 K 16, two TMEM S buffers) a step
+// ahead of O += P V (P read from TMEM over the S it came from, two O buffers
+// in turn) - and three warps decode: 32 keys each for K, all 64 for V, into
+// rings of shared-memory stages (128-byte swizzle).  The four roles are turned
+// by one warp in the second half of the grid, which spreads the decoding of an
+// SM's two CTAs over its schedulers.  The softmax half has 168 registers, the
+// other 88 (setmaxnreg; 256 x 128 at launch).
+//
+// Four roles share an SM's instruction caches, so every loop has one body:
+// the same kernel with its loops unrolled and peeled (121 KB of code) spent
+// more issue slots waiting for instructions than on anything else.
 //
 // Every mbarrier wait is bounded; no barrier can run two phases ahead of a
 // waiter: a stage's next phase needs its own release, a step's barriers
@@ -48,30 +54,32 @@ constexpr int kThreads = 256;
 constexpr int kRows = 128;          // rows of a tile
 constexpr int kBN = 64;             // keys per step
 constexpr int kDim = 64;
-constexpr int kStages = 3;
+constexpr int kKStages = 2, kVStages = 3;
 constexpr uint32_t kQTile = kRows * kDim * 2;
 constexpr uint32_t kKvTile = kBN * kDim * 2;
 constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kSCol = 0, kOCol = 128;
 constexpr float kGrowth = 4.f;      // log2 of how far a score may exceed the exponents' reference
-constexpr int kPBits = 11;          // p step is scaled to at most 2^kGrowth 2^kPBits
-constexpr float kVBack = 512.f;     // V's operand is (c - 7.5) / kVBack
+constexpr int kPBits = 11;          // probabilities are 2^kPBits p, at most 2^(kPBits + kGrowth)
+constexpr int kStepBits = 15;       // V's steps are scaled to below 2^kStepBits
+constexpr int kVBits = 9;           // and its codes are (c - 7.5) 2^-kVBits
 constexpr int kMaxCtas = 320;       // grid limit
 constexpr int kPartFloats = kRows * (kDim + 2);
 constexpr int kMaxSeqs = 2048, kMaxTiles = 8192;
 
-// factors of a stage's 64 tokens, and what is wrong with them
-struct Factors {
-  float ks[kBN], km[kBN], vs[kBN], vm[kBN];
+// What a V stage's 64 tokens need besides their codes and steps.
+struct Extra {
+  float mid[kBN];   // 0 where it is not finite
   uint32_t bad[2];  // bit t: token t's block is outside the pool
-  int vexp;         // p step was scaled by 2^(kPBits - vexp)
-  int pad;
+  uint32_t nan[2];  // bit t: token t's mid is not finite
+  int vexp;         // steps were scaled by 2^(kStepBits - vexp)
+  int pad[3];
 };
 
-// dynamic shared memory (1024-byte aligned): Q0 | Q1 | K ring | V ring | factors | barriers | tables
-constexpr uint32_t kOffK = 2 * kQTile, kOffV = kOffK + kStages * kKvTile;
-constexpr uint32_t kOffF = kOffV + kStages * kKvTile;
-constexpr uint32_t kOffBars = kOffF + kStages * sizeof(Factors);
+// dynamic shared memory (1024-byte aligned): Q0 | Q1 | K ring (high, low parts) | V ring | extras | barriers | tables
+constexpr uint32_t kOffK = 2 * kQTile, kOffV = kOffK + kKStages * 2 * kKvTile;
+constexpr uint32_t kOffX = kOffV + kVStages * kKvTile;
+constexpr uint32_t kOffBars = kOffX + kVStages * sizeof(Extra);
 constexpr uint32_t kOffTab = kOffBars + 256;
 
 // A tile cut at a CTA's end that began in it: its kv head, first row of q and
@@ -108,17 +116,70 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   return d;
 }
 
-// A wait of a whole warp: its lanes give up together or not at all.
-__device__ __forceinline__ bool warp_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// Two fp32 values rounded to T, finite ones to the largest finite value at most.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2_sat(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2_sat<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2_sat<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 
-// What every role knows of the batch: lengths per sequence, tiles, steps.
+// 16 columns of a warp's TMEM lanes.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// mbar_wait with one copy of the instruction.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t t0 = 0;
+#pragma unroll 1
+  while (!mbar_try_wait_sleep(addr, parity, 100000u)) {
+    const uint64_t t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > kWaitLimitNs) return false;
+  }
+  return true;
+}
+// The same for a whole warp: its lanes give up together or not at all.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait(bar, parity));
+}
+
+// What every role knows of the batch (in shared memory).
 struct Plan {
   const int32_t* len;    // [num_seqs] query rows
   const int32_t* ctx;    // [num_seqs] tokens in the pool
   const int32_t* q0;     // [num_seqs] first row
   const int32_t* tfirst; // [num_seqs + 1] tiles before a sequence
-  const int32_t* sfirst; // [tiles + 1] steps before a tile
-  int32_t num_seqs, tiles, steps;  // of one kv head
+  const int32_t* sfirst; // [tiles + 1] steps before a tile, of one kv head
+  const int32_t* tseq;   // [tiles] a tile's sequence
+  int32_t tiles;
 };
 
 __device__ __forceinline__ int last_le(const int32_t* v, int n, int x) {  // last i < n with v[i] <= x
@@ -131,41 +192,29 @@ __device__ __forceinline__ int last_le(const int32_t* v, int n, int x) {  // las
 }
 
 // A run of steps of one tile.
-struct Seg {
+struct Run {
   int kvh, tile, seq, qt;  // qt: the tile's number in its sequence
   int j0, n;               // its steps j0 .. j0 + n - 1 of n_kv
   int n_kv;
 };
 
-// Walks a CTA's steps [pos, end) tile by tile.
+// Walks a CTA's steps tile by tile.
 struct Cursor {
-  const Plan& pl;
-  int64_t pos, end;
-  int kvh, tile, seq;
-  __device__ Cursor(const Plan& p, int64_t a, int64_t e) : pl(p), pos(a), end(e), kvh(0), tile(0), seq(0) {
-    if (a >= e) return;
-    kvh = static_cast<int>(a / p.steps);
-    const int r = static_cast<int>(a - static_cast<int64_t>(kvh) * p.steps);
-    tile = last_le(p.sfirst, p.tiles, r);
-    seq = last_le(p.tfirst, p.num_seqs, tile);
-  }
-  __device__ bool more() const { return pos < end; }
-  __device__ Seg take() {  // the next run
-    Seg s;
+  int kvh, tile, j0, left;
+  __device__ Run take(const Plan& pl) {  // the next run (left > 0)
+    Run s;
     s.kvh = kvh;
     s.tile = tile;
-    s.seq = seq;
-    s.qt = tile - pl.tfirst[seq];
+    s.seq = pl.tseq[tile];
+    s.qt = tile - pl.tfirst[s.seq];
     s.n_kv = pl.sfirst[tile + 1] - pl.sfirst[tile];
-    s.j0 = static_cast<int>(pos - (static_cast<int64_t>(kvh) * pl.steps + pl.sfirst[tile]));
-    s.n = static_cast<int>(min(static_cast<int64_t>(s.n_kv - s.j0), end - pos));
-    pos += s.n;
-    if (pos < end && ++tile == pl.tiles) {
+    s.j0 = j0;
+    s.n = min(s.n_kv - j0, left);
+    left -= s.n;
+    j0 = 0;
+    if (++tile == pl.tiles) {
       tile = 0;
       ++kvh;
-      seq = last_le(pl.tfirst, pl.num_seqs, 0);
-    } else if (pos < end) {
-      while (pl.tfirst[seq + 1] <= tile) ++seq;  // sequences without rows have no tiles
     }
     return s;
   }
@@ -177,24 +226,24 @@ __global__ void __launch_bounds__(kThreads, 2)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const Int4PrefillParams& p = tp.a;
-  Factors* const fac = reinterpret_cast<Factors*>(smem + kOffF);
+  Extra* const ext = reinterpret_cast<Extra*>(smem + kOffX);
   uint64_t* const bar_q = reinterpret_cast<uint64_t*>(smem + kOffBars);  // [2] Q loaded
-  uint64_t* const bar_qfree = bar_q + 2;      // [2] Q K^T of the run in the buffer done
-  uint64_t* const bar_qread = bar_q + 4;      // [2] the softmax has its row sums
-  uint64_t* const bar_k = bar_q + 6;          // [kStages] K decoded
-  uint64_t* const bar_v = bar_k + kStages;    // [kStages] V decoded
-  uint64_t* const bar_kfree = bar_v + kStages;  // [kStages] softmax of the step done (so is its Q K^T)
-  uint64_t* const bar_vfree = bar_kfree + kStages;  // [kStages] P V done
-  uint64_t* const bar_s = bar_vfree + kStages;  // [2]
+  uint64_t* const bar_k = bar_q + 2;          // [kKStages] K decoded (two warps)
+  uint64_t* const bar_kfree = bar_k + kKStages;  // [kKStages] Q K^T done
+  uint64_t* const bar_v = bar_kfree + kKStages;  // [kVStages] V decoded
+  uint64_t* const bar_vfree = bar_v + kVStages;  // [kVStages] P V done
+  uint64_t* const bar_s = bar_vfree + kVStages;  // [2]
   uint64_t* const bar_p = bar_s + 2;          // [2]
   uint64_t* const bar_pv = bar_p + 2;         // [2]
-  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bar_pv + 2);
-  static_assert((6 + 4 * kStages + 6) * 8 + 4 <= 256, "barriers fit their area");
+  uint64_t* const bar_drain = bar_pv + 2;     // after a failed wait: every product issued so far is done
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bar_drain + 1);
+  static_assert((2 + 2 * kKStages + 2 * kVStages + 7) * 8 + 4 <= 256, "barriers fit their area");
   int32_t* const s_len = reinterpret_cast<int32_t*>(smem + kOffTab);
   int32_t* const s_ctx = s_len + p.num_seqs;
   int32_t* const s_q0 = s_ctx + p.num_seqs;
   int32_t* const s_tfirst = s_q0 + p.num_seqs;
   int32_t* const s_sfirst = s_tfirst + p.num_seqs + 1;
+  int32_t* const s_tseq = s_sfirst + tp.max_tiles + 1;
   __shared__ int32_t warp_sums[kThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int TQ = tp.tq, group = tp.group;
@@ -212,7 +261,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     int run = incl - v;
     total = 0;
-#pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) run += warp_sums[w];
       total += warp_sums[w];
@@ -259,6 +307,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       // keys 0 .. position of the tile's last row
       const int n = (s_ctx[s] - s_len[s] + min(s_len[s], (qt + 1) * TQ) + kBN - 1) / kBN;
       s_sfirst[t] = n;
+      s_tseq[t] = s;
       steps += n;
     }
     run = scan(steps, n_steps);
@@ -270,35 +319,44 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (tid == 0) s_sfirst[n_tiles] = n_steps;
     __syncthreads();
   }
-  const Plan plan{s_len, s_ctx, s_q0, s_tfirst, s_sfirst, p.num_seqs, n_tiles, n_steps};
-  const int64_t total_steps = static_cast<int64_t>(n_steps) * p.hkv;
-  const int act = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total_steps));
+  const Plan plan{s_len, s_ctx, s_q0, s_tfirst, s_sfirst, s_tseq, n_tiles};
+  const uint32_t total_steps = static_cast<uint32_t>(n_steps) * p.hkv;  // below 2^31
+  const uint32_t act = min(gridDim.x, total_steps);
   Cut* const cuts = reinterpret_cast<Cut*>(tp.part);
   float* const part = tp.part + kMaxCtas * (sizeof(Cut) / sizeof(float));
-  const int cta = blockIdx.x;
+  const uint32_t cta = blockIdx.x;
   if (cta >= act) {
     if (tid == 0) cuts[cta] = Cut{0, 0, 0, 0};
     return;
   }
-  auto cta_start = [&](int c) -> int64_t { return total_steps * c / act; };
-  const int64_t my_a = cta_start(cta), my_e = cta_start(cta + 1);
+  const uint32_t share = total_steps / act, extra = total_steps - share * act;
+  auto cta_start = [&](uint32_t c) -> uint32_t { return share * c + min(c, extra); };
+  const uint32_t my_a = cta_start(cta), my_e = cta_start(cta + 1);
+  const int n_mine = static_cast<int>(my_e - my_a);
+  Cursor first;
+  first.kvh = static_cast<int>(my_a / n_steps);
+  first.j0 = static_cast<int>(my_a - static_cast<uint32_t>(first.kvh) * n_steps);
+  first.tile = last_le(s_sfirst, n_tiles, first.j0);
+  first.j0 -= s_sfirst[first.tile];
+  first.left = n_mine;
   const uint32_t s_base = smem_u32(smem);
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_q + i, 1);
-      mbar_init(bar_qfree + i, 1);
-      mbar_init(bar_qread + i, 4);
       mbar_init(bar_s + i, 1);
       mbar_init(bar_p + i, 128);
       mbar_init(bar_pv + i, 1);
     }
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(bar_k + i, 1);
+    for (int i = 0; i < kKStages; ++i) {
+      mbar_init(bar_k + i, 2);
+      mbar_init(bar_kfree + i, 1);
+    }
+    for (int i = 0; i < kVStages; ++i) {
       mbar_init(bar_v + i, 1);
-      mbar_init(bar_kfree + i, 4);
       mbar_init(bar_vfree + i, 1);
     }
+    mbar_init(bar_drain, 1);
     fence_barrier_init();
   }
   if (warp == 0) {
@@ -314,245 +372,276 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp >= 4) {
     reg_dec<88>();
-    // roles of warps 4-7: Q loads + Q K^T, P V, decode K, decode V
-    const int role = (warp - 4) ^ (cta >= (static_cast<int>(gridDim.x) + 1) / 2 ? 2 : 0);
+    // roles of warps 4-7: issue, decode K rows 0-31, decode V, decode K rows 32-63
+    const int role = (warp - 4 + (cta >= (gridDim.x + 1) / 2 ? 1 : 0)) & 3;
     if (role == 0) {
       if (lane == 0) {
-        const uint32_t idesc = umma_idesc_f16(Elem<T>::code == PSB_BF16 ? 1 : 0, kRows, kBN, 0, 0);
+        const uint32_t idesc_s = umma_idesc_f16(Elem<T>::code == PSB_BF16 ? 1 : 0, kRows, kBN, 0, 0);
+        const uint32_t idesc_o = umma_idesc_f16(0, kRows, kDim, 0, 1);
         const uint64_t dq = umma_desc_sw128(s_base, 1024, 16);
         const uint64_t dk = umma_desc_sw128(s_base + kOffK, 1024, 16);
+        const uint64_t dv = umma_desc_sw128(s_base + kOffV, 1024, 8192);
         prefetch_tmap(&tm_q);
-        Cursor qc(plan, my_a, my_e), cc(plan, my_a, my_e);
-        int q_req = 0, q_seen = 0, g = 0;
+        Cursor qc = first, sc = first, oc = first;  // Q loads, S and O
+        int q_req = 0, q_seen = 0;
         auto load_q = [&]() {  // the next run's rows into buffer q_req & 1
-          const Seg s = qc.take();
+          const Run s = qc.take(plan);
           const int b = q_req & 1;
           mbar_arrive_expect_tx(bar_q + b, static_cast<uint32_t>(TQ * group) * kDim * 2);
           tma_load_3d(smem + b * kQTile, &tm_q, 0, s.kvh * group, plan.q0[s.seq] + s.qt * TQ, bar_q + b);
           ++q_req;
         };
-        load_q();
-        if (qc.more()) load_q();
-        for (int k = 0; cc.more() && !fail; ++k) {
-          const Seg s = cc.take();
-          const int b = k & 1;
-          if (!mbar_wait(bar_q + b, (k >> 1) & 1)) {
-            fail = true;
-            break;
-          }
-          ++q_seen;
-          const uint64_t dqs = dq + static_cast<uint64_t>(b * (kQTile >> 4));
-          for (int j = 0; j < s.n; ++j, ++g) {
-            const int st = g % kStages;
-            // S buffer g & 1 held S and then P of step g - 2
-            if ((g >= 2 && !mbar_wait(bar_pv + (g & 1), ((g - 2) >> 1) & 1)) ||
-                !mbar_wait(bar_k + st, (g / kStages) & 1)) {
-              fail = true;
-              break;
-            }
-            tc_fence_after();
-            const uint64_t dks = dk + static_cast<uint64_t>(st * (kKvTile >> 4));
-#pragma unroll
-            for (int kk = 0; kk < kDim / 16; ++kk)
-              umma_f16_ss(tmem + kSCol + (g & 1) * kBN, dqs + 2 * kk, dks + 2 * kk, idesc, kk > 0);
-            umma_commit(bar_s + (g & 1));
-          }
-          if (fail) break;
-          umma_commit(bar_qfree + b);
-          if (qc.more()) {  // run k + 2 goes into this buffer
-            if (!mbar_wait(bar_qfree + b, (k >> 1) & 1) || !mbar_wait(bar_qread + b, (k >> 1) & 1)) {
-              fail = true;
-              break;
-            }
+        int s_left = 0, o_left = 0, o_run = -1;
+        bool want_q = true;
+#pragma unroll 1
+        for (int g = 0; g <= n_mine; ++g) {
+          while (want_q && qc.left > 0) {  // the first two runs, then one after each run's end
             load_q();
+            want_q = q_req < 2;
           }
-        }
-        if (fail) {
-          flag_error(p.err, PSB_DEVERR_TIMEOUT);
-          for (int t = q_seen; t < q_req; ++t) (void)mbar_wait(bar_q + (t & 1), (t >> 1) & 1);
-        }
-      }
-    } else if (role == 1) {
-      if (lane == 0) {
-        const uint32_t idesc = umma_idesc_f16(0, kRows, kDim, 0, 1);
-        const uint64_t dv = umma_desc_sw128(s_base + kOffV, 1024, 8192);
-        Cursor cc(plan, my_a, my_e);
-        int g = 0, issued = 0;
-        for (int k = 0; cc.more() && !fail; ++k) {
-          const Seg s = cc.take();
-          const uint32_t obuf = tmem + kOCol + (k & 1) * kDim;
-          for (int j = 0; j < s.n; ++j, ++g) {
-            const int st = g % kStages;
-            if (!mbar_wait(bar_p + (g & 1), (g >> 1) & 1) || !mbar_wait(bar_v + st, (g / kStages) & 1)) {
+          want_q = false;
+          if (g < n_mine) {  // S of step g
+            if (s_left == 0) {
+              s_left = sc.take(plan).n;
+              if (!wait(bar_q + (q_seen & 1), (q_seen >> 1) & 1)) {
+                fail = true;
+                break;
+              }
+              ++q_seen;
+            }
+            const int st = g % kKStages;
+            // S buffer g & 1 held S and then P of step g - 2
+            if ((g >= 2 && !wait(bar_pv + (g & 1), ((g - 2) >> 1) & 1)) || !wait(bar_k + st, (g / kKStages) & 1)) {
               fail = true;
               break;
             }
             tc_fence_after();
+            const uint64_t dqs = dq + static_cast<uint64_t>(((q_seen - 1) & 1) * (kQTile >> 4));
+            const uint64_t dks = dk + static_cast<uint64_t>(st * (2 * kKvTile >> 4));
+#pragma unroll
+            for (int kk = 0; kk < 2 * kDim / 16; ++kk)  // the values rounded to T, then their rests
+              umma_f16_ss(tmem + kSCol + (g & 1) * kBN, dqs + 2 * (kk & 3), dks + (kk >> 2) * (kKvTile >> 4) + 2 * (kk & 3),
+                          idesc_s, kk > 0);
+            umma_commit(bar_s + (g & 1));
+            umma_commit(bar_kfree + st);
+            --s_left;
+          }
+          if (g > 0) {  // P V of step g - 1
+            const int h = g - 1, st = h % kVStages;
+            const bool begins = o_left == 0;
+            if (begins) {
+              o_left = oc.take(plan).n;
+              ++o_run;
+            }
+            if (!wait(bar_p + (h & 1), (h >> 1) & 1) || !wait(bar_v + st, (h / kVStages) & 1)) {
+              fail = true;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t obuf = tmem + kOCol + (o_run & 1) * kDim;
             const uint64_t dvs = dv + static_cast<uint64_t>(st * (kKvTile >> 4));
-            const uint32_t pcol = tmem + kSCol + (g & 1) * kBN;
+            const uint32_t pcol = tmem + kSCol + (h & 1) * kBN;
 #pragma unroll
             for (int kk = 0; kk < kBN / 16; ++kk)
-              umma_f16_ts(obuf, pcol + 8 * kk, dvs + 128 * kk, idesc, j > 0 || kk > 0);
-            umma_commit(bar_pv + (g & 1));
+              umma_f16_ts(obuf, pcol + 8 * kk, dvs + 128 * kk, idesc_o, !begins || kk > 0);
+            umma_commit(bar_pv + (h & 1));
             umma_commit(bar_vfree + st);
-            ++issued;
+            // at a run's end the softmax has read its last S: its Q may be overwritten
+            want_q = --o_left == 0;
           }
         }
         if (fail) {
           flag_error(p.err, PSB_DEVERR_TIMEOUT);
-          // let the products in flight land before shared memory and TMEM are released
-          if (issued > 0) (void)mbar_wait(bar_pv + ((issued - 1) & 1), ((issued - 1) >> 1) & 1);
+          // let the copies and products in flight land before shared memory and TMEM are released
+          for (int t = q_seen; t < q_req; ++t) (void)wait(bar_q + (t & 1), (t >> 1) & 1);
+          umma_commit(bar_drain);
+          (void)wait(bar_drain, 0);
         }
       }
     } else {
-      // ---- decode: lane l of a warp takes rows l and l + 32 of a step's 64 keys ----
-      const bool is_v = role == 3;
-      const uint32_t ring = s_base + (is_v ? kOffV : kOffK);
-      uint64_t* const bar_full = is_v ? bar_v : bar_k;
-      uint64_t* const bar_free = is_v ? bar_vfree : bar_kfree;
-      Cursor cc(plan, my_a, my_e);
-      Seg seg{};
-      int j = 0, left = 0;  // next step to look up: step j of seg, left of them
+      // ---- decode: lane l of a K warp takes one row of a step's 64 keys, of the V warp rows l and l + 32 ----
+      // The block id of a row is looked up two steps, its codes are loaded one
+      // step ahead of their decoding.
+      Cursor cc = first;
+      int left = 0, pos0 = 0, ctx = 0;  // of the run being looked up: steps left, first key of the next, tokens
       const int32_t* row = nullptr;
-      int ctx = 0;
-      // The pipeline of a lane's two rows: block ids of one step ahead of the
-      // codes' loads, those one step ahead of their decoding.
-      struct Rows {
-        uint4 c[2][2];
-        uint32_t par[2];
-        uint32_t flags;  // bits 0, 1: row's block is outside the pool; 2: first step of a run; 3: there is a step
+      int64_t tile0 = 0;
+      auto next_run = [&]() {
+        const Run s = cc.take(plan);
+        pos0 = s.j0 * kBN;
+        left = s.n;
+        row = p.tables + static_cast<int64_t>(s.seq) * p.table_stride;
+        ctx = plan.ctx[s.seq];
+        tile0 = p.layer_tiles + s.kvh;
       };
-      int64_t at[2] = {-1, -1};  // pool rows of the step after next, -1: nothing to read
-      uint32_t at_flags = 0;
-      auto look = [&]() {
-        at[0] = at[1] = -1;
-        at_flags = 0;
-        if (left == 0) {
-          if (!cc.more()) return;
-          seg = cc.take();
-          j = seg.j0;
-          left = seg.n;
-          row = p.tables + static_cast<int64_t>(seg.seq) * p.table_stride;
-          ctx = plan.ctx[seg.seq];
-          at_flags = 4;
-        }
-        at_flags |= 8;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t pos = j * kBN + lane + 32 * i;
-          if (static_cast<int>(pos) >= ctx) continue;
-          const uint32_t bi = static_cast<uint32_t>((static_cast<uint64_t>(pos) * tp.block_div) >> 32);
-          const int blk = __ldg(row + bi);
-          if (blk < 0 || blk >= p.num_blocks) {
-            at_flags |= 1u << i;
-          } else {
-            at[i] = int4_row(p.layer_tiles + static_cast<int64_t>(blk) * p.hkv + seg.kvh, is_v ? 1 : 0,
-                             static_cast<int>(pos - bi * p.block_size), p.block_size);
-          }
-        }
-        ++j;
-        --left;
+      // row r's place in the pool (-1: past the sequence, -2: its block is outside the pool)
+      auto place = [&](int r, int kv) -> int64_t {
+        const uint32_t pos = pos0 + r;
+        if (static_cast<int>(pos) >= ctx) return -1;
+        const uint32_t bi = static_cast<uint32_t>((static_cast<uint64_t>(pos) * tp.block_div) >> 32);
+        const int blk = __ldg(row + bi);
+        if (blk < 0 || blk >= p.num_blocks) return -2;
+        return int4_row(tile0 + static_cast<int64_t>(blk) * p.hkv, kv, static_cast<int>(pos - bi * p.block_size),
+                        p.block_size);
       };
-      auto load = [&](Rows& r) {
-        r.flags = at_flags;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          r.c[i][0] = r.c[i][1] = make_uint4(0, 0, 0, 0);
-          r.par[i] = 0;
-          if (at[i] >= 0) {
-            const uint4* src = reinterpret_cast<const uint4*>(p.codes + at[i] * (kDim / 2));
-            r.c[i][0] = __ldg(src);
-            r.c[i][1] = __ldg(src + 1);
-            r.par[i] = __ldg(reinterpret_cast<const uint32_t*>(p.params) + at[i]);
-          }
+      struct Row {
+        uint4 c[2];
+        uint32_t par;
+      };
+      auto load = [&](Row& r, int64_t at) {
+        r.c[0] = r.c[1] = make_uint4(0, 0, 0, 0);
+        r.par = 0;
+        if (at >= 0) {
+          const uint4* src = reinterpret_cast<const uint4*>(p.codes + at * (kDim / 2));
+          r.c[0] = __ldg(src);
+          r.c[1] = __ldg(src + 1);
+          r.par = __ldg(reinterpret_cast<const uint32_t*>(p.params) + at);
         }
       };
-      Rows cur, nxt;
-      look();
-      load(nxt);
-      look();
-      int vexp = 0;
-      float vlim = 0.f, vscale = 1.f;
-      for (int g = 0; (nxt.flags & 8) && !fail; ++g) {
-        cur = nxt;
-        load(nxt);
-        look();
-        const int st = g % kStages;
-        if (g >= kStages && !warp_ok(mbar_wait(bar_free + st, (g / kStages - 1) & 1))) {
-          fail = true;
-          break;
-        }
-        Factors& f = fac[st];
-        const uint32_t tile = ring + st * kKvTile;
-        const float2 p0 = unpack2<T>(cur.par[0]), p1 = unpack2<T>(cur.par[1]);
-        if (!is_v) {
-          // 128 + c (bf16) or 1024 + c (f16), elements in order
-          constexpr float kOff = Elem<T>::code == PSB_BF16 ? 135.5f : 1031.5f;
-          constexpr uint32_t kHigh = Elem<T>::code == PSB_BF16 ? 0x43434343u : 0x64646464u;
-          const float sc = p.scale_log2;
-          f.ks[lane] = p0.x * sc;
-          f.ks[lane + 32] = p1.x * sc;
-          f.km[lane] = fmaf(p0.x, -kOff, p0.y) * sc;
-          f.km[lane + 32] = fmaf(p1.x, -kOff, p1.y) * sc;
-          const uint32_t bad0 = __ballot_sync(0xffffffffu, cur.flags & 1), bad1 = __ballot_sync(0xffffffffu, cur.flags & 2);
-          if (lane == 0) {
-            f.bad[0] = bad0;
-            f.bad[1] = bad1;
-            if (bad0 | bad1) flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
+      if (role != 2) {
+        const int r = lane + (role == 3 ? 32 : 0);
+        const uint32_t dst = s_base + kOffK + r * 128;
+        Row cur, nxt{};
+        int64_t at = -1;
+#pragma unroll 1
+        for (int i = 0; i < n_mine + 2; ++i) {
+          cur = nxt;
+          load(nxt, at);
+          at = -1;
+          if (i < n_mine) {
+            if (left == 0) next_run();
+            at = place(r, 0);
+            pos0 += kBN;
+            --left;
           }
+          const int g = i - 2;
+          if (g < 0) continue;
+          const int st = g % kKStages;
+          if (g >= kKStages && !warp_wait(bar_kfree + st, (g / kKStages - 1) & 1)) {
+            fail = true;
+            break;
+          }
+          // value = step (c - 8) + (mid + step / 2); its rounding to T and the rest
+          const float2 pr = unpack2<T>(cur.par);
+          const float base = fmaf(pr.x, 0.5f, pr.y);
+          const uint64_t st2 = f2_pack(pr.x, pr.x), base2 = f2_pack(base, base), minus = f2_pack(-1.f, -1.f);
+          const uint64_t off2 = f2_pack(-8388616.f, -8388616.f);  // - (2^23 + 8)
+          const uint32_t tile = dst + st * 2 * kKvTile;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            const uint4 q = h == 0 ? cur.c[0] : cur.c[1];
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int r = lane + 32 * i;
-            const uint32_t* w = &cur.c[i][0].x;
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t t = w[c] & 0x0f0f0f0fu, u = (w[c] >> 4) & 0x0f0f0f0fu;
+              uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const uint32_t x = w[c], t = x & 0x0f0f0f0fu, u = (x >> 4) & 0x0f0f0f0fu;
-              const uint32_t m0 = __byte_perm(t, u, 0x5140), m1 = __byte_perm(t, u, 0x7362);
-              st_shared_v4(tile + r * 128 + ((c ^ (r & 7)) << 4), __byte_perm(m0, kHigh, 0x4140),
-                           __byte_perm(m0, kHigh, 0x4342), __byte_perm(m1, kHigh, 0x4140),
-                           __byte_perm(m1, kHigh, 0x4342));
+              for (int e = 0; e < 4; ++e) {  // elements 2 e and 2 e + 1 of the word: 2^23 + c
+                const uint64_t cc2 = f2_pack(__uint_as_float(__byte_perm(t, 0x4b000000u, 0x7440 | e)),
+                                             __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 | e)));
+                const uint64_t v = f2_fma(f2_add(cc2, off2), st2, base2);
+                const float2 vf = f2_unpack(v);
+                hi[e] = pack2_sat<T>(vf.x, vf.y);
+                const float2 hf = unpack2<T>(hi[e]);
+                const float2 rest = f2_unpack(f2_fma(f2_pack(hf.x, hf.y), minus, v));
+                lo[e] = pack2<T>(rest.x, rest.y);
+              }
+              const uint32_t to = tile + (((4 * h + c) ^ (r & 7)) << 4);
+              st_shared_v4(to, hi[0], hi[1], hi[2], hi[3]);
+              st_shared_v4(to + kKvTile, lo[0], lo[1], lo[2], lo[3]);
             }
           }
-        } else {
-          if (cur.flags & 4) {  // a run's first step
+          fence_proxy_async_smem();  // visible to the tensor core
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_k + st);
+        }
+      } else {
+        Row cur0, cur1, nxt0{}, nxt1{};
+        int64_t at0 = -1, at1 = -1;
+        uint32_t f_cur = 0, f_nxt = 0, f_at = 0;  // bits 0, 1: the row's block is outside the pool; 2: a run's first step
+        int vexp = 0;
+        float vlim = 0.f, vscale = 1.f;
+#pragma unroll 1
+        for (int i = 0; i < n_mine + 2; ++i) {
+          cur0 = nxt0;
+          cur1 = nxt1;
+          f_cur = f_nxt;
+          load(nxt0, at0);
+          load(nxt1, at1);
+          f_nxt = f_at;
+          at0 = at1 = -1;
+          f_at = 0;
+          if (i < n_mine) {
+            if (left == 0) {
+              next_run();
+              f_at = 4;
+            }
+            at0 = place(lane, 1);
+            at1 = place(lane + 32, 1);
+            f_at |= (at0 == -2 ? 1u : 0u) | (at1 == -2 ? 2u : 0u);
+            pos0 += kBN;
+            --left;
+          }
+          const int g = i - 2;
+          if (g < 0) continue;
+          const int st = g % kVStages;
+          if (g >= kVStages && !warp_wait(bar_vfree + st, (g / kVStages - 1) & 1)) {
+            fail = true;
+            break;
+          }
+          Extra& x = ext[st];
+          const float2 p0 = unpack2<T>(cur0.par), p1 = unpack2<T>(cur1.par);
+          if (f_cur & 4) {
             vlim = 0.f;
             vexp = 0;
             vscale = 1.f;
           }
           if (__any_sync(0xffffffffu, fmaxf(p0.x, p1.x) > vlim)) {
             float top = fmaxf(p0.x, p1.x);
-#pragma unroll
+#pragma unroll 1
             for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             vexp = max(-100, ilogb_f32(top)) + 1;  // top < 2^vexp
             vlim = exp2_int(min(vexp, 127));
-            vscale = exp2_int(kPBits - vexp);
+            vscale = exp2_int(kStepBits - vexp);
           }
-          f.vs[lane] = p0.x * vscale;
-          f.vs[lane + 32] = p1.x * vscale;
-          f.vm[lane] = p0.y;
-          f.vm[lane + 32] = p1.y;
-          if (lane == 0) f.vexp = vexp;
-          // (c - 7.5) 2^-9 in f16: the nibble pairs (i, i + 4) are the subnormals
-          // c 2^-24 (even i) and c 2^-20 (odd i); element 8 w + i + 4 h of a row
-          // sits at 8 w + 2 i + h
+          const bool fin0 = finite_f32(p0.y), fin1 = finite_f32(p1.y);
+          x.mid[lane] = fin0 ? p0.y : 0.f;
+          x.mid[lane + 32] = fin1 ? p1.y : 0.f;
+          const uint32_t bad0 = __ballot_sync(0xffffffffu, f_cur & 1), bad1 = __ballot_sync(0xffffffffu, f_cur & 2);
+          const uint32_t nan0 = __ballot_sync(0xffffffffu, !fin0), nan1 = __ballot_sync(0xffffffffu, !fin1);
+          if (lane == 0) {
+            x.bad[0] = bad0;
+            x.bad[1] = bad1;
+            x.nan[0] = nan0;
+            x.nan[1] = nan1;
+            x.vexp = vexp;
+            if (bad0 | bad1) flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
+          }
+          // step (c - 7.5) in f16: the nibble pairs (i, i + 4) are the subnormals
+          // c 2^-24 (even i) and c 2^-20 (odd i), which one exact fma turns into
+          // (c - 7.5) 2^-9; element 8 w + i + 4 h of a row sits at 8 w + 2 i + h
+          const uint32_t tile = s_base + kOffV + st * kKvTile + lane * 128;
+#pragma unroll 1
+          for (int h = 0; h < 4; ++h) {  // row h / 2, half h & 1
+            const uint4 q = h == 0 ? cur0.c[0] : h == 1 ? cur0.c[1] : h == 2 ? cur1.c[0] : cur1.c[1];
+            const float stf = (h < 2 ? p0.x : p1.x) * vscale;
+            const uint32_t st2 = pack2<__half>(stf, stf);
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int r = lane + 32 * i;
-            const uint32_t* w = &cur.c[i][0].x;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const uint32_t x = w[c], y = x >> 8;
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t a = w[c], b = a >> 8;
               // 2^15, 2^11 and - 7.5 / 512 as f16 pairs
-              st_shared_v4(tile + r * 128 + ((c ^ (r & 7)) << 4), hfma2(x & 0x000f000fu, 0x78007800u, 0xa380a380u),
-                           hfma2(x & 0x00f000f0u, 0x68006800u, 0xa380a380u),
-                           hfma2(y & 0x000f000fu, 0x78007800u, 0xa380a380u),
-                           hfma2(y & 0x00f000f0u, 0x68006800u, 0xa380a380u));
+              st_shared_v4(tile + (h >> 1) * (32 * 128) + (((4 * (h & 1) + c) ^ (lane & 7)) << 4),
+                           hmul2(hfma2(a & 0x000f000fu, 0x78007800u, 0xa380a380u), st2),
+                           hmul2(hfma2(a & 0x00f000f0u, 0x68006800u, 0xa380a380u), st2),
+                           hmul2(hfma2(b & 0x000f000fu, 0x78007800u, 0xa380a380u), st2),
+                           hmul2(hfma2(b & 0x00f000f0u, 0x68006800u, 0xa380a380u), st2));
             }
           }
+          fence_proxy_async_smem();  // visible to the tensor core
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_v + st);
         }
-        fence_proxy_async_smem();  // visible to the tensor core
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_full + st);
       }
       if (fail && lane == 0) flag_error(p.err, PSB_DEVERR_TIMEOUT);
     }
@@ -563,125 +652,71 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int rtok = row / group, rhead = row - rtok * group;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(warp * 32) << 16);
     const bool out16 = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ost % 8 == 0 && p.osh % 8 == 0;
-    // a run's output is written after the next run's first step (or at the
-    // end): by then its last P V is normally done
-    int pend_k = -1, pend_exp = 0;
+    Cursor cc = first;
+    Run s{};
+    int left = 0, k = -1;          // steps left of run s, its number
+    int last = -1;                 // last key of this row; rows past the tile's tokens see none
+    uint32_t t_o = 0;
+    float ref = 0.f, l = 0.f, z = 0.f;  // the exponents' reference; sums of 2^kPBits p and 2^kPBits p mid
+    bool fresh = true;
+    int vexp = 0;
+    // A run's output is written after the next run's first step (or at the
+    // end): by then its last P V is normally done.
+    bool pending = false;
+    int pend_exp = 0;
     float pend_l = 0.f, pend_z = 0.f, pend_m = 0.f;
-    Seg pend{};
-    auto write_pending = [&](int pg) -> bool {
-      if (!warp_ok(mbar_wait(bar_pv + (pg & 1), (pg >> 1) & 1))) return false;
-      tc_fence_after();
-      const uint32_t t_po = t_lane + kOCol + (pend_k & 1) * kDim;
-      const bool whole = pend.j0 == 0 && pend.n == pend.n_kv;
-      const int tok = pend.qt * TQ + rtok;
-      const bool live = rtok < TQ && tok < plan.len[pend.seq];
-      const float back = exp2_int(max(-126, min(127, pend_exp - kPBits))) * kVBack;  // of one unit of O
-      const float inv = !whole ? 1.f : pend_l == 0.f ? 0.f : 1.f / pend_l;
-      const float scale = back * inv, base = pend_z * inv;
-      float* const dst = part + static_cast<int64_t>(2 * cta + (pend.j0 > 0 ? 0 : 1)) * kPartFloats;
-      T* const out = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(plan.q0[pend.seq] + tok) * p.ost +
-                     static_cast<int64_t>(pend.kvh * group + rhead) * p.osh;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t ot[32];
-        tmem_ld32(t_po + 32 * h, ot);
-        tmem_wait_ld();
-        float o[32];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {  // columns 2 i, 2 i + 1 of a word are its elements i, i + 4
-            o[8 * w + i] = fmaf(__uint_as_float(ot[8 * w + 2 * i]), scale, base);
-            o[8 * w + i + 4] = fmaf(__uint_as_float(ot[8 * w + 2 * i + 1]), scale, base);
-          }
+    Run pend{};
+#pragma unroll 1
+    for (int g = 0;; ++g) {
+      if (left == 0) {
+        if (g > 0) {
+          pending = true;
+          pend = s;
+          pend_l = l;
+          pend_z = z;
+          pend_exp = vexp;
+          pend_m = fresh ? -INFINITY : ref;
         }
-        if (!whole) {
-          if (live)
-#pragma unroll
-            for (int d = 0; d < 32; d += 4)
-              *reinterpret_cast<float4*>(dst + row * kDim + 32 * h + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-        } else if (live) {
-          if (out16) {
-#pragma unroll
-            for (int d = 0; d < 32; d += 8)
-              *reinterpret_cast<uint4*>(out + 32 * h + d) = make_uint4(pack2<T>(o[d], o[d + 1]), pack2<T>(o[d + 2], o[d + 3]),
-                                                                       pack2<T>(o[d + 4], o[d + 5]), pack2<T>(o[d + 6], o[d + 7]));
-          } else {
-#pragma unroll
-            for (int d = 0; d < 32; ++d) out[32 * h + d] = Elem<T>::from_float(o[d]);
-          }
+        if (g < n_mine) {
+          s = cc.take(plan);
+          left = s.n;
+          ++k;
+          const int tok = s.qt * TQ + rtok, len = plan.len[s.seq];
+          last = rtok < TQ && tok < len ? plan.ctx[s.seq] - len + tok - s.j0 * kBN : -1;  // of the run's first step
+          t_o = t_lane + kOCol + (k & 1) * kDim;
+          ref = l = z = 0.f;
+          fresh = true;
+          vexp = 0;
         }
       }
-      if (!whole) *reinterpret_cast<float2*>(dst + kRows * kDim + 2 * row) = make_float2(pend_m, pend_l);
-      tc_fence_before();
-      pend_k = -1;
-      return true;
-    };
-    Cursor cc(plan, my_a, my_e);
-    int g = 0;
-    for (int k = 0; cc.more() && !fail; ++k) {
-      const Seg s = cc.take();
-      const int ctx = plan.ctx[s.seq], start = ctx - plan.len[s.seq];
-      const int tok = s.qt * TQ + rtok;
-      // last key of this row; rows past the tile's tokens see none
-      const int last = rtok < TQ && tok < plan.len[s.seq] ? start + tok : -1;
-      const uint32_t t_o = t_lane + kOCol + (k & 1) * kDim;
-      // sum of the row's q
-      if (!warp_ok(mbar_wait(bar_q + (k & 1), (k >> 1) & 1))) {
-        fail = true;
-        break;
-      }
-      float qsum = 0.f;
-      {
-        const uint32_t qrow = s_base + (k & 1) * kQTile + row * 128;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint4 v = ld_shared_v4(qrow + (((c + lane) & 7) << 4));
-          const float2 a = unpack2<T>(v.x), b = unpack2<T>(v.y), d = unpack2<T>(v.z), e = unpack2<T>(v.w);
-          qsum += ((a.x + a.y) + (b.x + b.y)) + ((d.x + d.y) + (e.x + e.y));
+      if (g < n_mine) {
+        const int st = g % kVStages;
+        if (!warp_wait(bar_s + (g & 1), (g >> 1) & 1) || !warp_wait(bar_v + st, (g / kVStages) & 1)) {
+          fail = true;
+          break;
         }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_qread + (k & 1));
-      float ref = 0.f, l = 0.f, z = 0.f;  // the exponents' reference; sums of p and p mid
-      bool fresh = true;
-      int vexp = 0;
-      auto step = [&](int i) -> bool {
-        const int st = g % kStages;
-        const uint32_t ph = (g / kStages) & 1;
-        if (!warp_ok(mbar_wait(bar_s + (g & 1), (g >> 1) & 1) && mbar_wait(bar_k + st, ph) && mbar_wait(bar_v + st, ph)))
-          return false;
         tc_fence_after();
-        const Factors& f = fac[st];
+        const Extra& f = ext[st];
         uint32_t sr[kBN];
         tmem_ld32(t_lane + kSCol + (g & 1) * kBN, sr);
         tmem_ld32(t_lane + kSCol + (g & 1) * kBN + 32, sr + 32);
         tmem_wait_ld();
-        // scores minus reference
-        const uint64_t qs2 = f2_pack(qsum, qsum), nref2 = f2_pack(-ref, -ref);
+        // exponents: scores minus reference, plus kPBits
+        const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), nref2 = f2_pack(kPBits - ref, kPBits - ref);
 #pragma unroll
-        for (int c = 0; c < kBN; c += 4) {
-          const float4 ks = ld_shared_f4(f.ks + c), km = ld_shared_f4(f.km + c);
-          const float2 a = f2_unpack(f2_fma(f2_pack(ks.x, ks.y), f2_pack(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])),
-                                            f2_fma(f2_pack(km.x, km.y), qs2, nref2)));
-          const float2 b = f2_unpack(f2_fma(f2_pack(ks.z, ks.w), f2_pack(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])),
-                                            f2_fma(f2_pack(km.z, km.w), qs2, nref2)));
+        for (int c = 0; c < kBN; c += 2) {
+          const float2 a = f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, nref2));
           sr[c] = __float_as_uint(a.x);
           sr[c + 1] = __float_as_uint(a.y);
-          sr[c + 2] = __float_as_uint(b.x);
-          sr[c + 3] = __float_as_uint(b.y);
         }
-        const int lim = last - (s.j0 + i) * kBN;  // last valid column
-        if (lim < kBN - 1) {
+        // bit c: the row sees key c of the step
+        const uint32_t seen0 = last >= 31 ? ~0u : last < 0 ? 0u : (2u << last) - 1;
+        const uint32_t seen1 = last >= 63 ? ~0u : last < 32 ? 0u : (2u << (last - 32)) - 1;
+        const uint32_t ok0 = seen0 & ~f.bad[0], ok1 = seen1 & ~f.bad[1];
+        if ((ok0 & ok1) != ~0u) {
 #pragma unroll
           for (int c = 0; c < kBN; ++c)
-            if (c > lim) sr[c] = __float_as_uint(-INFINITY);
-        }
-        const uint32_t bad0 = f.bad[0], bad1 = f.bad[1];
-        if (bad0 | bad1) {
-#pragma unroll
-          for (int c = 0; c < kBN; ++c)
-            if ((c < 32 ? bad0 : bad1) >> (c & 31) & 1) sr[c] = __float_as_uint(-INFINITY);
+            if (!((c < 32 ? ok0 : ok1) >> (c & 31) & 1)) sr[c] = __float_as_uint(-INFINITY);
         }
         float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
@@ -692,24 +727,28 @@ __global__ void __launch_bounds__(kThreads, 2)
         const float mx = fmaxf(mx0, mx1);
         // A row's reference moves when a score is above it by more than the
         // limit, or at its first score; O is rescaled then, or when the scale
-        // of p step changed.  The warp's TMEM access is collective.
+        // of V's steps changed.  The warp's TMEM access is collective.
         const int ve = f.vexp;
-        const bool grow = mx > (fresh ? -INFINITY : kGrowth);
-        if (__any_sync(0xffffffffu, grow) || (i > 0 && ve != vexp)) {
-          const float up = grow ? fminf(fmaxf(mx, -3e38f), 3e38f) : 0.f;
+        const bool begins = left == s.n;
+        const bool grow = mx > (fresh ? -INFINITY : kGrowth + kPBits);
+        if (__any_sync(0xffffffffu, grow) || (!begins && ve != vexp)) {
+          const float up = grow ? fminf(fmaxf(mx - kPBits, -3e38f), 3e38f) : 0.f;
           const float al = grow ? (fresh ? 0.f : ex2_approx(-up)) : 1.f;
-          if (i > 0) {  // O holds P V of the earlier steps once the last of them is done
-            if (!warp_ok(mbar_wait(bar_pv + ((g - 1) & 1), ((g - 1) >> 1) & 1))) return false;
+          if (!begins) {  // O holds P V of the earlier steps once the last of them is done
+            if (!warp_wait(bar_pv + ((g - 1) & 1), ((g - 1) >> 1) & 1)) {
+              fail = true;
+              break;
+            }
             tc_fence_after();
             const float ao = al * exp2_int(max(-126, vexp - ve));
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t ot[32];
-              tmem_ld32(t_o + 32 * h, ot);
+#pragma unroll 1
+            for (int h = 0; h < 4; ++h) {
+              uint32_t ot[16];
+              tmem_ld16(t_o + 16 * h, ot);
               tmem_wait_ld();
 #pragma unroll
-              for (int d = 0; d < 32; ++d) ot[d] = __float_as_uint(__uint_as_float(ot[d]) * ao);
-              tmem_st32(t_o + 32 * h, ot);
+              for (int d = 0; d < 16; ++d) ot[d] = __float_as_uint(__uint_as_float(ot[d]) * ao);
+              tmem_st16(t_o + 16 * h, ot);
             }
             tmem_wait_st();
           }
@@ -725,63 +764,92 @@ __global__ void __launch_bounds__(kThreads, 2)
         uint64_t l2 = f2_pack(0.f, 0.f), z2 = f2_pack(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < kBN; c += 4) {
-          const float4 vs = ld_shared_f4(f.vs + c), vm = ld_shared_f4(f.vm + c);
-          const uint64_t a = f2_pack(ex2_approx(__uint_as_float(sr[c])), ex2_approx(__uint_as_float(sr[c + 1])));
-          const uint64_t b = f2_pack(ex2_approx(__uint_as_float(sr[c + 2])), ex2_approx(__uint_as_float(sr[c + 3])));
+          const float4 vm = ld_shared_f4(f.mid + c);
+          const float a0 = ex2_approx(__uint_as_float(sr[c])), a1 = ex2_approx(__uint_as_float(sr[c + 1]));
+          const float b0 = ex2_approx(__uint_as_float(sr[c + 2])), b1 = ex2_approx(__uint_as_float(sr[c + 3]));
+          const uint64_t a = f2_pack(a0, a1), b = f2_pack(b0, b1);
           l2 = f2_add(l2, f2_add(a, b));
           z2 = f2_fma(a, f2_pack(vm.x, vm.y), z2);
           z2 = f2_fma(b, f2_pack(vm.z, vm.w), z2);
-          const float2 pa = f2_unpack(f2_mul(a, f2_pack(vs.x, vs.y))), pb = f2_unpack(f2_mul(b, f2_pack(vs.z, vs.w)));
-          pk[c / 2] = pack2<__half>(pa.x, pa.y);
-          pk[c / 2 + 1] = pack2<__half>(pb.x, pb.y);
+          pk[c / 2] = pack2<__half>(a0, a1);
+          pk[c / 2 + 1] = pack2<__half>(b0, b1);
         }
         const float2 lf = f2_unpack(l2), zf = f2_unpack(z2);
         l += lf.x + lf.y;
         z += zf.x + zf.y;
+        // a token that stands for NaN: for the rows that see it
+        if (((f.nan[0] & seen0) | (f.nan[1] & seen1)) != 0) z = __int_as_float(0x7fffffff);
         tmem_st32(t_lane + kSCol + (g & 1) * kBN, pk);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(bar_p + (g & 1));
-        __syncwarp();  // every lane has read the factors
-        if (lane == 0) mbar_arrive(bar_kfree + st);
-        return true;
-      };
-      if (!step(0) || (pend_k >= 0 && !write_pending(g - 1))) {
-        fail = true;
-        break;
       }
-      ++g;
-      for (int i = 1; i < s.n; ++i, ++g) {
-        if (!step(i)) {
+      if (pending) {
+        const int pg = min(g, n_mine) - 1;  // the run's last step
+        if (!warp_wait(bar_pv + (pg & 1), (pg >> 1) & 1)) {
           fail = true;
           break;
         }
+        tc_fence_after();
+        pending = false;
+        // run k is under way, or it is the one that has ended
+        const uint32_t t_po = t_lane + kOCol + ((g < n_mine ? k - 1 : k) & 1) * kDim;
+        const bool whole = pend.j0 == 0 && pend.n == pend.n_kv;
+        const int tok = pend.qt * TQ + rtok;
+        const bool live = rtok < TQ && tok < plan.len[pend.seq];
+        const float back = exp2_int(max(-126, min(127, pend_exp - kStepBits + kVBits)));  // of one unit of O
+        const float inv = !whole ? 1.f : pend_l == 0.f ? 0.f : 1.f / pend_l;
+        const float scale = back * inv, base = pend_z * inv;
+        float* const dst = part + static_cast<int64_t>(2 * cta + (pend.j0 > 0 ? 0 : 1)) * kPartFloats;
+        T* const out = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(plan.q0[pend.seq] + tok) * p.ost +
+                       static_cast<int64_t>(pend.kvh * group + rhead) * p.osh;
+#pragma unroll 1
+        for (int h = 0; h < 4; ++h) {
+          uint32_t ot[16];
+          tmem_ld16(t_po + 16 * h, ot);
+          tmem_wait_ld();
+          float o[16];
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // columns 2 i, 2 i + 1 of a word are its elements i, i + 4
+              o[8 * w + i] = fmaf(__uint_as_float(ot[8 * w + 2 * i]), scale, base);
+              o[8 * w + i + 4] = fmaf(__uint_as_float(ot[8 * w + 2 * i + 1]), scale, base);
+            }
+          }
+          if (live && !whole) {
+#pragma unroll
+            for (int d = 0; d < 16; d += 4)
+              *reinterpret_cast<float4*>(dst + row * kDim + 16 * h + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+          } else if (live && out16) {
+#pragma unroll
+            for (int d = 0; d < 16; d += 8)
+              *reinterpret_cast<uint4*>(out + 16 * h + d) = make_uint4(pack2<T>(o[d], o[d + 1]), pack2<T>(o[d + 2], o[d + 3]),
+                                                                       pack2<T>(o[d + 4], o[d + 5]), pack2<T>(o[d + 6], o[d + 7]));
+          } else if (live) {
+#pragma unroll
+            for (int d = 0; d < 16; ++d) out[16 * h + d] = Elem<T>::from_float(o[d]);
+          }
+          __syncwarp();  // the next read of TMEM is the whole warp's
+        }
+        if (!whole) *reinterpret_cast<float2*>(dst + kRows * kDim + 2 * row) = make_float2(pend_m, pend_l);
+        tc_fence_before();
       }
-      if (fail) break;
-      pend_k = k;
-      pend = s;
-      pend_l = l;
-      pend_z = z;
-      pend_exp = vexp;
-      pend_m = fresh ? -INFINITY : ref;
+      if (g >= n_mine) break;
+      --left;
+      last -= kBN;
     }
-    if (!fail && pend_k >= 0 && !write_pending(g - 1)) fail = true;
     if (fail && lane == 0) flag_error(p.err, PSB_DEVERR_TIMEOUT);
     if (warp == 0) {
-      // the tile that begins here and runs past the CTA's end, if any
+      // the tile that begins here and runs past the CTA's end, if any: the last run
       Cut c{0, 0, 0, 0};
-      const int64_t at = my_e - 1;
-      const int kvh = static_cast<int>(at / n_steps);
-      const int tile = last_le(s_sfirst, n_tiles, static_cast<int>(at - static_cast<int64_t>(kvh) * n_steps));
-      const int64_t t_a = static_cast<int64_t>(kvh) * n_steps + s_sfirst[tile];
-      const int64_t t_e = static_cast<int64_t>(kvh) * n_steps + s_sfirst[tile + 1];
-      if (t_a >= my_a && t_e > my_e) {
-        const int seq = last_le(s_tfirst, p.num_seqs, tile), first = (tile - s_tfirst[seq]) * TQ;
-        c.kvh = kvh;
-        c.row0 = s_q0[seq] + first;
-        c.tokens = min(TQ, s_len[seq] - first);
-        c.c1 = cta;
-        for (int c0 = cta + 1; c0 < act; c0 += 32) {  // CTAs that start before its end
+      const uint32_t t_a = my_e - static_cast<uint32_t>(s.j0 + s.n), t_e = t_a + static_cast<uint32_t>(s.n_kv);
+      if (!fail && s.j0 == 0 && t_e > my_e) {
+        c.kvh = s.kvh;
+        c.row0 = s_q0[s.seq] + s.qt * TQ;
+        c.tokens = min(TQ, s_len[s.seq] - s.qt * TQ);
+        c.c1 = static_cast<int32_t>(cta);
+        for (uint32_t c0 = cta + 1; c0 < act; c0 += 32) {  // CTAs that start before its end
           const bool in = c0 + lane < act && cta_start(min(c0 + lane, act)) < t_e;
           const int n = __popc(__ballot_sync(0xffffffffu, in));
           c.c1 += n;
@@ -870,7 +938,7 @@ __global__ void __launch_bounds__(kThreads) int4_prefill_combine_kernel(const Tc
 }
 
 size_t tc_smem(int num_seqs, int max_tiles) {
-  return 1024 + kOffTab + sizeof(int32_t) * (4 * static_cast<size_t>(num_seqs) + 1 + max_tiles + 1);
+  return 1024 + kOffTab + sizeof(int32_t) * (4 * static_cast<size_t>(num_seqs) + 1 + 2 * static_cast<size_t>(max_tiles) + 1);
 }
 
 int64_t tiles_bound(int total, int num_seqs, int tq) { return static_cast<int64_t>(total) / tq + num_seqs; }
@@ -883,7 +951,7 @@ bool int4_prefill_tc_geometry(int dtype, int total, int num_seqs, int q_heads, i
   if (!(dtype == PSB_BF16 || dtype == PSB_F16) || head_dim != kDim || group > kRows) return false;
   return num_seqs <= kMaxSeqs && tiles_bound(total, num_seqs, kRows / group) <= kMaxTiles &&
          static_cast<int64_t>(max_context + kBN) * block_size < (int64_t(1) << 32) &&
-         tiles_bound(total, num_seqs, kRows / group) * (max_context / kBN + 1) < (int64_t(1) << 31);
+         tiles_bound(total, num_seqs, kRows / group) * (max_context / kBN + 1) < (int64_t(1) << 31) / hkv;
 }
 
 size_t int4_prefill_tc_workspace() { return sizeof(Cut) * kMaxCtas + sizeof(float) * 2 * kMaxCtas * kPartFloats; }

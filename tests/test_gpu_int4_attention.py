@@ -351,3 +351,21 @@ def test_prefill_graph_and_second_stream():
         other = ops.paged_prefill_int4(*a)
     torch.cuda.synchronize()
     assert torch.equal(out, eager) and torch.equal(other, eager)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("which", [0, 1])
+def test_prefill_non_finite_rows_stay_behind_the_mask(which, dtype):
+    """A key or value stored as NaN reaches the rows that see its position and
+    no others, in its kv head alone."""
+    c = _prefill_case(35, [130, 70], [200, 70], 14, 2, 64, 16, dtype)
+    at = 150  # row 80 of the first sequence is the first that sees it
+    want, tol = _want_prefill(c)
+    c["pp"][c["layer"], c["table"][0, at // 16], 1, which, at % 16, 0] = 0.0
+    c["pp"][c["layer"], c["table"][0, at // 16], 1, which, at % 16, 1] = math.nan
+    got, err = _prefill(c)
+    assert err == 0
+    hit = torch.zeros(200, 14, dtype=torch.bool)
+    hit[80:130, 7:] = True
+    assert bool(torch.isnan(got[hit]).all())
+    _close(got[~hit], want[~hit], tol[~hit])

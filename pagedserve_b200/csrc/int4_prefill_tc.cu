@@ -41,6 +41,7 @@
 // alternate and step g + 2 needs step g's products.
 #include <algorithm>
 #include <atomic>
+#include <climits>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -224,7 +225,8 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
     int4_prefill_tc_kernel(const TcParams tp, const __grid_constant__ CUtensorMap tm_q) {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // (an offset, so that the compiler still knows it for shared memory)
+  uint8_t* const smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
   const Int4PrefillParams& p = tp.a;
   Extra* const ext = reinterpret_cast<Extra*>(smem + kOffX);
   uint64_t* const bar_q = reinterpret_cast<uint64_t*>(smem + kOffBars);  // [2] Q loaded
@@ -655,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     Cursor cc = first;
     Run s{};
     int left = 0, k = -1;          // steps left of run s, its number
-    int last = -1;                 // last key of this row; rows past the tile's tokens see none
+    int last = 0;                  // last key of this row, from the step's first
     uint32_t t_o = 0;
     float ref = 0.f, l = 0.f, z = 0.f;  // the exponents' reference; sums of 2^kPBits p and 2^kPBits p mid
     bool fresh = true;
@@ -682,7 +684,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           left = s.n;
           ++k;
           const int tok = s.qt * TQ + rtok, len = plan.len[s.seq];
-          last = rtok < TQ && tok < len ? plan.ctx[s.seq] - len + tok - s.j0 * kBN : -1;  // of the run's first step
+          // rows past the tile's tokens are not written: they need no mask
+          last = (rtok < TQ && tok < len ? plan.ctx[s.seq] - len + tok : INT_MAX) - s.j0 * kBN;
           t_o = t_lane + kOCol + (k & 1) * kDim;
           ref = l = z = 0.f;
           fresh = true;

@@ -5,13 +5,16 @@
 // Mathematics.  A row's values are mid + step (c - 7.5).  K goes to the tensor
 // cores as two operands of type T: each value rounded to T and what that
 // leaves out, rounded again (together 2^-17 of the value or less), so that S
-// needs nothing but the softmax's own scale.  V goes as f16 steps times codes:
-// step (c - 7.5) scaled by a power of two and rounded (2^-12), next to
-// probabilities rounded to f16 (2^-12); the mids, which no cancellation with
-// the codes may touch, are summed in fp32 beside the denominator.  The codes
-// could also stay bare with step and mid applied to S and P in fp32: that
-// reads four factors per key from shared memory in every softmax thread
-// (measured: 57% of the shared-memory cycles, no faster).
+// needs nothing but the softmax's own scale.  V is an f16 operand next to f16
+// probabilities, each rounded by 2^-12 at most: for bf16 step (c - 7.5), scaled
+// by a power of two; for f16, whose results show a second rounding of that
+// size (1.8 times the error of the attention over decoded rows), the bare
+// codes, which are exact, with the steps on the probabilities before their
+// rounding.  The mids, which no cancellation with the codes may touch, are
+// summed in fp32 beside the denominator.  K's codes could stay bare as well,
+// with step and mid applied to S: that reads four factors per key from shared
+// memory in every softmax thread (57% of the shared-memory cycles) and was no
+// faster.
 //
 // Tiles.  The q heads of a kv head read the same keys, so a tile's 128 rows
 // are TQ = 128 / group consecutive tokens times the group's heads (one TMA box
@@ -62,8 +65,13 @@ constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kSCol = 0, kOCol = 128;
 constexpr float kGrowth = 4.f;      // log2 of how far a score may exceed the exponents' reference
 constexpr int kPBits = 11;          // probabilities are 2^kPBits p, at most 2^(kPBits + kGrowth)
-constexpr int kStepBits = 15;       // V's steps are scaled to below 2^kStepBits
-constexpr int kVBits = 9;           // and its codes are (c - 7.5) 2^-kVBits
+constexpr int kVBits = 9;           // V's codes are (c - 7.5) 2^-kVBits
+// Where V's steps go, scaled to below 2^kStepBits: bf16, into V's operand;
+// f16, onto the probabilities (below 1, so that those stay below 2^15).
+template <typename T>
+constexpr bool kStepInV = Elem<T>::code == PSB_BF16;
+template <typename T>
+constexpr int kStepBits = kStepInV<T> ? 15 : 0;
 constexpr int kMaxCtas = 320;       // grid limit
 constexpr int kPartFloats = kRows * (kDim + 2);
 constexpr int kMaxSeqs = 2048, kMaxTiles = 8192;
@@ -71,9 +79,10 @@ constexpr int kMaxSeqs = 2048, kMaxTiles = 8192;
 // What a V stage's 64 tokens need besides their codes and steps.
 struct Extra {
   float mid[kBN];   // 0 where it is not finite
+  float step[kBN];  // scaled; f16 only
   uint32_t bad[2];  // bit t: token t's block is outside the pool
   uint32_t nan[2];  // bit t: token t's mid is not finite
-  int vexp;         // steps were scaled by 2^(kStepBits - vexp)
+  int vexp;         // steps were scaled by 2^(kStepBits<T> - vexp)
   int pad[3];
 };
 
@@ -604,11 +613,15 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             vexp = max(-100, ilogb_f32(top)) + 1;  // top < 2^vexp
             vlim = exp2_int(min(vexp, 127));
-            vscale = exp2_int(kStepBits - vexp);
+            vscale = exp2_int(max(-126, kStepBits<T> - vexp));
           }
           const bool fin0 = finite_f32(p0.y), fin1 = finite_f32(p1.y);
           x.mid[lane] = fin0 ? p0.y : 0.f;
           x.mid[lane + 32] = fin1 ? p1.y : 0.f;
+          if constexpr (!kStepInV<T>) {
+            x.step[lane] = p0.x * vscale;
+            x.step[lane + 32] = p1.x * vscale;
+          }
           const uint32_t bad0 = __ballot_sync(0xffffffffu, f_cur & 1), bad1 = __ballot_sync(0xffffffffu, f_cur & 2);
           const uint32_t nan0 = __ballot_sync(0xffffffffu, !fin0), nan1 = __ballot_sync(0xffffffffu, !fin1);
           if (lane == 0) {
@@ -619,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             x.vexp = vexp;
             if (bad0 | bad1) flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
           }
-          // step (c - 7.5) in f16: the nibble pairs (i, i + 4) are the subnormals
+          // codes in f16: the nibble pairs (i, i + 4) are the subnormals
           // c 2^-24 (even i) and c 2^-20 (odd i), which one exact fma turns into
           // (c - 7.5) 2^-9; element 8 w + i + 4 h of a row sits at 8 w + 2 i + h
           const uint32_t tile = s_base + kOffV + st * kKvTile + lane * 128;
@@ -628,16 +641,17 @@ __global__ void __launch_bounds__(kThreads, 2)
             const uint4 q = h == 0 ? cur0.c[0] : h == 1 ? cur0.c[1] : h == 2 ? cur1.c[0] : cur1.c[1];
             const float stf = (h < 2 ? p0.x : p1.x) * vscale;
             const uint32_t st2 = pack2<__half>(stf, stf);
+            auto scaled = [&](uint32_t v) { return kStepInV<T> ? hmul2(v, st2) : v; };
             const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const uint32_t a = w[c], b = a >> 8;
               // 2^15, 2^11 and - 7.5 / 512 as f16 pairs
               st_shared_v4(tile + (h >> 1) * (32 * 128) + (((4 * (h & 1) + c) ^ (lane & 7)) << 4),
-                           hmul2(hfma2(a & 0x000f000fu, 0x78007800u, 0xa380a380u), st2),
-                           hmul2(hfma2(a & 0x00f000f0u, 0x68006800u, 0xa380a380u), st2),
-                           hmul2(hfma2(b & 0x000f000fu, 0x78007800u, 0xa380a380u), st2),
-                           hmul2(hfma2(b & 0x00f000f0u, 0x68006800u, 0xa380a380u), st2));
+                           scaled(hfma2(a & 0x000f000fu, 0x78007800u, 0xa380a380u)),
+                           scaled(hfma2(a & 0x00f000f0u, 0x68006800u, 0xa380a380u)),
+                           scaled(hfma2(b & 0x000f000fu, 0x78007800u, 0xa380a380u)),
+                           scaled(hfma2(b & 0x00f000f0u, 0x68006800u, 0xa380a380u)));
             }
           }
           fence_proxy_async_smem();  // visible to the tensor core
@@ -774,8 +788,15 @@ __global__ void __launch_bounds__(kThreads, 2)
           l2 = f2_add(l2, f2_add(a, b));
           z2 = f2_fma(a, f2_pack(vm.x, vm.y), z2);
           z2 = f2_fma(b, f2_pack(vm.z, vm.w), z2);
-          pk[c / 2] = pack2<__half>(a0, a1);
-          pk[c / 2 + 1] = pack2<__half>(b0, b1);
+          if constexpr (kStepInV<T>) {
+            pk[c / 2] = pack2<__half>(a0, a1);
+            pk[c / 2 + 1] = pack2<__half>(b0, b1);
+          } else {
+            const float4 vs = ld_shared_f4(f.step + c);
+            const float2 pa = f2_unpack(f2_mul(a, f2_pack(vs.x, vs.y))), pb = f2_unpack(f2_mul(b, f2_pack(vs.z, vs.w)));
+            pk[c / 2] = pack2<__half>(pa.x, pa.y);
+            pk[c / 2 + 1] = pack2<__half>(pb.x, pb.y);
+          }
         }
         const float2 lf = f2_unpack(l2), zf = f2_unpack(z2);
         l += lf.x + lf.y;
@@ -800,7 +821,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const bool whole = pend.j0 == 0 && pend.n == pend.n_kv;
         const int tok = pend.qt * TQ + rtok;
         const bool live = rtok < TQ && tok < plan.len[pend.seq];
-        const float back = exp2_int(max(-126, min(127, pend_exp - kStepBits + kVBits)));  // of one unit of O
+        const float back = exp2_int(max(-126, min(127, pend_exp - kStepBits<T> + kVBits)));  // of one unit of O
         const float inv = !whole ? 1.f : pend_l == 0.f ? 0.f : 1.f / pend_l;
         const float scale = back * inv, base = pend_z * inv;
         float* const dst = part + static_cast<int64_t>(2 * cta + (pend.j0 > 0 ? 0 : 1)) * kPartFloats;

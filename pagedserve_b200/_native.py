@@ -159,5 +159,22 @@ def check(status: int, what: str) -> None:
     raise NativeError(f"{what} failed: {msg} [{status}]")
 
 
+_calls = None
+
+
+def calls():
+    """The module of csrc/calls.cpp (built beside the library; no fallback)."""
+    global _calls
+    if _calls is None:
+        load()  # the library it is linked to, or the error that it is missing
+        try:
+            from . import _calls as module
+        except ImportError as e:
+            raise RuntimeError(f"{os.path.join(_HERE, '_calls.so')} does not load ({e}); build it with "
+                               "`python -m pagedserve_b200.build`") from e
+        _calls = module
+    return _calls
+
+
 def describe_device_error(bits: int) -> str:
     return ", ".join(text for bit, text in DEVERR_BITS.items() if bits & bit) or "none"

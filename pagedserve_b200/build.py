@@ -1,4 +1,5 @@
-"""Build libpagedserve_b200.so in-tree with nvcc for sm_100a.
+"""Build libpagedserve_b200.so in-tree with nvcc for sm_100a, and _calls.so,
+the Python module of csrc/calls.cpp that calls it, with the host compiler.
 
     python -m pagedserve_b200.build            # incremental
     python -m pagedserve_b200.build --force    # rebuild everything
@@ -21,6 +22,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libpagedserve_b200.so")
+CALLS_SRC = os.path.join(CSRC, "calls.cpp")
+CALLS = os.path.join(PKG, "_calls.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr",
          "-I", os.path.join(ROOT, "include")]
@@ -50,6 +53,31 @@ def _compile(src: str, force: bool, extra: list[str]) -> str:
     return obj
 
 
+def _build_calls(force: bool) -> None:
+    """csrc/calls.cpp against this interpreter, this torch and LIB."""
+    import sysconfig
+
+    import torch
+    newest = max(os.path.getmtime(p) for p in (CALLS_SRC, os.path.join(ROOT, "include", "pagedserve_b200.h")))
+    if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= newest:
+        return
+    base = os.path.dirname(torch.__file__)
+    include = os.path.join(base, "include")
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", os.path.join(ROOT, "include"), "-isystem", include,
+           "-isystem", os.path.join(include, "torch", "csrc", "api", "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include"),
+           CALLS_SRC, "-o", CALLS + ".tmp", "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cuda",
+           "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-L", PKG, "-l:libpagedserve_b200.so",
+           "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"building {CALLS_SRC} failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(CALLS + ".tmp", CALLS)
+
+
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> str:
     os.makedirs(BUILD, exist_ok=True)
     extra = list(extra or [])
@@ -63,6 +91,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
+    _build_calls(force)
     if verbose:
         print(LIB)
     return LIB

@@ -581,9 +581,11 @@ def select_tokens(logits: torch.Tensor, eos_ids: torch.Tensor, remaining: torch.
 
 # -- 4-bit KV pool ---------------------------------------------------------------------------------------------
 #
-# A call's host time is most of a small batch's step, so the checks below read
-# every tensor attribute once, compare device indices rather than devices, and
-# leave the wording of an error to the branch that raises it.
+# A call's host time is most of a small batch's step: each function first hands
+# its arguments to its counterpart in csrc/calls.cpp, which checks and launches
+# the ordinary case in one call.  What that does not take (it returns None) is
+# checked here, with the errors' wording, and launched through the C ABI with
+# the copies that unusual strides need.
 
 INT4_MAX_HEAD_DIM = 256
 
@@ -610,27 +612,11 @@ def _call(dev: int, fn, what: str, *args) -> None:
         _native.check(status, what)
 
 
-class _Scratch(threading.local):
-    """Scratch of the split kernels: one growing buffer per host thread,
-    device and stream, so that no two calls that may overlap on the GPU share
-    one.  A call that is being captured gets a tensor of its own from the
-    graph's pool instead (a graph may be replayed on any stream)."""
-
-    def __init__(self):
-        self.buffers: dict[tuple[int, int], torch.Tensor] = {}
-
-    def get(self, nbytes: int, dev: int) -> torch.Tensor:
-        if (_raw_stream is None or torch._C._cuda_getDevice() != dev  # (whose capture could not be asked for)
-                or torch._C._cuda_isCurrentStreamCapturing()):
-            return torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{dev}")
-        stream = _raw_stream(dev)
-        buf = self.buffers.get((dev, stream))
-        if buf is None or buf.numel() < nbytes:
-            buf = self.buffers[(dev, stream)] = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{dev}")
-        return buf
-
-
-_scratch = _Scratch()
+def _done(result, what: str):
+    """What a call of csrc/calls.cpp returned: its result, or a failure's status."""
+    if type(result) is int:
+        _native.check(result, what)
+    return result
 
 
 def _int4_geometry(kv_codes: torch.Tensor, kv_params: torch.Tensor):
@@ -685,6 +671,11 @@ def reshape_and_cache_int4(key: torch.Tensor, value: torch.Tensor, kv_codes: tor
     ``kv_codes[layer]`` / ``kv_params[layer]`` at ``slot_mapping [T]`` (int64;
     negative: nothing is written; live slots distinct).
     """
+    if key.is_cuda:
+        done = (_native._calls or _native.calls()).write(key, value, kv_codes, kv_params, slot_mapping, layer, error_flag)
+        if done is not None:
+            _done(done, "reshape_and_cache_int4")
+            return
     nl, nb, hkv, bs, d, dtype, code = _int4_geometry(kv_codes, kv_params)
     t = _int4_rows(key, value, hkv, d, dtype)
     slot_mapping = _int4_slots(slot_mapping, t)
@@ -710,6 +701,11 @@ def rope_reshape_and_cache_int4(query: torch.Tensor, key: torch.Tensor, value: t
     Returns ``(query_out, key_out)`` with the same defaults: new tensors,
     ``query_out=query`` to rotate in place, ``key_out=False`` for none.
     """
+    if query_out is None and query.is_cuda:
+        done = (_native._calls or _native.calls()).rope_write(query, key, value, cos, sin, kv_codes, kv_params,
+                                                              slot_mapping, layer, key_out, error_flag)
+        if done is not None:
+            return _done(done, "rope_reshape_and_cache_int4")
     nl, nb, hkv, bs, d, dtype, code = _int4_geometry(kv_codes, kv_params)
     shape = query.shape
     if len(shape) != 3 or shape[2] != d:
@@ -763,6 +759,10 @@ def gather_cache_int4(kv_codes: torch.Tensor, kv_params: torch.Tensor, slot_mapp
     """``(key, value) [T, Hkv, D]``: the values a 4-bit pool holds at
     ``slot_mapping [T]`` (int64; zeros for a negative slot), in ``kv_params``'
     dtype (psb_gather_cache_int4)."""
+    if key_out is None and value_out is None and kv_codes.is_cuda:
+        done = (_native._calls or _native.calls()).gather(kv_codes, kv_params, slot_mapping, layer, error_flag)
+        if done is not None:
+            return _done(done, "gather_cache_int4")
     nl, nb, hkv, bs, d, dtype, code = _int4_geometry(kv_codes, kv_params)
     t = slot_mapping.shape[0] if slot_mapping.ndim == 1 else -1
     slot_mapping = _int4_slots(slot_mapping, t)
@@ -806,11 +806,16 @@ def paged_decode_int4(query: torch.Tensor, kv_codes: torch.Tensor, kv_params: to
     """``paged_decode`` over a 4-bit pool (psb_paged_decode_int4).
 
     ``query [B, Hq, D]`` or ``[B, Hq, 1, D]`` of ``kv_params``' dtype; tables,
-    lengths, ``max_context`` and ``scale`` as in ``paged_decode``.  The split-K
-    scratch is kept per host thread, device and stream (a captured call has
-    its own) unless ``workspace`` (``decode_int4_workspace_bytes``) is given,
-    which calls that may overlap on the GPU must not share.
+    lengths, ``max_context`` and ``scale`` as in ``paged_decode``.  Each call
+    takes its split-K scratch from PyTorch's allocator unless ``workspace``
+    (``decode_int4_workspace_bytes``) is given, which calls that may overlap
+    on the GPU must not share.
     """
+    if query.is_cuda:
+        done = (_native._calls or _native.calls()).decode(query, kv_codes, kv_params, block_tables, context_lens, layer,
+                                                          scale, out, max_context, workspace, error_flag)
+        if done is not None:
+            return _done(done, "paged_decode_int4")
     nl, nb, hkv, bs, d, dtype, code = _int4_geometry(kv_codes, kv_params)
     q3 = query.squeeze(2) if query.ndim == 4 else query
     shape = q3.shape
@@ -856,7 +861,8 @@ def paged_decode_int4(query: torch.Tensor, kv_codes: torch.Tensor, kv_params: to
     if o3.shape != shape or o3.dtype != dtype or os_[2] != 1:
         raise ValueError("out must match query's shape/dtype with unit stride along head_dim")
     if workspace is None:
-        workspace = _scratch.get(decode_int4_workspace_bytes(bsz, hq, hkv, d, bs, int(max_context), dtype), dev)
+        workspace = torch.empty(decode_int4_workspace_bytes(bsz, hq, hkv, d, bs, int(max_context), dtype),
+                                dtype=torch.uint8, device=query.device)
     else:
         _check_workspace(workspace)
     _call(dev, _native.load().psb_paged_decode_int4, "paged_decode_int4",
@@ -883,6 +889,12 @@ def paged_prefill_int4(q: torch.Tensor, kv_codes: torch.Tensor, kv_params: torch
     Hq, D]`` of ``kv_params``' dtype, the rest as in ``paged_prefill``.  Rows
     of ``out`` that belong to no sequence keep what they held.  Scratch as in
     ``paged_decode_int4`` (``prefill_int4_workspace_bytes``)."""
+    if q.is_cuda:
+        done = (_native._calls or _native.calls()).prefill(q, kv_codes, kv_params, cu_seqlens, max_seqlen, block_tables,
+                                                           context_lens, layer, scale, out, max_context, workspace,
+                                                           error_flag)
+        if done is not None:
+            return _done(done, "paged_prefill_int4")
     nl, nb, hkv, bs, d, dtype, code = _int4_geometry(kv_codes, kv_params)
     shape = q.shape
     if len(shape) != 3 or shape[2] != d:
@@ -927,7 +939,8 @@ def paged_prefill_int4(q: torch.Tensor, kv_codes: torch.Tensor, kv_params: torch
     if out.shape != shape or out.dtype != dtype or os_[2] != 1:
         raise ValueError("out must match q with unit stride along head_dim")
     if workspace is None:
-        workspace = _scratch.get(prefill_int4_workspace_bytes(t, batch, hq, hkv, d, bs, int(max_context), dtype), dev)
+        workspace = torch.empty(prefill_int4_workspace_bytes(t, batch, hq, hkv, d, bs, int(max_context), dtype),
+                                dtype=torch.uint8, device=q.device)
     else:
         _check_workspace(workspace)
     _call(dev, _native.load().psb_paged_prefill_int4, "paged_prefill_int4",
@@ -989,6 +1002,11 @@ def extend_step(table_store: torch.Tensor, req_rows: torch.Tensor, starts: torch
     free blocks, 256: a row named twice, 4: a bad row, start, count or width,
     32: ``total`` is not the sum) and gives slots of -1 and lengths of 0.
     """
+    if out is None and table_store.is_cuda:
+        done = (_native._calls or _native.calls()).extend(table_store, req_rows, starts, query_lens, free_blocks,
+                                                          free_state, total, block_size, out_width, error_flag)
+        if done is not None:
+            return _done(done, "extend_step")
     store, bsz, rows, starts, query_lens = _tables_args(table_store, req_rows, starts, query_lens, free_blocks,
                                                         free_state, ("req_rows", "starts", "query_lens"), error_flag)
     total = int(total)
@@ -1033,6 +1051,12 @@ def trim_tables(table_store: torch.Tensor, req_rows: torch.Tensor, held_lens: to
     free ring entry by entry, in table order, as ``BlockManager.free`` returns
     them.  Checked and refused as a whole, like ``extend_step``.
     """
+    if table_store.is_cuda:
+        done = (_native._calls or _native.calls()).trim(table_store, req_rows, held_lens, keep_lens, free_blocks,
+                                                        free_state, block_size, error_flag)
+        if done is not None:
+            _done(done, "trim_tables")
+            return
     store, bsz, rows, held_lens, keep_lens = _tables_args(table_store, req_rows, held_lens, keep_lens, free_blocks,
                                                           free_state, ("req_rows", "held_lens", "keep_lens"),
                                                           error_flag)

@@ -11,9 +11,15 @@
 // zeroes their store entries.  Taken in the same order, the ids are the ones
 // BlockManager hands out.
 //
-// Both are latency bound: integers only, a few hundred kilobytes at most.
+// Both are latency bound: integers only, a few hundred kilobytes at most, and
+// short code (a cold instruction cache costs a kernel of this size more than
+// its loads: the same work with 64-bit divisions, 40 KB of code, took 12.6 +
+// 8.2 us where this takes 9.6 + 6.8 us for 256 requests, by the profiler).  So positions and
+// counts are 32 bits (what is added to them is checked first), a division by
+// block_size is a shift where it is a power of two, and the grid walks rows of
+// the table instead of elements.
 // Every CTA scans the whole plan into shared memory itself (no second launch,
-// no grid-wide wait), then the grid strides over table entries and tokens.
+// no grid-wide wait), then the grid strides over table rows and tokens.
 // The ring and the counters are only read in that phase; the last CTA to
 // arrive (a ticket in free_state[2], reset by it) moves head and count, after
 // every CTA has read them.  A step that cannot be carried out whole - not
@@ -30,6 +36,7 @@ namespace {
 
 constexpr int kTabThreads = 256;
 constexpr int kTabWarps = kTabThreads / 32;
+constexpr int kPiece = 128;  // table columns a warp writes at a time
 
 struct TablesParams {
   int32_t* store;
@@ -38,7 +45,7 @@ struct TablesParams {
   const int32_t* rows;
   const int32_t* first;   // extend: starts; trim: held lengths
   const int32_t* second;  // extend: new tokens; trim: kept lengths
-  int32_t batch, block_size;
+  int32_t batch, block_size, shift;  // block_size is 2^shift, or shift is -1
   int32_t* ring;
   int32_t* state;
   int32_t ring_size;
@@ -52,29 +59,46 @@ struct TablesParams {
   int32_t* tables;
 };
 
-__device__ __forceinline__ int64_t blocks_for(int64_t tokens, int block_size) {
-  return (tokens + block_size - 1) / block_size;
+// Blocks of ``tokens`` (below 2^32) tokens.
+__device__ __forceinline__ uint32_t over(const TablesParams& p, uint32_t x) {
+  return p.shift >= 0 ? x >> p.shift : x / static_cast<uint32_t>(p.block_size);
+}
+__device__ __forceinline__ uint32_t blocks_for(const TablesParams& p, uint32_t tokens) {
+  return tokens == 0 ? 0 : over(p, tokens - 1) + 1;
 }
 
-// Exclusive scan over the CTA of one int64 per thread; also the total.
-__device__ int64_t scan_threads(int64_t v, int64_t* warp_sums, int64_t& total) {
+// Exclusive scan over the CTA of two values per thread (``a`` up to 2^40, ``b``
+// up to 2^40), and their totals.
+__device__ __forceinline__ void scan_threads(int64_t& a, int64_t& b, int64_t& a_total, int64_t& b_total) {
+  __shared__ int64_t sums[2][kTabWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t incl = v;
-#pragma unroll
+  const int64_t a0 = a, b0 = b;
+#pragma unroll 1
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += x;
+    const int64_t x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) {
+      a += x;
+      b += y;
+    }
   }
-  if (lane == 31) warp_sums[warp] = incl;
+  if (lane == 31) {
+    sums[0][warp] = a;
+    sums[1][warp] = b;
+  }
   __syncthreads();
-  int64_t run = incl - v;
-  total = 0;
+  a -= a0;
+  b -= b0;
+  a_total = b_total = 0;
+#pragma unroll 1
   for (int w = 0; w < kTabWarps; ++w) {
-    if (w < warp) run += warp_sums[w];
-    total += warp_sums[w];
+    const int64_t x = sums[0][w], y = sums[1][w];
+    if (w < warp) {
+      a += x;
+      b += y;
+    }
+    a_total += x;
+    b_total += y;
   }
-  __syncthreads();  // warp_sums may be used again
-  return run;
 }
 
 // The last CTA to get here moves the ring; called by every thread once the
@@ -112,149 +136,186 @@ __global__ void __launch_bounds__(kTabThreads) extend_step_kernel(const TablesPa
   int32_t* s_cu = sm;                        // [batch + 1] tokens before entry b
   int32_t* s_gr = s_cu + p.batch + 1;        // [batch + 1] new blocks before entry b
   uint32_t* seen = reinterpret_cast<uint32_t*>(s_gr + p.batch + 1);  // store rows named so far
-  __shared__ int64_t warp_sums[kTabWarps];
-  const int tid = threadIdx.x, BS = p.block_size;
+  const int tid = threadIdx.x, lane = tid & 31;
   for (int i = tid; i < (p.store_rows + 31) / 32; i += kTabThreads) seen[i] = 0;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int32_t head = p.state[0], count = p.state[1];
   __syncthreads();
   const int per = (p.batch + kTabThreads - 1) / kTabThreads;
   const int begin = min(tid * per, p.batch), end = min(begin + per, p.batch);
+  const uint32_t width = min(p.store_width, p.out_width);
   int64_t tok = 0, grow = 0;
   int32_t bits = 0;
+#pragma unroll 1
   for (int b = begin; b < end; ++b) {
     const int32_t row = p.rows[b], start = p.first[b], n = p.second[b];
     tok += max(n, 0);
     if (n < 0) bits |= PSB_DEVERR_CONTEXT;
-    if (row < 0) continue;  // a padding entry holds and takes nothing
-    const int64_t len = static_cast<int64_t>(start) + max(n, 0);
-    if (row >= p.store_rows || start < 0 || blocks_for(len, BS) > static_cast<int64_t>(min(p.store_width, p.out_width))) {
-      bits |= PSB_DEVERR_CONTEXT;
-      continue;
+    int32_t more = 0;
+    if (row >= 0) {  // (a padding entry holds and takes nothing)
+      const uint32_t need = blocks_for(p, static_cast<uint32_t>(max(start, 0)) + static_cast<uint32_t>(max(n, 0)));
+      if (row >= p.store_rows || start < 0 || need > width) {
+        bits |= PSB_DEVERR_CONTEXT;
+      } else {
+        if (mark_row(seen, row)) bits |= PSB_DEVERR_ROWS;
+        more = static_cast<int32_t>(need - blocks_for(p, start));
+      }
     }
-    if (mark_row(seen, row)) bits |= PSB_DEVERR_ROWS;
-    grow += blocks_for(len, BS) - blocks_for(start, BS);
+    s_gr[b] = more;
+    grow += more;
   }
   int64_t tok_total, grow_total;
-  int64_t tok_at = scan_threads(tok, warp_sums, tok_total);
-  int64_t grow_at = scan_threads(grow, warp_sums, grow_total);
-  const int32_t head = p.state[0], count = p.state[1];
+  scan_threads(tok, grow, tok_total, grow_total);
   if (tok_total != p.total) bits |= PSB_DEVERR_SEQLENS;
   if (head < 0 || head >= p.ring_size || count < 0 || count > p.ring_size || grow_total > count)
     bits |= PSB_DEVERR_POOL;
   const bool bad = __syncthreads_or(bits) != 0;
   if (bits != 0 && blockIdx.x == 0) flag_error(p.err, bits);
+#pragma unroll 1
   for (int b = begin; b < end; ++b) {
-    const int32_t row = p.rows[b], start = p.first[b], n = max(p.second[b], 0);
     // a refused step may hold counts that no int32 sum does: kept in range
-    s_cu[b] = static_cast<int32_t>(min(tok_at, static_cast<int64_t>(p.total)));
-    s_gr[b] = bad ? 0 : static_cast<int32_t>(grow_at);
-    tok_at += n;
-    if (!bad && row >= 0) grow_at += blocks_for(static_cast<int64_t>(start) + n, BS) - blocks_for(start, BS);
+    s_cu[b] = static_cast<int32_t>(min(tok, static_cast<int64_t>(p.total)));
+    tok += max(p.second[b], 0);
+    const int32_t more = s_gr[b];
+    s_gr[b] = bad ? 0 : static_cast<int32_t>(grow);
+    grow += more;
   }
+  const int32_t taken = bad ? 0 : static_cast<int32_t>(grow_total);
   if (tid == 0) {
     s_cu[p.batch] = static_cast<int32_t>(min(tok_total, static_cast<int64_t>(p.total)));
-    s_gr[p.batch] = bad ? 0 : static_cast<int32_t>(grow_total);
+    s_gr[p.batch] = taken;
   }
   __syncthreads();
 
-  const int64_t gtid = blockIdx.x * static_cast<int64_t>(kTabThreads) + tid;
-  const int64_t gstride = static_cast<int64_t>(gridDim.x) * kTabThreads;
-  // block ``j`` of entry b: one it holds, or its share of the ring
-  auto block_of = [&](int b, int32_t row, int64_t held, int64_t j) -> int32_t {
+  // block ``j`` of entry b, which holds ``held``: one of those, or its share of the ring
+  auto block_of = [&](int b, int32_t row, uint32_t held, uint32_t j) -> int32_t {
     if (j < held) return p.store[row * p.store_stride + j];
-    int64_t at = static_cast<int64_t>(head) + s_gr[b] + (j - held);
-    if (at >= p.ring_size) at -= p.ring_size;
+    uint32_t at = static_cast<uint32_t>(head) + static_cast<uint32_t>(s_gr[b]) + (j - held);  // below 2^32: two counts
+    if (at >= static_cast<uint32_t>(p.ring_size)) at -= p.ring_size;
     return p.ring[at];
   };
   if (blockIdx.x == 0) {
-    for (int b = tid; b <= p.batch; b += kTabThreads) p.cu[b] = s_cu[b];
-    for (int b = tid; b < p.batch; b += kTabThreads)
-      p.ctx[b] = bad || p.rows[b] < 0 ? 0 : p.first[b] + p.second[b];
+    for (int b = tid; b <= p.batch; b += kTabThreads) {
+      p.cu[b] = s_cu[b];
+      if (b < p.batch) p.ctx[b] = bad || p.rows[b] < 0 ? 0 : p.first[b] + p.second[b];
+    }
   }
-  // padded tables, and the new ids into the store
-  for (int64_t i = gtid; i < static_cast<int64_t>(p.batch) * p.out_width; i += gstride) {
-    const int b = static_cast<int>(i / p.out_width), j = static_cast<int>(i - static_cast<int64_t>(b) * p.out_width);
-    const int32_t row = p.rows[b];
-    int32_t v = 0;
-    if (!bad && row >= 0) {
-      const int64_t start = p.first[b], held = blocks_for(start, BS);
-      if (j < blocks_for(start + p.second[b], BS)) {
+  // padded tables, and the new ids into the store: a warp per piece of a row
+  const int pieces = (p.out_width + kPiece - 1) / kPiece;
+  const int64_t tasks = static_cast<int64_t>(p.batch) * pieces;
+#pragma unroll 1
+  for (int64_t t = blockIdx.x * kTabWarps + (tid >> 5); t < tasks; t += static_cast<int64_t>(gridDim.x) * kTabWarps) {
+    const int b = pieces == 1 ? static_cast<int>(t) : static_cast<int>(t / pieces);
+    const int j0 = static_cast<int>(t - static_cast<int64_t>(b) * pieces) * kPiece;
+    const int32_t row = bad ? -1 : p.rows[b];
+    uint32_t held = 0, need = 0;
+    if (row >= 0) {
+      const uint32_t start = p.first[b];
+      held = blocks_for(p, start);
+      need = blocks_for(p, start + static_cast<uint32_t>(p.second[b]));
+    }
+    int32_t* const out = p.tables + static_cast<int64_t>(b) * p.out_width;
+#pragma unroll 1
+    for (int j = j0 + lane; j < min(j0 + kPiece, p.out_width); j += 32) {
+      int32_t v = 0;
+      if (static_cast<uint32_t>(j) < need) {
         v = block_of(b, row, held, j);
         if (v < 0 || v >= p.ring_size) flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
-        if (j >= held) p.store[row * p.store_stride + j] = v;
+        if (static_cast<uint32_t>(j) >= held) p.store[row * p.store_stride + j] = v;
       }
+      out[j] = v;
     }
-    p.tables[i] = v;
   }
   // slot and position of every new token
-  for (int64_t i = gtid; i < p.total; i += gstride) {
-    int64_t slot = -1, pos = 0;
+#pragma unroll 1
+  for (uint32_t i = blockIdx.x * kTabThreads + tid; i < static_cast<uint32_t>(p.total); i += gridDim.x * kTabThreads) {
+    int64_t slot = -1;
+    uint32_t pos = 0;
     if (!bad) {
       const int b = entry_of(s_cu, p.batch, static_cast<int>(i));
       const int32_t row = p.rows[b];
       if (row >= 0) {
-        const int32_t start = p.first[b];
-        pos = static_cast<int64_t>(start) + (i - s_cu[b]);
-        const int64_t j = pos / BS;
-        const int32_t v = block_of(b, row, blocks_for(start, BS), j);
-        if (v >= 0 && v < p.ring_size) slot = static_cast<int64_t>(v) * BS + (pos - j * BS);
+        const uint32_t start = p.first[b];
+        pos = start + (i - static_cast<uint32_t>(s_cu[b]));
+        const uint32_t j = over(p, pos);
+        const int32_t v = block_of(b, row, blocks_for(p, start), j);
+        if (v >= 0 && v < p.ring_size)
+          slot = static_cast<int64_t>(v) * p.block_size + (pos - j * static_cast<uint32_t>(p.block_size));
       }
     }
     p.slots[i] = slot;
     p.positions[i] = pos;
   }
-  int64_t new_head = static_cast<int64_t>(head) + s_gr[p.batch];
-  if (new_head >= p.ring_size) new_head -= p.ring_size;
-  finish_ring(p, bad ? head : static_cast<int32_t>(new_head), count - s_gr[p.batch]);
+  uint32_t new_head = static_cast<uint32_t>(head) + static_cast<uint32_t>(taken);
+  if (!bad && new_head >= static_cast<uint32_t>(p.ring_size)) new_head -= p.ring_size;
+  finish_ring(p, static_cast<int32_t>(new_head), count - taken);
 }
 
 __global__ void __launch_bounds__(kTabThreads) trim_tables_kernel(const TablesParams p) {
   extern __shared__ int32_t sm[];
   int32_t* s_pre = sm;  // [batch + 1] blocks given back before entry b
   uint32_t* seen = reinterpret_cast<uint32_t*>(s_pre + p.batch + 1);
-  __shared__ int64_t warp_sums[kTabWarps];
-  const int tid = threadIdx.x, BS = p.block_size;
+  const int tid = threadIdx.x;
   for (int i = tid; i < (p.store_rows + 31) / 32; i += kTabThreads) seen[i] = 0;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int32_t head = p.state[0], count = p.state[1];
   __syncthreads();
   const int per = (p.batch + kTabThreads - 1) / kTabThreads;
   const int begin = min(tid * per, p.batch), end = min(begin + per, p.batch);
-  int64_t back = 0;
+  int64_t back = 0, unused = 0;
   int32_t bits = 0;
+#pragma unroll 1
   for (int b = begin; b < end; ++b) {
     const int32_t row = p.rows[b], held = p.first[b], keep = p.second[b];
-    if (row < 0) continue;
-    if (row >= p.store_rows || keep < 0 || keep > held || blocks_for(held, BS) > p.store_width) {
-      bits |= PSB_DEVERR_CONTEXT;
-      continue;
+    int32_t less = 0;
+    if (row >= 0) {
+      const uint32_t have = blocks_for(p, max(held, 0));
+      if (row >= p.store_rows || keep < 0 || keep > held || have > static_cast<uint32_t>(p.store_width)) {
+        bits |= PSB_DEVERR_CONTEXT;
+      } else {
+        if (mark_row(seen, row)) bits |= PSB_DEVERR_ROWS;
+        less = static_cast<int32_t>(have - blocks_for(p, keep));
+      }
     }
-    if (mark_row(seen, row)) bits |= PSB_DEVERR_ROWS;
-    back += blocks_for(held, BS) - blocks_for(keep, BS);
+    s_pre[b] = less;
+    back += less;
   }
-  int64_t back_total;
-  int64_t at = scan_threads(back, warp_sums, back_total);
-  const int32_t head = p.state[0], count = p.state[1];
+  int64_t back_total, unused_total;
+  scan_threads(back, unused, back_total, unused_total);
   if (head < 0 || head >= p.ring_size || count < 0 || count + back_total > p.ring_size) bits |= PSB_DEVERR_POOL;
   const bool bad = __syncthreads_or(bits) != 0;
   if (bits != 0 && blockIdx.x == 0) flag_error(p.err, bits);
   if (!bad) {  // the same for every thread of every CTA
+#pragma unroll 1
     for (int b = begin; b < end; ++b) {
-      s_pre[b] = static_cast<int32_t>(at);
-      if (p.rows[b] >= 0) at += blocks_for(p.first[b], BS) - blocks_for(p.second[b], BS);
+      const int32_t less = s_pre[b];
+      s_pre[b] = static_cast<int32_t>(back);
+      back += less;
     }
     __syncthreads();
-    const int64_t gstride = static_cast<int64_t>(gridDim.x) * kTabThreads;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kTabThreads) + tid; i < back_total; i += gstride) {
+#pragma unroll 1
+    for (uint32_t i = blockIdx.x * kTabThreads + tid; i < static_cast<uint32_t>(back_total); i += gridDim.x * kTabThreads) {
       const int b = entry_of(s_pre, p.batch, static_cast<int>(i));
-      const int64_t j = blocks_for(p.second[b], BS) + (i - s_pre[b]);
+      const uint32_t j = blocks_for(p, p.second[b]) + (i - static_cast<uint32_t>(s_pre[b]));
       int32_t* entry = p.store + p.rows[b] * p.store_stride + j;
       const int32_t v = *entry;
       if (v < 0 || v >= p.ring_size) flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
-      int64_t to = static_cast<int64_t>(head) + count + i;
+      int64_t to = static_cast<int64_t>(head) + count + i;  // below two rings
       if (to >= p.ring_size) to -= p.ring_size;
       p.ring[to] = v;
       *entry = 0;
     }
   }
   finish_ring(p, head, bad ? count : count + static_cast<int32_t>(back_total));
+}
+
+int32_t block_shift(int32_t block_size) {
+  if ((block_size & (block_size - 1)) != 0) return -1;
+  int32_t s = 0;
+  while ((1 << s) < block_size) ++s;
+  return s;
 }
 
 // Shared bytes of a launch: ``arrays`` prefixes over the batch and the bitmap.
@@ -271,7 +332,8 @@ int launch_tables(void (*kern)(TablesParams), const TablesParams& p, int arrays,
   if (!kernel_occupancy(reinterpret_cast<const void*>(kern), kTabThreads, smem, &occ)) return PSB_ERR_CUDA;
   const int64_t grid = std::max<int64_t>(1, std::min<int64_t>((work + kTabThreads - 1) / kTabThreads, sms));
   discard_stale_error();
-  kern<<<static_cast<unsigned>(grid), kTabThreads, smem, s>>>(p);
+  const cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kTabThreads), smem, s, p);
+  if (e != cudaSuccess) return record_cuda_error(e);
   return check_launch();
 }
 
@@ -303,6 +365,7 @@ extern "C" int psb_extend_step(int32_t* table_store, int64_t store_stride, int32
   p.second = query_lens;
   p.batch = batch;
   p.block_size = block_size;
+  p.shift = block_shift(block_size);
   p.ring = free_blocks;
   p.state = free_state;
   p.ring_size = num_blocks;
@@ -337,6 +400,7 @@ extern "C" int psb_trim_tables(int32_t* table_store, int64_t store_stride, int32
   p.second = keep_lens;
   p.batch = batch;
   p.block_size = block_size;
+  p.shift = block_shift(block_size);
   p.ring = free_blocks;
   p.state = free_state;
   p.ring_size = num_blocks;

@@ -849,6 +849,8 @@ def paged_decode_int4(query: torch.Tensor, kv_codes: torch.Tensor, kv_params: to
         max_context = width
     elif not 0 <= max_context <= width:
         raise ValueError("max_context must be at most block_tables' width in tokens")
+    if max_context >= 1 << 31:
+        raise ValueError("max_context must be below 2^31 tokens")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     _check_flag(error_flag)
     dev = _cuda_index(kv_codes, kv_params, q3, block_tables, context_lens, out, workspace, error_flag)
@@ -928,6 +930,8 @@ def paged_prefill_int4(q: torch.Tensor, kv_codes: torch.Tensor, kv_params: torch
         max_context = width
     elif max_context > width:
         raise ValueError("max_context must be at most block_tables' width in tokens")
+    if max_context >= 1 << 31:
+        raise ValueError("max_context must be below 2^31 tokens")
     if not 0 <= max_seqlen <= max_context:
         raise ValueError("max_seqlen must be at most max_context")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)

@@ -102,7 +102,9 @@ struct TcParams {
   Int4PrefillParams a;
   int32_t group, tq;      // q heads per kv head, tokens per tile
   int32_t max_tiles;      // room for the tile table
-  uint64_t block_div;     // 2^32 / block_size, rounded up
+  int32_t block_shift;    // block_size is 2^block_shift, or -1
+  uint32_t block_div;     // else 2^32 / block_size, rounded up
+  int64_t block_rows;     // pool rows from a block to the next
   float* part;            // workspace: cuts, then two partials per CTA
 };
 
@@ -476,24 +478,23 @@ __global__ void __launch_bounds__(kThreads, 2)
       Cursor cc = first;
       int left = 0, pos0 = 0, ctx = 0;  // of the run being looked up: steps left, first key of the next, tokens
       const int32_t* row = nullptr;
-      int64_t tile0 = 0;
+      int64_t row0 = 0;  // pool row of token 0 of block 0, K
       auto next_run = [&]() {
         const Run s = cc.take(plan);
         pos0 = s.j0 * kBN;
         left = s.n;
         row = p.tables + static_cast<int64_t>(s.seq) * p.table_stride;
         ctx = plan.ctx[s.seq];
-        tile0 = p.layer_tiles + s.kvh;
+        row0 = int4_row(p.layer_tiles + s.kvh, 0, 0, p.block_size);
       };
       // row r's place in the pool (-1: past the sequence, -2: its block is outside the pool)
       auto place = [&](int r, int kv) -> int64_t {
         const uint32_t pos = pos0 + r;
         if (static_cast<int>(pos) >= ctx) return -1;
-        const uint32_t bi = static_cast<uint32_t>((static_cast<uint64_t>(pos) * tp.block_div) >> 32);
+        const uint32_t bi = tp.block_shift >= 0 ? pos >> tp.block_shift : __umulhi(pos, tp.block_div);
         const int blk = __ldg(row + bi);
         if (blk < 0 || blk >= p.num_blocks) return -2;
-        return int4_row(tile0 + static_cast<int64_t>(blk) * p.hkv, kv, static_cast<int>(pos - bi * p.block_size),
-                        p.block_size);
+        return row0 + blk * tp.block_rows + (kv * p.block_size + pos - bi * p.block_size);
       };
       struct Row {
         uint4 c[2];
@@ -986,7 +987,11 @@ int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspa
   tp.group = p.hq / p.hkv;
   tp.tq = kRows / tp.group;
   tp.max_tiles = static_cast<int32_t>(tiles_bound(p.total, p.num_seqs, tp.tq));
-  tp.block_div = ((uint64_t(1) << 32) + p.block_size - 1) / p.block_size;
+  tp.block_shift = -1;
+  if ((p.block_size & (p.block_size - 1)) == 0)
+    for (tp.block_shift = 0; (1 << tp.block_shift) < p.block_size;) ++tp.block_shift;
+  tp.block_div = tp.block_shift >= 0 ? 0 : static_cast<uint32_t>(((uint64_t(1) << 32) + p.block_size - 1) / p.block_size);
+  tp.block_rows = static_cast<int64_t>(p.hkv) * 2 * p.block_size;
   tp.part = workspace;
   CUtensorMap tq;
   if (!encode_row_groups_map(&tq, p.q, p.total, p.hq, kDim, p.qst, p.qsh, tp.group, tp.tq,

@@ -473,9 +473,10 @@ size_t psb_paged_decode_int4_workspace_size(int32_t batch, int32_t q_heads, int3
  * K and V being the values the codes stand for; a sequence of length 0 gives
  * zeros.  query and out are of ``dtype`` = T.  The codes enter the products as
  * they are (exactly) and step and mid are applied to the sums in fp32, so the
- * only 16-bit rounding is that of step * probability before P V.  Lengths and
- * tables are read before the kernel waits on its stream predecessor, as
- * psb_paged_decode reads them.  Error behaviour is psb_paged_decode's.
+ * only 16-bit rounding is that of step * probability before P V.  Unlike
+ * psb_paged_decode it reads nothing before its stream predecessor has ended:
+ * lengths and tables may come from psb_extend_step.  Error behaviour is
+ * psb_paged_decode's.
  */
 int psb_paged_decode_int4(const void* query, int64_t q_stride_b, int64_t q_stride_h, void* out, int64_t o_stride_b,
                           int64_t o_stride_h, const void* kv_codes, const void* kv_params,
@@ -495,7 +496,11 @@ size_t psb_paged_prefill_int4_workspace_size(int32_t total_tokens, int32_t num_s
  * paged_prefill_int4: psb_paged_prefill over the 4-bit pool.  Sequence i's
  * query rows cu_seqlens[i] .. cu_seqlens[i+1] are the last positions of its
  * context_lens[i] tokens in the pool; rows of ``out`` behind the last sequence
- * are left as they were.  Error behaviour is psb_paged_prefill's.
+ * are left as they were.  16-bit roundings: K's values to T and what that
+ * leaves out (2^-17 together for bf16), the probabilities to f16 (bf16: V's
+ * step * code too; f16: with the steps on them).  A row that stands for NaN
+ * reaches the query rows that see it and no others.  Error behaviour is
+ * psb_paged_prefill's.
  */
 int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv_codes,
                            const void* kv_params, const int32_t* block_tables, int64_t table_stride,

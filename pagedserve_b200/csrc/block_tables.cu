@@ -139,7 +139,6 @@ __global__ void __launch_bounds__(kTabThreads) extend_step_kernel(const TablesPa
   const int tid = threadIdx.x, lane = tid & 31;
   for (int i = tid; i < (p.store_rows + 31) / 32; i += kTabThreads) seen[i] = 0;
   pdl_wait();
-  pdl_launch_dependents();
   const int32_t head = p.state[0], count = p.state[1];
   __syncthreads();
   const int per = (p.batch + kTabThreads - 1) / kTabThreads;
@@ -259,7 +258,6 @@ __global__ void __launch_bounds__(kTabThreads) trim_tables_kernel(const TablesPa
   const int tid = threadIdx.x;
   for (int i = tid; i < (p.store_rows + 31) / 32; i += kTabThreads) seen[i] = 0;
   pdl_wait();
-  pdl_launch_dependents();
   const int32_t head = p.state[0], count = p.state[1];
   __syncthreads();
   const int per = (p.batch + kTabThreads - 1) / kTabThreads;

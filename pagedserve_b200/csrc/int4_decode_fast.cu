@@ -26,20 +26,30 @@
 //
 // What bounds it.  A 16-token tile of head_dim 64 is 1152 bytes against 4096
 // in bf16, so the same bytes per second need 3.6 times the instructions of
-// paged_decode: the issue slots of the four schedulers bound it next to HBM.
-// Hence codes by AND, two tiles at a time (independent work, one vote and one
-// set of loop instructions for both), each token's four factors worked out by
-// one lane and handed round through shared memory, the exponents' reference
-// folded into the score's multiply-add, and addresses and validity worked out
-// for 32 items at once, one per lane.
+// paged_decode: the issue slots of the four schedulers bound it next to HBM
+// (about 150 instructions and 240 cycles a tile and scheduler).  Hence codes by
+// AND, two tiles at a time (independent work, one vote and one set of loop
+// instructions for both), each token's four factors worked out by one lane and
+// handed round through shared memory, the exponents' reference folded into the
+// score's multiply-add, and addresses and validity worked out for 32 items at
+// once, one per lane.  Measured: 256 sequences of 62 MB of cache 26.1 us (2.4
+// TB/s; the 16-bit pool's paged_decode 39 us), of which some 7 us do not depend
+// on the length; 3 sequences of 32 K tokens 13.3 us, of 128 K 10 us more (4 TB/s);
+// 64 sequences of 4 K at head_dim 128 43.9 us (3.5 TB/s).  Reading lengths and
+// tables before the wait for the stream predecessor saved 0.6 to 1.5 us a call,
+// but a predecessor that starts its dependents early (or has just left the GPU)
+// may not have written them yet.
 //
 // Split.  The items (32 tokens) of all sequences, in (kv head, sequence,
-// position) order, are dealt evenly over the consumer warps of the grid (one CTA
-// per SM).  Each has a private shared-memory ring, filled by bulk copies that
-// lane w of the CTA's copying warp issues for consumer w.  A sequence inside one warp's run is written
-// at once; pieces of one sequence within a CTA are joined in shared memory,
-// and only a sequence cut by a CTA boundary (at most one per CTA) leaves
-// partials, for int4_combine_kernel.
+// position) order, are dealt evenly over the warps of the grid (one CTA per
+// SM).  A warp loads its codes straight into registers, each part of the next
+// item as soon as this item's part has been used: bulk copies by a warp of
+// their own through shared memory took 2.5 times as long, a ring filled by
+// cp.async 187 instructions a tile, prefetches to L2 gained nothing.  12 warps
+// of 164 registers beat 8 of 244 where the tile fits (26.0 against 28.1 us).  A
+// sequence inside one warp's run is written at once; pieces of one sequence
+// within a CTA are joined in shared memory, and only a sequence cut by a CTA
+// boundary (at most one per CTA) leaves partials, for int4_combine_kernel.
 #include <algorithm>
 #include <type_traits>
 
@@ -53,7 +63,6 @@ namespace {
 
 constexpr int kMaxCtas = 160;       // grid limit (one CTA per SM; B200 has 148)
 constexpr int kMaxBatch = 2560;     // sequences whose lengths fit in shared memory
-constexpr int kMinItems = 1;        // items per warp below which fewer CTAs take part
 
 template <int D, int HT>
 struct Geo {
@@ -197,13 +206,14 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
   const int B = p.batch, BS = p.block_size;
   const int hgroups = (p.group + kRows - 1) / kRows;  // head tiles per kv head
   if (tid < 2 * kW) s_grp[tid] = -1;
+  pdl_wait();
+  pdl_launch_dependents();
   const int n_seq = build_prefix(p, pre, s_ctx, blockIdx.x == 0);
   const int n_items = n_seq * (p.hkv * hgroups);
-  const int act = min(static_cast<int>(gridDim.x), (n_items + kW * kMinItems - 1) / (kW * kMinItems));
+  const int act = min(static_cast<int>(gridDim.x), (n_items + kW - 1) / kW);
   Cut* const cuts = reinterpret_cast<Cut*>(p.part);
   float* const part = p.part + kMaxCtas * (sizeof(Cut) / sizeof(float));
   if (static_cast<int>(blockIdx.x) >= act) {
-    pdl_wait();
     if (tid == 0) cuts[blockIdx.x] = Cut{0, 0, 0, 0};
     return;
   }
@@ -271,10 +281,6 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
     if (my_e - my_a > 32) nxt = build_chunk(my_a + 32);
   }
 
-  // Only lengths and tables have been read so far; the pool and q may still be
-  // being written by the stream predecessor, the workspace be read by it.
-  pdl_wait();
-  pdl_launch_dependents();
   // Row pi(r) of a tile is the token at index r (0 .. 7; those of 8 .. 15 are 8
   // rows on) of the products: the four tokens of a lane group's V load are
   // adjacent rows, one run of memory.
@@ -916,7 +922,7 @@ int launch_fast(const Int4DecodeParams& p, cudaStream_t stream, int sms) {
   int occ = 0;
   if (!kernel_occupancy(reinterpret_cast<const void*>(kern), G::kThreads, smem, &occ) || occ < 1) return PSB_ERR_CUDA;
   const int64_t items = max_items(p.batch, p.hkv, p.group, G::kRows, p.max_context);
-  const int64_t want = (items + G::kWarps * kMinItems - 1) / (G::kWarps * kMinItems);
+  const int64_t want = (items + G::kWarps - 1) / G::kWarps;
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, std::min(sms, kMaxCtas))));
   discard_stale_error();
   cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(G::kThreads), smem, stream, p);

@@ -4,7 +4,9 @@
 // Generic path (fp32, or a geometry the tensor-core path does not cover): one
 // warp per (query row, q head), 32 keys per step (one key per lane for Q.K,
 // lanes over head_dim for P.V), values decoded to fp32 as they are read,
-// online softmax in fp32.
+// online softmax in fp32.  Bound by its arithmetic and by decoding every key
+// again for every row: 512 tokens on 8 K took 11.6 ms where the tensor-core
+// path takes 61 us.
 #include <algorithm>
 
 #include "common.cuh"

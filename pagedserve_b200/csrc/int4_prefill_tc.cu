@@ -39,6 +39,17 @@
 // the same kernel with its loops unrolled and peeled (121 KB of code) spent
 // more issue slots waiting for instructions than on anything else.
 //
+// What bounds it: instructions.  A step of one CTA is 3600 of them (softmax
+// 1300, K 1100, V 550, issue and waits the rest) and takes some 3300 cycles at
+// two CTAs an SM, half of the issue slots; the exponentials take 27% of their
+// pipe, the tensor pipe is 20% busy.  512 tokens on 8 K: 61 us (paged_prefill
+// over a 16-bit pool: 152 us), of which 20 us do not depend on the context
+// (plan, first look-ups, join); six chunks of 1 K: 135 us (181 us); 32 requests
+// of 5 tokens: 21.5 us (61 us).  Tried without gain: twelve warps (two threads
+// per row, or twice the decoding warps), a third S buffer, one warp per kind
+// of product, a join over the cut tiles only, the set-up before the wait for
+// the predecessor.
+//
 // Every mbarrier wait is bounded; no barrier can run two phases ahead of a
 // waiter: a stage's next phase needs its own release, a step's barriers
 // alternate and step g + 2 needs step g's products.

@@ -14,6 +14,12 @@
 // piece are one word.  Rows that are not 16-byte aligned, or whose pieces are
 // not a power of two, take a warp per row instead: lane l holds the element
 // pairs l, l + 32, ... and a pair is one byte of codes.
+//
+// Measured, write and read-back together: a 16 K-token pack of 14 + 2 heads of
+// head_dim 64 25.7 us (86 MB: 3.4 TB/s, half of the copy rate; a warp per row
+// took 131 us, a division per code 42 us), 1333 plain tokens of 8 heads of 128
+// in f16 10.1 us, 256 tokens 4.8 us.  The read-back issues in 72% of its
+// cycles: unpacking codes, not HBM, is what is left there.
 #include <algorithm>
 
 #include "common.cuh"

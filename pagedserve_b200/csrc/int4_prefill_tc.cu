@@ -76,6 +76,7 @@ constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kSCol = 0, kOCol = 128;
 constexpr float kGrowth = 4.f;      // log2 of how far a score may exceed the exponents' reference
 constexpr int kPBits = 11;          // probabilities are 2^kPBits p, at most 2^(kPBits + kGrowth)
+constexpr float kPUnit = 1.f / (1 << kPBits);
 constexpr int kVBits = 9;           // V's codes are (c - 7.5) 2^-kVBits
 // Where V's steps go, scaled to below 2^kStepBits: bf16, into V's operand;
 // f16, onto the probabilities (below 1, so that those stay below 2^15).
@@ -89,7 +90,7 @@ constexpr int kMaxSeqs = 2048, kMaxTiles = 8192;
 
 // What a V stage's 64 tokens need besides their codes and steps.
 struct Extra {
-  float mid[kBN];   // 0 where it is not finite
+  float mid[kBN];   // mid 2^-kPBits (next to 2^kPBits p); 0 where it is not finite
   float step[kBN];  // scaled; f16 only
   uint32_t bad[2];  // bit t: token t's block is outside the pool
   uint32_t nan[2];  // bit t: token t's mid is not finite
@@ -628,8 +629,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             vscale = exp2_int(max(-126, kStepBits<T> - vexp));
           }
           const bool fin0 = finite_f32(p0.y), fin1 = finite_f32(p1.y);
-          x.mid[lane] = fin0 ? p0.y : 0.f;
-          x.mid[lane + 32] = fin1 ? p1.y : 0.f;
+          x.mid[lane] = fin0 ? p0.y * kPUnit : 0.f;
+          x.mid[lane + 32] = fin1 ? p1.y * kPUnit : 0.f;
           if constexpr (!kStepInV<T>) {
             x.step[lane] = p0.x * vscale;
             x.step[lane + 32] = p1.x * vscale;
@@ -685,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     int left = 0, k = -1;          // steps left of run s, its number
     int last = 0;                  // last key of this row, from the step's first
     uint32_t t_o = 0;
-    float ref = 0.f, l = 0.f, z = 0.f;  // the exponents' reference; sums of 2^kPBits p and 2^kPBits p mid
+    float ref = 0.f, l = 0.f, z = 0.f;  // the exponents' reference; sums of 2^kPBits p and p mid
     bool fresh = true;
     int vexp = 0;
     // A run's output is written after the next run's first step (or at the
@@ -700,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (g > 0) {
           pending = true;
           pend = s;
-          pend_l = l;
+          pend_l = l * kPUnit;
           pend_z = z;
           pend_exp = vexp;
           pend_m = fresh ? -INFINITY : ref;
@@ -833,7 +834,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const bool whole = pend.j0 == 0 && pend.n == pend.n_kv;
         const int tok = pend.qt * TQ + rtok;
         const bool live = rtok < TQ && tok < plan.len[pend.seq];
-        const float back = exp2_int(max(-126, min(127, pend_exp - kStepBits<T> + kVBits)));  // of one unit of O
+        const float back = exp2_int(max(-126, min(127, pend_exp - kStepBits<T> + kVBits - kPBits)));  // of one unit of O
         const float inv = !whole ? 1.f : pend_l == 0.f ? 0.f : 1.f / pend_l;
         const float scale = back * inv, base = pend_z * inv;
         float* const dst = part + static_cast<int64_t>(2 * cta + (pend.j0 > 0 ? 0 : 1)) * kPartFloats;

@@ -369,3 +369,47 @@ def test_prefill_non_finite_rows_stay_behind_the_mask(which, dtype):
     hit[80:130, 7:] = True
     assert bool(torch.isnan(got[hit]).all())
     _close(got[~hit], want[~hit], tol[~hit])
+
+
+@pytest.mark.parametrize("power", [118, -100])
+@pytest.mark.parametrize("qlens,ctxs", [([70], [300]), ([1, 1], [77, 2000])])
+def test_values_at_the_ends_of_bf16(power, qlens, ctxs):
+    """V rows scaled by a power of two up to 2^118 (values to 1e36) or down to
+    2^-100 give results scaled by it: no sum inside over- or underflows."""
+    c = _prefill_case(36, qlens, ctxs, 14, 2, 64, 16, torch.bfloat16)
+    want, tol = _want_prefill(c)
+    c["pp"][:, :, :, 1] = (c["pp"][:, :, :, 1].double() * 2.0 ** power).bfloat16()
+    got, err = _prefill(c)
+    assert err == 0
+    _close(got.double() * 2.0 ** -power, want, tol)
+    if max(qlens) == 1:
+        got, err = _decode(c)
+        assert err == 0
+        _close(got.double() * 2.0 ** -power, want, tol)
+
+
+def test_offsets_past_32_bits():
+    """A pool whose codes are past 4 GB: rows written to its last blocks are
+    read back and attended to as from a small pool, bit for bit."""
+    from pagedserve_b200 import ops
+    gen = torch.Generator().manual_seed(37)
+    hq, hkv, d, bs, n, blocks = 14, 2, 64, 16, 100, 2_200_000
+    k, v = (torch.randn(n, hkv, d, generator=gen).bfloat16().cuda() for _ in range(2))
+    q = torch.randn(40, hq, d, generator=gen).bfloat16().cuda()
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 40], dtype=torch.int32, device="cuda")
+    outs = []
+    for num, ids in ((blocks, [blocks - 1 - 3 * i for i in range(7)]), (9, [8, 2, 3, 7, 0, 1, 5])):
+        codes = torch.empty(1, num, hkv, 2, bs, d // 2, dtype=torch.uint8, device="cuda")
+        params = torch.empty(1, num, hkv, 2, bs, 2, dtype=torch.bfloat16, device="cuda")
+        blk = torch.tensor(ids, device="cuda")
+        pos = torch.arange(n, device="cuda")
+        slots = blk[pos // bs] * bs + pos % bs
+        ops.reshape_and_cache_int4(k, v, codes, params, slots, 0)
+        table = blk.to(torch.int32)[None]
+        outs.append([*ops.gather_cache_int4(codes, params, slots, 0),
+                     ops.paged_decode_int4(q[:1], codes, params, table, lens, 0),
+                     ops.paged_prefill_int4(q, codes, params, table, lens, cu, 40, 0)])
+        del codes, params
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)

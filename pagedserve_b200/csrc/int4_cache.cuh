@@ -78,6 +78,13 @@ __device__ __forceinline__ float int4_value(uint32_t code, float step, float mid
   return fmaf(step, static_cast<float>(code) - kInt4Mid, mid);
 }
 
+// Code j of a word minus 7.5, exactly, without a conversion: c in bits 4-7 of
+// 2^19's mantissa is 2^19 + c.
+__device__ __forceinline__ float int4_centered(uint32_t w, int j) {
+  const uint32_t c = (j == 0 ? w << 4 : w >> (4 * j - 4)) & 0xf0u;
+  return __uint_as_float(c | 0x49000000u) - 524295.5f;
+}
+
 __device__ __forceinline__ bool finite_f32(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 // Packed fp32 pairs (sm_100 f32x2 instructions).

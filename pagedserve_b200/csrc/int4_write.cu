@@ -16,10 +16,11 @@
 // pairs l, l + 32, ... and a pair is one byte of codes.
 //
 // Measured, write and read-back together: a 16 K-token pack of 14 + 2 heads of
-// head_dim 64 25.7 us (86 MB: 3.4 TB/s, half of the copy rate; a warp per row
-// took 131 us, a division per code 42 us), 1333 plain tokens of 8 heads of 128
-// in f16 10.1 us, 256 tokens 4.8 us.  The read-back issues in 72% of its
-// cycles: unpacking codes, not HBM, is what is left there.
+// head_dim 64 21.9 us (86 MB: 3.9 TB/s, 60% of the copy rate; a warp per row
+// took 131 us, a division per code 42 us, index divisions and conversions of
+// codes by instructions of their own 25.5 us), 1333 plain tokens of 8 heads of
+// 128 in f16 8.8 us, 256 tokens 4.4 us.  Instructions, not HBM, are what is
+// left: 290 per 16 elements written, 170 per 8 read back.
 #include <algorithm>
 
 #include "common.cuh"
@@ -28,6 +29,41 @@
 
 namespace psb {
 namespace {
+
+// Division by a divisor of the launch: n / d = (mulhi(n, mul) + n) >> shift for
+// 0 <= n < 2^31, with shift = ceil(log2 d) and mul = floor(2^32 (2^shift - d) / d) + 1
+// (Granlund and Montgomery, Division by invariant integers using multiplication,
+// 1994); 64-bit indices divide.
+struct Divisor {
+  uint32_t d, mul, shift;
+};
+
+Divisor divisor(int64_t d) {
+  Divisor v{static_cast<uint32_t>(d), 0, 0};
+  while ((int64_t(1) << v.shift) < d) ++v.shift;
+  v.mul = static_cast<uint32_t>((((uint64_t(1) << v.shift) - static_cast<uint64_t>(d)) << 32) / static_cast<uint64_t>(d) + 1);
+  return v;
+}
+
+__device__ __forceinline__ int32_t divide(int32_t n, const Divisor& v) {
+  return static_cast<int32_t>((__umulhi(static_cast<uint32_t>(n), v.mul) + static_cast<uint32_t>(n)) >> v.shift);
+}
+__device__ __forceinline__ int64_t divide(int64_t n, const Divisor& v) { return n / v.d; }
+
+// log2 of a power of two, -1 for the rest.
+int log2_exact(int64_t n) {
+  if (n & (n - 1)) return -1;
+  int s = 0;
+  while ((int64_t(1) << s) < n) ++s;
+  return s;
+}
+
+// Pool row of kv (0 K, 1 V) of a slot for head h.
+template <typename P>
+__device__ __forceinline__ int64_t slot_row(const P& p, int64_t slot, int h, int kv) {
+  const int64_t blk = p.block_shift >= 0 ? slot >> p.block_shift : slot / p.block_size;
+  return int4_row(p.layer_tiles + blk * p.hkv + h, kv, static_cast<int>(slot - blk * p.block_size), p.block_size);
+}
 
 struct Int4WriteParams {
   const char* q;  // null without RoPE
@@ -46,7 +82,8 @@ struct Int4WriteParams {
   uint8_t* codes;
   char* params;
   const int64_t* slots;
-  int32_t tokens, hq, hkv, block_size, head_dim;
+  int32_t tokens, hq, hkv, block_size, block_shift, head_dim;
+  Divisor q_div, kv_div;  // pieces of a token's q rows, of its k and v rows (vector kernel)
   int64_t layer_tiles, pool_slots;
   int32_t* err;
 };
@@ -145,9 +182,7 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_kernel(const Int4Wri
     T step, mid;
     int4_row_params<T>(lo, hi, finite, step, mid);
     const float st = Elem<T>::to_float(step), md = Elem<T>::to_float(mid);
-    const int64_t blk = slot / p.block_size;
-    const int64_t row = int4_row(p.layer_tiles + blk * p.hkv + h, role - 1, static_cast<int>(slot - blk * p.block_size),
-                                 p.block_size);
+    const int64_t row = slot_row(p, slot, h, role - 1);
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
       const int j = lane + 32 * i;
@@ -248,11 +283,11 @@ __device__ __forceinline__ void rotate(Piece16<T>& a, Piece16<T>& b, const Piece
 // lanes hold one row.  The q rows of all tokens come first, then the k and v
 // rows, so that a warp's lanes share a path.  (Idx: int32 while every index fits.)
 template <typename T, bool ROPE, typename Idx>
-__global__ void __launch_bounds__(kWriteThreads) int4_write_vec_kernel(const Int4WriteParams p, int pieces) {
+__global__ void __launch_bounds__(kWriteThreads) int4_write_vec_kernel(const Int4WriteParams p, int log_pieces) {
   constexpr int VEC = Piece16<T>::kVec;
   pdl_launch_dependents();
   pdl_wait();
-  const int half = p.head_dim / 2;
+  const int half = p.head_dim / 2, pieces = 1 << log_pieces;
   const Idx q_tok = static_cast<Idx>(ROPE ? p.hq : 0) * pieces, kv_tok = static_cast<Idx>(2 * p.hkv) * pieces;
   const Idx q_total = q_tok * p.tokens, total = q_total + kv_tok * p.tokens;
   const int lane = threadIdx.x & 31;
@@ -261,10 +296,10 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_vec_kernel(const Int
     const Idx i = min(base + lane, total - 1);  // lanes past the end repeat the last piece: same bytes, same place
     const bool is_q = ROPE && i < q_total;
     const Idx u = is_q ? i : i - q_total, per = is_q ? q_tok : kv_tok;
-    const Idx t = u / per;
+    const Idx t = divide(u, is_q ? p.q_div : p.kv_div);
     const int r = static_cast<int>(u - t * per);
-    int h = r / pieces;
-    const int e0 = (r - h * pieces) * VEC;
+    int h = r >> log_pieces;
+    const int e0 = (r & (pieces - 1)) * VEC;
     int role = is_q ? 0 : 1;  // 0 q, 1 k, 2 v
     if (!is_q && h >= p.hkv) {
       role = 2;
@@ -319,9 +354,7 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_vec_kernel(const Int
     T step, mid;
     int4_row_params<T>(lo, hi, bad == 0.f, step, mid);
     const float st = Elem<T>::to_float(step), md = Elem<T>::to_float(mid);
-    const int64_t blk = slot / p.block_size;
-    const int64_t row = int4_row(p.layer_tiles + blk * p.hkv + h, role - 1, static_cast<int>(slot - blk * p.block_size),
-                                 p.block_size);
+    const int64_t row = slot_row(p, slot, h, role - 1);
     uint8_t* dst = p.codes + row * half + e0 / 2;
     const uint32_t ca = piece_codes(a, st, md), cb = piece_codes(b, st, md);
     if constexpr (VEC == 8) {
@@ -347,7 +380,8 @@ struct Int4GatherParams {
   char* v;
   int64_t vst, vsh;  // elements
   const int64_t* slots;
-  int32_t tokens, hkv, block_size, head_dim;
+  int32_t tokens, hkv, block_size, block_shift, head_dim;
+  Divisor tok_div, row_div;  // pieces of a token, of a row (vector kernel)
   int64_t layer_tiles, pool_slots;
   int32_t* err;
 };
@@ -371,9 +405,7 @@ __global__ void __launch_bounds__(kWriteThreads) int4_gather_kernel(const Int4Ga
     if (slot >= p.pool_slots) {
       if (r == 0 && j == 0) flag_error(p.err, PSB_DEVERR_SLOT_RANGE);
     } else if (slot >= 0) {
-      const int64_t blk = slot / p.block_size;
-      const int64_t row = int4_row(p.layer_tiles + blk * p.hkv + h, kv, static_cast<int>(slot - blk * p.block_size),
-                                   p.block_size);
+      const int64_t row = slot_row(p, slot, h, kv);
       const uint32_t c = p.codes[row * pairs + j];
       const T* pr = reinterpret_cast<const T*>(p.params) + row * 2;
       const float st = Elem<T>::to_float(pr[0]), md = Elem<T>::to_float(pr[1]);
@@ -386,19 +418,19 @@ __global__ void __launch_bounds__(kWriteThreads) int4_gather_kernel(const Int4Ga
   }
 }
 
-// One thread per VEC elements of a row.
-template <typename T>
+// One thread per VEC elements of a row.  (Idx: int32 while every index fits.)
+template <typename T, typename Idx>
 __global__ void __launch_bounds__(kWriteThreads) int4_gather_vec_kernel(const Int4GatherParams p) {
   constexpr int VEC = Piece16<T>::kVec;
   pdl_launch_dependents();
   pdl_wait();
   const int pieces = p.head_dim / VEC;
-  const int64_t per_tok = static_cast<int64_t>(2) * p.hkv * pieces, total = per_tok * p.tokens;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(kWriteThreads) + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * kWriteThreads) {
-    const int64_t t = i / per_tok;
-    int r = static_cast<int>(i - t * per_tok);
-    const int hv = r / pieces, e0 = (r - hv * pieces) * VEC;
+  const Idx per_tok = static_cast<Idx>(2) * p.hkv * pieces, total = per_tok * p.tokens;
+  for (Idx i = blockIdx.x * static_cast<Idx>(kWriteThreads) + threadIdx.x; i < total;
+       i += static_cast<Idx>(gridDim.x) * kWriteThreads) {
+    const Idx t = divide(i, p.tok_div);
+    const int r = static_cast<int>(i - t * per_tok);
+    const int hv = divide(r, p.row_div), e0 = (r - hv * pieces) * VEC;
     const int kv = hv >= p.hkv ? 1 : 0, h = hv - kv * p.hkv;
     const int64_t slot = __ldg(p.slots + t);
     Piece16<T> x;
@@ -406,15 +438,13 @@ __global__ void __launch_bounds__(kWriteThreads) int4_gather_vec_kernel(const In
     if (slot >= p.pool_slots) {
       if (r == 0) flag_error(p.err, PSB_DEVERR_SLOT_RANGE);
     } else if (slot >= 0) {
-      const int64_t blk = slot / p.block_size;
-      const int64_t row = int4_row(p.layer_tiles + blk * p.hkv + h, kv, static_cast<int>(slot - blk * p.block_size),
-                                   p.block_size);
+      const int64_t row = slot_row(p, slot, h, kv);
       const uint8_t* src = p.codes + row * (p.head_dim / 2) + e0 / 2;
       const uint32_t w = VEC == 8 ? *reinterpret_cast<const uint32_t*>(src) : *reinterpret_cast<const uint16_t*>(src);
       const T* pr = reinterpret_cast<const T*>(p.params) + row * 2;
       const float st = Elem<T>::to_float(pr[0]), md = Elem<T>::to_float(pr[1]);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) x.e[j] = Elem<T>::from_float(int4_value((w >> (4 * j)) & 15u, st, md));
+      for (int j = 0; j < VEC; ++j) x.e[j] = Elem<T>::from_float(fmaf(st, int4_centered(w, j), md));
     }
     x.store((kv ? reinterpret_cast<T*>(p.v) + t * p.vst + h * p.vsh : reinterpret_cast<T*>(p.k) + t * p.kst + h * p.ksh) + e0);
   }
@@ -466,7 +496,10 @@ int launch_write(const Int4WriteParams& p, cudaStream_t s, int sms) {
     // int32 indices while the last one and a grid stride past it fit
     const auto kern = units + static_cast<int64_t>(sms) * 8 * kWriteThreads < (int64_t(1) << 31)
                           ? int4_write_vec_kernel<T, ROPE, int32_t> : int4_write_vec_kernel<T, ROPE, int64_t>;
-    return launch_stream(kern, wave(reinterpret_cast<const void*>(kern), units, sms), s, p, pieces);
+    Int4WriteParams v = p;
+    v.q_div = divisor(static_cast<int64_t>(std::max(p.hq, 1)) * pieces);
+    v.kv_div = divisor(static_cast<int64_t>(2) * p.hkv * pieces);
+    return launch_stream(kern, wave(reinterpret_cast<const void*>(kern), units, sms), s, v, log2_exact(pieces));
   }
   const auto kern = int4_write_kernel<T, ROPE>;
   return launch_stream(kern, wave(reinterpret_cast<const void*>(kern), rows * 32, sms), s, p);
@@ -477,8 +510,13 @@ int launch_gather(const Int4GatherParams& p, cudaStream_t s, int sms) {
   constexpr int esz = sizeof(T), VEC = Piece16<T>::kVec;
   const int64_t elems = static_cast<int64_t>(p.tokens) * 2 * p.hkv * p.head_dim;
   if (p.head_dim % VEC == 0 && rows16(p.k, p.kst, p.ksh, esz) && rows16(p.v, p.vst, p.vsh, esz)) {
-    const auto kern = int4_gather_vec_kernel<T>;
-    return launch_stream(kern, wave(reinterpret_cast<const void*>(kern), elems / VEC, sms), s, p);
+    const int64_t units = elems / VEC;
+    const auto kern = units + static_cast<int64_t>(sms) * 8 * kWriteThreads < (int64_t(1) << 31)
+                          ? int4_gather_vec_kernel<T, int32_t> : int4_gather_vec_kernel<T, int64_t>;
+    Int4GatherParams v = p;
+    v.row_div = divisor(p.head_dim / VEC);
+    v.tok_div = divisor(static_cast<int64_t>(2) * p.hkv * (p.head_dim / VEC));
+    return launch_stream(kern, wave(reinterpret_cast<const void*>(kern), units, sms), s, v);
   }
   const auto kern = int4_gather_kernel<T>;
   return launch_stream(kern, wave(reinterpret_cast<const void*>(kern), elems / 2, sms), s, p);
@@ -528,6 +566,7 @@ extern "C" int psb_reshape_and_cache_int4(const void* key, int64_t key_stride_t,
   p.tokens = num_tokens;
   p.hkv = num_kv_heads;
   p.block_size = block_size;
+  p.block_shift = log2_exact(block_size);
   p.head_dim = head_dim;
   p.layer_tiles = static_cast<int64_t>(layer) * num_blocks * num_kv_heads;
   p.pool_slots = num_blocks * block_size;
@@ -582,6 +621,7 @@ extern "C" int psb_rope_reshape_and_cache_int4(
   p.hq = num_q_heads;
   p.hkv = num_kv_heads;
   p.block_size = block_size;
+  p.block_shift = log2_exact(block_size);
   p.head_dim = head_dim;
   p.layer_tiles = static_cast<int64_t>(layer) * num_blocks * num_kv_heads;
   p.pool_slots = num_blocks * block_size;
@@ -620,6 +660,7 @@ extern "C" int psb_gather_cache_int4(const void* kv_codes, const void* kv_params
   p.tokens = num_tokens;
   p.hkv = num_kv_heads;
   p.block_size = block_size;
+  p.block_shift = log2_exact(block_size);
   p.head_dim = head_dim;
   p.layer_tiles = static_cast<int64_t>(layer) * num_blocks * num_kv_heads;
   p.pool_slots = num_blocks * block_size;

@@ -54,7 +54,7 @@ int int4_decode_fast_launch(const Int4DecodeParams& p, int dtype, cudaStream_t s
 // scratch bytes and the launch.  q rows start on 16 bytes.
 bool int4_prefill_tc_geometry(int dtype, int total, int num_seqs, int q_heads, int hkv, int head_dim, int block_size,
                               int max_context);
-size_t int4_prefill_tc_workspace();
+size_t int4_prefill_tc_workspace(int total, int num_seqs, int q_heads, int hkv, int max_context);
 int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspace, cudaStream_t s);
 
 }  // namespace psb

@@ -153,7 +153,8 @@ extern "C" size_t psb_paged_prefill_int4_workspace_size(int32_t total_tokens, in
       (dtype != PSB_F32 && dtype != PSB_F16 && dtype != PSB_BF16))
     return 0;
   return int4_prefill_tc_geometry(dtype, total_tokens, num_seqs, q_heads, num_kv_heads, head_dim, block_size, max_context)
-             ? int4_prefill_tc_workspace() : 256;
+             ? int4_prefill_tc_workspace(total_tokens, num_seqs, q_heads, num_kv_heads, max_context)
+             : 256;
 }
 
 extern "C" int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv_codes,

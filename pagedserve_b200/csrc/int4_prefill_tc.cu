@@ -86,7 +86,7 @@ template <typename T>
 constexpr int kStepBits = kStepInV<T> ? 15 : 0;
 constexpr int kMaxCtas = 320;       // grid limit
 constexpr int kPartFloats = kRows * (kDim + 2);
-constexpr int kMaxSeqs = 2048, kMaxTiles = 8192;
+constexpr int kMaxSeqs = 2048, kMaxPairs = 4096;
 
 // What a V stage's 64 tokens need besides their codes and steps.
 struct Extra {
@@ -104,7 +104,7 @@ constexpr uint32_t kOffX = kOffV + kVStages * kKvTile;
 constexpr uint32_t kOffBars = kOffX + kVStages * sizeof(Extra);
 constexpr uint32_t kOffTab = kOffBars + 256;
 
-// A tile cut at a CTA's end that began in it: its kv head, first row of q and
+// A pair cut at a CTA's end that began in it: its kv head, first row of q and
 // tokens, and the last CTA with a piece (0: none).
 struct Cut {
   int32_t kvh, row0, c1, tokens;
@@ -113,11 +113,11 @@ struct Cut {
 struct TcParams {
   Int4PrefillParams a;
   int32_t group, tq;      // q heads per kv head, tokens per tile
-  int32_t max_tiles;      // room for the tile table
+  int32_t max_pairs;      // room for the pair table
   int32_t block_shift;    // block_size is 2^block_shift, or -1
   uint32_t block_div;     // else 2^32 / block_size, rounded up
   int64_t block_rows;     // pool rows from a block to the next
-  float* part;            // workspace: cuts, then two partials per CTA
+  float* part;            // workspace: cuts, then per CTA two pieces of a pair, two tiles each
 };
 
 template <int N>
@@ -200,10 +200,10 @@ struct Plan {
   const int32_t* len;    // [num_seqs] query rows
   const int32_t* ctx;    // [num_seqs] tokens in the pool
   const int32_t* q0;     // [num_seqs] first row
-  const int32_t* tfirst; // [num_seqs + 1] tiles before a sequence
-  const int32_t* sfirst; // [tiles + 1] steps before a tile, of one kv head
-  const int32_t* tseq;   // [tiles] a tile's sequence
-  int32_t tiles;
+  const int32_t* pfirst; // [num_seqs + 1] pairs before a sequence
+  const int32_t* sfirst; // [pairs + 1] steps before a pair, of one kv head
+  const int32_t* pseq;   // [pairs] a pair's sequence
+  int32_t pairs, tq;
 };
 
 __device__ __forceinline__ int last_le(const int32_t* v, int n, int x) {  // last i < n with v[i] <= x
@@ -215,29 +215,31 @@ __device__ __forceinline__ int last_le(const int32_t* v, int n, int x) {  // las
   return lo;
 }
 
-// A run of steps of one tile.
+// A run of steps of one pair of tiles.
 struct Run {
-  int kvh, tile, seq, qt;  // qt: the tile's number in its sequence
-  int j0, n;               // its steps j0 .. j0 + n - 1 of n_kv
+  int kvh, pair, seq, tok0;  // tok0: the pair's first token in its sequence
+  int j0, n;                 // its steps j0 .. j0 + n - 1 of n_kv
   int n_kv;
+  bool two;                  // there is a second tile
 };
 
-// Walks a CTA's steps tile by tile.
+// Walks a CTA's steps pair by pair.
 struct Cursor {
-  int kvh, tile, j0, left;
+  int kvh, pair, j0, left;
   __device__ Run take(const Plan& pl) {  // the next run (left > 0)
     Run s;
     s.kvh = kvh;
-    s.tile = tile;
-    s.seq = pl.tseq[tile];
-    s.qt = tile - pl.tfirst[s.seq];
-    s.n_kv = pl.sfirst[tile + 1] - pl.sfirst[tile];
+    s.pair = pair;
+    s.seq = pl.pseq[pair];
+    s.tok0 = (pair - pl.pfirst[s.seq]) * 2 * pl.tq;
+    s.two = s.tok0 + pl.tq < pl.len[s.seq];
+    s.n_kv = pl.sfirst[pair + 1] - pl.sfirst[pair];
     s.j0 = j0;
     s.n = min(s.n_kv - j0, left);
     left -= s.n;
     j0 = 0;
-    if (++tile == pl.tiles) {
-      tile = 0;
+    if (++pair == pl.pairs) {
+      pair = 0;
       ++kvh;
     }
     return s;
@@ -252,8 +254,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint8_t* const smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
   const Int4PrefillParams& p = tp.a;
   Extra* const ext = reinterpret_cast<Extra*>(smem + kOffX);
-  uint64_t* const bar_q = reinterpret_cast<uint64_t*>(smem + kOffBars);  // [2] Q loaded
-  uint64_t* const bar_k = bar_q + 2;          // [kKStages] K decoded (two warps)
+  uint64_t* const bar_q = reinterpret_cast<uint64_t*>(smem + kOffBars);  // a run's Q loaded
+  uint64_t* const bar_k = bar_q + 1;          // [kKStages] K decoded (two warps)
   uint64_t* const bar_kfree = bar_k + kKStages;  // [kKStages] Q K^T done
   uint64_t* const bar_v = bar_kfree + kKStages;  // [kVStages] V decoded
   uint64_t* const bar_vfree = bar_v + kVStages;  // [kVStages] P V done
@@ -262,16 +264,16 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* const bar_pv = bar_p + 2;         // [2]
   uint64_t* const bar_drain = bar_pv + 2;     // after a failed wait: every product issued so far is done
   uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bar_drain + 1);
-  static_assert((2 + 2 * kKStages + 2 * kVStages + 7) * 8 + 4 <= 256, "barriers fit their area");
+  static_assert((1 + 2 * kKStages + 2 * kVStages + 7) * 8 + 4 <= 256, "barriers fit their area");
   int32_t* const s_len = reinterpret_cast<int32_t*>(smem + kOffTab);
   int32_t* const s_ctx = s_len + p.num_seqs;
   int32_t* const s_q0 = s_ctx + p.num_seqs;
-  int32_t* const s_tfirst = s_q0 + p.num_seqs;
-  int32_t* const s_sfirst = s_tfirst + p.num_seqs + 1;
-  int32_t* const s_tseq = s_sfirst + tp.max_tiles + 1;
+  int32_t* const s_pfirst = s_q0 + p.num_seqs;
+  int32_t* const s_sfirst = s_pfirst + p.num_seqs + 1;
+  int32_t* const s_pseq = s_sfirst + tp.max_pairs + 1;
   __shared__ int32_t warp_sums[kThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int TQ = tp.tq, group = tp.group;
+  const int TQ = tp.tq, group = tp.group, PQ = 2 * TQ;  // tokens of a tile, of a pair
   pdl_wait();  // cu_seqlens, lengths and q may come from the stream predecessor
 
   // ---- the plan: every CTA builds the same tables ------------------------------
@@ -293,11 +295,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     return run;
   };
-  int n_tiles = 0, n_steps = 0;
+  int n_pairs = 0, n_steps = 0;
   {
     const int per = (p.num_seqs + kThreads - 1) / kThreads;
     const int s0 = min(tid * per, p.num_seqs), s1 = min(s0 + per, p.num_seqs);
-    int tiles = 0;
+    int pairs = 0;
     for (int s = s0; s < s1; ++s) {
       const int a = p.cu[s], b = p.cu[s + 1];
       // a malformed batch is reported by the caller's check and read nowhere
@@ -311,28 +313,28 @@ __global__ void __launch_bounds__(kThreads, 2)
       s_len[s] = len;
       s_ctx[s] = ctx;
       s_q0[s] = a;
-      tiles += (len + TQ - 1) / TQ;
+      pairs += (len + PQ - 1) / PQ;
     }
-    int run = scan(tiles, n_tiles);
+    int run = scan(pairs, n_pairs);
     for (int s = s0; s < s1; ++s) {
-      s_tfirst[s] = run;
-      run += (s_len[s] + TQ - 1) / TQ;
+      s_pfirst[s] = run;
+      run += (s_len[s] + PQ - 1) / PQ;
     }
-    if (tid == 0) s_tfirst[p.num_seqs] = n_tiles;
+    if (tid == 0) s_pfirst[p.num_seqs] = n_pairs;
     __syncthreads();
-    if (n_tiles > tp.max_tiles) {  // rows named by two sequences: a malformed batch
+    if (n_pairs > tp.max_pairs) {  // rows named by two sequences: a malformed batch
       if (tid == 0) flag_error(p.err, PSB_DEVERR_SEQLENS);
-      n_tiles = 0;
+      n_pairs = 0;
     }
-    const int tper = (n_tiles + kThreads - 1) / kThreads;
-    const int t0 = min(tid * tper, n_tiles), t1 = min(t0 + tper, n_tiles);
+    const int tper = (n_pairs + kThreads - 1) / kThreads;
+    const int t0 = min(tid * tper, n_pairs), t1 = min(t0 + tper, n_pairs);
     int steps = 0;
     for (int t = t0; t < t1; ++t) {
-      const int s = last_le(s_tfirst, p.num_seqs, t), qt = t - s_tfirst[s];
-      // keys 0 .. position of the tile's last row
-      const int n = (s_ctx[s] - s_len[s] + min(s_len[s], (qt + 1) * TQ) + kBN - 1) / kBN;
+      const int s = last_le(s_pfirst, p.num_seqs, t), qt = t - s_pfirst[s];
+      // keys 0 .. position of the pair's last row
+      const int n = (s_ctx[s] - s_len[s] + min(s_len[s], (qt + 1) * PQ) + kBN - 1) / kBN;
       s_sfirst[t] = n;
-      s_tseq[t] = s;
+      s_pseq[t] = s;
       steps += n;
     }
     run = scan(steps, n_steps);
@@ -341,10 +343,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       s_sfirst[t] = run;
       run += n;
     }
-    if (tid == 0) s_sfirst[n_tiles] = n_steps;
+    if (tid == 0) s_sfirst[n_pairs] = n_steps;
     __syncthreads();
   }
-  const Plan plan{s_len, s_ctx, s_q0, s_tfirst, s_sfirst, s_tseq, n_tiles};
+  const Plan plan{s_len, s_ctx, s_q0, s_pfirst, s_sfirst, s_pseq, n_pairs, TQ};
   const uint32_t total_steps = static_cast<uint32_t>(n_steps) * p.hkv;  // below 2^31
   const uint32_t act = min(gridDim.x, total_steps);
   Cut* const cuts = reinterpret_cast<Cut*>(tp.part);
@@ -361,14 +363,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   Cursor first;
   first.kvh = static_cast<int>(my_a / n_steps);
   first.j0 = static_cast<int>(my_a - static_cast<uint32_t>(first.kvh) * n_steps);
-  first.tile = last_le(s_sfirst, n_tiles, first.j0);
-  first.j0 -= s_sfirst[first.tile];
+  first.pair = last_le(s_sfirst, n_pairs, first.j0);
+  first.j0 -= s_sfirst[first.pair];
   first.left = n_mine;
   const uint32_t s_base = smem_u32(smem);
 
   if (tid == 0) {
+    mbar_init(bar_q, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar_q + i, 1);
       mbar_init(bar_s + i, 1);
       mbar_init(bar_p + i, 128);
       mbar_init(bar_pv + i, 1);
@@ -407,78 +409,101 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint64_t dk = umma_desc_sw128(s_base + kOffK, 1024, 16);
         const uint64_t dv = umma_desc_sw128(s_base + kOffV, 1024, 8192);
         prefetch_tmap(&tm_q);
-        Cursor qc = first, sc = first, oc = first;  // Q loads, S and O
-        int q_req = 0, q_seen = 0;
-        auto load_q = [&]() {  // the next run's rows into buffer q_req & 1
-          const Run s = qc.take(plan);
-          const int b = q_req & 1;
-          mbar_arrive_expect_tx(bar_q + b, static_cast<uint32_t>(TQ * group) * kDim * 2);
-          tma_load_3d(smem + b * kQTile, &tm_q, 0, s.kvh * group, plan.q0[s.seq] + s.qt * TQ, bar_q + b);
-          ++q_req;
-        };
-        int s_left = 0, o_left = 0, o_run = -1;
-        bool want_q = true;
+        // Half-steps (a step of one tile), in order: a step's first tile, its
+        // second.  Number i uses S buffer i & 1.  S runs two half-steps ahead of O.
+        Cursor sc = first, oc = first;
+        Run sr{}, orun{};
+        int s_left = 0, o_left = 0, sg = 0, og = 0, sh = 0, oh = 0;  // steps left of a run, step, tile
+        int runs = 0, q_wait = 0;     // Q loads asked for, and seen
+        bool s_more = true;           // (n_mine > 0)
 #pragma unroll 1
-        for (int g = 0; g <= n_mine; ++g) {
-          while (want_q && qc.left > 0) {  // the first two runs, then one after each run's end
-            load_q();
-            want_q = q_req < 2;
-          }
-          want_q = false;
-          if (g < n_mine) {  // S of step g
-            if (s_left == 0) {
-              s_left = sc.take(plan).n;
-              if (!wait(bar_q + (q_seen & 1), (q_seen >> 1) & 1)) {
+        for (int i = -2;; ++i) {
+          if (i >= 0) {  // P V of half-step i
+            if (oh == 0) {
+              if (o_left == 0) {
+                if (oc.left == 0) break;
+                orun = oc.take(plan);
+                o_left = orun.n;
+              }
+              if (!wait(bar_v + og % kVStages, (og / kVStages) & 1)) {
                 fail = true;
                 break;
               }
-              ++q_seen;
             }
-            const int st = g % kKStages;
-            // S buffer g & 1 held S and then P of step g - 2
-            if ((g >= 2 && !wait(bar_pv + (g & 1), ((g - 2) >> 1) & 1)) || !wait(bar_k + st, (g / kKStages) & 1)) {
+            if (!wait(bar_p + (i & 1), (i >> 1) & 1)) {
               fail = true;
               break;
             }
             tc_fence_after();
-            const uint64_t dqs = dq + static_cast<uint64_t>(((q_seen - 1) & 1) * (kQTile >> 4));
-            const uint64_t dks = dk + static_cast<uint64_t>(st * (2 * kKvTile >> 4));
-#pragma unroll
-            for (int kk = 0; kk < 2 * kDim / 16; ++kk)  // the values rounded to T, then their rests
-              umma_f16_ss(tmem + kSCol + (g & 1) * kBN, dqs + 2 * (kk & 3), dks + (kk >> 2) * (kKvTile >> 4) + 2 * (kk & 3),
-                          idesc_s, kk > 0);
-            umma_commit(bar_s + (g & 1));
-            umma_commit(bar_kfree + st);
-            --s_left;
-          }
-          if (g > 0) {  // P V of step g - 1
-            const int h = g - 1, st = h % kVStages;
-            const bool begins = o_left == 0;
-            if (begins) {
-              o_left = oc.take(plan).n;
-              ++o_run;
-            }
-            if (!wait(bar_p + (h & 1), (h >> 1) & 1) || !wait(bar_v + st, (h / kVStages) & 1)) {
-              fail = true;
-              break;
-            }
-            tc_fence_after();
-            const uint32_t obuf = tmem + kOCol + (o_run & 1) * kDim;
-            const uint64_t dvs = dv + static_cast<uint64_t>(st * (kKvTile >> 4));
-            const uint32_t pcol = tmem + kSCol + (h & 1) * kBN;
+            const uint64_t dvs = dv + static_cast<uint64_t>((og % kVStages) * (kKvTile >> 4));
+            const uint32_t pcol = tmem + kSCol + (i & 1) * kBN, ocol = tmem + kOCol + oh * kDim;
+            const bool begins = o_left == orun.n;
 #pragma unroll
             for (int kk = 0; kk < kBN / 16; ++kk)
-              umma_f16_ts(obuf, pcol + 8 * kk, dvs + 128 * kk, idesc_o, !begins || kk > 0);
-            umma_commit(bar_pv + (h & 1));
-            umma_commit(bar_vfree + st);
-            // at a run's end the softmax has read its last S: its Q may be overwritten
-            want_q = --o_left == 0;
+              umma_f16_ts(ocol, pcol + 8 * kk, dvs + 128 * kk, idesc_o, !begins || kk > 0);
+            umma_commit(bar_pv + (i & 1));
+            if (oh == (orun.two ? 1 : 0)) {
+              umma_commit(bar_vfree + og % kVStages);
+              oh = 0;
+              ++og;
+              --o_left;
+            } else {
+              oh = 1;
+            }
+          }
+          if (s_more) {  // S of half-step i + 2, whose buffer held S and then P of half-step i
+            if (i >= 0 && !wait(bar_pv + (i & 1), (i >> 1) & 1)) {
+              fail = true;
+              break;
+            }
+            if (sh == 0) {
+              if (s_left == 0) {  // a run begins: its Q, once the last S of the run before is done
+                sr = sc.take(plan);
+                s_left = sr.n;
+                if (i >= -1 && !wait(bar_s + ((i + 1) & 1), ((i + 1) >> 1) & 1)) {
+                  fail = true;
+                  break;
+                }
+                const uint32_t bytes = static_cast<uint32_t>(TQ * group) * kDim * 2;
+                mbar_arrive_expect_tx(bar_q, sr.two ? 2 * bytes : bytes);
+                const int row0 = plan.q0[sr.seq] + sr.tok0;
+                tma_load_3d(smem, &tm_q, 0, sr.kvh * group, row0, bar_q);
+                if (sr.two) tma_load_3d(smem + kQTile, &tm_q, 0, sr.kvh * group, row0 + TQ, bar_q);
+                ++runs;
+                if (!wait(bar_q, (runs - 1) & 1)) {
+                  fail = true;
+                  break;
+                }
+                q_wait = runs;
+              }
+              if (!wait(bar_k + sg % kKStages, (sg / kKStages) & 1)) {
+                fail = true;
+                break;
+              }
+            }
+            tc_fence_after();
+            const uint64_t dqs = dq + static_cast<uint64_t>(sh * (kQTile >> 4));
+            const uint64_t dks = dk + static_cast<uint64_t>((sg % kKStages) * (2 * kKvTile >> 4));
+#pragma unroll
+            for (int kk = 0; kk < 2 * kDim / 16; ++kk)  // the values rounded to T, then their rests
+              umma_f16_ss(tmem + kSCol + (i & 1) * kBN, dqs + 2 * (kk & 3), dks + (kk >> 2) * (kKvTile >> 4) + 2 * (kk & 3),
+                          idesc_s, kk > 0);
+            umma_commit(bar_s + (i & 1));
+            if (sh == (sr.two ? 1 : 0)) {
+              umma_commit(bar_kfree + sg % kKStages);
+              sh = 0;
+              ++sg;
+              --s_left;
+              s_more = s_left > 0 || sc.left > 0;
+            } else {
+              sh = 1;
+            }
           }
         }
         if (fail) {
           flag_error(p.err, PSB_DEVERR_TIMEOUT);
           // let the copies and products in flight land before shared memory and TMEM are released
-          for (int t = q_seen; t < q_req; ++t) (void)wait(bar_q + (t & 1), (t >> 1) & 1);
+          if (q_wait < runs) (void)wait(bar_q, (runs - 1) & 1);
           umma_commit(bar_drain);
           (void)wait(bar_drain, 0);
         }
@@ -681,55 +706,52 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int rtok = row / group, rhead = row - rtok * group;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(warp * 32) << 16);
     const bool out16 = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ost % 8 == 0 && p.osh % 8 == 0;
+    // Per tile: the exponents' reference; sums of 2^kPBits p and p mid; the last
+    // key of this row, from the step's first.  The tile at work is in the plain
+    // names, the other in the rest; a step's end swaps them.
+    float ref = 0.f, l = 0.f, z = 0.f, ref_o = 0.f, l_o = 0.f, z_o = 0.f;
+    int last = 0, last_o = 0, vexp = 0, vexp_o = 0;
+    bool fresh = true, fresh_o = true;
+    auto swap_tiles = [&]() {
+      auto sw = [](auto& a, auto& b) {
+        auto c = a;
+        a = b;
+        b = c;
+      };
+      sw(ref, ref_o);
+      sw(l, l_o);
+      sw(z, z_o);
+      sw(last, last_o);
+      sw(vexp, vexp_o);
+      sw(fresh, fresh_o);
+    };
     Cursor cc = first;
     Run s{};
-    int left = 0, k = -1;          // steps left of run s, its number
-    int last = 0;                  // last key of this row, from the step's first
-    uint32_t t_o = 0;
-    float ref = 0.f, l = 0.f, z = 0.f;  // the exponents' reference; sums of 2^kPBits p and p mid
-    bool fresh = true;
-    int vexp = 0;
-    // A run's output is written after the next run's first step (or at the
-    // end): by then its last P V is normally done.
-    bool pending = false;
-    int pend_exp = 0;
-    float pend_l = 0.f, pend_z = 0.f, pend_m = 0.f;
-    Run pend{};
+    int g = 0, i = 0;  // step, half-step
 #pragma unroll 1
-    for (int g = 0;; ++g) {
-      if (left == 0) {
-        if (g > 0) {
-          pending = true;
-          pend = s;
-          pend_l = l * kPUnit;
-          pend_z = z;
-          pend_exp = vexp;
-          pend_m = fresh ? -INFINITY : ref;
-        }
-        if (g < n_mine) {
-          s = cc.take(plan);
-          left = s.n;
-          ++k;
-          const int tok = s.qt * TQ + rtok, len = plan.len[s.seq];
-          // rows past the tile's tokens are not written: they need no mask
-          last = (rtok < TQ && tok < len ? plan.ctx[s.seq] - len + tok : INT_MAX) - s.j0 * kBN;
-          t_o = t_lane + kOCol + (k & 1) * kDim;
-          ref = l = z = 0.f;
-          fresh = true;
-          vexp = 0;
-        }
-      }
-      if (g < n_mine) {
-        const int st = g % kVStages;
-        if (!warp_wait(bar_s + (g & 1), (g >> 1) & 1) || !warp_wait(bar_v + st, (g / kVStages) & 1)) {
+    while (cc.left > 0 && !fail) {
+      s = cc.take(plan);
+      const int tiles = s.two ? 2 : 1, len = plan.len[s.seq], start = plan.ctx[s.seq] - len - s.j0 * kBN;
+      // rows past a tile's tokens are not written: they need no mask
+      const int tok = s.tok0 + rtok;
+      last = rtok < TQ && tok < len ? start + tok : INT_MAX;
+      last_o = rtok < TQ && tok + TQ < len ? start + tok + TQ : INT_MAX;
+      ref = l = z = ref_o = l_o = z_o = 0.f;
+      fresh = fresh_o = true;
+      vexp = vexp_o = 0;
+#pragma unroll 1
+      for (int hs = 0; hs < s.n * tiles; ++hs, ++i) {
+        const int h = s.two ? hs & 1 : 0, st = g % kVStages;
+        if (!warp_wait(bar_s + (i & 1), (i >> 1) & 1) || (h == 0 && !warp_wait(bar_v + st, (g / kVStages) & 1))) {
           fail = true;
           break;
         }
         tc_fence_after();
+        const uint32_t t_s = t_lane + kSCol + (i & 1) * kBN, t_o = t_lane + kOCol + h * kDim;
         const Extra& f = ext[st];
         uint32_t sr[kBN];
-        tmem_ld32(t_lane + kSCol + (g & 1) * kBN, sr);
-        tmem_ld32(t_lane + kSCol + (g & 1) * kBN + 32, sr + 32);
+        tmem_ld32(t_s, sr);
+        tmem_ld32(t_s + 32, sr + 32);
         tmem_wait_ld();
         // exponents: scores minus reference, plus kPBits
         const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), nref2 = f2_pack(kPBits - ref, kPBits - ref);
@@ -759,13 +781,14 @@ __global__ void __launch_bounds__(kThreads, 2)
         // limit, or at its first score; O is rescaled then, or when the scale
         // of V's steps changed.  The warp's TMEM access is collective.
         const int ve = f.vexp;
-        const bool begins = left == s.n;
+        const bool begins = hs < tiles;
         const bool grow = mx > (fresh ? -INFINITY : kGrowth + kPBits);
         if (__any_sync(0xffffffffu, grow) || (!begins && ve != vexp)) {
           const float up = grow ? fminf(fmaxf(mx - kPBits, -3e38f), 3e38f) : 0.f;
           const float al = grow ? (fresh ? 0.f : ex2_approx(-up)) : 1.f;
           if (!begins) {  // O holds P V of the earlier steps once the last of them is done
-            if (!warp_wait(bar_pv + ((g - 1) & 1), ((g - 1) >> 1) & 1)) {
+            const int before = i - tiles;  // the tile's last half-step
+            if (!warp_wait(bar_pv + (before & 1), (before >> 1) & 1)) {
               fail = true;
               break;
             }
@@ -816,75 +839,76 @@ __global__ void __launch_bounds__(kThreads, 2)
         z += zf.x + zf.y;
         // a token that stands for NaN: for the rows that see it
         if (((f.nan[0] & seen0) | (f.nan[1] & seen1)) != 0) z = __int_as_float(0x7fffffff);
-        tmem_st32(t_lane + kSCol + (g & 1) * kBN, pk);
+        tmem_st32(t_s, pk);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(bar_p + (g & 1));
+        mbar_arrive(bar_p + (i & 1));
+        last -= kBN;
+        if (h == tiles - 1) ++g;
+        if (s.two) swap_tiles();
       }
-      if (pending) {
-        const int pg = min(g, n_mine) - 1;  // the run's last step
-        if (!warp_wait(bar_pv + (pg & 1), (pg >> 1) & 1)) {
+      // the run's output, a tile at a time
+      const bool whole = s.n == s.n_kv;
+#pragma unroll 1
+      for (int h = 0; h < tiles && !fail; ++h) {
+        const int at = i - tiles + h;  // the tile's last half-step
+        if (!warp_wait(bar_pv + (at & 1), (at >> 1) & 1)) {
           fail = true;
           break;
         }
         tc_fence_after();
-        pending = false;
-        // run k is under way, or it is the one that has ended
-        const uint32_t t_po = t_lane + kOCol + ((g < n_mine ? k - 1 : k) & 1) * kDim;
-        const bool whole = pend.j0 == 0 && pend.n == pend.n_kv;
-        const int tok = pend.qt * TQ + rtok;
-        const bool live = rtok < TQ && tok < plan.len[pend.seq];
-        const float back = exp2_int(max(-126, min(127, pend_exp - kStepBits<T> + kVBits - kPBits)));  // of one unit of O
-        const float inv = !whole ? 1.f : pend_l == 0.f ? 0.f : 1.f / pend_l;
-        const float scale = back * inv, base = pend_z * inv;
-        float* const dst = part + static_cast<int64_t>(2 * cta + (pend.j0 > 0 ? 0 : 1)) * kPartFloats;
-        T* const out = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(plan.q0[pend.seq] + tok) * p.ost +
-                       static_cast<int64_t>(pend.kvh * group + rhead) * p.osh;
+        const int tok_h = tok + h * TQ;
+        const bool live = rtok < TQ && tok_h < len;
+        const float back = exp2_int(max(-126, min(127, vexp - kStepBits<T> + kVBits - kPBits)));  // of one unit of O
+        const float sum = l * kPUnit;
+        const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+        const float scale = back * inv, base = z * inv;
+        float* const dst = part + static_cast<int64_t>(4 * cta + (s.j0 > 0 ? 0 : 2) + h) * kPartFloats;
+        T* const out = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(plan.q0[s.seq] + tok_h) * p.ost +
+                       static_cast<int64_t>(s.kvh * group + rhead) * p.osh;
 #pragma unroll 1
-        for (int h = 0; h < 4; ++h) {
+        for (int q = 0; q < 4; ++q) {
           uint32_t ot[16];
-          tmem_ld16(t_po + 16 * h, ot);
+          tmem_ld16(t_lane + kOCol + h * kDim + 16 * q, ot);
           tmem_wait_ld();
           float o[16];
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // columns 2 i, 2 i + 1 of a word are its elements i, i + 4
-              o[8 * w + i] = fmaf(__uint_as_float(ot[8 * w + 2 * i]), scale, base);
-              o[8 * w + i + 4] = fmaf(__uint_as_float(ot[8 * w + 2 * i + 1]), scale, base);
+            for (int e = 0; e < 4; ++e) {  // columns 2 e, 2 e + 1 of a word are its elements e, e + 4
+              o[8 * w + e] = fmaf(__uint_as_float(ot[8 * w + 2 * e]), scale, base);
+              o[8 * w + e + 4] = fmaf(__uint_as_float(ot[8 * w + 2 * e + 1]), scale, base);
             }
           }
           if (live && !whole) {
 #pragma unroll
             for (int d = 0; d < 16; d += 4)
-              *reinterpret_cast<float4*>(dst + row * kDim + 16 * h + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+              *reinterpret_cast<float4*>(dst + row * kDim + 16 * q + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
           } else if (live && out16) {
 #pragma unroll
             for (int d = 0; d < 16; d += 8)
-              *reinterpret_cast<uint4*>(out + 16 * h + d) = make_uint4(pack2<T>(o[d], o[d + 1]), pack2<T>(o[d + 2], o[d + 3]),
+              *reinterpret_cast<uint4*>(out + 16 * q + d) = make_uint4(pack2<T>(o[d], o[d + 1]), pack2<T>(o[d + 2], o[d + 3]),
                                                                        pack2<T>(o[d + 4], o[d + 5]), pack2<T>(o[d + 6], o[d + 7]));
           } else if (live) {
 #pragma unroll
-            for (int d = 0; d < 16; ++d) out[16 * h + d] = Elem<T>::from_float(o[d]);
+            for (int d = 0; d < 16; ++d) out[16 * q + d] = Elem<T>::from_float(o[d]);
           }
           __syncwarp();  // the next read of TMEM is the whole warp's
         }
-        if (!whole) *reinterpret_cast<float2*>(dst + kRows * kDim + 2 * row) = make_float2(pend_m, pend_l);
-        tc_fence_before();
+        if (!whole) *reinterpret_cast<float2*>(dst + kRows * kDim + 2 * row) = make_float2(fresh ? -INFINITY : ref, sum);
+        if (s.two) swap_tiles();
       }
-      if (g >= n_mine) break;
-      --left;
-      last -= kBN;
+      tc_fence_before();  // the next run's first P V comes after its P
     }
     if (fail && lane == 0) flag_error(p.err, PSB_DEVERR_TIMEOUT);
     if (warp == 0) {
-      // the tile that begins here and runs past the CTA's end, if any: the last run
+      // the pair that begins here and runs past the CTA's end, if any: the last run
       Cut c{0, 0, 0, 0};
-      const uint32_t t_a = my_e - static_cast<uint32_t>(s.j0 + s.n), t_e = t_a + static_cast<uint32_t>(s.n_kv);
+      const uint32_t t_e = my_e - static_cast<uint32_t>(s.j0 + s.n) + static_cast<uint32_t>(s.n_kv);
       if (!fail && s.j0 == 0 && t_e > my_e) {
         c.kvh = s.kvh;
-        c.row0 = s_q0[s.seq] + s.qt * TQ;
-        c.tokens = min(TQ, s_len[s.seq] - s.qt * TQ);
+        c.row0 = s_q0[s.seq] + s.tok0;
+        c.tokens = min(PQ, s_len[s.seq] - s.tok0);
         c.c1 = static_cast<int32_t>(cta);
         for (uint32_t c0 = cta + 1; c0 < act; c0 += 32) {  // CTAs that start before its end
           const bool in = c0 + lane < act && cta_start(min(c0 + lane, act)) < t_e;
@@ -904,8 +928,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// Joins the partials of the tile that CTA blockIdx.x left cut at its end: a
-// quarter of the tile's rows per CTA, kWarpRows rows per warp, two elements a
+// Joins the partials of the pair that CTA blockIdx.x left cut at its end: a
+// quarter of a tile's rows per CTA, kWarpRows rows per warp, two elements a
 // lane, kBatch partials in flight.
 constexpr int kCombineRows = 32, kWarpRows = kCombineRows / (kThreads / 32), kBatch = 4;
 
@@ -916,10 +940,11 @@ __global__ void __launch_bounds__(kThreads) int4_prefill_combine_kernel(const Tc
   pdl_launch_dependents();
   const int c0 = blockIdx.x, lane = threadIdx.x & 31;
   const int4 cut = __ldcg(reinterpret_cast<const int4*>(tp.part) + c0);
-  const int row0 = blockIdx.y * kCombineRows + (threadIdx.x >> 5) * kWarpRows;
-  if (cut.z <= c0 || row0 >= cut.w * tp.group) return;
+  const int tile = blockIdx.y / (kRows / kCombineRows), tokens = cut.w - tile * tp.tq;  // tokens from the tile's first on
+  const int row0 = (blockIdx.y % (kRows / kCombineRows)) * kCombineRows + (threadIdx.x >> 5) * kWarpRows;
+  if (cut.z <= c0 || row0 >= min(tokens, tp.tq) * tp.group) return;
   const float* const part = tp.part + kMaxCtas * (sizeof(Cut) / sizeof(float));
-  auto piece_of = [&](int c) { return part + static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * kPartFloats; };
+  auto piece_of = [&](int c) { return part + static_cast<int64_t>(4 * c + (c == c0 ? 2 : 0) + tile) * kPartFloats; };
   float m[kWarpRows], l[kWarpRows];
   float2 o[kWarpRows];
 #pragma unroll
@@ -965,20 +990,26 @@ __global__ void __launch_bounds__(kThreads) int4_prefill_combine_kernel(const Tc
 #pragma unroll
   for (int r = 0; r < kWarpRows; ++r) {
     const int rtok = (row0 + r) / tp.group, rhead = row0 + r - rtok * tp.group;
-    if (rtok >= cut.w) continue;
+    if (rtok >= min(tokens, tp.tq)) continue;
     const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-    T* out = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(cut.y + rtok) * p.ost +
+    T* out = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(cut.y + tile * tp.tq + rtok) * p.ost +
              static_cast<int64_t>(cut.x * tp.group + rhead) * p.osh + 2 * lane;
     out[0] = Elem<T>::from_float(o[r].x * inv);
     out[1] = Elem<T>::from_float(o[r].y * inv);
   }
 }
 
-size_t tc_smem(int num_seqs, int max_tiles) {
-  return 1024 + kOffTab + sizeof(int32_t) * (4 * static_cast<size_t>(num_seqs) + 1 + 2 * static_cast<size_t>(max_tiles) + 1);
+size_t tc_smem(int num_seqs, int max_pairs) {
+  return 1024 + kOffTab + sizeof(int32_t) * (4 * static_cast<size_t>(num_seqs) + 1 + 2 * static_cast<size_t>(max_pairs) + 1);
 }
 
-int64_t tiles_bound(int total, int num_seqs, int tq) { return static_cast<int64_t>(total) / tq + num_seqs; }
+int64_t pairs_bound(int total, int num_seqs, int tq) { return static_cast<int64_t>(total) / (2 * tq) + num_seqs; }
+
+// An upper bound of the CTAs: of the steps, or the grid's limit.
+int64_t ctas_bound(int total, int num_seqs, int tq, int hkv, int max_context) {
+  return std::min<int64_t>(std::max<int64_t>(1, pairs_bound(total, num_seqs, tq) * hkv * ((max_context + kBN - 1) / kBN)),
+                           kMaxCtas);
+}
 
 }  // namespace
 
@@ -986,19 +1017,23 @@ bool int4_prefill_tc_geometry(int dtype, int total, int num_seqs, int q_heads, i
                               int max_context) {
   const int group = q_heads / hkv;
   if (!(dtype == PSB_BF16 || dtype == PSB_F16) || head_dim != kDim || group > kRows) return false;
-  return num_seqs <= kMaxSeqs && tiles_bound(total, num_seqs, kRows / group) <= kMaxTiles &&
+  const int64_t pairs = pairs_bound(total, num_seqs, kRows / group);
+  return num_seqs <= kMaxSeqs && pairs <= kMaxPairs &&
          static_cast<int64_t>(max_context + kBN) * block_size < (int64_t(1) << 32) &&
-         tiles_bound(total, num_seqs, kRows / group) * (max_context / kBN + 1) < (int64_t(1) << 31) / hkv;
+         pairs * (max_context / kBN + 1) < (int64_t(1) << 31) / hkv;
 }
 
-size_t int4_prefill_tc_workspace() { return sizeof(Cut) * kMaxCtas + sizeof(float) * 2 * kMaxCtas * kPartFloats; }
+size_t int4_prefill_tc_workspace(int total, int num_seqs, int q_heads, int hkv, int max_context) {
+  return sizeof(Cut) * kMaxCtas +
+         sizeof(float) * 4 * kPartFloats * static_cast<size_t>(ctas_bound(total, num_seqs, kRows / (q_heads / hkv), hkv, max_context));
+}
 
 int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspace, cudaStream_t s) {
   TcParams tp;
   tp.a = p;
   tp.group = p.hq / p.hkv;
   tp.tq = kRows / tp.group;
-  tp.max_tiles = static_cast<int32_t>(tiles_bound(p.total, p.num_seqs, tp.tq));
+  tp.max_pairs = static_cast<int32_t>(pairs_bound(p.total, p.num_seqs, tp.tq));
   tp.block_shift = -1;
   if ((p.block_size & (p.block_size - 1)) == 0)
     for (tp.block_shift = 0; (1 << tp.block_shift) < p.block_size;) ++tp.block_shift;
@@ -1013,7 +1048,7 @@ int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspa
   if (sms <= 0) return PSB_ERR_CUDA;
   const auto kern = dtype == PSB_BF16 ? int4_prefill_tc_kernel<__nv_bfloat16> : int4_prefill_tc_kernel<__half>;
   const auto comb = dtype == PSB_BF16 ? int4_prefill_combine_kernel<__nv_bfloat16> : int4_prefill_combine_kernel<__half>;
-  const size_t smem = tc_smem(p.num_seqs, tp.max_tiles);
+  const size_t smem = tc_smem(p.num_seqs, tp.max_pairs);
   // the register split draws on what the block was launched with
   static_assert(168 + 88 == 2 * 128, "two warpgroups' shares");
   static std::atomic<bool> checked[2];  // per element type
@@ -1026,14 +1061,13 @@ int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspa
   }
   int occ = 0;
   if (!kernel_occupancy(reinterpret_cast<const void*>(kern), kThreads, smem, &occ) || occ < 1) return PSB_ERR_CUDA;
-  // an upper bound of the steps
-  const int64_t steps = static_cast<int64_t>(tp.max_tiles) * p.hkv * ((p.max_context + kBN - 1) / kBN);
-  const int64_t grid = std::min<int64_t>(std::min<int64_t>(steps, kMaxCtas), static_cast<int64_t>(sms) * std::min(occ, 2));
+  const int64_t grid = std::min<int64_t>(ctas_bound(p.total, p.num_seqs, tp.tq, p.hkv, p.max_context),
+                                         static_cast<int64_t>(sms) * std::min(occ, 2));
   discard_stale_error();
   cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, s, tp, tq);
   if (e != cudaSuccess) return record_cuda_error(e);
   if (grid > 1) {
-    e = launch_pdl(comb, dim3(static_cast<unsigned>(grid - 1), kRows / kCombineRows), dim3(kThreads), 0, s, tp);
+    e = launch_pdl(comb, dim3(static_cast<unsigned>(grid - 1), 2 * kRows / kCombineRows), dim3(kThreads), 0, s, tp);
     if (e != cudaSuccess) return record_cuda_error(e);
   }
   return check_launch();

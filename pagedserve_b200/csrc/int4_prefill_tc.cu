@@ -18,41 +18,42 @@
 //
 // Tiles.  The q heads of a kv head read the same keys, so a tile's 128 rows
 // are TQ = 128 / group consecutive tokens times the group's heads (one TMA box
-// of [TQ, group, 64]): a short chunk of few tokens still fills a tile, and
-// each key tile is decoded once for all heads of the group.  A step is 64 keys.
-// The steps of all tiles, in (kv head, tile, step) order, are dealt evenly over
-// a persistent grid of two CTAs per SM; a tile cut by a CTA boundary leaves
-// fp32 partials that int4_prefill_combine_kernel joins (a single chunk on a
-// long prefix has fewer tiles than the GPU has SMs).
+// of [TQ, group, 64]): a short chunk of few tokens still fills a tile.  Two
+// consecutive tiles of a sequence make a pair and share each step's 64 decoded
+// keys.  The steps of all pairs, in (kv head, pair, step) order, are dealt
+// evenly over a persistent grid of two CTAs per SM; a pair cut by a CTA
+// boundary leaves fp32 partials that int4_prefill_combine_kernel joins (a single
+// chunk on a long prefix has fewer pairs than the GPU has SMs).
 //
 // CTA: eight warps.  Warps 0-3 are the softmax (thread r = TMEM lane r = row r
-// of the tile).  In warps 4-7 one lane issues the Q loads and the products -
-// S = Q K^T (eight tcgen05.mma M 128 N 64 K 16, two TMEM S buffers) a step
-// ahead of O += P V (P read from TMEM over the S it came from, two O buffers
-// in turn) - and three warps decode: 32 keys each for K, all 64 for V, into
-// rings of shared-memory stages (128-byte swizzle).  The four roles are turned
-// by one warp in the second half of the grid, which spreads the decoding of an
-// SM's two CTAs over its schedulers.  The softmax half has 168 registers, the
-// other 88 (setmaxnreg; 256 x 128 at launch).
+// of a tile), which takes the two tiles of a step in turn: half-steps.  In
+// warps 4-7 one lane issues the Q loads and the products - S = Q K^T (eight
+// tcgen05.mma M 128 N 64 K 16) two half-steps ahead of O += P V (P read from TMEM
+// over the S it came from; two S buffers in turn, one O per tile) - and three
+// warps decode: 32 keys each for K, all 64 for V, into rings of shared-memory
+// stages (128-byte swizzle).  The four roles are turned by one warp in the
+// second half of the grid, which spreads the decoding of an SM's two CTAs over
+// its schedulers.  The softmax half has 160 registers, the other 96 (setmaxnreg;
+// 256 x 128 at launch).
 //
 // Four roles share an SM's instruction caches, so every loop has one body:
 // the same kernel with its loops unrolled and peeled (121 KB of code) spent
 // more issue slots waiting for instructions than on anything else.
 //
-// What bounds it: instructions.  A step of one CTA is 3600 of them (softmax
-// 1300, K 1100, V 550, issue and waits the rest) and takes some 3300 cycles at
-// two CTAs an SM, half of the issue slots; the exponentials take 27% of their
-// pipe, the tensor pipe is 20% busy.  512 tokens on 8 K: 61 us (paged_prefill
-// over a 16-bit pool: 152 us), of which 20 us do not depend on the context
-// (plan, first look-ups, join); six chunks of 1 K: 135 us (181 us); 32 requests
-// of 5 tokens: 21.5 us (61 us).  Tried without gain: twelve warps (two threads
-// per row, or twice the decoding warps), a third S buffer, one warp per kind
-// of product, a join over the cut tiles only, the set-up before the wait for
-// the predecessor.
+// What bounds it: the softmax's chain (wait, TMEM, scale, maximum, exponentials,
+// TMEM: some 2400 cycles a half-step, at two warps a scheduler), then V's
+// decoding (3300 a step); half of the issue slots are used, the exponentials
+// take 31% of their pipe.  With one tile a step, V's decoding bounded it and 512
+// tokens on 32 K took 200 us where this takes 160.  512 tokens on 8 K: 59 us
+// (paged_prefill over a 16-bit pool: 152 us), of which 20 us do not depend on
+// the context (plan, first look-ups, join); six chunks of 1 K: 125 us (181 us);
+// 32 requests of 5 tokens: 21 us (61 us).  Tried without gain: twelve warps (two
+// threads per row, or twice the decoding warps), a third S buffer, one issuing
+// warp per kind of product, the set-up before the wait for the predecessor.
 //
 // Every mbarrier wait is bounded; no barrier can run two phases ahead of a
-// waiter: a stage's next phase needs its own release, a step's barriers
-// alternate and step g + 2 needs step g's products.
+// waiter: a stage's next phase needs its own release, the half-steps' barriers
+// alternate, and a half-step's buffer is written again only after its products.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -104,16 +105,19 @@ constexpr uint32_t kOffX = kOffV + kVStages * kKvTile;
 constexpr uint32_t kOffBars = kOffX + kVStages * sizeof(Extra);
 constexpr uint32_t kOffTab = kOffBars + 256;
 
-// A pair cut at a CTA's end that began in it: its kv head, first row of q and
-// tokens, and the last CTA with a piece (0: none).
+// A pair that several CTAs have a piece of: its kv head, first row of q and
+// tokens, and the first and last of the CTAs (first | last << 16; the same: it
+// is not cut).  One entry per pair of every kv head where those are fewer than
+// the CTAs, else one per CTA, for the pair it leaves unfinished.
 struct Cut {
-  int32_t kvh, row0, c1, tokens;
+  int32_t kvh, row0, ctas, tokens;
 };
 
 struct TcParams {
   Int4PrefillParams a;
   int32_t group, tq;      // q heads per kv head, tokens per tile
   int32_t max_pairs;      // room for the pair table
+  int32_t by_pair;        // cuts are kept per pair
   int32_t block_shift;    // block_size is 2^block_shift, or -1
   uint32_t block_div;     // else 2^32 / block_size, rounded up
   int64_t block_rows;     // pool rows from a block to the next
@@ -352,8 +356,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   Cut* const cuts = reinterpret_cast<Cut*>(tp.part);
   float* const part = tp.part + kMaxCtas * (sizeof(Cut) / sizeof(float));
   const uint32_t cta = blockIdx.x;
+  if (tp.by_pair && cta == 0) {  // entries of pairs there is room for but that do not exist
+    const int spare = tp.max_pairs - n_pairs;
+    for (int i = tid; i < spare * p.hkv; i += kThreads)
+      cuts[(i / spare) * tp.max_pairs + n_pairs + i % spare] = Cut{0, 0, 0, 0};
+  }
   if (cta >= act) {
-    if (tid == 0) cuts[cta] = Cut{0, 0, 0, 0};
+    if (!tp.by_pair && tid == 0) cuts[cta] = Cut{0, 0, 0, 0};
     return;
   }
   const uint32_t share = total_steps / act, extra = total_steps - share * act;
@@ -398,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   bool fail = false;
 
   if (warp >= 4) {
-    reg_dec<88>();
+    reg_dec<96>();
     // roles of warps 4-7: issue, decode K rows 0-31, decode V, decode K rows 32-63
     const int role = (warp - 4 + (cta >= (gridDim.x + 1) / 2 ? 1 : 0)) & 3;
     if (role == 0) {
@@ -700,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (fail && lane == 0) flag_error(p.err, PSB_DEVERR_TIMEOUT);
     }
   } else {
-    reg_inc<168>();
+    reg_inc<160>();
     // ---- softmax warps ------------------------------------------------------
     const int row = warp * 32 + lane;
     const int rtok = row / group, rhead = row - rtok * group;
@@ -906,18 +915,26 @@ __global__ void __launch_bounds__(kThreads, 2)
       Cut c{0, 0, 0, 0};
       const uint32_t t_e = my_e - static_cast<uint32_t>(s.j0 + s.n) + static_cast<uint32_t>(s.n_kv);
       if (!fail && s.j0 == 0 && t_e > my_e) {
-        c.kvh = s.kvh;
-        c.row0 = s_q0[s.seq] + s.tok0;
-        c.tokens = min(PQ, s_len[s.seq] - s.tok0);
-        c.c1 = static_cast<int32_t>(cta);
+        uint32_t c1 = cta;
         for (uint32_t c0 = cta + 1; c0 < act; c0 += 32) {  // CTAs that start before its end
           const bool in = c0 + lane < act && cta_start(min(c0 + lane, act)) < t_e;
           const int n = __popc(__ballot_sync(0xffffffffu, in));
-          c.c1 += n;
+          c1 += n;
           if (n < 32) break;
         }
+        c = Cut{s.kvh, s_q0[s.seq] + s.tok0, static_cast<int32_t>(cta | c1 << 16), min(PQ, s_len[s.seq] - s.tok0)};
       }
-      if (lane == 0) cuts[cta] = c;
+      if (lane == 0) {
+        if (!tp.by_pair) {
+          cuts[cta] = c;
+        } else {  // the pairs that begin here: whole ones, and the last
+          cc = first;
+          while (cc.left > 0) {
+            const Run r = cc.take(plan);
+            if (r.j0 == 0) cuts[r.kvh * tp.max_pairs + r.pair] = cc.left > 0 ? Cut{0, 0, 0, 0} : c;
+          }
+        }
+      }
     }
   }
   tc_fence_before();
@@ -928,21 +945,22 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// Joins the partials of the pair that CTA blockIdx.x left cut at its end: a
-// quarter of a tile's rows per CTA, kWarpRows rows per warp, two elements a
-// lane, kBatch partials in flight.
-constexpr int kCombineRows = 32, kWarpRows = kCombineRows / (kThreads / 32), kBatch = 4;
+// Joins the partials of the pair in entry blockIdx.x: kCombineRows of a tile's
+// rows per CTA, kWarpRows rows per warp, two elements a lane, kBatch partials
+// in flight (they come from L2: a round of loads costs more than their bytes).
+constexpr int kCombineThreads = 256, kCombineRows = 16, kWarpRows = kCombineRows / (kCombineThreads / 32), kBatch = 8;
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) int4_prefill_combine_kernel(const TcParams tp) {
+__global__ void __launch_bounds__(kCombineThreads) int4_prefill_combine_kernel(const TcParams tp) {
   const Int4PrefillParams& p = tp.a;
   pdl_wait();
   pdl_launch_dependents();
-  const int c0 = blockIdx.x, lane = threadIdx.x & 31;
-  const int4 cut = __ldcg(reinterpret_cast<const int4*>(tp.part) + c0);
+  const int lane = threadIdx.x & 31;
+  const int4 cut = __ldcg(reinterpret_cast<const int4*>(tp.part) + blockIdx.x);
+  const int c0 = cut.z & 0xffff, c1 = cut.z >> 16;
   const int tile = blockIdx.y / (kRows / kCombineRows), tokens = cut.w - tile * tp.tq;  // tokens from the tile's first on
   const int row0 = (blockIdx.y % (kRows / kCombineRows)) * kCombineRows + (threadIdx.x >> 5) * kWarpRows;
-  if (cut.z <= c0 || row0 >= min(tokens, tp.tq) * tp.group) return;
+  if (c1 <= c0 || row0 >= min(tokens, tp.tq) * tp.group) return;
   const float* const part = tp.part + kMaxCtas * (sizeof(Cut) / sizeof(float));
   auto piece_of = [&](int c) { return part + static_cast<int64_t>(4 * c + (c == c0 ? 2 : 0) + tile) * kPartFloats; };
   float m[kWarpRows], l[kWarpRows];
@@ -953,7 +971,7 @@ __global__ void __launch_bounds__(kThreads) int4_prefill_combine_kernel(const Tc
     l[r] = 0.f;
     o[r] = make_float2(0.f, 0.f);
   }
-  for (int c = c0; c <= cut.z; c += kBatch) {
+  for (int c = c0; c <= c1; c += kBatch) {
     float2 ml[kBatch][kWarpRows], v[kBatch][kWarpRows];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
@@ -961,7 +979,7 @@ __global__ void __launch_bounds__(kThreads) int4_prefill_combine_kernel(const Tc
       for (int r = 0; r < kWarpRows; ++r) {
         ml[j][r] = make_float2(-INFINITY, 0.f);
         v[j][r] = make_float2(0.f, 0.f);
-        if (c + j <= cut.z) {
+        if (c + j <= c1) {
           const float* pc = piece_of(c + j);
           ml[j][r] = __ldcg(reinterpret_cast<const float2*>(pc + kRows * kDim + 2 * (row0 + r)));
           v[j][r] = __ldcg(reinterpret_cast<const float2*>(pc + (row0 + r) * kDim) + lane);
@@ -1050,7 +1068,7 @@ int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspa
   const auto comb = dtype == PSB_BF16 ? int4_prefill_combine_kernel<__nv_bfloat16> : int4_prefill_combine_kernel<__half>;
   const size_t smem = tc_smem(p.num_seqs, tp.max_pairs);
   // the register split draws on what the block was launched with
-  static_assert(168 + 88 == 2 * 128, "two warpgroups' shares");
+  static_assert(160 + 96 == 2 * 128, "two warpgroups' shares");
   static std::atomic<bool> checked[2];  // per element type
   if (!checked[dtype == PSB_BF16].load(std::memory_order_relaxed)) {
     cudaFuncAttributes fa;
@@ -1063,11 +1081,13 @@ int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspa
   if (!kernel_occupancy(reinterpret_cast<const void*>(kern), kThreads, smem, &occ) || occ < 1) return PSB_ERR_CUDA;
   const int64_t grid = std::min<int64_t>(ctas_bound(p.total, p.num_seqs, tp.tq, p.hkv, p.max_context),
                                          static_cast<int64_t>(sms) * std::min(occ, 2));
+  const int64_t entries = std::min<int64_t>(static_cast<int64_t>(tp.max_pairs) * p.hkv, grid - 1);
+  tp.by_pair = entries < grid - 1;
   discard_stale_error();
   cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, s, tp, tq);
   if (e != cudaSuccess) return record_cuda_error(e);
   if (grid > 1) {
-    e = launch_pdl(comb, dim3(static_cast<unsigned>(grid - 1), 2 * kRows / kCombineRows), dim3(kThreads), 0, s, tp);
+    e = launch_pdl(comb, dim3(static_cast<unsigned>(entries), 2 * kRows / kCombineRows), dim3(kCombineThreads), 0, s, tp);
     if (e != cudaSuccess) return record_cuda_error(e);
   }
   return check_launch();

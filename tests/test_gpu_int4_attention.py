@@ -413,3 +413,23 @@ def test_offsets_past_32_bits():
         del codes, params
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,qlens", [(14, 2, [18, 19, 36, 37, 72, 73]), (8, 1, [16, 17, 32, 33, 48]),
+                                          (128, 1, [1, 2, 3, 5]), (3, 3, [128, 129, 256, 257])])
+def test_prefill_tile_boundaries(dtype, hq, hkv, qlens):
+    """Chunks that end at, just behind and between the ends of the tiles of
+    128 rows (128 / group tokens) and of their pairs, alone and together."""
+    ctxs = [n + 61 * i for i, n in enumerate(qlens)]
+    c = _prefill_case(38, qlens, ctxs, hq, hkv, 64, 16, dtype)
+    got, err = _prefill(c)
+    want, tol = _want_prefill(c)
+    assert err == 0
+    _close(got, want, tol)
+    for i in (1, len(qlens) - 1):
+        one = _prefill_case(39 + i, [qlens[i]], [ctxs[i] + 700], hq, hkv, 64, 16, dtype)
+        got, err = _prefill(one)
+        want, tol = _want_prefill(one)
+        assert err == 0
+        _close(got, want, tol)

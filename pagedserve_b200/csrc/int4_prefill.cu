@@ -133,10 +133,10 @@ int launch_generic(const Int4PrefillParams& p, cudaStream_t s) {
 }
 
 // cu_seqlens sanity, so a malformed batch is reported.
-__global__ void check_seqlens_kernel(const int32_t* cu, int32_t n, int32_t total, int32_t* err) {
+__global__ void check_seqlens_kernel(const int32_t* cu, int32_t n, int32_t total, int32_t max_seqlen, int32_t* err) {
   for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
     const int a = cu[i], b = cu[i + 1];
-    if (a < 0 || b < a || b > total || (i == 0 && a != 0)) flag_error(err, PSB_DEVERR_SEQLENS);
+    if (a < 0 || b < a || b > total || (i == 0 && a != 0) || b - a > max_seqlen) flag_error(err, PSB_DEVERR_SEQLENS);
   }
 }
 
@@ -209,7 +209,7 @@ extern "C" int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (error_flag != nullptr) {
     discard_stale_error();
-    check_seqlens_kernel<<<1, 256, 0, s>>>(cu_seqlens, num_seqs, total_tokens, error_flag);
+    check_seqlens_kernel<<<1, 256, 0, s>>>(cu_seqlens, num_seqs, total_tokens, max_seqlen, error_flag);
   }
   // the tensor-core path reads q by TMA: 16-byte bases and strides
   const bool aligned = q_stride_t % 8 == 0 && q_stride_h % 8 == 0 && q_stride_t > 0 && q_stride_h > 0 &&

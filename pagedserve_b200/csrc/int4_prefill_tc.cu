@@ -49,7 +49,7 @@
 // the context (plan, first look-ups, join); six chunks of 1 K: 125 us (181 us);
 // 32 requests of 5 tokens: 21 us (61 us).  Tried without gain: twelve warps (two
 // threads per row, or twice the decoding warps), a third S buffer, one issuing
-// warp per kind of product, the set-up before the wait for the predecessor.
+// warp per kind of product.
 //
 // Every mbarrier wait is bounded; no barrier can run two phases ahead of a
 // waiter: a stage's next phase needs its own release, the half-steps' barriers
@@ -278,6 +278,28 @@ __global__ void __launch_bounds__(kThreads, 2)
   __shared__ int32_t warp_sums[kThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int TQ = tp.tq, group = tp.group, PQ = 2 * TQ;  // tokens of a tile, of a pair
+  if (tid == 0) {
+    mbar_init(bar_q, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_s + i, 1);
+      mbar_init(bar_p + i, 128);
+      mbar_init(bar_pv + i, 1);
+    }
+    for (int i = 0; i < kKStages; ++i) {
+      mbar_init(bar_k + i, 2);
+      mbar_init(bar_kfree + i, 1);
+    }
+    for (int i = 0; i < kVStages; ++i) {
+      mbar_init(bar_v + i, 1);
+      mbar_init(bar_vfree + i, 1);
+    }
+    mbar_init(bar_drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(s_tmem, kTmemCols);
+    tmem_relinquish();
+  }
   pdl_wait();  // cu_seqlens, lengths and q may come from the stream predecessor
 
   // ---- the plan: every CTA builds the same tables ------------------------------
@@ -307,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int s = s0; s < s1; ++s) {
       const int a = p.cu[s], b = p.cu[s + 1];
       // a malformed batch is reported by the caller's check and read nowhere
-      int len = a < 0 || b < a || b > p.total ? 0 : b - a;
+      int len = a < 0 || b < a || b > p.total ? 0 : min(b - a, p.max_seqlen);
       int ctx = p.ctx[s];
       if (len > 0 && (ctx < len || ctx > p.max_context)) {
         if (blockIdx.x == 0) flag_error(p.err, PSB_DEVERR_CONTEXT);
@@ -363,6 +385,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   if (cta >= act) {
     if (!tp.by_pair && tid == 0) cuts[cta] = Cut{0, 0, 0, 0};
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {  // nothing to do but to give the columns back
+      tc_fence_after();
+      tmem_dealloc(*s_tmem, kTmemCols);
+    }
     return;
   }
   const uint32_t share = total_steps / act, extra = total_steps - share * act;
@@ -377,28 +405,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   first.left = n_mine;
   const uint32_t s_base = smem_u32(smem);
 
-  if (tid == 0) {
-    mbar_init(bar_q, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar_s + i, 1);
-      mbar_init(bar_p + i, 128);
-      mbar_init(bar_pv + i, 1);
-    }
-    for (int i = 0; i < kKStages; ++i) {
-      mbar_init(bar_k + i, 2);
-      mbar_init(bar_kfree + i, 1);
-    }
-    for (int i = 0; i < kVStages; ++i) {
-      mbar_init(bar_v + i, 1);
-      mbar_init(bar_vfree + i, 1);
-    }
-    mbar_init(bar_drain, 1);
-    fence_barrier_init();
-  }
-  if (warp == 0) {
-    tmem_alloc(s_tmem, kTmemCols);
-    tmem_relinquish();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -958,8 +964,8 @@ __global__ void __launch_bounds__(kCombineThreads) int4_prefill_combine_kernel(c
   const int lane = threadIdx.x & 31;
   const int4 cut = __ldcg(reinterpret_cast<const int4*>(tp.part) + blockIdx.x);
   const int c0 = cut.z & 0xffff, c1 = cut.z >> 16;
-  const int tile = blockIdx.y / (kRows / kCombineRows), tokens = cut.w - tile * tp.tq;  // tokens from the tile's first on
-  const int row0 = (blockIdx.y % (kRows / kCombineRows)) * kCombineRows + (threadIdx.x >> 5) * kWarpRows;
+  const int tile = blockIdx.z, tokens = cut.w - tile * tp.tq;  // tokens from the tile's first on
+  const int row0 = blockIdx.y * kCombineRows + (threadIdx.x >> 5) * kWarpRows;
   if (c1 <= c0 || row0 >= min(tokens, tp.tq) * tp.group) return;
   const float* const part = tp.part + kMaxCtas * (sizeof(Cut) / sizeof(float));
   auto piece_of = [&](int c) { return part + static_cast<int64_t>(4 * c + (c == c0 ? 2 : 0) + tile) * kPartFloats; };
@@ -1086,8 +1092,11 @@ int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspa
   discard_stale_error();
   cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, s, tp, tq);
   if (e != cudaSuccess) return record_cuda_error(e);
-  if (grid > 1) {
-    e = launch_pdl(comb, dim3(static_cast<unsigned>(entries), 2 * kRows / kCombineRows), dim3(kCombineThreads), 0, s, tp);
+  if (grid > 1 && p.max_seqlen > 0) {
+    // only rows that a sequence of max_seqlen tokens has
+    const int rows = std::min(p.max_seqlen, tp.tq) * tp.group;
+    e = launch_pdl(comb, dim3(static_cast<unsigned>(entries), (rows + kCombineRows - 1) / kCombineRows, p.max_seqlen > tp.tq ? 2 : 1),
+                   dim3(kCombineThreads), 0, s, tp);
     if (e != cudaSuccess) return record_cuda_error(e);
   }
   return check_launch();

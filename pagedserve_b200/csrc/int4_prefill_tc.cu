@@ -57,6 +57,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cmath>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -121,6 +122,9 @@ struct TcParams {
   int32_t block_shift;    // block_size is 2^block_shift, or -1
   uint32_t block_div;     // else 2^32 / block_size, rounded up
   int64_t block_rows;     // pool rows from a block to the next
+  // scale log2 e as k_sign * scale: K carries the sign (0: a scale of 0), so that
+  // the largest S has the largest score
+  float k_sign, scale;
   float* part;            // workspace: cuts, then per CTA two pieces of a pair, two tiles each
 };
 
@@ -587,8 +591,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           // value = step (c - 8) + (mid + step / 2); its rounding to T and the rest
           const float2 pr = unpack2<T>(cur.par);
-          const float base = fmaf(pr.x, 0.5f, pr.y);
-          const uint64_t st2 = f2_pack(pr.x, pr.x), base2 = f2_pack(base, base), minus = f2_pack(-1.f, -1.f);
+          const float base = fmaf(pr.x, 0.5f, pr.y) * tp.k_sign, step = pr.x * tp.k_sign;
+          const uint64_t st2 = f2_pack(step, step), base2 = f2_pack(base, base), minus = f2_pack(-1.f, -1.f);
           const uint64_t off2 = f2_pack(-8388616.f, -8388616.f);  // - (2^23 + 8)
           const uint32_t tile = dst + st * 2 * kKvTile;
 #pragma unroll 1
@@ -764,22 +768,16 @@ __global__ void __launch_bounds__(kThreads, 2)
         tc_fence_after();
         const uint32_t t_s = t_lane + kSCol + (i & 1) * kBN, t_o = t_lane + kOCol + h * kDim;
         const Extra& f = ext[st];
+        const uint4 odd = *reinterpret_cast<const uint4*>(f.bad);  // bad, nan
+        const int ve = f.vexp;
         uint32_t sr[kBN];
         tmem_ld32(t_s, sr);
         tmem_ld32(t_s + 32, sr + 32);
         tmem_wait_ld();
-        // exponents: scores minus reference, plus kPBits
-        const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), nref2 = f2_pack(kPBits - ref, kPBits - ref);
-#pragma unroll
-        for (int c = 0; c < kBN; c += 2) {
-          const float2 a = f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, nref2));
-          sr[c] = __float_as_uint(a.x);
-          sr[c + 1] = __float_as_uint(a.y);
-        }
         // bit c: the row sees key c of the step
         const uint32_t seen0 = last >= 31 ? ~0u : last < 0 ? 0u : (2u << last) - 1;
         const uint32_t seen1 = last >= 63 ? ~0u : last < 32 ? 0u : (2u << (last - 32)) - 1;
-        const uint32_t ok0 = seen0 & ~f.bad[0], ok1 = seen1 & ~f.bad[1];
+        const uint32_t ok0 = seen0 & ~odd.x, ok1 = seen1 & ~odd.y;
         if ((ok0 & ok1) != ~0u) {
 #pragma unroll
           for (int c = 0; c < kBN; ++c)
@@ -791,11 +789,11 @@ __global__ void __launch_bounds__(kThreads, 2)
           mx0 = fmax3(mx0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
           mx1 = fmax3(mx1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
         }
-        const float mx = fmaxf(mx0, mx1);
+        // exponents are scores minus reference, plus kPBits
+        const float mx = fmaf(fmaxf(mx0, mx1), tp.scale, kPBits - ref);
         // A row's reference moves when a score is above it by more than the
         // limit, or at its first score; O is rescaled then, or when the scale
         // of V's steps changed.  The warp's TMEM access is collective.
-        const int ve = f.vexp;
         const bool begins = hs < tiles;
         const bool grow = mx > (fresh ? -INFINITY : kGrowth + kPBits);
         if (__any_sync(0xffffffffu, grow) || (!begins && ve != vexp)) {
@@ -824,17 +822,17 @@ __global__ void __launch_bounds__(kThreads, 2)
           z *= al;
           ref += up;
           fresh = fresh && !grow;
-#pragma unroll
-          for (int c = 0; c < kBN; ++c) sr[c] = __float_as_uint(__uint_as_float(sr[c]) - up);
         }
         vexp = ve;
         uint32_t pk[kBN / 2];
         uint64_t l2 = f2_pack(0.f, 0.f), z2 = f2_pack(0.f, 0.f);
+        const uint64_t scale2 = f2_pack(tp.scale, tp.scale), nref2 = f2_pack(kPBits - ref, kPBits - ref);
 #pragma unroll
         for (int c = 0; c < kBN; c += 4) {
           const float4 vm = ld_shared_f4(f.mid + c);
-          const float a0 = ex2_approx(__uint_as_float(sr[c])), a1 = ex2_approx(__uint_as_float(sr[c + 1]));
-          const float b0 = ex2_approx(__uint_as_float(sr[c + 2])), b1 = ex2_approx(__uint_as_float(sr[c + 3]));
+          const float2 xa = f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, nref2));
+          const float2 xb = f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), scale2, nref2));
+          const float a0 = ex2_approx(xa.x), a1 = ex2_approx(xa.y), b0 = ex2_approx(xb.x), b1 = ex2_approx(xb.y);
           const uint64_t a = f2_pack(a0, a1), b = f2_pack(b0, b1);
           l2 = f2_add(l2, f2_add(a, b));
           z2 = f2_fma(a, f2_pack(vm.x, vm.y), z2);
@@ -853,7 +851,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         l += lf.x + lf.y;
         z += zf.x + zf.y;
         // a token that stands for NaN: for the rows that see it
-        if (((f.nan[0] & seen0) | (f.nan[1] & seen1)) != 0) z = __int_as_float(0x7fffffff);
+        if (((odd.z & seen0) | (odd.w & seen1)) != 0) z = __int_as_float(0x7fffffff);
         tmem_st32(t_s, pk);
         tmem_wait_st();
         tc_fence_before();
@@ -1063,6 +1061,8 @@ int int4_prefill_tc_launch(const Int4PrefillParams& p, int dtype, float* workspa
     for (tp.block_shift = 0; (1 << tp.block_shift) < p.block_size;) ++tp.block_shift;
   tp.block_div = tp.block_shift >= 0 ? 0 : static_cast<uint32_t>(((uint64_t(1) << 32) + p.block_size - 1) / p.block_size);
   tp.block_rows = static_cast<int64_t>(p.hkv) * 2 * p.block_size;
+  tp.k_sign = p.scale_log2 > 0.f ? 1.f : p.scale_log2 < 0.f ? -1.f : p.scale_log2;  // (a NaN stays)
+  tp.scale = p.scale_log2 == 0.f ? 1.f : std::fabs(p.scale_log2);
   tp.part = workspace;
   CUtensorMap tq;
   if (!encode_row_groups_map(&tq, p.q, p.total, p.hq, kDim, p.qst, p.qsh, tp.group, tp.tq,

@@ -433,3 +433,18 @@ def test_prefill_tile_boundaries(dtype, hq, hkv, qlens):
         want, tol = _want_prefill(one)
         assert err == 0
         _close(got, want, tol)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-3])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float16, 64), (torch.float32, 64), (torch.bfloat16, 80)])
+def test_scales_of_either_sign(scale, dtype, d):
+    c = _prefill_case(50, [70, 1, 40], [300, 77, 40], 14, 2, d, 16, dtype)
+    got, err = _prefill(c, scale=scale)
+    want, tol = _want_prefill(c, scale=scale)
+    assert err == 0
+    _close(got, want, tol)
+    c["q"] = c["q"][:3]
+    got, err = _decode(c, scale=scale)
+    want, tol = _want_decode(c, scale=scale)
+    assert err == 0
+    _close(got, want, tol)

@@ -40,14 +40,14 @@
 // the same kernel with its loops unrolled and peeled (121 KB of code) spent
 // more issue slots waiting for instructions than on anything else.
 //
-// What bounds it: the softmax's chain (wait, TMEM, scale, maximum, exponentials,
+// What bounds it: the softmax's chain (wait, TMEM, maximum, scale, exponentials,
 // TMEM: some 2400 cycles a half-step, at two warps a scheduler), then V's
 // decoding (3300 a step); half of the issue slots are used, the exponentials
-// take 31% of their pipe.  With one tile a step, V's decoding bounded it and 512
-// tokens on 32 K took 200 us where this takes 160.  512 tokens on 8 K: 59 us
-// (paged_prefill over a 16-bit pool: 152 us), of which 20 us do not depend on
-// the context (plan, first look-ups, join); six chunks of 1 K: 125 us (181 us);
-// 32 requests of 5 tokens: 21 us (61 us).  Tried without gain: twelve warps (two
+// take a third of their pipe.  With one tile a step, V's decoding bounded it and
+// 512 tokens on 32 K took 200 us where this takes 155.  512 tokens on 8 K: 55.5
+// us (paged_prefill over a 16-bit pool: 152 us), of which 18 us do not depend on
+// the context (plan, first look-ups, join); six chunks of 1 K: 119 us (181 us);
+// 32 requests of 5 tokens: 18.3 us (61 us).  Tried without gain: twelve warps (two
 // threads per row, or twice the decoding warps), a third S buffer, one issuing
 // warp per kind of product.
 //

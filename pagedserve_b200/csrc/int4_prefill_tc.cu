@@ -40,13 +40,14 @@
 // the same kernel with its loops unrolled and peeled (121 KB of code) spent
 // more issue slots waiting for instructions than on anything else.
 //
-// What bounds it: the softmax's chain (wait, TMEM, maximum, scale, exponentials,
-// TMEM: some 2400 cycles a half-step, at two warps a scheduler), then V's
-// decoding (3300 a step); half of the issue slots are used, the exponentials
-// take a third of their pipe.  With one tile a step, V's decoding bounded it and
-// 512 tokens on 32 K took 200 us where this takes 155.  512 tokens on 8 K: 55.5
+// What bounds it: the chain of a half-step, 2300 cycles: the softmax (TMEM,
+// maximum, exponentials, TMEM: 1750, at two warps a scheduler) and the issuing
+// lane (1700: twelve products and their commits), each waiting for the other's
+// last; V's decoding is busy 3000 of the 4600 of a step, half of the issue slots
+// are used, the exponentials take a third of their pipe.  With one tile a step, V's decoding bounded it and
+// 512 tokens on 32 K took 200 us where this takes 150.  512 tokens on 8 K: 54.7
 // us (paged_prefill over a 16-bit pool: 152 us), of which 18 us do not depend on
-// the context (plan, first look-ups, join); six chunks of 1 K: 119 us (181 us);
+// the context (plan, first look-ups, join); six chunks of 1 K: 118 us (181 us);
 // 32 requests of 5 tokens: 18.3 us (61 us).  Tried without gain: twelve warps (two
 // threads per row, or twice the decoding warps), a third S buffer, one issuing
 // warp per kind of product.
@@ -187,8 +188,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 
 // mbar_wait with one copy of the instruction.
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-  const uint32_t addr = smem_u32(bar);
+__device__ __forceinline__ bool wait_at(uint32_t addr, uint32_t parity) {
   uint64_t t0 = 0;
 #pragma unroll 1
   while (!mbar_try_wait_sleep(addr, parity, 100000u)) {
@@ -198,6 +198,18 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
   }
   return true;
 }
+// The issuing lane keeps shared addresses and the descriptors' low words (their
+// high ones are constant) in 32 bits: it is as busy as the softmax.
+__device__ __forceinline__ void commit_at(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return wait_at(smem_u32(bar), parity); }
 // The same for a whole warp: its lanes give up together or not at all.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, wait(bar, parity));
@@ -429,100 +441,118 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint64_t dv = umma_desc_sw128(s_base + kOffV, 1024, 8192);
         prefetch_tmap(&tm_q);
         // Half-steps (a step of one tile), in order: a step's first tile, its
-        // second.  Number i uses S buffer i & 1.  S runs two half-steps ahead of O.
+        // second.  Number i uses S buffer i & 1 (b8: 8 times that, ph: the
+        // parity of its use, i >> 1).  S runs two half-steps ahead of O.
+        const uint32_t a_q = smem_u32(bar_q), a_k = smem_u32(bar_k), a_kfree = smem_u32(bar_kfree), a_v = smem_u32(bar_v),
+                       a_vfree = smem_u32(bar_vfree), a_s = smem_u32(bar_s), a_p = smem_u32(bar_p), a_pv = smem_u32(bar_pv);
+        const uint32_t qlo = static_cast<uint32_t>(dq), klo = static_cast<uint32_t>(dk), vlo = static_cast<uint32_t>(dv);
+        const uint32_t shi = static_cast<uint32_t>(dk >> 32), vhi = static_cast<uint32_t>(dv >> 32);  // (Q's and K's are alike)
+        const uint32_t box = static_cast<uint32_t>(TQ * group) * kDim * 2;
         Cursor sc = first, oc = first;
-        Run sr{}, orun{};
-        int s_left = 0, o_left = 0, sg = 0, og = 0, sh = 0, oh = 0;  // steps left of a run, step, tile
-        int runs = 0, q_wait = 0;     // Q loads asked for, and seen
-        bool s_more = true;           // (n_mine > 0)
+        int s_left = 0, o_left = 0;     // steps left of the runs of S and O
+        uint32_t s_two = 0, o_two = 0;  // whether they have a second tile
+        uint32_t sh = 0, oh = 0;        // tile of the step
+        uint32_t k_st = 0, k_ph = 0, v_st = 0, v_ph = 0, q_ph = 1, b8 = 0, ph = 1;
+        bool begins = false, s_more = true, started = false;
+        bool q_flight = false;          // a copy of Q is on its way
 #pragma unroll 1
         for (int i = -2;; ++i) {
           if (i >= 0) {  // P V of half-step i
             if (oh == 0) {
               if (o_left == 0) {
                 if (oc.left == 0) break;
-                orun = oc.take(plan);
-                o_left = orun.n;
+                const Run r = oc.take(plan);
+                o_left = r.n;
+                o_two = r.two;
+                begins = true;
               }
-              if (!wait(bar_v + og % kVStages, (og / kVStages) & 1)) {
+              if (!wait_at(a_v + 8 * v_st, v_ph)) {
                 fail = true;
                 break;
               }
             }
-            if (!wait(bar_p + (i & 1), (i >> 1) & 1)) {
+            if (!wait_at(a_p + b8, ph)) {
               fail = true;
               break;
             }
             tc_fence_after();
-            const uint64_t dvs = dv + static_cast<uint64_t>((og % kVStages) * (kKvTile >> 4));
-            const uint32_t pcol = tmem + kSCol + (i & 1) * kBN, ocol = tmem + kOCol + oh * kDim;
-            const bool begins = o_left == orun.n;
+            const uint32_t pcol = tmem + kSCol + 8 * b8, ocol = tmem + kOCol + oh * kDim, vd = vlo + v_st * (kKvTile >> 4);
 #pragma unroll
             for (int kk = 0; kk < kBN / 16; ++kk)
-              umma_f16_ts(ocol, pcol + 8 * kk, dvs + 128 * kk, idesc_o, !begins || kk > 0);
-            umma_commit(bar_pv + (i & 1));
-            if (oh == (orun.two ? 1 : 0)) {
-              umma_commit(bar_vfree + og % kVStages);
+              umma_f16_ts(ocol, pcol + 8 * kk, desc_of(vd + 128 * kk, vhi), idesc_o, !begins || kk > 0);
+            commit_at(a_pv + b8);
+            if (oh == o_two) {
+              commit_at(a_vfree + 8 * v_st);
               oh = 0;
-              ++og;
+              if (++v_st == kVStages) {
+                v_st = 0;
+                v_ph ^= 1;
+              }
               --o_left;
+              begins = false;
             } else {
               oh = 1;
             }
           }
           if (s_more) {  // S of half-step i + 2, whose buffer held S and then P of half-step i
-            if (i >= 0 && !wait(bar_pv + (i & 1), (i >> 1) & 1)) {
+            if (i >= 0 && !wait_at(a_pv + b8, ph)) {
               fail = true;
               break;
             }
             if (sh == 0) {
               if (s_left == 0) {  // a run begins: its Q, once the last S of the run before is done
-                sr = sc.take(plan);
-                s_left = sr.n;
-                if (i >= -1 && !wait(bar_s + ((i + 1) & 1), ((i + 1) >> 1) & 1)) {
+                const Run r = sc.take(plan);
+                s_left = r.n;
+                s_two = r.two;
+                if (started && !wait_at(a_s + (b8 ^ 8), b8 == 0 ? ph : ph ^ 1)) {
                   fail = true;
                   break;
                 }
-                const uint32_t bytes = static_cast<uint32_t>(TQ * group) * kDim * 2;
-                mbar_arrive_expect_tx(bar_q, sr.two ? 2 * bytes : bytes);
-                const int row0 = plan.q0[sr.seq] + sr.tok0;
-                tma_load_3d(smem, &tm_q, 0, sr.kvh * group, row0, bar_q);
-                if (sr.two) tma_load_3d(smem + kQTile, &tm_q, 0, sr.kvh * group, row0 + TQ, bar_q);
-                ++runs;
-                if (!wait(bar_q, (runs - 1) & 1)) {
+                started = true;
+                mbar_arrive_expect_tx(bar_q, box << s_two);
+                const int row0 = plan.q0[r.seq] + r.tok0;
+                tma_load_3d(smem, &tm_q, 0, r.kvh * group, row0, bar_q);
+                if (r.two) tma_load_3d(smem + kQTile, &tm_q, 0, r.kvh * group, row0 + TQ, bar_q);
+                q_ph ^= 1;
+                q_flight = true;
+                if (!wait_at(a_q, q_ph)) {
                   fail = true;
                   break;
                 }
-                q_wait = runs;
+                q_flight = false;
               }
-              if (!wait(bar_k + sg % kKStages, (sg / kKStages) & 1)) {
+              if (!wait_at(a_k + 8 * k_st, k_ph)) {
                 fail = true;
                 break;
               }
             }
             tc_fence_after();
-            const uint64_t dqs = dq + static_cast<uint64_t>(sh * (kQTile >> 4));
-            const uint64_t dks = dk + static_cast<uint64_t>((sg % kKStages) * (2 * kKvTile >> 4));
+            const uint32_t scol = tmem + kSCol + 8 * b8, qd = qlo + sh * (kQTile >> 4), kd = klo + k_st * (2 * kKvTile >> 4);
 #pragma unroll
             for (int kk = 0; kk < 2 * kDim / 16; ++kk)  // the values rounded to T, then their rests
-              umma_f16_ss(tmem + kSCol + (i & 1) * kBN, dqs + 2 * (kk & 3), dks + (kk >> 2) * (kKvTile >> 4) + 2 * (kk & 3),
+              umma_f16_ss(scol, desc_of(qd + 2 * (kk & 3), shi), desc_of(kd + (kk >> 2) * (kKvTile >> 4) + 2 * (kk & 3), shi),
                           idesc_s, kk > 0);
-            umma_commit(bar_s + (i & 1));
-            if (sh == (sr.two ? 1 : 0)) {
-              umma_commit(bar_kfree + sg % kKStages);
+            commit_at(a_s + b8);
+            if (sh == s_two) {
+              commit_at(a_kfree + 8 * k_st);
               sh = 0;
-              ++sg;
+              if (++k_st == kKStages) {
+                k_st = 0;
+                k_ph ^= 1;
+              }
               --s_left;
               s_more = s_left > 0 || sc.left > 0;
             } else {
               sh = 1;
             }
           }
+          b8 ^= 8;
+          if (b8 == 0) ph ^= 1;
         }
         if (fail) {
           flag_error(p.err, PSB_DEVERR_TIMEOUT);
           // let the copies and products in flight land before shared memory and TMEM are released
-          if (q_wait < runs) (void)wait(bar_q, (runs - 1) & 1);
+          if (q_flight) (void)wait_at(a_q, q_ph);
           umma_commit(bar_drain);
           (void)wait(bar_drain, 0);
         }

@@ -50,7 +50,8 @@
 // the context (plan, first look-ups, join); six chunks of 1 K: 118 us (181 us);
 // 32 requests of 5 tokens: 18.3 us (61 us).  Tried without gain: twelve warps (two
 // threads per row, or twice the decoding warps), a third S buffer, one issuing
-// warp per kind of product.
+// warp per kind of product; P through shared memory, which frees S's buffer as
+// soon as it is read, cost more than it parted (172 against 150 us on 32 K).
 //
 // Every mbarrier wait is bounded; no barrier can run two phases ahead of a
 // waiter: a stage's next phase needs its own release, the half-steps' barriers

@@ -293,7 +293,11 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_vec_kernel(const Int
   const int lane = threadIdx.x & 31;
   for (Idx base = (blockIdx.x * static_cast<Idx>(kWriteThreads) + threadIdx.x) & ~static_cast<Idx>(31); base < total;
        base += static_cast<Idx>(gridDim.x) * kWriteThreads) {
-    const Idx i = min(base + lane, total - 1);  // lanes past the end repeat the last piece: same bytes, same place
+    // Lanes past the end take part in the warp's shuffles and votes only: each of
+    // them holds the last piece, not a row, so its extremes are not the row's and
+    // it stores nothing.
+    const bool live = base + lane < total;
+    const Idx i = min(base + lane, total - 1);
     const bool is_q = ROPE && i < q_total;
     const Idx u = is_q ? i : i - q_total, per = is_q ? q_tok : kv_tok;
     const Idx t = divide(u, is_q ? p.q_div : p.kv_div);
@@ -312,7 +316,7 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_vec_kernel(const Int
     a.load(src);
     b.load(src + half);
     int64_t slot = -1;
-    if (role) slot = __ldg(p.slots + t);
+    if (role && live) slot = __ldg(p.slots + t);
     if (ROPE && role < 2) {
       const T* cs = reinterpret_cast<const T*>(p.cos) + t * p.cst + e0;
       const T* sn = reinterpret_cast<const T*>(p.sin) + t * p.cst + e0;
@@ -324,10 +328,10 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_vec_kernel(const Int
       rotate(a, b, c1, c2, s1, s2);
     }
     if (ROPE) {
-      __syncwarp();  // in place: lanes that repeat the last piece have read it before it is written
+      __syncwarp();  // in place: the lanes past the end have read the last piece before its own lane writes it
       T* dst = role == 0 ? reinterpret_cast<T*>(p.qo) + t * p.qost + h * p.qosh + e0
                          : role == 1 && p.ko ? reinterpret_cast<T*>(p.ko) + t * p.kost + h * p.kosh + e0 : nullptr;
-      if (dst != nullptr) {
+      if (dst != nullptr && live) {
         a.store(dst);
         b.store(dst + half);
       }

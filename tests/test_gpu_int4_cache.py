@@ -208,3 +208,35 @@ def test_side_stream_and_graph():
     assert torch.equal(dc.cpu(), want_c) and torch.equal(dp.cpu(), want_p)
     k2, v2 = ops.gather_cache_int4(dc, dp, ds, 0)
     assert torch.equal(gk, k2) and torch.equal(gv, v2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rope", [False, True])
+@pytest.mark.parametrize("hq,hkv,d,tokens", [(14, 2, 64, 1), (14, 2, 64, 3), (14, 2, 64, 7), (3, 1, 128, 1),
+                                             (5, 3, 32, 5), (1, 1, 256, 1)])
+def test_last_row_of_a_partly_filled_warp(dtype, rope, hq, hkv, d, tokens):
+    """A token count whose pieces do not fill the last warp, the last slot live
+    and the last V row's extremes outside its last piece: the row's codes are
+    the whole row's, whichever lanes hold copies of that piece."""
+    from pagedserve_b200 import ops
+    gen = torch.Generator().manual_seed(d + tokens)
+    bs, layers, layer = 16, 2, 1
+    codes, params = _pool(gen, layers, 3, hkv, bs, d, dtype)
+    q = torch.randn(tokens, hq, d, generator=gen).to(dtype)
+    k = torch.randn(tokens, hkv, d, generator=gen).to(dtype)
+    v = torch.randn(tokens, hkv, d, generator=gen).to(dtype)
+    v[-1, -1, 0], v[-1, -1, d // 2] = 9.0, -7.0
+    ang = torch.rand(tokens, d, generator=gen, dtype=torch.float64) * 6.3
+    cos, sin = ang.cos().to(dtype), ang.sin().to(dtype)
+    slots = torch.randperm(3 * bs, generator=gen)[:tokens]
+    kw = ref.rotate(k, cos[:, None], sin[:, None]) if rope else k
+    want_c, want_p = _expect(codes, params, layer, slots, kw, v, bs)
+    for _ in range(3):
+        dc, dp = codes.cuda(), params.cuda()
+        if rope:
+            oq, ok = ops.rope_reshape_and_cache_int4(q.cuda(), k.cuda(), v.cuda(), cos.cuda(), sin.cuda(), dc, dp,
+                                                     slots.cuda(), layer)
+            assert torch.equal(oq.cpu(), ref.rotate(q, cos[:, None], sin[:, None])) and torch.equal(ok.cpu(), kw)
+        else:
+            ops.reshape_and_cache_int4(k.cuda(), v.cuda(), dc, dp, slots.cuda(), layer)
+        assert torch.equal(dc.cpu(), want_c) and torch.equal(dp.cpu(), want_p)

@@ -527,9 +527,12 @@ int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h
  * A step that cannot be carried out whole changes neither the store nor the
  * free list and is flagged: not enough free blocks (PSB_DEVERR_POOL), a row
  * named twice (PSB_DEVERR_ROWS), a row out of range, a negative start or count,
- * more blocks than store_width or out_width (PSB_DEVERR_CONTEXT), total not the
+ * more blocks than store_width or out_width (PSB_DEVERR_CONTEXT), an id outside
+ * the pool among those it would take (PSB_DEVERR_BLOCK_RANGE), total not the
  * sum of query_lens (PSB_DEVERR_SEQLENS).  Every slot is then -1, every length
- * and table entry 0.  Calls on one free list must not overlap on the GPU.
+ * and table entry 0.  A step that is carried out over a row that already holds
+ * such an id flags it, copies it to block_tables (whose readers skip it) and
+ * gives its tokens slot -1.  Calls on one free list must not overlap on the GPU.
  */
 int psb_extend_step(int32_t* table_store, int64_t store_stride, int32_t store_rows, int32_t store_width,
                     const int32_t* req_rows, const int32_t* starts, const int32_t* query_lens, int32_t batch,
@@ -543,7 +546,8 @@ int psb_extend_step(int32_t* table_store, int64_t store_stride, int32_t store_ro
  * ceil(keep / block_size) go to the tail of the ring, entry by entry in table
  * order, and their store entries become 0.  Rows, checks and the all-or-nothing
  * rule are psb_extend_step's (keep > held is PSB_DEVERR_CONTEXT, more blocks
- * than the ring has room for PSB_DEVERR_POOL).
+ * than the ring has room for PSB_DEVERR_POOL, an id outside the pool among those
+ * given back PSB_DEVERR_BLOCK_RANGE: none is).
  */
 int psb_trim_tables(int32_t* table_store, int64_t store_stride, int32_t store_rows, int32_t store_width,
                     const int32_t* req_rows, const int32_t* held_lens, const int32_t* keep_lens, int32_t batch,

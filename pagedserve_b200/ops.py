@@ -1004,7 +1004,8 @@ def extend_step(table_store: torch.Tensor, req_rows: torch.Tensor, starts: torch
     does.  ``req_rows[b] < 0`` marks a padding entry.  A step that cannot be
     carried out whole changes nothing, sets ``error_flag`` (128: not enough
     free blocks, 256: a row named twice, 4: a bad row, start, count or width,
-    32: ``total`` is not the sum) and gives slots of -1 and lengths of 0.
+    1: an id outside the pool would be taken, 32: ``total`` is not the sum) and
+    gives slots of -1 and lengths of 0.
     """
     if out is None and table_store.is_cuda:
         done = (_native._calls or _native.calls()).extend(table_store, req_rows, starts, query_lens, free_blocks,

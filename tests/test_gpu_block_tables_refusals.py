@@ -1,0 +1,89 @@
+"""Refused table calls as a whole: ids outside the pool."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BLOCK_RANGE = 1
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.fail("CUDA device required for -m gpu tests")
+
+
+def _dev(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _flag():
+    return torch.zeros(1, dtype=torch.int32, device="cuda")
+
+
+class _Tables:
+    def __init__(self, blocks, rows, width, bs=16, order=None):
+        from pagedserve_b200 import ops
+        self.ops, self.bs = ops, bs
+        self.free, self.state = ops.free_list(blocks, "cuda", order)
+        self.store = torch.zeros(rows, width, dtype=torch.int32, device="cuda")
+        self.err = _flag()
+
+    def extend(self, rows, starts, new, flag=True):
+        return self.ops.extend_step(self.store, _dev(rows), _dev(starts), _dev(new), self.free, self.state, sum(new),
+                                    self.bs, error_flag=self.err if flag else None)
+
+    def trim(self, rows, held, keep):
+        self.ops.trim_tables(self.store, _dev(rows), _dev(held), _dev(keep), self.free, self.state, self.bs,
+                             error_flag=self.err)
+
+    def copy(self):
+        return self.store.tolist(), self.ring(), self.state.tolist()
+
+    def same(self, before):
+        return self.copy() == before
+
+    def ring(self):
+        head, count = self.state.tolist()[:2]
+        ids = self.free.tolist()
+        return [ids[(head + i) % len(ids)] for i in range(count)]
+
+
+@pytest.mark.parametrize("bad", [-1, 400, 1 << 30])
+@pytest.mark.parametrize("batch,width,new", [(2, 6, 40), (40, 300, 150)])
+def test_trim_of_an_id_outside_the_pool_changes_nothing(bad, batch, width, new):
+    """Whichever entry it is found in, and however many CTAs the call has."""
+    t = _Tables(400, batch, width)
+    rows = list(range(batch))
+    t.extend(rows, [0] * batch, [new] * batch)
+    last = -(-new // 16) - 1
+    for row, col in ((0, 0), (batch - 1, last)):
+        good = t.store[row, col].item()
+        t.store[row, col] = bad
+        before = t.copy()
+        t.trim(rows, [new] * batch, [0] * batch)
+        assert int(t.err.item()) == BLOCK_RANGE and t.same(before)
+        t.err.zero_()
+        t.store[row, col] = good
+    # an id that is kept is not looked at
+    t.store[0, 0] = bad
+    t.trim(rows, [new] * batch, [16] * batch)
+    assert int(t.err.item()) == 0 and t.store[0, 0].item() == bad
+    assert len(t.ring()) == 400 - batch and all(0 <= i < 400 for i in t.ring())
+
+
+@pytest.mark.parametrize("bad", [-1, 9, 1 << 30])
+def test_extend_over_an_id_outside_the_pool_changes_nothing(bad):
+    t = _Tables(9, 3, 6, order=[4, 2, 0, 1, 3, 5, 6, 7, 8])
+    t.free[2] = bad
+    t.state.copy_(_dev([7, 9, 0, 0]))  # 7, 8, 4, 2, bad, ...
+    before = t.copy()
+    cu, ctx, slots, pos, tables = t.extend([0, 2], [0, 0], [33, 20])  # 3 + 2 blocks
+    assert int(t.err.item()) & BLOCK_RANGE and t.same(before)
+    assert bool((slots == -1).all()) and bool((ctx == 0).all()) and bool((tables == 0).all())
+    t.err.zero_()
+    t.extend([0, 2], [0, 0], [33, 16])  # the four before it
+    assert int(t.err.item()) == 0 and t.store[0, :4].tolist() == [7, 8, 4, 0] and t.store[2, 0].item() == 2

@@ -51,7 +51,8 @@ enum {
   PSB_DEVERR_SEQLENS = 32,      /* cu_seqlens not non-decreasing within [0, total] */
   PSB_DEVERR_LIMIT = 64,        /* psb_select_tokens: a row had no tokens left to generate */
   PSB_DEVERR_POOL = 128,        /* extend_step / trim_tables: not enough free blocks, or a malformed free list */
-  PSB_DEVERR_ROWS = 256         /* extend_step / trim_tables: a store row named twice */
+  PSB_DEVERR_ROWS = 256,        /* extend_step / trim_tables: a store row named twice */
+  PSB_DEVERR_REFUSED = 512      /* an extend_step was refused: table calls refuse until this is cleared */
 };
 
 /* per-row status bits written by psb_select_tokens */
@@ -533,6 +534,14 @@ int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h
  * and table entry 0.  A step that is carried out over a row that already holds
  * such an id flags it, copies it to block_tables (whose readers skip it) and
  * gives its tokens slot -1.  Calls on one free list must not overlap on the GPU.
+ *
+ * What is planned behind a step that turns out refused (its trim_tables, the
+ * next step) names blocks that were never taken.  So a refused step also sets
+ * PSB_DEVERR_REFUSED, and while ``error_flag`` holds that bit extend_step and
+ * trim_tables refuse, adding no other bit; the caller clears it once it has
+ * planned anew.  Calls without an error_flag, or with different ones, do not
+ * learn of it: then trim_tables' held_lens must be the step's context_lens (0
+ * where it was refused).
  */
 int psb_extend_step(int32_t* table_store, int64_t store_stride, int32_t store_rows, int32_t store_width,
                     const int32_t* req_rows, const int32_t* starts, const int32_t* query_lens, int32_t batch,

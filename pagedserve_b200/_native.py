@@ -27,6 +27,7 @@ DEVERR_BITS = {
     64: "a row had no tokens left to generate",
     128: "not enough free blocks, or a malformed free list",
     256: "a table-store row was named twice",
+    512: "an extend_step was refused (table calls refuse until the flag is cleared)",
 }
 
 _c_void_p, _i32, _i64, _f32, _sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t

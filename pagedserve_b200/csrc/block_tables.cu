@@ -27,6 +27,10 @@
 // start or count, more blocks than a row holds, an id outside the pool among
 // those taken or given back - changes neither the store nor the free list
 // (words of the ring that are not on the list are scratch).
+// What was planned behind a refused step (the trim of the same captured step,
+// the next step) counts on blocks the requests never got, and the host cannot
+// take it back in time: a refused extend_step also leaves PSB_DEVERR_REFUSED in
+// error_flag, and while that is set both kernels refuse.
 #include <algorithm>
 
 #include "common.cuh"
@@ -118,6 +122,12 @@ __device__ __forceinline__ void finish_ring(const TablesParams& p, int32_t head,
   }
 }
 
+// Whether an earlier step was refused and the host has not cleared the flag.
+// (A CTA of the step that is being refused may see its own: the same answer.)
+__device__ __forceinline__ bool refused_before(const TablesParams& p) {
+  return p.err != nullptr && (*static_cast<volatile const int32_t*>(p.err) & PSB_DEVERR_REFUSED) != 0;
+}
+
 // Marks entry b's row in the CTA's bitmap; true when it was marked before.
 __device__ __forceinline__ bool mark_row(uint32_t* seen, int32_t row) {
   const uint32_t bit = 1u << (row & 31);
@@ -143,6 +153,7 @@ __global__ void __launch_bounds__(kTabThreads) extend_step_kernel(const TablesPa
   for (int i = tid; i < (p.store_rows + 31) / 32; i += kTabThreads) seen[i] = 0;
   pdl_wait();
   const int32_t head = p.state[0], count = p.state[1];
+  const bool stopped = refused_before(p);
   __syncthreads();
   const int per = (p.batch + kTabThreads - 1) / kTabThreads;
   const int begin = min(tid * per, p.batch), end = min(begin + per, p.batch);
@@ -187,8 +198,8 @@ __global__ void __launch_bounds__(kTabThreads) extend_step_kernel(const TablesPa
       }
     }
   }
-  const bool bad = __syncthreads_or(bits) != 0;
-  if (bits != 0 && blockIdx.x == 0) flag_error(p.err, bits);
+  const bool bad = __syncthreads_or(stopped || bits != 0) != 0;
+  if (bits != 0 && !stopped && blockIdx.x == 0) flag_error(p.err, bits | PSB_DEVERR_REFUSED);
 #pragma unroll 1
   for (int b = begin; b < end; ++b) {
     // a refused step may hold counts that no int32 sum does: kept in range
@@ -277,6 +288,7 @@ __global__ void __launch_bounds__(kTabThreads) trim_tables_kernel(const TablesPa
   for (int i = tid; i < (p.store_rows + 31) / 32; i += kTabThreads) seen[i] = 0;
   pdl_wait();
   const int32_t head = p.state[0], count = p.state[1];
+  const bool stopped = refused_before(p);
   __syncthreads();
   const int per = (p.batch + kTabThreads - 1) / kTabThreads;
   const int begin = min(tid * per, p.batch), end = min(begin + per, p.batch);
@@ -301,8 +313,8 @@ __global__ void __launch_bounds__(kTabThreads) trim_tables_kernel(const TablesPa
   int64_t back_total, unused_total;
   scan_threads(back, unused, back_total, unused_total);
   if (head < 0 || head >= p.ring_size || count < 0 || count + back_total > p.ring_size) bits |= PSB_DEVERR_POOL;
-  const bool bad = __syncthreads_or(bits) != 0;
-  if (bits != 0 && blockIdx.x == 0) flag_error(p.err, bits);
+  const bool bad = __syncthreads_or(stopped || bits != 0) != 0;
+  if (bits != 0 && !stopped && blockIdx.x == 0) flag_error(p.err, bits);
   bool outside = false;  // an id of this CTA's share is outside the pool
   auto place_of = [&](uint32_t i) -> int32_t* {  // the i-th entry to come back
     const int b = entry_of(s_pre, p.batch, static_cast<int>(i));

@@ -1005,7 +1005,9 @@ def extend_step(table_store: torch.Tensor, req_rows: torch.Tensor, starts: torch
     carried out whole changes nothing, sets ``error_flag`` (128: not enough
     free blocks, 256: a row named twice, 4: a bad row, start, count or width,
     1: an id outside the pool would be taken, 32: ``total`` is not the sum) and
-    gives slots of -1 and lengths of 0.
+    gives slots of -1 and lengths of 0.  It also sets bit 512, with which every
+    ``extend_step`` and ``trim_tables`` on that flag is refused in turn - they
+    count on blocks that were not taken - until the flag is cleared.
     """
     if out is None and table_store.is_cuda:
         done = (_native._calls or _native.calls()).extend(table_store, req_rows, starts, query_lens, free_blocks,
@@ -1054,7 +1056,9 @@ def trim_tables(table_store: torch.Tensor, req_rows: torch.Tensor, held_lens: to
     (psb_trim_tables): entry b of ``held_lens[b]`` tokens keeps
     ``keep_lens[b]`` (0: it has finished).  The blocks go to the tail of the
     free ring entry by entry, in table order, as ``BlockManager.free`` returns
-    them.  Checked and refused as a whole, like ``extend_step``.
+    them.  Checked and refused as a whole, like ``extend_step``.  Behind a step
+    of ``extend_step`` that may have been refused, pass its ``error_flag`` (the
+    trim is then refused too) or its ``context_lens`` as ``held_lens``.
     """
     if table_store.is_cuda:
         done = (_native._calls or _native.calls()).trim(table_store, req_rows, held_lens, keep_lens, free_blocks,

@@ -1,4 +1,5 @@
-"""Refused table calls as a whole: ids outside the pool."""
+"""Refused table calls as a whole: ids outside the pool, and a refused
+extend_step followed by the calls that were planned behind it."""
 
 from __future__ import annotations
 
@@ -7,7 +8,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-BLOCK_RANGE = 1
+BLOCK_RANGE, POOL, REFUSED = 1, 128, 512
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -87,3 +88,58 @@ def test_extend_over_an_id_outside_the_pool_changes_nothing(bad):
     t.err.zero_()
     t.extend([0, 2], [0, 0], [33, 16])  # the four before it
     assert int(t.err.item()) == 0 and t.store[0, :4].tolist() == [7, 8, 4, 0] and t.store[2, 0].item() == 2
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_what_follows_a_refused_step_changes_nothing(captured):
+    """extend_step, then the planned trim_tables: when the step was refused for
+    lack of blocks, the trim does not hand out blocks the request never got
+    (block 0 belongs to another request), nor does a next step whose starts
+    have moved on use them; once the flag is cleared all goes on."""
+    t = _Tables(6, 4, 8)
+    t.extend([3], [0], [16 * 4])                  # request 3: blocks 0 .. 3
+    t.extend([1], [0], [10])                      # request 1: block 4
+    assert int(t.err.item()) == 0 and t.ring() == [5]
+    rows, starts, new, zero = _dev([1]), _dev([10]), _dev([30]), _dev([0])  # two blocks more: one is there
+    before = t.copy()
+
+    def step():
+        out = t.ops.extend_step(t.store, rows, starts, new, t.free, t.state, 30, 16, error_flag=t.err)
+        t.ops.trim_tables(t.store, rows, starts + new, zero, t.free, t.state, 16, error_flag=t.err)
+        return out
+
+    if captured:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+            new.fill_(1)  # (the next replay's plan: 30 tokens are not its total)
+        new.fill_(30)
+        torch.cuda.synchronize()
+        g.replay()
+    else:
+        out = step()
+    assert int(t.err.item()) == POOL | REFUSED and t.same(before)
+    # the step behind it, planned as if the first had been carried out
+    cu, ctx, slots, pos, tables = t.extend([1], [40], [1])
+    assert bool((slots == -1).all()) and bool((ctx == 0).all()) and bool((tables == 0).all())
+    assert int(t.err.item()) == POOL | REFUSED and t.same(before)
+    # the host has seen it: request 3 makes room, request 1 goes on where it was
+    t.err.zero_()
+    t.trim([3], [64], [0])
+    t.extend([1], [10], [30])
+    assert int(t.err.item()) == 0
+    assert t.store[1, :4].tolist() == [4, 5, 0, 0] and t.ring() == [1, 2, 3]
+
+
+def test_held_lengths_from_the_step_itself():
+    """Without a flag: a trim whose held lengths are the step's context_lens
+    gives nothing back when the step was refused."""
+    t = _Tables(6, 4, 8)
+    t.extend([3, 1], [0, 0], [64, 10])
+    before = t.copy()
+    _, lens, _, _, _ = t.extend([1], [10], [30], flag=False)
+    t.ops.trim_tables(t.store, _dev([1]), lens, _dev([0]), t.free, t.state, 16)
+    assert t.same(before)
+    _, lens, _, _, _ = t.extend([1], [10], [20], flag=False)
+    t.ops.trim_tables(t.store, _dev([1]), lens, _dev([0]), t.free, t.state, 16)
+    assert t.ring() == [4, 5]

@@ -528,7 +528,8 @@ int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h
  * A step that cannot be carried out whole changes neither the store nor the
  * free list and is flagged: not enough free blocks (PSB_DEVERR_POOL), a row
  * named twice (PSB_DEVERR_ROWS), a row out of range, a negative start or count,
- * more blocks than store_width or out_width (PSB_DEVERR_CONTEXT), an id outside
+ * more blocks than store_width or out_width, a length past 2^31 - 1
+ * (PSB_DEVERR_CONTEXT), an id outside
  * the pool among those it would take (PSB_DEVERR_BLOCK_RANGE), total not the
  * sum of query_lens (PSB_DEVERR_SEQLENS).  Every slot is then -1, every length
  * and table entry 0.  A step that is carried out over a row that already holds

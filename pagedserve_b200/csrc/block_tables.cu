@@ -167,8 +167,8 @@ __global__ void __launch_bounds__(kTabThreads) extend_step_kernel(const TablesPa
     if (n < 0) bits |= PSB_DEVERR_CONTEXT;
     int32_t more = 0;
     if (row >= 0) {  // (a padding entry holds and takes nothing)
-      const uint32_t need = blocks_for(p, static_cast<uint32_t>(max(start, 0)) + static_cast<uint32_t>(max(n, 0)));
-      if (row >= p.store_rows || start < 0 || need > width) {
+      const uint32_t tokens = static_cast<uint32_t>(max(start, 0)) + static_cast<uint32_t>(max(n, 0)), need = blocks_for(p, tokens);
+      if (row >= p.store_rows || start < 0 || need > width || tokens > INT32_MAX) {
         bits |= PSB_DEVERR_CONTEXT;
       } else {
         if (mark_row(seen, row)) bits |= PSB_DEVERR_ROWS;

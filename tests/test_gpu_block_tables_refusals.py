@@ -1,5 +1,5 @@
-"""Refused table calls as a whole: ids outside the pool, and a refused
-extend_step followed by the calls that were planned behind it."""
+"""Refused table calls as a whole: ids outside the pool, a refused extend_step
+followed by the calls that were planned behind it, and lengths past 2^31."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-BLOCK_RANGE, POOL, REFUSED = 1, 128, 512
+BLOCK_RANGE, CONTEXT, POOL, REFUSED = 1, 4, 128, 512
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -143,3 +143,15 @@ def test_held_lengths_from_the_step_itself():
     _, lens, _, _, _ = t.extend([1], [10], [20], flag=False)
     t.ops.trim_tables(t.store, _dev([1]), lens, _dev([0]), t.free, t.state, 16)
     assert t.ring() == [4, 5]
+
+
+def test_a_length_past_31_bits_is_refused():
+    bs = 1 << 20
+    t = _Tables(4, 2, 4096, bs=bs)
+    before = t.copy()
+    _, ctx, slots, _, _ = t.extend([0, 1], [0, 2 ** 31 - 16], [5, 16])
+    assert int(t.err.item()) & CONTEXT and t.same(before)
+    assert bool((ctx == 0).all()) and bool((slots == -1).all())
+    t.err.zero_()
+    _, ctx, _, pos, _ = t.extend([0, 1], [0, 2 ** 31 - 16], [5, 15])
+    assert int(t.err.item()) == 0 and ctx.tolist() == [5, 2 ** 31 - 1] and pos[-1].item() == 2 ** 31 - 2

@@ -133,7 +133,10 @@ int psb_paged_decode_workspace_init(void* workspace, size_t workspace_bytes, int
  * dependent launch), possibly while the kernels this library launched just
  * before (reshape_and_cache, decode, combine, varlen_prefill) still run:
  * they must be written by an earlier kernel that is not one of those (an
- * ordinary launch such as pack_step's, or a host copy).  Calls sharing one
+ * ordinary launch such as pack_step's, or a host copy).  Behind extend_step, a
+ * programmatic dependent launch itself, at least one ordinary launch (a
+ * model's embedding, norm or projection) must lie on the stream between it and
+ * this call.  Calls sharing one
  * workspace must not overlap on the GPU.
  */
 int psb_paged_decode(const void* query, int64_t q_stride_b, int64_t q_stride_h, void* out, int64_t o_stride_b,
@@ -532,7 +535,11 @@ int psb_paged_prefill_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h
  * (PSB_DEVERR_CONTEXT), an id outside
  * the pool among those it would take (PSB_DEVERR_BLOCK_RANGE), total not the
  * sum of query_lens (PSB_DEVERR_SEQLENS).  Every slot is then -1, every length
- * and table entry 0.  A step that is carried out over a row that already holds
+ * and table entry 0.  The outputs may be read by any kernel that waits for its
+ * stream predecessor before it reads: the writes, the 4-bit pool's kernels and
+ * the prefills do; psb_paged_decode and psb_paged_decode_append read lengths and
+ * tables before, and need an ordinary launch in between (see there).  A step
+ * that is carried out over a row that already holds
  * such an id flags it, copies it to block_tables (whose readers skip it) and
  * gives its tokens slot -1.  Calls on one free list must not overlap on the GPU.
  *

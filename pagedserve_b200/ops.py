@@ -1001,7 +1001,9 @@ def extend_step(table_store: torch.Tensor, req_rows: torch.Tensor, starts: torch
     taken from the head of the free ring (``free_list``) in entry order and
     appended to its row of ``table_store``; returns ``(cu_seqlens,
     context_lens, slot_mapping, positions, block_tables)`` as ``pack_step``
-    does.  ``req_rows[b] < 0`` marks a padding entry.  A step that cannot be
+    does.  Between this call and a ``paged_decode`` over a 16-bit pool, which
+    reads lengths and tables ahead of its stream predecessor, there must be an
+    ordinary launch (any PyTorch operator).  ``req_rows[b] < 0`` marks a padding entry.  A step that cannot be
     carried out whole changes nothing, sets ``error_flag`` (128: not enough
     free blocks, 256: a row named twice, 4: a bad row, start, count or width,
     1: an id outside the pool would be taken, 32: ``total`` is not the sum) and

@@ -342,3 +342,54 @@ def test_engine_serves_from_int4_pools():
         assert len(tokens) == m
         assert tokens[0] == int(reference_prefill_logits(model, torch.tensor(p, device="cuda")).argmax())
     assert runs[0] == runs[1]
+
+
+def test_device_tables_feed_the_16_bit_pool():
+    """extend_step, an ordinary launch, the rotary write and paged_decode over
+    16-bit pools as one replayed capture whose tables change with every
+    replay: the rows of a step on the host's tables."""
+    gen = torch.Generator().manual_seed(11)
+    hq, hkv, d, bs, blocks, width = 14, 2, 64, 16, 40, 12
+    kc, vc = (torch.zeros(1, blocks, hkv, bs, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    wk, wv = kc.clone(), vc.clone()
+    free, state = ops.free_list(blocks, "cuda")
+    manager = BlockManager(blocks, bs)
+    store = torch.zeros(4, width, dtype=torch.int32, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    angles = torch.arange(400)[:, None] * torch.exp(-torch.arange(0, d, 2) / d * 9)[None]
+    cos = torch.cat([angles, angles], -1).cos().bfloat16().cuda()
+    sin = torch.cat([angles, angles], -1).sin().bfloat16().cuda()
+    rows, held = [2, 0, 3], [0, 0, 0]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    plan, starts, news = i32(rows), i32(held), i32([1, 1, 1])
+    q, k, v = (_rand(gen, 3, h, d) for h in (hq, hkv, hkv))
+    for r in rows:
+        manager.allocate(str(r), 1)
+    ops.paged_decode(q, kc, vc, i32([[0] * width] * 3), i32([1] * 3), 0)  # the workspace, before the capture
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        _, ctx, slots, pos, tables = ops.extend_step(store, plan, starts, news, free, state, 3, bs, error_flag=err)
+        c, s = cos.index_select(0, pos), sin.index_select(0, pos)
+        qr, _ = ops.rope_reshape_and_cache(q, k, v, c, s, kc, vc, slots, 0, key_out=False)
+        out = ops.paged_decode(qr, kc, vc, tables, ctx, 0)
+        starts += 1
+    for step in range(60):
+        for buf in (q, k, v):
+            buf.copy_(_rand(gen, *buf.shape))
+        if step:
+            for r in rows:
+                if manager.blocks_needed(step + 1) > manager.blocks_needed(step):
+                    manager.allocate_blocks(str(r), 1)
+        g.replay()
+        ids = [manager.get_blocks(str(r)) for r in rows]
+        tab = i32([b + [0] * (width - len(b)) for b in ids])
+        slot = torch.tensor([b[step // bs] * bs + step % bs for b in ids], device="cuda")
+        at = torch.full((3,), step, device="cuda")
+        wq, _ = ops.rope_reshape_and_cache(q, k, v, cos.index_select(0, at), sin.index_select(0, at), wk, wv, slot, 0,
+                                           key_out=False)
+        torch.cuda.synchronize()
+        want = ops.paged_decode(wq, wk, wv, tab, i32([step + 1] * 3), 0)
+        assert torch.equal(out, want) and torch.equal(kc, wk) and torch.equal(vc, wv)
+    assert err.item() == 0
+    g.reset()

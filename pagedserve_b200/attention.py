@@ -446,6 +446,7 @@ def paged_decode_attention_with_write(query: torch.Tensor, key: torch.Tensor, va
     if key.get_device() != dev or value.get_device() != dev:
         raise ValueError("new K/V must be on the query's device")
     if _is_int4(kv):  # the row's minimum and maximum are needed before its codes: a launch of its own
+        key, value = (t if t.stride(-1) == 1 else t.contiguous() for t in (key, value))
         _write_rows(kv, key, value, _slots(cache, request_ids, positions, query.device), layer)
         return _decode_int4(meta, cache, query, layer)
     out = _launch(meta, cache, query, layer, key, value)

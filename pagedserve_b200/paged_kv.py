@@ -227,6 +227,7 @@ class KVCache:
         """Quantise ``key, value [T, Hkv, D]`` into ``slots [T]``."""
         if not key.is_cuda:
             raise ValueError("4-bit pools are written and read on a CUDA device")
+        key, value = (t if t.stride(-1) == 1 else t.contiguous() for t in (key, value))  # (a copy_ takes any strides)
         ops.reshape_and_cache_int4(key, value, self.kv_codes, self.kv_params, slots, layer)
 
     def _read_rows(self, layer: int, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -393,3 +393,36 @@ def test_device_tables_feed_the_16_bit_pool():
         assert torch.equal(out, want) and torch.equal(kc, wk) and torch.equal(vc, wv)
     assert err.item() == 0
     g.reset()
+
+
+@pytest.mark.parametrize("d", [64, 6])
+def test_cache_takes_rows_of_any_strides(d):
+    """Rows whose elements are not adjacent go into a 4-bit cache as they do
+    into a 16-bit one, by token, by block and in the fused decode call."""
+    gen = torch.Generator().manual_seed(12)
+    bs, hkv = 4, 2
+    caches = [PagedKVCache(num_blocks=6, num_layers=1, num_kv_heads=hkv, head_dim=d, block_size=bs,
+                           dtype=torch.bfloat16, kv_bits=4) for _ in range(2)]
+    for c in caches:
+        c.allocate("A", 6)
+        c.kv_cache.kv_codes.zero_()
+        c.kv_cache.kv_params.zero_()
+
+    def strided(t):
+        wide = torch.zeros(*t.shape, 2, dtype=t.dtype, device=t.device)
+        wide[..., 0] = t
+        return wide[..., 0]
+
+    token = [_rand(gen, hkv, d) for _ in range(2)]
+    block = [_rand(gen, hkv, bs, d) for _ in range(2)]
+    new = [_rand(gen, 1, hkv, 1, d) for _ in range(2)]
+    q = _rand(gen, 1, 4, 1, d)
+    outs = []
+    for c, view in zip(caches, (lambda t: t, strided)):
+        for pos in range(5):
+            c.write_token("A", 0, pos, *(view(t) for t in token))
+        c.kv_cache.write_block(0, 5, *(view(t) for t in block))
+        outs.append(paged_decode_attention_with_write(view(q), view(new[0]), view(new[1]), c, ["A"], [5], 0))
+    assert torch.equal(outs[0], outs[1])
+    assert torch.equal(caches[0].kv_cache.kv_codes, caches[1].kv_cache.kv_codes)
+    assert torch.equal(caches[0].kv_cache.kv_params, caches[1].kv_cache.kv_params)

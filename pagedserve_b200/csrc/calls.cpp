@@ -10,7 +10,9 @@
 // Tensor, tensors on another device than the current one - and launches
 // nothing then: ops.py goes on with its own checks, which hold the errors'
 // wording and the copies that unusual strides need.  A C entry's failure comes
-// back as its status, an int.
+// back as its status, an int.  Allocations and launches may wait (for a lock, for
+// memory, for room in the stream's launch queue), so they run without the
+// interpreter's lock, as the calls through ctypes do.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -125,15 +127,19 @@ psb_stream_t stream_of(int dev) {
   return reinterpret_cast<psb_stream_t>(c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream());
 }
 
+// Lets other threads have the interpreter while it lives.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 PyObject* none() { Py_RETURN_NONE; }
-PyObject* status_or(int status, PyObject* result) {
-  if (status == PSB_OK) return result;
-  Py_XDECREF(result);
-  return PyLong_FromLong(status);
-}
-PyObject* wrap_or_same(PyObject* given, const Tensor& t) {
-  if (given != Py_None) return Py_NewRef(given);
-  return THPVariable_Wrap(t);
+PyObject* true_or(int status) { return status == PSB_OK ? Py_NewRef(Py_True) : PyLong_FromLong(status); }
+PyObject* out_or(int status, PyObject* given, const Tensor& t) {
+  if (status != PSB_OK) return PyLong_FromLong(status);
+  return given != Py_None ? Py_NewRef(given) : THPVariable_Wrap(t);
 }
 
 // write(key, value, kv_codes, kv_params, slot_mapping, layer, error_flag) -> True
@@ -150,12 +156,15 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor *k = cuda_tensor(a[0], dev), *v = cuda_tensor(a[1], dev), *slots = cuda_tensor(a[4], dev);
   if (!rows_like(k, p, p.heads) || !rows_like(v, p, p.heads) || k->size(0) != v->size(0) || !slots_like(slots, k->size(0)))
     return none();
-  return status_or(psb_reshape_and_cache_int4(k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(), v->stride(0),
-                                              v->stride(1), p.codes->data_ptr(), p.params->data_ptr(),
-                                              static_cast<const int64_t*>(slots->data_ptr()), k->size(0), layer, p.layers,
-                                              p.blocks, p.heads, p.block_size, p.dim, p.code, flag_ptr(flag),
-                                              stream_of(dev)),
-                   Py_NewRef(Py_True));
+  int status;
+  {
+    const Unlocked unlocked;
+    status = psb_reshape_and_cache_int4(k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(), v->stride(0),
+                                        v->stride(1), p.codes->data_ptr(), p.params->data_ptr(),
+                                        static_cast<const int64_t*>(slots->data_ptr()), k->size(0), layer, p.layers,
+                                        p.blocks, p.heads, p.block_size, p.dim, p.code, flag_ptr(flag), stream_of(dev));
+  }
+  return true_or(status);
   END_HANDLE_TH_ERRORS
 }
 
@@ -182,15 +191,19 @@ PyObject* rope_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return none();
   const bool keep = a[9] == Py_None;
   if (!plain_order(*q) || (keep && !plain_order(*k))) return none();
-  const Tensor qo = new_tensor(q->sizes(), p.dtype, dev);
-  Tensor ko;
-  if (keep) ko = new_tensor(k->sizes(), p.dtype, dev);
-  const int status = psb_rope_reshape_and_cache_int4(
-      q->data_ptr(), q->stride(0), q->stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), k->data_ptr(), k->stride(0),
-      k->stride(1), keep ? ko.data_ptr() : nullptr, keep ? ko.stride(0) : 0, keep ? ko.stride(1) : 0, v->data_ptr(),
-      v->stride(0), v->stride(1), cos->data_ptr(), sin->data_ptr(), cos->stride(0), p.codes->data_ptr(),
-      p.params->data_ptr(), static_cast<const int64_t*>(slots->data_ptr()), t, q->size(1), layer, p.layers, p.blocks,
-      p.heads, p.block_size, p.dim, p.code, flag_ptr(flag), stream_of(dev));
+  Tensor qo, ko;
+  int status;
+  {
+    const Unlocked unlocked;
+    qo = new_tensor(q->sizes(), p.dtype, dev);
+    if (keep) ko = new_tensor(k->sizes(), p.dtype, dev);
+    status = psb_rope_reshape_and_cache_int4(
+        q->data_ptr(), q->stride(0), q->stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), k->data_ptr(),
+        k->stride(0), k->stride(1), keep ? ko.data_ptr() : nullptr, keep ? ko.stride(0) : 0, keep ? ko.stride(1) : 0,
+        v->data_ptr(), v->stride(0), v->stride(1), cos->data_ptr(), sin->data_ptr(), cos->stride(0),
+        p.codes->data_ptr(), p.params->data_ptr(), static_cast<const int64_t*>(slots->data_ptr()), t, q->size(1), layer,
+        p.layers, p.blocks, p.heads, p.block_size, p.dim, p.code, flag_ptr(flag), stream_of(dev));
+  }
   if (status != PSB_OK) return PyLong_FromLong(status);
   return Py_BuildValue("(NN)", THPVariable_Wrap(qo), keep ? THPVariable_Wrap(ko) : Py_NewRef(Py_None));
   END_HANDLE_TH_ERRORS
@@ -210,11 +223,17 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor* slots = cuda_tensor(a[2], dev);
   if (!slots_like(slots, -1)) return none();
   const int64_t t = slots->size(0);
-  const Tensor k = new_tensor({t, p.heads, p.dim}, p.dtype, dev), v = new_tensor({t, p.heads, p.dim}, p.dtype, dev);
-  const int status = psb_gather_cache_int4(p.codes->data_ptr(), p.params->data_ptr(),
-                                           static_cast<const int64_t*>(slots->data_ptr()), k.data_ptr(), k.stride(0),
-                                           k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), t, layer, p.layers,
-                                           p.blocks, p.heads, p.block_size, p.dim, p.code, flag_ptr(flag), stream_of(dev));
+  Tensor k, v;
+  int status;
+  {
+    const Unlocked unlocked;
+    k = new_tensor({t, p.heads, p.dim}, p.dtype, dev);
+    v = new_tensor({t, p.heads, p.dim}, p.dtype, dev);
+    status = psb_gather_cache_int4(p.codes->data_ptr(), p.params->data_ptr(),
+                                   static_cast<const int64_t*>(slots->data_ptr()), k.data_ptr(), k.stride(0), k.stride(1),
+                                   v.data_ptr(), v.stride(0), v.stride(1), t, layer, p.layers, p.blocks, p.heads,
+                                   p.block_size, p.dim, p.code, flag_ptr(flag), stream_of(dev));
+  }
   if (status != PSB_OK) return PyLong_FromLong(status);
   return Py_BuildValue("(NN)", THPVariable_Wrap(k), THPVariable_Wrap(v));
   END_HANDLE_TH_ERRORS
@@ -268,19 +287,24 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !read_attention(a + 3, dev, p, batch, &t))
     return none();
   if (t.out ? !rows(*t.out) || t.out->size(0) != batch || t.out->size(1) != heads : !plain_order(*q)) return none();
-  const Tensor out = t.out ? *t.out : new_tensor(q->sizes(), p.dtype, dev);
-  const Tensor ws = t.ws ? *t.ws
-                         : new_tensor({static_cast<int64_t>(psb_paged_decode_int4_workspace_size(
-                                          batch, heads, p.heads, p.dim, p.block_size, t.max_context, p.code))},
-                                      at::kByte, dev);
-  return status_or(psb_paged_decode_int4(q->data_ptr(), q->stride(0), q->stride(1), out.data_ptr(), out.stride(0),
-                                         out.stride(1), p.codes->data_ptr(), p.params->data_ptr(),
-                                         static_cast<const int32_t*>(t.tables->data_ptr()), t.tables->stride(0),
-                                         static_cast<const int32_t*>(t.ctx->data_ptr()), batch, heads, t.layer, p.layers,
-                                         p.blocks, p.heads, p.block_size, p.dim, p.code, t.max_context,
-                                         static_cast<float>(t.scale), ws.data_ptr(), ws.nbytes(), flag_ptr(t.flag),
-                                         stream_of(dev)),
-                   wrap_or_same(a[7], out));
+  Tensor out;
+  int status;
+  {
+    const Unlocked unlocked;
+    out = t.out ? *t.out : new_tensor(q->sizes(), p.dtype, dev);
+    const Tensor ws = t.ws ? *t.ws
+                           : new_tensor({static_cast<int64_t>(psb_paged_decode_int4_workspace_size(
+                                            batch, heads, p.heads, p.dim, p.block_size, t.max_context, p.code))},
+                                        at::kByte, dev);
+    status = psb_paged_decode_int4(q->data_ptr(), q->stride(0), q->stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                                   p.codes->data_ptr(), p.params->data_ptr(),
+                                   static_cast<const int32_t*>(t.tables->data_ptr()), t.tables->stride(0),
+                                   static_cast<const int32_t*>(t.ctx->data_ptr()), batch, heads, t.layer, p.layers,
+                                   p.blocks, p.heads, p.block_size, p.dim, p.code, t.max_context,
+                                   static_cast<float>(t.scale), ws.data_ptr(), ws.nbytes(), flag_ptr(t.flag),
+                                   stream_of(dev));
+  }
+  return out_or(status, a[7], out);
   END_HANDLE_TH_ERRORS
 }
 
@@ -301,20 +325,24 @@ PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (heads <= 0 || heads > kI32 || heads % p.heads || !read_attention(a + 5, dev, p, batch, &t) || most > t.max_context)
     return none();
   if (t.out ? !rows_like(t.out, p, heads) || t.out->size(0) != total : !plain_order(*q)) return none();
-  const Tensor out = t.out ? *t.out : new_tensor(q->sizes(), p.dtype, dev);
-  const Tensor ws = t.ws ? *t.ws
-                         : new_tensor({static_cast<int64_t>(psb_paged_prefill_int4_workspace_size(
-                                          total, batch, heads, p.heads, p.dim, p.block_size, t.max_context, p.code))},
-                                      at::kByte, dev);
-  return status_or(psb_paged_prefill_int4(q->data_ptr(), q->stride(0), q->stride(1), p.codes->data_ptr(),
-                                          p.params->data_ptr(), static_cast<const int32_t*>(t.tables->data_ptr()),
-                                          t.tables->stride(0), static_cast<const int32_t*>(t.ctx->data_ptr()),
-                                          out.data_ptr(), out.stride(0), out.stride(1),
-                                          static_cast<const int32_t*>(cu->data_ptr()), batch, total, most, t.max_context,
-                                          heads, t.layer, p.layers, p.blocks, p.heads, p.block_size, p.dim, p.code,
-                                          static_cast<float>(t.scale), ws.data_ptr(), ws.nbytes(), flag_ptr(t.flag),
-                                          stream_of(dev)),
-                   wrap_or_same(a[9], out));
+  Tensor out;
+  int status;
+  {
+    const Unlocked unlocked;
+    out = t.out ? *t.out : new_tensor(q->sizes(), p.dtype, dev);
+    const Tensor ws = t.ws ? *t.ws
+                           : new_tensor({static_cast<int64_t>(psb_paged_prefill_int4_workspace_size(
+                                            total, batch, heads, p.heads, p.dim, p.block_size, t.max_context, p.code))},
+                                        at::kByte, dev);
+    status = psb_paged_prefill_int4(q->data_ptr(), q->stride(0), q->stride(1), p.codes->data_ptr(), p.params->data_ptr(),
+                                    static_cast<const int32_t*>(t.tables->data_ptr()), t.tables->stride(0),
+                                    static_cast<const int32_t*>(t.ctx->data_ptr()), out.data_ptr(), out.stride(0),
+                                    out.stride(1), static_cast<const int32_t*>(cu->data_ptr()), batch, total, most,
+                                    t.max_context, heads, t.layer, p.layers, p.blocks, p.heads, p.block_size, p.dim,
+                                    p.code, static_cast<float>(t.scale), ws.data_ptr(), ws.nbytes(), flag_ptr(t.flag),
+                                    stream_of(dev));
+  }
+  return out_or(status, a[9], out);
   END_HANDLE_TH_ERRORS
 }
 
@@ -355,14 +383,20 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (a[8] == Py_None) width = t.store->size(1);
   else if (!as_int(a[8], &width)) return none();
   if (width <= 0) return none();
-  const Tensor cu = new_tensor({t.batch + 1}, at::kInt, dev), ctx = new_tensor({t.batch}, at::kInt, dev);
-  const Tensor slots = new_tensor({total}, at::kLong, dev), pos = new_tensor({total}, at::kLong, dev);
-  const Tensor tables = new_tensor({t.batch, width}, at::kInt, dev);
-  const int status = psb_extend_step(
-      ints(*t.store), t.store->stride(0), t.store->size(0), t.store->size(1), ints(*t.rows), ints(*t.first),
-      ints(*t.second), t.batch, ints(*t.free), t.free->size(0), ints(*t.state), total, block, ints(cu), ints(ctx),
-      static_cast<int64_t*>(slots.data_ptr()), static_cast<int64_t*>(pos.data_ptr()), ints(tables), width,
-      flag_ptr(t.flag), stream_of(dev));
+  Tensor cu, ctx, slots, pos, tables;
+  int status;
+  {
+    const Unlocked unlocked;
+    cu = new_tensor({t.batch + 1}, at::kInt, dev);
+    ctx = new_tensor({t.batch}, at::kInt, dev);
+    slots = new_tensor({total}, at::kLong, dev);
+    pos = new_tensor({total}, at::kLong, dev);
+    tables = new_tensor({t.batch, width}, at::kInt, dev);
+    status = psb_extend_step(ints(*t.store), t.store->stride(0), t.store->size(0), t.store->size(1), ints(*t.rows),
+                             ints(*t.first), ints(*t.second), t.batch, ints(*t.free), t.free->size(0), ints(*t.state),
+                             total, block, ints(cu), ints(ctx), static_cast<int64_t*>(slots.data_ptr()),
+                             static_cast<int64_t*>(pos.data_ptr()), ints(tables), width, flag_ptr(t.flag), stream_of(dev));
+  }
   if (status != PSB_OK) return PyLong_FromLong(status);
   return Py_BuildValue("(NNNNN)", THPVariable_Wrap(cu), THPVariable_Wrap(ctx), THPVariable_Wrap(slots),
                        THPVariable_Wrap(pos), THPVariable_Wrap(tables));
@@ -377,10 +411,14 @@ PyObject* trim(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tables t;
   int64_t block;
   if (!read_tables(a, a[7], dev, &t) || !as_int(a[6], &block) || block <= 0) return none();
-  return status_or(psb_trim_tables(ints(*t.store), t.store->stride(0), t.store->size(0), t.store->size(1), ints(*t.rows),
-                                   ints(*t.first), ints(*t.second), t.batch, ints(*t.free), t.free->size(0),
-                                   ints(*t.state), block, flag_ptr(t.flag), stream_of(dev)),
-                   Py_NewRef(Py_True));
+  int status;
+  {
+    const Unlocked unlocked;
+    status = psb_trim_tables(ints(*t.store), t.store->stride(0), t.store->size(0), t.store->size(1), ints(*t.rows),
+                             ints(*t.first), ints(*t.second), t.batch, ints(*t.free), t.free->size(0), ints(*t.state),
+                             block, flag_ptr(t.flag), stream_of(dev));
+  }
+  return true_or(status);
   END_HANDLE_TH_ERRORS
 }
 

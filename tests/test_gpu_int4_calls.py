@@ -132,3 +132,54 @@ def test_tables_on_another_stream_and_strided_plans():
     want = run(torch.cuda.current_stream(), lambda t: t)
     for got in (run(torch.cuda.Stream(), lambda t: t), run(torch.cuda.Stream(), _strided)):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def _calls_of(c):
+    """One call of each entry point, by name."""
+    store = torch.zeros(6, 12, dtype=torch.int32, device="cuda")
+    free, state = ops.free_list(40, "cuda")
+    rows, zero, one = (torch.tensor([x], dtype=torch.int32, device="cuda") for x in (2, 0, 1))
+    pool = (c["codes"], c["params"])
+    return {
+        "write": lambda: ops.reshape_and_cache_int4(c["k"], c["v"], *pool, c["slots"], 1),
+        "rope_write": lambda: ops.rope_reshape_and_cache_int4(c["q"], c["k"], c["v"], c["cos"], c["sin"], *pool, c["slots"], 1),
+        "gather": lambda: ops.gather_cache_int4(*pool, c["slots"], 1),
+        "decode": lambda: ops.paged_decode_int4(c["q"], *pool, c["table"], c["lens"], 1),
+        "prefill": lambda: ops.paged_prefill_int4(c["q"], *pool, c["table"], c["lens"], c["cu"], 1, 1),
+        "extend": lambda: ops.extend_step(store, rows, zero, zero, free, state, 0, 16),
+        "trim": lambda: ops.trim_tables(store, rows, zero, zero, free, state, 16),
+    }
+
+
+@pytest.mark.parametrize("name", ["write", "rope_write", "gather", "decode", "prefill", "extend", "trim"])
+def test_a_full_launch_queue_stops_no_other_thread(name):
+    """A thread that waits for room in its stream's launch queue leaves the
+    interpreter to the others: behind a kernel of about a second, more calls
+    than the queue holds, and a second thread that looks at the clock."""
+    import threading
+    import time
+    call = _calls_of(_case())[name]
+    call()
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    took = []
+
+    def launches():
+        begin = time.perf_counter()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(1_500_000_000)
+            for _ in range(1500):
+                call()
+        took.append(time.perf_counter() - begin)
+
+    worker = threading.Thread(target=launches)
+    worker.start()
+    last, gap = time.perf_counter(), 0.0
+    while worker.is_alive():
+        time.sleep(0.001)
+        now = time.perf_counter()
+        last, gap = now, max(gap, now - last)
+    worker.join()
+    torch.cuda.synchronize()
+    assert took[0] > 0.4  # the queue was full
+    assert gap < 0.25

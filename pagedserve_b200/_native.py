@@ -173,6 +173,10 @@ def calls():
         except ImportError as e:
             raise RuntimeError(f"{os.path.join(_HERE, '_calls.so')} does not load ({e}); build it with "
                                "`python -m pagedserve_b200.build`") from e
+        from .build import calls_target
+        if module.built_for != calls_target():
+            raise RuntimeError(f"{module.__file__} was built for {module.built_for}, this is {calls_target()}; build it "
+                               "again with `python -m pagedserve_b200.build`")
         _calls = module
     return _calls
 

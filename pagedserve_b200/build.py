@@ -53,29 +53,49 @@ def _compile(src: str, force: bool, extra: list[str]) -> str:
     return obj
 
 
-def _build_calls(force: bool) -> None:
-    """csrc/calls.cpp against this interpreter, this torch and LIB."""
+def calls_target() -> str:
+    """The torch, interpreter and C++ ABI that _calls.so is compiled for: it uses their internals."""
     import sysconfig
 
     import torch
-    newest = max(os.path.getmtime(p) for p in (CALLS_SRC, os.path.join(ROOT, "include", "pagedserve_b200.h")))
-    if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= newest:
-        return
+    return f"torch {torch.__version__}, {sysconfig.get_config_var('EXT_SUFFIX')}, abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+
+
+def _calls_command() -> list[str]:
+    """The compiler's command, but for its output: csrc/calls.cpp against this interpreter, this torch and LIB."""
+    import sysconfig
+
+    import torch
     base = os.path.dirname(torch.__file__)
     include = os.path.join(base, "include")
     cuda = os.path.dirname(os.path.dirname(nvcc()))
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-I", os.path.join(ROOT, "include"), "-isystem", include,
-           "-isystem", os.path.join(include, "torch", "csrc", "api", "include"),
-           "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include"),
-           CALLS_SRC, "-o", CALLS + ".tmp", "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cuda",
-           "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-L", PKG, "-l:libpagedserve_b200.so",
-           "-Wl,-rpath,$ORIGIN"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DPSB_BUILT_FOR="{calls_target()}"',
+            "-I", os.path.join(ROOT, "include"), "-isystem", include,
+            "-isystem", os.path.join(include, "torch", "csrc", "api", "include"),
+            "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include"),
+            CALLS_SRC, "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cuda",
+            "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-L", PKG, "-l:libpagedserve_b200.so",
+            "-Wl,-rpath,$ORIGIN"]
+
+
+def _build_calls(force: bool) -> None:
+    """_calls.so, unless it is newer than its sources and made by the same command for the same target."""
+    cmd = _calls_command()
+    key, stamp = "\n".join(cmd), os.path.join(BUILD, "calls.key")
+    newest = max(os.path.getmtime(p) for p in (CALLS_SRC, os.path.join(ROOT, "include", "pagedserve_b200.h")))
+    if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= newest and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == key:
+                return
+    tmp = f"{CALLS}.{os.getpid()}.tmp"  # builds at once do not write into each other's
+    res = subprocess.run(cmd + ["-o", tmp], capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"building {CALLS_SRC} failed:\n{res.stdout}\n{res.stderr}")
-    os.replace(CALLS + ".tmp", CALLS)
+    os.replace(tmp, CALLS)
+    with open(f"{stamp}.{os.getpid()}.tmp", "w") as f:
+        f.write(key)
+    os.replace(f.name, stamp)
 
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> str:

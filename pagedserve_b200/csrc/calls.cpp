@@ -429,4 +429,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__calls() {
+  PyObject* m = PyModule_Create(&module);
+  // what it was compiled against (build.py's calls_target), for the loader to compare
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", PSB_BUILT_FOR) != 0) Py_CLEAR(m);
+  return m;
+}

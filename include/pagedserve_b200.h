@@ -477,7 +477,9 @@ size_t psb_paged_decode_int4_workspace_size(int32_t batch, int32_t q_heads, int3
  * K and V being the values the codes stand for; a sequence of length 0 gives
  * zeros.  query and out are of ``dtype`` = T.  The codes enter the products as
  * they are (exactly) and step and mid are applied to the sums in fp32, so the
- * only 16-bit rounding is that of step * probability before P V.  Unlike
+ * only 16-bit rounding is that of step * probability before P V.  Queries and
+ * keys may be as large as bf16 holds while scale * q . k and its terms stay below
+ * 2^117 (past that a result may be NaN).  Unlike
  * psb_paged_decode it reads nothing before its stream predecessor has ended:
  * lengths and tables may come from psb_extend_step.  Error behaviour is
  * psb_paged_decode's.

@@ -125,6 +125,7 @@ __device__ __forceinline__ void mma_f16_first(float* d, uint32_t a0, uint32_t a1
 constexpr float kGrowth = 4.f;     // a score may exceed the exponents' reference by this (log2) before it is moved
 constexpr int kPBits = 11;         // p step is scaled to at most 2^kGrowth 2^kPBits = 2^15
 constexpr float kTwo24 = 16777216.f;
+constexpr float kUnit = 1024.f;    // 2^24 (codes) over 2^14 (the largest |q|): of a unit of the scores' accumulator
 
 __device__ __forceinline__ int items_of(int ctx) { return ctx <= 0 ? 1 : (ctx + 31) >> 5; }
 
@@ -286,12 +287,16 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
   // adjacent rows, one run of memory.
   auto pi = [](int r) { return (r >> 1) + 4 * (r & 1); };
   uint32_t qb[HT][kM][2];         // B fragments of q
-  float qs[HT][2];                // sum(q) of heads 2 t, 2 t + 1
+  float qs[HT][2];                // sum(q) 2^(14 - qe) of heads 2 t, 2 t + 1
   float o[HT][kM][4];             // (element of row g | g + 8) x (head 2 t | 2 t + 1)
   float sp[HT][4];                // sums of the rounded, scaled p step
   float nref[HT][2];              // minus the exponents' reference
   float l[HT][2], z[HT][2];       // sum p, sum p mid
-  float kfac = 0.f;               // score of one unit of the accumulator, per step
+  // A unit of the accumulator is a score of 2^24 2^-14 2^qe sc per step, a unit of
+  // sum(q) 2^-14 2^qe sc per unit of the value: 2^qe (the head tile's largest |q|)
+  // last, as it may be anything bf16 holds.  (The former is up to 2^10 times the
+  // scores it makes up: those end at 2^117.)
+  float kexp = 1.f;               // 2^qe
   float vscale = 1.f, vlim = 0.f; // scale of p step; the largest step it allows
   int n_pieces = 0;
   const float sc = p.scale_log2;
@@ -421,9 +426,9 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
       }
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const int qe = top > 0.f ? max(-100, min(100, ilogb_f32(top))) : 0;
+      const int qe = top > 0.f ? max(-113, ilogb_f32(top)) : 0;
       const float qsc = exp2_int(14 - qe);
-      kfac = sc * kTwo24 * exp2_int(qe - 14);
+      kexp = exp2_int(qe);
 #pragma unroll
       for (int ht = 0; ht < HT; ++ht) {
         float sum = 0.f;
@@ -431,14 +436,16 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
         for (int w = 0; w < kWords; ++w) {
           const float2 a0 = unpack2<T>(x[ht][w].x), a1 = unpack2<T>(x[ht][w].y), a2 = unpack2<T>(x[ht][w].z),
                        a3 = unpack2<T>(x[ht][w].w);
-          sum += ((a0.x + a0.y) + (a1.x + a1.y)) + ((a2.x + a2.y) + (a3.x + a3.y));
           // elements (i, i + 4) of the word, for products 4 (w / 2) + i; odd
           // products' codes are 16 times as large
           const float q16 = qsc * 0.0625f;
-          qb[ht][4 * (w >> 1) + 0][w & 1] = pack2<__half>(a0.x * qsc, a2.x * qsc);
-          qb[ht][4 * (w >> 1) + 1][w & 1] = pack2<__half>(a0.y * q16, a2.y * q16);
-          qb[ht][4 * (w >> 1) + 2][w & 1] = pack2<__half>(a1.x * qsc, a3.x * qsc);
-          qb[ht][4 * (w >> 1) + 3][w & 1] = pack2<__half>(a1.y * q16, a3.y * q16);
+          const float2 b0 = make_float2(a0.x * qsc, a0.y * q16), b1 = make_float2(a1.x * qsc, a1.y * q16),
+                       b2 = make_float2(a2.x * qsc, a2.y * q16), b3 = make_float2(a3.x * qsc, a3.y * q16);
+          sum += (fmaf(16.f, b0.y, b0.x) + fmaf(16.f, b1.y, b1.x)) + (fmaf(16.f, b2.y, b2.x) + fmaf(16.f, b3.y, b3.x));
+          qb[ht][4 * (w >> 1) + 0][w & 1] = pack2<__half>(b0.x, b2.x);
+          qb[ht][4 * (w >> 1) + 1][w & 1] = pack2<__half>(b0.y, b2.y);
+          qb[ht][4 * (w >> 1) + 2][w & 1] = pack2<__half>(b1.x, b3.x);
+          qb[ht][4 * (w >> 1) + 3][w & 1] = pack2<__half>(b1.y, b3.y);
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -491,7 +498,8 @@ __global__ void __launch_bounds__(Geo<D, HT>::kThreads, 1) int4_decode_kernel(co
           vscale = nv;
         }
         // the code's -7.5 goes with mid
-        factors[lane] = make_float4(kp.x * kfac, fmaf(kp.x, -7.5f, kp.y) * sc, vp.x * vscale, vp.y);
+        factors[lane] = make_float4(kp.x * (sc * kUnit) * kexp, fmaf(kp.x, -7.5f, kp.y) * (sc * 0x1p-14f) * kexp,
+                                    vp.x * vscale, vp.y);
         load_par();
       }
       // ---- S^T = K Q^T ---------------------------------------------------------

@@ -448,3 +448,44 @@ def test_scales_of_either_sign(scale, dtype, d):
     want, tol = _want_decode(c, scale=scale)
     assert err == 0
     _close(got, want, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 2, 128), (24, 2, 64)])
+@pytest.mark.parametrize("power", [-110, 90, 105, 120])
+def test_decode_queries_at_the_ends_of_bf16(power, hq, hkv, d):
+    """Queries scaled by a power of two up to 2^120 (values to 2^122) and keys
+    by its inverse: the same scores, so the same outputs."""
+    c = _decode_case(40, [77, 2000, 16], hq, hkv, d, 16, torch.bfloat16)
+    want, tol = _want_decode(c)
+    c["q"] = (c["q"].double() * 2.0 ** power).bfloat16()
+    c["pp"][:, :, :, 0] = (c["pp"][:, :, :, 0].double() * 2.0 ** -power).bfloat16()
+    got, err = _decode(c)
+    assert err == 0
+    _close(got, want, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("power", [60, 114])
+def test_decode_scores_as_large_as_they_may_be(power, hq, hkv, d):
+    """Keys to 2^116, so scores to 2^117: where one score is ahead of the
+    others by more than their roundings, its value row is the result."""
+    c = _decode_case(41, [77, 2000, 5], hq, hkv, d, 16, torch.bfloat16)
+    for name in ("params", "pp"):
+        c[name][:, :, :, 0] = (c[name][:, :, :, 0].double() * 2.0 ** power).bfloat16()
+    got, err = _decode(c)
+    assert err == 0 and bool(torch.isfinite(got).all())
+    h, seen = ref.HALF_STEP[torch.bfloat16], 0
+    for b, n in enumerate(c["lens"]):
+        (k, _, _, _), (v, dev, _, _) = ref.sequence_rows(c["codes"], c["params"], c["layer"], c["table"][b], n, 16)
+        for a in range(hq):
+            kh = a // (hq // hkv)
+            s = (c["q"][b, a].double() @ k[kh].T) * d ** -0.5
+            best = s.topk(2)
+            # sums of D + 8 fp32 products of codes up to 15 and offsets: 2^-10 of the largest is far above their roundings
+            if best.values[0] - best.values[1] < 2.0 ** -10 * s.abs().max():
+                continue
+            seen += 1
+            at = int(best.indices[0])
+            tol = h * v[kh, at].abs() + h * dev[kh, at].abs() + 2.0 ** -20 * v[kh, at].abs() + 1e-12
+            assert bool(((got[b, a].double() - v[kh, at]).abs() <= tol).all())
+    assert seen > hq

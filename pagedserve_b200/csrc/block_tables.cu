@@ -14,7 +14,8 @@
 // Both are latency bound: integers only, a few hundred kilobytes at most, and
 // short code (a cold instruction cache costs a kernel of this size more than
 // its loads: the same work with 64-bit divisions, 40 KB of code, took 12.6 +
-// 8.2 us where this takes 9.6 + 6.8 us for 256 requests, by the profiler).  So positions and
+// 8.2 us where this takes 10.4 + 6.1 us for 256 requests, by the profiler; 10.0 us
+// for both in a replayed graph).  So positions and
 // counts are 32 bits (what is added to them is checked first), a division by
 // block_size is a shift where it is a power of two, and the grid walks rows of
 // the table instead of elements.

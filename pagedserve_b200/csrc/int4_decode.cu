@@ -7,9 +7,11 @@
 // that about eight CTAs per SM exist; a sequence of several chunks leaves
 // (max, sum, output) partials that int4_merge_kernel, launched next on the
 // same stream, joins in chunk order.  It is bound by its arithmetic (every code
-// becomes an fp32 product per q head): 256 sequences of 62 MB took 2069 us
-// where the tensor-core path takes 25, so 16-bit types come here only for
-// geometries that path does not take.
+// becomes an fp32 product per q head): 256 sequences of 62 MB in blocks of 8 take
+// 1546 us where the tensor-core path takes 26 in blocks of 16, so 16-bit types
+// come here only for what that path does not take: head_dim other than 64 and
+// 128, block_size no multiple of 16, rows of q or out off 16 bytes, more than
+// 2560 sequences.
 #include <algorithm>
 
 #include "common.cuh"

@@ -26,16 +26,19 @@
 //
 // What bounds it.  A 16-token tile of head_dim 64 is 1152 bytes against 4096
 // in bf16, so the same bytes per second need 3.6 times the instructions of
-// paged_decode: the issue slots of the four schedulers bound it next to HBM
-// (about 150 instructions and 240 cycles a tile and scheduler).  Hence codes by
-// AND, two tiles at a time (independent work, one vote and one set of loop
-// instructions for both), each token's four factors worked out by one lane and
-// handed round through shared memory, the exponents' reference folded into the
-// score's multiply-add, and addresses and validity worked out for 32 items at
-// once, one per lane.  Measured: 256 sequences of 62 MB of cache 26.1 us (2.4
-// TB/s; the 16-bit pool's paged_decode 39 us), of which some 7 us do not depend
-// on the length; 3 sequences of 32 K tokens 13.3 us, of 128 K 10 us more (4 TB/s);
-// 64 sequences of 4 K at head_dim 128 43.9 us (3.5 TB/s).  Reading lengths and
+// paged_decode (about 150 a tile): hence codes by AND, two tiles at a time
+// (independent work, one vote and one set of loop instructions for both), each
+// token's four factors worked out by one lane and handed round through shared
+// memory, the exponents' reference folded into the score's multiply-add, and
+// addresses and validity worked out for 32 items at once, one per lane.  They
+// take 43% of the issue slots now (37% at head_dim 128, ALU 40%): what is left is
+// latency.  A scheduler has three warps (two at head_dim 128) to cover it, each
+// with one item's codes on their way; the stalls per issue are loads 1.8 (long
+// scoreboard), fixed-latency results 1.3, shared memory 0.6.  Measured: 256
+// sequences of 62 MB of cache 26.2 us (2.4 TB/s; the 16-bit pool's paged_decode
+// 39 us), of which some 7 us do not depend on the length; 3 sequences of 32 K
+// tokens 13.4 us, of 128 K 10 us more (4 TB/s); 64 sequences of 4 K at head_dim
+// 128 43.7 us (3.5 TB/s).  Reading lengths and
 // tables before the wait for the stream predecessor saved 0.6 to 1.5 us a call,
 // but a predecessor that starts its dependents early (or has just left the GPU)
 // may not have written them yet.

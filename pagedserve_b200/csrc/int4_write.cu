@@ -16,7 +16,7 @@
 // pairs l, l + 32, ... and a pair is one byte of codes.
 //
 // Measured, write and read-back together: a 16 K-token pack of 14 + 2 heads of
-// head_dim 64 21.9 us (86 MB: 3.9 TB/s, 60% of the copy rate; a warp per row
+// head_dim 64 22.2 us (86 MB: 3.9 TB/s, 60% of the copy rate; a warp per row
 // took 131 us, a division per code 42 us, index divisions and conversions of
 // codes by instructions of their own 25.5 us), 1333 plain tokens of 8 heads of
 // 128 in f16 8.8 us, 256 tokens 4.4 us.  Instructions, not HBM, are what is

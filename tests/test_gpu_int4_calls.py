@@ -181,5 +181,5 @@ def test_a_full_launch_queue_stops_no_other_thread(name):
         last, gap = now, max(gap, now - last)
     worker.join()
     torch.cuda.synchronize()
-    assert took[0] > 0.4  # the queue was full
-    assert gap < 0.25
+    assert took[0] > 0.4  # the queue was full, most of that time
+    assert gap < took[0] / 2

@@ -50,9 +50,11 @@ enum {
   PSB_DEVERR_TIMEOUT = 16,      /* an async copy / MMA wait exceeded its bound */
   PSB_DEVERR_SEQLENS = 32,      /* cu_seqlens not non-decreasing within [0, total] */
   PSB_DEVERR_LIMIT = 64,        /* psb_select_tokens: a row had no tokens left to generate */
-  PSB_DEVERR_POOL = 128,        /* extend_step / trim_tables: not enough free blocks, or a malformed free list */
-  PSB_DEVERR_ROWS = 256,        /* extend_step / trim_tables: a store row named twice */
-  PSB_DEVERR_REFUSED = 512      /* an extend_step was refused: table calls refuse until this is cleared */
+  PSB_DEVERR_POOL = 128,        /* table calls: not enough free blocks, or a malformed free list */
+  PSB_DEVERR_ROWS = 256,        /* table calls: a store row named twice */
+  PSB_DEVERR_REFUSED = 512,     /* an extend_step or fork_tables was refused: table calls refuse until this is cleared */
+  PSB_DEVERR_SHARED = 1024,     /* release_tables: a block that would be kept in part has other holders */
+  PSB_DEVERR_LOGITS = 2048      /* verify_tokens: a row or a temperature that stands for no probabilities */
 };
 
 /* per-row status bits written by psb_select_tokens */
@@ -572,6 +574,118 @@ int psb_trim_tables(int32_t* table_store, int64_t store_stride, int32_t store_ro
                     const int32_t* req_rows, const int32_t* held_lens, const int32_t* keep_lens, int32_t batch,
                     int32_t* free_blocks, int32_t num_blocks, int32_t* free_state, int32_t block_size,
                     int32_t* error_flag, psb_stream_t stream);
+
+/*
+ * fork_tables: rows that share their parents' pages.  Entry b makes row
+ * child_rows[b] of the table store (which must hold nothing) a continuation of the
+ * first lens[b] tokens of row parent_rows[b]: it shares the whole blocks among
+ * them, and where lens[b] ends inside a block it gets one of its own from the head
+ * of the free ring (in entry order; the ring is psb_extend_step's).  copy_src[b] /
+ * copy_dst[b] (int32 [batch]) name the blocks whose contents have to be copied for
+ * that, psb_copy_blocks' arguments; -1 where there is nothing to copy.
+ * ``shares`` int32 [2, num_blocks], zero when every block has one holder at most:
+ * its first row counts a block's holders beyond the first, the second is scratch
+ * of psb_release_tables and zero between calls.  Blocks that extend_step hands out
+ * need no entry there; rows that share blocks give them back with
+ * psb_release_tables, not psb_trim_tables.  A child may not be a parent of the same
+ * call; one parent may have many children.  child_rows[b] < 0 is padding.
+ *
+ * Refused as a whole and flagged, changing nothing but copy_src and copy_dst (all
+ * -1), like an extend_step: PSB_DEVERR_CONTEXT (a row or length out of range),
+ * PSB_DEVERR_ROWS (a child named twice or as a parent), PSB_DEVERR_POOL (not
+ * enough free blocks), PSB_DEVERR_BLOCK_RANGE (an id outside the pool), with
+ * PSB_DEVERR_REFUSED, under which it refuses in turn.
+ */
+int psb_fork_tables(int32_t* table_store, int64_t store_stride, int32_t store_rows, int32_t store_width,
+                    const int32_t* parent_rows, const int32_t* child_rows, const int32_t* lens, int32_t batch,
+                    int32_t* shares, int32_t* free_blocks, int32_t num_blocks, int32_t* free_state,
+                    int32_t block_size, int32_t* copy_src, int32_t* copy_dst, int32_t* error_flag,
+                    psb_stream_t stream);
+
+/*
+ * release_tables: psb_trim_tables for rows that may share blocks.  Entry b of
+ * held_lens[b] tokens keeps keep_lens[b] of them.  Of the blocks behind those, in
+ * entry and table order, one that others hold too loses a holder (shares), any other
+ * goes to the tail of the ring; the entries become 0.  Checked and refused as a
+ * whole like psb_trim_tables; also PSB_DEVERR_SHARED where a row would keep a part
+ * of a block (and write to the rest of it) that others still hold behind the call,
+ * PSB_DEVERR_POOL where a block is released more often than it is held.
+ */
+int psb_release_tables(int32_t* table_store, int64_t store_stride, int32_t store_rows, int32_t store_width,
+                       const int32_t* req_rows, const int32_t* held_lens, const int32_t* keep_lens, int32_t batch,
+                       int32_t* shares, int32_t* free_blocks, int32_t num_blocks, int32_t* free_state,
+                       int32_t block_size, int32_t* error_flag, psb_stream_t stream);
+
+/*
+ * copy_blocks: block dst[i] of every layer and pool becomes what block src[i] is.
+ * ``pools`` and ``block_bytes`` are host arrays: up to four pools of num_layers x
+ * num_blocks blocks of that many bytes back to back.  A pair with a negative id is
+ * skipped, one with an id past the pool is skipped and flagged
+ * (PSB_DEVERR_BLOCK_RANGE).  The destinations are distinct and none is a source.
+ */
+int psb_copy_blocks(void* const* pools, const int64_t* block_bytes, int32_t num_pools, const int32_t* src,
+                    const int32_t* dst, int32_t pairs, int32_t num_layers, int64_t num_blocks, int32_t* error_flag,
+                    psb_stream_t stream);
+
+/*
+ * paged_decode_shared: psb_paged_decode for a batch whose sequences share long
+ * prefixes.  Sequences cu_groups[g] .. cu_groups[g + 1] - 1 (int32 [num_groups + 1],
+ * non-decreasing within [0, batch]) agree in their first prefix_lens[g] tokens: their
+ * tables name the same blocks there, or blocks of the same contents.  Those are read
+ * once per group, through the table of its longest sequence (the first of them), and
+ * a prefix ends with that sequence at the latest; a sequence shorter than its
+ * prefix sees its own context_lens[b] tokens of it, one of none gets zeros.
+ * Sequences of no group, or alone in one, are read on their own.
+ * Taken: bf16/f16, head_dim 64 or 128, up to 16 q heads per kv head, block sizes 16,
+ * 32, 64 and multiples of 64, up to 2048 sequences and groups, query strides and bases
+ * of 16 bytes; PSB_ERR_UNSUPPORTED otherwise (psb_paged_decode answers those, one
+ * sequence at a time).  ``scale`` is positive.  Lengths, groups and tables are read
+ * behind the stream predecessor's end.  A malformed cu_groups is flagged
+ * (PSB_DEVERR_SEQLENS) and no prefix is shared; a length outside [0, max_context] or
+ * a negative prefix is flagged (PSB_DEVERR_CONTEXT) and clamped; a block outside the
+ * pool is flagged (PSB_DEVERR_BLOCK_RANGE), never read, and leaves the rows that
+ * see it unspecified.  The workspace (psb_paged_decode_shared_workspace_size, 0 for
+ * what is not taken) needs no initialisation; calls that overlap on the GPU need one
+ * each.  Probabilities are rounded to the cache's type before P V; all else is fp32.
+ */
+size_t psb_paged_decode_shared_workspace_size(int32_t batch, int32_t num_groups, int32_t q_heads,
+                                              int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                              int32_t max_context, int32_t dtype);
+int psb_paged_decode_shared(const void* query, int64_t q_stride_b, int64_t q_stride_h, void* out, int64_t o_stride_b,
+                            int64_t o_stride_h, const void* k_cache, const void* v_cache, const int32_t* block_tables,
+                            int64_t table_stride, const int32_t* context_lens, const int32_t* cu_groups,
+                            const int32_t* prefix_lens, int32_t batch, int32_t num_groups, int32_t q_heads,
+                            int32_t layer, int32_t num_layers, int64_t num_blocks, int32_t num_kv_heads,
+                            int32_t block_size, int32_t head_dim, int32_t dtype, int32_t max_context, float scale,
+                            void* workspace, size_t workspace_bytes, int32_t* error_flag, psb_stream_t stream);
+
+/*
+ * verify_tokens: drafted tokens against the target's probabilities, with given random
+ * numbers; without drafts, sampling at a temperature.
+ *
+ * Sequence b has rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of the step: it was fed
+ * ``tokens`` [total] int64 there (the last token it has, then its drafts), and the
+ * row of ``logits`` [total, vocab] (dtype, row stride ``row_stride``) of each stands for
+ * p = softmax(logits / temperature[b]), or, where that fp32 temperature is 0, all of p
+ * on the first maximum (NaN counted largest, as psb_select_tokens).  Draft tokens[r + 1] is
+ * judged by row r: with q the row of ``draft_probs`` [total, vocab] (probs_dtype; what the
+ * draft was drawn from; NULL: all of q on the draft), it is taken if
+ * uniforms[r, 0] q(d) < p(d).  At the first row whose draft is not taken the new token
+ * is drawn from max(p - q, 0) (from p where that is nothing), at the sequence's last row,
+ * or one whose draft is outside [0, vocab), from p: the first token whose cumulative
+ * weight is above uniforms[r, 1] times the sum.  uniforms [total, 2] fp32 in [0, 1).
+ * new_tokens [total] int64: the drafts taken and the new token from cu_seqlens[b] on, -1
+ * in all other rows; counts [batch] int32: how many (0 for a sequence of no rows).
+ * Sums, weights and comparisons are those of 64-bit arithmetic.  A row with a NaN, with
+ * +infinity or with nothing but -infinity, and a temperature that is NaN, negative or
+ * infinite, are treated as temperature 0 and flagged (PSB_DEVERR_LOGITS); entries of
+ * draft_probs that are NaN or negative count as 0.  A malformed cu_seqlens is flagged
+ * (PSB_DEVERR_SEQLENS), the sequence's count 0.
+ */
+int psb_verify_tokens(const void* logits, int64_t row_stride, int32_t total, int32_t vocab, int32_t dtype,
+                      const int64_t* tokens, const int32_t* cu_seqlens, int32_t batch, const float* uniforms,
+                      const float* temperature, const void* draft_probs, int64_t probs_stride, int32_t probs_dtype,
+                      int64_t* new_tokens, int32_t* counts, int32_t* error_flag, psb_stream_t stream);
 
 /*
  * bounded_wait_check: a self-test with no counterpart in the reference.  One

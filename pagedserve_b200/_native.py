@@ -27,7 +27,9 @@ DEVERR_BITS = {
     64: "a row had no tokens left to generate",
     128: "not enough free blocks, or a malformed free list",
     256: "a table-store row was named twice",
-    512: "an extend_step was refused (table calls refuse until the flag is cleared)",
+    512: "an extend_step or fork_tables was refused (table calls refuse until the flag is cleared)",
+    1024: "a block that would be kept in part has other holders",
+    2048: "a row of logits or a temperature that stands for no probabilities",
 }
 
 _c_void_p, _i32, _i64, _f32, _sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
@@ -117,6 +119,22 @@ SIGNATURES = {
     "psb_trim_tables": (ctypes.c_int, [
         _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _i32, _c_void_p, _i32,
         _c_void_p, _c_void_p]),
+    "psb_fork_tables": (ctypes.c_int, [
+        _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p, _i32, _c_void_p,
+        _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "psb_release_tables": (ctypes.c_int, [
+        _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p, _i32, _c_void_p,
+        _i32, _c_void_p, _c_void_p]),
+    "psb_copy_blocks": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p, _i32, _i32, _i64, _c_void_p, _c_void_p]),
+    "psb_paged_decode_shared_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "psb_paged_decode_shared": (ctypes.c_int, [
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,
+        _c_void_p, _i32, _i32, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _c_void_p, _sz, _c_void_p,
+        _c_void_p]),
+    "psb_verify_tokens": (ctypes.c_int, [
+        _c_void_p, _i64, _i32, _i32, _i32, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p, _i64, _i32,
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
 }
 
 _lock = threading.Lock()

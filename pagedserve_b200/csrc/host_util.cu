@@ -241,6 +241,23 @@ bool encode_row_groups_map(CUtensorMap* map, const void* base, int64_t rows, int
   return true;
 }
 
+bool encode_box_map(CUtensorMap* map, const void* base, const int64_t dims[3], const int64_t strides[2], const int box[3],
+                    CUtensorMapDataType dt) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t d[3] = {static_cast<cuuint64_t>(dims[0]), static_cast<cuuint64_t>(dims[1]), static_cast<cuuint64_t>(dims[2])};
+  const cuuint64_t s[2] = {static_cast<cuuint64_t>(strides[0]), static_cast<cuuint64_t>(strides[1])};
+  const cuuint32_t b[3] = {static_cast<cuuint32_t>(box[0]), static_cast<cuuint32_t>(box[1]), static_cast<cuuint32_t>(box[2])};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, dt, 3, const_cast<void*>(base), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    g_last_cuda_error = 10000 + static_cast<int>(r);
+    return false;
+  }
+  return true;
+}
+
 bool encode_pool_map(CUtensorMap* map, const void* base, int64_t tiles, int block_size, int head_dim,
                      CUtensorMapDataType dt) {
   auto fn = encode_fn();

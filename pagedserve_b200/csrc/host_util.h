@@ -99,6 +99,11 @@ bool encode_rows_map(CUtensorMap* map, const void* base, int64_t rows, int heads
 bool encode_row_groups_map(CUtensorMap* map, const void* base, int64_t rows, int heads, int head_dim, int64_t row_stride,
                            int64_t head_stride, int box_heads, int box_rows, CUtensorMapDataType dt);
 
+// 3-D tiled map: ``dims`` elements (innermost first), ``strides`` bytes of the two
+// outer ones, box ``box``, 128-byte swizzle (box[0] elements are 128 bytes).
+bool encode_box_map(CUtensorMap* map, const void* base, const int64_t dims[3], const int64_t strides[2], const int box[3],
+                    CUtensorMapDataType dt);
+
 // 3D tensor map over a paged K or V pool [layers * blocks * kv heads tiles,
 // block_size rows, head_dim]: one box is one (layer, block, kv head) tile of
 // block_size x head_dim, 128-byte swizzled.

@@ -17,6 +17,11 @@
   write, read-back and attention over a pool of 4-bit codes
 * ``extend_step``, ``trim_tables``  ``pack_step`` with the block allocation
   on the device too, and its reverse (``BlockManager``'s free list as a ring)
+* ``fork_tables``, ``copy_blocks``, ``release_tables``  rows that share pages:
+  several continuations of one prompt
+* ``paged_decode_shared``  ``paged_decode`` for a batch that shares long prefixes
+* ``verify_tokens``      drafted tokens against the target's probabilities, and
+  sampling at a temperature, from given random numbers
 
 Every function requires CUDA tensors, launches on the current stream and
 returns without synchronising.  There is no CPU path.
@@ -1091,3 +1096,251 @@ def trim_tables(table_store: torch.Tensor, req_rows: torch.Tensor, held_lens: to
     _call(dev, _native.load().psb_trim_tables, "trim_tables",
           table_store.data_ptr(), *store, rows.data_ptr(), held_lens.data_ptr(), keep_lens.data_ptr(), bsz,
           free_blocks.data_ptr(), free_blocks.shape[0], free_state.data_ptr(), int(block_size), _ptr(error_flag))
+
+
+# -- several continuations of one prompt -------------------------------------------------------------------------
+
+
+def share_counts(num_blocks: int, device: torch.device | str) -> torch.Tensor:
+    """``shares`` for ``fork_tables`` and ``release_tables``: int32
+    ``[2, num_blocks]`` of zeros, every block of a pool with one holder at most."""
+    if num_blocks <= 0:
+        raise ValueError("num_blocks must be positive")
+    return torch.zeros((2, num_blocks), dtype=torch.int32, device=device)
+
+
+def _check_shares(shares: torch.Tensor, num_blocks: int) -> None:
+    if shares.dtype != torch.int32 or shares.shape != (2, num_blocks) or not shares.is_contiguous():
+        raise ValueError(f"shares must be a contiguous int32 [2, {num_blocks}] tensor like free_blocks")
+
+
+def fork_tables(table_store: torch.Tensor, parent_rows: torch.Tensor, child_rows: torch.Tensor, lens: torch.Tensor,
+                shares: torch.Tensor, free_blocks: torch.Tensor, free_state: torch.Tensor, block_size: int,
+                error_flag: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows that share their parents' pages (psb_fork_tables).
+
+    Entry b makes row ``child_rows[b]`` of ``table_store`` (which holds nothing)
+    a continuation of the first ``lens[b]`` tokens of row ``parent_rows[b]``: it
+    shares their whole blocks (counted in ``shares``, ``share_counts``), and where
+    they end inside a block it gets one of its own from the free ring.  Returns
+    ``(src, dst)`` int32 ``[B]``: the blocks ``copy_blocks`` has to copy for that
+    (-1: none).  One parent may have many children; a child is no parent of the
+    same call; ``child_rows[b] < 0`` is padding.  Rows that share blocks give them
+    back with ``release_tables`` (not ``trim_tables``).  Checked and refused as a
+    whole, like ``extend_step``.
+    """
+    store, bsz, parents, children, lens = _tables_args(table_store, parent_rows, child_rows, lens, free_blocks, free_state,
+                                                       ("parent_rows", "child_rows", "lens"), error_flag)
+    _check_shares(shares, free_blocks.shape[0])
+    if block_size <= 0:
+        raise ValueError("block_size must be positive")
+    dev = _cuda_index(table_store, parents, children, lens, shares, free_blocks, free_state, error_flag)
+    src, dst = lens.new_empty(bsz), lens.new_empty(bsz)
+    _call(dev, _native.load().psb_fork_tables, "fork_tables",
+          table_store.data_ptr(), *store, parents.data_ptr(), children.data_ptr(), lens.data_ptr(), bsz, shares.data_ptr(),
+          free_blocks.data_ptr(), free_blocks.shape[0], free_state.data_ptr(), int(block_size), src.data_ptr(),
+          dst.data_ptr(), _ptr(error_flag))
+    return src, dst
+
+
+def release_tables(table_store: torch.Tensor, req_rows: torch.Tensor, held_lens: torch.Tensor, keep_lens: torch.Tensor,
+                   shares: torch.Tensor, free_blocks: torch.Tensor, free_state: torch.Tensor, block_size: int,
+                   error_flag: torch.Tensor | None = None) -> None:
+    """``trim_tables`` for rows that may share blocks (psb_release_tables).
+
+    Of the blocks past what entry b keeps, in entry and table order, one that
+    others hold too loses a holder, any other goes to the tail of the free ring.
+    ``keep_lens[b]`` may end inside a block only if nobody else holds that block
+    afterwards: the call is refused otherwise (``error_flag`` 1024).
+    """
+    store, bsz, rows, held_lens, keep_lens = _tables_args(table_store, req_rows, held_lens, keep_lens, free_blocks,
+                                                          free_state, ("req_rows", "held_lens", "keep_lens"),
+                                                          error_flag)
+    _check_shares(shares, free_blocks.shape[0])
+    if block_size <= 0:
+        raise ValueError("block_size must be positive")
+    dev = _cuda_index(table_store, rows, held_lens, keep_lens, shares, free_blocks, free_state, error_flag)
+    _call(dev, _native.load().psb_release_tables, "release_tables",
+          table_store.data_ptr(), *store, rows.data_ptr(), held_lens.data_ptr(), keep_lens.data_ptr(), bsz,
+          shares.data_ptr(), free_blocks.data_ptr(), free_blocks.shape[0], free_state.data_ptr(), int(block_size),
+          _ptr(error_flag))
+
+
+def copy_blocks(pools, src: torch.Tensor, dst: torch.Tensor, error_flag: torch.Tensor | None = None) -> None:
+    """Block ``dst[i]`` of every layer becomes what block ``src[i]`` is, in each of
+    ``pools`` (psb_copy_blocks): up to four contiguous tensors ``[num_layers,
+    num_blocks, ...]`` of any types, e.g. ``(k_cache, v_cache)`` or ``(kv_codes,
+    kv_params)``.  ``src, dst [N]`` int32; a pair with a negative id is skipped.
+    Destinations are distinct and none is a source.
+    """
+    pools = tuple(pools)
+    if not 1 <= len(pools) <= 4:
+        raise ValueError("pools must be one to four tensors")
+    if src.dtype != torch.int32 or src.ndim != 1 or dst.dtype != torch.int32 or dst.shape != src.shape:
+        raise ValueError("src and dst must be int32 [N]")
+    lead = tuple(pools[0].shape[:2])
+    for x in pools:
+        if x.ndim < 3 or tuple(x.shape[:2]) != lead or not x.is_contiguous() or x.numel() == 0:
+            raise ValueError("pools must be contiguous [num_layers, num_blocks, ...] of the same layers and blocks")
+    _check_flag(error_flag)
+    src, dst = src.contiguous(), dst.contiguous()
+    dev = _cuda_index(*pools, src, dst, error_flag)
+    n = len(pools)
+    ptrs = (ctypes.c_void_p * n)(*[x.data_ptr() for x in pools])
+    sizes = (ctypes.c_int64 * n)(*[x.numel() // (lead[0] * lead[1]) * x.element_size() for x in pools])
+    _call(dev, _native.load().psb_copy_blocks, "copy_blocks", ptrs, sizes, n, src.data_ptr(), dst.data_ptr(), src.shape[0],
+          lead[0], lead[1], _ptr(error_flag))
+
+
+@functools.lru_cache(maxsize=1024)
+def decode_shared_workspace_bytes(batch: int, groups: int, q_heads: int, hkv: int, head_dim: int, block_size: int,
+                                  max_context: int, dtype: torch.dtype) -> int:
+    """Scratch of one ``paged_decode_shared`` call; 0 for a geometry that ``paged_decode`` answers in its place."""
+    return int(_native.load().psb_paged_decode_shared_workspace_size(batch, groups, q_heads, hkv, head_dim, block_size,
+                                                                     max_context, dtype_code(dtype)))
+
+
+def paged_decode_shared(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                        context_lens: torch.Tensor, cu_groups: torch.Tensor, prefix_lens: torch.Tensor, layer: int,
+                        scale: float | None = None, out: torch.Tensor | None = None, max_context: int | None = None,
+                        workspace: torch.Tensor | None = None, error_flag: torch.Tensor | None = None) -> torch.Tensor:
+    """``paged_decode`` for a batch whose sequences share long prefixes (psb_paged_decode_shared).
+
+    Sequences ``cu_groups[g] .. cu_groups[g + 1] - 1`` (int32 ``[G + 1]``) agree in
+    their first ``prefix_lens[g]`` tokens (int32 ``[G]``): their rows of
+    ``block_tables`` name the same blocks there (``fork_tables``), or blocks of the
+    same contents.  The prefix is read and multiplied once for the whole group, what
+    lies behind it sequence by sequence.  Sequences of no group are on their own;
+    one without tokens gets zeros.  Returns ``out`` with ``query``'s shape
+    (``[B, Hq, D]`` or ``[B, Hq, 1, D]``) and dtype.
+
+    Prefixes are shared for bf16/f16, head_dim 64 or 128, up to 16 q heads per kv
+    head, blocks of 16, 32, 64 or a multiple of 64 tokens, up to 2048 sequences; other
+    geometries are answered by ``paged_decode``, each sequence on its own.  ``scale`` must be positive.
+    """
+    nl, nb, hkv, bs, d = _pool_geometry(k_cache, v_cache)
+    q3 = query.squeeze(2) if query.ndim == 4 and query.shape[2] == 1 else query
+    if q3.ndim != 3 or q3.shape[2] != d:
+        raise ValueError("query must be [B, Hq, D] or [B, Hq, 1, D]")
+    bsz, hq, _ = q3.shape
+    if bsz == 0:
+        raise ValueError("Batch must not be empty")
+    if hq == 0 or hq % hkv:
+        raise ValueError("Query heads must be divisible by KV heads")
+    if q3.dtype != k_cache.dtype:
+        raise ValueError("Query dtype must match cache dtype")
+    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.shape[0] != bsz:
+        raise ValueError("block_tables must be int32 [B, max_blocks]")
+    if context_lens.dtype != torch.int32 or context_lens.shape != (bsz,):
+        raise ValueError("context_lens must be int32 [B]")
+    if prefix_lens.dtype != torch.int32 or prefix_lens.ndim != 1:
+        raise ValueError("prefix_lens must be int32 [G]")
+    groups = prefix_lens.shape[0]
+    if cu_groups.dtype != torch.int32 or cu_groups.shape != (groups + 1,):
+        raise ValueError("cu_groups must be int32 [G + 1]")
+    if not 0 <= layer < nl:
+        raise ValueError("Invalid layer")
+    width = block_tables.shape[1] * bs
+    max_context = width if max_context is None else int(max_context)
+    if not 0 <= max_context <= width:
+        raise ValueError(f"max_context must lie in [0, {width}] (the block tables' width)")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError("scale must be positive")
+    _check_flag(error_flag)
+    if out is None:
+        out = torch.empty_like(query)
+    o3 = out.squeeze(2) if out.ndim == 4 and out.shape[2] == 1 else out
+    if o3.shape != q3.shape or o3.stride(2) != 1 or o3.dtype != q3.dtype:
+        raise ValueError("out must match query's shape/dtype with unit stride along head_dim")
+    if block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    context_lens, cu_groups, prefix_lens = context_lens.contiguous(), cu_groups.contiguous(), prefix_lens.contiguous()
+    need = decode_shared_workspace_bytes(bsz, groups, hq, hkv, d, bs, max_context, q3.dtype)
+    if need == 0 or (k_cache.data_ptr() | v_cache.data_ptr()) & 15 or nl * nb * hkv > 0x7fffffff:
+        _cuda_index(q3, k_cache, v_cache, block_tables, context_lens, cu_groups, prefix_lens, out, error_flag)
+        with torch.cuda.device(q3.device):
+            paged_decode(q3, k_cache, v_cache, block_tables, context_lens, layer, scale=scale, out=o3, max_context=max_context,
+                         error_flag=error_flag)
+        return out
+    qs = q3.stride()
+    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or qs[0] <= 0 or qs[1] <= 0 or q3.data_ptr() & 15:
+        q3 = q3.contiguous() if not q3.is_contiguous() else q3.clone()
+        qs = (hq * d, d, 1)
+    dev = _cuda_index(q3, k_cache, v_cache, block_tables, context_lens, cu_groups, prefix_lens, out, workspace, error_flag)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q3.device)
+    else:
+        _check_workspace(workspace)
+    os_ = o3.stride()
+    _call(dev, _native.load().psb_paged_decode_shared, "paged_decode_shared",
+          q3.data_ptr(), qs[0], qs[1], o3.data_ptr(), os_[0], os_[1], k_cache.data_ptr(), v_cache.data_ptr(),
+          block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(), cu_groups.data_ptr(),
+          prefix_lens.data_ptr(), bsz, groups, hq, layer, nl, nb, hkv, bs, d, _DTYPES[q3.dtype], max_context, scale,
+          workspace.data_ptr(), workspace.nbytes, _ptr(error_flag))
+    return out
+
+
+def verify_tokens(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.Tensor, uniforms: torch.Tensor,
+                  temperature: torch.Tensor, draft_probs: torch.Tensor | None = None,
+                  error_flag: torch.Tensor | None = None, out: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Drafted tokens against the target's probabilities, from given random numbers (psb_verify_tokens).
+
+    Sequence b was fed ``tokens[cu_seqlens[b] : cu_seqlens[b + 1]]`` (int64
+    ``[T]``): its last token, then its drafts; ``logits [T, V]`` are the rows that
+    step gave.  Row r stands for ``p = softmax(logits[r] / temperature[b])`` (fp32
+    ``[B]``; 0: the first maximum); the draft ``d = tokens[r + 1]``, drawn from
+    ``q = draft_probs[r]`` (``[T, V]``; None: a draft that was looked up), is taken
+    if ``uniforms[r, 0] q(d) < p(d)`` (fp32 ``[T, 2]`` in [0, 1)).  At the first row
+    whose draft is not taken the new token is drawn from ``max(p - q, 0)`` with
+    ``uniforms[r, 1]``, at the last row (or one whose draft is -1) from p, so
+    the tokens are distributed as if each had been drawn from p.  A batch of
+    one row a sequence is plain sampling.
+
+    Returns ``(new_tokens [T] int64, counts [B] int32)`` (``out``: the same two):
+    sequence b's new tokens from ``cu_seqlens[b]`` on, -1 behind them, and how many;
+    its cache keeps ``counts[b]`` of the rows fed (``trim_tables`` takes the rest).
+    Decided as in 64-bit arithmetic.  A row without probabilities (NaN, +inf, all
+    -inf) is treated as temperature 0 and flagged (2048).
+    """
+    if logits.ndim != 2 or logits.shape[1] == 0:
+        raise ValueError("logits must be [T, V]")
+    t, v = (int(x) for x in logits.shape)
+    code = dtype_code(logits.dtype)
+    if logits.stride(1) != 1 or (t > 1 and logits.stride(0) < v):
+        logits = logits.contiguous()
+    if tokens.dtype != torch.int64 or tokens.shape != (t,):
+        raise ValueError("tokens must be int64 [T]")
+    if cu_seqlens.dtype != torch.int32 or cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens must be int32 [B + 1]")
+    b = cu_seqlens.shape[0] - 1
+    if b == 0 and t > 0:
+        raise ValueError("logits hold rows but cu_seqlens no sequence")
+    if uniforms.dtype != torch.float32 or uniforms.shape != (t, 2):
+        raise ValueError("uniforms must be float32 [T, 2]")
+    if temperature.dtype != torch.float32 or temperature.shape != (b,):
+        raise ValueError("temperature must be float32 [B]")
+    tokens, cu_seqlens, uniforms, temperature = (x.contiguous() for x in (tokens, cu_seqlens, uniforms, temperature))
+    qcode = 0
+    if draft_probs is not None:
+        if draft_probs.shape != (t, v):
+            raise ValueError("draft_probs must be [T, V] like logits")
+        qcode = dtype_code(draft_probs.dtype)
+        if draft_probs.stride(1) != 1 or (t > 1 and draft_probs.stride(0) < v):
+            draft_probs = draft_probs.contiguous()
+    _check_flag(error_flag)
+    if out is None:
+        new, counts = tokens.new_empty(t), cu_seqlens.new_empty(b)
+    else:
+        new, counts = out
+        if (new.dtype != torch.int64 or new.shape != (t,) or not new.is_contiguous() or counts.dtype != torch.int32
+                or counts.shape != (b,) or not counts.is_contiguous()):
+            raise ValueError("out must be contiguous (new_tokens [T] int64, counts [B] int32)")
+        if t and new.data_ptr() == tokens.data_ptr():
+            raise ValueError("new_tokens may not be tokens itself")
+    dev = _cuda_index(logits, tokens, cu_seqlens, uniforms, temperature, draft_probs, new, counts, error_flag)
+    _call(dev, _native.load().psb_verify_tokens, "verify_tokens",
+          logits.data_ptr(), logits.stride(0), t, v, code, tokens.data_ptr(), cu_seqlens.data_ptr(), b, uniforms.data_ptr(),
+          temperature.data_ptr(), _ptr(draft_probs), 0 if draft_probs is None else draft_probs.stride(0), qcode,
+          new.data_ptr(), counts.data_ptr(), _ptr(error_flag))
+    return new, counts

@@ -676,16 +676,20 @@ int psb_paged_decode_shared(const void* query, int64_t q_stride_b, int64_t q_str
  * weight is above uniforms[r, 1] times the sum.  uniforms [total, 2] fp32 in [0, 1).
  * new_tokens [total] int64: the drafts taken and the new token from cu_seqlens[b] on, -1
  * in all other rows; counts [batch] int32: how many (0 for a sequence of no rows).
- * Sums, weights and comparisons are those of 64-bit arithmetic.  A row with a NaN, with
- * +infinity or with nothing but -infinity, and a temperature that is NaN, negative or
- * infinite, are treated as temperature 0 and flagged (PSB_DEVERR_LOGITS); entries of
- * draft_probs that are NaN or negative count as 0.  A malformed cu_seqlens is flagged
- * (PSB_DEVERR_SEQLENS), the sequence's count 0.
+ * Decided as 64-bit arithmetic does, but that weights below 2^-900 of a row's largest
+ * are none.  A row that stands for no probabilities (a NaN, +infinity, nothing but
+ * -infinity) takes no draft, gives its first maximum and is flagged
+ * (PSB_DEVERR_LOGITS); a temperature that is NaN, negative or infinite is flagged and
+ * taken for 0; entries of draft_probs that are NaN or negative count as 0.  A
+ * malformed cu_seqlens is flagged (PSB_DEVERR_SEQLENS), the sequence's count 0.  The
+ * workspace needs no initialisation; calls that overlap on the GPU need one each.
  */
+size_t psb_verify_tokens_workspace_size(int32_t batch);
 int psb_verify_tokens(const void* logits, int64_t row_stride, int32_t total, int32_t vocab, int32_t dtype,
                       const int64_t* tokens, const int32_t* cu_seqlens, int32_t batch, const float* uniforms,
                       const float* temperature, const void* draft_probs, int64_t probs_stride, int32_t probs_dtype,
-                      int64_t* new_tokens, int32_t* counts, int32_t* error_flag, psb_stream_t stream);
+                      int64_t* new_tokens, int32_t* counts, void* workspace, size_t workspace_bytes,
+                      int32_t* error_flag, psb_stream_t stream);
 
 /*
  * bounded_wait_check: a self-test with no counterpart in the reference.  One

@@ -73,6 +73,20 @@ bool prefer_max_shared(const void* func) {
   return true;
 }
 
+bool prefer_shared_percent(const void* func, int percent) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const auto key = std::make_pair(dev, reinterpret_cast<uintptr_t>(func));
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (!g_l1_set.insert(key).second) return true;
+  const cudaError_t e = cudaFuncSetAttribute(func, cudaFuncAttributePreferredSharedMemoryCarveout, percent);
+  if (e != cudaSuccess) {
+    g_l1_set.erase(key);
+    return record_cuda_error(e), false;
+  }
+  return true;
+}
+
 bool prefer_max_l1(const void* func) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return false;

@@ -30,6 +30,10 @@ bool prefer_max_shared(const void* func);
 // bytes in flight.
 bool prefer_max_l1(const void* func);
 
+// The same, but with ``percent`` of the largest shared-memory carve-out, for
+// kernels that need a little of it.
+bool prefer_shared_percent(const void* func, int percent);
+
 // CTAs of ``func`` that fit on one SM at ``threads`` threads and ``smem``
 // dynamic shared bytes under the full carve-out: registers (per warp, in
 // units of 256), shared memory (plus static and the per-CTA reservation),

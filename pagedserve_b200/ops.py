@@ -1301,7 +1301,7 @@ def verify_tokens(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     sequence b's new tokens from ``cu_seqlens[b]`` on, -1 behind them, and how many;
     its cache keeps ``counts[b]`` of the rows fed (``trim_tables`` takes the rest).
     Decided as in 64-bit arithmetic.  A row without probabilities (NaN, +inf, all
-    -inf) is treated as temperature 0 and flagged (2048).
+    -inf) takes no draft, gives its first maximum and is flagged (2048).
     """
     if logits.ndim != 2 or logits.shape[1] == 0:
         raise ValueError("logits must be [T, V]")
@@ -1339,8 +1339,9 @@ def verify_tokens(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
         if t and new.data_ptr() == tokens.data_ptr():
             raise ValueError("new_tokens may not be tokens itself")
     dev = _cuda_index(logits, tokens, cu_seqlens, uniforms, temperature, draft_probs, new, counts, error_flag)
+    workspace = torch.empty(max(1, 2 * b), dtype=torch.int64, device=logits.device)  # 16 bytes a sequence
     _call(dev, _native.load().psb_verify_tokens, "verify_tokens",
           logits.data_ptr(), logits.stride(0), t, v, code, tokens.data_ptr(), cu_seqlens.data_ptr(), b, uniforms.data_ptr(),
           temperature.data_ptr(), _ptr(draft_probs), 0 if draft_probs is None else draft_probs.stride(0), qcode,
-          new.data_ptr(), counts.data_ptr(), _ptr(error_flag))
+          new.data_ptr(), counts.data_ptr(), workspace.data_ptr(), workspace.nbytes, _ptr(error_flag))
     return new, counts

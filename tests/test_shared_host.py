@@ -147,9 +147,10 @@ def test_c_entries_refuse_without_a_gpu():
     for kw in (dict(dt=0), dict(d=96), dict(bs=8), dict(qb=895), dict(q=p + 2), dict(qb=0)):
         assert dec(**kw) == unsup
     assert dec() == ws and dec(ws=p, wsn=64) == ws and dec(batch=0) == 0
-    ver = lambda **kw: lib.psb_verify_tokens(*{**dict(x=p, rs=30, t=5, v=30, dt=0, tok=p, cu=p, b=2, u=p, heat=p, q=None, qs=0, qd=0, out=p, n=p, err=None,
-                                                      s=None), **kw}.values())
+    ver = lambda **kw: lib.psb_verify_tokens(*{**dict(x=p, rs=30, t=5, v=30, dt=0, tok=p, cu=p, b=2, u=p, heat=p, q=None, qs=0, qd=0, out=p, n=p, ws=p,
+                                                      wsn=64, err=None, s=None), **kw}.values())
     for kw in (dict(t=-1), dict(v=0), dict(b=-1), dict(rs=29), dict(dt=9), dict(q=p, qs=29), dict(q=p, qs=30, qd=9), dict(b=0), dict(x=None), dict(heat=None),
                dict(x=p + 1), dict(out=None)):
         assert ver(**kw) == inv
     assert ver(t=0, b=0) == 0
+    assert ver(ws=None) == ws and ver(ws=p + 8) == ws and ver(wsn=31) == ws and lib.psb_verify_tokens_workspace_size(2) == 32

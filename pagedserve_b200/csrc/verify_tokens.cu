@@ -10,8 +10,8 @@
 // above u1 times the weights' sum.  Tokens so emitted are distributed as if each
 // had been drawn from p.  Without drafts it is sampling at a temperature.
 //
-// One cluster of CTAs per sequence.  It reads the sequence's rows in batches of four,
-// each warp a consecutive part of one row: the maximum, its place at temperature 0,
+// One cluster of CTAs per sequence.  It reads the sequence's rows in batches (of
+// four; few sequences, bound by latency: of eight), each warp a consecutive part of one row: the maximum, its place at temperature 0,
 // and the sum of exponentials in one pass, joined through distributed shared memory.
 // Rows behind the first rejection are not read by later batches.  The sample is
 // then found in the part that the random number falls in, cut once more for all of
@@ -47,9 +47,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCtas = 16;      // CTAs of a cluster
-constexpr int kMaxRows = 4;       // rows read before the drafts among them are looked at
+constexpr int kMaxRows = 8;       // rows read before the drafts among them are looked at, at most
 constexpr int kOwnElems = 96;     // of the vocabulary per thread of a sequence up to which it does its 64-bit work itself
-constexpr int kRestCtas = 8;      // of a cluster of the second launch
 constexpr float kErr = 1.8e-6f;   // of an fp32 weight or a sum of them, relative
 constexpr float kLargest = 1 << 20;  // octaves that logits may span for fp32
 
@@ -578,6 +577,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
   const int seq = blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   fill_table(s_sums);
+  if (tid == 0) s_found = 0;
   cl.group.sync();  // every CTA has begun: its shared memory may be read and written
   pdl_wait();
   if (kLater) pdl_launch_dependents();
@@ -608,10 +608,12 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
   auto in_fp32 = [&](float m) { return c > 1e-30 && c < 1e30 && fabsf(m * fast.c) < kLargest; };
 
   // ---- the rows, until a draft is not taken ---------------------------------------
+  // rows behind a rejection are read for nothing, but a batch takes 5 us however few its rows
+  const int most = ctas == kMaxCtas ? kMaxRows : kMaxRows / 2;
   int stop = r1 - 1, in_batch = 0, wpr = kWarps;
 #pragma unroll 1
-  for (int b0 = r0, batch = 0; b0 < r1; b0 += kMaxRows, ++batch) {
-    const int rows = min(kMaxRows, r1 - b0);
+  for (int b0 = r0, batch = 0; b0 < r1; b0 += most, ++batch) {
+    const int rows = min(most, r1 - b0);
     if (batch > 0) __syncthreads();  // s_part and s_row are read no more
     // what the drafts' tests need, on its way
     int d = -1;
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
       }
     }
     // wpr warps of every CTA to a row, each a part of it
-    wpr = rows == 1 ? kWarps : rows == 2 ? kWarps / 2 : kWarps / 4;
+    wpr = rows == 1 ? kWarps : rows == 2 ? kWarps / 2 : rows <= 4 ? kWarps / 4 : kWarps / 8;
     const int i = warp / wpr;
     if (i < rows) {
       const Row<T> row = row_of<T>(p, b0 + i);
@@ -789,7 +791,6 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
   const double u = static_cast<double>(__ldg(p.uniforms + 2 * static_cast<int64_t>(stop) + 1));
   if (mode != kRest && in_fp32(top) && u >= 1e-18) {
     // from the sums that are there; (a target of 0 falls on the first token of any weight, however small)
-    if (tid == 0) s_found = 0;
     if (tid < wpr) s_of_part[tid] = s_part[in_batch][tid].sum * power(s_part[in_batch][tid].octave - at_stop.octave);
     fast.unit(at_stop.octave);
     const int of_d = mode == kWithout ? (d + row.skip) / n : -1;
@@ -819,8 +820,6 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
       __syncthreads();
       if (tid < kWarps) s_sums.warp[tid] = tid < wpr ? s_of_part[tid] : 0.0;
       sums = cl.exchange();
-    } else {
-      cl.group.sync();  // (s_found is set up)
     }
     const double target = u * all_of(sums, ctas), room = 2.0 * kErr * target;
     double run = 0;
@@ -942,7 +941,11 @@ int launch(const VerifyParams& p, cudaStream_t s) {
   }
   discard_stale_error();
   cudaError_t e = launch_clusters(kern, p.batch, ctas, p, s);
-  if (e == cudaSuccess && later) e = launch_clusters(rest, std::min(p.batch, std::max(1, 2 * sms / kRestCtas)), kRestCtas, p, s);
+  // Small clusters for many draws, larger ones for few: drafts with probabilities are
+  // mostly drawn for, samples one in ten (of 256: eight CTAs 48 us, four 53; all of
+  // 256: 172 and 127).
+  const int more = p.probs != nullptr || p.batch > 2 * sms ? 4 : 8;
+  if (e == cudaSuccess && later) e = launch_clusters(rest, std::min(p.batch, std::max(1, 2 * sms / more)), more, p, s);
   if (e != cudaSuccess) return record_cuda_error(e);
   return check_launch();
 }

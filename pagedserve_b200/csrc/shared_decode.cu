@@ -211,6 +211,42 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// The products and their commits, by the one lane for which ``on`` holds, in code
+// that the whole warp runs through: operands then stay in uniform registers (issued
+// from a branch of one lane, each product took 70 cycles for its operands' moves).
+__device__ __forceinline__ void mma_ss(bool on, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(static_cast<uint32_t>(on))
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(bool on, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(static_cast<uint32_t>(on))
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(bool on, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(static_cast<uint32_t>(on))
+      : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+  return on != 0;
+}
+// mbar_wait by a whole warp: its lanes give up together or not at all.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+
 // A run of steps of one tile.
 struct Run {
   int kvh, tile, grp, b0, n_seq;  // tile of its kv head, group, first sequence and how many
@@ -257,16 +293,15 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
   uint64_t* const bar_q = reinterpret_cast<uint64_t*>(smem + Geo::kOffBars);
+  // of step x, its stage x % kStages (a barrier's next phase needs this one's products):
   uint64_t* const bar_k = bar_q + 1;               // [kStages] K landed
-  uint64_t* const bar_kfree = bar_k + kStages;     // [kStages] Q K^T done
-  uint64_t* const bar_v = bar_kfree + kStages;     // [kStages] V landed
-  uint64_t* const bar_vfree = bar_v + kStages;     // [kStages] P V done
-  uint64_t* const bar_s = bar_vfree + kStages;     // [2] S written
-  uint64_t* const bar_p = bar_s + 2;               // [2] P written over it
-  uint64_t* const bar_pv = bar_p + 2;              // [2] P V done
-  uint64_t* const bar_drain = bar_pv + 2;          // after a failed wait: every product issued so far is done
+  uint64_t* const bar_s = bar_k + kStages;         // [kStages] Q K^T done: S written, the stage's K free
+  uint64_t* const bar_v = bar_s + kStages;         // [kStages] V landed
+  uint64_t* const bar_pv = bar_v + kStages;        // [kStages] P V done: the stage's V free
+  uint64_t* const bar_p = bar_pv + kStages;        // [2] P written over S, in S buffer x & 1
+  uint64_t* const bar_drain = bar_p + 2;           // after a failed wait: every product issued so far is done
   uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bar_drain + 1);
-  static_assert((8 + 4 * kStages) * 8 + 4 <= 256, "barriers fit their area");
+  static_assert((4 + 4 * kStages) * 8 + 4 <= 256, "barriers fit their area");
   const Plan plan(reinterpret_cast<int32_t*>(smem + Geo::kOffPlan), p.batch, p.groups);
   int32_t* const tfirst = plan.lead + p.groups;    // [groups + 1] tiles before a group, of one kv head
   int32_t* const sfirst = tfirst + p.groups + 1;   // [groups + 1] steps before a group, of one kv head
@@ -276,15 +311,11 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     mbar_init(bar_q, 1);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(bar_k + i, 1);
-      mbar_init(bar_kfree + i, 1);
-      mbar_init(bar_v + i, 1);
-      mbar_init(bar_vfree + i, 1);
-    }
-    for (int i = 0; i < 2; ++i) {
       mbar_init(bar_s + i, 1);
-      mbar_init(bar_p + i, kRows);
+      mbar_init(bar_v + i, 1);
       mbar_init(bar_pv + i, 1);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(bar_p + i, kRows);
     mbar_init(bar_drain, 1);
     fence_barrier_init();
   }
@@ -351,102 +382,97 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   bool fail = false;
 
   if (warp == 4) {
-    if (lane == 0) {
-      constexpr int kFmt = Elem<T>::code == PSB_BF16 ? 1 : 0;
-      const uint32_t idesc_s = umma_idesc_f16(kFmt, kRows, kBN, 0, 0);
-      const uint32_t idesc_o = umma_idesc_f16(kFmt, kRows, kHalf, 0, 1);
-      const uint32_t s_base = smem_u32(smem);
-      const uint64_t dq = umma_desc_sw128(s_base, 1024, 16);
-      const uint64_t dk = umma_desc_sw128(s_base + Geo::kOffK, 1024, 16);
-      const uint64_t dv = umma_desc_sw128(s_base + Geo::kOffV, 1024, 8192);
-      prefetch_tmap(&tm_q);
-      const uint32_t box = static_cast<uint32_t>(TQ * group) * 128 * kH;
-      Cursor sc = first, oc = first;
-      int s_left = 0, o_left = 0, q_seen = 0;
-      uint32_t k_st = 0, k_ph = 0, v_st = 0, v_ph = 0;
-      bool begins = false, q_flight = false;
-      // step i uses S buffer i & 1, for the (i >> 1)-th time; S runs two steps ahead of O
+    // ---- products ----
+    constexpr int kFmt = Elem<T>::code == PSB_BF16 ? 1 : 0;
+    constexpr uint32_t idesc_s = umma_idesc_f16(kFmt, kRows, kBN, 0, 0), idesc_o = umma_idesc_f16(kFmt, kRows, D, 0, 1);
+    const bool on = elect_one();
+    const uint32_t s_base = smem_u32(smem);
+    const uint64_t dq = umma_desc_sw128(s_base, 1024, 16);
+    const uint64_t dk = umma_desc_sw128(s_base + Geo::kOffK, 1024, 16);
+    const uint64_t dv = umma_desc_sw128(s_base + Geo::kOffV, 1024, kKvHalf);  // (of D 128 the second half's dims lie a half tile on)
+    if (on) prefetch_tmap(&tm_q);
+    const uint32_t box = static_cast<uint32_t>(TQ * group) * 128 * kH;
+    Cursor sc = first, oc = first;
+    int s_left = 0, o_left = 0, q_seen = 0;
+    uint32_t k_st = 0, k_ph = 0, v_st = 0, v_ph = 0;
+    bool begins = false, q_flight = false;
+    // step i uses S buffer i & 1, for the (i >> 1)-th time; S runs two steps ahead of O
 #pragma unroll 1
-      for (int i = -2; i < n_mine; ++i) {
-        if (i >= 0) {  // P V of step i
-          if (o_left == 0) {
-            o_left = oc.take(plan, tfirst, TQ, p.groups, n_tiles).n;
-            begins = true;
-          }
-          if (!mbar_wait(bar_v + v_st, v_ph) || !mbar_wait(bar_p + (i & 1), (i >> 1) & 1)) {
-            fail = true;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t pcol = tmem + kSCol + (i & 1) * kBN;
-#pragma unroll
-          for (int h = 0; h < kH; ++h) {
-            const uint64_t vd = dv + static_cast<uint64_t>((v_st * kH + h) * (kKvHalf >> 4));
-#pragma unroll
-            for (int kk = 0; kk < kBN / 16; ++kk)
-              umma_f16_ts(tmem + kOCol + h * kHalf, pcol + 8 * kk, vd + 128 * kk, idesc_o, !begins || kk > 0);
-          }
-          umma_commit(bar_pv + (i & 1));
-          umma_commit(bar_vfree + v_st);
-          if (++v_st == kStages) {
-            v_st = 0;
-            v_ph ^= 1;
-          }
-          --o_left;
-          begins = false;
+    for (int i = -2; i < n_mine; ++i) {
+      if (i >= 0) {  // P V of step i
+        if (o_left == 0) {
+          o_left = oc.take(plan, tfirst, TQ, p.groups, n_tiles).n;
+          begins = true;
         }
-        if (i + 2 < n_mine) {  // S of step i + 2, whose buffer held S and then P of step i
-          if (i >= 0 && !mbar_wait(bar_pv + (i & 1), (i >> 1) & 1)) {
+        if (!warp_wait(bar_v + v_st, v_ph) || !warp_wait(bar_p + (i & 1), (i >> 1) & 1)) {
+          fail = true;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t pcol = tmem + kSCol + (i & 1) * kBN;
+        const uint64_t vd = dv + static_cast<uint64_t>(v_st * kH * (kKvHalf >> 4));
+#pragma unroll
+        for (int kk = 0; kk < kBN / 16; ++kk) mma_ts(on, tmem + kOCol, pcol + 8 * kk, vd + 128 * kk, idesc_o, !begins || kk > 0);
+        mma_commit(on, smem_u32(bar_pv + v_st));
+        --o_left;
+        begins = false;
+      }
+      if (i + 2 < n_mine) {  // S of step i + 2, whose buffer held S and then P of step i
+        if (i >= 0 && !warp_wait(bar_pv + v_st, v_ph)) {
+          fail = true;
+          break;
+        }
+        if (s_left == 0) {  // a run begins: its Q, once the last S of the run before (step i + 1) is done
+          const uint32_t b_st = k_st == 0 ? kStages - 1 : k_st - 1, b_ph = k_st == 0 ? k_ph ^ 1 : k_ph;
+          if (i > -2 && !warp_wait(bar_s + b_st, b_ph)) {
             fail = true;
             break;
           }
-          if (s_left == 0) {  // a run begins: its Q, once the last S of the run before is done
-            if (i > -2 && !mbar_wait(bar_s + ((i + 1) & 1), ((i + 1) >> 1) & 1)) {
-              fail = true;
-              break;
-            }
-            const Run r = sc.take(plan, tfirst, TQ, p.groups, n_tiles);
-            s_left = r.n;
+          const Run r = sc.take(plan, tfirst, TQ, p.groups, n_tiles);
+          s_left = r.n;
+          if (on) {
             mbar_arrive_expect_tx(bar_q, box);
 #pragma unroll
             for (int h = 0; h < kH; ++h) tma_load_3d(smem + h * kQHalf, &tm_q, h * kHalf, r.kvh * group, r.b0, bar_q);
-            q_flight = true;
-            if (!mbar_wait(bar_q, q_seen & 1)) {
-              fail = true;
-              break;
-            }
-            ++q_seen;
-            q_flight = false;
           }
-          if (!mbar_wait(bar_k + k_st, k_ph)) {
+          q_flight = true;
+          if (!warp_wait(bar_q, q_seen & 1)) {
             fail = true;
             break;
           }
-          tc_fence_after();
-#pragma unroll
-          for (int h = 0; h < kH; ++h) {
-            const uint64_t qd = dq + static_cast<uint64_t>(h * (kQHalf >> 4));
-            const uint64_t kd = dk + static_cast<uint64_t>((k_st * kH + h) * (kKvHalf >> 4));
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_f16_ss(tmem + kSCol + (i & 1) * kBN, qd + 2 * kk, kd + 2 * kk, idesc_s, h > 0 || kk > 0);
-          }
-          umma_commit(bar_s + (i & 1));
-          umma_commit(bar_kfree + k_st);
-          if (++k_st == kStages) {
-            k_st = 0;
-            k_ph ^= 1;
-          }
-          --s_left;
+          ++q_seen;
+          q_flight = false;
         }
+        if (!warp_wait(bar_k + k_st, k_ph)) {
+          fail = true;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t kd = dk + static_cast<uint64_t>(k_st * kH * (kKvHalf >> 4));
+#pragma unroll
+        for (int h = 0; h < kH; ++h) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ss(on, tmem + kSCol + (i & 1) * kBN, dq + h * (kQHalf >> 4) + 2 * kk, kd + h * (kKvHalf >> 4) + 2 * kk, idesc_s, h > 0 || kk > 0);
+        }
+        mma_commit(on, smem_u32(bar_s + k_st));
+        if (++k_st == kStages) {
+          k_st = 0;
+          k_ph ^= 1;
+        }
+        --s_left;
       }
-      if (fail) {
-        flag_error(p.err, PSB_DEVERR_TIMEOUT);
-        // let the copy and the products in flight land before shared memory and TMEM are released
-        if (q_flight) (void)mbar_wait(bar_q, q_seen & 1);
-        umma_commit(bar_drain);
-        (void)mbar_wait(bar_drain, 0);
+      if (i >= 0 && ++v_st == kStages) {
+        v_st = 0;
+        v_ph ^= 1;
       }
+    }
+    if (fail) {
+      if (on) flag_error(p.err, PSB_DEVERR_TIMEOUT);
+      // let the copy and the products in flight land before shared memory and TMEM are released
+      if (q_flight) (void)warp_wait(bar_q, q_seen & 1);
+      mma_commit(on, smem_u32(bar_drain));
+      (void)warp_wait(bar_drain, 0);
     }
   } else if (warp == 5) {
     // ---- copies: K of step x, then V of step x - 1 (the products need V later) ----
@@ -507,11 +533,11 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     };
     int x = 0;
     for (; x <= n_mine; ++x) {
-      if (x < n_mine && !issue(wk, x, &tm_k, bar_k, bar_kfree, Geo::kOffK)) {
+      if (x < n_mine && !issue(wk, x, &tm_k, bar_k, bar_s, Geo::kOffK)) {
         fail = true;
         break;
       }
-      if (x > 0 && !issue(wv, x - 1, &tm_v, bar_v, bar_vfree, Geo::kOffV)) {
+      if (x > 0 && !issue(wv, x - 1, &tm_v, bar_v, bar_pv, Geo::kOffV)) {
         fail = true;
         ++x;  // K of step x is on its way
         break;
@@ -538,7 +564,8 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       int have = pre - r.j0 * kBN;  // keys there are, from the run's first on
       float ms = -INFINITY, l = 0.f;  // the exponents' reference (times sc), the sum
       for (int j = 0; j < r.n; ++j, ++g, have -= kBN) {
-        if (!mbar_wait(bar_s + (g & 1), (g >> 1) & 1)) {
+        const uint32_t st = g % kStages, ph = (g / kStages) & 1;
+        if (!mbar_wait(bar_s + st, ph)) {
           fail = true;
           break;
         }
@@ -552,8 +579,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
           // V rows behind the prefix (another token's, or never loaded) must
           // not reach P V, where 0 * NaN would be NaN: this thread's arrival
           // lets P V read the stage
-          const int st = g % kStages;
-          if (!mbar_wait(bar_v + st, (g / kStages) & 1)) {
+          if (!mbar_wait(bar_v + st, ph)) {
             fail = true;
             break;
           }
@@ -582,7 +608,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
           const float ms_new = grow ? mxs : ms;
           const float alpha = ms == -INFINITY ? 0.f : ex2_approx(ms - ms_new);  // (a step has at least one key)
           if (j > 0) {  // O holds P V of the earlier steps once the last of them is done
-            if (!mbar_wait(bar_pv + ((g - 1) & 1), ((g - 1) >> 1) & 1)) {
+            if (!mbar_wait(bar_pv + (g - 1) % kStages, ((g - 1) / kStages) & 1)) {
               fail = true;
               break;
             }
@@ -621,7 +647,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       }
       if (fail) break;
       // the run's partial; the next run's first P V comes after its P
-      if (!__all_sync(0xffffffffu, mbar_wait(bar_pv + ((g - 1) & 1), ((g - 1) >> 1) & 1))) {
+      if (!warp_wait(bar_pv + (g - 1) % kStages, ((g - 1) / kStages) & 1)) {
         fail = true;
         break;
       }

@@ -7,22 +7,28 @@
 //   o = (o1 2^(m1 - m) + o2 2^(m2 - m)) / l,
 // so the shared part is computed for all of a group's query rows at once, where
 // it is a matrix product (tcgen05), and each sequence's own part by itself, where
-// it is a stream from HBM (mma.sync, as the plain decode).  Three launches:
+// it is a stream from HBM (mma.sync, as the plain decode).  shared_main_kernel does both
+// in one grid of one CTA per SM, so that the stream goes on under the products (and a
+// short call pays one launch and one plan for both); each leaves fp32 partials, which
+// shared_join_kernel joins.
 //
-//  shared_prefix_kernel  a tile is 128 rows: TQ = 128 / heads consecutive
-//    sequences of a group times the q heads of one kv head (one TMA box of
-//    [TQ, heads, 64]).  The steps (64 keys) of all tiles, in (kv head, group,
-//    tile, step) order, are dealt evenly over a persistent grid; every run of
-//    steps leaves an fp32 partial.
-//  shared_own_kernel     the 16-token slices of what is each sequence's own, in
-//    (kv heads, sequence, slice) order, dealt evenly over the warps of the grid;
-//    every run of slices leaves an fp32 partial.
-//  shared_join_kernel    joins the partials of each row.
+//  Prefixes: a tile is 128 rows: TQ = 128 / heads consecutive sequences of a group
+//    times the q heads of one kv head (one TMA box of [TQ, heads, 64]).  Two
+//    consecutive tiles make a pair and share each step's 64 keys (a tile by itself reads
+//    a step's K and V, 32 KB for D 128, in the time of its products: beyond what L2
+//    gives all SMs); of a pair with one tile, the two streams below take the steps in
+//    turn.  The steps of all pairs, in (kv head, group, pair, step) order, are dealt
+//    evenly, by their tiles, over the CTAs; every run of steps leaves partials.
+//  Own parts: the 16-token slices of what is each sequence's own, in (kv heads,
+//    sequence, slice) order, are dealt evenly over four warps of every CTA; every run
+//    of slices leaves a partial.
 //
-// The first two do not depend on each other: the second starts while the first
-// runs (it needs no tensor memory, and its registers and shared memory fit
-// beside two CTAs of the first), so the stream from HBM goes on under the
-// matrix products.
+// A CTA's 16 warps: two streams of four are the softmax (thread r is row r of a tile and
+// lane r of TMEM); two issue the products of a stream each (one warp for both spent 1400
+// cycles a stream and step on waits and operands, the softmax takes 1050), one the
+// copies of K, one those of V; four have the own parts.  A stream has two S buffers in
+// TMEM: S = Q K^T of its next step but one is issued behind O += P V of this one, whose
+// P, two keys a column, was written over S.
 //
 // Which of a group's tables the prefix is read through: that of the sequence
 // with the most tokens (the first of those), and the prefix ends with it.  A
@@ -30,6 +36,7 @@
 // captured batch has no tokens at all): keys that it does not see, masked in the
 // tile, would still meet its probabilities of 0, and 0 times infinity is no number.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -41,35 +48,37 @@ namespace psb {
 namespace {
 
 constexpr int kMaxBatch = 2048;      // sequences (and groups) whose plan fits shared memory beside the rings
-constexpr int kTcThreads = 192;      // warps 0-3: softmax; warp 4: products; warp 5: copies
+constexpr int kOwnWarps = 4, kFirstOwn = 12;  // warps 0-7: softmax, two streams; 8, 9: their products; 10, 11: copies of K, of V; 12-15: own parts
+constexpr int kThreads = 512;
+// Registers: 128 a thread at launch, and the shares they are dealt anew in.
+constexpr int kSoftmaxRegs = 136, kOtherRegs = 112, kOwnRegs = 128;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs + 128 * kOwnRegs <= kThreads * 128, "the shares fit the launch");
 constexpr int kRows = 128;           // rows of a tile
 constexpr int kBN = 64;              // keys per step
 constexpr int kHalf = 64;            // dims of one 128-byte line
 constexpr uint32_t kQHalf = kRows * 128;   // bytes of 64 dims of a Q tile
 constexpr uint32_t kKvHalf = kBN * 128;    // of a K or V tile
-constexpr uint32_t kTmemCols = 256;
-constexpr uint32_t kSCol = 0, kOCol = 128;
+// TMEM: of each stream two S buffers, then each stream's O
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kSCol = 0, kOCol = 4 * kBN;
 constexpr float kRescaleLog2 = 8.f;  // O is rescaled when a row's maximum grows by more than 2^8
-constexpr int kMinSteps = 4;         // steps per CTA below which the grid shrinks
-constexpr int kMaxTcCtas = 320;
-
-constexpr int kOwnWarps = 4, kOwnThreads = kOwnWarps * 32;
-constexpr int kOwnMinItems = 4;      // slices per warp below which fewer warps work
-constexpr int kMaxOwnCtas = 320;
+constexpr int kMinCost = 4;          // steps of a tile per CTA below which the grid shrinks (at least 2: see Cursor)
+constexpr int kOwnMinItems = 2;      // slices per warp below which fewer warps work
+constexpr int kMaxCtas = 160;        // (B200 has 148 SMs)
 
 template <int D>
 struct TcGeom {
   static constexpr int kH = D / kHalf;
-  static constexpr int kStages = D == 64 ? 3 : 2;
-  static constexpr uint32_t kOffK = kH * kQHalf;
+  static constexpr int kStages = D == 64 ? 4 : 2;  // (a power of two)
+  static constexpr uint32_t kOffK = 2 * kH * kQHalf;  // behind a Q tile for each stream
   static constexpr uint32_t kOffV = kOffK + kStages * kH * kKvHalf;
   static constexpr uint32_t kOffBars = kOffV + kStages * kH * kKvHalf;
-  static constexpr uint32_t kOffPlan = kOffBars + 256;
+  static constexpr uint32_t kOffRing = (kOffBars + 320 + 1023) / 1024 * 1024;
 };
 
 template <int D, int HP>
 struct OwnGeom {
-  static constexpr int kRing = 2;                 // slots per warp
+  static constexpr int kRing = D == 64 && HP == 2 ? 3 : 2;  // slots per warp
   static constexpr int kTile = 16 * D * 2;        // 16 tokens of one kv head
   static constexpr int kKV = HP * kTile;
   static constexpr int kSlot = 2 * kKV;
@@ -90,16 +99,15 @@ struct SharedParams {
   const int32_t* prefix;
   int32_t batch, groups, hkv, group, layer, block_size, max_context;
   int32_t tq;          // sequences per tile
-  int32_t max_tiles;   // tiles of one kv head there is room for
-  int32_t max_warps;   // warps of the own kernel
+  int32_t max_tiles, max_pairs;  // of one kv head there is room for
   int64_t num_blocks;
   float scale_log2;    // scale log2(e), positive
   // workspace
-  int2* tile_info;     // [hkv * max_tiles] a tile's first partial and how many
+  int2* tile_info;     // [hkv * max_tiles] a tile's first partial, how many, how far apart (<< 16)
   int2* seq_info;      // [batch] a sequence's tile in each kv head (-1: none) and its place there
   int2* own_info;      // [hkv * batch] a (kv heads, sequence) pair's first partial and how many
   float* tile_part;    // partials of the tiles: [D / 4][128] x 4 sums, then [128] (maximum, sum)
-  float* own_part;     // partials of the pairs: [16][D] sums, then [16] (maximum, sum)
+  float* own_part;     // partials of the (kv heads, sequence) pairs: [D / 4][16] x 4 sums, then [16] (maximum, sum)
   int32_t* err;
 };
 
@@ -116,42 +124,71 @@ __device__ __forceinline__ int last_le(const int32_t* v, int n, int x) {  // las
 }
 
 // ---------------------------------------------------------------------------
-// the plan: what both kernels know of the batch, built by every CTA
+// the plan: what every CTA knows of the batch
 // ---------------------------------------------------------------------------
 struct Plan {
   int32_t* ctx;     // [batch] tokens
+  int32_t* start;   // [batch] first token of a sequence's own part
+  int32_t* slices;  // [batch + 1] slices before a sequence, of one (kv heads)
   int32_t* cu;      // [groups + 1]
   int32_t* pre;     // [groups] shared tokens (0: the group's sequences are on their own)
   int32_t* lead;    // [groups] the sequence whose table holds them
-  __host__ __device__ static size_t ints(int batch, int groups) {
-    return static_cast<size_t>(batch) + 3 * static_cast<size_t>(groups) + 1;
+  // before a group, of one kv head:
+  int32_t* tiles;   // [groups + 1]
+  int32_t* pairs;   // [groups + 1]
+  int32_t* cost;    // [groups + 1] steps, counted once for each tile
+  int groups, tq, n_tiles, n_pairs, n_cost, n_slices;
+  __host__ __device__ static size_t ints(int batch, int groups) { return 3 * static_cast<size_t>(batch) + 1 + 6 * static_cast<size_t>(groups) + 4; }
+  __device__ Plan(int32_t* at, int batch, int n, int q) : groups(n), tq(q) {
+    ctx = at;
+    start = ctx + batch;
+    slices = start + batch;
+    cu = slices + batch + 1;
+    pre = cu + n + 1;
+    lead = pre + n;
+    tiles = lead + n;
+    pairs = tiles + n + 1;
+    cost = pairs + n + 1;
   }
-  __device__ Plan(int32_t* at, int batch, int groups) : ctx(at), cu(at + batch), pre(cu + groups + 1), lead(pre + groups) {}
+  __device__ __forceinline__ int steps_of(int g) const { return (pre[g] + kBN - 1) / kBN; }
 };
 
-template <int THREADS>
-__device__ void build_plan(const SharedParams& p, const Plan& pl) {
+// A warp's exclusive scan of one value a lane, and the total.
+__device__ __forceinline__ int scan_warp(int v, int& total) {
+  int incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, incl, o);
+    if ((threadIdx.x & 31) >= o) incl += x;
+  }
+  total = __shfl_sync(0xffffffffu, incl, 31);
+  return incl - v;
+}
+
+__device__ void build_plan(const SharedParams& p, Plan& pl) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool report = blockIdx.x == 0;
-  for (int b = tid; b < p.batch; b += THREADS) {
+  bool bad = false;
+  for (int b = tid; b < p.batch; b += kThreads) {
     int n = __ldcg(p.ctx + b);
     if (n < 0 || n > p.max_context) {
       if (report) flag_error(p.err, PSB_DEVERR_CONTEXT);
       n = n < 0 ? 0 : p.max_context;
     }
     pl.ctx[b] = n;
+    pl.start[b] = 0;
   }
-  bool bad = false;
-  for (int g = tid; g <= p.groups; g += THREADS) {
+  for (int g = kThreads - 1 - tid; g <= p.groups; g += kThreads) {  // (from the other end: in the same round of loads)
     const int a = __ldcg(p.cu + g), prev = g == 0 ? 0 : __ldcg(p.cu + g - 1);
     bad = bad || a < prev || prev < 0 || a > p.batch;
     pl.cu[g] = a;
+    if (g < p.groups) pl.pre[g] = __ldcg(p.prefix + g);
   }
   bad = __syncthreads_or(bad) != 0;
   if (bad && report && tid == 0) flag_error(p.err, PSB_DEVERR_SEQLENS);
-  for (int g = warp; g < p.groups; g += THREADS / 32) {
+  for (int g = warp; g < p.groups; g += kThreads / 32) {
     // malformed groups: every sequence on its own
-    const int b0 = bad ? 0 : pl.cu[g], b1 = bad ? 0 : pl.cu[g + 1];
+    const int b0 = bad ? 0 : pl.cu[g], b1 = bad ? 0 : pl.cu[g + 1], n = pl.pre[g];
     int best = -1, at = 0;
     for (int b = b0 + lane; b < b1; b += 32) {
       if (pl.ctx[b] > best) {
@@ -159,48 +196,78 @@ __device__ void build_plan(const SharedParams& p, const Plan& pl) {
         at = b;
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const int x = __shfl_xor_sync(0xffffffffu, best, o), y = __shfl_xor_sync(0xffffffffu, at, o);
-      if (x > best || (x == best && y < at)) {
-        best = x;
-        at = y;
-      }
-    }
+    const int most = __reduce_max_sync(0xffffffffu, best);
+    at = __reduce_min_sync(0xffffffffu, best == most ? at : INT_MAX);
+    // one sequence shares with nobody: all of it is its own
+    const int pre = b1 - b0 < 2 ? 0 : max(0, min(n, most));
+    if (pre > 0)
+      for (int b = b0 + lane; b < b1; b += 32)
+        if (pl.ctx[b] >= pre) pl.start[b] = pre;
+    __syncwarp();
     if (lane == 0) {
-      const int n = __ldcg(p.prefix + g);
       if (n < 0 && report) flag_error(p.err, PSB_DEVERR_CONTEXT);
-      // one sequence shares with nobody: all of it is its own
-      pl.pre[g] = b1 - b0 < 2 ? 0 : max(0, min(n, best));
+      pl.pre[g] = pre;
       pl.lead[g] = at;
     }
   }
   __syncthreads();
+  if (warp == 0) {  // the groups' tiles
+    const int per = (p.groups + 31) / 32, g0 = min(lane * per, p.groups), g1 = min(g0 + per, p.groups);
+    auto tiles_of = [&](int g) { return pl.pre[g] > 0 ? (pl.cu[g + 1] - pl.cu[g] + p.tq - 1) / p.tq : 0; };
+    int tiles = 0, pairs = 0, cost = 0;
+    for (int g = g0; g < g1; ++g) {
+      const int n = tiles_of(g);
+      tiles += n;
+      pairs += (n + 1) >> 1;
+      cost += n * pl.steps_of(g);
+    }
+    int all_tiles, all_pairs, all_cost;
+    tiles = scan_warp(tiles, all_tiles);
+    pairs = scan_warp(pairs, all_pairs);
+    cost = scan_warp(cost, all_cost);
+    for (int g = g0; g < g1; ++g) {
+      pl.tiles[g] = tiles;
+      pl.pairs[g] = pairs;
+      pl.cost[g] = cost;
+      const int n = tiles_of(g);
+      tiles += n;
+      pairs += (n + 1) >> 1;
+      cost += n * pl.steps_of(g);
+    }
+    if (lane == 0) {
+      pl.tiles[p.groups] = all_tiles;
+      pl.pairs[p.groups] = all_pairs;
+      pl.cost[p.groups] = all_cost;
+    }
+  } else if (warp == 1) {  // the sequences' slices
+    const int per = (p.batch + 31) / 32, b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
+    auto slices_of = [&](int b) { return pl.ctx[b] > pl.start[b] ? (pl.ctx[b] + 15) / 16 - pl.start[b] / 16 : 0; };
+    int n = 0, all;
+    for (int b = b0; b < b1; ++b) n += slices_of(b);
+    n = scan_warp(n, all);
+    for (int b = b0; b < b1; ++b) {
+      pl.slices[b] = n;
+      n += slices_of(b);
+    }
+    if (lane == 0) pl.slices[p.batch] = all;
+  }
+  __syncthreads();
+  pl.n_tiles = pl.tiles[p.groups];
+  pl.n_pairs = pl.pairs[p.groups];
+  pl.n_cost = pl.cost[p.groups];
+  pl.n_slices = pl.slices[p.batch];
 }
 
-// Exclusive scan of one value per thread over the CTA, and the total.
-template <int THREADS>
-__device__ __forceinline__ int scan_cta(int v, int& total) {
-  __shared__ int32_t sums[THREADS / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += x;
+// ``n`` units dealt evenly over ``parts``: part i has [start(i), start(i + 1)).
+struct Deal {
+  uint32_t n, parts, share, extra;
+  __device__ Deal(uint32_t units, uint32_t over) : n(units), parts(over), share(over ? units / over : 0), extra(over ? units - share * over : 0) {}
+  __device__ __forceinline__ uint32_t start(uint32_t i) const { return share * i + min(i, extra); }
+  __device__ __forceinline__ uint32_t part_of(uint32_t unit) const {
+    const uint32_t head = extra * (share + 1);
+    return unit < head ? unit / (share + 1) : extra + (unit - head) / share;
   }
-  __syncthreads();
-  if (lane == 31) sums[warp] = incl;
-  __syncthreads();
-  int run = incl - v;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) run += sums[w];
-    total += sums[w];
-  }
-  return run;
-}
+};
 
 // ---------------------------------------------------------------------------
 // the shared part
@@ -239,43 +306,98 @@ __device__ __forceinline__ void mma_commit(bool on, uint32_t bar) {
       "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(static_cast<uint32_t>(on))
       : "memory");
 }
+__device__ __forceinline__ void box_load(bool on, uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(static_cast<uint32_t>(on))
+      : "memory");
+}
+__device__ __forceinline__ void expect_bytes(bool on, uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes), "r"(static_cast<uint32_t>(on))
+      : "memory");
+}
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+// A value that every lane has alike, where the compiler cannot tell.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_or_sync(0xffffffffu, x); }
 __device__ __forceinline__ bool elect_one() {
   uint32_t on;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
   return on != 0;
 }
 // mbar_wait by a whole warp: its lanes give up together or not at all.
+__device__ __forceinline__ bool warp_wait_at(uint32_t bar, uint32_t parity) {
+  uint64_t t0 = 0;
+#pragma unroll 1
+  while (!__any_sync(0xffffffffu, mbar_try_wait_sleep(bar, parity, 100000u))) {
+    const uint64_t t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    if (__all_sync(0xffffffffu, t - t0 > kWaitLimitNs)) return false;
+  }
+  return true;
+}
+template <int S>
+struct Stream {
+  static constexpr int value = S;
+};
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
 
-// A run of steps of one tile.
+// A run of steps of one pair of tiles.
 struct Run {
-  int kvh, tile, grp, b0, n_seq;  // tile of its kv head, group, first sequence and how many
-  int j0, n;                      // its steps
+  int kvh, pair, tile, grp;  // pair of its kv head and its first tile, group
+  int b0, n_seq;             // first sequence, sequences from it to the group's end
+  int j0, n;                 // its steps
+  int in_grp;                // pair of its group
+  bool two;                  // there is a second tile
 };
 
-// Walks a CTA's steps tile by tile.
+// Walks a CTA's steps pair by pair.  A step of a pair costs 2 (one tile: 1) and belongs
+// to the CTA that its last unit of cost was dealt to: a CTA that was dealt two units
+// or more in a pair has steps there.
 struct Cursor {
-  int kvh, tile, grp, in_grp, j0, left;
-  __device__ Run take(const Plan& pl, const int32_t* tfirst, int tq, int groups, int n_tiles) {
+  int kvh, grp, in_grp, j0, left;  // left: cost
+  // To the step that the unit at ``pos`` of the whole list is in, or begins; returns its first unit.
+  __device__ uint32_t seek(const Plan& pl, uint32_t pos) {
+    kvh = static_cast<int>(pos / pl.n_cost);
+    const int r = static_cast<int>(pos - static_cast<uint32_t>(kvh) * pl.n_cost);
+    grp = last_le(pl.cost, pl.groups, r);  // (of groups without steps the last: it has some)
+    const int steps = pl.steps_of(grp), off = r - pl.cost[grp];
+    in_grp = off / (2 * steps);
+    const int in_pair = off - in_grp * 2 * steps;
+    j0 = two(pl) ? in_pair >> 1 : in_pair;
+    return pos - (two(pl) ? in_pair & 1 : 0);
+  }
+  __device__ bool two(const Plan& pl) const { return 2 * in_grp + 1 < pl.tiles[grp + 1] - pl.tiles[grp]; }
+  __device__ Run take(const Plan& pl) {  // the next run (left > 0)
     Run r;
     r.kvh = kvh;
-    r.tile = tile;
+    r.pair = pl.pairs[grp] + in_grp;
+    r.tile = pl.tiles[grp] + 2 * in_grp;
     r.grp = grp;
-    r.b0 = pl.cu[grp] + in_grp * tq;
-    r.n_seq = min(tq, pl.cu[grp + 1] - r.b0);
+    r.in_grp = in_grp;
+    r.b0 = pl.cu[grp] + in_grp * 2 * pl.tq;
+    r.n_seq = pl.cu[grp + 1] - r.b0;
+    r.two = two(pl);
     r.j0 = j0;
-    r.n = min((pl.pre[grp] + kBN - 1) / kBN - j0, left);
-    left -= r.n;
+    r.n = min(pl.steps_of(grp) - j0, r.two ? left >> 1 : left);
+    left -= r.two ? 2 * r.n : r.n;
     j0 = 0;
     if (left > 0) {
       ++in_grp;
-      if (++tile == n_tiles) {
-        tile = 0;
+      if (pl.pairs[grp] + in_grp == pl.n_pairs) {
         grp = 0;
         in_grp = 0;
         ++kvh;
       }
-      while (tile >= tfirst[grp + 1]) {  // groups without tiles are passed over
+      while (pl.pairs[grp] + in_grp >= pl.pairs[grp + 1]) {  // groups without pairs are passed over
         ++grp;
         in_grp = 0;
       }
@@ -284,403 +406,58 @@ struct Cursor {
   }
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kTcThreads, 2)
-    shared_prefix_kernel(const SharedParams p, const __grid_constant__ CUtensorMap tm_q,
-                         const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
-  using Geo = TcGeom<D>;
-  constexpr int kH = Geo::kH, kStages = Geo::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* const smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
-  uint64_t* const bar_q = reinterpret_cast<uint64_t*>(smem + Geo::kOffBars);
-  // of step x, its stage x % kStages (a barrier's next phase needs this one's products):
-  uint64_t* const bar_k = bar_q + 1;               // [kStages] K landed
-  uint64_t* const bar_s = bar_k + kStages;         // [kStages] Q K^T done: S written, the stage's K free
-  uint64_t* const bar_v = bar_s + kStages;         // [kStages] V landed
-  uint64_t* const bar_pv = bar_v + kStages;        // [kStages] P V done: the stage's V free
-  uint64_t* const bar_p = bar_pv + kStages;        // [2] P written over S, in S buffer x & 1
-  uint64_t* const bar_drain = bar_p + 2;           // after a failed wait: every product issued so far is done
-  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bar_drain + 1);
-  static_assert((4 + 4 * kStages) * 8 + 4 <= 256, "barriers fit their area");
-  const Plan plan(reinterpret_cast<int32_t*>(smem + Geo::kOffPlan), p.batch, p.groups);
-  int32_t* const tfirst = plan.lead + p.groups;    // [groups + 1] tiles before a group, of one kv head
-  int32_t* const sfirst = tfirst + p.groups + 1;   // [groups + 1] steps before a group, of one kv head
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int TQ = p.tq, group = p.group;
-  if (tid == 0) {
-    mbar_init(bar_q, 1);
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(bar_k + i, 1);
-      mbar_init(bar_s + i, 1);
-      mbar_init(bar_v + i, 1);
-      mbar_init(bar_pv + i, 1);
+// One stream's steps of a CTA, in order: of pairs of tiles every step, of single tiles
+// those whose number, counted in half-steps (a step of one stream) of the CTA, is its own.
+struct Steps {
+  Cursor c;
+  Run r;
+  int x, half, g0;  // step of the run; half-steps and steps of the CTA before the run
+  bool begins;      // the first of the run
+  __device__ explicit Steps(const Cursor& first) : c(first), x(0), half(0), g0(0), begins(true) {
+    r.n = 0;
+    r.two = false;
+  }
+  // Takes the next run up when this one's steps are through; false: there is none.
+  __device__ __forceinline__ bool more(const Plan& pl, int s) {
+    while (x >= r.n) {
+      if (c.left == 0) return false;
+      half += r.two ? 2 * r.n : r.n;
+      g0 += r.n;
+      r = c.take(pl);
+      x = r.two ? 0 : (half + s) & 1;
+      begins = true;
     }
-    for (int i = 0; i < 2; ++i) mbar_init(bar_p + i, kRows);
-    mbar_init(bar_drain, 1);
-    fence_barrier_init();
+    return true;
   }
-  if (warp == 0) {
-    tmem_alloc(s_tmem, kTmemCols);
-    tmem_relinquish();
+  __device__ __forceinline__ void next() {
+    x += r.two ? 1 : 2;
+    begins = false;
   }
-  pdl_wait();  // lengths, groups, tables, q and the pools may come from the stream predecessor
-  pdl_launch_dependents();  // (after the wait: the own kernel counts on it)
+};
 
-  build_plan<kTcThreads>(p, plan);
-  int n_tiles, n_steps;
-  {
-    const int per = (p.groups + kTcThreads - 1) / kTcThreads;
-    const int g0 = min(tid * per, p.groups), g1 = min(g0 + per, p.groups);
-    auto tiles_of = [&](int g) { return plan.pre[g] > 0 ? (plan.cu[g + 1] - plan.cu[g] + TQ - 1) / TQ : 0; };
-    auto steps_of = [&](int g) { return tiles_of(g) * ((plan.pre[g] + kBN - 1) / kBN); };
-    int tiles = 0, steps = 0;
-    for (int g = g0; g < g1; ++g) {
-      tiles += tiles_of(g);
-      steps += steps_of(g);
-    }
-    int t = scan_cta<kTcThreads>(tiles, n_tiles), s = scan_cta<kTcThreads>(steps, n_steps);
-    for (int g = g0; g < g1; ++g) {
-      tfirst[g] = t;
-      sfirst[g] = s;
-      t += tiles_of(g);
-      s += steps_of(g);
-    }
-    if (tid == 0) {
-      tfirst[p.groups] = n_tiles;
-      sfirst[p.groups] = n_steps;
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *s_tmem;
-  const uint32_t total = static_cast<uint32_t>(n_steps) * p.hkv;  // below 2^31
-  const uint32_t act = min(gridDim.x, (total + kMinSteps - 1) / kMinSteps), cta = blockIdx.x;
-  if (cta >= act) {
-    __syncthreads();  // every warp has read the address
-    if (warp == 0) tmem_dealloc(tmem, kTmemCols);
-    return;
-  }
-  const uint32_t share = total / act, extra = total - share * act;
-  const uint32_t my_a = share * cta + min(cta, extra);
-  const int n_mine = static_cast<int>(share + (cta < extra ? 1 : 0));
-  auto cta_of = [&](uint32_t step) {  // the CTA a step was dealt to
-    const uint32_t head = extra * (share + 1);
-    return step < head ? step / (share + 1) : extra + (step - head) / share;
-  };
-  Cursor first;
-  {
-    first.kvh = static_cast<int>(my_a / n_steps);
-    const int r = static_cast<int>(my_a - static_cast<uint32_t>(first.kvh) * n_steps);
-    first.grp = last_le(sfirst, p.groups, r);  // (of groups without steps the last: it has some)
-    const int n = (plan.pre[first.grp] + kBN - 1) / kBN;
-    first.in_grp = (r - sfirst[first.grp]) / n;
-    first.j0 = r - sfirst[first.grp] - first.in_grp * n;
-    first.tile = tfirst[first.grp] + first.in_grp;
-    first.left = n_mine;
-  }
-  bool fail = false;
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-  if (warp == 4) {
-    // ---- products ----
-    constexpr int kFmt = Elem<T>::code == PSB_BF16 ? 1 : 0;
-    constexpr uint32_t idesc_s = umma_idesc_f16(kFmt, kRows, kBN, 0, 0), idesc_o = umma_idesc_f16(kFmt, kRows, D, 0, 1);
-    const bool on = elect_one();
-    const uint32_t s_base = smem_u32(smem);
-    const uint64_t dq = umma_desc_sw128(s_base, 1024, 16);
-    const uint64_t dk = umma_desc_sw128(s_base + Geo::kOffK, 1024, 16);
-    const uint64_t dv = umma_desc_sw128(s_base + Geo::kOffV, 1024, kKvHalf);  // (of D 128 the second half's dims lie a half tile on)
-    if (on) prefetch_tmap(&tm_q);
-    const uint32_t box = static_cast<uint32_t>(TQ * group) * 128 * kH;
-    Cursor sc = first, oc = first;
-    int s_left = 0, o_left = 0, q_seen = 0;
-    uint32_t k_st = 0, k_ph = 0, v_st = 0, v_ph = 0;
-    bool begins = false, q_flight = false;
-    // step i uses S buffer i & 1, for the (i >> 1)-th time; S runs two steps ahead of O
-#pragma unroll 1
-    for (int i = -2; i < n_mine; ++i) {
-      if (i >= 0) {  // P V of step i
-        if (o_left == 0) {
-          o_left = oc.take(plan, tfirst, TQ, p.groups, n_tiles).n;
-          begins = true;
-        }
-        if (!warp_wait(bar_v + v_st, v_ph) || !warp_wait(bar_p + (i & 1), (i >> 1) & 1)) {
-          fail = true;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t pcol = tmem + kSCol + (i & 1) * kBN;
-        const uint64_t vd = dv + static_cast<uint64_t>(v_st * kH * (kKvHalf >> 4));
-#pragma unroll
-        for (int kk = 0; kk < kBN / 16; ++kk) mma_ts(on, tmem + kOCol, pcol + 8 * kk, vd + 128 * kk, idesc_o, !begins || kk > 0);
-        mma_commit(on, smem_u32(bar_pv + v_st));
-        --o_left;
-        begins = false;
-      }
-      if (i + 2 < n_mine) {  // S of step i + 2, whose buffer held S and then P of step i
-        if (i >= 0 && !warp_wait(bar_pv + v_st, v_ph)) {
-          fail = true;
-          break;
-        }
-        if (s_left == 0) {  // a run begins: its Q, once the last S of the run before (step i + 1) is done
-          const uint32_t b_st = k_st == 0 ? kStages - 1 : k_st - 1, b_ph = k_st == 0 ? k_ph ^ 1 : k_ph;
-          if (i > -2 && !warp_wait(bar_s + b_st, b_ph)) {
-            fail = true;
-            break;
-          }
-          const Run r = sc.take(plan, tfirst, TQ, p.groups, n_tiles);
-          s_left = r.n;
-          if (on) {
-            mbar_arrive_expect_tx(bar_q, box);
-#pragma unroll
-            for (int h = 0; h < kH; ++h) tma_load_3d(smem + h * kQHalf, &tm_q, h * kHalf, r.kvh * group, r.b0, bar_q);
-          }
-          q_flight = true;
-          if (!warp_wait(bar_q, q_seen & 1)) {
-            fail = true;
-            break;
-          }
-          ++q_seen;
-          q_flight = false;
-        }
-        if (!warp_wait(bar_k + k_st, k_ph)) {
-          fail = true;
-          break;
-        }
-        tc_fence_after();
-        const uint64_t kd = dk + static_cast<uint64_t>(k_st * kH * (kKvHalf >> 4));
-#pragma unroll
-        for (int h = 0; h < kH; ++h) {
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_ss(on, tmem + kSCol + (i & 1) * kBN, dq + h * (kQHalf >> 4) + 2 * kk, kd + h * (kKvHalf >> 4) + 2 * kk, idesc_s, h > 0 || kk > 0);
-        }
-        mma_commit(on, smem_u32(bar_s + k_st));
-        if (++k_st == kStages) {
-          k_st = 0;
-          k_ph ^= 1;
-        }
-        --s_left;
-      }
-      if (i >= 0 && ++v_st == kStages) {
-        v_st = 0;
-        v_ph ^= 1;
-      }
+// 16-byte asynchronous copies, grouped
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// Until the oldest of ``flight`` (1 .. N) groups has landed.
+template <int N>
+__device__ __forceinline__ void copy_wait_oldest(uint32_t flight) {
+  if constexpr (N > 1) {
+    if (flight >= N) {
+      copy_wait<N - 1>();
+      return;
     }
-    if (fail) {
-      if (on) flag_error(p.err, PSB_DEVERR_TIMEOUT);
-      // let the copy and the products in flight land before shared memory and TMEM are released
-      if (q_flight) (void)warp_wait(bar_q, q_seen & 1);
-      mma_commit(on, smem_u32(bar_drain));
-      (void)warp_wait(bar_drain, 0);
-    }
-  } else if (warp == 5) {
-    // ---- copies: K of step x, then V of step x - 1 (the products need V later) ----
-    if (lane == 0) {
-      prefetch_tmap(&tm_k);
-      prefetch_tmap(&tm_v);
-    }
-    const int bs = p.block_size, box_rows = min(bs, kBN), boxes = kBN / box_rows;
-    const int64_t layer0 = static_cast<int64_t>(p.layer) * p.num_blocks;
-    struct Walk {
-      Cursor c;
-      int left, j, kvh, n_blk, chunk;  // steps left of the run, its next step; entries of the prefix, chunk of 32 at hand
-      const int32_t* row;
-      int32_t id;                      // this lane's entry of the chunk
-    };
-    Walk wk{first, 0, 0, 0, 0, -1, nullptr, 0}, wv = wk;
-    auto issue = [&](Walk& w, int x, const CUtensorMap* tm, uint64_t* bar, uint64_t* bar_free, uint32_t off) -> bool {
-      if (w.left == 0) {
-        const Run r = w.c.take(plan, tfirst, TQ, p.groups, n_tiles);
-        w.left = r.n;
-        w.j = r.j0;
-        w.kvh = r.kvh;
-        w.n_blk = (plan.pre[r.grp] + bs - 1) / bs;
-        w.row = p.tables + static_cast<int64_t>(plan.lead[r.grp]) * p.table_stride;
-        w.chunk = -1;
-      }
-      const int st = x % kStages;
-      if (x >= kStages && !__all_sync(0xffffffffu, mbar_wait(bar_free + st, (x / kStages - 1) & 1))) return false;
-      // the step's blocks, from block i0 on at row y (a block of more than a step's keys: a part of one)
-      const int i0 = w.j * kBN / bs, y = bs > kBN ? w.j * kBN - i0 * bs : 0;
-      const int n = min(boxes, w.n_blk - i0);  // blocks behind the prefix are not loaded: their keys are masked
-      if (lane == 0) mbar_arrive_expect_tx(bar + st, static_cast<uint32_t>(n * box_rows) * 128 * kH);
-      for (int b = 0; b < n; ++b) {
-        const int i = i0 + b;
-        if ((i >> 5) != w.chunk) {
-          w.chunk = i >> 5;
-          const int mine = w.chunk * 32 + lane;
-          w.id = 0;
-          if (mine < w.n_blk) {
-            w.id = __ldcg(w.row + mine);
-            if (w.id < 0 || w.id >= p.num_blocks) {  // flagged, and another block's keys read in its place
-              flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
-              w.id = 0;
-            }
-          }
-        }
-        const int32_t blk = __shfl_sync(0xffffffffu, w.id, i & 31);
-        if (lane == 0) {
-          const int32_t tile = static_cast<int32_t>((layer0 + blk) * p.hkv + w.kvh);
-#pragma unroll
-          for (int h = 0; h < kH; ++h)
-            tma_load_3d(smem + off + (st * kH + h) * kKvHalf + b * box_rows * 128, tm, h * kHalf, y, tile, bar + st);
-        }
-      }
-      ++w.j;
-      --w.left;
-      return true;
-    };
-    int x = 0;
-    for (; x <= n_mine; ++x) {
-      if (x < n_mine && !issue(wk, x, &tm_k, bar_k, bar_s, Geo::kOffK)) {
-        fail = true;
-        break;
-      }
-      if (x > 0 && !issue(wv, x - 1, &tm_v, bar_v, bar_pv, Geo::kOffV)) {
-        fail = true;
-        ++x;  // K of step x is on its way
-        break;
-      }
-    }
-    if (fail && lane == 0) {
-      flag_error(p.err, PSB_DEVERR_TIMEOUT);
-      // copies still in flight: the newest of each stage, K of the steps below x, V of those below x - 1
-      for (int t = max(0, min(x, n_mine) - kStages); t < min(x, n_mine); ++t) (void)mbar_wait(bar_k + t % kStages, (t / kStages) & 1);
-      for (int t = max(0, x - 1 - kStages); t < x - 1; ++t) (void)mbar_wait(bar_v + t % kStages, (t / kStages) & 1);
-    }
+    copy_wait_oldest<N - 1>(flight);
   } else {
-    // ---- softmax: thread r is row r of the tile and lane r of TMEM ----
-    const int row = warp * 32 + lane;
-    const int rseq = row / group;
-    const uint32_t t_lane = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    const float sc = p.scale_log2;
-    Cursor cc = first;
-    int g = 0;
-    while (cc.left > 0 && !fail) {
-      const Run r = cc.take(plan, tfirst, TQ, p.groups, n_tiles);
-      const int pre = plan.pre[r.grp];
-      const bool live = rseq < r.n_seq;
-      int have = pre - r.j0 * kBN;  // keys there are, from the run's first on
-      float ms = -INFINITY, l = 0.f;  // the exponents' reference (times sc), the sum
-      for (int j = 0; j < r.n; ++j, ++g, have -= kBN) {
-        const uint32_t st = g % kStages, ph = (g / kStages) & 1;
-        if (!mbar_wait(bar_s + st, ph)) {
-          fail = true;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t t_s = t_lane + kSCol + (g & 1) * kBN;
-        uint32_t sr[kBN];
-        tmem_ld32(t_s, sr);
-        tmem_ld32(t_s + 32, sr + 32);
-        tmem_wait_ld();
-        if (have < kBN) {
-          // V rows behind the prefix (another token's, or never loaded) must
-          // not reach P V, where 0 * NaN would be NaN: this thread's arrival
-          // lets P V read the stage
-          if (!mbar_wait(bar_v + st, ph)) {
-            fail = true;
-            break;
-          }
-          if (row < kBN && row >= have) {
-#pragma unroll
-            for (int h = 0; h < kH; ++h) {
-              const uint32_t vrow = smem_u32(smem) + Geo::kOffV + (st * kH + h) * kKvHalf + row * 128;
-#pragma unroll
-              for (int c = 0; c < 128; c += 16) st_shared_zero16(vrow + c);
-            }
-            fence_proxy_async_smem();  // visible to the tensor core
-          }
-#pragma unroll
-          for (int c = 0; c < kBN; ++c)
-            if (c >= have) sr[c] = __float_as_uint(-INFINITY);
-        }
-        float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < kBN; c += 4) {
-          mx0 = max3(mx0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-          mx1 = max3(mx1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
-        }
-        const float mxs = fmaxf(mx0, mx1) * sc;
-        const bool grow = mxs > ms + kRescaleLog2;
-        if (__any_sync(0xffffffffu, grow)) {  // (the warp's TMEM access is collective)
-          const float ms_new = grow ? mxs : ms;
-          const float alpha = ms == -INFINITY ? 0.f : ex2_approx(ms - ms_new);  // (a step has at least one key)
-          if (j > 0) {  // O holds P V of the earlier steps once the last of them is done
-            if (!mbar_wait(bar_pv + (g - 1) % kStages, ((g - 1) / kStages) & 1)) {
-              fail = true;
-              break;
-            }
-            tc_fence_after();
-#pragma unroll 1
-            for (int q = 0; q < D; q += 32) {
-              uint32_t ot[32];
-              tmem_ld32(t_lane + kOCol + q, ot);
-              tmem_wait_ld();
-#pragma unroll
-              for (int d = 0; d < 32; ++d) ot[d] = __float_as_uint(__uint_as_float(ot[d]) * alpha);
-              tmem_st32(t_lane + kOCol + q, ot);
-            }
-            tmem_wait_st();
-          }
-          l *= alpha;
-          ms = ms_new;
-        }
-        const float mu = ms == -INFINITY ? 0.f : ms;
-        uint32_t pk[kBN / 2];
-        const uint64_t sc2 = pair2(sc, sc), nmu2 = pair2(-mu, -mu);
-        uint64_t rs2 = pair2(0.f, 0.f);
-#pragma unroll
-        for (int c = 0; c < kBN; c += 2) {
-          const float2 a = unpair2(fma2(pair2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, nmu2));
-          const float x0 = ex2_approx(a.x), x1 = ex2_approx(a.y);
-          rs2 = add2(rs2, pair2(x0, x1));
-          pk[c / 2] = pack2<T>(x0, x1);
-        }
-        const float2 rs = unpair2(rs2);
-        l += rs.x + rs.y;
-        tmem_st32(t_s, pk);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(bar_p + (g & 1));
-      }
-      if (fail) break;
-      // the run's partial; the next run's first P V comes after its P
-      if (!warp_wait(bar_pv + (g - 1) % kStages, ((g - 1) / kStages) & 1)) {
-        fail = true;
-        break;
-      }
-      tc_fence_after();
-      const int ord = r.kvh * n_tiles + r.tile;
-      float* const part = p.tile_part + static_cast<int64_t>(cta + ord) * tile_floats(D);
-#pragma unroll 1
-      for (int q = 0; q < D; q += 32) {
-        uint32_t ot[32];
-        tmem_ld32(t_lane + kOCol + q, ot);
-        tmem_wait_ld();
-        if (live) {
-#pragma unroll
-          for (int d = 0; d < 32; d += 4)
-            reinterpret_cast<float4*>(part)[((q + d) >> 2) * kRows + row] =
-                make_float4(__uint_as_float(ot[d]), __uint_as_float(ot[d + 1]), __uint_as_float(ot[d + 2]), __uint_as_float(ot[d + 3]));
-        }
-        __syncwarp();
-      }
-      if (live) reinterpret_cast<float2*>(part + kRows * D)[row] = make_float2(ms, l);
-      if (r.j0 == 0 && tid == 0) {
-        const uint32_t end = my_a + static_cast<uint32_t>(g) - r.n + (pre + kBN - 1) / kBN;  // the tile's last step + 1
-        p.tile_info[r.kvh * p.max_tiles + r.tile] = make_int2(static_cast<int>(cta) + ord, static_cast<int>(cta_of(end - 1) - cta) + 1);
-      }
-      tc_fence_before();
-    }
-    if (fail && lane == 0) flag_error(p.err, PSB_DEVERR_TIMEOUT);
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 0) {
-    tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+    copy_wait<0>();
   }
 }
 
@@ -690,120 +467,46 @@ __global__ void __launch_bounds__(kTcThreads, 2)
 // As the plain decode: a warp streams its slices (16 tokens of HP kv heads)
 // through a ring of its own with 16-byte cp.async copies.  HP = 2 (up to 8 q
 // heads per kv head): rows 0-7 of the m16n8k16 tile are one kv head's q heads,
-// rows 8-15 the next one's.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint64_t policy) {
-  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// floor(n w / warps) and its reverse, for items dealt over warps
-struct Deal {
-  int64_t n;
-  int warps;
-  __device__ __forceinline__ int64_t start(int w) const { return n * w / warps; }
-  __device__ __forceinline__ int warp_of(int64_t item) const { return static_cast<int>(((item + 1) * warps - 1) / n); }
-};
-
-template <typename T, int D, int HP>
-__global__ void __launch_bounds__(kOwnThreads) shared_own_kernel(const SharedParams p) {
+// rows 8-15 the next one's.  HP = 1: up to 16 q heads of one kv head; HI: there are
+// more than 8 (else the upper rows' registers are not kept).
+template <typename T, int D, int HP, bool HI>
+__device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& plan, uint8_t* ring_all) {
   using Geo = OwnGeom<D, HP>;
   constexpr int kRing = Geo::kRing, kSteps = D / 16, kCols = D / 8;  // k steps; 16-byte columns of a row
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* const ring_all = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
-  const Plan plan(reinterpret_cast<int32_t*>(ring_all + Geo::kBytes), p.batch, p.groups);
-  int32_t* const s_start = plan.lead + p.groups;  // [batch] first token of its own
-  int32_t* const bpre = s_start + p.batch;        // [batch + 1] slices before a sequence
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr bool kHi = HP == 2 || HI;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - kFirstOwn;
   const int gq = lane >> 2, t = lane & 3;
   const int G = p.group, B = p.batch, hgs = p.hkv / HP;
-  // No wait for the stream predecessor here: this launch begins once every CTA
-  // of shared_prefix_kernel has begun, which each does behind a wait for what
-  // came before (and everything is read through L2).  What it waits for, at its
-  // end, is that kernel itself, so that its own end is the end of both.
-  pdl_launch_dependents();
-  build_plan<kOwnThreads>(p, plan);
-  for (int b = tid; b < B; b += kOwnThreads) s_start[b] = 0;
-  __syncthreads();
-  for (int g = warp; g < p.groups; g += kOwnWarps)
-    if (plan.pre[g] > 0)
-      for (int b = plan.cu[g] + lane; b < plan.cu[g + 1]; b += 32)
-        if (plan.ctx[b] >= plan.pre[g]) s_start[b] = plan.pre[g];
-  __syncthreads();
-  auto slices_of = [&](int b) { return max(0, (plan.ctx[b] + 15) / 16 - s_start[b] / 16) * (plan.ctx[b] > s_start[b] ? 1 : 0); };
-  int n_slices;
-  {
-    const int per = (B + kOwnThreads - 1) / kOwnThreads;
-    const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
-    int n = 0;
-    for (int b = b0; b < b1; ++b) n += slices_of(b);
-    int run = scan_cta<kOwnThreads>(n, n_slices);
-    for (int b = b0; b < b1; ++b) {
-      bpre[b] = run;
-      run += slices_of(b);
-    }
-    if (tid == 0) bpre[B] = n_slices;
-    __syncthreads();
-  }
-  const int64_t items = static_cast<int64_t>(n_slices) * hgs;
-  const Deal deal{items, static_cast<int>(min(static_cast<int64_t>(gridDim.x * kOwnWarps), max(int64_t(1), items / kOwnMinItems)))};
-  // warps in order of their place in a CTA: few warps are spread over the SMs
-  const int gw = warp * gridDim.x + blockIdx.x;
-  // what the join needs: tiles of the sequences, partials of the pairs
-  const int gt = blockIdx.x * kOwnThreads + tid, gts = gridDim.x * kOwnThreads;
-  if (gt < B) {
-    for (int b = gt; b < B; b += gts) {
-      int2 at = make_int2(-1, 0);
-      if (s_start[b] > 0) {
-        int g = last_le(plan.cu, p.groups, b), tiles = 0;  // (of empty groups the last: it holds b)
-        for (int i = 0; i < g; ++i)
-          if (plan.pre[i] > 0) tiles += (plan.cu[i + 1] - plan.cu[i] + p.tq - 1) / p.tq;
-        const int m = b - plan.cu[g];
-        at = make_int2(tiles + m / p.tq, m % p.tq);
-      }
-      p.seq_info[b] = at;
-    }
-  }
-  for (int s = gt; s < B * hgs; s += gts) {
-    const int hg = s / B, b = s - hg * B;
-    int2 at = make_int2(0, 0);
-    if (bpre[b + 1] > bpre[b]) {
-      const int64_t a = static_cast<int64_t>(hg) * n_slices + bpre[b], e = static_cast<int64_t>(hg) * n_slices + bpre[b + 1];
-      const int w0 = deal.warp_of(a), w1 = deal.warp_of(e - 1);
-      at = make_int2(w0 + s, w1 - w0 + 1);
-    }
-    p.own_info[s] = at;
-  }
-
-  const bool works = gw < deal.warps && items > 0;
-  const int64_t my_a = works ? deal.start(gw) : 0, my_e = works ? deal.start(gw + 1) : 0;
-  uint8_t* const ring = ring_all + warp * kRing * Geo::kSlot;
-  const uint32_t ring_u = smem_u32(ring);
+  const uint32_t items = static_cast<uint32_t>(plan.n_slices) * hgs;  // below 2^31
+  const Deal deal(items, min(gridDim.x * kOwnWarps, (items + kOwnMinItems - 1) / kOwnMinItems));
+  // warps in order of their place in a CTA: few are spread over the SMs
+  const uint32_t gw = warp * gridDim.x + blockIdx.x;
+  const uint32_t my_a = gw < deal.parts ? deal.start(gw) : 0, my_e = gw < deal.parts ? deal.start(gw + 1) : 0;
+  const uint32_t ring_u = smem_u32(ring_all) + warp * kRing * Geo::kSlot;
   const uint64_t policy = l2_policy_evict_first();
   const int64_t layer0 = static_cast<int64_t>(p.layer) * p.num_blocks;
-  const bool row_lo = gq < G, row_hi = HP == 2 ? gq < G : gq + 8 < G;
+  const bool row_lo = gq < G, row_hi = kHi && (HP == 2 ? gq < G : gq + 8 < G);
 
   // A chunk: up to 32 consecutive slices of the warp's range, one a lane: its
   // place in the pool (-1: its block is outside), the valid tokens [lo, hi), and
   // whether a pair or the range begins or ends with it.
   struct Chunk {
-    int64_t beg;
+    uint32_t beg;
     int n;
     int32_t blk, row, meta, pair;
   };
-  auto build_chunk = [&](int64_t beg) -> Chunk {
+  auto build_chunk = [&](uint32_t beg) -> Chunk {
     Chunk c;
     c.beg = beg;
-    c.n = static_cast<int>(min(int64_t(32), my_e - beg));
+    c.n = static_cast<int>(min(32u, my_e - beg));
     c.blk = -1;
     c.row = c.meta = c.pair = 0;
     if (lane < c.n) {
-      const int64_t i = beg + lane;
-      const int hg = static_cast<int>(i / n_slices), r = static_cast<int>(i - static_cast<int64_t>(hg) * n_slices);
-      const int b = last_le(bpre, B, r);  // (of sequences without slices the last: it has some)
-      const int j = r - bpre[b], pos = (s_start[b] / 16 + j) * 16;
-      const int lo = max(0, s_start[b] - pos), hi = min(16, plan.ctx[b] - pos);
+      const uint32_t i = beg + lane, hg = i / plan.n_slices;
+      const int r = static_cast<int>(i - hg * plan.n_slices);
+      const int b = last_le(plan.slices, B, r);  // (of sequences without slices the last: it has some)
+      const int j = r - plan.slices[b], pos = (plan.start[b] / 16 + j) * 16;
+      const int lo = max(0, plan.start[b] - pos), hi = min(16, plan.ctx[b] - pos);
       const int bi = pos / p.block_size;
       c.row = pos - bi * p.block_size;
       c.blk = __ldcg(p.tables + static_cast<int64_t>(b) * p.table_stride + bi);
@@ -811,7 +514,7 @@ __global__ void __launch_bounds__(kOwnThreads) shared_own_kernel(const SharedPar
         flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
         c.blk = -1;
       }
-      c.meta = lo | hi << 5 | (j == 0 || i == my_a ? 1 << 10 : 0) | (r + 1 == bpre[b + 1] || i == my_e - 1 ? 1 << 11 : 0);
+      c.meta = lo | hi << 5 | (j == 0 || i == my_a ? 1 << 10 : 0) | (r + 1 == plan.slices[b + 1] || i == my_e - 1 ? 1 << 11 : 0);
       c.pair = hg * B + b;
     }
     return c;
@@ -866,6 +569,28 @@ __global__ void __launch_bounds__(kOwnThreads) shared_own_kernel(const SharedPar
     }
   };
   while (c_ok && issued < static_cast<uint32_t>(kRing)) issue_one();
+  // (while the first copies are on their way) what the join needs: the partials of
+  // the pairs, the tiles of the sequences
+  const int gt = blockIdx.x * (kOwnWarps * 32) + warp * 32 + lane, gts = gridDim.x * (kOwnWarps * 32);
+  for (int s = gt; s < B * hgs; s += gts) {
+    const int hg = s / B, b = s - hg * B;
+    int2 at = make_int2(0, 0);
+    if (plan.slices[b + 1] > plan.slices[b]) {
+      const uint32_t before = static_cast<uint32_t>(hg) * plan.n_slices;
+      const uint32_t w0 = deal.part_of(before + plan.slices[b]), w1 = deal.part_of(before + plan.slices[b + 1] - 1);
+      at = make_int2(static_cast<int>(w0) + s, static_cast<int>(w1 - w0) + 1);
+    }
+    p.own_info[s] = at;
+  }
+  for (int b = gt; b < B; b += gts) {
+    int2 at = make_int2(-1, 0);
+    if (plan.start[b] > 0) {
+      const int g = last_le(plan.cu, p.groups, b);  // (of empty groups the last: it holds b)
+      const int m = b - plan.cu[g];
+      at = make_int2(plan.tiles[g] + m / p.tq, m % p.tq);
+    }
+    p.seq_info[b] = at;
+  }
 
   uint32_t qa[kSteps][4];
   float o[kCols][4];
@@ -894,7 +619,7 @@ __global__ void __launch_bounds__(kOwnThreads) shared_own_kernel(const SharedPar
 #pragma unroll
       for (int n = 0; n < kCols; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     }
-    if (issued - consumed == static_cast<uint32_t>(kRing)) copy_wait<kRing - 1>(); else copy_wait<0>();
+    copy_wait_oldest<kRing>(issued - consumed);
     __syncwarp();
     if ((mt >> 12) & 1) {
       float s[2][4];
@@ -936,11 +661,11 @@ __global__ void __launch_bounds__(kOwnThreads) shared_own_kernel(const SharedPar
         }
       }
       float mb_lo = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-      float mb_hi = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+      float mb_hi = kHi ? fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])) : 0.f;
       mb_lo = fmaxf(mb_lo, __shfl_xor_sync(0xffffffffu, mb_lo, 1));
-      mb_hi = fmaxf(mb_hi, __shfl_xor_sync(0xffffffffu, mb_hi, 1));
+      if (kHi) mb_hi = fmaxf(mb_hi, __shfl_xor_sync(0xffffffffu, mb_hi, 1));
       mb_lo = fmaxf(mb_lo, __shfl_xor_sync(0xffffffffu, mb_lo, 2));
-      mb_hi = fmaxf(mb_hi, __shfl_xor_sync(0xffffffffu, mb_hi, 2));
+      if (kHi) mb_hi = fmaxf(mb_hi, __shfl_xor_sync(0xffffffffu, mb_hi, 2));
       // every slice holds a valid token: the new maxima are finite (or the scores are not numbers)
       const float mn_lo = fmaxf(m_lo, mb_lo), mn_hi = fmaxf(m_hi, mb_hi);
       const float al_lo = ex2_approx((m_lo - mn_lo) * p.scale_log2), al_hi = ex2_approx((m_hi - mn_hi) * p.scale_log2);
@@ -952,8 +677,8 @@ __global__ void __launch_bounds__(kOwnThreads) shared_own_kernel(const SharedPar
       for (int nt = 0; nt < 2; ++nt) {
         pr[nt][0] = ex2_approx(fmaf(s[nt][0], p.scale_log2, -ms_lo));
         pr[nt][1] = ex2_approx(fmaf(s[nt][1], p.scale_log2, -ms_lo));
-        pr[nt][2] = ex2_approx(fmaf(s[nt][2], p.scale_log2, -ms_hi));
-        pr[nt][3] = ex2_approx(fmaf(s[nt][3], p.scale_log2, -ms_hi));
+        pr[nt][2] = kHi ? ex2_approx(fmaf(s[nt][2], p.scale_log2, -ms_hi)) : 0.f;
+        pr[nt][3] = kHi ? ex2_approx(fmaf(s[nt][3], p.scale_log2, -ms_hi)) : 0.f;
       }
       l_lo = l_lo * al_lo + ((pr[0][0] + pr[0][1]) + (pr[1][0] + pr[1][1]));
       l_hi = l_hi * al_hi + ((pr[0][2] + pr[0][3]) + (pr[1][2] + pr[1][3]));
@@ -961,8 +686,10 @@ __global__ void __launch_bounds__(kOwnThreads) shared_own_kernel(const SharedPar
       for (int n = 0; n < kCols; ++n) {
         o[n][0] *= al_lo;
         o[n][1] *= al_lo;
-        o[n][2] *= al_hi;
-        o[n][3] *= al_hi;
+        if (kHi) {
+          o[n][2] *= al_hi;
+          o[n][3] *= al_hi;
+        }
       }
       const uint32_t pa0 = pack2<T>(pr[0][0], pr[0][1]), pa1 = pack2<T>(pr[0][2], pr[0][3]);
       const uint32_t pa2 = pack2<T>(pr[1][0], pr[1][1]), pa3 = pack2<T>(pr[1][2], pr[1][3]);
@@ -978,7 +705,15 @@ __global__ void __launch_bounds__(kOwnThreads) shared_own_kernel(const SharedPar
           b1 &= keep[1];
           b2 &= keep[0];
           b3 &= keep[1];
-          if constexpr (HP == 1) {
+          if constexpr (!kHi) {
+            float x[4] = {o[2 * dp][0], o[2 * dp][1], 0.f, 0.f}, y[4] = {o[2 * dp + 1][0], o[2 * dp + 1][1], 0.f, 0.f};
+            mma_16816<T>(x, pa0, 0u, pa2, 0u, b0, b1);
+            mma_16816<T>(y, pa0, 0u, pa2, 0u, b2, b3);
+            o[2 * dp][0] = x[0];
+            o[2 * dp][1] = x[1];
+            o[2 * dp + 1][0] = y[0];
+            o[2 * dp + 1][1] = y[1];
+          } else if constexpr (HP == 1) {
             mma_16816<T>(o[2 * dp], pa0, pa1, pa2, pa3, b0, b1);
             mma_16816<T>(o[2 * dp + 1], pa0, pa1, pa2, pa3, b2, b3);
           } else {
@@ -1006,44 +741,423 @@ __global__ void __launch_bounds__(kOwnThreads) shared_own_kernel(const SharedPar
       lh += __shfl_xor_sync(0xffffffffu, lh, 2);
       float* const part = p.own_part + static_cast<int64_t>(gw + pair) * own_floats(D);
       float2* const ml = reinterpret_cast<float2*>(part + 16 * D);
+      // dims 8 n + 2 t, + 1 of rows gq and gq + 8: halves of column group 2 n + t / 2
 #pragma unroll
       for (int n = 0; n < kCols; ++n) {
-        if (row_lo) *reinterpret_cast<float2*>(part + gq * D + 8 * n + 2 * t) = make_float2(o[n][0], o[n][1]);
-        if (row_hi) *reinterpret_cast<float2*>(part + (gq + 8) * D + 8 * n + 2 * t) = make_float2(o[n][2], o[n][3]);
+        float* const at = part + (2 * n + (t >> 1)) * 64 + 2 * (t & 1);
+        if (row_lo) *reinterpret_cast<float2*>(at + 4 * gq) = make_float2(o[n][0], o[n][1]);
+        if (row_hi) *reinterpret_cast<float2*>(at + 4 * (gq + 8)) = make_float2(o[n][2], o[n][3]);
       }
       if (t == 0 && row_lo) ml[gq] = make_float2(m_lo * p.scale_log2, ll);
       if (t == 0 && row_hi) ml[gq + 8] = make_float2(m_hi * p.scale_log2, lh);
     }
   }
-  pdl_wait();  // shared_prefix_kernel's end (see above)
+}
+
+template <typename T, int D, int HP, bool HI>
+__global__ void __launch_bounds__(kThreads, 1)
+    shared_main_kernel(const SharedParams p, const __grid_constant__ CUtensorMap tm_q,
+                       const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+  using Geo = TcGeom<D>;
+  constexpr int kH = Geo::kH, kStages = Geo::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
+  uint64_t* const bar_q = reinterpret_cast<uint64_t*>(smem + Geo::kOffBars);  // [2] a stream's Q landed
+  uint64_t* const bar_k = bar_q + 2;               // [kStages] K landed
+  uint64_t* const bar_kfree = bar_k + kStages;     // [kStages] Q K^T of the step done (two arrivals: both streams', or one's twice)
+  uint64_t* const bar_v = bar_kfree + kStages;     // [kStages] V landed
+  uint64_t* const bar_vfree = bar_v + kStages;     // [kStages] P V of the step done (the same)
+  // of each stream, two in turn (a barrier's next phase needs this one's products):
+  uint64_t* const bar_s = bar_vfree + kStages;     // [2][2] S written
+  uint64_t* const bar_p = bar_s + 4;               // [2][2] P written over it
+  uint64_t* const bar_pv = bar_p + 4;              // [2][2] P V done
+  uint64_t* const bar_drain = bar_pv + 4;          // [2] after a failed wait: every product of the stream issued so far is done
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bar_drain + 2);
+  static_assert((16 + 4 * kStages) * 8 + 4 <= 320, "barriers fit their area");
+  Plan plan(reinterpret_cast<int32_t*>(smem + Geo::kOffRing + OwnGeom<D, HP>::kBytes), p.batch, p.groups, p.tq);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int TQ = p.tq, group = p.group;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(bar_k + i, 1);
+      mbar_init(bar_kfree + i, 2);
+      mbar_init(bar_v + i, 1);
+      mbar_init(bar_vfree + i, 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_q + i, 1);
+      mbar_init(bar_drain + i, 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar_s + i, 1);
+      mbar_init(bar_p + i, kRows);
+      mbar_init(bar_pv + i, 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(s_tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  pdl_wait();  // lengths, groups, tables, q and the pools may come from the stream predecessor
+  pdl_launch_dependents();
+  tc_fence_before();
+  build_plan(p, plan);  // (its barriers are also those behind the set-up above)
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  const uint32_t total = static_cast<uint32_t>(plan.n_cost) * p.hkv;  // below 2^31
+  const Deal deal(total, min(gridDim.x, (total + kMinCost - 1) / kMinCost));
+  const uint32_t cta = blockIdx.x;
+  Cursor first;
+  first.left = 0;
+  if (cta < deal.parts) {
+    Cursor end;
+    const uint32_t my_e = deal.start(cta + 1), e = my_e == total ? total : end.seek(plan, my_e);
+    first.left = static_cast<int>(e - first.seek(plan, deal.start(cta)));
+  }
+  bool fail = false;
+
+  // ---- products of stream s ----
+  auto products = [&](auto stream) {
+    constexpr int s = decltype(stream)::value;
+    constexpr int kFmt = Elem<T>::code == PSB_BF16 ? 1 : 0;
+    constexpr uint32_t idesc_s = umma_idesc_f16(kFmt, kRows, kBN, 0, 0), idesc_o = umma_idesc_f16(kFmt, kRows, D, 0, 1);
+    const bool on = elect_one();
+    const uint32_t s_base = smem_u32(smem);
+    // descriptors: their low words (addresses) move, their high ones do not
+    const uint64_t dq = umma_desc_sw128(s_base + s * kH * kQHalf, 1024, 16);
+    const uint64_t dk = umma_desc_sw128(s_base + Geo::kOffK, 1024, 16);
+    const uint64_t dv = umma_desc_sw128(s_base + Geo::kOffV, 1024, kKvHalf);  // (of D 128 the second half's dims lie a half tile on)
+    const uint32_t qlo = static_cast<uint32_t>(dq), klo = static_cast<uint32_t>(dk), vlo = static_cast<uint32_t>(dv);
+    const uint32_t khi = static_cast<uint32_t>(dk >> 32), vhi = static_cast<uint32_t>(dv >> 32);  // (Q's is K's)
+    const uint32_t a_q = smem_u32(bar_q + s), a_k = smem_u32(bar_k), a_kfree = smem_u32(bar_kfree), a_v = smem_u32(bar_v),
+                   a_vfree = smem_u32(bar_vfree), a_s = smem_u32(bar_s + 2 * s), a_p = smem_u32(bar_p + 2 * s), a_pv = smem_u32(bar_pv + 2 * s);
+    if (on) prefetch_tmap(&tm_q);
+    const uint32_t box = static_cast<uint32_t>(TQ * group) * 128 * kH;
+    const uint32_t ocol = tmem + kOCol + s * D, scol = tmem + kSCol + 2 * s * kBN;
+    Steps hs(first);
+    // What P V has to know of a step, from its S two steps before: its number in the
+    // CTA's list, whether the run begins (bit 30) and is a pair's (bit 31); of none: kNone.
+    constexpr uint32_t kNone = 0xffffffffu, kBegins = 1u << 30, kTwo = 1u << 31;
+    uint32_t now = kNone, then = kNone, q_ph = 0;
+    bool q_flight = false;
+#pragma unroll 1
+    for (int k = -2;; ++k) {
+      const uint32_t b = k & 1, ph = (k >> 1) & 1;
+      if (k >= 0) {  // P V of step k
+        if (now == kNone) break;
+        const uint32_t g = now & (kBegins - 1), st = g % kStages;
+        if (!warp_wait_at(a_v + 8 * st, (g / kStages) & 1) || !warp_wait_at(a_p + 8 * b, ph)) {
+          fail = true;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t pcol = scol + b * kBN, vd = vlo + st * (kH * kKvHalf >> 4);
+#pragma unroll
+        for (int kk = 0; kk < kBN / 16; ++kk) mma_ts(on, ocol, pcol + 8 * kk, desc_of(vd + 128 * kk, vhi), idesc_o, (now & kBegins) == 0 || kk > 0);
+        mma_commit(on, a_pv + 8 * b);
+        mma_commit(on, a_vfree + 8 * st);
+        if ((now & kTwo) == 0) mma_commit(on, a_vfree + 8 * st);
+      }
+      now = then;
+      then = kNone;
+      if (hs.more(plan, s)) {  // S of step k + 2, whose buffer held P of step k
+        if (hs.begins) {  // the run's Q, once the last S of the run before (step k + 1) is done
+          if (k >= -1 && !warp_wait_at(a_s + 8 * (b ^ 1), ((k + 1) >> 1) & 1)) {
+            fail = true;
+            break;
+          }
+          expect_bytes(on, a_q, box);
+#pragma unroll
+          for (int h = 0; h < kH; ++h)
+            box_load(on, s_base + (s * kH + h) * kQHalf, &tm_q, h * kHalf, hs.r.kvh * group, hs.r.b0 + (hs.r.two ? s * TQ : 0), a_q);
+          q_flight = true;
+          if (!warp_wait_at(a_q, q_ph)) {
+            fail = true;
+            break;
+          }
+          q_ph ^= 1;
+          q_flight = false;
+        }
+        const uint32_t g = uniform(hs.g0 + hs.x), st = g % kStages;
+        then = uniform(g | (hs.begins ? kBegins : 0) | (hs.r.two ? kTwo : 0));
+        if (!warp_wait_at(a_k + 8 * st, (g / kStages) & 1) || (k >= 0 && !warp_wait_at(a_pv + 8 * b, ph))) {
+          fail = true;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t kd = klo + st * (kH * kKvHalf >> 4);
+#pragma unroll
+        for (int h = 0; h < kH; ++h) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ss(on, scol + b * kBN, desc_of(qlo + h * (kQHalf >> 4) + 2 * kk, khi), desc_of(kd + h * (kKvHalf >> 4) + 2 * kk, khi), idesc_s, h > 0 || kk > 0);
+        }
+        mma_commit(on, a_s + 8 * b);
+        mma_commit(on, a_kfree + 8 * st);
+        if ((then & kTwo) == 0) mma_commit(on, a_kfree + 8 * st);
+        hs.next();
+      }
+    }
+    if (fail) {
+      if (on) flag_error(p.err, PSB_DEVERR_TIMEOUT);
+      // let the copy and the products in flight land before shared memory and TMEM are released
+      if (q_flight) (void)warp_wait_at(a_q, q_ph);
+      mma_commit(on, smem_u32(bar_drain + s));
+      (void)warp_wait_at(smem_u32(bar_drain + s), 0);
+    }
+  };
+  auto copies = [&]() {
+    // ---- copies: of K, or of V ----
+    const CUtensorMap* const tm = warp == 10 ? &tm_k : &tm_v;
+    const uint32_t a_full = smem_u32(warp == 10 ? bar_k : bar_v), a_free = smem_u32(warp == 10 ? bar_kfree : bar_vfree);
+    const uint32_t ring = smem_u32(smem) + (warp == 10 ? Geo::kOffK : Geo::kOffV);
+    const bool on = elect_one();
+    if (on) prefetch_tmap(tm);
+    const int bs = p.block_size, box_rows = min(bs, kBN), boxes = kBN / box_rows;
+    const int64_t layer0 = static_cast<int64_t>(p.layer) * p.num_blocks;
+    const uint32_t box_bytes = static_cast<uint32_t>(box_rows) * 128;
+    Cursor cc = first;
+    uint32_t g = 0;  // steps so far
+#pragma unroll 1
+    while (cc.left > 0 && !fail) {
+      const Run r = cc.take(plan);
+      int i0 = r.j0 * kBN / bs, y = r.j0 * kBN - i0 * bs;  // the next step's first block, and its row there (a block of more than a step's keys)
+      const int n_blk = (plan.pre[r.grp] + bs - 1) / bs;
+      const int32_t* const row = p.tables + static_cast<int64_t>(plan.lead[r.grp]) * p.table_stride;
+      int chunk = -1;   // 32 entries of the table at hand, one a lane
+      int32_t id = 0;
+#pragma unroll 1
+      for (int x = 0; x < r.n; ++x, ++g) {
+        const uint32_t st = uniform(g) % kStages;
+        if (g >= kStages && !warp_wait_at(a_free + 8 * st, (g / kStages - 1) & 1)) {
+          fail = true;
+          break;
+        }
+        const int n = min(boxes, n_blk - i0);  // blocks behind the prefix are not loaded: their keys are masked
+        expect_bytes(on, a_full + 8 * st, static_cast<uint32_t>(n) * box_bytes * kH);
+        uint32_t dst = ring + st * (kH * kKvHalf);
+#pragma unroll 1
+        for (int b = 0; b < n; ++b, dst += box_bytes) {
+          const int i = i0 + b;
+          if ((i >> 5) != chunk) {
+            chunk = i >> 5;
+            const int mine = chunk * 32 + lane;
+            id = 0;
+            if (mine < n_blk) {
+              id = __ldcg(row + mine);
+              if (id < 0 || id >= p.num_blocks) {  // flagged, and another block's keys read in its place
+                flag_error(p.err, PSB_DEVERR_BLOCK_RANGE);
+                id = 0;
+              }
+            }
+            __syncwarp();
+          }
+          const int32_t tile = static_cast<int32_t>((layer0 + __shfl_sync(0xffffffffu, id, i & 31)) * p.hkv + r.kvh);
+#pragma unroll
+          for (int h = 0; h < kH; ++h) box_load(on, dst + h * kKvHalf, tm, h * kHalf, y, tile, a_full + 8 * st);
+        }
+        if (bs > kBN) {
+          y += kBN;
+          if (y == bs) {
+            y = 0;
+            ++i0;
+          }
+        } else {
+          i0 += boxes;
+        }
+      }
+    }
+    if (fail) {
+      if (on) flag_error(p.err, PSB_DEVERR_TIMEOUT);
+      // copies still in flight: the newest of each stage
+      for (uint32_t t = g > kStages ? g - kStages : 0; t < g; ++t) (void)warp_wait_at(a_full + 8 * (t % kStages), (t / kStages) & 1);
+    }
+  };
+  if (warp >= kFirstOwn) {
+    own_parts<T, D, HP, HI>(p, plan, smem + Geo::kOffRing);
+  } else if (warp >= 8) {
+    fewer_registers<kOtherRegs>();
+    if (warp == 8) products(Stream<0>());
+    else if (warp == 9) products(Stream<1>());
+    else copies();
+  } else {
+    more_registers<kSoftmaxRegs>();
+    // ---- softmax: thread r of a stream is row r of the tile and lane r of TMEM ----
+    const int s = warp >> 2, row = tid - 128 * s;
+    const int rseq = row / group;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const float sc = p.scale_log2;
+    Cursor cc = first;
+    int half = 0, g0 = 0, k = 0;  // half-steps and steps before the run, this stream's steps so far
+    while (cc.left > 0 && !fail) {
+      const Run r = cc.take(plan);
+      const int pre = plan.pre[r.grp];
+      const int mine = (half + s) & 1;  // which of each two half-steps is this stream's
+      const bool live = rseq < TQ && rseq + (r.two ? s * TQ : 0) < r.n_seq;
+      float ms = -INFINITY, l = 0.f;    // the exponents' reference (times sc), the sum
+      bool begun = false;
+      for (int x = r.two ? 0 : mine; x < r.n; x += r.two ? 1 : 2, ++k) {
+        const int b = k & 1;
+        const uint32_t ph = (k >> 1) & 1;
+        if (!mbar_wait(bar_s + 2 * s + b, ph)) {
+          fail = true;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t t_s = t_lane + kSCol + (2 * s + b) * kBN, t_o = t_lane + kOCol + s * D;
+        const int have = pre - (r.j0 + x) * kBN;  // keys there are, from the step's first on
+        uint32_t sr[kBN];
+        tmem_ld32(t_s, sr);
+        tmem_ld32(t_s + 32, sr + 32);
+        tmem_wait_ld();
+        if (have < kBN) {
+          // V rows behind the prefix (another token's, or never loaded) must
+          // not reach P V, where 0 * NaN would be NaN: this thread's arrival
+          // lets P V read the stage
+          {  // (both streams of a pair, each before its own P V)
+            const int g = g0 + x, st = g % kStages;
+            if (!mbar_wait(bar_v + st, (g / kStages) & 1)) {
+              fail = true;
+              break;
+            }
+            if (row < kBN && row >= have) {
+#pragma unroll
+              for (int h = 0; h < kH; ++h) {
+                const uint32_t vrow = smem_u32(smem) + Geo::kOffV + (st * kH + h) * kKvHalf + row * 128;
+#pragma unroll
+                for (int c = 0; c < 128; c += 16) st_shared_zero16(vrow + c);
+              }
+              fence_proxy_async_smem();  // visible to the tensor core
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < kBN; ++c)
+            if (c >= have) sr[c] = __float_as_uint(-INFINITY);
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kBN; c += 4) {
+          mx0 = max3(mx0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+          mx1 = max3(mx1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+        }
+        const float mxs = fmaxf(mx0, mx1) * sc;
+        const bool grow = mxs > ms + kRescaleLog2;
+        if (__any_sync(0xffffffffu, grow)) {  // (the warp's TMEM access is collective)
+          const float ms_new = grow ? mxs : ms;
+          const float alpha = ms == -INFINITY ? 0.f : ex2_approx(ms - ms_new);  // (a step has at least one key)
+          if (begun) {  // O holds P V of the earlier half-steps once the last of them is done
+            if (!mbar_wait(bar_pv + 2 * s + (b ^ 1), ((k - 1) >> 1) & 1)) {
+              fail = true;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int q = 0; q < D; q += 32) {
+              uint32_t ot[32];
+              tmem_ld32(t_o + q, ot);
+              tmem_wait_ld();
+#pragma unroll
+              for (int d = 0; d < 32; ++d) ot[d] = __float_as_uint(__uint_as_float(ot[d]) * alpha);
+              tmem_st32(t_o + q, ot);
+            }
+            tmem_wait_st();
+          }
+          l *= alpha;
+          ms = ms_new;
+        }
+        begun = true;
+        const float mu = ms == -INFINITY ? 0.f : ms;
+        uint32_t pk[kBN / 2];
+        const uint64_t sc2 = pair2(sc, sc), nmu2 = pair2(-mu, -mu);
+        uint64_t rs2 = pair2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < kBN; c += 2) {
+          const float2 a = unpair2(fma2(pair2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, nmu2));
+          const float x0 = ex2_approx(a.x), x1 = ex2_approx(a.y);
+          rs2 = add2(rs2, pair2(x0, x1));
+          pk[c / 2] = pack2<T>(x0, x1);
+        }
+        const float2 rs = unpair2(rs2);
+        l += rs.x + rs.y;
+        tmem_st32(t_s, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar_p + 2 * s + b);
+      }
+      if (fail) break;
+      // the run's partial; the next run's first P V comes after its P
+      const int ord = r.kvh * plan.n_pairs + r.pair;
+      float* const part = p.tile_part + static_cast<int64_t>(2 * (cta + ord) + s) * tile_floats(D);
+      if (begun) {
+        if (!warp_wait(bar_pv + 2 * s + ((k - 1) & 1), ((k - 1) >> 1) & 1)) {
+          fail = true;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll 1
+        for (int q = 0; q < D; q += 32) {
+          uint32_t ot[32];
+          tmem_ld32(t_lane + kOCol + s * D + q, ot);
+          tmem_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 4)
+              reinterpret_cast<float4*>(part)[((q + d) >> 2) * kRows + row] =
+                  make_float4(__uint_as_float(ot[d]), __uint_as_float(ot[d + 1]), __uint_as_float(ot[d + 2]), __uint_as_float(ot[d + 3]));
+          }
+          __syncwarp();
+        }
+        tc_fence_before();
+      }
+      if (live) reinterpret_cast<float2*>(part + kRows * D)[row] = make_float2(ms, l);  // (of a stream without steps: none)
+      if (r.j0 == 0 && tid == 0) {
+        const int steps = plan.steps_of(r.grp);
+        const uint32_t begin = static_cast<uint32_t>(r.kvh) * plan.n_cost + plan.cost[r.grp] + 2 * r.in_grp * steps;
+        const int ctas = static_cast<int>(deal.part_of(begin + (r.two ? 2 : 1) * steps - 1) - cta) + 1;
+        int2* const info = p.tile_info + r.kvh * p.max_tiles + r.tile;
+        const int slot = 2 * static_cast<int>(cta + ord);
+        info[0] = r.two ? make_int2(slot, ctas | 2 << 16) : make_int2(slot, 2 * ctas | 1 << 16);
+        if (r.two) info[1] = make_int2(slot + 1, ctas | 2 << 16);
+      }
+      half += r.two ? 2 * r.n : r.n;
+      g0 += r.n;
+    }
+    if (fail && lane == 0) flag_error(p.err, PSB_DEVERR_TIMEOUT);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
 }
 
 // ---------------------------------------------------------------------------
 // the join
 // ---------------------------------------------------------------------------
-// One row (a sequence's q head) per D / 4 lanes, four partials in flight (they
+// A lane has a row (a sequence's q head of one kv head) and four of its dims, a warp 32
+// consecutive rows, whose partials lie side by side; eight partials in flight (they
 // come from L2: a round of loads costs more than their bytes).
-constexpr int kJoinThreads = 128, kBatch = 4;
+constexpr int kJoinThreads = 128, kBatch = 8;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedParams p, int hp) {
-  constexpr int kLanes = D / 4, kRowsWarp = 32 / kLanes;
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int64_t u = (static_cast<int64_t>(blockIdx.x) * (kJoinThreads / 32) + (threadIdx.x >> 5)) * kRowsWarp + lane / kLanes;
-  const int hq = p.hkv * p.group;
-  if (u >= static_cast<int64_t>(p.batch) * hq) return;
-  const int c4 = lane % kLanes, b = static_cast<int>(u / hq), head = static_cast<int>(u - static_cast<int64_t>(b) * hq);
-  const int kvh = head / p.group, gh = head - kvh * p.group;
+  const int c4 = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5), kvh = blockIdx.z;
+  const int u = blockIdx.x * 32 + lane;
+  if (u >= p.batch * p.group) return;
+  const int b = u / p.group, gh = u - b * p.group;
   const int s = (kvh / hp) * p.batch + b;
   const int2 seq = __ldcg(p.seq_info + b), own = __ldcg(p.own_info + s);
   int2 tile = make_int2(0, 0);
   if (seq.x >= 0) tile = __ldcg(p.tile_info + kvh * p.max_tiles + seq.x);
   const int trow = seq.y * p.group + gh, orow = (hp == 2 ? (kvh & 1) * 8 : 0) + gh;
+  const int tiles = tile.y & 0xffff, apart = tile.y >> 16, n = tiles + own.y;
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int n = tile.y + own.y;
   for (int i0 = 0; i0 < n; i0 += kBatch) {
     float2 ml[kBatch];
     float4 v[kBatch];
@@ -1052,14 +1166,13 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
       const int i = i0 + j;
       ml[j] = make_float2(-INFINITY, 0.f);
       v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i < tile.y) {
-        const float* part = p.tile_part + static_cast<int64_t>(tile.x + i) * tile_floats(D);
-        ml[j] = __ldcg(reinterpret_cast<const float2*>(part + kRows * D) + trow);
-        v[j] = __ldcg(reinterpret_cast<const float4*>(part) + c4 * kRows + trow);
-      } else if (i < n) {
-        const float* part = p.own_part + static_cast<int64_t>(own.x + i - tile.y) * own_floats(D);
-        ml[j] = __ldcg(reinterpret_cast<const float2*>(part + 16 * D) + orow);
-        v[j] = __ldcg(reinterpret_cast<const float4*>(part + orow * D) + c4);
+      if (i < n) {
+        const bool of_tile = i < tiles;
+        const float* const part = of_tile ? p.tile_part + static_cast<int64_t>(tile.x + i * apart) * tile_floats(D)
+                                          : p.own_part + static_cast<int64_t>(own.x + i - tiles) * own_floats(D);
+        const int rows = of_tile ? kRows : 16, row = of_tile ? trow : orow;
+        ml[j] = __ldcg(reinterpret_cast<const float2*>(part + rows * D) + row);
+        v[j] = __ldcg(reinterpret_cast<const float4*>(part) + c4 * rows + row);
       }
     }
     float mn = m;
@@ -1074,6 +1187,7 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
     o.w *= a;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
+      if (ml[j].x == -INFINITY) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);  // nothing was summed (nor written)
       const float w = ex2_approx(ml[j].x - mu);
       l = fmaf(ml[j].y, w, l);
       o.x = fmaf(v[j].x, w, o.x);
@@ -1083,11 +1197,17 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* const out = reinterpret_cast<T*>(p.out) + b * p.osb + head * p.osh + 4 * c4;
-  out[0] = Elem<T>::from_float(o.x * inv);
-  out[1] = Elem<T>::from_float(o.y * inv);
-  out[2] = Elem<T>::from_float(o.z * inv);
-  out[3] = Elem<T>::from_float(o.w * inv);
+  T* const out = reinterpret_cast<T*>(p.out) + b * p.osb + (kvh * p.group + gh) * p.osh + 4 * c4;
+  const uint32_t lo = pack2<T>(o.x * inv, o.y * inv), hi = pack2<T>(o.z * inv, o.w * inv);
+  if (reinterpret_cast<uintptr_t>(out) % 8 == 0) {
+    *reinterpret_cast<uint2*>(out) = make_uint2(lo, hi);
+  } else {
+    uint16_t* const o16 = reinterpret_cast<uint16_t*>(out);
+    o16[0] = static_cast<uint16_t>(lo);
+    o16[1] = static_cast<uint16_t>(lo >> 16);
+    o16[2] = static_cast<uint16_t>(hi);
+    o16[3] = static_cast<uint16_t>(hi >> 16);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1100,14 +1220,15 @@ bool takes(int batch, int groups, int q_heads, int hkv, int head_dim, int block_
   if (group > 16 || block_size < 16 || block_size % 16 || !(64 % block_size == 0 || block_size % 64 == 0)) return false;
   const int64_t steps = (static_cast<int64_t>(max_context) + kBN) / kBN, tiles = batch / (kRows / group) + std::min(groups, batch / 2) + 1;
   return static_cast<int64_t>(batch) * hkv < (1 << 24) && steps * tiles < (int64_t(1) << 31) / hkv &&
-         static_cast<int64_t>(max_context) * batch / 16 < (int64_t(1) << 31) / 2;
+         (static_cast<int64_t>(max_context) / 16 + 2) * batch < (int64_t(1) << 31) / hkv;
 }
 
 struct Layout {
-  int max_tiles;
+  int max_tiles, max_pairs;
   size_t tile_info, seq_info, own_info, tile_part, own_part, bytes;
   Layout(int batch, int groups, int group, int hkv, int d) {
     max_tiles = batch / (kRows / group) + std::min(groups, batch / 2) + 1;
+    max_pairs = batch / (2 * (kRows / group)) + std::min(groups, batch / 2) + 1;
     size_t at = 0;
     auto take = [&](size_t n) {
       const size_t r = at;
@@ -1117,8 +1238,8 @@ struct Layout {
     tile_info = take(sizeof(int2) * static_cast<size_t>(hkv) * max_tiles);
     seq_info = take(sizeof(int2) * static_cast<size_t>(batch));
     own_info = take(sizeof(int2) * static_cast<size_t>(hkv) * batch);
-    tile_part = take(sizeof(float) * tile_floats(d) * (static_cast<size_t>(hkv) * max_tiles + kMaxTcCtas));
-    own_part = take(sizeof(float) * own_floats(d) * (static_cast<size_t>(hkv) * batch + static_cast<size_t>(kMaxOwnCtas) * kOwnWarps));
+    tile_part = take(sizeof(float) * tile_floats(d) * 2 * (static_cast<size_t>(hkv) * max_pairs + kMaxCtas));
+    own_part = take(sizeof(float) * own_floats(d) * (static_cast<size_t>(hkv) * batch + static_cast<size_t>(kMaxCtas) * kOwnWarps));
     bytes = at;
   }
 };
@@ -1128,7 +1249,7 @@ int launch(SharedParams p, int num_layers, cudaStream_t s) {
   const CUtensorMapDataType dt = Elem<T>::code == PSB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const int sms = device_sm_count();
   if (sms <= 0) return PSB_ERR_CUDA;
-  const bool two = D == 64 && p.group <= 8 && p.hkv % 2 == 0;  // (a tile of two heads of D 128 takes too many registers)
+  const bool two = D == 64 && p.group <= 8 && p.hkv % 2 == 0;
   CUtensorMap tq, tk, tv;
   const int64_t tiles = static_cast<int64_t>(num_layers) * p.num_blocks * p.hkv, hq = static_cast<int64_t>(p.hkv) * p.group;
   const int64_t qdims[3] = {D, hq, p.batch}, qstr[2] = {p.qsh * 2, p.qsb * 2}, kdims[3] = {D, p.block_size, tiles},
@@ -1137,25 +1258,27 @@ int launch(SharedParams p, int num_layers, cudaStream_t s) {
   if (!encode_box_map(&tq, p.q, qdims, qstr, qbox, dt) || !encode_box_map(&tk, p.k_cache, kdims, kstr, kbox, dt) ||
       !encode_box_map(&tv, p.v_cache, kdims, kstr, kbox, dt))
     return PSB_ERR_CUDA;
-  const auto pre = shared_prefix_kernel<T, D>;
-  const auto own = two ? shared_own_kernel<T, D, D == 64 ? 2 : 1> : shared_own_kernel<T, D, 1>;
-  const auto join = shared_join_kernel<T, D>;
-  const size_t pre_smem = 1024 + TcGeom<D>::kOffPlan + sizeof(int32_t) * (Plan::ints(p.batch, p.groups) + 2 * (static_cast<size_t>(p.groups) + 1));
-  const size_t own_smem = 1024 + (two ? OwnGeom<D, D == 64 ? 2 : 1>::kBytes : OwnGeom<D, 1>::kBytes) +
-                          sizeof(int32_t) * (Plan::ints(p.batch, p.groups) + 2 * static_cast<size_t>(p.batch) + 1);
-  int occ = 0, own_occ = 0;
-  if (!kernel_occupancy(reinterpret_cast<const void*>(pre), kTcThreads, pre_smem, &occ) || occ < 1 ||
-      !kernel_occupancy(reinterpret_cast<const void*>(own), kOwnThreads, own_smem, &own_occ) || own_occ < 1)
-    return PSB_ERR_CUDA;
+  // (a tile of two heads of D 128 takes too many registers)
+  const bool hi = !two && p.group > 8;
+  const auto kern = two ? shared_main_kernel<T, D, D == 64 ? 2 : 1, false> : hi ? shared_main_kernel<T, D, 1, true> : shared_main_kernel<T, D, 1, false>;
+  const void* const f = reinterpret_cast<const void*>(kern);
+  static std::atomic<bool> checked[3];  // (of each instantiation) the shares draw on the launch's registers
+  if (!checked[two ? 2 : hi].load(std::memory_order_relaxed)) {
+    cudaFuncAttributes fa;
+    const cudaError_t fe = cudaFuncGetAttributes(&fa, f);
+    if (fe != cudaSuccess) return record_cuda_error(fe);
+    if (fa.numRegs != 128) return PSB_ERR_UNSUPPORTED;
+    checked[two ? 2 : hi].store(true, std::memory_order_relaxed);
+  }
+  const size_t smem = 1024 + TcGeom<D>::kOffRing + (two ? OwnGeom<D, D == 64 ? 2 : 1>::kBytes : OwnGeom<D, 1>::kBytes) +
+                      sizeof(int32_t) * Plan::ints(p.batch, p.groups);
+  int occ = 0;
+  if (!kernel_occupancy(f, kThreads, smem, &occ)) return PSB_ERR_CUDA;
+  if (occ < 1) return PSB_ERR_UNSUPPORTED;
   discard_stale_error();
-  const int pre_grid = std::min(kMaxTcCtas, sms * std::min(occ, 2));
-  cudaError_t e = launch_pdl(pre, dim3(pre_grid), dim3(kTcThreads), pre_smem, s, p, tq, tk, tv);
+  cudaError_t e = launch_pdl(kern, dim3(std::min(kMaxCtas, sms)), dim3(kThreads), smem, s, p, tq, tk, tv);
   if (e != cudaSuccess) return record_cuda_error(e);
-  const int own_grid = std::min(kMaxOwnCtas, sms * std::min(own_occ, 2));
-  e = launch_pdl(own, dim3(own_grid), dim3(kOwnThreads), own_smem, s, p);
-  if (e != cudaSuccess) return record_cuda_error(e);
-  const int64_t rows = static_cast<int64_t>(p.batch) * hq, per = kJoinThreads / (D / 4);
-  e = launch_pdl(join, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(kJoinThreads), 0, s, p, two ? 2 : 1);
+  e = launch_pdl(shared_join_kernel<T, D>, dim3((p.batch * p.group + 31) / 32, D / 4 / (kJoinThreads / 32), p.hkv), dim3(kJoinThreads), 0, s, p, two ? 2 : 1);
   if (e != cudaSuccess) return record_cuda_error(e);
   return check_launch();
 }
@@ -1216,6 +1339,7 @@ extern "C" int psb_paged_decode_shared(const void* query, int64_t q_stride_b, in
   p.max_context = max_context;
   p.tq = kRows / group;
   p.max_tiles = lay.max_tiles;
+  p.max_pairs = lay.max_pairs;
   p.num_blocks = num_blocks;
   p.scale_log2 = scale * 1.4426950408889634f;
   char* const ws = static_cast<char*>(workspace);

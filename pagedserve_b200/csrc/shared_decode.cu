@@ -47,7 +47,8 @@
 namespace psb {
 namespace {
 
-constexpr int kMaxBatch = 2048;      // sequences (and groups) whose plan fits shared memory beside the rings
+constexpr int kMaxBatch = 2048;      // sequences, and groups (fewer where their plan does not fit shared memory beside the rings)
+constexpr size_t kMaxSmem = 227 * 1024;
 constexpr int kOwnWarps = 4, kFirstOwn = 12;  // warps 0-7: softmax, two streams; 8, 9: their products; 10, 11: copies of K, of V; 12-15: own parts
 constexpr int kThreads = 512;
 // Registers: 128 a thread at launch, and the shares they are dealt anew in.
@@ -62,24 +63,26 @@ constexpr uint32_t kKvHalf = kBN * 128;    // of a K or V tile
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kSCol = 0, kOCol = 4 * kBN;
 constexpr float kRescaleLog2 = 8.f;  // O is rescaled when a row's maximum grows by more than 2^8
-constexpr int kMinCost = 4;          // steps of a tile per CTA below which the grid shrinks (at least 2: see Cursor)
+constexpr int kMinCost = 8;          // steps of a tile per CTA below which the grid shrinks (at least 2: see Cursor)
 constexpr int kOwnMinItems = 2;      // slices per warp below which fewer warps work
 constexpr int kMaxCtas = 160;        // (B200 has 148 SMs)
 
 template <int D>
 struct TcGeom {
   static constexpr int kH = D / kHalf;
-  static constexpr int kStages = D == 64 ? 4 : 2;  // (a power of two)
+  static constexpr int kStages = D == 64 ? 4 : 2;
   static constexpr uint32_t kOffK = 2 * kH * kQHalf;  // behind a Q tile for each stream
   static constexpr uint32_t kOffV = kOffK + kStages * kH * kKvHalf;
+  static constexpr uint32_t kBarBytes = 384;
   static constexpr uint32_t kOffBars = kOffV + kStages * kH * kKvHalf;
-  static constexpr uint32_t kOffRing = (kOffBars + 320 + 1023) / 1024 * 1024;
+  static constexpr uint32_t kOffRing = (kOffBars + kBarBytes + 1023) / 1024 * 1024;
 };
 
 template <int D, int HP>
 struct OwnGeom {
-  static constexpr int kRing = D == 64 && HP == 2 ? 3 : 2;  // slots per warp
-  static constexpr int kTile = 16 * D * 2;        // 16 tokens of one kv head
+  static constexpr int kRing = D == 64 ? 3 : 2;  // slots per warp
+  static constexpr int kBox = 16 * 128;          // 16 tokens of one kv head, 64 dims
+  static constexpr int kTile = D / kHalf * kBox;
   static constexpr int kKV = HP * kTile;
   static constexpr int kSlot = 2 * kKV;
   static constexpr int kBytes = kOwnWarps * kRing * kSlot;
@@ -314,6 +317,15 @@ __device__ __forceinline__ void box_load(bool on, uint32_t dst, const CUtensorMa
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(static_cast<uint32_t>(on))
       : "memory");
 }
+// the same, of what is read once
+__device__ __forceinline__ void box_load_once(bool on, uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %7;\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(static_cast<uint32_t>(on)), "l"(policy)
+      : "memory");
+}
 __device__ __forceinline__ void expect_bytes(bool on, uint32_t bar, uint32_t bytes) {
   asm volatile(
       "{\n\t.reg .pred q;\n\t"
@@ -337,7 +349,7 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ bool warp_wait_at(uint32_t bar, uint32_t parity) {
   uint64_t t0 = 0;
 #pragma unroll 1
-  while (!__any_sync(0xffffffffu, mbar_try_wait_sleep(bar, parity, 100000u))) {
+  while (!__all_sync(0xffffffffu, mbar_try_wait_sleep(bar, parity, 100000u))) {
     const uint64_t t = globaltimer_ns();
     if (t0 == 0) t0 = t;
     if (__all_sync(0xffffffffu, t - t0 > kWaitLimitNs)) return false;
@@ -440,39 +452,19 @@ __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.
 template <int N>
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// 16-byte asynchronous copies, grouped
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint64_t policy) {
-  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-// Until the oldest of ``flight`` (1 .. N) groups has landed.
-template <int N>
-__device__ __forceinline__ void copy_wait_oldest(uint32_t flight) {
-  if constexpr (N > 1) {
-    if (flight >= N) {
-      copy_wait<N - 1>();
-      return;
-    }
-    copy_wait_oldest<N - 1>(flight);
-  } else {
-    copy_wait<0>();
-  }
-}
-
 // ---------------------------------------------------------------------------
 // each sequence's own part
 // ---------------------------------------------------------------------------
 // As the plain decode: a warp streams its slices (16 tokens of HP kv heads)
-// through a ring of its own with 16-byte cp.async copies.  HP = 2 (up to 8 q
-// heads per kv head): rows 0-7 of the m16n8k16 tile are one kv head's q heads,
-// rows 8-15 the next one's.  HP = 1: up to 16 q heads of one kv head; HI: there are
-// more than 8 (else the upper rows' registers are not kept).
+// through a ring of its own.  HP = 2 (up to 8 q heads per kv head): rows 0-7 of the
+// m16n8k16 tile are one kv head's q heads, rows 8-15 the next one's.  HP = 1: up to 16
+// q heads of one kv head; HI: there are more than 8 (else the upper rows' registers are
+// not kept).  The copies are boxes of 16 tokens and 64 dims, one instruction each: with
+// 16 bytes a lane and instruction, half of a warp's time and more went into issuing them.
 template <typename T, int D, int HP, bool HI>
-__device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& plan, uint8_t* ring_all) {
+__device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& plan, const CUtensorMap* tm_k, const CUtensorMap* tm_v, uint8_t* ring_all, uint64_t* bars_all) {
   using Geo = OwnGeom<D, HP>;
-  constexpr int kRing = Geo::kRing, kSteps = D / 16, kCols = D / 8;  // k steps; 16-byte columns of a row
+  constexpr int kRing = Geo::kRing, kH = D / kHalf, kSteps = D / 16, kCols = D / 8;  // k steps; 16-byte columns of a row
   constexpr bool kHi = HP == 2 || HI;
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - kFirstOwn;
   const int gq = lane >> 2, t = lane & 3;
@@ -483,6 +475,12 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
   const uint32_t gw = warp * gridDim.x + blockIdx.x;
   const uint32_t my_a = gw < deal.parts ? deal.start(gw) : 0, my_e = gw < deal.parts ? deal.start(gw + 1) : 0;
   const uint32_t ring_u = smem_u32(ring_all) + warp * kRing * Geo::kSlot;
+  const uint32_t bars = smem_u32(bars_all) + warp * kRing * 8;  // a slot's copies landed
+  const bool on = elect_one();
+  if (on) {
+    prefetch_tmap(tm_k);
+    prefetch_tmap(tm_v);
+  }
   const uint64_t policy = l2_policy_evict_first();
   const int64_t layer0 = static_cast<int64_t>(p.layer) * p.num_blocks;
   const bool row_lo = gq < G, row_hi = kHi && (HP == 2 ? gq < G : gq + 8 < G);
@@ -537,21 +535,16 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
     const uint32_t dst = ring_u + slot * Geo::kSlot;
     const int32_t blk = __shfl_sync(0xffffffffu, cur.blk, ib), r0 = __shfl_sync(0xffffffffu, cur.row, ib);
     const int32_t mt = __shfl_sync(0xffffffffu, cur.meta, ib), pair = __shfl_sync(0xffffffffu, cur.pair, ib);
+    const uint32_t bar = bars + slot * 8;
+    expect_bytes(on, bar, blk >= 0 ? Geo::kSlot : 0);
     if (blk >= 0) {
-      const int hg = pair / B;
+      const int32_t tile = static_cast<int32_t>((layer0 + blk) * p.hkv + pair / B * HP);
 #pragma unroll
-      for (int hs = 0; hs < HP; ++hs) {
-        const int64_t at = (((layer0 + blk) * p.hkv + hg * HP + hs) * p.block_size + r0) * (D * 2);
-#pragma unroll
-        for (int i = 0; i < 16 * kCols / 32; ++i) {
-          const int c = lane + 32 * i, r = c / kCols, col = c % kCols;
-          const uint32_t d = dst + hs * Geo::kTile + r * (D * 2) + ((col ^ (r & 7)) << 4);
-          copy16(d, p.k_cache + at + c * 16, policy);
-          copy16(d + Geo::kKV, p.v_cache + at + c * 16, policy);
-        }
+      for (int x = 0; x < HP * kH; ++x) {
+        box_load_once(on, dst + x * Geo::kBox, tm_k, x % kH * kHalf, r0, tile + x / kH, bar, policy);
+        box_load_once(on, dst + Geo::kKV + x * Geo::kBox, tm_v, x % kH * kHalf, r0, tile + x / kH, bar, policy);
       }
     }
-    copy_commit();
     if (lane == static_cast<int>(slot)) {
       meta = mt | (blk >= 0 ? 1 << 12 : 0);
       meta_pair = pair;
@@ -619,8 +612,11 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
 #pragma unroll
       for (int n = 0; n < kCols; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     }
-    copy_wait_oldest<kRing>(issued - consumed);
-    __syncwarp();
+    if (!warp_wait_at(bars + slot * 8, (consumed / kRing) & 1)) {
+      if (on) flag_error(p.err, PSB_DEVERR_TIMEOUT);
+      for (uint32_t i = consumed + 1; i != issued; ++i) (void)warp_wait_at(bars + i % kRing * 8, (i / kRing) & 1);  // the other copies in flight
+      return;
+    }
     if ((mt >> 12) & 1) {
       float s[2][4];
 #pragma unroll
@@ -629,11 +625,11 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
 #pragma unroll
         for (int hs = 0; hs < HP; ++hs) {
           acc[hs][0] = acc[hs][1] = acc[hs][2] = acc[hs][3] = 0.f;  // (of its rows, half are the other head's: not used)
-          const uint32_t krow = base + hs * Geo::kTile + (nt * 8 + (lane & 7)) * (D * 2);
+          const uint32_t krow = base + hs * Geo::kTile + (nt * 8 + (lane & 7)) * 128;
 #pragma unroll
           for (int kp = 0; kp < kSteps / 2; ++kp) {  // two k steps a load
             uint32_t b0, b1, b2, b3;
-            ldsm_x4(krow + (((kp * 4 + (lane >> 3)) ^ (lane & 7)) << 4), b0, b1, b2, b3);
+            ldsm_x4(krow + (kp >> 1) * Geo::kBox + ((((kp & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4), b0, b1, b2, b3);
             mma_16816<T>(acc[hs], qa[2 * kp][0], qa[2 * kp][1], qa[2 * kp][2], qa[2 * kp][3], b0, b1);
             mma_16816<T>(acc[hs], qa[2 * kp + 1][0], qa[2 * kp + 1][1], qa[2 * kp + 1][2], qa[2 * kp + 1][3], b2, b3);
           }
@@ -696,11 +692,11 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
       const int vr = ((lane >> 3) & 1) * 8 + (lane & 7);
 #pragma unroll
       for (int hs = 0; hs < HP; ++hs) {
-        const uint32_t vrow = base + Geo::kKV + hs * Geo::kTile + vr * (D * 2);
+        const uint32_t vrow = base + Geo::kKV + hs * Geo::kTile + vr * 128;
 #pragma unroll
         for (int dp = 0; dp < kCols / 2; ++dp) {
           uint32_t b0, b1, b2, b3;
-          ldsm_x4_t(vrow + (((dp * 2 + (lane >> 4)) ^ (vr & 7)) << 4), b0, b1, b2, b3);
+          ldsm_x4_t(vrow + (dp >> 2) * Geo::kBox + ((((dp & 3) * 2 + (lane >> 4)) ^ (vr & 7)) << 4), b0, b1, b2, b3);
           b0 &= keep[0];
           b1 &= keep[1];
           b2 &= keep[0];
@@ -757,23 +753,26 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
 template <typename T, int D, int HP, bool HI>
 __global__ void __launch_bounds__(kThreads, 1)
     shared_main_kernel(const SharedParams p, const __grid_constant__ CUtensorMap tm_q,
-                       const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+                       const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                       const __grid_constant__ CUtensorMap tm_ko, const __grid_constant__ CUtensorMap tm_vo) {
   using Geo = TcGeom<D>;
   constexpr int kH = Geo::kH, kStages = Geo::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
   uint64_t* const bar_q = reinterpret_cast<uint64_t*>(smem + Geo::kOffBars);  // [2] a stream's Q landed
   uint64_t* const bar_k = bar_q + 2;               // [kStages] K landed
-  uint64_t* const bar_kfree = bar_k + kStages;     // [kStages] Q K^T of the step done (two arrivals: both streams', or one's twice)
+  uint64_t* const bar_kfree = bar_k + kStages;     // [kStages] Q K^T of the step done (two arrivals: both streams', or its one's twice)
   uint64_t* const bar_v = bar_kfree + kStages;     // [kStages] V landed
   uint64_t* const bar_vfree = bar_v + kStages;     // [kStages] P V of the step done (the same)
   // of each stream, two in turn (a barrier's next phase needs this one's products):
   uint64_t* const bar_s = bar_vfree + kStages;     // [2][2] S written
   uint64_t* const bar_p = bar_s + 4;               // [2][2] P written over it
   uint64_t* const bar_pv = bar_p + 4;              // [2][2] P V done
-  uint64_t* const bar_drain = bar_pv + 4;          // [2] after a failed wait: every product of the stream issued so far is done
-  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bar_drain + 2);
-  static_assert((16 + 4 * kStages) * 8 + 4 <= 320, "barriers fit their area");
+  uint64_t* const bar_drain = bar_pv + 4;          // [2] every product of the stream is done
+  uint64_t* const bar_own = bar_drain + 2;         // [4][ring] of the own parts' warps: a slot's copies landed
+  constexpr int kOwnBars = kOwnWarps * OwnGeom<D, HP>::kRing;
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bar_own + kOwnBars);
+  static_assert((16 + 4 * kStages + kOwnBars) * 8 + 4 <= Geo::kBarBytes, "barriers fit their area");
   Plan plan(reinterpret_cast<int32_t*>(smem + Geo::kOffRing + OwnGeom<D, HP>::kBytes), p.batch, p.groups, p.tq);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int TQ = p.tq, group = p.group;
@@ -793,6 +792,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar_p + i, kRows);
       mbar_init(bar_pv + i, 1);
     }
+    for (int i = 0; i < kOwnBars; ++i) mbar_init(bar_own + i, 1);
     fence_barrier_init();
   }
   if (warp == 0) {
@@ -835,10 +835,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (on) prefetch_tmap(&tm_q);
     const uint32_t box = static_cast<uint32_t>(TQ * group) * 128 * kH;
     const uint32_t ocol = tmem + kOCol + s * D, scol = tmem + kSCol + 2 * s * kBN;
+    // Until a stage's copies of ``round`` have landed.  Its use before may have been
+    // the other stream's, and a wait for a barrier's phase passes while the phase before
+    // is still open; so first until that use is over.  (That wait is of one phase at a
+    // time: this stream's step before, two back at most, had landed, and was asked for
+    // when the use before the last was over.  The next phase needs this step.)
+    auto landed = [&](uint32_t full, uint32_t free, uint32_t st, uint32_t round) {
+      return (round == 0 || warp_wait_at(free + 8 * st, (round - 1) & 1)) && warp_wait_at(full + 8 * st, round & 1);
+    };
     Steps hs(first);
     // What P V has to know of a step, from its S two steps before: its number in the
-    // CTA's list, whether the run begins (bit 30) and is a pair's (bit 31); of none: kNone.
-    constexpr uint32_t kNone = 0xffffffffu, kBegins = 1u << 30, kTwo = 1u << 31;
+    // CTA's list, how many of its keys there are (bits 24 to 29; 0: all), whether the run
+    // begins (bit 30) and is a pair's (bit 31); of none: kNone.
+    constexpr uint32_t kNone = 0xffffffffu, kStep = (1u << 24) - 1, kBegins = 1u << 30, kTwo = 1u << 31;
     uint32_t now = kNone, then = kNone, q_ph = 0;
     bool q_flight = false;
 #pragma unroll 1
@@ -846,10 +855,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t b = k & 1, ph = (k >> 1) & 1;
       if (k >= 0) {  // P V of step k
         if (now == kNone) break;
-        const uint32_t g = now & (kBegins - 1), st = g % kStages;
-        if (!warp_wait_at(a_v + 8 * st, (g / kStages) & 1) || !warp_wait_at(a_p + 8 * b, ph)) {
+        const uint32_t g = now & kStep, st = g % kStages, round = g / kStages;
+        if (!landed(a_v, a_vfree, st, round) || !warp_wait_at(a_p + 8 * b, ph)) {
           fail = true;
           break;
+        }
+        const uint32_t have = (now >> 24) & 63;
+        if (have != 0) {
+          // V rows behind the prefix (another token's, or never loaded) must not reach
+          // P V, where 0 * NaN would be NaN
+          const uint32_t v0 = s_base + Geo::kOffV + st * (kH * kKvHalf);
+          for (uint32_t c = have * 8 + lane; c < kBN * 8; c += 32) {
+#pragma unroll
+            for (int h = 0; h < kH; ++h) st_shared_zero16(v0 + h * kKvHalf + c * 16);
+          }
+          fence_proxy_async_smem();  // visible to the tensor core
+          __syncwarp();
         }
         tc_fence_after();
         const uint32_t pcol = scol + b * kBN, vd = vlo + st * (kH * kKvHalf >> 4);
@@ -879,9 +900,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           q_ph ^= 1;
           q_flight = false;
         }
-        const uint32_t g = uniform(hs.g0 + hs.x), st = g % kStages;
-        then = uniform(g | (hs.begins ? kBegins : 0) | (hs.r.two ? kTwo : 0));
-        if (!warp_wait_at(a_k + 8 * st, (g / kStages) & 1) || (k >= 0 && !warp_wait_at(a_pv + 8 * b, ph))) {
+        const uint32_t g = uniform(hs.g0 + hs.x), st = g % kStages, round = g / kStages;
+        const int have = plan.pre[hs.r.grp] - (hs.r.j0 + hs.x) * kBN;
+        then = uniform(g | (have < kBN ? have << 24 : 0) | (hs.begins ? kBegins : 0) | (hs.r.two ? kTwo : 0));
+        if (!landed(a_k, a_kfree, st, round) || (k >= 0 && !warp_wait_at(a_pv + 8 * b, ph))) {
           fail = true;
           break;
         }
@@ -901,11 +923,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (fail) {
       if (on) flag_error(p.err, PSB_DEVERR_TIMEOUT);
-      // let the copy and the products in flight land before shared memory and TMEM are released
       if (q_flight) (void)warp_wait_at(a_q, q_ph);
-      mma_commit(on, smem_u32(bar_drain + s));
-      (void)warp_wait_at(smem_u32(bar_drain + s), 0);
     }
+    // the copy, the products and their commits in flight land before shared memory and TMEM are released
+    mma_commit(on, smem_u32(bar_drain + s));
+    (void)warp_wait_at(smem_u32(bar_drain + s), 0);
   };
   auto copies = [&]() {
     // ---- copies: of K, or of V ----
@@ -975,7 +997,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
   if (warp >= kFirstOwn) {
-    own_parts<T, D, HP, HI>(p, plan, smem + Geo::kOffRing);
+    own_parts<T, D, HP, HI>(p, plan, &tm_ko, &tm_vo, smem + Geo::kOffRing, bar_own);
   } else if (warp >= 8) {
     fewer_registers<kOtherRegs>();
     if (warp == 8) products(Stream<0>());
@@ -989,7 +1011,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float sc = p.scale_log2;
     Cursor cc = first;
-    int half = 0, g0 = 0, k = 0;  // half-steps and steps before the run, this stream's steps so far
+    int half = 0, k = 0;  // half-steps before the run, this stream's steps so far
     while (cc.left > 0 && !fail) {
       const Run r = cc.take(plan);
       const int pre = plan.pre[r.grp];
@@ -1012,25 +1034,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld32(t_s + 32, sr + 32);
         tmem_wait_ld();
         if (have < kBN) {
-          // V rows behind the prefix (another token's, or never loaded) must
-          // not reach P V, where 0 * NaN would be NaN: this thread's arrival
-          // lets P V read the stage
-          {  // (both streams of a pair, each before its own P V)
-            const int g = g0 + x, st = g % kStages;
-            if (!mbar_wait(bar_v + st, (g / kStages) & 1)) {
-              fail = true;
-              break;
-            }
-            if (row < kBN && row >= have) {
-#pragma unroll
-              for (int h = 0; h < kH; ++h) {
-                const uint32_t vrow = smem_u32(smem) + Geo::kOffV + (st * kH + h) * kKvHalf + row * 128;
-#pragma unroll
-                for (int c = 0; c < 128; c += 16) st_shared_zero16(vrow + c);
-              }
-              fence_proxy_async_smem();  // visible to the tensor core
-            }
-          }
 #pragma unroll
           for (int c = 0; c < kBN; ++c)
             if (c >= have) sr[c] = __float_as_uint(-INFINITY);
@@ -1121,7 +1124,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (r.two) info[1] = make_int2(slot + 1, ctas | 2 << 16);
       }
       half += r.two ? 2 * r.n : r.n;
-      g0 += r.n;
     }
     if (fail && lane == 0) flag_error(p.err, PSB_DEVERR_TIMEOUT);
   }
@@ -1137,18 +1139,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 // the join
 // ---------------------------------------------------------------------------
 // A lane has a row (a sequence's q head of one kv head) and four of its dims, a warp 32
-// consecutive rows, whose partials lie side by side; eight partials in flight (they
-// come from L2: a round of loads costs more than their bytes).
-constexpr int kJoinThreads = 128, kBatch = 8;
+// consecutive rows, whose partials lie side by side; a CTA's four warps take a quarter
+// of the partials each (they come from L2: rounds of loads, not bytes, are what it
+// costs; one warp for all of 33 partials took 10 us).
+constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32, kBatch = 4;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedParams p, int hp) {
+  __shared__ float2 s_ml[kJoinWarps][32];
+  __shared__ float4 s_o[kJoinWarps][32];
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int c4 = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5), kvh = blockIdx.z;
-  const int u = blockIdx.x * 32 + lane;
-  if (u >= p.batch * p.group) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c4 = blockIdx.y, kvh = blockIdx.z;
+  const int u = min(static_cast<int>(blockIdx.x) * 32 + lane, p.batch * p.group - 1);  // (the last row again behind the last)
   const int b = u / p.group, gh = u - b * p.group;
   const int s = (kvh / hp) * p.batch + b;
   const int2 seq = __ldcg(p.seq_info + b), own = __ldcg(p.own_info + s);
@@ -1158,12 +1162,36 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
   const int tiles = tile.y & 0xffff, apart = tile.y >> 16, n = tiles + own.y;
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < n; i0 += kBatch) {
+  auto add = [&](const float2* ml, const float4* v, int count) {
+    float mn = m;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (j < count) mn = fmaxf(mn, ml[j].x);
+    const float mu = mn == -INFINITY ? 0.f : mn, a = ex2_approx(m - mu);
+    m = mn;
+    l *= a;
+    o.x *= a;
+    o.y *= a;
+    o.z *= a;
+    o.w *= a;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (j >= count || ml[j].x == -INFINITY) continue;  // nothing was summed (nor written)
+      const float w = ex2_approx(ml[j].x - mu);
+      l = fmaf(ml[j].y, w, l);
+      o.x = fmaf(v[j].x, w, o.x);
+      o.y = fmaf(v[j].y, w, o.y);
+      o.z = fmaf(v[j].z, w, o.z);
+      o.w = fmaf(v[j].w, w, o.w);
+    }
+  };
+#pragma unroll 1
+  for (int i0 = warp; i0 < n; i0 += kBatch * kJoinWarps) {
     float2 ml[kBatch];
     float4 v[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const int i = i0 + j;
+      const int i = i0 + j * kJoinWarps;
       ml[j] = make_float2(-INFINITY, 0.f);
       v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i < n) {
@@ -1175,26 +1203,22 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
         v[j] = __ldcg(reinterpret_cast<const float4*>(part) + c4 * rows + row);
       }
     }
-    float mn = m;
+    add(ml, v, kBatch);
+  }
+  s_ml[warp][lane] = make_float2(m, l);
+  s_o[warp][lane] = o;
+  __syncthreads();
+  if (warp != 0 || static_cast<int>(blockIdx.x) * 32 + lane >= p.batch * p.group) return;
+  {
+    static_assert(kBatch >= kJoinWarps - 1, "the other warps' sums in one go");
+    float2 ml[kBatch];
+    float4 v[kBatch];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) mn = fmaxf(mn, ml[j].x);
-    const float mu = mn == -INFINITY ? 0.f : mn, a = ex2_approx(m - mu);
-    m = mn;
-    l *= a;
-    o.x *= a;
-    o.y *= a;
-    o.z *= a;
-    o.w *= a;
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      if (ml[j].x == -INFINITY) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);  // nothing was summed (nor written)
-      const float w = ex2_approx(ml[j].x - mu);
-      l = fmaf(ml[j].y, w, l);
-      o.x = fmaf(v[j].x, w, o.x);
-      o.y = fmaf(v[j].y, w, o.y);
-      o.z = fmaf(v[j].z, w, o.z);
-      o.w = fmaf(v[j].w, w, o.w);
+    for (int j = 0; j < kJoinWarps - 1; ++j) {
+      ml[j] = s_ml[j + 1][lane];
+      v[j] = s_o[j + 1][lane];
     }
+    add(ml, v, kJoinWarps - 1);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* const out = reinterpret_cast<T*>(p.out) + b * p.osb + (kvh * p.group + gh) * p.osh + 4 * c4;
@@ -1213,11 +1237,20 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+bool two_heads(int group, int hkv, int d) { return d == 64 && group <= 8 && hkv % 2 == 0; }  // (D 128: too many registers)
+
+size_t main_smem(int batch, int groups, int group, int hkv, int d) {
+  const size_t fixed = d == 128 ? TcGeom<128>::kOffRing + OwnGeom<128, 1>::kBytes
+                                : TcGeom<64>::kOffRing + (two_heads(group, hkv, d) ? OwnGeom<64, 2>::kBytes : OwnGeom<64, 1>::kBytes);
+  return 1024 + fixed + sizeof(int32_t) * Plan::ints(batch, groups);
+}
+
 bool takes(int batch, int groups, int q_heads, int hkv, int head_dim, int block_size, int dtype, int max_context) {
   if (!(dtype == PSB_BF16 || dtype == PSB_F16) || !(head_dim == 64 || head_dim == 128)) return false;
   if (batch <= 0 || batch > kMaxBatch || groups < 0 || groups > kMaxBatch || hkv <= 0 || q_heads <= 0 || q_heads % hkv) return false;
   const int group = q_heads / hkv;
   if (group > 16 || block_size < 16 || block_size % 16 || !(64 % block_size == 0 || block_size % 64 == 0)) return false;
+  if (main_smem(batch, groups, group, hkv, head_dim) > kMaxSmem || hkv > 65535) return false;
   const int64_t steps = (static_cast<int64_t>(max_context) + kBN) / kBN, tiles = batch / (kRows / group) + std::min(groups, batch / 2) + 1;
   return static_cast<int64_t>(batch) * hkv < (1 << 24) && steps * tiles < (int64_t(1) << 31) / hkv &&
          (static_cast<int64_t>(max_context) / 16 + 2) * batch < (int64_t(1) << 31) / hkv;
@@ -1249,14 +1282,15 @@ int launch(SharedParams p, int num_layers, cudaStream_t s) {
   const CUtensorMapDataType dt = Elem<T>::code == PSB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const int sms = device_sm_count();
   if (sms <= 0) return PSB_ERR_CUDA;
-  const bool two = D == 64 && p.group <= 8 && p.hkv % 2 == 0;
-  CUtensorMap tq, tk, tv;
+  const bool two = two_heads(p.group, p.hkv, D);
+  CUtensorMap tq, tk, tv, tko, tvo;
   const int64_t tiles = static_cast<int64_t>(num_layers) * p.num_blocks * p.hkv, hq = static_cast<int64_t>(p.hkv) * p.group;
   const int64_t qdims[3] = {D, hq, p.batch}, qstr[2] = {p.qsh * 2, p.qsb * 2}, kdims[3] = {D, p.block_size, tiles},
                 kstr[2] = {D * 2, static_cast<int64_t>(p.block_size) * D * 2};
-  const int qbox[3] = {kHalf, p.group, p.tq}, kbox[3] = {kHalf, std::min(p.block_size, kBN), 1};
+  const int qbox[3] = {kHalf, p.group, p.tq}, kbox[3] = {kHalf, std::min(p.block_size, kBN), 1}, obox[3] = {kHalf, 16, 1};
   if (!encode_box_map(&tq, p.q, qdims, qstr, qbox, dt) || !encode_box_map(&tk, p.k_cache, kdims, kstr, kbox, dt) ||
-      !encode_box_map(&tv, p.v_cache, kdims, kstr, kbox, dt))
+      !encode_box_map(&tv, p.v_cache, kdims, kstr, kbox, dt) || !encode_box_map(&tko, p.k_cache, kdims, kstr, obox, dt) ||
+      !encode_box_map(&tvo, p.v_cache, kdims, kstr, obox, dt))
     return PSB_ERR_CUDA;
   // (a tile of two heads of D 128 takes too many registers)
   const bool hi = !two && p.group > 8;
@@ -1270,15 +1304,14 @@ int launch(SharedParams p, int num_layers, cudaStream_t s) {
     if (fa.numRegs != 128) return PSB_ERR_UNSUPPORTED;
     checked[two ? 2 : hi].store(true, std::memory_order_relaxed);
   }
-  const size_t smem = 1024 + TcGeom<D>::kOffRing + (two ? OwnGeom<D, D == 64 ? 2 : 1>::kBytes : OwnGeom<D, 1>::kBytes) +
-                      sizeof(int32_t) * Plan::ints(p.batch, p.groups);
+  const size_t smem = main_smem(p.batch, p.groups, p.group, p.hkv, D);
   int occ = 0;
   if (!kernel_occupancy(f, kThreads, smem, &occ)) return PSB_ERR_CUDA;
   if (occ < 1) return PSB_ERR_UNSUPPORTED;
   discard_stale_error();
-  cudaError_t e = launch_pdl(kern, dim3(std::min(kMaxCtas, sms)), dim3(kThreads), smem, s, p, tq, tk, tv);
+  cudaError_t e = launch_pdl(kern, dim3(std::min(kMaxCtas, sms)), dim3(kThreads), smem, s, p, tq, tk, tv, tko, tvo);
   if (e != cudaSuccess) return record_cuda_error(e);
-  e = launch_pdl(shared_join_kernel<T, D>, dim3((p.batch * p.group + 31) / 32, D / 4 / (kJoinThreads / 32), p.hkv), dim3(kJoinThreads), 0, s, p, two ? 2 : 1);
+  e = launch_pdl(shared_join_kernel<T, D>, dim3((p.batch * p.group + 31) / 32, D / 4, p.hkv), dim3(kJoinThreads), 0, s, p, two ? 2 : 1);
   if (e != cudaSuccess) return record_cuda_error(e);
   return check_launch();
 }

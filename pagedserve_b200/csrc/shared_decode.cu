@@ -447,6 +447,12 @@ struct Steps {
   }
 };
 
+// An 8 by 8 tile of 16-bit values, row i / 4 and columns 2 (i % 4), + 1 in lane i, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -455,17 +461,17 @@ __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec
 // ---------------------------------------------------------------------------
 // each sequence's own part
 // ---------------------------------------------------------------------------
-// As the plain decode: a warp streams its slices (16 tokens of HP kv heads)
-// through a ring of its own.  HP = 2 (up to 8 q heads per kv head): rows 0-7 of the
-// m16n8k16 tile are one kv head's q heads, rows 8-15 the next one's.  HP = 1: up to 16
-// q heads of one kv head; HI: there are more than 8 (else the upper rows' registers are
-// not kept).  The copies are boxes of 16 tokens and 64 dims, one instruction each: with
-// 16 bytes a lane and instruction, half of a warp's time and more went into issuing them.
-template <typename T, int D, int HP, bool HI>
+// A warp streams its slices (16 tokens of HP kv heads) through a ring of its own, by
+// boxes of 16 tokens, 64 dims and the HP heads (with 16 bytes a lane and instruction,
+// half of a warp's time and more went into issuing the copies).  Its products are
+//   S^T = K Q^T   of 16 tokens by 8 q heads,   O^T += V^T P^T   of 16 dims by 8 q heads,
+// (m16n8k16; P^T by an 8 by 8 transposition in registers): q heads as columns, because
+// their tile is the narrower side, and a kv head has as few as 4 of them.  NT: such
+// tiles of a kv head (1 or 2).
+template <typename T, int D, int HP, int NT>
 __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& plan, const CUtensorMap* tm_k, const CUtensorMap* tm_v, uint8_t* ring_all, uint64_t* bars_all) {
   using Geo = OwnGeom<D, HP>;
-  constexpr int kRing = Geo::kRing, kH = D / kHalf, kSteps = D / 16, kCols = D / 8;  // k steps; 16-byte columns of a row
-  constexpr bool kHi = HP == 2 || HI;
+  constexpr int kRing = Geo::kRing, kH = D / kHalf, kSteps = D / 16;  // steps of 16 dims
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - kFirstOwn;
   const int gq = lane >> 2, t = lane & 3;
   const int G = p.group, B = p.batch, hgs = p.hkv / HP;
@@ -483,7 +489,6 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
   }
   const uint64_t policy = l2_policy_evict_first();
   const int64_t layer0 = static_cast<int64_t>(p.layer) * p.num_blocks;
-  const bool row_lo = gq < G, row_hi = kHi && (HP == 2 ? gq < G : gq + 8 < G);
 
   // A chunk: up to 32 consecutive slices of the warp's range, one a lane: its
   // place in the pool (-1: its block is outside), the valid tokens [lo, hi), and
@@ -540,9 +545,9 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
     if (blk >= 0) {
       const int32_t tile = static_cast<int32_t>((layer0 + blk) * p.hkv + pair / B * HP);
 #pragma unroll
-      for (int x = 0; x < HP * kH; ++x) {
-        box_load_once(on, dst + x * Geo::kBox, tm_k, x % kH * kHalf, r0, tile + x / kH, bar, policy);
-        box_load_once(on, dst + Geo::kKV + x * Geo::kBox, tm_v, x % kH * kHalf, r0, tile + x / kH, bar, policy);
+      for (int h = 0; h < kH; ++h) {
+        box_load_once(on, dst + h * Geo::kBox, tm_k, h * kHalf, r0, tile, bar, policy);
+        box_load_once(on, dst + Geo::kKV + h * Geo::kBox, tm_v, h * kHalf, r0, tile, bar, policy);
       }
     }
     if (lane == static_cast<int>(slot)) {
@@ -585,9 +590,9 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
     p.seq_info[b] = at;
   }
 
-  uint32_t qa[kSteps][4];
-  float o[kCols][4];
-  float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
+  uint32_t q[HP][NT][kSteps][2];  // columns: q heads gq (+ 8)
+  float o[HP][NT][kSteps][4];     // dims gq, gq + 8 of 16, of q heads 2 t, 2 t + 1 (+ 8)
+  float m[HP][NT][2], l[HP][NT][2];  // of these heads: the maximum, this lane's share of the sum
   int32_t pair = 0;
   while (consumed != issued) {
     const uint32_t slot = consumed % kRing;
@@ -597,20 +602,23 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
     if ((mt >> 10) & 1) {  // a pair (or the range) begins: its q rows
       pair = __shfl_sync(0xffffffffu, meta_pair, slot);
       const int hg = pair / B, b = pair - hg * B;
-      const T* qb = reinterpret_cast<const T*>(p.q) + b * p.qsb + 2 * t;
-      const T* qlo = qb + static_cast<int64_t>(hg * HP * G + gq) * p.qsh;
-      const T* qhi = qb + static_cast<int64_t>(HP == 2 ? (hg * 2 + 1) * G + gq : hg * G + gq + 8) * p.qsh;
+      const T* const qb = reinterpret_cast<const T*>(p.q) + b * p.qsb + 2 * t;
 #pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) {
-        qa[ks][0] = row_lo ? __ldcg(reinterpret_cast<const uint32_t*>(qlo + 16 * ks)) : 0u;
-        qa[ks][1] = row_hi ? __ldcg(reinterpret_cast<const uint32_t*>(qhi + 16 * ks)) : 0u;
-        qa[ks][2] = row_lo ? __ldcg(reinterpret_cast<const uint32_t*>(qlo + 16 * ks + 8)) : 0u;
-        qa[ks][3] = row_hi ? __ldcg(reinterpret_cast<const uint32_t*>(qhi + 16 * ks + 8)) : 0u;
+      for (int hs = 0; hs < HP; ++hs) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int h = nt * 8 + gq;
+          const T* const row = qb + static_cast<int64_t>((hg * HP + hs) * G + h) * p.qsh;
+#pragma unroll
+          for (int ks = 0; ks < kSteps; ++ks) {
+            q[hs][nt][ks][0] = h < G ? __ldcg(reinterpret_cast<const uint32_t*>(row + 16 * ks)) : 0u;
+            q[hs][nt][ks][1] = h < G ? __ldcg(reinterpret_cast<const uint32_t*>(row + 16 * ks + 8)) : 0u;
+            o[hs][nt][ks][0] = o[hs][nt][ks][1] = o[hs][nt][ks][2] = o[hs][nt][ks][3] = 0.f;
+          }
+          m[hs][nt][0] = m[hs][nt][1] = -INFINITY;
+          l[hs][nt][0] = l[hs][nt][1] = 0.f;
+        }
       }
-      m_lo = m_hi = -INFINITY;
-      l_lo = l_hi = 0.f;
-#pragma unroll
-      for (int n = 0; n < kCols; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     }
     if (!warp_wait_at(bars + slot * 8, (consumed / kRing) & 1)) {
       if (on) flag_error(p.err, PSB_DEVERR_TIMEOUT);
@@ -618,111 +626,96 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
       return;
     }
     if ((mt >> 12) & 1) {
-      float s[2][4];
+      float s[HP][NT][4];  // tokens gq, gq + 8 of q heads 2 t, 2 t + 1 (+ 8)
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        float acc[HP][4];
+      for (int hs = 0; hs < HP; ++hs) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[hs][nt][0] = s[hs][nt][1] = s[hs][nt][2] = s[hs][nt][3] = 0.f;
+      }
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) {
 #pragma unroll
         for (int hs = 0; hs < HP; ++hs) {
-          acc[hs][0] = acc[hs][1] = acc[hs][2] = acc[hs][3] = 0.f;  // (of its rows, half are the other head's: not used)
-          const uint32_t krow = base + hs * Geo::kTile + (nt * 8 + (lane & 7)) * 128;
+          uint32_t a0, a1, a2, a3;
+          ldsm_x4(base + ((ks >> 2) * HP + hs) * Geo::kBox + (((lane >> 3) & 1) * 8 + (lane & 7)) * 128 +
+                      ((((ks & 3) * 2 + (lane >> 4)) ^ (lane & 7)) << 4), a0, a1, a2, a3);
 #pragma unroll
-          for (int kp = 0; kp < kSteps / 2; ++kp) {  // two k steps a load
-            uint32_t b0, b1, b2, b3;
-            ldsm_x4(krow + (kp >> 1) * Geo::kBox + ((((kp & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4), b0, b1, b2, b3);
-            mma_16816<T>(acc[hs], qa[2 * kp][0], qa[2 * kp][1], qa[2 * kp][2], qa[2 * kp][3], b0, b1);
-            mma_16816<T>(acc[hs], qa[2 * kp + 1][0], qa[2 * kp + 1][1], qa[2 * kp + 1][2], qa[2 * kp + 1][3], b2, b3);
-          }
+          for (int nt = 0; nt < NT; ++nt) mma_16816<T>(s[hs][nt], a0, a1, a2, a3, q[hs][nt][ks][0], q[hs][nt][ks][1]);
         }
-        s[nt][0] = acc[0][0];
-        s[nt][1] = acc[0][1];
-        s[nt][2] = acc[HP - 1][2];
-        s[nt][3] = acc[HP - 1][3];
       }
-      uint32_t keep[2] = {0xffffffffu, 0xffffffffu};  // of V's rows: what is masked may hold anything (even NaN)
+      uint32_t keep[2] = {0xffffffffu, 0xffffffffu};  // of V's rows 2 t, + 1 and 8 + 2 t, + 1: what is masked may hold anything (even NaN)
       if (hi < 16 || lo > 0) {
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          keep[nt] = 0;
+        for (int e = 0; e < 2; ++e) {
+          const int k = 8 * e + 2 * t;
+          keep[e] = (k >= lo && k < hi ? 0x0000ffffu : 0u) | (k + 1 >= lo && k + 1 < hi ? 0xffff0000u : 0u);
+          const int row = 8 * e + gq;
+          if (row < lo || row >= hi) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int tok = nt * 8 + 2 * t + e;
-            if (tok >= lo && tok < hi) {
-              keep[nt] |= e == 0 ? 0x0000ffffu : 0xffff0000u;
-            } else {
-              s[nt][e] = -INFINITY;
-              s[nt][2 + e] = -INFINITY;
+            for (int hs = 0; hs < HP; ++hs) {
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) s[hs][nt][2 * e] = s[hs][nt][2 * e + 1] = -INFINITY;
             }
           }
         }
       }
-      float mb_lo = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-      float mb_hi = kHi ? fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])) : 0.f;
-      mb_lo = fmaxf(mb_lo, __shfl_xor_sync(0xffffffffu, mb_lo, 1));
-      if (kHi) mb_hi = fmaxf(mb_hi, __shfl_xor_sync(0xffffffffu, mb_hi, 1));
-      mb_lo = fmaxf(mb_lo, __shfl_xor_sync(0xffffffffu, mb_lo, 2));
-      if (kHi) mb_hi = fmaxf(mb_hi, __shfl_xor_sync(0xffffffffu, mb_hi, 2));
-      // every slice holds a valid token: the new maxima are finite (or the scores are not numbers)
-      const float mn_lo = fmaxf(m_lo, mb_lo), mn_hi = fmaxf(m_hi, mb_hi);
-      const float al_lo = ex2_approx((m_lo - mn_lo) * p.scale_log2), al_hi = ex2_approx((m_hi - mn_hi) * p.scale_log2);
-      m_lo = mn_lo;
-      m_hi = mn_hi;
-      const float ms_lo = mn_lo * p.scale_log2, ms_hi = mn_hi * p.scale_log2;
-      float pr[2][4];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        pr[nt][0] = ex2_approx(fmaf(s[nt][0], p.scale_log2, -ms_lo));
-        pr[nt][1] = ex2_approx(fmaf(s[nt][1], p.scale_log2, -ms_lo));
-        pr[nt][2] = kHi ? ex2_approx(fmaf(s[nt][2], p.scale_log2, -ms_hi)) : 0.f;
-        pr[nt][3] = kHi ? ex2_approx(fmaf(s[nt][3], p.scale_log2, -ms_hi)) : 0.f;
-      }
-      l_lo = l_lo * al_lo + ((pr[0][0] + pr[0][1]) + (pr[1][0] + pr[1][1]));
-      l_hi = l_hi * al_hi + ((pr[0][2] + pr[0][3]) + (pr[1][2] + pr[1][3]));
-#pragma unroll
-      for (int n = 0; n < kCols; ++n) {
-        o[n][0] *= al_lo;
-        o[n][1] *= al_lo;
-        if (kHi) {
-          o[n][2] *= al_hi;
-          o[n][3] *= al_hi;
-        }
-      }
-      const uint32_t pa0 = pack2<T>(pr[0][0], pr[0][1]), pa1 = pack2<T>(pr[0][2], pr[0][3]);
-      const uint32_t pa2 = pack2<T>(pr[1][0], pr[1][1]), pa3 = pack2<T>(pr[1][2], pr[1][3]);
-      const int vr = ((lane >> 3) & 1) * 8 + (lane & 7);
+      float mx[HP][NT][2];
 #pragma unroll
       for (int hs = 0; hs < HP; ++hs) {
-        const uint32_t vrow = base + Geo::kKV + hs * Geo::kTile + vr * 128;
 #pragma unroll
-        for (int dp = 0; dp < kCols / 2; ++dp) {
-          uint32_t b0, b1, b2, b3;
-          ldsm_x4_t(vrow + (dp >> 2) * Geo::kBox + ((((dp & 3) * 2 + (lane >> 4)) ^ (vr & 7)) << 4), b0, b1, b2, b3);
-          b0 &= keep[0];
-          b1 &= keep[1];
-          b2 &= keep[0];
-          b3 &= keep[1];
-          if constexpr (!kHi) {
-            float x[4] = {o[2 * dp][0], o[2 * dp][1], 0.f, 0.f}, y[4] = {o[2 * dp + 1][0], o[2 * dp + 1][1], 0.f, 0.f};
-            mma_16816<T>(x, pa0, 0u, pa2, 0u, b0, b1);
-            mma_16816<T>(y, pa0, 0u, pa2, 0u, b2, b3);
-            o[2 * dp][0] = x[0];
-            o[2 * dp][1] = x[1];
-            o[2 * dp + 1][0] = y[0];
-            o[2 * dp + 1][1] = y[1];
-          } else if constexpr (HP == 1) {
-            mma_16816<T>(o[2 * dp], pa0, pa1, pa2, pa3, b0, b1);
-            mma_16816<T>(o[2 * dp + 1], pa0, pa1, pa2, pa3, b2, b3);
-          } else {
-            // the rows that are this head's, added in registers: zeros in the
-            // other head's probabilities would still make NaN of an infinite value
-            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_16816<T>(x, pa0, pa1, pa2, pa3, b0, b1);
-            mma_16816<T>(y, pa0, pa1, pa2, pa3, b2, b3);
-            o[2 * dp][2 * hs] += x[2 * hs];
-            o[2 * dp][2 * hs + 1] += x[2 * hs + 1];
-            o[2 * dp + 1][2 * hs] += y[2 * hs];
-            o[2 * dp + 1][2 * hs + 1] += y[2 * hs + 1];
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) mx[hs][nt][e] = fmaxf(s[hs][nt][e], s[hs][nt][2 + e]);
+        }
+      }
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+#pragma unroll
+        for (int hs = 0; hs < HP; ++hs) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) mx[hs][nt][e] = fmaxf(mx[hs][nt][e], __shfl_xor_sync(0xffffffffu, mx[hs][nt][e], x));
           }
+        }
+      }
+      uint32_t pr[HP][NT][2];  // P^T: tokens 2 t, + 1 (+ 8) of q head gq
+#pragma unroll
+      for (int hs = 0; hs < HP; ++hs) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float ex[4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            // every slice holds a valid token: the new maximum is finite (or the scores are not numbers)
+            const float mn = fmaxf(m[hs][nt][e], mx[hs][nt][e]), alpha = ex2_approx((m[hs][nt][e] - mn) * p.scale_log2), ms = mn * p.scale_log2;
+            m[hs][nt][e] = mn;
+            ex[e] = ex2_approx(fmaf(s[hs][nt][e], p.scale_log2, -ms));
+            ex[2 + e] = ex2_approx(fmaf(s[hs][nt][2 + e], p.scale_log2, -ms));
+            l[hs][nt][e] = fmaf(l[hs][nt][e], alpha, ex[e] + ex[2 + e]);
+#pragma unroll
+            for (int ks = 0; ks < kSteps; ++ks) {
+              o[hs][nt][ks][e] *= alpha;
+              o[hs][nt][ks][2 + e] *= alpha;
+            }
+          }
+          pr[hs][nt][0] = transposed(pack2<T>(ex[0], ex[1]));
+          pr[hs][nt][1] = transposed(pack2<T>(ex[2], ex[3]));
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) {
+#pragma unroll
+        for (int hs = 0; hs < HP; ++hs) {
+          uint32_t a0, a1, a2, a3;
+          ldsm_x4_t(base + Geo::kKV + ((ks >> 2) * HP + hs) * Geo::kBox + ((lane >> 4) * 8 + (lane & 7)) * 128 +
+                        ((((ks & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4), a0, a1, a2, a3);
+          a0 &= keep[0];
+          a1 &= keep[0];
+          a2 &= keep[1];
+          a3 &= keep[1];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_16816<T>(o[hs][nt][ks], a0, a1, a2, a3, pr[hs][nt][0], pr[hs][nt][1]);
         }
       }
     }
@@ -730,27 +723,33 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
     ++consumed;
     if (c_ok) issue_one();  // refill the slot just read
     if ((mt >> 11) & 1) {   // the pair's or the range's end: its partial
-      float ll = l_lo, lh = l_hi;
-      ll += __shfl_xor_sync(0xffffffffu, ll, 1);
-      lh += __shfl_xor_sync(0xffffffffu, lh, 1);
-      ll += __shfl_xor_sync(0xffffffffu, ll, 2);
-      lh += __shfl_xor_sync(0xffffffffu, lh, 2);
       float* const part = p.own_part + static_cast<int64_t>(gw + pair) * own_floats(D);
       float2* const ml = reinterpret_cast<float2*>(part + 16 * D);
-      // dims 8 n + 2 t, + 1 of rows gq and gq + 8: halves of column group 2 n + t / 2
 #pragma unroll
-      for (int n = 0; n < kCols; ++n) {
-        float* const at = part + (2 * n + (t >> 1)) * 64 + 2 * (t & 1);
-        if (row_lo) *reinterpret_cast<float2*>(at + 4 * gq) = make_float2(o[n][0], o[n][1]);
-        if (row_hi) *reinterpret_cast<float2*>(at + 4 * (gq + 8)) = make_float2(o[n][2], o[n][3]);
+      for (int hs = 0; hs < HP; ++hs) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float sum = l[hs][nt][e];
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            const int h = nt * 8 + 2 * t + e, row = hs * 8 + h;
+            if (h >= G) continue;
+#pragma unroll
+            for (int ks = 0; ks < kSteps; ++ks) {
+#pragma unroll
+              for (int u = 0; u < 2; ++u) part[(4 * ks + 2 * u + (gq >> 2)) * 64 + 4 * row + (gq & 3)] = o[hs][nt][ks][2 * u + e];
+            }
+            if (gq == 0) ml[row] = make_float2(m[hs][nt][e] * p.scale_log2, sum);
+          }
+        }
       }
-      if (t == 0 && row_lo) ml[gq] = make_float2(m_lo * p.scale_log2, ll);
-      if (t == 0 && row_hi) ml[gq + 8] = make_float2(m_hi * p.scale_log2, lh);
     }
   }
 }
 
-template <typename T, int D, int HP, bool HI>
+template <typename T, int D, int HP, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
     shared_main_kernel(const SharedParams p, const __grid_constant__ CUtensorMap tm_q,
                        const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -997,7 +996,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
   if (warp >= kFirstOwn) {
-    own_parts<T, D, HP, HI>(p, plan, &tm_ko, &tm_vo, smem + Geo::kOffRing, bar_own);
+    own_parts<T, D, HP, NT>(p, plan, &tm_ko, &tm_vo, smem + Geo::kOffRing, bar_own);
   } else if (warp >= 8) {
     fewer_registers<kOtherRegs>();
     if (warp == 8) products(Stream<0>());
@@ -1287,14 +1286,14 @@ int launch(SharedParams p, int num_layers, cudaStream_t s) {
   const int64_t tiles = static_cast<int64_t>(num_layers) * p.num_blocks * p.hkv, hq = static_cast<int64_t>(p.hkv) * p.group;
   const int64_t qdims[3] = {D, hq, p.batch}, qstr[2] = {p.qsh * 2, p.qsb * 2}, kdims[3] = {D, p.block_size, tiles},
                 kstr[2] = {D * 2, static_cast<int64_t>(p.block_size) * D * 2};
-  const int qbox[3] = {kHalf, p.group, p.tq}, kbox[3] = {kHalf, std::min(p.block_size, kBN), 1}, obox[3] = {kHalf, 16, 1};
+  const int qbox[3] = {kHalf, p.group, p.tq}, kbox[3] = {kHalf, std::min(p.block_size, kBN), 1}, obox[3] = {kHalf, 16, two ? 2 : 1};
   if (!encode_box_map(&tq, p.q, qdims, qstr, qbox, dt) || !encode_box_map(&tk, p.k_cache, kdims, kstr, kbox, dt) ||
       !encode_box_map(&tv, p.v_cache, kdims, kstr, kbox, dt) || !encode_box_map(&tko, p.k_cache, kdims, kstr, obox, dt) ||
       !encode_box_map(&tvo, p.v_cache, kdims, kstr, obox, dt))
     return PSB_ERR_CUDA;
   // (a tile of two heads of D 128 takes too many registers)
   const bool hi = !two && p.group > 8;
-  const auto kern = two ? shared_main_kernel<T, D, D == 64 ? 2 : 1, false> : hi ? shared_main_kernel<T, D, 1, true> : shared_main_kernel<T, D, 1, false>;
+  const auto kern = two ? shared_main_kernel<T, D, D == 64 ? 2 : 1, 1> : hi ? shared_main_kernel<T, D, 1, 2> : shared_main_kernel<T, D, 1, 1>;
   const void* const f = reinterpret_cast<const void*>(kern);
   static std::atomic<bool> checked[3];  // (of each instantiation) the shares draw on the launch's registers
   if (!checked[two ? 2 : hi].load(std::memory_order_relaxed)) {

@@ -1,5 +1,5 @@
-// The host side of the 4-bit pool's and the block tables' calls for the common
-// case, as one Python call each: the arguments' checks, the outputs and the
+// The host side of the 4-bit pool's, the block tables' and the shared prefixes'
+// calls for the common case, as one Python call each: the arguments' checks, the outputs and the
 // scratch, then the C entry.
 //
 // A step's smallest calls are bound by the host: of a single sequence's decode
@@ -422,9 +422,188 @@ PyObject* trim(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Holder counts: int32 [2, blocks of the ring].
+bool shares_like(const Tensor* t, const Tables& of) {
+  return t && t->dim() == 2 && t->scalar_type() == at::kInt && t->size(0) == 2 && t->size(1) == of.free->size(0) && t->is_contiguous();
+}
+
+// fork(table_store, parent_rows, child_rows, lens, free_blocks, free_state, shares, block_size, error_flag)
+// -> (src, dst), new
+PyObject* fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9) return none();
+  const int dev = c10::cuda::current_device();
+  Tables t;
+  int64_t block;
+  if (!read_tables(a, a[8], dev, &t) || !as_int(a[7], &block) || block <= 0) return none();
+  const Tensor* shares = cuda_tensor(a[6], dev);
+  if (!shares_like(shares, t)) return none();
+  Tensor src, dst;
+  int status;
+  {
+    const Unlocked unlocked;
+    src = new_tensor({t.batch}, at::kInt, dev);
+    dst = new_tensor({t.batch}, at::kInt, dev);
+    status = psb_fork_tables(ints(*t.store), t.store->stride(0), t.store->size(0), t.store->size(1), ints(*t.rows),
+                             ints(*t.first), ints(*t.second), t.batch, ints(*shares), ints(*t.free), t.free->size(0),
+                             ints(*t.state), block, ints(src), ints(dst), flag_ptr(t.flag), stream_of(dev));
+  }
+  if (status != PSB_OK) return PyLong_FromLong(status);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(src), THPVariable_Wrap(dst));
+  END_HANDLE_TH_ERRORS
+}
+
+// release(table_store, req_rows, held_lens, keep_lens, free_blocks, free_state, shares, block_size, error_flag) -> True
+PyObject* release(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9) return none();
+  const int dev = c10::cuda::current_device();
+  Tables t;
+  int64_t block;
+  if (!read_tables(a, a[8], dev, &t) || !as_int(a[7], &block) || block <= 0) return none();
+  const Tensor* shares = cuda_tensor(a[6], dev);
+  if (!shares_like(shares, t)) return none();
+  int status;
+  {
+    const Unlocked unlocked;
+    status = psb_release_tables(ints(*t.store), t.store->stride(0), t.store->size(0), t.store->size(1), ints(*t.rows),
+                                ints(*t.first), ints(*t.second), t.batch, ints(*shares), ints(*t.free), t.free->size(0),
+                                ints(*t.state), block, flag_ptr(t.flag), stream_of(dev));
+  }
+  return true_or(status);
+  END_HANDLE_TH_ERRORS
+}
+
+// copy(pools, src, dst, error_flag) -> True; pools: a tuple
+PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !PyTuple_CheckExact(a[0])) return none();
+  const int dev = c10::cuda::current_device();
+  const Py_ssize_t count = PyTuple_GET_SIZE(a[0]);
+  const Tensor *src = cuda_tensor(a[1], dev), *dst = cuda_tensor(a[2], dev), *flag;
+  if (count < 1 || count > 4 || !i32_vector(src, -1) || !i32_vector(dst, src->size(0)) || !optional_tensor(a[3], dev, &flag) ||
+      !flag_like(flag))
+    return none();
+  void* pools[4];
+  int64_t bytes[4], layers = 0, blocks = 0;
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    const Tensor* const t = cuda_tensor(PyTuple_GET_ITEM(a[0], i), dev);
+    if (!t || t->dim() < 3 || t->numel() == 0 || !t->is_contiguous() || t->size(0) > kI32 || t->size(1) > kI32) return none();
+    if (i > 0 && (t->size(0) != layers || t->size(1) != blocks)) return none();
+    layers = t->size(0);
+    blocks = t->size(1);
+    pools[i] = t->data_ptr();
+    bytes[i] = static_cast<int64_t>(t->nbytes()) / (layers * blocks);
+  }
+  int status;
+  {
+    const Unlocked unlocked;
+    status = psb_copy_blocks(pools, bytes, static_cast<int32_t>(count), ints(*src), ints(*dst), src->size(0), layers, blocks,
+                             flag_ptr(flag), stream_of(dev));
+  }
+  return true_or(status);
+  END_HANDLE_TH_ERRORS
+}
+
+// decode_shared(query, k_cache, v_cache, block_tables, context_lens, cu_groups, prefix_lens, layer, scale, out, max_context,
+//               workspace, error_flag) -> out
+PyObject* decode_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 13) return none();
+  const int dev = c10::cuda::current_device();
+  const Tensor *q = cuda_tensor(a[0], dev), *k = cuda_tensor(a[1], dev), *v = cuda_tensor(a[2], dev);
+  const Tensor *tables = cuda_tensor(a[3], dev), *ctx = cuda_tensor(a[4], dev), *cu = cuda_tensor(a[5], dev), *pre = cuda_tensor(a[6], dev);
+  const Tensor *out, *ws, *flag;
+  int64_t layer, most;
+  if (!q || !k || !v || !tables || k->dim() != 5 || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() ||
+      !k->is_contiguous() || !v->is_contiguous() || k->numel() == 0 || !as_int(a[7], &layer) || layer < 0 || layer >= k->size(0))
+    return none();
+  const int64_t layers = k->size(0), blocks = k->size(1), hkv = k->size(2), block = k->size(3), dim = k->size(4);
+  const ScalarType type = k->scalar_type();
+  auto rows = [&](const Tensor& t) {
+    const int64_t d = t.dim();
+    return (d == 3 || (d == 4 && t.size(2) == 1)) && t.size(d - 1) == dim && t.stride(d - 1) == 1 && t.scalar_type() == type;
+  };
+  if ((type != at::kHalf && type != at::kBFloat16) || block > kI32 || layers * hkv > kI32 / blocks || !rows(*q)) return none();
+  const int64_t batch = q->size(0), heads = q->size(1);
+  if (batch <= 0 || batch > kI32 || heads <= 0 || heads > kI32 || heads % hkv || q->stride(0) <= 0 || q->stride(1) <= 0 ||
+      q->stride(0) % 8 || q->stride(1) % 8 || !aligned16(q->data_ptr()) || !aligned16(k->data_ptr()) || !aligned16(v->data_ptr()))
+    return none();
+  if (tables->dim() != 2 || tables->scalar_type() != at::kInt || tables->size(0) != batch || tables->stride(1) != 1 || tables->stride(0) < 0 ||
+      !i32_vector(ctx, batch) || !i32_vector(pre, -1) || !i32_vector(cu, pre->size(0) + 1) || tables->size(1) > kI32 / block)
+    return none();
+  const int64_t width = tables->size(1) * block;
+  double scale;
+  if (a[8] == Py_None) scale = 1.0 / std::sqrt(static_cast<double>(dim));
+  else if (PyFloat_CheckExact(a[8])) scale = PyFloat_AS_DOUBLE(a[8]);
+  else return none();
+  if (!(scale > 0.0) || !std::isfinite(scale)) return none();
+  if (a[10] == Py_None) most = width;
+  else if (!as_int(a[10], &most) || most < 0 || most > width) return none();
+  if (!optional_tensor(a[9], dev, &out) || !optional_tensor(a[11], dev, &ws) || !optional_tensor(a[12], dev, &flag) || !flag_like(flag) ||
+      (ws && (!ws->is_contiguous() || !aligned16(ws->data_ptr()))))
+    return none();
+  if (out ? !rows(*out) || out->size(0) != batch || out->size(1) != heads : !plain_order(*q)) return none();
+  const size_t need = psb_paged_decode_shared_workspace_size(batch, pre->size(0), heads, hkv, dim, block, most, dtype_code(type));
+  if (need == 0) return none();
+  Tensor o;
+  int status;
+  {
+    const Unlocked unlocked;
+    o = out ? *out : new_tensor(q->sizes(), type, dev);
+    const Tensor w = ws ? *ws : new_tensor({static_cast<int64_t>(need)}, at::kByte, dev);
+    status = psb_paged_decode_shared(q->data_ptr(), q->stride(0), q->stride(1), o.data_ptr(), o.stride(0), o.stride(1), k->data_ptr(),
+                                     v->data_ptr(), ints(*tables), tables->stride(0), ints(*ctx), ints(*cu), ints(*pre), batch,
+                                     pre->size(0), heads, layer, layers, blocks, hkv, block, dim, dtype_code(type), most,
+                                     static_cast<float>(scale), w.data_ptr(), w.nbytes(), flag_ptr(flag), stream_of(dev));
+  }
+  return out_or(status, a[9], o);
+  END_HANDLE_TH_ERRORS
+}
+
+// verify(logits, tokens, cu_seqlens, uniforms, temperature, draft_probs, error_flag) -> (new_tokens, counts), new
+PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) return none();
+  const int dev = c10::cuda::current_device();
+  const Tensor *x = cuda_tensor(a[0], dev), *tokens = cuda_tensor(a[1], dev), *cu = cuda_tensor(a[2], dev);
+  const Tensor *u = cuda_tensor(a[3], dev), *heat = cuda_tensor(a[4], dev), *probs, *flag;
+  if (!x || !u || !optional_tensor(a[5], dev, &probs) || !optional_tensor(a[6], dev, &flag) || !flag_like(flag) || x->dim() != 2)
+    return none();
+  const int64_t rows = x->size(0), vocab = x->size(1);
+  auto matrix = [&](const Tensor& t) {
+    return t.dim() == 2 && t.size(0) == rows && t.size(1) == vocab && t.stride(1) == 1 && t.stride(0) >= vocab && dtype_code(t.scalar_type()) >= 0;
+  };
+  if (rows <= 0 || rows > kI32 || vocab <= 0 || vocab > kI32 || !matrix(*x) || (probs && !matrix(*probs)) || !slots_like(tokens, rows) ||
+      !i32_vector(cu, -1) || cu->size(0) < 2)
+    return none();
+  const int64_t batch = cu->size(0) - 1;
+  if (u->scalar_type() != at::kFloat || u->dim() != 2 || u->size(0) != rows || u->size(1) != 2 || !u->is_contiguous() || !heat ||
+      heat->scalar_type() != at::kFloat || heat->dim() != 1 || heat->size(0) != batch || !heat->is_contiguous())
+    return none();
+  Tensor fresh, counts;
+  int status;
+  {
+    const Unlocked unlocked;
+    fresh = new_tensor({rows}, at::kLong, dev);
+    counts = new_tensor({batch}, at::kInt, dev);
+    const Tensor ws = new_tensor({static_cast<int64_t>(psb_verify_tokens_workspace_size(batch))}, at::kByte, dev);
+    status = psb_verify_tokens(x->data_ptr(), x->stride(0), rows, vocab, dtype_code(x->scalar_type()),
+                               static_cast<const int64_t*>(tokens->data_ptr()), ints(*cu), batch, static_cast<const float*>(u->data_ptr()),
+                               static_cast<const float*>(heat->data_ptr()), probs ? probs->data_ptr() : nullptr,
+                               probs ? probs->stride(0) : 0, probs ? dtype_code(probs->scalar_type()) : 0,
+                               static_cast<int64_t*>(fresh.data_ptr()), ints(counts), ws.data_ptr(), ws.nbytes(), flag_ptr(flag),
+                               stream_of(dev));
+  }
+  if (status != PSB_OK) return PyLong_FromLong(status);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(fresh), THPVariable_Wrap(counts));
+  END_HANDLE_TH_ERRORS
+}
+
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(write), ENTRY(rope_write), ENTRY(gather), ENTRY(decode), ENTRY(prefill),
-                         ENTRY(extend), ENTRY(trim), {nullptr, nullptr, 0, nullptr}};
+                         ENTRY(extend), ENTRY(trim), ENTRY(fork), ENTRY(release), ENTRY(copy),
+                         ENTRY(decode_shared), ENTRY(verify), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

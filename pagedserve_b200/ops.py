@@ -1129,6 +1129,11 @@ def fork_tables(table_store: torch.Tensor, parent_rows: torch.Tensor, child_rows
     back with ``release_tables`` (not ``trim_tables``).  Checked and refused as a
     whole, like ``extend_step``.
     """
+    if table_store.is_cuda:
+        done = (_native._calls or _native.calls()).fork(table_store, parent_rows, child_rows, lens, free_blocks, free_state,
+                                                        shares, block_size, error_flag)
+        if done is not None:
+            return _done(done, "fork_tables")
     store, bsz, parents, children, lens = _tables_args(table_store, parent_rows, child_rows, lens, free_blocks, free_state,
                                                        ("parent_rows", "child_rows", "lens"), error_flag)
     _check_shares(shares, free_blocks.shape[0])
@@ -1153,6 +1158,12 @@ def release_tables(table_store: torch.Tensor, req_rows: torch.Tensor, held_lens:
     ``keep_lens[b]`` may end inside a block only if nobody else holds that block
     afterwards: the call is refused otherwise (``error_flag`` 1024).
     """
+    if table_store.is_cuda:
+        done = (_native._calls or _native.calls()).release(table_store, req_rows, held_lens, keep_lens, free_blocks,
+                                                           free_state, shares, block_size, error_flag)
+        if done is not None:
+            _done(done, "release_tables")
+            return
     store, bsz, rows, held_lens, keep_lens = _tables_args(table_store, req_rows, held_lens, keep_lens, free_blocks,
                                                           free_state, ("req_rows", "held_lens", "keep_lens"),
                                                           error_flag)
@@ -1174,6 +1185,11 @@ def copy_blocks(pools, src: torch.Tensor, dst: torch.Tensor, error_flag: torch.T
     Destinations are distinct and none is a source.
     """
     pools = tuple(pools)
+    if src.is_cuda:
+        done = (_native._calls or _native.calls()).copy(pools, src, dst, error_flag)
+        if done is not None:
+            _done(done, "copy_blocks")
+            return
     if not 1 <= len(pools) <= 4:
         raise ValueError("pools must be one to four tensors")
     if src.dtype != torch.int32 or src.ndim != 1 or dst.dtype != torch.int32 or dst.shape != src.shape:
@@ -1216,8 +1232,16 @@ def paged_decode_shared(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
     Prefixes are shared for bf16/f16, head_dim 64 or 128, up to 16 q heads per kv
     head, blocks of 16, 32, 64 or a multiple of 64 tokens, up to 2048 sequences; other
-    geometries are answered by ``paged_decode``, each sequence on its own.  ``scale`` must be positive.
+    geometries, and batches whose
+    plan does not fit shared memory (from some 900 sequences in as many groups on), are answered by ``paged_decode``, each
+    sequence on its own.  ``scale`` must be positive.
     """
+    if query.is_cuda:
+        done = (_native._calls or _native.calls()).decode_shared(query, k_cache, v_cache, block_tables, context_lens, cu_groups,
+                                                                 prefix_lens, layer, scale, out, max_context, workspace,
+                                                                 error_flag)
+        if done is not None:
+            return _done(done, "paged_decode_shared")
     nl, nb, hkv, bs, d = _pool_geometry(k_cache, v_cache)
     q3 = query.squeeze(2) if query.ndim == 4 and query.shape[2] == 1 else query
     if q3.ndim != 3 or q3.shape[2] != d:
@@ -1303,6 +1327,11 @@ def verify_tokens(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     Decided as in 64-bit arithmetic.  A row without probabilities (NaN, +inf, all
     -inf) takes no draft, gives its first maximum and is flagged (2048).
     """
+    if out is None and logits.is_cuda:
+        done = (_native._calls or _native.calls()).verify(logits, tokens, cu_seqlens, uniforms, temperature, draft_probs,
+                                                          error_flag)
+        if done is not None:
+            return _done(done, "verify_tokens")
     if logits.ndim != 2 or logits.shape[1] == 0:
         raise ValueError("logits must be [T, V]")
     t, v = (int(x) for x in logits.shape)

@@ -14,6 +14,10 @@ Public surface:
   ``ops.*_int4``
 * ``ops.extend_step / trim_tables`` - block allocation and release on the
   device, so that a step needs no host bookkeeping
+* ``PagedKVCache.fork`` / ``ops.fork_tables / release_tables / copy_blocks`` -
+  requests that share the blocks of one prompt, on the host's tables or the
+  device's; ``ops.paged_decode_shared`` reads such a prompt once for all of
+  them, ``ops.verify_tokens`` samples and checks drafted tokens
 * ``select_next_tokens`` / ``read_selection`` - the step's greedy argmax and
   stop test on the device, one host sync per batch (replaces the per-row
   ``.item()`` loop of pagedserve/engine/continuous_batcher.py:333-360)

@@ -194,7 +194,12 @@ class PagedModelRunner:
         op = ops.rope_reshape_and_cache_int4 if self.kv_bits == 4 else ops.rope_reshape_and_cache
         return op(q, k, v, cos, sin, self.k_cache, self.v_cache, slots, layer, key_out=key_out)
 
-    def _paged_decode(self, q, block_tables, context_lens, layer: int, max_context: int, out=None):
+    def _paged_decode(self, q, block_tables, context_lens, layer: int, max_context: int, out=None, groups=None):
+        if groups is not None:
+            if self.kv_bits == 4:
+                raise ValueError("groups need a 16-bit pool")
+            return ops.paged_decode_shared(q, self.k_cache, self.v_cache, block_tables, context_lens, *groups, layer,
+                                           scale=self.scale, out=out, max_context=max_context)
         op = ops.paged_decode_int4 if self.kv_bits == 4 else ops.paged_decode
         return op(q, self.k_cache, self.v_cache, block_tables, context_lens, layer, scale=self.scale, out=out,
                   max_context=max_context)
@@ -244,16 +249,20 @@ class PagedModelRunner:
 
     # -- decode ---------------------------------------------------------------
     def decode(self, tokens: torch.Tensor, positions: torch.Tensor, block_tables: torch.Tensor,
-               context_lens: torch.Tensor, slots: torch.Tensor, max_context: int | None = None) -> torch.Tensor:
+               context_lens: torch.Tensor, slots: torch.Tensor, max_context: int | None = None,
+               groups: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
         """One decode token per row: ``tokens, positions, slots [B]`` int64
         (token b sits at ``positions[b]`` and its K/V goes to ``slots[b]``),
         ``block_tables [B, W]`` / ``context_lens [B]`` int32 with
-        ``context_lens[b] == positions[b] + 1``.  Returns logits ``[B, V]``
+        ``context_lens[b] == positions[b] + 1``.  ``groups``: ``(cu_groups,
+        prefix_lens)`` of rows whose sequences begin alike, as
+        ``ops.paged_decode_shared`` takes them (16-bit pools; read once per
+        group, else the same result).  Returns logits ``[B, V]``
         (``_forward_paged_batch``'s ``[B, 1, V]`` without the unit axis)."""
         max_context = block_tables.shape[1] * self.block_size if max_context is None else max_context
 
         def attend(q_rot, _k, _v, layer):
-            return self._paged_decode(q_rot, block_tables, context_lens, layer, max_context)
+            return self._paged_decode(q_rot, block_tables, context_lens, layer, max_context, groups=groups)
         return self._layers(tokens, positions, slots, attend, want_keys=False)
 
     # -- packed prefill ----------------------------------------------------------

@@ -13,9 +13,11 @@ raised follow the reference so callers can switch without edits:
 
 Added for the batched path: ``PagedKVCache.table_rows`` (a padded int32
 table for a list of requests, built in one numpy pass) and
-``PagedKVCache.slot_of`` (the int64 slot a position maps to); and pools that
+``PagedKVCache.slot_of`` (the int64 slot a position maps to); pools that
 hold 4-bit codes (``kv_bits=4``: ``kv_codes`` and ``kv_params`` in place of
-``k_cache`` and ``v_cache``, the layout of ``ops.reshape_and_cache_int4``).
+``k_cache`` and ``v_cache``, the layout of ``ops.reshape_and_cache_int4``); and
+requests that share their first blocks (``fork``; ``shared_prefixes`` tells a
+decode step which).
 """
 
 from __future__ import annotations
@@ -45,6 +47,7 @@ class BlockManager:
             raise ValueError("free_order must be a permutation of range(num_blocks)")
         self._free: deque[int] = deque(order)
         self._owned: dict[str, list[int]] = {}
+        self._shares: dict[int, int] = {}  # holders of a block beyond the first (of shared blocks alone)
 
     @property
     def free_blocks(self) -> int:
@@ -83,11 +86,50 @@ class BlockManager:
         self._owned[request_id].extend(blocks)
         return list(blocks)
 
+    def fork(self, parent_id: str, request_id: str, num_tokens: int) -> tuple[list[int], tuple[int, int] | None]:
+        """Blocks for a request that continues the first ``num_tokens`` tokens of
+        ``parent_id``: the parent's whole blocks, shared, and where those tokens end
+        inside a block one from the free list, returned with the block it has to be a
+        copy of: ``(blocks, (source, copy) or None)``."""
+        if parent_id not in self._owned:
+            raise KeyError(f"Unknown request: {parent_id!r}")
+        if request_id in self._owned:
+            raise ValueError(f"Request {request_id!r} already has blocks")
+        parent = self._owned[parent_id]
+        if self.blocks_needed(num_tokens) > len(parent):
+            raise ValueError(f"Request {parent_id!r} holds fewer than {num_tokens} tokens")
+        whole = num_tokens // self.block_size
+        pair = None
+        blocks = parent[:whole]
+        if num_tokens % self.block_size:
+            pair = (parent[whole], self._take(1)[0])
+            blocks = blocks + [pair[1]]
+        for blk in parent[:whole]:
+            self._shares[blk] = self._shares.get(blk, 0) + 1
+        self._owned[request_id] = blocks
+        return list(blocks), pair
+
+    def holders(self, block: int) -> int:
+        """How many requests hold a block that is not free."""
+        return 1 + self._shares.get(block, 0)
+
     def free(self, request_id: str) -> None:
-        """Return all of a request's blocks to the tail of the free list."""
+        """Return all of a request's blocks to the tail of the free list (of a block
+        that others hold, the last of them does)."""
         if request_id not in self._owned:
             raise KeyError(f"Unknown request: {request_id!r}")
-        self._free.extend(self._owned.pop(request_id))
+        blocks = self._owned.pop(request_id)
+        if not self._shares:
+            self._free.extend(blocks)
+            return
+        for blk in blocks:
+            others = self._shares.get(blk, 0)
+            if others == 0:
+                self._free.append(blk)
+            elif others == 1:
+                del self._shares[blk]
+            else:
+                self._shares[blk] = others - 1
 
     def get_blocks(self, request_id: str) -> list[int]:
         if request_id not in self._owned:
@@ -188,6 +230,23 @@ class KVCache:
     def total_bytes(self) -> int:
         return self.num_blocks * self.block_bytes
 
+    def copy_blocks(self, source: list[int], copy: list[int]) -> None:
+        """Blocks ``copy`` become, in every layer, what blocks ``source`` are (one launch on a CUDA device)."""
+        if len(source) != len(copy):
+            raise ValueError("source and copy differ in length")
+        for blk in (*source, *copy):
+            self._check_block(blk)
+        if not source:
+            return
+        pools = (self.kv_codes, self.kv_params) if self.kv_bits == 4 else (self.k_cache, self.v_cache)
+        if self.device.type == "cuda":
+            pair = torch.tensor([source, copy], dtype=torch.int32).to(pools[0].device)
+            with torch.cuda.device(pools[0].device):
+                ops.copy_blocks(pools, pair[0], pair[1])
+            return
+        for pool in pools:
+            pool[:, copy] = pool[:, source]
+
     def _check_layer(self, layer: int) -> None:
         if not 0 <= layer < self.num_layers:
             raise IndexError(f"Invalid layer: {layer}; valid range is [0, {self.num_layers})")
@@ -265,7 +324,35 @@ class PagedKVCache:
             raise ValueError(f"Request {request_id!r} already exists")
         if num_tokens < 0:
             raise ValueError("num_tokens cannot be negative")
-        blocks = self.block_manager.allocate(request_id=request_id, num_tokens=num_tokens)
+        self._adopt(request_id, num_tokens, self.block_manager.allocate(request_id=request_id, num_tokens=num_tokens))
+
+    def fork(self, parent_id: str, request_ids, num_tokens: int | None = None) -> None:
+        """Requests that continue the first ``num_tokens`` tokens of ``parent_id`` (default: all of them).
+
+        They share the parent's whole blocks; of a block in which those tokens end
+        each gets a copy of its own, in one launch for all of them.  Parent and
+        children are then requests like any other: appended to, read, and freed in
+        any order.  If the free list does not have a block for each copy,
+        RuntimeError and nothing has changed."""
+        self._validate_request(parent_id)
+        request_ids = list(request_ids)
+        num_tokens = self._counts[parent_id] if num_tokens is None else num_tokens
+        if not 0 <= num_tokens <= self._counts[parent_id]:
+            raise ValueError(f"num_tokens must lie in [0, {self._counts[parent_id]}]")
+        for i, request_id in enumerate(request_ids):
+            if request_id in self._tables or request_id in request_ids[:i]:
+                raise ValueError(f"Request {request_id!r} already exists")
+        if num_tokens % self.block_size and len(request_ids) > self.free_blocks:
+            raise RuntimeError(f"Not enough KV blocks: required={len(request_ids)}, free={self.free_blocks}")
+        pairs = []
+        for request_id in request_ids:
+            blocks, pair = self.block_manager.fork(parent_id, request_id, num_tokens)
+            self._adopt(request_id, num_tokens, blocks)
+            if pair is not None:
+                pairs.append(pair)
+        self.kv_cache.copy_blocks([a for a, _ in pairs], [b for _, b in pairs])
+
+    def _adopt(self, request_id: str, num_tokens: int, blocks: list[int]) -> None:
         table = BlockTable()
         table._owner = self
         table._row = self._store_row()
@@ -452,6 +539,28 @@ class PagedKVCache:
         if have < width:
             dst[:, :have] = self._store[rows, :have]
             dst[:, have:] = 0
+
+    def shared_prefixes(self, request_ids) -> tuple[np.ndarray, np.ndarray]:
+        """``(cu_groups [G + 1], prefix_lens [G])`` int32 for ``ops.paged_decode_shared``
+        over these requests in this order: neighbours with the same first block are a
+        group, the blocks that all of it begins with are its prefix."""
+        rows = self._rows_of(request_ids)
+        n = len(rows)
+        if n == 0:
+            return np.zeros(1, dtype=np.int32), np.zeros(0, dtype=np.int32)
+        first, have = self._store[rows, 0], self._store_blocks[rows]
+        new = np.ones(n, dtype=bool)
+        new[1:] = (first[1:] != first[:-1]) | (have[1:] == 0) | (have[:-1] == 0)
+        cu = np.append(np.flatnonzero(new), n).astype(np.int32)
+        prefix = np.zeros(len(cu) - 1, dtype=np.int32)
+        for g in np.flatnonzero(np.diff(cu) > 1):
+            members = rows[cu[g]:cu[g + 1]]
+            most = int(self._store_blocks[members].min())
+            tables = self._store[members, :most]
+            differs = np.flatnonzero((tables != tables[0]).any(axis=0))
+            blocks = int(differs[0]) if len(differs) else most
+            prefix[g] = min(blocks * self.block_size, int(self._store_tokens[members].min()))
+        return cu, prefix
 
     def store_token_counts(self, rows: np.ndarray) -> np.ndarray:
         """int64 token counts of store ``rows``."""

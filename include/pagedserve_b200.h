@@ -594,7 +594,11 @@ int psb_trim_tables(int32_t* table_store, int64_t store_stride, int32_t store_ro
  * -1), like an extend_step: PSB_DEVERR_CONTEXT (a row or length out of range),
  * PSB_DEVERR_ROWS (a child named twice or as a parent), PSB_DEVERR_POOL (not
  * enough free blocks), PSB_DEVERR_BLOCK_RANGE (an id outside the pool), with
- * PSB_DEVERR_REFUSED, under which it refuses in turn.
+ * PSB_DEVERR_REFUSED, under which it refuses in turn.  A batch whose plan (12 bytes an
+ * entry, a bit per store row) is over 200 KB is PSB_ERR_UNSUPPORTED.
+ * fork_tables, release_tables and copy_blocks are programmatic dependent launches
+ * that start their dependents early: as behind psb_extend_step, an ordinary launch
+ * must lie between them and psb_paged_decode (not psb_paged_decode_shared).
  */
 int psb_fork_tables(int32_t* table_store, int64_t store_stride, int32_t store_rows, int32_t store_width,
                     const int32_t* parent_rows, const int32_t* child_rows, const int32_t* lens, int32_t batch,
@@ -637,7 +641,8 @@ int psb_copy_blocks(void* const* pools, const int64_t* block_bytes, int32_t num_
  * prefix sees its own context_lens[b] tokens of it, one of none gets zeros.
  * Sequences of no group, or alone in one, are read on their own.
  * Taken: bf16/f16, head_dim 64 or 128, up to 16 q heads per kv head, block sizes 16,
- * 32, 64 and multiples of 64, up to 2048 sequences and groups, query strides and bases
+ * 32, 64 and multiples of 64, up to 2048 sequences and groups as long as 12 bytes a
+ * sequence and 24 a group fit 33 KB (of 2048 sequences: 380 groups), query strides and bases
  * of 16 bytes; PSB_ERR_UNSUPPORTED otherwise (psb_paged_decode answers those, one
  * sequence at a time).  ``scale`` is positive.  Lengths, groups and tables are read
  * behind the stream predecessor's end.  A malformed cu_groups is flagged

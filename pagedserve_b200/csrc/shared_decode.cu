@@ -30,6 +30,15 @@
 // TMEM: S = Q K^T of its next step but one is issued behind O += P V of this one, whose
 // P, two keys a column, was written over S.
 //
+// Measured (a pass among others, of which 5 us are the two launches and 4 the plan): 8
+// sequences on 1 K shared tokens 14 us, 64 on 4 K 20, 32 groups of 8 on 1.5 K 27; 256 on 2 K
+// with 1 K each of their own 41, its 130 MB in 32 at 4 TB/s (the plain decode of the
+// same contexts: 720 MB); 96 on 30 K, D 128, 89, its 47 GFLOP in 70: a pair's step takes 2050
+// cycles where its exponentials are 1024 and its products 1300 (64 keys a step: Q is
+// read from shared memory again for each; 128 keys do not fit TMEM beside two O).  Tried
+// and not faster: a third stage of V, boxes asked into L2 ahead, the products' bookkeeping
+// moved behind P V's issue, own slices of 32 tokens.
+//
 // Which of a group's tables the prefix is read through: that of the sequence
 // with the most tokens (the first of those), and the prefix ends with it.  A
 // sequence that is shorter than the prefix is read on its own (an idle row of a
@@ -63,7 +72,10 @@ constexpr uint32_t kKvHalf = kBN * 128;    // of a K or V tile
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kSCol = 0, kOCol = 4 * kBN;
 constexpr float kRescaleLog2 = 8.f;  // O is rescaled when a row's maximum grows by more than 2^8
-constexpr int kMinCost = 8;          // steps of a tile per CTA below which the grid shrinks (at least 2: see Cursor)
+// Steps of a tile per CTA below which the grid shrinks, beyond a quarter of the SMs and below (at
+// least 2: see Cursor).  Fewer steps are more partials: 256 sequences on 2 K take 2 us more
+// with 4 everywhere, 8 on 1 K 2 us more with 8.
+constexpr int kMinCost = 8, kMinCostFew = 4;
 constexpr int kOwnMinItems = 2;      // slices per warp below which fewer warps work
 constexpr int kMaxCtas = 160;        // (B200 has 148 SMs)
 
@@ -156,16 +168,27 @@ struct Plan {
   __device__ __forceinline__ int steps_of(int g) const { return (pre[g] + kBN - 1) / kBN; }
 };
 
-// A warp's exclusive scan of one value a lane, and the total.
-__device__ __forceinline__ int scan_warp(int v, int& total) {
-  int incl = v;
+// A warp's exclusive scans of N values a lane, and the totals.
+template <int N>
+__device__ __forceinline__ void scan_warp(int (&v)[N], int (&total)[N]) {
+  int incl[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) incl[i] = v[i];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, incl, o);
-    if ((threadIdx.x & 31) >= o) incl += x;
+    int x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __shfl_up_sync(0xffffffffu, incl[i], o);
+    if ((threadIdx.x & 31) >= o) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) incl[i] += x[i];
+    }
   }
-  total = __shfl_sync(0xffffffffu, incl, 31);
-  return incl - v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    total[i] = __shfl_sync(0xffffffffu, incl[i], 31);
+    v[i] = incl[i] - v[i];
+  }
 }
 
 __device__ void build_plan(const SharedParams& p, Plan& pl) {
@@ -217,42 +240,39 @@ __device__ void build_plan(const SharedParams& p, Plan& pl) {
   if (warp == 0) {  // the groups' tiles
     const int per = (p.groups + 31) / 32, g0 = min(lane * per, p.groups), g1 = min(g0 + per, p.groups);
     auto tiles_of = [&](int g) { return pl.pre[g] > 0 ? (pl.cu[g + 1] - pl.cu[g] + p.tq - 1) / p.tq : 0; };
-    int tiles = 0, pairs = 0, cost = 0;
+    int v[3] = {0, 0, 0}, all[3];  // tiles, pairs, cost
     for (int g = g0; g < g1; ++g) {
       const int n = tiles_of(g);
-      tiles += n;
-      pairs += (n + 1) >> 1;
-      cost += n * pl.steps_of(g);
+      v[0] += n;
+      v[1] += (n + 1) >> 1;
+      v[2] += n * pl.steps_of(g);
     }
-    int all_tiles, all_pairs, all_cost;
-    tiles = scan_warp(tiles, all_tiles);
-    pairs = scan_warp(pairs, all_pairs);
-    cost = scan_warp(cost, all_cost);
+    scan_warp(v, all);
     for (int g = g0; g < g1; ++g) {
-      pl.tiles[g] = tiles;
-      pl.pairs[g] = pairs;
-      pl.cost[g] = cost;
+      pl.tiles[g] = v[0];
+      pl.pairs[g] = v[1];
+      pl.cost[g] = v[2];
       const int n = tiles_of(g);
-      tiles += n;
-      pairs += (n + 1) >> 1;
-      cost += n * pl.steps_of(g);
+      v[0] += n;
+      v[1] += (n + 1) >> 1;
+      v[2] += n * pl.steps_of(g);
     }
     if (lane == 0) {
-      pl.tiles[p.groups] = all_tiles;
-      pl.pairs[p.groups] = all_pairs;
-      pl.cost[p.groups] = all_cost;
+      pl.tiles[p.groups] = all[0];
+      pl.pairs[p.groups] = all[1];
+      pl.cost[p.groups] = all[2];
     }
   } else if (warp == 1) {  // the sequences' slices
     const int per = (p.batch + 31) / 32, b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
     auto slices_of = [&](int b) { return pl.ctx[b] > pl.start[b] ? (pl.ctx[b] + 15) / 16 - pl.start[b] / 16 : 0; };
-    int n = 0, all;
-    for (int b = b0; b < b1; ++b) n += slices_of(b);
-    n = scan_warp(n, all);
+    int n[1] = {0}, all[1];
+    for (int b = b0; b < b1; ++b) n[0] += slices_of(b);
+    scan_warp(n, all);
     for (int b = b0; b < b1; ++b) {
-      pl.slices[b] = n;
-      n += slices_of(b);
+      pl.slices[b] = n[0];
+      n[0] += slices_of(b);
     }
-    if (lane == 0) pl.slices[p.batch] = all;
+    if (lane == 0) pl.slices[p.batch] = all[0];
   }
   __syncthreads();
   pl.n_tiles = pl.tiles[p.groups];
@@ -357,7 +377,7 @@ __device__ __forceinline__ bool warp_wait_at(uint32_t bar, uint32_t parity) {
   return true;
 }
 template <int S>
-struct Stream {
+struct Int {
   static constexpr int value = S;
 };
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
@@ -805,14 +825,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
   const uint32_t total = static_cast<uint32_t>(plan.n_cost) * p.hkv;  // below 2^31
-  const Deal deal(total, min(gridDim.x, (total + kMinCost - 1) / kMinCost));
+  const Deal deal(total, min(gridDim.x, max((total + kMinCost - 1) / kMinCost, min((total + kMinCostFew - 1) / kMinCostFew, gridDim.x / 4))));
   const uint32_t cta = blockIdx.x;
   Cursor first;
   first.left = 0;
-  if (cta < deal.parts) {
-    Cursor end;
-    const uint32_t my_e = deal.start(cta + 1), e = my_e == total ? total : end.seek(plan, my_e);
-    first.left = static_cast<int>(e - first.seek(plan, deal.start(cta)));
+  if (cta < deal.parts) {  // odd lanes look where the CTA's steps end, even ones where they begin
+    const uint32_t at = deal.start(cta + (lane & 1));
+    Cursor c;
+    const uint32_t unit = at == total ? total : c.seek(plan, at);
+    first.kvh = __shfl_sync(0xffffffffu, c.kvh, 0);
+    first.grp = __shfl_sync(0xffffffffu, c.grp, 0);
+    first.in_grp = __shfl_sync(0xffffffffu, c.in_grp, 0);
+    first.j0 = __shfl_sync(0xffffffffu, c.j0, 0);
+    first.left = static_cast<int>(__shfl_sync(0xffffffffu, unit, 1) - __shfl_sync(0xffffffffu, unit, 0));
   }
   bool fail = false;
 
@@ -999,8 +1024,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     own_parts<T, D, HP, NT>(p, plan, &tm_ko, &tm_vo, smem + Geo::kOffRing, bar_own);
   } else if (warp >= 8) {
     fewer_registers<kOtherRegs>();
-    if (warp == 8) products(Stream<0>());
-    else if (warp == 9) products(Stream<1>());
+    if (warp == 8) products(Int<0>());
+    else if (warp == 9) products(Int<1>());
     else copies();
   } else {
     more_registers<kSoftmaxRegs>();
@@ -1140,10 +1165,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 // A lane has a row (a sequence's q head of one kv head) and four of its dims, a warp 32
 // consecutive rows, whose partials lie side by side; a CTA's four warps take a quarter
 // of the partials each (they come from L2: rounds of loads, not bytes, are what it
-// costs; one warp for all of 33 partials took 10 us).
-constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32, kBatch = 4;
+// costs; one warp for all of 33 partials took 10 us).  BATCH: a warp's partials in flight,
+// eight of a few CTAs (those 33: 2 us less than with four), four of many (3000 CTAs: the
+// registers of eight would cost 3 us).
+constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32;
 
-template <typename T, int D>
+template <typename T, int D, int BATCH>
 __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedParams p, int hp) {
   __shared__ float2 s_ml[kJoinWarps][32];
   __shared__ float4 s_o[kJoinWarps][32];
@@ -1161,11 +1188,11 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
   const int tiles = tile.y & 0xffff, apart = tile.y >> 16, n = tiles + own.y;
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](const float2* ml, const float4* v, int count) {
+  auto add = [&](auto batch, const float2* ml, const float4* v) {
+    constexpr int kBatch = decltype(batch)::value;
     float mn = m;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      if (j < count) mn = fmaxf(mn, ml[j].x);
+    for (int j = 0; j < kBatch; ++j) mn = fmaxf(mn, ml[j].x);
     const float mu = mn == -INFINITY ? 0.f : mn, a = ex2_approx(m - mu);
     m = mn;
     l *= a;
@@ -1175,7 +1202,7 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
     o.w *= a;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      if (j >= count || ml[j].x == -INFINITY) continue;  // nothing was summed (nor written)
+      if (ml[j].x == -INFINITY) continue;  // nothing was summed (nor written)
       const float w = ex2_approx(ml[j].x - mu);
       l = fmaf(ml[j].y, w, l);
       o.x = fmaf(v[j].x, w, o.x);
@@ -1184,8 +1211,9 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
       o.w = fmaf(v[j].w, w, o.w);
     }
   };
-#pragma unroll 1
-  for (int i0 = warp; i0 < n; i0 += kBatch * kJoinWarps) {
+  // partials i0, i0 + 4, .. of the row, ``batch`` in flight
+  auto round = [&](auto batch, int i0) {
+    constexpr int kBatch = decltype(batch)::value;
     float2 ml[kBatch];
     float4 v[kBatch];
 #pragma unroll
@@ -1202,22 +1230,23 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
         v[j] = __ldcg(reinterpret_cast<const float4*>(part) + c4 * rows + row);
       }
     }
-    add(ml, v, kBatch);
-  }
+    add(batch, ml, v);
+  };
+#pragma unroll 1
+  for (int i0 = warp; i0 < n; i0 += BATCH * kJoinWarps) round(Int<BATCH>(), i0);
   s_ml[warp][lane] = make_float2(m, l);
   s_o[warp][lane] = o;
   __syncthreads();
   if (warp != 0 || static_cast<int>(blockIdx.x) * 32 + lane >= p.batch * p.group) return;
   {
-    static_assert(kBatch >= kJoinWarps - 1, "the other warps' sums in one go");
-    float2 ml[kBatch];
-    float4 v[kBatch];
+    float2 ml[kJoinWarps - 1];
+    float4 v[kJoinWarps - 1];
 #pragma unroll
     for (int j = 0; j < kJoinWarps - 1; ++j) {
       ml[j] = s_ml[j + 1][lane];
       v[j] = s_o[j + 1][lane];
     }
-    add(ml, v, kJoinWarps - 1);
+    add(Int<kJoinWarps - 1>(), ml, v);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* const out = reinterpret_cast<T*>(p.out) + b * p.osb + (kvh * p.group + gh) * p.osh + 4 * c4;
@@ -1310,7 +1339,9 @@ int launch(SharedParams p, int num_layers, cudaStream_t s) {
   discard_stale_error();
   cudaError_t e = launch_pdl(kern, dim3(std::min(kMaxCtas, sms)), dim3(kThreads), smem, s, p, tq, tk, tv, tko, tvo);
   if (e != cudaSuccess) return record_cuda_error(e);
-  e = launch_pdl(shared_join_kernel<T, D>, dim3((p.batch * p.group + 31) / 32, D / 4, p.hkv), dim3(kJoinThreads), 0, s, p, two ? 2 : 1);
+  const dim3 join((p.batch * p.group + 31) / 32, D / 4, p.hkv);
+  const bool few = static_cast<int64_t>(join.x) * join.y * join.z <= 4 * sms;
+  e = launch_pdl(few ? shared_join_kernel<T, D, 8> : shared_join_kernel<T, D, 4>, join, dim3(kJoinThreads), 0, s, p, two ? 2 : 1);
   if (e != cudaSuccess) return record_cuda_error(e);
   return check_launch();
 }

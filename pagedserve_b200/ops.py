@@ -1127,7 +1127,8 @@ def fork_tables(table_store: torch.Tensor, parent_rows: torch.Tensor, child_rows
     (-1: none).  One parent may have many children; a child is no parent of the
     same call; ``child_rows[b] < 0`` is padding.  Rows that share blocks give them
     back with ``release_tables`` (not ``trim_tables``).  Checked and refused as a
-    whole, like ``extend_step``.
+    whole, like ``extend_step``; and as behind it there must be an ordinary launch
+    between this call, ``copy_blocks`` or ``release_tables`` and ``paged_decode``.
     """
     if table_store.is_cuda:
         done = (_native._calls or _native.calls()).fork(table_store, parent_rows, child_rows, lens, free_blocks, free_state,
@@ -1231,10 +1232,9 @@ def paged_decode_shared(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     (``[B, Hq, D]`` or ``[B, Hq, 1, D]``) and dtype.
 
     Prefixes are shared for bf16/f16, head_dim 64 or 128, up to 16 q heads per kv
-    head, blocks of 16, 32, 64 or a multiple of 64 tokens, up to 2048 sequences; other
-    geometries, and batches whose
-    plan does not fit shared memory (from some 900 sequences in as many groups on), are answered by ``paged_decode``, each
-    sequence on its own.  ``scale`` must be positive.
+    head, blocks of 16, 32, 64 or a multiple of 64 tokens, up to 2048 sequences
+    (12 bytes a sequence and 24 a group have to fit 33 KB); the rest is answered by
+    ``paged_decode``, each sequence on its own.  ``scale`` must be positive.
     """
     if query.is_cuda:
         done = (_native._calls or _native.calls()).decode_shared(query, k_cache, v_cache, block_tables, context_lens, cu_groups,

@@ -20,11 +20,13 @@
 // changed; counts, then ranks).  A call that cannot be carried out whole changes
 // nothing, as extend_step and trim_tables.
 //
-// The work is dealt over the warps in units of up to 128 blocks of one entry, in
-// entry and table order, four blocks a lane whose loads and atomics are in
+// The work is dealt over the warps in units of up to 256 blocks of one entry, in
+// entry and table order, eight blocks a lane whose loads and atomics are in
 // flight together; what a phase has read stays in shared memory for the next (where
 // it fits; else it is read again).  (One block a thread and a search for its entry
-// each time: 28 us for 255 forks of 250 blocks and 70 us for their release.)
+// each time: 28 us for 255 forks of 250 blocks and 70 us for their release; so 14 and
+// 21, with units of 128 14 and 28.)  4 forks of 50 blocks: 8 and 10, three or four dependent
+// loads and as many barriers.
 //
 // release: first every item takes one off its block's counter and leaves its
 // number, if it is the highest, in the scratch word.  Behind the barrier a counter
@@ -45,7 +47,7 @@ namespace {
 constexpr int kPageThreads = 512;
 constexpr int kPageWarps = kPageThreads / 32;
 constexpr int kPageCtas = 16;  // CTAs of the cluster, at most
-constexpr int kUnit = 128, kLanes = kUnit / 32;  // blocks of a unit, and of each lane
+constexpr int kUnit = 256, kLanes = kUnit / 32;  // blocks of a unit, and of each lane
 constexpr size_t kPagesSmem = 200 * 1024;
 
 struct PagesParams {

@@ -31,9 +31,9 @@
 // P, two keys a column, was written over S.
 //
 // Measured (a pass among others, of which 5 us are the two launches and 4 the plan): 8
-// sequences on 1 K shared tokens 14 us, 64 on 4 K 20, 32 groups of 8 on 1.5 K 27; 256 on 2 K
-// with 1 K each of their own 41, its 130 MB in 32 at 4 TB/s (the plain decode of the
-// same contexts: 720 MB); 96 on 30 K, D 128, 89, its 47 GFLOP in 70: a pair's step takes 2050
+// sequences on 1 K shared tokens 12 us, 64 on 4 K 19, 32 groups of 8 on 1.5 K 26; 256 on 2 K
+// with 1 K each of their own 41, its 130 MB in 30 at 4.3 TB/s (the plain decode of the
+// same contexts: 720 MB); 96 on 30 K, D 128, 86, its 47 GFLOP in 66: a pair's step takes 2050
 // cycles where its exponentials are 1024 and its products 1300 (64 keys a step: Q is
 // read from shared memory again for each; 128 keys do not fit TMEM beside two O).  Tried
 // and not faster: a third stage of V, boxes asked into L2 ahead, the products' bookkeeping
@@ -72,10 +72,19 @@ constexpr uint32_t kKvHalf = kBN * 128;    // of a K or V tile
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kSCol = 0, kOCol = 4 * kBN;
 constexpr float kRescaleLog2 = 8.f;  // O is rescaled when a row's maximum grows by more than 2^8
-// Steps of a tile per CTA below which the grid shrinks, beyond a quarter of the SMs and below (at
-// least 2: see Cursor).  Fewer steps are more partials: 256 sequences on 2 K take 2 us more
-// with 4 everywhere, 8 on 1 K 2 us more with 8.
-constexpr int kMinCost = 8, kMinCostFew = 4;
+// What a step costs, of a pair of tiles and of a single one: D 128 1.40 and 0.97 us over 30 K
+// keys (by tiles, CTAs of singles alone end 10 us after those of pairs; all of it 88.5 us, so
+// 84.5); D 64 by tiles (256 on 2 K 46.0 us, as D 128 46.7).
+// kMin: cost per CTA below which the grid shrinks, beyond a quarter of the SMs and below
+// (kMinFew; at least two pairs' steps less one: see Cursor).  Fewer steps are more partials:
+// 256 sequences on 2 K take 2 us more with the lower one everywhere, 8 on 1 K 2 us more
+// with the higher one.
+template <int D>
+struct Cost {
+  static constexpr int kPair = D == 64 ? 2 : 3, kTile = D == 64 ? 1 : 2;
+  static constexpr int kMin = 4 * kPair, kMinFew = 4 * kTile;
+  static_assert(kMinFew >= 2 * kPair - 1 && kMin >= kMinFew, "every CTA has a step");
+};
 constexpr int kOwnMinItems = 2;      // slices per warp below which fewer warps work
 constexpr int kMaxCtas = 160;        // (B200 has 148 SMs)
 
@@ -151,7 +160,7 @@ struct Plan {
   // before a group, of one kv head:
   int32_t* tiles;   // [groups + 1]
   int32_t* pairs;   // [groups + 1]
-  int32_t* cost;    // [groups + 1] steps, counted once for each tile
+  int32_t* cost;    // [groups + 1]
   int groups, tq, n_tiles, n_pairs, n_cost, n_slices;
   __host__ __device__ static size_t ints(int batch, int groups) { return 3 * static_cast<size_t>(batch) + 1 + 6 * static_cast<size_t>(groups) + 4; }
   __device__ Plan(int32_t* at, int batch, int n, int q) : groups(n), tq(q) {
@@ -191,6 +200,7 @@ __device__ __forceinline__ void scan_warp(int (&v)[N], int (&total)[N]) {
   }
 }
 
+template <int D>
 __device__ void build_plan(const SharedParams& p, Plan& pl) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool report = blockIdx.x == 0;
@@ -240,12 +250,13 @@ __device__ void build_plan(const SharedParams& p, Plan& pl) {
   if (warp == 0) {  // the groups' tiles
     const int per = (p.groups + 31) / 32, g0 = min(lane * per, p.groups), g1 = min(g0 + per, p.groups);
     auto tiles_of = [&](int g) { return pl.pre[g] > 0 ? (pl.cu[g + 1] - pl.cu[g] + p.tq - 1) / p.tq : 0; };
+    auto cost_of = [](int n) { return (n >> 1) * Cost<D>::kPair + (n & 1) * Cost<D>::kTile; };  // a step of n tiles
     int v[3] = {0, 0, 0}, all[3];  // tiles, pairs, cost
     for (int g = g0; g < g1; ++g) {
       const int n = tiles_of(g);
       v[0] += n;
       v[1] += (n + 1) >> 1;
-      v[2] += n * pl.steps_of(g);
+      v[2] += cost_of(n) * pl.steps_of(g);
     }
     scan_warp(v, all);
     for (int g = g0; g < g1; ++g) {
@@ -255,7 +266,7 @@ __device__ void build_plan(const SharedParams& p, Plan& pl) {
       const int n = tiles_of(g);
       v[0] += n;
       v[1] += (n + 1) >> 1;
-      v[2] += n * pl.steps_of(g);
+      v[2] += cost_of(n) * pl.steps_of(g);
     }
     if (lane == 0) {
       pl.tiles[p.groups] = all[0];
@@ -391,10 +402,11 @@ struct Run {
   bool two;                  // there is a second tile
 };
 
-// Walks a CTA's steps pair by pair.  A step of a pair costs 2 (one tile: 1) and belongs
-// to the CTA that its last unit of cost was dealt to: a CTA that was dealt two units
-// or more in a pair has steps there.
+// Walks a CTA's steps pair by pair.  A step belongs to the CTA that its last unit of cost
+// was dealt to: a CTA that was dealt a step's cost or more in a pair has steps there.
+template <int D>
 struct Cursor {
+  static constexpr int kPairCost = Cost<D>::kPair, kTileCost = Cost<D>::kTile;
   int kvh, grp, in_grp, j0, left;  // left: cost
   // To the step that the unit at ``pos`` of the whole list is in, or begins; returns its first unit.
   __device__ uint32_t seek(const Plan& pl, uint32_t pos) {
@@ -402,10 +414,10 @@ struct Cursor {
     const int r = static_cast<int>(pos - static_cast<uint32_t>(kvh) * pl.n_cost);
     grp = last_le(pl.cost, pl.groups, r);  // (of groups without steps the last: it has some)
     const int steps = pl.steps_of(grp), off = r - pl.cost[grp];
-    in_grp = off / (2 * steps);
-    const int in_pair = off - in_grp * 2 * steps;
-    j0 = two(pl) ? in_pair >> 1 : in_pair;
-    return pos - (two(pl) ? in_pair & 1 : 0);
+    in_grp = off / (kPairCost * steps);
+    const int in_pair = off - in_grp * kPairCost * steps, of_step = two(pl) ? kPairCost : kTileCost;
+    j0 = in_pair / of_step;
+    return pos - (in_pair - j0 * of_step);
   }
   __device__ bool two(const Plan& pl) const { return 2 * in_grp + 1 < pl.tiles[grp + 1] - pl.tiles[grp]; }
   __device__ Run take(const Plan& pl) {  // the next run (left > 0)
@@ -419,8 +431,8 @@ struct Cursor {
     r.n_seq = pl.cu[grp + 1] - r.b0;
     r.two = two(pl);
     r.j0 = j0;
-    r.n = min(pl.steps_of(grp) - j0, r.two ? left >> 1 : left);
-    left -= r.two ? 2 * r.n : r.n;
+    r.n = min(pl.steps_of(grp) - j0, r.two ? left / kPairCost : left / kTileCost);
+    left -= r.n * (r.two ? kPairCost : kTileCost);
     j0 = 0;
     if (left > 0) {
       ++in_grp;
@@ -440,12 +452,13 @@ struct Cursor {
 
 // One stream's steps of a CTA, in order: of pairs of tiles every step, of single tiles
 // those whose number, counted in half-steps (a step of one stream) of the CTA, is its own.
+template <int D>
 struct Steps {
-  Cursor c;
+  Cursor<D> c;
   Run r;
   int x, half, g0;  // step of the run; half-steps and steps of the CTA before the run
   bool begins;      // the first of the run
-  __device__ explicit Steps(const Cursor& first) : c(first), x(0), half(0), g0(0), begins(true) {
+  __device__ explicit Steps(const Cursor<D>& first) : c(first), x(0), half(0), g0(0), begins(true) {
     r.n = 0;
     r.two = false;
   }
@@ -821,17 +834,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();  // lengths, groups, tables, q and the pools may come from the stream predecessor
   pdl_launch_dependents();
   tc_fence_before();
-  build_plan(p, plan);  // (its barriers are also those behind the set-up above)
+  build_plan<D>(p, plan);  // (its barriers are also those behind the set-up above)
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
+  using C = Cost<D>;
   const uint32_t total = static_cast<uint32_t>(plan.n_cost) * p.hkv;  // below 2^31
-  const Deal deal(total, min(gridDim.x, max((total + kMinCost - 1) / kMinCost, min((total + kMinCostFew - 1) / kMinCostFew, gridDim.x / 4))));
+  const Deal deal(total, min(gridDim.x, max((total + C::kMin - 1) / C::kMin, min((total + C::kMinFew - 1) / C::kMinFew, gridDim.x / 4))));
   const uint32_t cta = blockIdx.x;
-  Cursor first;
+  Cursor<D> first;
   first.left = 0;
   if (cta < deal.parts) {  // odd lanes look where the CTA's steps end, even ones where they begin
     const uint32_t at = deal.start(cta + (lane & 1));
-    Cursor c;
+    Cursor<D> c;
     const uint32_t unit = at == total ? total : c.seek(plan, at);
     first.kvh = __shfl_sync(0xffffffffu, c.kvh, 0);
     first.grp = __shfl_sync(0xffffffffu, c.grp, 0);
@@ -867,7 +881,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto landed = [&](uint32_t full, uint32_t free, uint32_t st, uint32_t round) {
       return (round == 0 || warp_wait_at(free + 8 * st, (round - 1) & 1)) && warp_wait_at(full + 8 * st, round & 1);
     };
-    Steps hs(first);
+    Steps<D> hs(first);
     // What P V has to know of a step, from its S two steps before: its number in the
     // CTA's list, how many of its keys there are (bits 24 to 29; 0: all), whether the run
     // begins (bit 30) and is a pair's (bit 31); of none: kNone.
@@ -963,7 +977,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int bs = p.block_size, box_rows = min(bs, kBN), boxes = kBN / box_rows;
     const int64_t layer0 = static_cast<int64_t>(p.layer) * p.num_blocks;
     const uint32_t box_bytes = static_cast<uint32_t>(box_rows) * 128;
-    Cursor cc = first;
+    Cursor<D> cc = first;
     uint32_t g = 0;  // steps so far
 #pragma unroll 1
     while (cc.left > 0 && !fail) {
@@ -1034,7 +1048,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rseq = row / group;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float sc = p.scale_log2;
-    Cursor cc = first;
+    Cursor<D> cc = first;
     int half = 0, k = 0;  // half-steps before the run, this stream's steps so far
     while (cc.left > 0 && !fail) {
       const Run r = cc.take(plan);
@@ -1140,8 +1154,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (live) reinterpret_cast<float2*>(part + kRows * D)[row] = make_float2(ms, l);  // (of a stream without steps: none)
       if (r.j0 == 0 && tid == 0) {
         const int steps = plan.steps_of(r.grp);
-        const uint32_t begin = static_cast<uint32_t>(r.kvh) * plan.n_cost + plan.cost[r.grp] + 2 * r.in_grp * steps;
-        const int ctas = static_cast<int>(deal.part_of(begin + (r.two ? 2 : 1) * steps - 1) - cta) + 1;
+        const uint32_t begin = static_cast<uint32_t>(r.kvh) * plan.n_cost + plan.cost[r.grp] + C::kPair * r.in_grp * steps;
+        const int ctas = static_cast<int>(deal.part_of(begin + (r.two ? C::kPair : C::kTile) * steps - 1) - cta) + 1;
         int2* const info = p.tile_info + r.kvh * p.max_tiles + r.tile;
         const int slot = 2 * static_cast<int>(cta + ord);
         info[0] = r.two ? make_int2(slot, ctas | 2 << 16) : make_int2(slot, 2 * ctas | 1 << 16);
@@ -1280,7 +1294,7 @@ bool takes(int batch, int groups, int q_heads, int hkv, int head_dim, int block_
   if (group > 16 || block_size < 16 || block_size % 16 || !(64 % block_size == 0 || block_size % 64 == 0)) return false;
   if (main_smem(batch, groups, group, hkv, head_dim) > kMaxSmem || hkv > 65535) return false;
   const int64_t steps = (static_cast<int64_t>(max_context) + kBN) / kBN, tiles = batch / (kRows / group) + std::min(groups, batch / 2) + 1;
-  return static_cast<int64_t>(batch) * hkv < (1 << 24) && steps * tiles < (int64_t(1) << 31) / hkv &&
+  return static_cast<int64_t>(batch) * hkv < (1 << 24) && steps * tiles < (int64_t(1) << 30) / hkv &&
          (static_cast<int64_t>(max_context) / 16 + 2) * batch < (int64_t(1) << 31) / hkv;
 }
 

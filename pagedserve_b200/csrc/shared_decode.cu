@@ -18,7 +18,7 @@
 //    a step's K and V, 32 KB for D 128, in the time of its products: beyond what L2
 //    gives all SMs); of a pair with one tile, the two streams below take the steps in
 //    turn.  The steps of all pairs, in (kv head, group, pair, step) order, are dealt
-//    evenly, by their tiles, over the CTAs; every run of steps leaves partials.
+//    evenly, by what they cost, over the CTAs; every run of steps leaves partials.
 //  Own parts: the 16-token slices of what is each sequence's own, in (kv heads,
 //    sequence, slice) order, are dealt evenly over four warps of every CTA; every run
 //    of slices leaves a partial.
@@ -123,7 +123,7 @@ struct SharedParams {
   const int32_t* prefix;
   int32_t batch, groups, hkv, group, layer, block_size, max_context;
   int32_t tq;          // sequences per tile
-  int32_t max_tiles, max_pairs;  // of one kv head there is room for
+  int32_t max_tiles;   // of one kv head there is room for
   int64_t num_blocks;
   float scale_log2;    // scale log2(e), positive
   // workspace
@@ -161,7 +161,7 @@ struct Plan {
   int32_t* tiles;   // [groups + 1]
   int32_t* pairs;   // [groups + 1]
   int32_t* cost;    // [groups + 1]
-  int groups, tq, n_tiles, n_pairs, n_cost, n_slices;
+  int groups, tq, n_pairs, n_cost, n_slices;
   __host__ __device__ static size_t ints(int batch, int groups) { return 3 * static_cast<size_t>(batch) + 1 + 6 * static_cast<size_t>(groups) + 4; }
   __device__ Plan(int32_t* at, int batch, int n, int q) : groups(n), tq(q) {
     ctx = at;
@@ -286,7 +286,6 @@ __device__ void build_plan(const SharedParams& p, Plan& pl) {
     if (lane == 0) pl.slices[p.batch] = all[0];
   }
   __syncthreads();
-  pl.n_tiles = pl.tiles[p.groups];
   pl.n_pairs = pl.pairs[p.groups];
   pl.n_cost = pl.cost[p.groups];
   pl.n_slices = pl.slices[p.batch];
@@ -1416,7 +1415,6 @@ extern "C" int psb_paged_decode_shared(const void* query, int64_t q_stride_b, in
   p.max_context = max_context;
   p.tq = kRows / group;
   p.max_tiles = lay.max_tiles;
-  p.max_pairs = lay.max_pairs;
   p.num_blocks = num_blocks;
   p.scale_log2 = scale * 1.4426950408889634f;
   char* const ws = static_cast<char*>(workspace);

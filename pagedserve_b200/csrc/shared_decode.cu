@@ -624,7 +624,7 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
 
   uint32_t q[HP][NT][kSteps][2];  // columns: q heads gq (+ 8)
   float o[HP][NT][kSteps][4];     // dims gq, gq + 8 of 16, of q heads 2 t, 2 t + 1 (+ 8)
-  float m[HP][NT][2], l[HP][NT][2];  // of these heads: the maximum, this lane's share of the sum
+  float m[HP][NT][2], l[HP][NT][2];  // of these heads: the exponents' reference (a maximum, scaled), this lane's share of the sum
   int32_t pair = 0;
   while (consumed != issued) {
     const uint32_t slot = consumed % kRing;
@@ -691,23 +691,37 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
           }
         }
       }
-      float mx[HP][NT][2];
+      // A new reference, and O and the sums brought to it, where a score is above the old
+      // one by more than 2^8 (nearly always the first slices alone)
+      bool grow = false;
 #pragma unroll
       for (int hs = 0; hs < HP; ++hs) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) mx[hs][nt][e] = fmaxf(s[hs][nt][e], s[hs][nt][2 + e]);
+          for (int e = 0; e < 2; ++e) grow = grow || fmaxf(s[hs][nt][e], s[hs][nt][2 + e]) * p.scale_log2 > m[hs][nt][e] + kRescaleLog2;
         }
       }
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) {
+      if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int hs = 0; hs < HP; ++hs) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) mx[hs][nt][e] = fmaxf(mx[hs][nt][e], __shfl_xor_sync(0xffffffffu, mx[hs][nt][e], x));
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(s[hs][nt][e], s[hs][nt][2 + e]);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+              // every slice holds a valid token: the new reference is finite (or the scores are not numbers)
+              const float mn = fmaxf(m[hs][nt][e], mx * p.scale_log2), alpha = ex2_approx(m[hs][nt][e] - mn);
+              m[hs][nt][e] = mn;
+              l[hs][nt][e] *= alpha;
+#pragma unroll
+              for (int ks = 0; ks < kSteps; ++ks) {
+                o[hs][nt][ks][e] *= alpha;
+                o[hs][nt][ks][2 + e] *= alpha;
+              }
+            }
           }
         }
       }
@@ -719,17 +733,9 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
           float ex[4];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            // every slice holds a valid token: the new maximum is finite (or the scores are not numbers)
-            const float mn = fmaxf(m[hs][nt][e], mx[hs][nt][e]), alpha = ex2_approx((m[hs][nt][e] - mn) * p.scale_log2), ms = mn * p.scale_log2;
-            m[hs][nt][e] = mn;
-            ex[e] = ex2_approx(fmaf(s[hs][nt][e], p.scale_log2, -ms));
-            ex[2 + e] = ex2_approx(fmaf(s[hs][nt][2 + e], p.scale_log2, -ms));
-            l[hs][nt][e] = fmaf(l[hs][nt][e], alpha, ex[e] + ex[2 + e]);
-#pragma unroll
-            for (int ks = 0; ks < kSteps; ++ks) {
-              o[hs][nt][ks][e] *= alpha;
-              o[hs][nt][ks][2 + e] *= alpha;
-            }
+            ex[e] = ex2_approx(fmaf(s[hs][nt][e], p.scale_log2, -m[hs][nt][e]));
+            ex[2 + e] = ex2_approx(fmaf(s[hs][nt][2 + e], p.scale_log2, -m[hs][nt][e]));
+            l[hs][nt][e] += ex[e] + ex[2 + e];
           }
           pr[hs][nt][0] = transposed(pack2<T>(ex[0], ex[1]));
           pr[hs][nt][1] = transposed(pack2<T>(ex[2], ex[3]));
@@ -773,7 +779,7 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
 #pragma unroll
               for (int u = 0; u < 2; ++u) part[(4 * ks + 2 * u + (gq >> 2)) * 64 + 4 * row + (gq & 3)] = o[hs][nt][ks][2 * u + e];
             }
-            if (gq == 0) ml[row] = make_float2(m[hs][nt][e] * p.scale_log2, sum);
+            if (gq == 0) ml[row] = make_float2(m[hs][nt][e], sum);
           }
         }
       }

@@ -32,7 +32,7 @@
 //
 // Measured (a pass among others, of which 5 us are the two launches and 4 the plan): 8
 // sequences on 1 K shared tokens 12 us, 64 on 4 K 19, 32 groups of 8 on 1.5 K 26; 256 on 2 K
-// with 1 K each of their own 41, its 130 MB in 30 at 4.3 TB/s (the plain decode of the
+// with 1 K each of their own 40, its 130 MB in 30 at 4.3 TB/s (the plain decode of the
 // same contexts: 720 MB); 96 on 30 K, D 128, 86, its 47 GFLOP in 66: a pair's step takes 2050
 // cycles where its exponentials are 1024 and its products 1300 (64 keys a step: Q is
 // read from shared memory again for each; 128 keys do not fit TMEM beside two O).  Tried

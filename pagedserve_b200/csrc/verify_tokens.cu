@@ -399,7 +399,7 @@ struct Exact {
   double c16;    // sixteenths of an octave per logit
   double magic;  // 1.5 2^52 - m
   double bias;   // taken from the logits first where their exponents are beyond 2^40 (m is 0 then)
-  float low;     // logits up to it have none
+  float low;     // logits up to it have none (no logit lies between it and the exact border)
   bool far;
   const double* table;
   __device__ Exact(double c, float top, const double* t) : c16(16.0 * c), table(t) {
@@ -407,7 +407,8 @@ struct Exact {
     far = !(fabs(m) < 1099511627776.0);
     bias = far ? static_cast<double>(top) : 0.0;
     magic = 6755399441055744.0 - (far ? 0.0 : rint(m));
-    low = top + static_cast<float>(-900.0 / c);
+    // rounded down twice, so that it is below the maximum however small 900 / c is beside it
+    low = __double2float_rd(__dsub_rd(static_cast<double>(top), 900.0 / c));
   }
   __device__ __forceinline__ double weight(float x) const {
     double xd = static_cast<double>(x);

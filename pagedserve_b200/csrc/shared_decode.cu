@@ -46,6 +46,7 @@
 // tile, would still meet its probabilities of 0, and 0 times infinity is no number.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -647,7 +648,7 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
             q[hs][nt][ks][1] = h < G ? __ldcg(reinterpret_cast<const uint32_t*>(row + 16 * ks + 8)) : 0u;
             o[hs][nt][ks][0] = o[hs][nt][ks][1] = o[hs][nt][ks][2] = o[hs][nt][ks][3] = 0.f;
           }
-          m[hs][nt][0] = m[hs][nt][1] = -INFINITY;
+          m[hs][nt][0] = m[hs][nt][1] = -FLT_MAX;  // (not -infinity: beside it a score of -infinity would be no number)
           l[hs][nt][0] = l[hs][nt][1] = 0.f;
         }
       }
@@ -712,7 +713,6 @@ __device__ __forceinline__ void own_parts(const SharedParams& p, const Plan& pla
               float mx = fmaxf(s[hs][nt][e], s[hs][nt][2 + e]);
 #pragma unroll
               for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-              // every slice holds a valid token: the new reference is finite (or the scores are not numbers)
               const float mn = fmaxf(m[hs][nt][e], mx * p.scale_log2), alpha = ex2_approx(m[hs][nt][e] - mn);
               m[hs][nt][e] = mn;
               l[hs][nt][e] *= alpha;

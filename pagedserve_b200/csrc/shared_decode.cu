@@ -1221,7 +1221,8 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
     o.w *= a;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      if (ml[j].x == -INFINITY) continue;  // nothing was summed (nor written)
+      // nothing was summed (nor written); a sum that is no number, of scores that are none, is not nothing
+      if (ml[j].x == -INFINITY && ml[j].y == 0.f) continue;
       const float w = ex2_approx(ml[j].x - mu);
       l = fmaf(ml[j].y, w, l);
       o.x = fmaf(v[j].x, w, o.x);

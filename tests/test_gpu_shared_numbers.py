@@ -67,3 +67,53 @@ def test_nothing_but_scores_of_minus_infinity(kw):
     got = b.run().cpu()
     # the second sequence's prefix is the first one's too, whose last three tokens alone are left to it
     assert bool((got[1:3] == 0).all()) and torch.equal(got[3], want[3]) and bool(torch.isfinite(got[0]).all())
+
+
+def _same_but(b, got, want, rows):
+    """The other rows are what they were."""
+    keep = torch.ones(want.shape[:2], dtype=torch.bool)
+    for where in rows:
+        keep[where] = False
+    assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("kw", GEOMETRIES, ids=range(len(GEOMETRIES)))
+def test_an_own_part_of_one_token_that_is_no_number(kw):
+    """The first token behind a fork: its key is NaN, so is the row, however finite the prefix's part is."""
+    b = Batch([_same(160, [1, 1, 30, 0])], alone=[1, 40], **kw)
+    group = b.hq // b.hkv
+    want = b.run().cpu()
+    assert bool(torch.isfinite(want).all())
+    h = b.hkv - 1
+    heads = slice(h * group, (h + 1) * group)
+    for i, pos in ((1, 160), (4, 0)):
+        blk = b.tables[i][pos // b.bs]
+        b.k[b.layer, blk, h, pos % b.bs] = math.nan
+    got = b.run().cpu()
+    assert bool(got[1, heads].isnan().all()) and bool(got[4, heads].isnan().all())
+    _same_but(b, got, want, [(1, heads), (4, heads)])
+
+
+@pytest.mark.parametrize("kw", GEOMETRIES, ids=range(len(GEOMETRIES)))
+def test_a_prefix_of_one_token_that_is_no_number(kw):
+    b = Batch([_same(1, [0, 5, 40]), _same(64, [3, 3])], **kw)
+    group = b.hq // b.hkv
+    want = b.run().cpu()
+    for t in b.tables[:3]:  # every sequence holds a copy of the block the prefix ends in
+        b.k[b.layer, t[0], 0, 0] = math.nan
+    got = b.run().cpu()
+    assert bool(got[:3, :group].isnan().all())
+    _same_but(b, got, want, [(slice(0, 3), slice(0, group))])
+
+
+@pytest.mark.parametrize("kw", GEOMETRIES, ids=range(len(GEOMETRIES)))
+@pytest.mark.parametrize("shape", [dict(groups=[_same(300, [0, 20, 33]), _same(70, [1] * 20)], alone=[50]), dict(groups=[_same(4000, [5, 600])])], ids=["short", "long"])
+def test_queries_that_are_no_numbers(kw, shape):
+    b = Batch(**shape, **kw)
+    want = b.run().cpu()
+    b.q[1, 0, 7] = math.nan
+    b.q[0, b.hq - 1] = math.nan
+    b.q[-1] = math.nan
+    got = b.run().cpu()
+    assert bool(got[1, 0].isnan().all()) and bool(got[0, -1].isnan().all()) and bool(got[-1].isnan().all())
+    _same_but(b, got, want, [(1, 0), (0, b.hq - 1), (-1,)])

@@ -639,7 +639,8 @@ int psb_copy_blocks(void* const* pools, const int64_t* block_bytes, int32_t num_
  * once per group, through the table of its longest sequence (the first of them), and
  * a prefix ends with that sequence at the latest; a sequence shorter than its
  * prefix sees its own context_lens[b] tokens of it, one of none gets zeros.
- * Sequences of no group, or alone in one, are read on their own.
+ * Sequences of no group, or alone in one, are read on their own
+ * (cu_groups holds one element where num_groups is 0, and is never NULL).
  * Taken: bf16/f16, head_dim 64 or 128, up to 16 q heads per kv head, block sizes 16,
  * 32, 64 and multiples of 64, up to 2048 sequences and groups as long as 12 bytes a
  * sequence and 24 a group fit 33 KB (of 2048 sequences: 380 groups), query strides and bases

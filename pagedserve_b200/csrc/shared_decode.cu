@@ -1389,7 +1389,7 @@ extern "C" int psb_paged_decode_shared(const void* query, int64_t q_stride_b, in
       !(dtype == PSB_F32 || dtype == PSB_F16 || dtype == PSB_BF16) || !(scale > 0.f) || !(scale < INFINITY))
     return PSB_ERR_INVALID;
   if (batch == 0) return PSB_OK;
-  if (!query || !out || !k_cache || !v_cache || !block_tables || !context_lens || (num_groups > 0 && (!cu_groups || !prefix_lens)))
+  if (!query || !out || !k_cache || !v_cache || !block_tables || !context_lens || !cu_groups || (num_groups > 0 && !prefix_lens))
     return PSB_ERR_INVALID;
   auto al16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
   if (!takes(batch, num_groups, q_heads, num_kv_heads, head_dim, block_size, dtype, max_context) || !al16(query) || !al16(k_cache) ||

@@ -1284,8 +1284,10 @@ def paged_decode_shared(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     if need == 0 or (k_cache.data_ptr() | v_cache.data_ptr()) & 15 or nl * nb * hkv > 0x7fffffff:
         _cuda_index(q3, k_cache, v_cache, block_tables, context_lens, cu_groups, prefix_lens, out, error_flag)
         with torch.cuda.device(q3.device):
-            paged_decode(q3, k_cache, v_cache, block_tables, context_lens, layer, scale=scale, out=o3, max_context=max_context,
-                         error_flag=error_flag)
+            # paged_decode may read lengths and tables while the library's launch in front of it still writes them: the
+            # copy of the lengths is the ordinary work that has to lie between
+            paged_decode(q3, k_cache, v_cache, block_tables, context_lens.clone(), layer, scale=scale, out=o3,
+                         max_context=max_context, error_flag=error_flag)
         return out
     qs = q3.stride()
     if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or qs[0] <= 0 or qs[1] <= 0 or q3.data_ptr() & 15:

@@ -2,9 +2,13 @@
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
-from pagedserve_b200 import _native
+import pytest
+import torch
+
+from pagedserve_b200 import _native, ops
 
 
 def _buffer():
@@ -19,3 +23,36 @@ def test_no_groups_need_their_one_bound_all_the_same():
                                                        None, None)
     assert call(None, None) == _native.PSB_ERR_INVALID and call(None, p) == _native.PSB_ERR_INVALID
     assert call(p, None) == _native.PSB_ERR_WORKSPACE  # the lengths of no prefix may be missing
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+@pytest.fixture
+def one_by_one(monkeypatch):
+    """paged_decode's arguments where paged_decode_shared leaves a batch to it, on the CPU."""
+    calls = []
+
+    def decode(q, k, v, tables, lens, layer, **kw):
+        calls.append(dict(kw, q=q, tables=tables, lens=lens, layer=layer))
+        kw["out"].zero_()
+    monkeypatch.setattr(ops, "_cuda_index", lambda *tensors: 0)
+    monkeypatch.setattr(ops, "paged_decode", decode)
+    monkeypatch.setattr(torch.cuda, "device", lambda *_: contextlib.nullcontext())
+    return calls
+
+
+def _batch(d=96, batch=3):
+    pool = torch.zeros(2, 9, 2, 16, d, dtype=torch.bfloat16)
+    return [torch.zeros(batch, 14, d, dtype=torch.bfloat16), pool, pool, torch.zeros(batch, 4, dtype=torch.int32), _i32([5 + i % 7 for i in range(batch)]),
+            _i32([0, 2]), _i32([3]), 1]
+
+
+@pytest.mark.parametrize("args", [_batch(), _batch(64, 2049)], ids=["dims", "sequences"])
+def test_what_is_answered_one_by_one_has_work_of_the_stream_in_front(one_by_one, args):
+    """paged_decode reads lengths before its predecessor has ended: it gets a copy of them, which is made behind that."""
+    out = ops.paged_decode_shared(*args)
+    call, = one_by_one
+    assert torch.equal(call["lens"], args[4]) and call["lens"].data_ptr() != args[4].data_ptr()
+    assert call["layer"] == 1 and call["tables"] is args[3] and call["out"].data_ptr() == out.data_ptr() and call["max_context"] == 64

@@ -1235,6 +1235,9 @@ def paged_decode_shared(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     head, blocks of 16, 32, 64 or a multiple of 64 tokens, up to 2048 sequences
     (12 bytes a sequence and 24 a group have to fit 33 KB); the rest is answered by
     ``paged_decode``, each sequence on its own.  ``scale`` must be positive.
+    ``workspace``: ``decode_shared_workspace_bytes`` of scratch (where that is 0,
+    ``decode_workspace_bytes``; of less there, the call takes its own); without it the
+    scratch comes from PyTorch's allocator.  Calls that may overlap need one each.
     """
     if query.is_cuda:
         done = (_native._calls or _native.calls()).decode_shared(query, k_cache, v_cache, block_tables, context_lens, cu_groups,
@@ -1282,12 +1285,18 @@ def paged_decode_shared(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     context_lens, cu_groups, prefix_lens = context_lens.contiguous(), cu_groups.contiguous(), prefix_lens.contiguous()
     need = decode_shared_workspace_bytes(bsz, groups, hq, hkv, d, bs, max_context, q3.dtype)
     if need == 0 or (k_cache.data_ptr() | v_cache.data_ptr()) & 15 or nl * nb * hkv > 0x7fffffff:
-        _cuda_index(q3, k_cache, v_cache, block_tables, context_lens, cu_groups, prefix_lens, out, error_flag)
+        _cuda_index(q3, k_cache, v_cache, block_tables, context_lens, cu_groups, prefix_lens, out, workspace, error_flag)
+        # scratch as of the calls that share: the caller's, or the allocator's (paged_decode's own is one for all streams)
+        need = decode_workspace_bytes(bsz, hq, hkv, d, bs, max_context, q3.dtype)
+        if workspace is not None:
+            _check_workspace(workspace)
+        if workspace is None or workspace.nbytes < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q3.device)
         with torch.cuda.device(q3.device):
             # paged_decode may read lengths and tables while the library's launch in front of it still writes them: the
             # copy of the lengths is the ordinary work that has to lie between
             paged_decode(q3, k_cache, v_cache, block_tables, context_lens.clone(), layer, scale=scale, out=o3,
-                         max_context=max_context, error_flag=error_flag)
+                         max_context=max_context, workspace=workspace, error_flag=error_flag)
         return out
     qs = q3.stride()
     if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or qs[0] <= 0 or qs[1] <= 0 or q3.data_ptr() & 15:

@@ -53,3 +53,27 @@ def test_directly_behind_a_step_that_writes_tables(d, batch):
     for i, (tables, ctx) in enumerate(seen):
         want = ops.paged_decode(q[i], k, v, tables, ctx, 0)
         assert torch.equal(got[i], want) and int(ctx[0]) == 7 * (i // 2) + 4 + 3 * (i % 2)
+
+
+@pytest.mark.parametrize("batch", [dict(hq=4, hkv=2, d=96), dict(hq=14, hkv=2, dtype=torch.float32), dict(hq=4, hkv=2)], ids=["dims", "f32", "plan"])
+def test_two_streams_at_once(batch):
+    """Calls on two streams, and one with a workspace of the caller's: each has its own scratch."""
+    from pagedserve_b200 import ops
+    pairs = batch == dict(hq=4, hkv=2)
+    cases = [Batch([_same(17, [1500 + g % 60, 3]) for g in range(1100 if pairs else 20)], seed=s, **batch) for s in (1, 2)]
+    args = [(b.q.cuda(), b.k.cuda(), b.v.cuda(), b.table.cuda(), _i32(b.lens), _i32(b.cu), _i32(b.prefix), b.layer) for b in cases]
+    for b in cases:
+        assert ops.decode_shared_workspace_bytes(len(b.lens), len(b.prefix), b.hq, b.hkv, b.d, b.bs, b.table.shape[1] * b.bs, b.dtype) == 0
+    b = cases[0]
+    need = ops.decode_workspace_bytes(len(b.lens), b.hq, b.hkv, b.d, b.bs, b.table.shape[1] * b.bs, b.dtype)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    want = [ops.paged_decode(*a[:5], a[7]) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    for _ in range(10):
+        got = []
+        for s, a, w in zip(streams, args, (ws, None)):
+            with torch.cuda.stream(s):
+                got.append(ops.paged_decode_shared(*a, workspace=w))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))

@@ -56,3 +56,17 @@ def test_what_is_answered_one_by_one_has_work_of_the_stream_in_front(one_by_one,
     call, = one_by_one
     assert torch.equal(call["lens"], args[4]) and call["lens"].data_ptr() != args[4].data_ptr()
     assert call["layer"] == 1 and call["tables"] is args[3] and call["out"].data_ptr() == out.data_ptr() and call["max_context"] == 64
+
+
+def test_scratch_of_what_is_answered_one_by_one(one_by_one, monkeypatch):
+    """The caller's where it is large enough, else the allocator's: never the buffer that every stream's paged_decode uses."""
+    args = _batch()
+    need = ops.decode_workspace_bytes(3, 14, 2, 96, 16, 64, torch.bfloat16)
+    assert need > 0
+    own, small = torch.empty(need, dtype=torch.uint8), torch.empty(16, dtype=torch.uint8)
+    for given in (own, small, None):
+        ops.paged_decode_shared(*args, workspace=given)
+    first, second, third = (c["workspace"] for c in one_by_one)
+    assert first is own and second is not small and second.nbytes >= need and third.nbytes >= need
+    with pytest.raises(ValueError, match="16 bytes"):
+        ops.paged_decode_shared(*args, workspace=torch.empty(need + 8, dtype=torch.uint8)[8:])

@@ -666,6 +666,14 @@ int psb_paged_decode_shared(const void* query, int64_t q_stride_b, int64_t q_str
                             void* workspace, size_t workspace_bytes, int32_t* error_flag, psb_stream_t stream);
 
 /*
+ * check_groups: flags what psb_paged_decode_shared would flag of cu_groups and
+ * prefix_lens (PSB_DEVERR_SEQLENS, PSB_DEVERR_CONTEXT), for a batch that
+ * psb_paged_decode answers in its place.  An ordinary launch.
+ */
+int psb_check_groups(const int32_t* cu_groups, const int32_t* prefix_lens, int32_t batch, int32_t num_groups,
+                     int32_t* error_flag, psb_stream_t stream);
+
+/*
  * verify_tokens: drafted tokens against the target's probabilities, with given random
  * numbers; without drafts, sampling at a temperature.
  *

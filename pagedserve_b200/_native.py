@@ -135,6 +135,7 @@ SIGNATURES = {
     "psb_verify_tokens": (ctypes.c_int, [
         _c_void_p, _i64, _i32, _i32, _i32, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p, _i64, _i32,
         _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p, _c_void_p]),
+    "psb_check_groups": (ctypes.c_int, [_c_void_p, _c_void_p, _i32, _i32, _c_void_p, _c_void_p]),
     "psb_verify_tokens_workspace_size": (_sz, [_i32]),
 }
 

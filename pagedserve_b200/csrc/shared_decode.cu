@@ -1282,6 +1282,17 @@ __global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const SharedP
   }
 }
 
+// The groups' checks by themselves, as build_plan makes them.
+__global__ void check_groups_kernel(const int32_t* cu, const int32_t* prefix, int32_t batch, int32_t groups, int32_t* err) {
+  int32_t bits = 0;
+  for (int g = threadIdx.x; g <= groups; g += blockDim.x) {
+    const int a = cu[g], prev = g == 0 ? 0 : cu[g - 1];
+    if (a < prev || prev < 0 || a > batch) bits |= PSB_DEVERR_SEQLENS;
+    if (g < groups && prefix[g] < 0) bits |= PSB_DEVERR_CONTEXT;
+  }
+  if (bits != 0) flag_error(err, bits);
+}
+
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
@@ -1370,6 +1381,15 @@ int launch(SharedParams p, int num_layers, cudaStream_t s) {
 }  // namespace psb
 
 using namespace psb;
+
+extern "C" int psb_check_groups(const int32_t* cu_groups, const int32_t* prefix_lens, int32_t batch, int32_t num_groups, int32_t* error_flag,
+                                psb_stream_t stream) {
+  if (batch < 0 || num_groups < 0 || !cu_groups || (num_groups > 0 && !prefix_lens)) return PSB_ERR_INVALID;
+  if (!error_flag) return PSB_OK;
+  discard_stale_error();
+  check_groups_kernel<<<1, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(cu_groups, prefix_lens, batch, num_groups, error_flag);
+  return check_launch();
+}
 
 extern "C" size_t psb_paged_decode_shared_workspace_size(int32_t batch, int32_t num_groups, int32_t q_heads, int32_t num_kv_heads,
                                                          int32_t head_dim, int32_t block_size, int32_t max_context, int32_t dtype) {

@@ -1285,7 +1285,10 @@ def paged_decode_shared(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     context_lens, cu_groups, prefix_lens = context_lens.contiguous(), cu_groups.contiguous(), prefix_lens.contiguous()
     need = decode_shared_workspace_bytes(bsz, groups, hq, hkv, d, bs, max_context, q3.dtype)
     if need == 0 or (k_cache.data_ptr() | v_cache.data_ptr()) & 15 or nl * nb * hkv > 0x7fffffff:
-        _cuda_index(q3, k_cache, v_cache, block_tables, context_lens, cu_groups, prefix_lens, out, workspace, error_flag)
+        dev = _cuda_index(q3, k_cache, v_cache, block_tables, context_lens, cu_groups, prefix_lens, out, workspace, error_flag)
+        if error_flag is not None:
+            _call(dev, _native.load().psb_check_groups, "paged_decode_shared", cu_groups.data_ptr(), prefix_lens.data_ptr(), bsz,
+                  groups, error_flag.data_ptr())
         # scratch as of the calls that share: the caller's, or the allocator's (paged_decode's own is one for all streams)
         need = decode_workspace_bytes(bsz, hq, hkv, d, bs, max_context, q3.dtype)
         if workspace is not None:

@@ -77,3 +77,22 @@ def test_two_streams_at_once(batch):
                 got.append(ops.paged_decode_shared(*a, workspace=w))
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("d", [64, 96])
+@pytest.mark.parametrize("cu,prefix,bits", [([0, 3, 5], [100, 80], 0), ([0, 5, 3], [100, 80], 32), ([-1, 3, 5], [100, 80], 32), ([0, 3, 99], [100, 80], 32),
+                                            ([0, 3, 5], [-5, 80], 4), ([0, 7, 5], [4, -1], 36), ([0], [], 0), ([7], [], 32), ([-1], [], 32)])
+def test_malformed_groups_are_flagged(d, cu, prefix, bits):
+    """Whichever kernel answers: the flag is the same, and every sequence is read on its own."""
+    from pagedserve_b200 import ops
+    b = Batch([_same(100, [20, 40, 3]), _same(80, [2, 2])], alone=[33], d=d, hq=4)
+    want, tol = b.expected()
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = ops.paged_decode_shared(b.q.cuda(), b.k.cuda(), b.v.cuda(), b.table.cuda(), _i32(b.lens), _i32(cu), _i32(prefix), b.layer, error_flag=err)
+    assert int(err) == bits and ((got.cpu().double() - want).abs() <= tol).all()
+    many = torch.arange(1000, dtype=torch.int32, device="cuda")  # more groups than threads
+    err.zero_()
+    many[701] = 5
+    ops.paged_decode_shared(b.q.cuda(), b.k.cuda(), b.v.cuda(), b.table.cuda(), _i32(b.lens), many.clamp(max=6), torch.zeros(999, dtype=torch.int32, device="cuda"),
+                            b.layer, error_flag=err)
+    assert int(err) == 32

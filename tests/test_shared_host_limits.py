@@ -70,3 +70,22 @@ def test_scratch_of_what_is_answered_one_by_one(one_by_one, monkeypatch):
     assert first is own and second is not small and second.nbytes >= need and third.nbytes >= need
     with pytest.raises(ValueError, match="16 bytes"):
         ops.paged_decode_shared(*args, workspace=torch.empty(need + 8, dtype=torch.uint8)[8:])
+
+
+def test_groups_are_checked_where_each_sequence_is_answered_by_itself(one_by_one, monkeypatch):
+    args, seen = _batch(), []
+    monkeypatch.setattr(ops, "_call", lambda dev, fn, what, *a: seen.append(a))
+    err = torch.zeros(1, dtype=torch.int32)
+    ops.paged_decode_shared(*args, error_flag=err)
+    assert seen == [(args[5].data_ptr(), args[6].data_ptr(), 3, 1, err.data_ptr())]
+    ops.paged_decode_shared(*args)  # nobody to tell
+    assert len(seen) == 1 and len(one_by_one) == 2
+
+
+def test_check_groups_refuses():
+    lib = _native.load()
+    keep, p = _buffer()
+    inv = _native.PSB_ERR_INVALID
+    assert lib.psb_check_groups(None, p, 1, 1, p, None) == inv and lib.psb_check_groups(p, None, 1, 1, p, None) == inv
+    assert lib.psb_check_groups(p, p, -1, 1, p, None) == inv and lib.psb_check_groups(p, p, 1, -1, p, None) == inv
+    assert lib.psb_check_groups(p, None, 1, 0, None, None) == 0

@@ -22,11 +22,16 @@
 // sample in a hundred at V = 152 K.  Weights in 64 bits for every row cost a multiple
 // of the read, so they are used where fp32 leaves the answer open.  An fp32 weight
 // 2^(x c - octave) (c = log2(e) / t, the octave an integer near the maximum's, so that
-// parts are joined exactly) is off by 2^-19 of itself at most, but for those below
-// 2^-32: rounding the exponent, below 32, 2^-20 ln 2; rounding c, 32 times 2^-25 ln 2
-// next to the maximum's; the exponential 2^-22; the sum of a piece's eight three times
-// 2^-24.  All further sums are in 64 bits.  A draft's test or a sample closer to its
-// border than twice that is done again in 64 bits, as is what is drawn from
+// parts are joined exactly), up to 31 octaves below the maximum's, is off by 1.08e-6 +
+// 21.5 dc of itself at most: rounding the exponent, below 32, 2^-20 ln 2; c, which is off by
+// dc of itself (2^-24 at most, known for each temperature), 31 dc ln 2 next to the
+// maximum's; the exponential 2^-22; the sum of a piece's eight three times 2^-24.
+// Those further below are off by more (4.3e-6 down to 62 octaves; what is left is nothing)
+// but they are few: of V, 2^-31 V next to the maximum's.  fp32 is asked only about sums
+// of 2^-26 V and more of it (of the whole row, V up to 2^25; of a sample, by its target),
+// where these are 2^-5 at most of what is compared, and cost it another 2e-7 with the octave's
+// rounding.  All further sums are in 64 bits.  A draft's test or a sample closer to its
+// border than twice all that is done again in 64 bits, as is what is drawn from
 // max(p - q, 0), where little may be left of much.
 #include <cooperative_groups.h>
 
@@ -49,7 +54,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCtas = 16;      // CTAs of a cluster
 constexpr int kMaxRows = 8;       // rows read before the drafts among them are looked at, at most
 constexpr int kOwnElems = 96;     // of the vocabulary per thread of a sequence up to which it does its 64-bit work itself
-constexpr float kErr = 1.8e-6f;   // of an fp32 weight or a sum of them, relative
+constexpr double kErr = 1.3e-6, kErrOfC = 21.5;  // of a sum of fp32 weights, relative: kErr + kErrOfC times c's
+constexpr double kLeast = 1.0 / (1 << 26);       // of the largest weight, times the vocabulary: sums that this holds for
+constexpr int kMostFast = 1 << 25;               // vocabulary
 constexpr float kLargest = 1 << 20;  // octaves that logits may span for fp32
 
 struct VerifyParams {
@@ -605,8 +612,11 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
   const double c = exponent_of(temp);
   const bool hot = c > 0;
   Fast fast(c);
-  // whether fp32 weights of a row with this maximum are good to kErr
-  auto in_fp32 = [&](float m) { return c > 1e-30 && c < 1e30 && fabsf(m * fast.c) < kLargest; };
+  // whether fp32 weights of a row with this maximum are good to error()
+  auto in_fp32 = [&](float m) { return c > 1e-30 && c < 1e30 && fabsf(m * fast.c) < kLargest && p.vocab <= kMostFast; };
+  auto error = [&]() {  // (c is log2(e) / temp: no division)
+    return kErr + kErrOfC * 0.6931471805599453 * fabs(fma(static_cast<double>(fast.c), static_cast<double>(temp), -1.4426950408889634));
+  };
 
   // ---- the rows, until a draft is not taken ---------------------------------------
   // rows behind a rejection are read for nothing, but a batch takes 5 us however few its rows
@@ -722,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
             const bool sure = exact >= 0 && lane == from;
             const double sum = sure ? exact : ex.from_fast(part.sum, part.octave, part.max, fast.c);
             state = uq * sum < e ? 1 : 0;
-            if (!sure && (!in_fp32(part.max) || fabs(uq * sum - e) <= 2.0 * kErr * e)) state = 2;
+            if (!sure && (!in_fp32(part.max) || fabs(uq * sum - e) <= 2.0 * error() * e)) state = 2;
           }
         }
         const uint32_t other = __ballot_sync(0xffffffffu, lane >= from && lane < rows && state != 1);
@@ -790,8 +800,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
   const int d = next >= 0 && next < p.vocab ? static_cast<int>(next) : -1;
   const int mode = d < 0 ? kWhole : kProbs ? kRest : kWithout;
   const double u = static_cast<double>(__ldg(p.uniforms + 2 * static_cast<int64_t>(stop) + 1));
-  if (mode != kRest && in_fp32(top) && u >= 1e-18) {
-    // from the sums that are there; (a target of 0 falls on the first token of any weight, however small)
+  if (mode != kRest && in_fp32(top)) {
+    // from the sums that are there
     if (tid < wpr) s_of_part[tid] = s_part[in_batch][tid].sum * power(s_part[in_batch][tid].octave - at_stop.octave);
     fast.unit(at_stop.octave);
     const int of_d = mode == kWithout ? (d + row.skip) / n : -1;
@@ -822,9 +832,9 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyParams 
       if (tid < kWarps) s_sums.warp[tid] = tid < wpr ? s_of_part[tid] : 0.0;
       sums = cl.exchange();
     }
-    const double target = u * all_of(sums, ctas), room = 2.0 * kErr * target;
+    const double target = u * all_of(sums, ctas), room = 2.0 * error() * target;
     double run = 0;
-    if (first_above(sums, ctas, target, run) == me) {
+    if (target >= kLeast * p.vocab && first_above(sums, ctas, target, run) == me) {
       const int w = first_above(s_of_part, wpr, target, run);
       if (w >= 0) {
         const int a0 = part_at(w), a1 = part_at(w + 1);

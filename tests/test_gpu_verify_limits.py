@@ -64,3 +64,56 @@ def test_neighbours_of_the_maximum_at_low_temperatures():
     for u1 in (0.0, 0.5, 0.99):
         u = torch.full((8, 2), u1)
         _check(rows, torch.zeros(8, dtype=torch.int64), list(range(9)), u, heat, None)
+
+
+def _borders():
+    """Rows whose fp32 weights are off by nearly all that they can be, with random numbers next to a border.
+
+    A logit of 0 at the end, equal ones some 60 octaves below it in front: the k-th of them ends at k w of the sum.  Their
+    fp32 weight is off by the rounding of c = log2(e) / t, times 60, and by that of their exponent: temperatures and logits
+    are looked for where both are large and of one sign.  The random number is a hair beside the border."""
+    import numpy as np
+    rng = np.random.default_rng(0)
+    found = []
+    heats = np.float32(1.4426950408889634 / (1.0 + rng.random(4000) / 64))
+    c = 1.4426950408889634 / heats.astype(np.float64)
+    of_c = c.astype(np.float32).astype(np.float64) / c - 1
+    for sign in (1, -1):  # weights too large, too small
+        for i in np.argsort(sign * of_c)[:12]:  # c32 below c: weights above theirs
+            x = -(np.float32(62.0) + rng.random(4000).astype(np.float32) * 2)
+            y = x.astype(np.float64) * c[i].astype(np.float32).astype(np.float64)
+            up = y.astype(np.float32).astype(np.float64) - y
+            x = x[np.argmax(sign * up)]
+            w = np.exp(np.float64(x) / np.float64(heats[i]))
+            total = 1 + 12800 * w
+            for k in range(24, 48):  # the random number that is closest to the border on the wrong side
+                u = np.float32(k * w / total)
+                while sign * (np.float64(u) * total - k * w) <= 2e-8 * k * w:
+                    u = np.nextafter(u, np.float32(sign))
+                if sign * (np.float64(u) * total / (k * w) - 1) < 7e-8:
+                    found.append((float(heats[i]), float(x), float(u)))
+                    break
+    return found
+
+
+def test_next_to_borders_where_fp32_is_worst():
+    cases = _borders()
+    assert len(cases) > 16
+    cases = (cases * 10)[:150]  # so many that one CTA has a row: its first warp's first tokens are cut no further
+    logits = torch.full((len(cases), 12801), 0.0)
+    u = torch.zeros(len(cases), 2)
+    for r, (_, x, u1) in enumerate(cases):
+        logits[r, :12800] = x
+        u[r, 1] = u1
+    new, _ = _check(logits, torch.zeros(len(cases), dtype=torch.int64), list(range(len(cases) + 1)), u, torch.tensor([h for h, _, _ in cases]), None)
+    assert bool((new >= 23).all()) and bool((new <= 48).all())
+
+
+@pytest.mark.parametrize("probs", [None, torch.float32])
+@pytest.mark.parametrize("u1", [0.0, 1e-30, 1e-18, 2.0 ** -40, 1e-9, 1e-6, 1e-4, 2e-3, 1 - 2.0 ** -24])
+def test_small_random_numbers(u1, probs):
+    """They fall on the first tokens, however little weight those have."""
+    for heat, vocab, ns in ((0.25, 3001, [1, 3, 2, 5] * 4), (1.0, 60000, [1, 2] * 3), (0.7, 777, [2] * 40)):
+        args = list(_inputs(ns, vocab, torch.float32, probs, 23, heat=torch.full((len(ns),), heat), spread=4.0))
+        args[3][:, 1] = u1
+        _check(*args)

@@ -257,6 +257,7 @@ struct Sums {  // in shared memory
   double warp[kWarps];
   double ctas[2][kMaxCtas];  // the CTAs' sums, two exchanges in turn
   double table[16];          // 2^(i / 16)
+  int open[kWarps][4], n_open[kWarps];  // elements of a warp's part that wait for the row's sum
 };
 
 __device__ __forceinline__ void fill_table(Sums& s) {
@@ -466,10 +467,11 @@ __device__ __forceinline__ Row<T> row_of(const VerifyParams& p, int r) {
 enum Mode { kWhole = 0, kWithout = 1, kRest = 2 };
 
 // The new token of row ``r`` in 64 bits, by a cluster.  ``z``: the row's sum in 64 bits,
-// or in fp32.  max(e - q z, 0) needs it before the first weight; summed are e and q
-// apart where e > q z by the fp32 z, so one pass gives z and, with it, the sum.  (An element
-// on the wrong side of that is within 4e-6 of e = q z: the sum is off by less than
-// 1e-11 of itself, one sample in 10^6.)
+// or in fp32.  max(e - q z, 0) needs it before the first weight; summed are e and
+// q apart where e > q z by the fp32 z, so one pass gives z and, with it, the sum.  Elements
+// that z's error (2.7e-6) leaves open, within 2^-18 of e (one in a row of 152 K, or all of them
+// where q is next to p), wait until z is known, four a warp; where one meets a fifth the sum is
+// taken again.  (Counted by the fp32 z, they misplaced what is drawn where little is left: 1.5 us of 36.)
 template <typename T, typename Q>
 __device__ void draw(const VerifyParams& p, Cluster& cl, int r, int d, int mode, float top, double c, double z) {
   constexpr bool kProbs = !std::is_same<Q, NoProbs>::value;
@@ -515,6 +517,8 @@ __device__ void draw(const VerifyParams& p, Cluster& cl, int r, int d, int mode,
   while (true) {
     if (kProbs && mode == kRest) {
       double e = 0, q = 0, whole = 0;
+      if (lane == 0) cl.sums->n_open[warp] = 0;
+      __syncwarp();
       row.template each<1>(c0, c1, [&](const Piece<T>& x, int k) {
         double w[n], v[n];
         ex.piece(x, w);
@@ -522,18 +526,36 @@ __device__ void draw(const VerifyParams& p, Cluster& cl, int r, int d, int mode,
 #pragma unroll
         for (int i = 0; i < n; ++i) {
           whole += w[i];
-          if (w[i] > v[i] * z) {
+          const int left = __double2hiint(fma(-v[i], z, w[i]));  // (sign and exponent are enough)
+          if ((left & 0x7fffffff) + (18 << 20) <= __double2hiint(w[i])) {
+            const int at = atomicAdd(&cl.sums->n_open[warp], 1);
+            if (at < 4) cl.sums->open[warp][at] = row.first(k) + i;
+          } else if (left >= 0) {
             e += w[i];
             q += v[i];
           }
         }
       });
       z = all_of(cl.exchange(warp_sum(whole)), cl.ctas);
-      sums = cl.exchange(fma(-z, warp_sum(q), warp_sum(e)));
+      double rest = fma(-z, q, e);
+      const int n_open = cl.sums->n_open[warp];
+      if constexpr (kProbs) {
+        if (lane < min(n_open, 4)) {
+          const int d0 = cl.sums->open[warp][lane];
+          rest += fmax(fma(-z, prob_at<Q>(p.probs, static_cast<int64_t>(r) * p.probs_stride + d0), ex.weight(Elem<T>::to_float(row.x[d0]))), 0.0);
+        }
+      }
+      if (n_open > 4) rest = __longlong_as_double(0x7ff8000000000000ll);  // (no number: what every CTA sees of it)
+      sums = cl.exchange(warp_sum(rest));
+      all = all_of(sums, cl.ctas);
+      if (all != all) {
+        sums = cl.exchange(sum_of(row, weights, c0, c1));
+        all = all_of(sums, cl.ctas);
+      }
     } else {
       sums = cl.exchange(sum_of(row, weights, c0, c1));
+      all = all_of(sums, cl.ctas);
     }
-    all = all_of(sums, cl.ctas);
     if (all > 0 || mode == kWhole) break;
     mode = kWhole;  // nothing is left of p: from p itself
   }

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_gpu_verify_tokens import _check, _inputs
+from tests.test_gpu_verify_tokens import _check, _inputs, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -117,3 +117,32 @@ def test_small_random_numbers(u1, probs):
         args = list(_inputs(ns, vocab, torch.float32, probs, 23, heat=torch.full((len(ns),), heat), spread=4.0))
         args[3][:, 1] = u1
         _check(*args)
+
+
+@pytest.mark.parametrize("near", [1e-7, 1e-6, 1e-5, 1e-4, 1e-2])
+@pytest.mark.parametrize("batch,vocab", [(60, 400), (5, 9001), (80, 50000)])
+def test_drafts_from_nearly_the_target(near, batch, vocab):
+    """Probabilities within ``near`` of the target's, drafts refused all the same: the token is drawn from the little that is left.
+
+    The target and its weights' sum are good to 3e-12 each, against what is left in all, about near / 4; next to a border
+    of the 64-bit rule by no more than that a token's neighbour may be drawn."""
+    g = torch.Generator().manual_seed(vocab)
+    logits = torch.randn(2 * batch, vocab, generator=g) * 1.5
+    p = torch.softmax(logits.double() / 0.9, -1)
+    probs = (p * (1 + near * (2 * torch.rand(p.shape, generator=g, dtype=torch.float64) - 1))).float()
+    over = (probs.double() / p - 1)[::2]
+    tokens = torch.zeros(2 * batch, dtype=torch.int64)
+    tokens[1::2] = over.argmax(-1)
+    u = torch.rand(2 * batch, 2, generator=g)
+    u[:, 0] = 1 - 2.0 ** -24
+    assert bool((over.amax(-1) > 1.2e-7).all())  # u0 q is above p, by 2^-24 of it at least
+    heat = torch.full((batch,), 0.9)
+    p = torch.softmax(logits.double() / heat[0].double(), -1)
+    new, counts = _run(logits, tokens, list(range(0, 2 * batch + 1, 2)), u, heat, probs)
+    assert counts.tolist() == [1] * batch
+    w = (p - probs.double()).clamp(min=0)[::2]
+    c = w.cumsum(-1)
+    all_, at = c[:, -1], new[::2, None]
+    assert bool((w.gather(1, at)[:, 0] > 0).all())
+    target, room = u[::2, 1].double() * all_, 2 * 6e-12 + 1e-9 * all_
+    assert bool((c.gather(1, at)[:, 0] + room > target).all()) and bool(((c - w).gather(1, at)[:, 0] - room <= target).all())

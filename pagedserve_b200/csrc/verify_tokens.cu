@@ -583,9 +583,9 @@ __device__ void draw(const VerifyParams& p, Cluster& cl, int r, int d, int mode,
 }
 
 // log2(e) / temperature; 0 for temperature 0 and what is taken for it: no temperature
-// (NaN, negative, infinite), or one whose inverse fp32 does not hold.
+// (NaN, negative, infinite).
 __device__ __forceinline__ double exponent_of(float temperature) {
-  return temperature >= 1e-37f && temperature < INFINITY ? 1.4426950408889634 / static_cast<double>(temperature) : 0.0;
+  return temperature > 0.f && temperature < INFINITY ? 1.4426950408889634 / static_cast<double>(temperature) : 0.0;
 }
 
 __device__ __forceinline__ bool finite(float m) { return m > -INFINITY && m < INFINITY; }

@@ -146,3 +146,19 @@ def test_drafts_from_nearly_the_target(near, batch, vocab):
     assert bool((w.gather(1, at)[:, 0] > 0).all())
     target, room = u[::2, 1].double() * all_, 2 * 6e-12 + 1e-9 * all_
     assert bool((c.gather(1, at)[:, 0] + room > target).all()) and bool(((c - w).gather(1, at)[:, 0] - room <= target).all())
+
+
+@pytest.mark.parametrize("heat", [1e-37, 1.1e-38, 1e-39, 1e-42, 2.0 ** -149])
+@pytest.mark.parametrize("batch", [3, 200])
+def test_the_least_temperatures(heat, batch):
+    """Any temperature above 0 is one: equal maxima share p, and logits that differ by the least fp32 values by e or so."""
+    vocab = 70000 if batch == 200 else 50
+    logits = torch.full((batch, vocab), -2.0)
+    logits[:, [7, 20, 33]] = 3.0
+    # all tokens about 0, the first ones a few temperatures below
+    logits[1::2] = -1e30
+    logits[1::2, 5:15] = -float(torch.tensor(heat)) * torch.arange(9, -1, -1, dtype=torch.float64).float()
+    u = torch.rand(batch, 2, generator=torch.Generator().manual_seed(4))
+    args = (logits, torch.zeros(batch, dtype=torch.int64), list(range(batch + 1)), u, torch.full((batch,), heat), None)
+    new, _ = _check(*args)
+    assert batch == 3 or len(set(new[::2].tolist())) == 3 and len(set(new[1::2].tolist())) > 2

@@ -799,6 +799,11 @@ def decode_int4_workspace_bytes(batch: int, q_heads: int, hkv: int, head_dim: in
                                                         dtype_code(dtype)))
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    return a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes and a.device == b.device
+
+
 def _check_workspace(workspace: torch.Tensor) -> None:
     if not workspace.is_contiguous() or workspace.data_ptr() % 16:
         raise ValueError("workspace must be contiguous and start on 16 bytes")
@@ -1381,6 +1386,9 @@ def verify_tokens(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
             raise ValueError("out must be contiguous (new_tokens [T] int64, counts [B] int32)")
         if t and new.data_ptr() == tokens.data_ptr():
             raise ValueError("new_tokens may not be tokens itself")
+        for x in (new, counts):
+            if any(_overlap(x, y) for y in (tokens, cu_seqlens, uniforms, temperature, counts if x is new else new)):
+                raise ValueError("out may not overlap the inputs, nor each other")
     dev = _cuda_index(logits, tokens, cu_seqlens, uniforms, temperature, draft_probs, new, counts, error_flag)
     workspace = torch.empty(max(1, 2 * b), dtype=torch.int64, device=logits.device)  # 16 bytes a sequence
     _call(dev, _native.load().psb_verify_tokens, "verify_tokens",

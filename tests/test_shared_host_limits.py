@@ -89,3 +89,17 @@ def test_check_groups_refuses():
     assert lib.psb_check_groups(None, p, 1, 1, p, None) == inv and lib.psb_check_groups(p, None, 1, 1, p, None) == inv
     assert lib.psb_check_groups(p, p, -1, 1, p, None) == inv and lib.psb_check_groups(p, p, 1, -1, p, None) == inv
     assert lib.psb_check_groups(p, None, 1, 0, None, None) == 0
+
+
+def test_verify_tokens_writes_over_none_of_its_inputs():
+    logits, u, heat = torch.zeros(5, 30), torch.zeros(5, 2), torch.ones(2)
+    ids, bounds = torch.zeros(16, dtype=torch.int64), torch.zeros(16, dtype=torch.int32)
+    bounds[:3] = _i32([0, 2, 5])
+    new, counts = torch.zeros(5, dtype=torch.int64), torch.zeros(2, dtype=torch.int32)
+    for out in ((ids[1:6], counts), (ids[4:9], counts), (new, bounds[1:3]), (new, bounds[2:4]), (u.view(torch.int64).view(-1), counts),
+                (new, heat.view(torch.int32)), (new, new.view(torch.int32)[4:6])):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.verify_tokens(logits, ids[:5], bounds[:3], u, heat, out=out)
+    for out in ((ids[5:10], counts), (new, bounds[3:5])):  # side by side is apart
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.verify_tokens(logits, ids[:5], bounds[:3], u, heat, out=out)

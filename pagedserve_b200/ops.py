@@ -801,7 +801,8 @@ def decode_int4_workspace_bytes(batch: int, q_heads: int, hkv: int, head_dim: in
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two contiguous tensors share memory."""
-    return a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes and a.device == b.device
+    return (a.nbytes > 0 and b.nbytes > 0 and a.device == b.device
+            and a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes)
 
 
 def _check_workspace(workspace: torch.Tensor) -> None:

@@ -103,3 +103,6 @@ def test_verify_tokens_writes_over_none_of_its_inputs():
     for out in ((ids[5:10], counts), (new, bounds[3:5])):  # side by side is apart
         with pytest.raises(ValueError, match="CUDA"):
             ops.verify_tokens(logits, ids[:5], bounds[:3], u, heat, out=out)
+    with pytest.raises(ValueError, match="CUDA"):  # nothing shares nothing
+        ops.verify_tokens(logits[:0], ids[4:4], torch.zeros(3, dtype=torch.int32), u[:0], heat, out=(ids[6:6], counts))
+    assert not ops._overlap(ids[6:6], ids) and ops._overlap(ids[6:7], ids)

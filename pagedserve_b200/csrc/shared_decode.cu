@@ -1033,11 +1033,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (fail) {
-      if (on) flag_error(p.err, PSB_DEVERR_TIMEOUT);
-      // copies still in flight: the newest of each stage
-      for (uint32_t t = g > kStages ? g - kStages : 0; t < g; ++t) (void)warp_wait_at(a_full + 8 * (t % kStages), (t / kStages) & 1);
-    }
+    if (fail && on) flag_error(p.err, PSB_DEVERR_TIMEOUT);
+    // the newest copies of each stage land before the CTA ends, also where the products gave up waiting for others
+    for (uint32_t t = g > kStages ? g - kStages : 0; t < g; ++t) (void)warp_wait_at(a_full + 8 * (t % kStages), (t / kStages) & 1);
   };
   if (warp >= kFirstOwn) {
     own_parts<T, D, HP, NT>(p, plan, &tm_ko, &tm_vo, smem + Geo::kOffRing, bar_own);
@@ -1065,7 +1063,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int x = r.two ? 0 : mine; x < r.n; x += r.two ? 1 : 2, ++k) {
         const int b = k & 1;
         const uint32_t ph = (k >> 1) & 1;
-        if (!mbar_wait(bar_s + 2 * s + b, ph)) {
+        // (by whole warps, here and below: lanes that gave up by themselves would leave the others' TMEM access short of them)
+        if (!warp_wait(bar_s + 2 * s + b, ph)) {
           fail = true;
           break;
         }
@@ -1093,7 +1092,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float ms_new = grow ? mxs : ms;
           const float alpha = ms == -INFINITY ? 0.f : ex2_approx(ms - ms_new);  // (a step has at least one key)
           if (begun) {  // O holds P V of the earlier half-steps once the last of them is done
-            if (!mbar_wait(bar_pv + 2 * s + (b ^ 1), ((k - 1) >> 1) & 1)) {
+            if (!warp_wait(bar_pv + 2 * s + (b ^ 1), ((k - 1) >> 1) & 1)) {
               fail = true;
               break;
             }

@@ -445,6 +445,7 @@ def paged_decode_attention_with_write(query: torch.Tensor, key: torch.Tensor, va
     dev = query.get_device()
     if key.get_device() != dev or value.get_device() != dev:
         raise ValueError("new K/V must be on the query's device")
+    _check_writable(cache, request_ids, positions)
     if _is_int4(kv):  # the row's minimum and maximum are needed before its codes: a launch of its own
         key, value = (t if t.stride(-1) == 1 else t.contiguous() for t in (key, value))
         _write_rows(kv, key, value, _slots(cache, request_ids, positions, query.device), layer)
@@ -535,12 +536,19 @@ def _slots(cache, request_ids, positions, device):
     def build():
         slots = np.fromiter((cache.slot_of(r, p) if hasattr(cache, "slot_of") else _slot(cache, r, p)
                              for r, p in zip(request_ids, positions)), dtype=np.int64, count=len(request_ids))
+        _check_writable(cache, request_ids, positions)
         host = torch.from_numpy(slots)
         if device.type == "cuda":
             host = host.pin_memory()
         return host.to(device, non_blocking=True)
 
     return _memo(cache, "slots", request_ids, positions, device, build)
+
+
+def _check_writable(cache, request_ids, positions) -> None:
+    """Refuses a write into blocks that several requests hold (a reference cache shares none)."""
+    if hasattr(cache, "check_writable"):
+        cache.check_writable(request_ids, positions)
 
 
 def _slot(cache, request_id: str, position: int) -> int:

@@ -332,7 +332,8 @@ class PagedKVCache:
         They share the parent's whole blocks; of a block in which those tokens end
         each gets a copy of its own, in one launch for all of them.  Parent and
         children are then requests like any other: appended to, read, and freed in
-        any order.  If the free list does not have a block for each copy,
+        any order; only a token in a block that others hold too is not written again
+        (``check_writable``).  If the free list does not have a block for each copy,
         RuntimeError and nothing has changed."""
         self._validate_request(parent_id)
         request_ids = list(request_ids)
@@ -469,6 +470,18 @@ class PagedKVCache:
         bs = self.block_size
         return self._tables[request_id].get_physical_block(token_position // bs), token_position % bs
 
+    def check_writable(self, request_ids, positions) -> None:
+        """ValueError where a token lies in a block that other requests hold too
+        (``fork``): written through one of them it would change for all."""
+        shares = self.block_manager._shares
+        if not shares:
+            return
+        rows = self._rows_of(request_ids)
+        at = np.fromiter(positions, dtype=np.int64, count=len(rows)) // self.block_size
+        for request_id, block in zip(request_ids, self._store[rows, at].tolist()):
+            if block in shares:
+                raise ValueError(f"Block {block} of request {request_id!r} is held by other requests too")
+
     def write_token(self, request_id: str, layer: int, token_position: int, key: torch.Tensor,
                     value: torch.Tensor) -> None:
         """Write one token's ``[Hkv, D]`` K/V at its logical position."""
@@ -479,6 +492,7 @@ class PagedKVCache:
             raise ValueError(f"Expected K/V shape {shape}; got key={tuple(key.shape)}, value={tuple(value.shape)}")
         if key.dtype != self.kv_cache.dtype or value.dtype != self.kv_cache.dtype:
             raise ValueError(f"K/V tensors must have dtype {self.kv_cache.dtype}")
+        self.check_writable((request_id,), (token_position,))
         if self.kv_cache.kv_bits == 4:
             kv = self.kv_cache
             if key.device != kv.kv_codes.device or value.device != kv.kv_codes.device:

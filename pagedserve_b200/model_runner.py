@@ -196,8 +196,6 @@ class PagedModelRunner:
 
     def _paged_decode(self, q, block_tables, context_lens, layer: int, max_context: int, out=None, groups=None):
         if groups is not None:
-            if self.kv_bits == 4:
-                raise ValueError("groups need a 16-bit pool")
             return ops.paged_decode_shared(q, self.k_cache, self.v_cache, block_tables, context_lens, *groups, layer,
                                            scale=self.scale, out=out, max_context=max_context)
         op = ops.paged_decode_int4 if self.kv_bits == 4 else ops.paged_decode
@@ -259,6 +257,8 @@ class PagedModelRunner:
         ``ops.paged_decode_shared`` takes them (16-bit pools; read once per
         group, else the same result).  Returns logits ``[B, V]``
         (``_forward_paged_batch``'s ``[B, 1, V]`` without the unit axis)."""
+        if groups is not None and self.kv_bits == 4:  # (before the first layer writes its keys)
+            raise ValueError("groups need a 16-bit pool")
         max_context = block_tables.shape[1] * self.block_size if max_context is None else max_context
 
         def attend(q_rot, _k, _v, layer):

@@ -653,6 +653,7 @@ int psb_copy_blocks(void* const* pools, const int64_t* block_bytes, int32_t num_
  * see it unspecified.  The workspace (psb_paged_decode_shared_workspace_size, 0 for
  * what is not taken) needs no initialisation; calls that overlap on the GPU need one
  * each.  Probabilities are rounded to the cache's type before P V; all else is fp32.
+ * Scores of -infinity have no weight; what is no number reaches the rows that see it.
  */
 size_t psb_paged_decode_shared_workspace_size(int32_t batch, int32_t num_groups, int32_t q_heads,
                                               int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
@@ -690,12 +691,13 @@ int psb_check_groups(const int32_t* cu_groups, const int32_t* prefix_lens, int32
  * weight is above uniforms[r, 1] times the sum.  uniforms [total, 2] fp32 in [0, 1).
  * new_tokens [total] int64: the drafts taken and the new token from cu_seqlens[b] on, -1
  * in all other rows; counts [batch] int32: how many (0 for a sequence of no rows).
- * Decided as 64-bit arithmetic does, but that weights below 2^-900 of a row's largest
- * are none.  A row that stands for no probabilities (a NaN, +infinity, nothing but
+ * Decided as 64-bit arithmetic does (the weights good to 3e-12 of themselves), but that
+ * weights below 2^-900 of a row's largest are none.  A row that stands for no probabilities (a NaN, +infinity, nothing but
  * -infinity) takes no draft, gives its first maximum and is flagged
  * (PSB_DEVERR_LOGITS); a temperature that is NaN, negative or infinite is flagged and
  * taken for 0; entries of draft_probs that are NaN or negative count as 0.  A
- * malformed cu_seqlens is flagged (PSB_DEVERR_SEQLENS), the sequence's count 0.  The
+ * malformed cu_seqlens is flagged (PSB_DEVERR_SEQLENS), the sequence's count 0, and
+ * new_tokens is unspecified where it names rows out of order.  The
  * workspace needs no initialisation; calls that overlap on the GPU need one each.
  */
 size_t psb_verify_tokens_workspace_size(int32_t batch);

@@ -30,12 +30,13 @@
 // TMEM: S = Q K^T of its next step but one is issued behind O += P V of this one, whose
 // P, two keys a column, was written over S.
 //
-// Measured (a pass among others, of which 5 us are the two launches and 4 the plan): 8
-// sequences on 1 K shared tokens 12 us, 64 on 4 K 19, 32 groups of 8 on 1.5 K 26; 256 on 2 K
+// Measured (a call among others, of which 5 us are the two launches and 3 to 4 the plan): 8
+// sequences on 1 K shared tokens 12 us, 64 on 4 K 20, 32 groups of 8 on 1.5 K 27; 256 on 2 K
 // with 1 K each of their own 40, its 130 MB in 30 at 4.3 TB/s (the plain decode of the
 // same contexts: 720 MB); 96 on 30 K, D 128, 86, its 47 GFLOP in 66: a pair's step takes 2050
 // cycles where its exponentials are 1024 and its products 1300 (64 keys a step: Q is
-// read from shared memory again for each; 128 keys do not fit TMEM beside two O).  Tried
+// read from shared memory again for each; two S of 128 keys and two O of 128 dims fill TMEM,
+// so 128 keys a step would leave each stream one S to write and read in turn).  Tried
 // and not faster: a third stage of V, boxes asked into L2 ahead, the products' bookkeeping
 // moved behind P V's issue, own slices of 32 tokens.
 //
@@ -1350,7 +1351,8 @@ int launch(SharedParams p, int num_layers, cudaStream_t s) {
       !encode_box_map(&tv, p.v_cache, kdims, kstr, kbox, dt) || !encode_box_map(&tko, p.k_cache, kdims, kstr, obox, dt) ||
       !encode_box_map(&tvo, p.v_cache, kdims, kstr, obox, dt))
     return PSB_ERR_CUDA;
-  // (a tile of two heads of D 128 takes too many registers)
+  // (a tile of two heads of D 128 takes too many registers; that of 9 to 16 q heads spills 240 bytes a
+  // thread there, 32 sequences of 32 / 2 heads on 4 K with 256 each of their own in 25 us: paged_decode 1660)
   const bool hi = !two && p.group > 8;
   const auto kern = two ? shared_main_kernel<T, D, D == 64 ? 2 : 1, 1> : hi ? shared_main_kernel<T, D, 1, 2> : shared_main_kernel<T, D, 1, 1>;
   const void* const f = reinterpret_cast<const void*>(kern);

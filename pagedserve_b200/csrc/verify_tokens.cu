@@ -540,8 +540,14 @@ __device__ void draw(const VerifyParams& p, Cluster& cl, int r, int d, int mode,
       double rest = fma(-z, q, e);
       const int n_open = cl.sums->n_open[warp];
       if constexpr (kProbs) {
-        if (lane < min(n_open, 4)) {
-          const int d0 = cl.sums->open[warp][lane];
+        if (n_open <= 4 && lane < n_open) {  // lane i the i-th of them, in whatever order they came: the sum is always the same
+          const int* const all_open = cl.sums->open[warp];
+          int d0 = 0;
+          for (int j = 0; j < n_open; ++j) {
+            int smaller = 0;
+            for (int i = 0; i < n_open; ++i) smaller += all_open[i] < all_open[j];
+            if (smaller == lane) d0 = all_open[j];
+          }
           rest += fmax(fma(-z, prob_at<Q>(p.probs, static_cast<int64_t>(r) * p.probs_stride + d0), ex.weight(Elem<T>::to_float(row.x[d0]))), 0.0);
         }
       }

@@ -117,3 +117,13 @@ def test_queries_that_are_no_numbers(kw, shape):
     got = b.run().cpu()
     assert bool(got[1, 0].isnan().all()) and bool(got[0, -1].isnan().all()) and bool(got[-1].isnan().all())
     _same_but(b, got, want, [(1, 0), (0, b.hq - 1), (-1,)])
+
+
+@pytest.mark.parametrize("kw", GEOMETRIES, ids=range(len(GEOMETRIES)))
+def test_idle_rows_whose_queries_are_no_numbers(kw):
+    b = Batch([(200, [0, 230, 0, 201, 199]), (64, [0, 0])], alone=[0, 40], **kw)
+    want = b.run().cpu()
+    idle = [i for i, n in enumerate(b.lens) if n == 0]
+    b.q[idle] = math.nan
+    got = b.run().cpu()
+    assert bool((got[idle] == 0).all()) and torch.equal(got, want)

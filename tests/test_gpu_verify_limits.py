@@ -162,3 +162,18 @@ def test_the_least_temperatures(heat, batch):
     args = (logits, torch.zeros(batch, dtype=torch.int64), list(range(batch + 1)), u, torch.full((batch,), heat), None)
     new, _ = _check(*args)
     assert batch == 3 or len(set(new[::2].tolist())) == 3 and len(set(new[1::2].tolist())) > 2
+
+
+@pytest.mark.parametrize("probs", [None, torch.float16])
+def test_a_vocabulary_beyond_the_fp32_weights(probs):
+    """More tokens than fp32's sums are asked about: all of it in 64 bits."""
+    vocab = (1 << 25) + 3
+    g = torch.Generator().manual_seed(6)
+    logits = (torch.rand(2, vocab, generator=g) * 3).half()
+    tokens = torch.tensor([0, 12345678])
+    q = None
+    if probs is not None:
+        q = torch.zeros(2, vocab, dtype=probs)
+        q[0, 100:2100] = 5e-4
+    for u in ([[0.5, 0.3], [0.1, 0.99999]], [[0.0, 0.7], [0.9, 1e-7]]):
+        _check(logits, tokens, [0, 2], torch.tensor(u), torch.tensor([0.8]), q)
